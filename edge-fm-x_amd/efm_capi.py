@@ -148,6 +148,30 @@ SIGNATURES = {
                                                  c_void_p, c_void_p, c_void_p]),
     "efm_decode_norm_lm_head_top1": (c_int32, [c_int32, c_int64, c_float, c_void_p, c_void_p, c_void_p, c_void_p,
                                                c_void_p, c_void_p, c_size_t, c_void_p]),
+    "efm_fp4_packed_bytes": (c_size_t, [c_int64, c_int64]),
+    "efm_fp4_quantize": (c_int32, [c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "efm_fp4_pack": (c_int32, [c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "efm_linear_fp4_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64]),
+    "efm_linear_fp4": (c_int32, [c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_void_p,
+                                 c_size_t, c_void_p]),
+    "efm_fused_gate_up_swiglu_fp4_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64]),
+    "efm_fused_gate_up_swiglu_fp4": (c_int32, [c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p,
+                                               c_size_t, c_void_p]),
+    "efm_qk_norm_rope_write_kv": (c_int32, [POINTER(AttentionCtx), c_void_p, c_int64, c_void_p, c_void_p, c_float,
+                                            c_void_p, c_void_p, c_void_p, c_uint32, c_uint32, c_uint32, c_void_p,
+                                            c_void_p, c_int32, c_int32, c_int32, c_int32, c_void_p]),
+    "efm_kv_fp4_bytes": (c_size_t, [POINTER(AttentionCtx), c_uint32]),
+    "efm_qk_norm_rope_write_kv_fp4": (c_int32, [POINTER(AttentionCtx), c_void_p, c_int64, c_void_p, c_void_p, c_float,
+                                                c_void_p, c_void_p, c_uint32, c_uint32, c_uint32, c_void_p, c_void_p,
+                                                c_int32, c_int32, c_int32, c_int32, c_void_p]),
+    "efm_kv_fp4_read": (c_int32, [POINTER(AttentionCtx), c_void_p, c_uint32, c_uint32, c_uint32, c_void_p, c_void_p,
+                                  c_void_p]),
+    "efm_attention_decode_kv_fp4_workspace_bytes": (c_size_t, [POINTER(AttentionCtx), c_uint32]),
+    "efm_attention_decode_kv_fp4": (c_int32, [POINTER(AttentionCtx), c_void_p, c_void_p, c_uint32, c_void_p, c_uint32,
+                                              c_void_p, c_uint32, c_void_p, c_size_t, c_void_p]),
+    "efm_attention_prefill_kv_fp4_workspace_bytes": (c_size_t, [POINTER(AttentionCtx), c_uint32, c_uint32]),
+    "efm_attention_prefill_kv_fp4": (c_int32, [POINTER(AttentionCtx), c_void_p, c_void_p, c_uint32, c_void_p, c_uint32,
+                                               c_uint32, c_int32, c_void_p, c_size_t, c_void_p]),
 }
 
 

@@ -477,6 +477,103 @@ int efm_decode_norm_lm_head_top1(int32_t hidden, int64_t vocab, float eps, const
                                  int32_t* token_out, void* workspace, size_t workspace_bytes,
                                  hipStream_t stream);
 
+/* ------------------------------------------------------------------------------------
+ * FP4 weights and cache. No counterpart in the reference, whose operators are 16-bit.
+ *
+ * The format is the OCP microscaling FP4 (E2M1 elements, E8M0 scales): groups of 32
+ * consecutive values share a scale 2^(b - 127) held in a byte b (255: the group is NaN); an
+ * element is a 4-bit code, sign in bit 3, magnitude 0, 0.5, 1, 1.5, 2, 3, 4, 6 for codes 0 to
+ * 7. An element's value (magnitude times scale) is exact in bf16. Quantisation takes the
+ * least scale with max |x| <= 7 * scale (at least 2^-125) and rounds x / scale to the nearest
+ * magnitude, of two as near to the one with the even code, so that the error is at most half
+ * a step of the grid; a group that holds a NaN or an infinity is stored as NaN.
+ * ---------------------------------------------------------------------------------- */
+
+/* Weights in the interchange form: codes [out, in / 2], element 2 i of a row in the low half
+ * of byte i, and scales [out, in / 32]. in_features must be a multiple of 32.
+ * efm_fp4_quantize makes them from bf16 weights [out, in]; efm_fp4_pack lays them out for the
+ * kernels below, once, into efm_fp4_packed_bytes(in, out) bytes (0: bad shape). w, codes and
+ * packed must be 16-byte aligned. */
+size_t efm_fp4_packed_bytes(int64_t in_features, int64_t out_features);
+int efm_fp4_quantize(int64_t in_features, int64_t out_features, const void* w, uint8_t* codes, uint8_t* scales,
+                     hipStream_t stream);
+int efm_fp4_pack(int64_t in_features, int64_t out_features, const uint8_t* codes, const uint8_t* scales, void* packed,
+                 hipStream_t stream);
+
+/* efm_linear with packed FP4 weights: y[m, out] = x[m, in] . W^T (+ bias[out]), x and bias
+ * bf16, fp32 accumulate, y bf16 or fp32. Any m; few rows are bound by the weights' bytes, a
+ * quarter of bf16's. workspace: efm_linear_fp4_workspace_bytes (0: none is used), no initial
+ * contents required; calls that share one must be stream-ordered. Deterministic. */
+size_t efm_linear_fp4_workspace_bytes(int64_t m, int64_t in_features, int64_t out_features);
+int efm_linear_fp4(int64_t m, int64_t in_features, int64_t out_features, const void* x, const void* w_packed,
+                   const void* bias, void* y, int32_t out_dtype, void* workspace, size_t workspace_bytes,
+                   hipStream_t stream);
+
+/* efm_fused_gate_up_swiglu with packed FP4 weights: W = [up; gate], [2 * inter, hidden],
+ * packed as one matrix; inter must be a multiple of 16.
+ * out[m, i] = bf16(silu(bf16(g_i)) * bf16(u_i)). */
+size_t efm_fused_gate_up_swiglu_fp4_workspace_bytes(int64_t m, int64_t hidden, int64_t inter);
+int efm_fused_gate_up_swiglu_fp4(int64_t m, int64_t hidden, int64_t inter, const void* x, const void* w_packed, void* out,
+                                 void* workspace, size_t workspace_bytes, hipStream_t stream);
+
+/* Norm of queries and keys per head, position rotation and cache write in one pass. Row t of
+ * qkv [seq_len, qkv_stride_n] (0: (Hq + 2 Hkv) * hd) holds q, k and v of a token. For a head
+ * x of q or k: y = x * rsqrt(mean(x^2) + eps) * w with w = q_norm_w or k_norm_w, bf16 [hd]
+ * shared by the heads (NULL: y = x); with EFM_POS_ROPE_LLAMA the pair (d, d + hd/2) of y is
+ * then rotated by pos * theta^(-2d/hd) / rope_scale (the angle is reduced in 64 bits). y is
+ * rounded to bf16 once. Queries go to q_out (strides ctx->q_stride_*; may be the q columns of
+ * qkv itself; NULL: they are not computed), keys and values to cache rows base .. base +
+ * seq_len - 1 (strides ctx->k_stride_* and ctx->kv_stride_*), base = *d_kv_len - seq_len when
+ * d_kv_len is not NULL (device-resident, graph-stable; a length outside [seq_len, max_rows]
+ * writes nothing, q_out included). The token's position is its cache row plus
+ * ctx->q_rope_pos_offset (keys: k_rope_pos_offset), or with position_ids
+ * [3, position_stride] (M-RoPE; sections sum to hd/2) the id of the pair's section.
+ * Rows behind the last one written are left as they are. Stands beside
+ * efm_prefill_rope_write_kv for models that normalise queries and keys. */
+int efm_qk_norm_rope_write_kv(const efm_attention_ctx* ctx, const void* qkv, int64_t qkv_stride_n, const void* q_norm_w,
+                              const void* k_norm_w, float eps, void* q_out, void* k_cache, void* v_cache,
+                              uint32_t max_rows, uint32_t seq_len, uint32_t base, const uint32_t* d_kv_len,
+                              const int32_t* position_ids, int32_t position_stride, int32_t section0, int32_t section1,
+                              int32_t section2, hipStream_t stream);
+
+/* The same into one layer's FP4 cache of efm_kv_fp4_bytes(ctx, max_rows) bytes (16-byte
+ * aligned, no initial contents required): keys and values are quantised in groups of 32
+ * channels of a head, keys from their unrounded values (computed in 64 bits, so that the codes
+ * are the formula's own). max_rows belongs to the cache: every call on it passes the same.
+ * ctx->k_stride_* and kv_stride_* are not used. Without norm weights and with EFM_POS_NONE the
+ * call quantises rows as they are. */
+size_t efm_kv_fp4_bytes(const efm_attention_ctx* ctx, uint32_t max_rows);
+int efm_qk_norm_rope_write_kv_fp4(const efm_attention_ctx* ctx, const void* qkv, int64_t qkv_stride_n,
+                                  const void* q_norm_w, const void* k_norm_w, float eps, void* q_out, void* cache,
+                                  uint32_t max_rows, uint32_t seq_len, uint32_t base, const uint32_t* d_kv_len,
+                                  const int32_t* position_ids, int32_t position_stride, int32_t section0,
+                                  int32_t section1, int32_t section2, hipStream_t stream);
+/* Rows first .. first + rows - 1 of the cache as bf16, [rows, Hkv, hd] (either output may be
+ * NULL); exact. */
+int efm_kv_fp4_read(const efm_attention_ctx* ctx, const void* cache, uint32_t max_rows, uint32_t first, uint32_t rows,
+                    void* k_out, void* v_out, hipStream_t stream);
+
+/* efm_attention_decode over an FP4 cache: q [1, Hq, hd] (ctx->q_stride_h), o [1, Hq, hd]. The
+ * cache holds keys as they are multiplied, so pos_encoding must be EFM_POS_NONE. The number of
+ * attended rows is min(*d_kv_len, max_kv_len) when d_kv_len != NULL, else kv_len; none: o is
+ * zero. fp32 softmax, P rounded to bf16 for the PV product. Rows past the attended ones are
+ * never part of the result, whatever they hold. workspace:
+ * efm_attention_decode_kv_fp4_workspace_bytes(ctx, max_kv_len or kv_len) bytes (0: none), no
+ * initial contents required; calls that share one must be stream-ordered. */
+size_t efm_attention_decode_kv_fp4_workspace_bytes(const efm_attention_ctx* ctx, uint32_t max_kv_len);
+int efm_attention_decode_kv_fp4(const efm_attention_ctx* ctx, const void* q, const void* cache, uint32_t max_rows, void* o,
+                                uint32_t kv_len, const uint32_t* d_kv_len, uint32_t max_kv_len, void* workspace,
+                                size_t workspace_bytes, hipStream_t stream);
+
+/* efm_attention_prefill over an FP4 cache whose first kv_len rows include the queries' own:
+ * q [qo_len, Hq, hd] (ctx->q_stride_*), o [qo_len, Hq * hd] contiguous, kv_len >= qo_len; when
+ * causal, query i sees keys j <= i + (kv_len - qo_len). pos_encoding must be EFM_POS_NONE.
+ * workspace: efm_attention_prefill_kv_fp4_workspace_bytes bytes (0: none), as above. */
+size_t efm_attention_prefill_kv_fp4_workspace_bytes(const efm_attention_ctx* ctx, uint32_t qo_len, uint32_t kv_len);
+int efm_attention_prefill_kv_fp4(const efm_attention_ctx* ctx, const void* q, const void* cache, uint32_t max_rows,
+                                 void* o, uint32_t qo_len, uint32_t kv_len, int32_t causal, void* workspace,
+                                 size_t workspace_bytes, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,581 @@
+"""GPU tests of the FP4 weights and cache and of the per-head norms, against plain 64-bit forms (_fp4_ref).
+
+Tolerances are derived: half a step of the output's type (bf16 2^-8, relative), what the documented roundings inside an
+operator can move, and the rounding of fp32 sums. Quantised values have to be equal."""
+import math
+
+import pytest
+import torch
+
+import _fp4_ref as R
+import efm_capi as C
+from _util import ptr, stream
+
+pytestmark = pytest.mark.gpu
+
+HALF = 2.0 ** -8   # bf16
+HEADS = [pytest.param(14, 2, 64, id="0p5b"), pytest.param(12, 2, 128, id="1p5b"), pytest.param(28, 4, 128, id="7b")]
+
+
+def _buf(nbytes, fill=0):
+    return torch.full((max(int(nbytes), 256),), fill, dtype=torch.uint8, device="cuda")
+
+
+def _gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def _bf(g, *size, std=1.0):
+    return (torch.randn(*size, generator=g) * std).to(torch.bfloat16)
+
+
+def _within(got, ref, tol, what=""):
+    got, err = got.double().cpu(), None
+    assert got.shape == ref.shape
+    assert torch.equal(torch.isnan(got), torch.isnan(ref)), f"{what}: NaN in other places"
+    err = (got - ref).abs()
+    bad = ~(err <= tol) & ~torch.isnan(ref)
+    assert not bad.any(), f"{what}: {int(bad.sum())} of {bad.numel()} off, worst {float((err - tol)[bad].max())} past its tolerance"
+
+
+# ---------------------------------------------------------------- weights
+
+def _quantize(w):
+    out, k = w.shape
+    codes = torch.zeros(out, k // 2, dtype=torch.uint8, device="cuda")
+    scales = torch.zeros(out, k // 32, dtype=torch.uint8, device="cuda")
+    wd = w.cuda()
+    C.call("efm_fp4_quantize", k, out, ptr(wd), ptr(codes), ptr(scales), stream())
+    torch.cuda.synchronize()
+    return codes, scales
+
+
+def _pack(codes, scales):
+    out, k = codes.shape[0], codes.shape[1] * 2
+    packed = _buf(C.load().efm_fp4_packed_bytes(k, out), 0xff)
+    cd, sd = codes.cuda().contiguous(), scales.cuda().contiguous()
+    C.call("efm_fp4_pack", k, out, ptr(cd), ptr(sd), ptr(packed), stream())
+    torch.cuda.synchronize()
+    return packed
+
+
+def test_quantize_equals_the_definition(gpu):
+    """Random rows of several magnitudes, borders of the grid under every scale's mantissa, zeros, the smallest and the
+    largest bf16 values, and groups with NaN and infinities."""
+    g = _gen(1)
+    w = _bf(g, 24, 96) * torch.exp2(torch.randint(-130, 125, (24, 3), generator=g).float()).repeat_interleave(32, 1).bfloat16()
+    ties = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, -0.25, -0.75, -1.25, -1.75, -2.5, -3.5, -5.0, 6, 7] * 2)
+    w[0, :32], w[1, :32], w[2, :32] = ties, ties * 2.0 ** -120, ties * 2.0 ** 100
+    w[3, :32] = 0
+    w[4, :32] = 2.0 ** -133
+    w[5, :32] = torch.finfo(torch.bfloat16).max
+    w[6, 0], w[6, 32], w[6, 64] = math.nan, math.inf, -math.inf
+    w[7, :32] = torch.linspace(-7.03125, 7.03125, 32).bfloat16()   # 7.03125 is past 7: the next scale
+    codes, scales = _quantize(w)
+    code, byte = R.quantize(w)
+    assert torch.equal(scales.cpu(), byte)
+    assert torch.equal(codes.cpu(), R.halves(code))
+
+
+def _linear(x, packed, k, out, bias=None, f32=False, fill_ws=0xff):
+    m = x.shape[0]
+    y = torch.full((m, out), math.nan, dtype=torch.float32 if f32 else torch.bfloat16, device="cuda")
+    ws = _buf(C.load().efm_linear_fp4_workspace_bytes(m, k, out), fill_ws)
+    C.call("efm_linear_fp4", m, k, out, ptr(x), ptr(packed), ptr(bias), ptr(y), C.EFM_DTYPE_F32 if f32 else C.EFM_DTYPE_BF16,
+           ptr(ws), ws.numel(), stream())
+    torch.cuda.synchronize()
+    return y
+
+
+def _weights(g, out, k):
+    """Codes and scales of any bit pattern with scales around 2^-7, as a checkpoint of the format may hold."""
+    code = torch.randint(0, 16, (out, k), generator=g).to(torch.uint8)
+    byte = torch.randint(117, 123, (out, k // 32), generator=g).to(torch.uint8)
+    return code, byte
+
+
+def _product(x, w):
+    """(x w^T, bound of its fp32 error): chains of K / 32 products of 32 terms, 2^-23 an addition, of the sum of
+    magnitudes; sums of waves and slices of K are 64 additions more at most."""
+    k = x.shape[1]
+    return x @ w.T, (k / 32 + 32 + 64) * 2.0 ** -23 * (x.abs() @ w.abs().T)
+
+
+SHAPES = [(1, 32, 1), (1, 896, 1152), (1, 160, 17), (1, 18944, 100), (2, 96, 33), (5, 4864, 896), (16, 1536, 300), (17, 544, 48),
+          (31, 992, 130), (33, 288, 64), (64, 2048, 272), (100, 160, 4608), (129, 896, 257), (300, 1536, 640), (1000, 512, 384)]
+
+
+@pytest.mark.parametrize("m,k,out", SHAPES)
+@pytest.mark.parametrize("bias,f32", [(False, False), (True, True)])
+def test_linear(gpu, m, k, out, bias, f32):
+    g = _gen(m * 7 + k + out)
+    code, byte = _weights(g, out, k)
+    x, b = _bf(g, m, k), _bf(g, out)
+    y = _linear(x.cuda(), _pack(R.halves(code), byte), k, out, b.cuda() if bias else None, f32)
+    ref, tol = _product(x.double(), R.values(code, byte))
+    if bias:
+        ref = ref + b.double()
+        tol = tol + 2.0 ** -23 * ref.abs()
+    _within(y, ref, tol if f32 else tol + HALF * (ref.abs() + tol), f"{m} x {k} -> {out}")
+
+
+@pytest.mark.parametrize("m,hidden,inter", [(1, 896, 4864), (1, 32, 16), (3, 1536, 64), (16, 160, 112), (24, 1536, 8960),
+                                            (40, 544, 48), (70, 896, 80), (200, 256, 272), (600, 512, 320)])
+def test_swiglu(gpu, m, hidden, inter):
+    g = _gen(m + hidden + inter)
+    code, byte = _weights(g, 2 * inter, hidden)
+    x = _bf(g, m, hidden)
+    packed, y = _pack(R.halves(code), byte), torch.full((m, inter), math.nan, dtype=torch.bfloat16, device="cuda")
+    ws = _buf(C.load().efm_fused_gate_up_swiglu_fp4_workspace_bytes(m, hidden, inter), 0xff)
+    xd = x.cuda()
+    C.call("efm_fused_gate_up_swiglu_fp4", m, hidden, inter, ptr(xd), ptr(packed), ptr(y), ptr(ws), ws.numel(), stream())
+    torch.cuda.synchronize()
+    (up, gate), (eu, eg) = (t.chunk(2, 1) for t in _product(x.double(), R.values(code, byte)))
+    silu = gate * torch.sigmoid(gate)
+    du, dg = eu + HALF * (up.abs() + eu), eg + HALF * (gate.abs() + eg)
+    tol = 1.1 * dg * (up.abs() + du) + silu.abs() * du   # |silu'| < 1.1
+    _within(y, silu * up, tol + (HALF + 2.0 ** -20) * ((silu * up).abs() + tol), f"{m} {hidden} {inter}")
+
+
+@pytest.mark.parametrize("m", [1, 20, 200])
+def test_linear_nan_stays_in_its_place(gpu, m):
+    """A NaN group reaches its own output column alone, a NaN row of x its own row; rows and columns that pad the tiles
+    reach nothing."""
+    g = _gen(3)
+    k, out = 160, 19
+    code, byte = _weights(g, out, k)
+    byte[7, 4] = 255
+    x = _bf(g, m, k)
+    y = _linear(x.cuda(), _pack(R.halves(code), byte), k, out).cpu()
+    bad = torch.isnan(y)
+    assert bad[:, 7].all() and int(bad.sum()) == m
+    if m > 1:
+        x[m - 1, 3] = math.inf
+        x[m - 1, 4] = math.nan
+        bad = torch.isnan(_linear(x.cuda(), _pack(R.halves(code), byte), k, out).cpu())
+        assert bad[m - 1].all() and bad[:, 7].all() and int(bad.sum()) == m + out - 1
+
+
+@pytest.mark.parametrize("m,k,out", [(1, 4864, 896), (24, 8960, 512), (200, 1024, 640)])
+def test_linear_repeats_and_runs_in_a_graph(gpu, m, k, out):
+    """Captured on a side stream and replayed with other inputs, eager work between: bit for bit the eager result."""
+    g = _gen(m + 5)
+    code, byte = _weights(g, out, k)
+    packed, x = _pack(R.halves(code), byte), _bf(g, m, k).cuda()
+    y = torch.empty(m, out, dtype=torch.bfloat16, device="cuda")
+    ws = _buf(C.load().efm_linear_fp4_workspace_bytes(m, k, out))
+    s, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=s, capture_error_mode="thread_local"):
+        C.call("efm_linear_fp4", m, k, out, ptr(x), ptr(packed), None, ptr(y), C.EFM_DTYPE_BF16, ptr(ws), ws.numel(), s.cuda_stream)
+    for rep in range(3):
+        x.copy_(_bf(g, m, k))
+        y.fill_(math.nan)
+        torch.randn(1 << 18, device="cuda").sum()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, _linear(x, packed, k, out)), f"replay {rep}"
+
+
+# ---------------------------------------------------------------- norm, rotation, write
+
+def _positions(base, S, half, off=0):
+    return (base + off + torch.arange(S, dtype=torch.int64))[:, None].expand(S, half)
+
+
+def _write(ctx, fp4, qkv, qw, kw, q_out, dst, room, S, base, d_len=None, pos=None, sec=(0, 0, 0), eps=1e-6, stride=0, on=None):
+    C.call("efm_qk_norm_rope_write_kv" + ("_fp4" if fp4 else ""), ctx, ptr(qkv), stride, ptr(qw), ptr(kw), eps, ptr(q_out),
+           *[ptr(d) for d in dst], room, S, base, ptr(d_len), ptr(pos), 0 if pos is None else pos.shape[1], *sec,
+           on if on is not None else stream())
+
+
+def _read(ctx, cache, room, first, rows, hkv, hd):
+    k, v = (torch.empty(rows, hkv, hd, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    C.call("efm_kv_fp4_read", ctx, ptr(cache), room, first, rows, ptr(k), ptr(v), stream())
+    torch.cuda.synchronize()
+    return k.cpu().double(), v.cpu().double()
+
+
+def _y_tol(y, x, w, eps):
+    """fp32 work on a pair: sums of hd squares, sqrt, division, sine and cosine, products: 2^-18 of the pair's larger
+    magnitude covers some 30 roundings; then half a step of bf16."""
+    n = R.norm_rope(x, w, eps, None, 1.0).abs()
+    pair = n + n.roll(x.shape[-1] // 2, -1)
+    return HALF * y.abs() + 2.0 ** -18 * pair
+
+
+@pytest.mark.parametrize("hq,hkv,hd", HEADS)
+@pytest.mark.parametrize("S,base", [(1, 0), (1, 63), (5, 3), (33, 31), (130, 1000000)])
+@pytest.mark.parametrize("norm", [True, False])
+@pytest.mark.parametrize("fp4", [False, True])
+def test_write(gpu, hq, hkv, hd, S, base, norm, fp4):
+    """Queries, keys and values of a prompt or a step; rows of the cache around the written ones stay as they were."""
+    g = _gen(S + base + hd)
+    width = (hq + 2 * hkv) * hd
+    qkv = _bf(g, S, width + 8, std=1.5)
+    qkv[:, :hd] *= 100.0
+    qw, kw = (1 + _bf(g, hd, std=0.2), 1 + _bf(g, hd, std=0.2)) if norm else (None, None)
+    room = base + S + 40
+    ctx = C.make_attention_ctx(hq, hkv, hd, rope_theta=1e6)
+    x = qkv[:, :width].double().view(S, -1, hd)
+    q_out = torch.full((S, hq, hd), math.nan, dtype=torch.bfloat16, device="cuda")
+    dev = [None if t is None else t.cuda() for t in (qkv, qw, kw)]
+    pos = _positions(base, S, hd // 2)
+    q = R.norm_rope(x[:, :hq], qw, 1e-6, pos, 1e6)
+    k = R.norm_rope(x[:, hq:hq + hkv], kw, 1e-6, pos, 1e6)
+    if fp4:
+        cache = _buf(C.load().efm_kv_fp4_bytes(ctx, room), 0x5a)
+        _write(ctx, True, *dev, q_out, [cache], room, S, base, stride=width + 8)
+        kk, vv = _read(ctx, cache, room, base, S, hkv, hd)
+        assert torch.equal(kk, R.rounded(k)) and torch.equal(vv, R.rounded(x[:, hq + hkv:]))
+        fresh = _buf(C.load().efm_kv_fp4_bytes(ctx, room), 0x5a)
+        lo, n = max(0, base - 40), min(base, 40)
+        for first, rows in ((lo, n), (base + S, room - base - S)):
+            if rows:
+                for a, b in zip(_read(ctx, cache, room, first, rows, hkv, hd), _read(ctx, fresh, room, first, rows, hkv, hd)):
+                    assert torch.equal(a, b), "a row beside the written ones changed"
+    else:
+        kc, vc = (torch.full((room, hkv, hd), 7.0, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+        _write(ctx, False, *dev, q_out, [kc, vc], room, S, base, stride=width + 8)
+        torch.cuda.synchronize()
+        _within(kc[base:base + S], k, _y_tol(k, x[:, hq:hq + hkv], kw, 1e-6), "keys")
+        assert torch.equal(vc[base:base + S].cpu(), qkv[:, (hq + hkv) * hd:width].reshape(S, hkv, hd))
+        for c in (kc, vc):
+            assert (c[:base] == 7).all() and (c[base + S:] == 7).all()
+    torch.cuda.synchronize()
+    _within(q_out, q, _y_tol(q, x[:, :hq], qw, 1e-6), "queries")
+
+
+@pytest.mark.parametrize("fp4", [False, True])
+def test_write_mrope_offsets_strides_and_in_place(gpu, fp4):
+    """M-RoPE ids with sections; without ids, offsets of queries and keys that differ; a strided bf16 cache; the queries
+    written over their own columns."""
+    g = _gen(9)
+    hq, hkv, hd, S, base, room = 16, 2, 128, 37, 11, 64
+    width = (hq + 2 * hkv) * hd
+    qkv, qw, kw = _bf(g, S, width), 1 + _bf(g, hd, std=0.2), 1 + _bf(g, hd, std=0.2)
+    x = qkv.double().view(S, -1, hd)
+    ids = torch.randint(0, 5000, (3, S + 3), generator=g, dtype=torch.int32)
+    sec = (16, 24, 24)
+    by_id = torch.cat([ids[i, :S, None].expand(S, n) for i, n in enumerate(sec)], 1)
+    for pos, qp, kp, off in ((ids, by_id, by_id, (0, 0)), (None, _positions(base, S, 64, 5), _positions(base, S, 64, 70000), (5, 70000))):
+        ctx = C.make_attention_ctx(hq, hkv, hd, rope_theta=1e4, rope_scale=2.0, q_rope_pos_offset=off[0], k_rope_pos_offset=off[1],
+                                   q_stride_n=width, k_stride_n=2 * hkv * hd, kv_stride_n=2 * hkv * hd, k_stride_h=2 * hd,
+                                   kv_stride_h=2 * hd)
+        q, k = R.norm_rope(x[:, :hq], qw, 1e-5, qp, 1e4, 2.0), R.norm_rope(x[:, hq:hq + hkv], kw, 1e-5, kp, 1e4, 2.0)
+        d = qkv.cuda()
+        pd = None if pos is None else pos.cuda()
+        s = sec if pos is not None else (0, 0, 0)
+        kv = torch.full((room, hkv, 2, hd), 7.0, dtype=torch.bfloat16, device="cuda")
+        cache = _buf(C.load().efm_kv_fp4_bytes(ctx, room))
+        dst = [cache] if fp4 else [kv[:, :, 0], kv[:, :, 1]]
+        _write(ctx, fp4, d, qw.cuda(), kw.cuda(), d, dst, room, S, base, pos=pd, sec=s, eps=1e-5)
+        torch.cuda.synchronize()
+        got = d.cpu().view(S, -1, hd)
+        _within(got[:, :hq], q, _y_tol(q, x[:, :hq], qw, 1e-5), "queries")
+        assert torch.equal(got[:, hq:], qkv.view(S, -1, hd)[:, hq:])
+        if fp4:
+            kk, vv = _read(ctx, cache, room, base, S, hkv, hd)
+            assert torch.equal(kk, R.rounded(k)) and torch.equal(vv, R.rounded(x[:, hq + hkv:]))
+        else:
+            _within(kv[base:base + S, :, 0], k, _y_tol(k, x[:, hq:hq + hkv], kw, 1e-5), "keys")
+            assert torch.equal(kv[base:base + S, :, 1].cpu(), qkv.view(S, -1, hd)[:, hq + hkv:])
+
+
+@pytest.mark.parametrize("fp4", [False, True])
+@pytest.mark.parametrize("length", [0, 2, 3, 50, 64, 65])
+def test_write_at_a_device_length(gpu, fp4, length):
+    """Three rows that end at *d_kv_len; a length outside [3, 64] writes nothing. Equal to the call with the host's base."""
+    g = _gen(2)
+    hq, hkv, hd, S, room = 12, 2, 128, 3, 64
+    ctx = C.make_attention_ctx(hq, hkv, hd)
+    qkv, w = _bf(g, S, (hq + 2 * hkv) * hd).cuda(), (1 + _bf(g, hd, std=0.2)).cuda()
+    d_len = torch.tensor([length], dtype=torch.int32, device="cuda")
+    outs = []
+    for by_device in (True, False):
+        q = torch.full((S, hq, hd), 7.0, dtype=torch.bfloat16, device="cuda")
+        dst = [_buf(C.load().efm_kv_fp4_bytes(ctx, room), 0x11)] if fp4 else \
+            [torch.full((room, hkv, hd), 7.0, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+        if by_device:
+            _write(ctx, fp4, qkv, w, w, q, dst, room, S, 0, d_len=d_len)
+        elif S <= length <= room:
+            _write(ctx, fp4, qkv, w, w, q, dst, room, S, length - S)
+        torch.cuda.synchronize()
+        outs.append([q] + dst)
+    for a, b in zip(*outs):
+        assert torch.equal(a, b)
+
+
+def test_write_without_queries_and_read_of_one_side(gpu):
+    g = _gen(4)
+    ctx = C.make_attention_ctx(14, 2, 64, rope=False)
+    qkv = _bf(g, 9, 18 * 64)
+    x = qkv.double().view(9, 18, 64)
+    cache = _buf(C.load().efm_kv_fp4_bytes(ctx, 9))
+    _write(ctx, True, qkv.cuda(), None, None, None, [cache], 9, 9, 0, eps=0.0)
+    k = torch.empty(4, 2, 64, dtype=torch.bfloat16, device="cuda")
+    C.call("efm_kv_fp4_read", ctx, ptr(cache), 9, 5, 4, ptr(k), None, stream())
+    v = torch.empty(4, 2, 64, dtype=torch.bfloat16, device="cuda")
+    C.call("efm_kv_fp4_read", ctx, ptr(cache), 9, 5, 4, None, ptr(v), stream())
+    torch.cuda.synchronize()
+    assert torch.equal(k.cpu().double(), R.rounded(x[5:, 14:16])) and torch.equal(v.cpu().double(), R.rounded(x[5:, 16:]))
+
+
+def test_write_fp4_groups_that_are_not_finite(gpu):
+    g = _gen(6)
+    hq, hkv, hd = 12, 2, 128
+    ctx = C.make_attention_ctx(hq, hkv, hd, rope=False)
+    qkv = _bf(g, 4, (hq + 2 * hkv) * hd)
+    x = qkv.view(4, -1, hd)
+    x[1, hq, 40], x[2, hq + 1, 0], x[3, hq + 2, 127], x[0, hq + 3, 64] = math.nan, math.inf, -math.inf, math.nan
+    cache = _buf(C.load().efm_kv_fp4_bytes(ctx, 4))
+    _write(ctx, True, qkv.cuda(), None, None, None, [cache], 4, 4, 0)
+    k, v = _read(ctx, cache, 4, 0, 4, hkv, hd)
+    for got, ref in ((k, R.rounded(x[:, hq:hq + hkv])), (v, R.rounded(x[:, hq + hkv:]))):
+        assert int(torch.isnan(ref).sum()) == 64
+        assert torch.equal(torch.isnan(got), torch.isnan(ref)) and torch.equal(got.nan_to_num(0), ref.nan_to_num(0))
+
+
+# ---------------------------------------------------------------- attention
+
+def _fill(ctx, k, v, room, stale=0xff):
+    """A cache of `room` rows whose first hold k, v [kv, hkv, hd]; the rest holds `stale` bytes (0xff: NaN groups)."""
+    kv, hkv, hd = k.shape
+    hq = ctx.num_qo_heads
+    cache = _buf(C.load().efm_kv_fp4_bytes(ctx, room), stale)
+    if kv:
+        rows = torch.cat([torch.zeros(kv, hq * hd, dtype=torch.bfloat16), k.flatten(1), v.flatten(1)], 1).cuda()
+        none = C.make_attention_ctx(hq, hkv, hd, rope=False)
+        _write(none, True, rows, None, None, None, [cache], room, kv, 0)
+    torch.cuda.synchronize()
+    return cache
+
+
+def _decode(ctx, q, cache, room, kv, d_len=None, bound=0):
+    ws = _buf(C.load().efm_attention_decode_kv_fp4_workspace_bytes(ctx, bound or kv), 0xff)
+    o = torch.full((1, ctx.num_qo_heads, ctx.head_dim), 9.0, dtype=torch.bfloat16, device="cuda")
+    C.call("efm_attention_decode_kv_fp4", ctx, ptr(q), ptr(cache), room, ptr(o), kv, ptr(d_len), bound, ptr(ws), ws.numel(), stream())
+    torch.cuda.synchronize()
+    return o
+
+
+def _rows(ctx, q, cache, room, n, kv, causal=True):
+    ws = _buf(C.load().efm_attention_prefill_kv_fp4_workspace_bytes(ctx, n, kv), 0xff)
+    o = torch.full((n, ctx.num_qo_heads, ctx.head_dim), 9.0, dtype=torch.bfloat16, device="cuda")
+    C.call("efm_attention_prefill_kv_fp4", ctx, ptr(q), ptr(cache), room, ptr(o), n, kv, int(causal), ptr(ws), ws.numel(), stream())
+    torch.cuda.synchronize()
+    return o
+
+
+def _qkv(seed, n, kv, hq, hkv, hd):
+    g = _gen(seed)
+    k = _bf(g, kv, hkv, hd)
+    k[..., 5] *= 6
+    return _bf(g, n, hq, hd), k, _bf(g, kv, hkv, hd)
+
+
+@pytest.mark.parametrize("hq,hkv,hd", HEADS + [pytest.param(2, 2, 128, id="mha"), pytest.param(16, 2, 64, id="8of64"),
+                                                pytest.param(3, 1, 64, id="3of64")])
+@pytest.mark.parametrize("kv", [0, 1, 31, 32, 33, 257, 1000, 4099])
+def test_decode(gpu, hq, hkv, hd, kv):
+    """Host length, and the same with the length on the device under a larger bound; rows past it hold NaN groups."""
+    q, k, v = _qkv(kv + hd, 1, kv, hq, hkv, hd)
+    room = kv + 77
+    ctx = C.make_attention_ctx(hq, hkv, hd, rope=False)
+    cache = _fill(ctx, k, v, room)
+    ref, tol = R.attention(q.double(), R.rounded(k), R.rounded(v), False)
+    _within(_decode(ctx, q.cuda(), cache, room, kv), ref, tol, "host length")
+    d_len = torch.tensor([kv], dtype=torch.int32, device="cuda")
+    _within(_decode(ctx, q.cuda(), cache, room, 0, d_len, room), ref, tol, "device length")
+
+
+def test_decode_long(gpu):
+    q, k, v = _qkv(1, 1, 40001, 28, 4, 128)
+    ctx = C.make_attention_ctx(28, 4, 128, rope=False)
+    cache = _fill(ctx, k, v, 65536)
+    ref, tol = R.attention(q.double(), R.rounded(k), R.rounded(v), False)
+    _within(_decode(ctx, q.cuda(), cache, 65536, 40001), ref, tol)
+    d_len = torch.tensor([40001], dtype=torch.int32, device="cuda")
+    _within(_decode(ctx, q.cuda(), cache, 65536, 0, d_len, 65536), ref, tol)
+
+
+def test_decode_length_beyond_the_bound(gpu):
+    """*d_kv_len past max_kv_len attends max_kv_len rows."""
+    q, k, v = _qkv(8, 1, 200, 12, 2, 128)
+    ctx = C.make_attention_ctx(12, 2, 128, rope=False)
+    cache = _fill(ctx, k, v, 200)
+    d_len = torch.tensor([4000000], dtype=torch.int32, device="cuda")
+    ref, tol = R.attention(q.double(), R.rounded(k[:150]), R.rounded(v[:150]), False)
+    _within(_decode(ctx, q.cuda(), cache, 200, 0, d_len, 150), ref, tol)
+
+
+ROWS = [(1, 1), (1, 40), (2, 2), (7, 7), (16, 100), (33, 33), (37, 800), (5, 3001), (130, 130), (200, 1111), (515, 515), (700, 1500)]
+
+
+@pytest.mark.parametrize("hq,hkv,hd", HEADS)
+@pytest.mark.parametrize("n,kv", ROWS)
+@pytest.mark.parametrize("causal", [True, False])
+def test_rows(gpu, hq, hkv, hd, n, kv, causal):
+    q, k, v = _qkv(n + kv, n, kv, hq, hkv, hd)
+    room = kv + 5
+    ctx = C.make_attention_ctx(hq, hkv, hd, rope=False)
+    ref, tol = R.attention(q.double(), R.rounded(k), R.rounded(v), causal)
+    _within(_rows(ctx, q.cuda(), _fill(ctx, k, v, room), room, n, kv, causal), ref, tol)
+
+
+@pytest.mark.parametrize("hq,hkv,hd", [(1, 1, 128), (8, 4, 64), (24, 6, 128), (16, 2, 128)])
+@pytest.mark.parametrize("n,kv", [(19, 150), (300, 400)])
+def test_rows_head_layouts(gpu, hq, hkv, hd, n, kv):
+    q, k, v = _qkv(n, n, kv, hq, hkv, hd)
+    ctx = C.make_attention_ctx(hq, hkv, hd, rope=False)
+    ref, tol = R.attention(q.double(), R.rounded(k), R.rounded(v), True)
+    _within(_rows(ctx, q.cuda(), _fill(ctx, k, v, kv), kv, n, kv), ref, tol)
+
+
+@pytest.mark.parametrize("n", [1, 21, 600])
+def test_rows_strided_queries(gpu, n):
+    """Queries inside a wider buffer with the heads apart: strides of ctx."""
+    hq, hkv, hd, kv = 12, 2, 128, n + 90
+    q, k, v = _qkv(n, n, kv, hq, hkv, hd)
+    wide = torch.full((n, hq, 2, hd), math.nan, dtype=torch.bfloat16)
+    wide[:, :, 1] = q
+    wide = wide.cuda()
+    ctx = C.make_attention_ctx(hq, hkv, hd, rope=False, q_stride_n=hq * 2 * hd, q_stride_h=2 * hd)
+    ref, tol = R.attention(q.double(), R.rounded(k), R.rounded(v), True)
+    _within(_rows(ctx, wide[:, :, 1], _fill(ctx, k, v, kv), kv, n, kv), ref, tol)
+    if n == 1:
+        _within(_decode(ctx, wide[:, :, 1], _fill(ctx, k, v, kv), kv, kv), ref, tol)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("n,kv", [(1, 300), (40, 300), (700, 900)])
+def test_nan_groups_reach_the_rows_that_see_them(gpu, hd, n, kv):
+    """A NaN group of a key makes NaN of every row that sees the key, one of a value of that head's channels of the group
+    in those rows; rows before it, and the other KV head, keep their results."""
+    hq, hkv, at = 12, 2, kv - max(1, n // 2)
+    q, k, v = _qkv(n, n, kv, hq, hkv, hd)
+    ctx = C.make_attention_ctx(hq, hkv, hd, rope=False)
+    for what in ("key", "value"):
+        kk, vv = k.clone(), v.clone()
+        if what == "key":
+            kk[at, 1, 3] = math.nan
+        else:
+            vv[at, 0, 33] = math.inf
+        rk, rv = R.rounded(kk), R.rounded(vv)
+        ref, tol = R.attention(q.double(), rk.nan_to_num(0), rv.nan_to_num(0), True)
+        clean = torch.arange(n) + kv - n < at
+        if what == "key":
+            ref[~clean, hq // 2:] = math.nan
+        else:
+            ref[~clean, :hq // 2, 32:64] = math.nan
+        assert n == 1 or clean.any()
+        _within(_rows(ctx, q.cuda(), _fill(ctx, kk, vv, kv), kv, n, kv), ref, tol, what)
+        if n == 1:
+            _within(_decode(ctx, q.cuda(), _fill(ctx, kk, vv, kv + 9), kv + 9, kv), ref, tol, what + ", decode")
+
+
+@pytest.mark.parametrize("n", [1, 50, 600])
+def test_large_scores(gpu, n):
+    """Scores of thousands: one key takes all the weight, whichever wave or split holds it."""
+    hq, hkv, hd, kv = 12, 2, 128, n + 1200
+    q, k, v = _qkv(5, n, kv, hq, hkv, hd)
+    q, k = q * 16, k * 16
+    ctx = C.make_attention_ctx(hq, hkv, hd, rope=False)
+    ref, tol = R.attention(q.double(), R.rounded(k), R.rounded(v), True)
+    _within(_rows(ctx, q.cuda(), _fill(ctx, k, v, kv), kv, n, kv), ref, tol)
+
+
+def test_decode_in_a_graph(gpu):
+    """Two captured steps of different heads share a workspace, and follow the length on the device."""
+    lib = C.load()
+    shapes = [(28, 4, 128, 5000), (14, 2, 64, 900)]
+    bufs = []
+    for hq, hkv, hd, room in shapes:
+        q, k, v = _qkv(room, 1, room, hq, hkv, hd)
+        ctx = C.make_attention_ctx(hq, hkv, hd, rope=False)
+        bufs.append((ctx, q.cuda(), _fill(ctx, k, v, room), room, torch.empty(1, hq, hd, dtype=torch.bfloat16, device="cuda")))
+    d_len = torch.tensor([1], dtype=torch.int32, device="cuda")
+    ws = _buf(max(lib.efm_attention_decode_kv_fp4_workspace_bytes(b[0], b[3]) for b in bufs))
+    s, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=s, capture_error_mode="thread_local"):
+        for ctx, q, cache, room, o in bufs:
+            C.call("efm_attention_decode_kv_fp4", ctx, ptr(q), ptr(cache), room, ptr(o), 0, ptr(d_len), room, ptr(ws), ws.numel(), s.cuda_stream)
+    for length in (700, 33, 900, 1):
+        d_len.fill_(length)
+        ws.fill_(0xff)
+        torch.randn(1 << 18, device="cuda").sum()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        for ctx, q, cache, room, o in bufs:
+            assert torch.equal(o, _decode(ctx, q, cache, room, 0, d_len, room))
+
+
+# ---------------------------------------------------------------- together
+
+def test_layer_step_and_prompt(gpu):
+    """A layer with FP4 weights over an FP4 cache, as a program runs it: a prompt of 45 rows, then steps of one row with the
+    length on the device. Each operator's output is checked against 64 bits on the inputs that it was given."""
+    g = _gen(12)
+    hidden, hq, hkv, hd, inter, room, S = 512, 8, 2, 64, 1024, 64, 45
+    width = (hq + 2 * hkv) * hd
+    mats = {n: _weights(g, o, k) for n, o, k in (("qkv", width, hidden), ("o", hidden, hq * hd), ("gu", 2 * inter, hidden), ("down", hidden, inter))}
+    packed = {n: _pack(R.halves(c), b) for n, (c, b) in mats.items()}
+    w64 = {n: R.values(c, b) for n, (c, b) in mats.items()}
+    qw, kw, bias = 1 + _bf(g, hd, std=0.2), 1 + _bf(g, hd, std=0.2), _bf(g, width)
+    rope, ctx = C.make_attention_ctx(hq, hkv, hd), C.make_attention_ctx(hq, hkv, hd, rope=False)
+    cache = _buf(C.load().efm_kv_fp4_bytes(ctx, room), 0xff)
+    d_len = torch.tensor([S], dtype=torch.int32, device="cuda")
+    dev = [t.cuda() for t in (qw, kw, bias)]
+    keys, vals = torch.zeros(0, hkv, hd, dtype=torch.float64), torch.zeros(0, hkv, hd, dtype=torch.float64)
+
+    def check_linear(y, x, name, b=None):
+        ref, tol = _product(x.cpu().double(), w64[name])
+        if b is not None:
+            ref = ref + b.double()
+        _within(y, ref, tol + 2.0 ** -23 * ref.abs() + HALF * (ref.abs() + tol), name)
+
+    base = 0
+    for n in (S, 1, 1, 1):
+        x = _bf(g, n, hidden).cuda()
+        qkv = _linear(x, packed["qkv"], hidden, width, dev[2])
+        check_linear(qkv, x, "qkv", bias)
+        q = torch.empty(n, hq, hd, dtype=torch.bfloat16, device="cuda")
+        if n == 1:
+            d_len += 1
+            _write(rope, True, qkv, dev[0], dev[1], q, [cache], room, 1, 0, d_len=d_len)
+        else:
+            _write(rope, True, qkv, dev[0], dev[1], q, [cache], room, n, 0)
+        rows = qkv.cpu().double().view(n, -1, hd)
+        pos = _positions(base, n, hd // 2)
+        keys = torch.cat([keys, R.rounded(R.norm_rope(rows[:, hq:hq + hkv], kw, 1e-6, pos, 1e6))])
+        vals = torch.cat([vals, R.rounded(rows[:, hq + hkv:])])
+        base += n
+        att = _rows(ctx, q, cache, room, n, base) if n > 1 else _decode(ctx, q, cache, room, 0, d_len, room)
+        ref, tol = R.attention(q.cpu().double(), keys, vals, True)
+        _within(att, ref, tol, "attention")
+        check_linear(_linear(att.view(n, -1), packed["o"], hq * hd, hidden), att.view(n, -1), "o")
+        mid = torch.empty(n, inter, dtype=torch.bfloat16, device="cuda")
+        ws = _buf(C.load().efm_fused_gate_up_swiglu_fp4_workspace_bytes(n, hidden, inter))
+        C.call("efm_fused_gate_up_swiglu_fp4", n, hidden, inter, ptr(x), ptr(packed["gu"]), ptr(mid), ptr(ws), ws.numel(), stream())
+        check_linear(_linear(mid, packed["down"], inter, hidden), mid, "down")
+
+
+def test_same_stream_order_on_a_side_stream(gpu):
+    """Write, read and attention queued on a side stream follow each other without host waits."""
+    hq, hkv, hd, kv = 12, 2, 128, 400
+    q, k, v = _qkv(3, 1, kv, hq, hkv, hd)
+    ctx = C.make_attention_ctx(hq, hkv, hd, rope=False)
+    rows = torch.cat([torch.zeros(kv, hq * hd, dtype=torch.bfloat16), k.flatten(1), v.flatten(1)], 1).cuda()
+    cache, qd = _buf(C.load().efm_kv_fp4_bytes(ctx, kv), 0xff), q.cuda()
+    ws = _buf(C.load().efm_attention_decode_kv_fp4_workspace_bytes(ctx, kv))
+    o = torch.empty(1, hq, hd, dtype=torch.bfloat16, device="cuda")
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    _write(ctx, True, rows, None, None, None, [cache], kv, kv, 0, on=s.cuda_stream)
+    C.call("efm_attention_decode_kv_fp4", ctx, ptr(qd), ptr(cache), kv, ptr(o), kv, None, 0, ptr(ws), ws.numel(), s.cuda_stream)
+    s.synchronize()
+    ref, tol = R.attention(q.double(), R.rounded(k), R.rounded(v), False)
+    _within(o, ref, tol)
