@@ -15,11 +15,15 @@
 
 #include <algorithm>
 #include <cmath>
+#include <utility>
 
 namespace efm {
 
 int validate_attention_ctx(const efm_attention_ctx* c, const char* who);
 int prefill_cus();
+
+constexpr int kKvFp4MaxSplits = 512;
+constexpr float kKvFp4Lazy = 8.f;
 
 struct KvFp4Args {
     const bf16_t* q;
@@ -34,255 +38,587 @@ struct KvFp4Args {
     int Hq, Hkv, G, causal;
     int rows;                  // S * G
     int split_tiles, splits;   // 32-key tiles of a split
+    int tiles;                 // of all keys there may be
+    int cus;
     float scale;               // log2(e) / sqrt(HD)
 };
 
-__device__ __forceinline__ float max_over_groups(float v) {
-    v = fmaxf(v, __shfl_xor(v, 16, kWave));
-    return fmaxf(v, __shfl_xor(v, 32, kWave));
+// Values of lanes l, l + 16, l + 32 and l + 48 combined, in all four.
+template <typename F>
+__device__ __forceinline__ float over_groups(float v, F f) {
+    auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = f(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return f(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 
+// What a lane holds of a 32-key tile: of each of its two 16-key operands a key's words and scale
+// bytes, and 8 consecutive keys' words of one octet of channels with their scale bytes.
 template <int HD>
 struct KvFp4Tile {
-    static constexpr int W = HD / 32;      // words a lane takes of a key
-    uint32_t k[2][W], ks[2];
-    uint32_t v[8];
-    uint2 vs;
+    static constexpr int W = HD / 32;
+    uint32_t k[2][W], ks[2], v[8], vs[2];
 };
 
-template <int HD, int NW>
-__global__ __launch_bounds__(NW * kWave) void kv_fp4_attn_kernel(KvFp4Args a) {
+// The softmax step of NT tiles of 32 keys for the lane's row: s, its products with keys key0 .. key0 + 7
+// of each tile, to weights; m, sum and the outputs so far follow a maximum larger by 2^kKvFp4Lazy in
+// weights, which is rare past a row's first keys: weights of up to that and their sums are as exact in
+// bf16 and fp32 as those of up to 1. pf: the weights as second operands of the second product.
+template <int MT, int NT>
+__device__ __forceinline__ void kv_fp4_softmax(const f32x4_t (*s)[2], int key0, bool masked, int sees, float scale, float& m,
+                                               float& sum, f32x4_t* o, bf16x8_t* pf) {
+    // v_maximum3_f32 takes three operands as they are; a NaN among them leaves m, and makes the row's sum NaN
+    auto larger = [](float x, float y) { return __builtin_elementwise_maximum(x, y); };
+    float p[NT][8], tops[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) p[t][i] = s[t][i / 4][i % 4];
+        if (masked) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) p[t][i] = key0 + 32 * t + i < sees ? p[t][i] : -INFINITY;
+        }
+        tops[t] = larger(larger(larger(larger(p[t][0], p[t][1]), p[t][2]), larger(larger(p[t][3], p[t][4]), p[t][5])), larger(p[t][6], p[t][7]));
+    }
+    float top = NT == 1 ? tops[0] : larger(tops[0], tops[NT - 1]);
+    top = larger(m, over_groups(top, larger));
+    if (__any(top > m + kKvFp4Lazy / scale)) {
+        const float alpha = top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - top) * scale);
+        sum *= alpha;
+#pragma unroll
+        for (int i = 0; i < MT; ++i) o[i] *= alpha;
+        m = top;
+    }
+    const float ref = m == -INFINITY ? 0.f : m * scale;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) p[t][i] = __builtin_amdgcn_exp2f(fmaf(p[t][i], scale, -ref));
+        sum += ((p[t][0] + p[t][1]) + (p[t][2] + p[t][3])) + ((p[t][4] + p[t][5]) + (p[t][6] + p[t][7]));
+        pf[t] = __builtin_bit_cast(bf16x8_t, pack8(p[t]));
+    }
+}
+
+// NaN in the channels of key k's NaN groups, for the rows that see it.
+template <int HD, int NQ>
+__device__ __forceinline__ void kv_fp4_put_nan(const uint8_t* vs, const KvFp4Layout& lay, int k, int g, const int* sees,
+                                               f32x4_t (*o)[HD / 16]) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const int oct = HD == 128 ? 4 * g + r : (4 * g + r) % 8;
+        const bool bad = vs[lay.v_scale(k, oct)] == kFp4ScaleNan;
+#pragma unroll
+        for (int n = 0; n < NQ; ++n)
+#pragma unroll
+            for (int i = 0; i < HD / 16; ++i)
+                if (bad && k < sees[n]) o[n][i][r] = __builtin_nanf("");
+    }
+}
+
+// NQ x 16 rows a workgroup; the waves walk the tiles of its split. Bound by memory while rows are
+// few: 4.25 bits a value, two tiles of loads (4.3 KB each a wave) under way.
+template <int HD, int NW, int NQ>
+__global__ __launch_bounds__(NW * kWave, NQ == 1 ? (HD == 128 ? 3 : 4) : NQ == 2 ? 2 : 1) void kv_fp4_attn_kernel(KvFp4Args a) {
     constexpr int W = HD / 32, MT = HD / 16;   // channel tiles of O^T
     constexpr int LDO = HD + 4;
     __shared__ float so[NW][16][LDO];
-    __shared__ float sml[NW][16][2];
+    __shared__ float sml[NQ][NW][16][2];
     const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, l = lane % 16, g = lane / 16;
-    const int r0 = blockIdx.x * 16, kvh = blockIdx.y, split = blockIdx.z;
-    uint32_t L = a.kv_len;
-    if (a.d_kv_len != nullptr) L = min(a.d_kv_len[0], a.max_kv_len);
-    const int row = r0 + l, tok = row / a.G, head = kvh * a.G + row % a.G;
-    const bool row_on = row < a.rows;
-    // keys that the lane's row sees, and that any row of the block does
-    const int sees = !row_on ? 0 : a.causal ? (int)L - (int)a.S + tok + 1 : (int)L;
-    const int last = min(r0 + 15, a.rows - 1) / a.G;
-    const int block_sees = a.causal ? (int)L - (int)a.S + last + 1 : (int)L;
-    const int first_sees = a.causal ? (int)L - (int)a.S + r0 / a.G + 1 : (int)L;   // the fewest
-    const int tile_end = min((block_sees + 31) / 32, (split + 1) * a.split_tiles);
-
+    // row blocks from the last, which see the most keys, the KV heads side by side
+    const int r0 = ((int)(gridDim.x / a.Hkv) - 1 - (int)(blockIdx.x / a.Hkv)) * (16 * NQ), kvh = blockIdx.x % a.Hkv, split = blockIdx.z;
     const KvFp4Layout lay(a.T, a.Hkv, HD);
-    const uint8_t* const kc = a.cache + lay.k(kvh);
-    const uint8_t* const vc = a.cache + lay.v(kvh);
-    const uint8_t* const ksc = a.cache + lay.ks(kvh);
-    const uint8_t* const vsc = a.cache + lay.vs(kvh);
-    const int oct = HD == 128 ? l : l % 8;                     // the lane's octet of channels
-    const int oshift = HD == 128 ? 0 : 16 * (l / 8);           // head_dim 64: two lanes share an octet
-
-    bf16x8_t qf[W];
-#pragma unroll
-    for (int w = 0; w < W; ++w) {
-        uint4 u = make_uint4(0, 0, 0, 0);
-        if (row_on) u = *reinterpret_cast<const uint4*>(a.q + (int64_t)tok * a.q_sn + (int64_t)head * a.q_sh + 32 * w + 8 * g);
-        qf[w] = __builtin_bit_cast(bf16x8_t, u);
-    }
-    f32x4_t o[MT];
-#pragma unroll
-    for (int i = 0; i < MT; ++i) o[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    float m = -INFINITY, sum = 0.f;
-
-    for (int t = split * a.split_tiles + wave; t < tile_end; t += NW) {
-        KvFp4Tile<HD> c;
+    const int oct = HD == 128 ? l : l % 8;            // the lane's octet of channels
+    const int oshift = HD == 128 ? 0 : 16 * (l / 8);  // head_dim 64: two lanes share an octet
+    const int kr = 8 * (l / 4) + l % 4;               // the lane's key in the first operand; the second's is 4 on
+    // 64-bit bases of the head, 32-bit offsets within it (max_rows <= 2^24)
+    const uint8_t* const kc = a.cache + lay.k(kvh) + kr * (HD / 2) + g * (HD / 8);
+    const uint8_t* const vc = a.cache + lay.v(kvh) + (g * (HD / 8) + oct) * 32;
+    const uint8_t* const ksc = a.cache + lay.ks(kvh) + kr * W;
+    const uint8_t* const vsc = a.cache + lay.vs(kvh) + (g * W + oct / 4) * 8;
+    auto load = [&](KvFp4Tile<HD>& c, int t) {
+        const uint32_t ko = (uint32_t)t * (32 * HD / 2), so_ = (uint32_t)t * (32 * W);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const size_t key = (size_t)t * 32 + 8 * (l / 4) + 4 * i + l % 4;
-            const uint8_t* p = kc + key * (HD / 2) + g * (HD / 8);
+            const uint8_t* p = kc + ko + i * (4 * HD / 2);
             if constexpr (HD == 128) {
                 const uint4 u = load_stream16(p);
                 c.k[i][0] = u.x, c.k[i][1] = u.y, c.k[i][2] = u.z, c.k[i][3] = u.w;
-                c.ks[i] = *reinterpret_cast<const uint32_t*>(ksc + key * 4);
+                c.ks[i] = *reinterpret_cast<const uint32_t*>(ksc + so_ + i * 4 * W);
             } else {
                 const uint2 u = *reinterpret_cast<const uint2*>(p);
                 c.k[i][0] = u.x, c.k[i][1] = u.y;
-                c.ks[i] = *reinterpret_cast<const uint16_t*>(ksc + key * 2);
+                c.ks[i] = *reinterpret_cast<const uint16_t*>(ksc + so_ + i * 4 * W);
             }
-        }
-        const size_t blk = (size_t)t * 4 + g;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const uint4 u = load_stream16(vc + (blk * (HD / 8) + oct) * 32 + 16 * i);
+            const uint4 u = load_stream16(vc + ko + 16 * i);
             c.v[4 * i] = u.x, c.v[4 * i + 1] = u.y, c.v[4 * i + 2] = u.z, c.v[4 * i + 3] = u.w;
         }
-        c.vs = *reinterpret_cast<const uint2*>(vsc + (blk * W + oct / 4) * 8);
+        const uint2 u = *reinterpret_cast<const uint2*>(vsc + so_);
+        c.vs[0] = u.x, c.vs[1] = u.y;
+    };
+    // the first tile is requested before the length is known: the cache holds it
+    int t = split * a.split_tiles + wave;
+    KvFp4Tile<HD> ta, tb;
+    if (t < min(a.tiles, (split + 1) * a.split_tiles)) load(ta, t);
+    uint32_t L = a.kv_len;
+    if (a.d_kv_len != nullptr) L = min(a.d_kv_len[0], a.max_kv_len);
+    // keys that the lane's row of query tile n sees
+    int sees[NQ];
+    bf16x8_t qf[NQ][W];
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+        const int row = r0 + 16 * n + l, tok = row / a.G, head = kvh * a.G + row % a.G;
+        const bool on = row < a.rows;
+        sees[n] = !on ? 0 : a.causal ? (int)L - (int)a.S + tok + 1 : (int)L;
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            uint4 u = make_uint4(0, 0, 0, 0);
+            if (on) u = *reinterpret_cast<const uint4*>(a.q + (int64_t)tok * a.q_sn + (int64_t)head * a.q_sh + 32 * w + 8 * g);
+            qf[n][w] = __builtin_bit_cast(bf16x8_t, u);
+        }
+    }
+    // keys that any row sees, and that every row sees
+    const int last = min(r0 + 16 * NQ - 1, a.rows - 1) / a.G;
+    const int any_sees = a.causal ? (int)L - (int)a.S + last + 1 : (int)L;
+    const int all_see = r0 + 16 * NQ > a.rows ? 0 : a.causal ? (int)L - (int)a.S + r0 / a.G + 1 : (int)L;
+    const int tile_end = min((any_sees + 31) / 32, (split + 1) * a.split_tiles);
 
-        f32x4_t s[2];
+    f32x4_t o[NQ][MT];
+    float m[NQ], sum[NQ];   // largest product and sum of a row's weights, of the lane's keys
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+        m[n] = -INFINITY, sum[n] = 0.f;
+#pragma unroll
+        for (int i = 0; i < MT; ++i) o[n][i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    }
+    auto process = [&](KvFp4Tile<HD>& c, int t) {
+        // S^T: the lane gets keys key0 + 4 i + r of its row. The conversion takes the scale's exponent
+        // bits alone, so the word's other scales need not be cleared.
+        f32x4_t s[NQ][2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            s[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int w = 0; w < W; ++w)
-                s[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                    fp4_unpack8(c.k[i][w], fp4_scale((c.ks[i] >> (8 * w)) & 255)), qf[w], s[i], 0, 0, 0);
-        }
-        // the lane's keys: key0 + 4 i + r
-        const int key0 = t * 32 + 8 * g;
-        float p[8];
+            for (int n = 0; n < NQ; ++n) s[n][i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int i = 0; i < 8; ++i) p[i] = s[i / 4][i % 4] * a.scale;
-        if (t * 32 + 32 > first_sees || r0 + 16 > a.rows) {
+            for (int w = 0; w < W; ++w) {
+                const bf16x8_t kf = fp4_unpack8(c.k[i][w], fp4_scale_at(c.ks[i], w));
 #pragma unroll
-            for (int i = 0; i < 8; ++i) p[i] = key0 + i < sees ? p[i] : -INFINITY;
-        }
-        float top = p[0];
-#pragma unroll
-        for (int i = 1; i < 8; ++i) top = fmaxf(top, p[i]);
-        top = fmaxf(m, max_over_groups(top));
-        if (__any(top > m)) {
-            const float alpha = top == -INFINITY ? 1.f : exp2f(m - top);
-            sum *= alpha;
-#pragma unroll
-            for (int i = 0; i < MT; ++i) o[i] *= alpha;
-            m = top;
-        }
-        const float ref = m == -INFINITY ? 0.f : m;
-        float part = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            p[i] = exp2f(p[i] - ref);
-            part += p[i];
-        }
-        sum += part;
-        const bf16x8_t pf = __builtin_bit_cast(bf16x8_t, pack8(p));
-
-        // values of keys past the end are zero, and so are NaN groups, whose rows get their NaN below
-        uint32_t vb[8];
-        bool nan = false;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            vb[i] = ((i < 4 ? c.vs.x : c.vs.y) >> (8 * (i % 4))) & 255;
-            const bool off = key0 + i >= (int)L;
-            if (off || vb[i] == kFp4ScaleNan) {
-                nan |= !off;
-                c.v[i] = 0;
-                if (off) vb[i] = 0;
+                for (int n = 0; n < NQ; ++n)
+                    s[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[n][w], s[n][i], 0, 0, 0);
             }
         }
-        const bool any_nan = __any(nan);
-#pragma unroll
-        for (int b = 0; b < MT / 2; ++b) {
-            uint32_t e[8];
+        const int key0 = t * 32 + 8 * g;
+        // Values of keys past the end are made zero, and so are NaN groups; the rows that see those get
+        // their NaN below.
+        bool nan = false;
+        const bool cut = t * 32 + 32 > (int)L;
+        const uint32_t ff = ((c.vs[0] & 0x7f7f7f7fu) + 0x01010101u) & c.vs[0], fg = ((c.vs[1] & 0x7f7f7f7fu) + 0x01010101u) & c.vs[1];
+        if (cut || __any(((ff | fg) & 0x80808080u) != 0)) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float sc = fp4_scale(vb[i] == kFp4ScaleNan ? 0 : vb[i]);
-                const uint32_t word = c.v[i] >> oshift;
-                e[i] = b == 0 ? fp4_pair<0>(word, sc) : b == 1 ? fp4_pair<1>(word, sc)
-                     : b == 2 ? fp4_pair<2>(word, sc) : fp4_pair<3>(word, sc);
-            }
-            uint4 lo, hi;
-            lo.x = __builtin_amdgcn_perm(e[1], e[0], 0x05040100), hi.x = __builtin_amdgcn_perm(e[1], e[0], 0x07060302);
-            lo.y = __builtin_amdgcn_perm(e[3], e[2], 0x05040100), hi.y = __builtin_amdgcn_perm(e[3], e[2], 0x07060302);
-            lo.z = __builtin_amdgcn_perm(e[5], e[4], 0x05040100), hi.z = __builtin_amdgcn_perm(e[5], e[4], 0x07060302);
-            lo.w = __builtin_amdgcn_perm(e[7], e[6], 0x05040100), hi.w = __builtin_amdgcn_perm(e[7], e[6], 0x07060302);
-            o[2 * b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, lo), pf, o[2 * b], 0, 0, 0);
-            o[2 * b + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, hi), pf, o[2 * b + 1], 0, 0, 0);
-        }
-        if (any_nan) {
-            // the output of a row that sees a key with a NaN group is NaN in the group's channels
-            for (int k = 0; k < 32; ++k) {
-                if (t * 32 + k >= (int)L) break;
-                const bool seen = t * 32 + k < sees;
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int ch = HD == 128 ? 8 * (4 * g + r) : 8 * ((4 * g + r) % 8);
-                    const bool bad = vsc[((size_t)(t * 4 + k / 8) * W + ch / 32) * 8 + k % 8] == kFp4ScaleNan;
-#pragma unroll
-                    for (int i = 0; i < MT; ++i)
-                        if (bad && seen) o[i][r] = __builtin_nanf("");
+                const uint32_t byte = (c.vs[i / 4] >> (8 * (i % 4))) & 255;
+                const bool off = key0 + i >= (int)L;
+                if (off || byte == kFp4ScaleNan) {
+                    nan |= !off;
+                    c.v[i] = 0;
+                    c.vs[i / 4] &= ~(255u << (8 * (i % 4)));
                 }
             }
+            nan = __any(nan);
         }
+        bf16x8_t pf[NQ];
+#pragma unroll
+        for (int n = 0; n < NQ; ++n)
+            kv_fp4_softmax<MT, 1>(&s[n], key0, t * 32 + 32 > all_see, sees[n], a.scale, m[n], sum[n], o[n], &pf[n]);
+        // O^T: byte b of the words is two channels of each key; pairs of keys of one channel are put
+        // together for the first operand
+        [&]<int... B>(std::integer_sequence<int, B...>) {
+            ([&] {
+                uint32_t e[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) e[i] = fp4_pair<B>(c.v[i] >> oshift, fp4_scale_at(c.vs[i / 4], i % 4));
+                uint4 lo, hi;
+                lo.x = __builtin_amdgcn_perm(e[1], e[0], 0x05040100), hi.x = __builtin_amdgcn_perm(e[1], e[0], 0x07060302);
+                lo.y = __builtin_amdgcn_perm(e[3], e[2], 0x05040100), hi.y = __builtin_amdgcn_perm(e[3], e[2], 0x07060302);
+                lo.z = __builtin_amdgcn_perm(e[5], e[4], 0x05040100), hi.z = __builtin_amdgcn_perm(e[5], e[4], 0x07060302);
+                lo.w = __builtin_amdgcn_perm(e[7], e[6], 0x05040100), hi.w = __builtin_amdgcn_perm(e[7], e[6], 0x07060302);
+#pragma unroll
+                for (int n = 0; n < NQ; ++n) {
+                    o[n][2 * B] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, lo), pf[n], o[n][2 * B], 0, 0, 0);
+                    o[n][2 * B + 1] =
+                        __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, hi), pf[n], o[n][2 * B + 1], 0, 0, 0);
+                }
+            }(), ...);
+        }(std::make_integer_sequence<int, MT / 2>{});
+        if (nan)
+            for (int k = t * 32; k < min(t * 32 + 32, (int)L); ++k)
+                kv_fp4_put_nan<HD, NQ>(a.cache + lay.vs(kvh), lay, k, g, sees, o);
+    };
+    // two tiles' registers in turn: the next tile is requested before a tile is multiplied
+    while (t < tile_end) {
+        load(tb, min(t + NW, tile_end - 1));
+        process(ta, t);
+        t += NW;
+        if (t >= tile_end) break;
+        load(ta, min(t + NW, tile_end - 1));
+        process(tb, t);
+        t += NW;
     }
-    sum += __shfl_xor(sum, 16, kWave);
-    sum += __shfl_xor(sum, 32, kWave);
-    if (g == 0) sml[wave][l][0] = m, sml[wave][l][1] = sum;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        const int op = 4 * g + r, d = HD == 128 ? 8 * op : 8 * (op % 8) + 4 * (op / 8);
-#pragma unroll
-        for (int i = 0; i < MT; i += 4)
-            *reinterpret_cast<float4*>(&so[wave][l][d + i]) = make_float4(o[i][r], o[i + 1][r], o[i + 2][r], o[i + 3][r]);
+    for (int n = 0; n < NQ; ++n) {
+        const float den = over_groups(sum[n], [](float x, float y) { return x + y; });
+        if (g == 0) sml[n][wave][l][0] = m[n] * a.scale, sml[n][wave][l][1] = den;
     }
-    __syncthreads();
-    for (int e = threadIdx.x; e < 16 * (HD / 4); e += NW * kWave) {
-        const int r = e / (HD / 4), d = e % (HD / 4) * 4, gr = r0 + r;
-        if (gr >= a.rows) continue;
-        float M = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < NW; ++w) M = fmaxf(M, sml[w][r][0]);
-        float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
-        float den = 0.f;
+    for (int n = 0; n < NQ; ++n) {
+        if (n > 0) __syncthreads();
 #pragma unroll
-        for (int w = 0; w < NW; ++w) {
-            const float f = M == -INFINITY ? 1.f : exp2f(sml[w][r][0] - M);
-            const float4 x = *reinterpret_cast<const float4*>(&so[w][r][d]);
-            t.x += f * x.x, t.y += f * x.y, t.z += f * x.z, t.w += f * x.w;
-            den += f * sml[w][r][1];
+        for (int r = 0; r < 4; ++r) {
+            const int op = 4 * g + r, d = HD == 128 ? 8 * op : 8 * (op % 8) + 4 * (op / 8);
+#pragma unroll
+            for (int i = 0; i < MT; i += 4)
+                *reinterpret_cast<float4*>(&so[wave][l][d + i]) = make_float4(o[n][i][r], o[n][i + 1][r], o[n][i + 2][r], o[n][i + 3][r]);
         }
-        if (a.splits == 1) {
-            const float inv = den == 0.f ? 0.f : 1.f / den;
-            const int tk = gr / a.G, h = kvh * a.G + gr % a.G;
-            *reinterpret_cast<uint2*>(a.o + ((int64_t)tk * a.Hq + h) * HD + d) =
-                make_uint2(pack_bf16x2(t.x * inv, t.y * inv), pack_bf16x2(t.z * inv, t.w * inv));
-        } else {
-            const int64_t at = ((int64_t)split * a.Hkv + kvh) * a.rows + gr;
-            *reinterpret_cast<float4*>(a.o_part + at * HD + d) = t;
-            if (d == 0) *reinterpret_cast<float2*>(a.ml_part + at * 2) = make_float2(M, den);
+        __syncthreads();
+        for (int e = threadIdx.x; e < 16 * (HD / 4); e += NW * kWave) {
+            const int r = e / (HD / 4), d = e % (HD / 4) * 4, gr = r0 + 16 * n + r;
+            if (gr >= a.rows) continue;
+            float M = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < NW; ++w) M = fmaxf(M, sml[n][w][r][0]);
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+            float den = 0.f;
+#pragma unroll
+            for (int w = 0; w < NW; ++w) {
+                const float f = M == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(sml[n][w][r][0] - M);
+                const float4 x = *reinterpret_cast<const float4*>(&so[w][r][d]);
+                acc.x += f * x.x, acc.y += f * x.y, acc.z += f * x.z, acc.w += f * x.w;
+                den += f * sml[n][w][r][1];
+            }
+            if (a.splits == 1) {
+                const float inv = den == 0.f ? 0.f : 1.f / den;
+                const int tk = gr / a.G, h = kvh * a.G + gr % a.G;
+                *reinterpret_cast<uint2*>(a.o + ((int64_t)tk * a.Hq + h) * HD + d) =
+                    make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+            } else {
+                const int64_t at = ((int64_t)split * a.Hkv + kvh) * a.rows + gr;
+                if (tile_end > split * a.split_tiles) *reinterpret_cast<float4*>(a.o_part + at * HD + d) = acc;
+                if (d == 0) *reinterpret_cast<float2*>(a.ml_part + at * 2) = make_float2(M, den);
+            }
         }
     }
 }
 
-// HD / 4 lanes a row: the outputs of its splits, weighted by exp2(m_s - max m).
-template <int HD>
+// Joins the splits of a row, weighted by exp2(m_s - max m): NT threads a row, HD / 4 across its
+// channels by P lanes that take every P-th split each and are added in order. Many rows have few
+// splits: a wave each; a decode step's few rows have many: a workgroup each.
+template <int HD, int NT>
 __global__ __launch_bounds__(256) void kv_fp4_merge_kernel(KvFp4Args a) {
-    const int per = 256 / (HD / 4);
-    const int64_t r = (int64_t)blockIdx.x * per + threadIdx.x / (HD / 4);
-    const int d = threadIdx.x % (HD / 4) * 4;
+    constexpr int C = HD / 4, P = NT / C, CH = 8, K = NT == 256 ? kKvFp4MaxSplits / 256 : 1, RW = 256 / NT;
+    __shared__ float wt[RW][K * NT], red_max[4], red_sum[4];
+    __shared__ float4 part[RW][P][C];
     const int64_t all = (int64_t)a.Hkv * a.rows;
-    if (r >= all) return;
-    uint32_t L = a.kv_len;
-    if (a.d_kv_len != nullptr) L = min(a.d_kv_len[0], a.max_kv_len);
-    const int used = min(a.splits, ((int)L + a.split_tiles * 32 - 1) / (a.split_tiles * 32));
-    float M = -INFINITY;
-    for (int s = 0; s < used; ++s) M = fmaxf(M, a.ml_part[(s * all + r) * 2]);
-    float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
+    const int rw = threadIdx.x / NT, tid = threadIdx.x % NT, c = tid % C, lane_p = tid / C;
+    const int64_t r = (int64_t)blockIdx.x * RW + rw, rr = min(r, all - 1);
+    // Every split has written its (maximum, sum); one that has no keys for the row has (-inf, 0), and
+    // perhaps no output. The first outputs are requested before that is known.
+    float4 x[CH];
+    const float* const op = a.o_part + rr * HD + c * 4;
+    auto request = [&](int s0) {
+#pragma unroll
+        for (int k = 0; k < CH; ++k)
+            x[k] = s0 + k * P < a.splits ? *reinterpret_cast<const float4*>(op + (int64_t)(s0 + k * P) * all * HD) : make_float4(0.f, 0.f, 0.f, 0.f);
+    };
+    request(lane_p);
+    float ms[K], ls[K], M = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        const int s = k * NT + tid;
+        const float2 ml = s < a.splits ? *reinterpret_cast<const float2*>(a.ml_part + ((int64_t)s * all + rr) * 2) : make_float2(-INFINITY, 0.f);
+        ms[k] = ml.x, ls[k] = ml.y;
+        M = fmaxf(M, ml.x);
+    }
+    M = wave_max_uniform(M);
+    if constexpr (NT == 256) {
+        if (tid % kWave == 0) red_max[tid / kWave] = M;
+        __syncthreads();
+        M = fmaxf(fmaxf(red_max[0], red_max[1]), fmaxf(red_max[2], red_max[3]));
+    }
     float den = 0.f;
-    for (int s = 0; s < used; ++s) {
-        const float2 ml = *reinterpret_cast<const float2*>(a.ml_part + (s * all + r) * 2);
-        const float f = M == -INFINITY ? 1.f : exp2f(ml.x - M);
-        const float4 x = *reinterpret_cast<const float4*>(a.o_part + (s * all + r) * HD + d);
-        t.x += f * x.x, t.y += f * x.y, t.z += f * x.z, t.w += f * x.w;
-        den += f * ml.y;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        const int s = k * NT + tid;
+        const bool used = ls[k] != 0.f || ms[k] != -INFINITY;
+        const float f = M == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ms[k] - M);
+        if (s < a.splits) wt[rw][s] = used ? f : -1.f;
+        if (used) den += f * ls[k];
+    }
+    den = wave_total(den);
+    if constexpr (NT == 256) {
+        if (tid % kWave == 0) red_sum[tid / kWave] = den;
+    }
+    __syncthreads();
+    if constexpr (NT == 256) den = (red_sum[0] + red_sum[1]) + (red_sum[2] + red_sum[3]);
+    float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s0 = lane_p; s0 < a.splits; s0 += CH * P) {
+        if (s0 != lane_p) request(s0);
+#pragma unroll
+        for (int k = 0; k < CH; ++k) {
+            const float f = s0 + k * P < a.splits ? wt[rw][s0 + k * P] : -1.f;
+            if (f < 0.f) continue;
+            t.x += f * x[k].x, t.y += f * x[k].y, t.z += f * x[k].z, t.w += f * x[k].w;
+        }
+    }
+    part[rw][lane_p][c] = t;
+    __syncthreads();
+    if (lane_p > 0 || r >= all) return;
+#pragma unroll
+    for (int p = 1; p < P; ++p) {
+        const float4 y = part[rw][p][c];
+        t.x += y.x, t.y += y.y, t.z += y.z, t.w += y.w;
     }
     const float inv = den == 0.f ? 0.f : 1.f / den;
     const int kvh = (int)(r / a.rows), gr = (int)(r % a.rows), tk = gr / a.G, h = kvh * a.G + gr % a.G;
-    *reinterpret_cast<uint2*>(a.o + ((int64_t)tk * a.Hq + h) * HD + d) =
+    *reinterpret_cast<uint2*>(a.o + ((int64_t)tk * a.Hq + h) * HD + c * 4) =
         make_uint2(pack_bf16x2(t.x * inv, t.y * inv), pack_bf16x2(t.z * inv, t.w * inv));
 }
 
+// Many rows: four waves with 32 rows each share the keys. 64 keys (a stage) at a time the waves make
+// a quarter of the stage's operands each, the codes of the next stage unpacked into LDS in the order
+// in which the lanes take them, while the present stage is multiplied: unpacking costs a row an eighth
+// of what it does above, and is hidden behind the matrix cores' other work.
+template <int HD>
+__global__ __launch_bounds__(256, 2) void kv_fp4_rows_kernel(KvFp4Args a) {
+    constexpr int W = HD / 32, MT = HD / 16, NQ = 2;
+    constexpr int FRAGS = 2 * W + MT;                // 1 KB operands of a 32-key tile: keys [2][W], values [MT]
+    __shared__ uint4 frag[2][2][FRAGS][kWave];       // [buffer][tile of the stage]
+    const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), l = lane % 16, g = lane / 16;
+    // Row blocks from the last, which see the most keys, the KV heads side by side. Where all workgroups
+    // are resident at once, two to a CU, the second to arrive at a CU is the lighter the heavier its first.
+    int rank = blockIdx.x;
+    if ((int)gridDim.x > a.cus && (int)gridDim.x <= 2 * a.cus && rank >= a.cus) rank = (int)gridDim.x - 1 - (rank - a.cus);
+    const int r0 = ((int)(gridDim.x / a.Hkv) - 1 - rank / a.Hkv) * (64 * NQ), kvh = rank % a.Hkv, split = blockIdx.z;
+    const KvFp4Layout lay(a.T, a.Hkv, HD);
+    const int L = (int)a.kv_len;
+    int sees[NQ];
+    bf16x8_t qf[NQ][W];
+    const int w0 = r0 + wave * 16 * NQ;
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+        const int row = w0 + 16 * n + l, tok = row / a.G, head = kvh * a.G + row % a.G;
+        const bool on = row < a.rows;
+        sees[n] = !on ? 0 : a.causal ? L - (int)a.S + tok + 1 : L;
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            uint4 u = make_uint4(0, 0, 0, 0);
+            if (on) u = *reinterpret_cast<const uint4*>(a.q + (int64_t)tok * a.q_sn + (int64_t)head * a.q_sh + 32 * w + 8 * g);
+            qf[n][w] = __builtin_bit_cast(bf16x8_t, u);
+        }
+    }
+    // keys that any row of the workgroup sees; that any and every row of the wave sees
+    const int last = min(r0 + 64 * NQ - 1, a.rows - 1) / a.G;
+    const int any_sees = a.causal ? L - (int)a.S + last + 1 : L;
+    const int wave_sees = w0 >= a.rows ? 0 : a.causal ? L - (int)a.S + min(w0 + 16 * NQ - 1, a.rows - 1) / a.G + 1 : L;
+    const int all_see = w0 + 16 * NQ > a.rows ? 0 : a.causal ? L - (int)a.S + w0 / a.G + 1 : L;
+    const int stage0 = split * a.split_tiles / 2, stage_end = min((any_sees + 63) / 64, (split + 1) * a.split_tiles / 2);
+
+    // this wave's part of a stage: tile wave / 2, operand wave % 2 of the keys, bytes (HD / 64) (wave % 2) on of
+    // the values' words
+    const int part = wave % 2;
+    const int oct = HD == 128 ? l : l % 8, oshift = (HD == 128 ? 0 : 16 * (l / 8)) + part * (HD / 8);
+    const int kr = (wave / 2) * 32 + 8 * (l / 4) + 4 * part + l % 4;
+    const uint8_t* const kc = a.cache + lay.k(kvh) + kr * (HD / 2) + g * (HD / 8);
+    const uint8_t* const vc = a.cache + lay.v(kvh) + (((wave / 2) * 4 + g) * (HD / 8) + oct) * 32;
+    const uint8_t* const ksc = a.cache + lay.ks(kvh) + kr * W;
+    const uint8_t* const vsc = a.cache + lay.vs(kvh) + (((wave / 2) * 4 + g) * W + oct / 4) * 8;
+    const int tile_max = (int)(a.T / 32) - 1;   // the cache's last tile; a stage may end past it
+    uint32_t ck[W], cks, cv[8], cvs[2];
+    bool saw_nan = false;
+    auto load = [&](int st) {
+        const int t = min(2 * st + wave / 2, tile_max) - wave / 2;   // the bases are at the wave's tile of stage 0
+        const int ko = t * (32 * HD / 2), sof = t * (32 * W);
+        if constexpr (HD == 128) {
+            const uint4 u = *reinterpret_cast<const uint4*>(kc + ko);
+            ck[0] = u.x, ck[1] = u.y, ck[2] = u.z, ck[3] = u.w;
+            cks = *reinterpret_cast<const uint32_t*>(ksc + sof);
+        } else {
+            const uint2 u = *reinterpret_cast<const uint2*>(kc + ko);
+            ck[0] = u.x, ck[1] = u.y;
+            cks = *reinterpret_cast<const uint16_t*>(ksc + sof);
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint4 u = *reinterpret_cast<const uint4*>(vc + ko + 16 * i);
+            cv[4 * i] = u.x, cv[4 * i + 1] = u.y, cv[4 * i + 2] = u.z, cv[4 * i + 3] = u.w;
+        }
+        const uint2 u = *reinterpret_cast<const uint2*>(vsc + sof);
+        cvs[0] = u.x, cvs[1] = u.y;
+    };
+    // unpack the codes at hand, of stage st, into a buffer; values past the end and NaN groups as zeros
+    auto unpack = [&](int st, int b) {
+        uint4 (*const f)[kWave] = frag[b][wave / 2];
+#pragma unroll
+        for (int w = 0; w < W; ++w) f[part * W + w][lane] = __builtin_bit_cast(uint4, fp4_unpack8(ck[w], fp4_scale_at(cks, w)));
+        const int key0 = (2 * st + wave / 2) * 32 + 8 * g;
+        const uint32_t ff = ((cvs[0] & 0x7f7f7f7fu) + 0x01010101u) & cvs[0], fg = ((cvs[1] & 0x7f7f7f7fu) + 0x01010101u) & cvs[1];
+        if (st * 64 + 64 > L || __any(((ff | fg) & 0x80808080u) != 0)) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const uint32_t byte = (cvs[i / 4] >> (8 * (i % 4))) & 255;
+                const bool off = key0 + i >= L;
+                if (off || byte == kFp4ScaleNan) {
+                    saw_nan |= !off;
+                    cv[i] = 0;
+                    cvs[i / 4] &= ~(255u << (8 * (i % 4)));
+                }
+            }
+        }
+        [&]<int... B>(std::integer_sequence<int, B...>) {
+            ([&] {
+                uint32_t e[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) e[i] = fp4_pair<B>(cv[i] >> oshift, fp4_scale_at(cvs[i / 4], i % 4));
+                uint4 lo, hi;
+                lo.x = __builtin_amdgcn_perm(e[1], e[0], 0x05040100), hi.x = __builtin_amdgcn_perm(e[1], e[0], 0x07060302);
+                lo.y = __builtin_amdgcn_perm(e[3], e[2], 0x05040100), hi.y = __builtin_amdgcn_perm(e[3], e[2], 0x07060302);
+                lo.z = __builtin_amdgcn_perm(e[5], e[4], 0x05040100), hi.z = __builtin_amdgcn_perm(e[5], e[4], 0x07060302);
+                lo.w = __builtin_amdgcn_perm(e[7], e[6], 0x05040100), hi.w = __builtin_amdgcn_perm(e[7], e[6], 0x07060302);
+                f[2 * W + part * (MT / 2) + 2 * B][lane] = lo;
+                f[2 * W + part * (MT / 2) + 2 * B + 1][lane] = hi;
+            }(), ...);
+        }(std::make_integer_sequence<int, MT / 4>{});
+    };
+
+    f32x4_t o[NQ][MT];
+    float m[NQ], sum[NQ];
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+        m[n] = -INFINITY, sum[n] = 0.f;
+#pragma unroll
+        for (int i = 0; i < MT; ++i) o[n][i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    }
+    auto meet = [&]() {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+    if (stage0 < stage_end) {
+        load(stage0);
+        unpack(stage0, 0);
+        load(min(stage0 + 1, stage_end - 1));
+    }
+    for (int st = stage0; st < stage_end; ++st) {
+        const int b = (st - stage0) & 1;
+        meet();   // this stage is in LDS, and the other buffer is read out
+        if (st + 1 < stage_end) unpack(st + 1, 1 - b);
+        load(min(st + 2, stage_end - 1));
+        if (st * 64 >= wave_sees) continue;
+        f32x4_t s[NQ][2][2];
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+#pragma unroll
+                for (int n = 0; n < NQ; ++n) s[n][tt][i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int w = 0; w < W; ++w) {
+                    const bf16x8_t kf = __builtin_bit_cast(bf16x8_t, frag[b][tt][i * W + w][lane]);
+#pragma unroll
+                    for (int n = 0; n < NQ; ++n)
+                        s[n][tt][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[n][w], s[n][tt][i], 0, 0, 0);
+                }
+            }
+        bf16x8_t pf[NQ][2];
+#pragma unroll
+        for (int n = 0; n < NQ; ++n)
+            kv_fp4_softmax<MT, 2>(s[n], st * 64 + 8 * g, st * 64 + 64 > all_see, sees[n], a.scale, m[n], sum[n], o[n], pf[n]);
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                const bf16x8_t vf = __builtin_bit_cast(bf16x8_t, frag[b][tt][2 * W + i][lane]);
+#pragma unroll
+                for (int n = 0; n < NQ; ++n)
+                    o[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[n][tt], o[n][i], 0, 0, 0);
+            }
+    }
+    // NaN groups of values reach the outputs of the rows that see them
+    meet();
+    int* const flag = reinterpret_cast<int*>(&frag[0][0][0][0]);
+    const bool wave_saw = __any(saw_nan);
+    if (lane == 0) flag[wave] = wave_saw;
+    meet();
+    if (flag[0] | flag[1] | flag[2] | flag[3])
+        for (int k = stage0 * 64; k < min(wave_sees, stage_end * 64); ++k)
+            kv_fp4_put_nan<HD, NQ>(a.cache + lay.vs(kvh), lay, k, g, sees, o);
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+        const float den = over_groups(sum[n], [](float x, float y) { return x + y; });
+        const int gr = w0 + 16 * n + l;
+        if (gr >= a.rows) continue;
+        const float inv = den == 0.f ? 0.f : 1.f / den;
+        const int tk = gr / a.G, h = kvh * a.G + gr % a.G;
+        const int64_t at = ((int64_t)split * a.Hkv + kvh) * a.rows + gr;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int op = 4 * g + r, d = HD == 128 ? 8 * op : 8 * (op % 8) + 4 * (op / 8);
+            if (a.splits == 1) {
+                bf16_t* const dst = a.o + ((int64_t)tk * a.Hq + h) * HD + d;
+#pragma unroll
+                for (int i = 0; i < MT; i += 4)
+                    *reinterpret_cast<uint2*>(dst + i) = make_uint2(pack_bf16x2(o[n][i][r] * inv, o[n][i + 1][r] * inv),
+                                                                   pack_bf16x2(o[n][i + 2][r] * inv, o[n][i + 3][r] * inv));
+            } else if (stage_end > stage0) {
+#pragma unroll
+                for (int i = 0; i < MT; i += 4)
+                    *reinterpret_cast<float4*>(a.o_part + at * HD + d + i) = make_float4(o[n][i][r], o[n][i + 1][r], o[n][i + 2][r], o[n][i + 3][r]);
+            }
+        }
+        if (a.splits > 1 && g == 0) *reinterpret_cast<float2*>(a.ml_part + at * 2) = make_float2(m[n] * a.scale, den);
+    }
+}
+
 struct KvFp4Plan {
-    int split_tiles, splits;
-    size_t o_bytes, ml_bytes;
+    bool shared;                           // kv_fp4_rows_kernel
+    int nw, nq, split_tiles, splits;
+    size_t o_bytes, ml_bytes;              // partial outputs and (maximum, sum)
+    size_t total() const { return o_bytes + ml_bytes; }
 };
 
-static KvFp4Plan kv_fp4_plan(const efm_attention_ctx* c, uint32_t S, uint32_t kv_len) {
-    const int G = (int)(c->num_qo_heads / c->num_kv_heads);
-    const int64_t rows = (int64_t)S * G, blocks = (rows + 15) / 16 * c->num_kv_heads;
+// Measured on 256 CUs (us). One row: 200 keys of 14/2 heads 3.8 in one workgroup a head, 6.3 split; 500
+// keys of 12/2 heads 5.4 and 6.6; 700 keys of 12/2 heads 6.8 and 6.6, of 14/2 heads of 64 5.5 and 6.3; 2000
+// keys of 28/4 heads 7.2 in workgroups of four waves, 7.4 of eight; 32771 keys 11.9 with up to 512
+// workgroups, 10.9 with 256. Rows, kv_fp4_attn_kernel with 16 and with 32 rows a workgroup and
+// kv_fp4_rows_kernel: 37 rows behind 8000 of 12/2 heads 13 / 16 / 20, 512 behind 512 of 28/4 heads 22 / 17 /
+// 29, 4096 of 28/4 heads - / 163 / 144, 8192 - / 583 / 489, 2048 behind 2048 - / 121 / 113, 2048 alone - /
+// 58 / 62, 1500 behind 2000 - / 89 / 106, 6000 of 16/2 heads - / 190 / 165.
+static KvFp4Plan kv_fp4_plan(const efm_attention_ctx* c, uint32_t S, uint32_t kv_len, bool causal) {
+    const int64_t Hkv = c->num_kv_heads, rows = (int64_t)S * (c->num_qo_heads / Hkv), cus = prefill_cus();
     const int tiles = (int)((kv_len + 31) / 32);
-    // two workgroups of 4 waves a CU, and at least a tile for each wave of a split
-    const int64_t want = std::max<int64_t>(1, 512 / std::max<int64_t>(1, blocks));
-    KvFp4Plan p;
-    p.split_tiles = std::max(4, (int)((tiles + want - 1) / want));
+    auto blocks_of = [&](int n) { return (rows + n - 1) / n * Hkv; };
+    KvFp4Plan p = {};
+    // The shared kernel's 128-row workgroups pay where they fill the CUs several times, or just twice and
+    // differ little in their keys.
+    const int64_t shared = blocks_of(128);
+    p.shared = c->head_dim == 128 && S > 1 &&
+               (2 * shared >= 5 * cus || (4 * shared >= 7 * cus && shared <= 2 * cus && (!causal || kv_len >= S + S / 2)));
+    p.nq = blocks_of(16) >= 2 * cus ? 2 : 1;
+    p.nw = p.nq == 2 ? 4 : 8;
+    const int64_t blocks = p.shared ? shared : blocks_of(16 * p.nq);
+    int least = p.nw;   // tiles of a split: one for each wave
+    if (S == 1) {
+        // few tiles: one workgroup a head and no second launch; else four waves until there is one a CU
+        const int alone = (c->head_dim == 64 ? 3 : 2) * 8;
+        if (tiles <= alone) least = alone;
+        else if ((tiles + 3) / 4 * blocks <= cus) p.nw = least = 4;
+    }
+    const int64_t want = std::max<int64_t>(1, cus / blocks);   // one workgroup a CU where keys are split
+    p.split_tiles = std::max({least, (int)((tiles + want - 1) / want), (tiles + kKvFp4MaxSplits - 1) / kKvFp4MaxSplits});
+    p.split_tiles += p.split_tiles % 2;   // whole stages
     p.splits = std::max(1, (tiles + p.split_tiles - 1) / p.split_tiles);
-    p.o_bytes = p.splits == 1 ? 0 : (size_t)p.splits * c->num_kv_heads * rows * c->head_dim * sizeof(float);
-    p.ml_bytes = p.splits == 1 ? 0 : (size_t)p.splits * c->num_kv_heads * rows * 2 * sizeof(float);
+    if (p.splits > 1) {
+        p.o_bytes = (size_t)p.splits * Hkv * rows * c->head_dim * sizeof(float);
+        p.ml_bytes = (size_t)p.splits * Hkv * rows * 2 * sizeof(float);
+    }
     return p;
 }
 
@@ -303,11 +639,12 @@ static int kv_fp4_attention(const char* who, const efm_attention_ctx* ctx, const
         return set_error(EFM_ERR_INVALID_ARGUMENT, "%s: pointers must be 16-byte aligned", who);
     if (S == 0) return EFM_OK;
     const int hd = (int)ctx->head_dim;
-    const KvFp4Plan p = kv_fp4_plan(ctx, S, bound);
-    if (p.splits > 1 && (workspace == nullptr || workspace_bytes < p.o_bytes + p.ml_bytes))
-        return set_error(EFM_ERR_WORKSPACE, "%s: workspace of %zu bytes required", who, p.o_bytes + p.ml_bytes);
-    if (p.splits > 1 && (reinterpret_cast<uintptr_t>(workspace) & 15u) != 0)
+    const KvFp4Plan p = kv_fp4_plan(ctx, S, bound, causal != 0);
+    if (p.total() > 0 && (workspace == nullptr || workspace_bytes < p.total()))
+        return set_error(EFM_ERR_WORKSPACE, "%s: workspace of %zu bytes required", who, p.total());
+    if (p.total() > 0 && (reinterpret_cast<uintptr_t>(workspace) & 15u) != 0)
         return set_error(EFM_ERR_INVALID_ARGUMENT, "%s: workspace must be 16-byte aligned", who);
+    const KvFp4Layout lay(KvFp4Layout::rows(max_rows), (int)ctx->num_kv_heads, hd);
     KvFp4Args a;
     a.q = static_cast<const bf16_t*>(q);
     a.cache = static_cast<const uint8_t*>(cache);
@@ -315,7 +652,7 @@ static int kv_fp4_attention(const char* who, const efm_attention_ctx* ctx, const
     a.o_part = static_cast<float*>(workspace);
     a.ml_part = reinterpret_cast<float*>(static_cast<char*>(workspace) + p.o_bytes);
     a.d_kv_len = d_kv_len;
-    a.T = KvFp4Layout::rows(max_rows);
+    a.T = lay.T;
     a.q_sn = ctx->q_stride_n ? ctx->q_stride_n : (int64_t)ctx->num_qo_heads * hd;
     a.q_sh = ctx->q_stride_h ? ctx->q_stride_h : hd;
     a.kv_len = kv_len;
@@ -328,16 +665,25 @@ static int kv_fp4_attention(const char* who, const efm_attention_ctx* ctx, const
     a.rows = (int)S * a.G;
     a.split_tiles = p.split_tiles;
     a.splits = p.splits;
+    a.tiles = (int)((bound + 31) / 32);
+    a.cus = prefill_cus();
     a.scale = 1.4426950408889634f / sqrtf((float)hd);
-    const dim3 grid((a.rows + 15) / 16, a.Hkv, p.splits);
-    const unsigned merge = (unsigned)(((int64_t)a.Hkv * a.rows + 256 / (hd / 4) - 1) / (256 / (hd / 4)));
-    if (hd == 128) {
-        hipLaunchKernelGGL((kv_fp4_attn_kernel<128, 4>), grid, dim3(256), 0, stream, a);
-        if (p.splits > 1) hipLaunchKernelGGL(kv_fp4_merge_kernel<128>, dim3(merge), dim3(256), 0, stream, a);
-    } else {
-        hipLaunchKernelGGL((kv_fp4_attn_kernel<64, 4>), grid, dim3(256), 0, stream, a);
-        if (p.splits > 1) hipLaunchKernelGGL(kv_fp4_merge_kernel<64>, dim3(merge), dim3(256), 0, stream, a);
-    }
+    const int block = p.shared ? 128 : 16 * p.nq;
+    const dim3 grid((unsigned)((a.rows + block - 1) / block * a.Hkv), 1, p.splits);
+    const int64_t all = (int64_t)a.Hkv * a.rows;
+    auto launch = [&](auto hdc) {
+        constexpr int HD = decltype(hdc)::value;
+        if (p.shared) hipLaunchKernelGGL(kv_fp4_rows_kernel<128>, grid, dim3(256), 0, stream, a);
+        else if (p.nq == 2) hipLaunchKernelGGL((kv_fp4_attn_kernel<HD, 4, 2>), grid, dim3(256), 0, stream, a);
+        else if (p.nw == 4) hipLaunchKernelGGL((kv_fp4_attn_kernel<HD, 4, 1>), grid, dim3(256), 0, stream, a);
+        else hipLaunchKernelGGL((kv_fp4_attn_kernel<HD, 8, 1>), grid, dim3(512), 0, stream, a);
+        if (p.splits > 1 && p.splits <= kWave && all >= 256)
+            hipLaunchKernelGGL((kv_fp4_merge_kernel<HD, kWave>), dim3((unsigned)((all + 3) / 4)), dim3(256), 0, stream, a);
+        else if (p.splits > 1)
+            hipLaunchKernelGGL((kv_fp4_merge_kernel<HD, 256>), dim3((unsigned)all), dim3(256), 0, stream, a);
+    };
+    if (hd == 128) launch(std::integral_constant<int, 128>{});
+    else launch(std::integral_constant<int, 64>{});
     return check_launch(who);
 }
 
@@ -347,8 +693,7 @@ using namespace efm;
 
 extern "C" size_t efm_attention_decode_kv_fp4_workspace_bytes(const efm_attention_ctx* ctx, uint32_t max_kv_len) {
     if (validate_attention_ctx(ctx, "attention_decode_kv_fp4_workspace_bytes") != EFM_OK) return 0;
-    const KvFp4Plan p = kv_fp4_plan(ctx, 1, max_kv_len);
-    return p.o_bytes + p.ml_bytes;
+    return kv_fp4_plan(ctx, 1, max_kv_len, false).total();
 }
 
 extern "C" int efm_attention_decode_kv_fp4(const efm_attention_ctx* ctx, const void* q, const void* cache, uint32_t max_rows,
@@ -361,8 +706,7 @@ extern "C" int efm_attention_decode_kv_fp4(const efm_attention_ctx* ctx, const v
 extern "C" size_t efm_attention_prefill_kv_fp4_workspace_bytes(const efm_attention_ctx* ctx, uint32_t qo_len,
                                                                uint32_t kv_len) {
     if (validate_attention_ctx(ctx, "attention_prefill_kv_fp4_workspace_bytes") != EFM_OK) return 0;
-    const KvFp4Plan p = kv_fp4_plan(ctx, qo_len, kv_len);
-    return p.o_bytes + p.ml_bytes;
+    return kv_fp4_plan(ctx, qo_len, kv_len, true).total();   // calls that `causal` sends elsewhere need none
 }
 
 extern "C" int efm_attention_prefill_kv_fp4(const efm_attention_ctx* ctx, const void* q, const void* cache, uint32_t max_rows,

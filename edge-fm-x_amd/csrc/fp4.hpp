@@ -27,6 +27,12 @@ constexpr int kFp4MinExp = -125;
 // The scale as fp32 (byte 0 comes out as 0, which the conversion reads as 2^-127).
 __device__ __forceinline__ float fp4_scale(uint32_t byte) { return __uint_as_float(byte << 23); }
 
+// Byte i of a word of scale bytes, for the conversions, which take the exponent bits alone: the
+// word's other bytes are not cleared from the sign and mantissa.
+__device__ __forceinline__ float fp4_scale_at(uint32_t bytes, int i) {
+    return __uint_as_float(i < 3 ? bytes << (23 - 8 * i) : bytes >> 1);
+}
+
 // Codes 2 B and 2 B + 1 of a word (low half byte first) as packed bf16.
 template <int B>
 __device__ __forceinline__ uint32_t fp4_pair(uint32_t word, float scale) {
