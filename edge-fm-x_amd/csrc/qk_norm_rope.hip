@@ -8,9 +8,17 @@
 // once a token and shared by its heads through LDS. Keys of an FP4 cache are computed in 64 bits
 // throughout, a small part of the row's work: a value next to a border of the grid lands on its
 // own side, whatever the order of a sum.
+//
+// Bound by memory once there are many tokens: 4096 tokens of 28/4 heads of 128 into a bf16 cache read
+// and write 76 MB in 14.4 us (5.2 TB/s, a copy's rate), into an FP4 cache 70 MB in 16 us. A token by itself
+// takes 3.1 us (bf16) and 4.3 us (FP4), of which an empty launch is 2: the rest is one chain of a load,
+// the angle's sine and cosine in 64 bits, the norm's sum, and the store. Reading 4096 such rows of an FP4
+// cache back (8.4 MB written) takes 5 us.
 #include "fp4.hpp"
 
+#include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 namespace efm {
 
@@ -36,38 +44,81 @@ struct QkWriteArgs {
     double turns[kMaxHalfDim];   // theta^(-2 d / hd) / rope_scale / (2 pi)
 };
 
-// Row y of 8 values from the lane's 8 and, in `other`, those of the lane that holds the other half
-// of its pairs; lo: this lane holds the first half.
-template <typename T>
-__device__ __forceinline__ void turn8(T* x, const double2* cs, int lane_mask, bool lo) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const T o = __shfl_xor(x[e], lane_mask, kWave);
-        const T c = (T)cs[e].x, s = (T)cs[e].y;
-        x[e] = lo ? x[e] * c - o * s : x[e] * c + o * s;
-    }
+// Sum over the LANES lanes of a row, alike in all of them.
+template <int LANES>
+__device__ __forceinline__ float row_sum(float v) {
+    v += dpp_f32<0xB1>(v);
+    v += dpp_f32<0x4E>(v);
+    v += dpp_f32<0x141>(v);
+    return LANES == 16 ? v + dpp_f32<0x140>(v) : v;
 }
+
+template <int LANES>
+__device__ __forceinline__ double row_sum(double v) {
+#pragma unroll
+    for (int m = 1; m < LANES; m *= 2) v += __shfl_xor(v, m, kWave);
+    return v;
+}
+
+// The value of the lane that holds the other half of this lane's pairs, LANES / 2 away.
+template <int LANES>
+__device__ __forceinline__ float row_other(float v) {
+    return LANES == 16 ? dpp_f32<0x128>(v) : dpp_f32<0x141>(dpp_f32<0x1B>(v));
+}
+
+template <int LANES>
+__device__ __forceinline__ double row_other(double v) { return __shfl_xor(v, LANES / 2, kWave); }
+
+__device__ __forceinline__ float inv_sqrt(float v) { return rsqrtf(v); }
+__device__ __forceinline__ double inv_sqrt(double v) { return 1.0 / sqrt(v); }
 
 template <typename T, int LANES>
 __device__ __forceinline__ void norm8(T* x, uint4 weight, T eps) {
     T sum = 0;
 #pragma unroll
     for (int e = 0; e < 8; ++e) sum += x[e] * x[e];
-#pragma unroll
-    for (int m = 1; m < LANES; m *= 2) sum += __shfl_xor(sum, m, kWave);
-    const T r = (T)1 / sqrt(sum / (T)(8 * LANES) + eps);
+    const T r = inv_sqrt(row_sum<LANES>(sum) / (T)(8 * LANES) + eps);
     float w[8];
     unpack8(weight, w);
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] = x[e] * r * (T)w[e];
 }
 
-// One workgroup a token; HD / 8 lanes a head.
-template <int HD, bool FP4>
-__global__ __launch_bounds__(256) void qk_norm_rope_write_kernel(QkWriteArgs a) {
-    constexpr int LANES = HD / 8, HALF = HD / 2;
-    __shared__ double2 cs[2][HALF];   // [query, key] (cos, sin)
-    const uint32_t t = blockIdx.x;
+// cs: (cos, sin), the sine negated for lanes of the first half.
+template <typename T, int LANES, typename CS>
+__device__ __forceinline__ void turn8(T* x, CS cs) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const T o = row_other<LANES>(x[e]);
+        const auto v = cs(e);
+        x[e] = x[e] * (T)v.x + o * (T)v.y;
+    }
+}
+
+// HD / 8 lanes a row of a head, 64 / (HD / 8) rows a wave. TOKENS: a workgroup takes that many
+// consecutive tokens, and a wave their rows of a head, so that all its lanes do the same (a row of
+// Q, K or V) and the words of a V block's rows leave together. Otherwise a workgroup takes one token,
+// and a wave several heads of it. Either way a lane keeps its token and channels: sines and cosines
+// stay in its registers for the queries, and the next two rows are on their way while it works on one.
+template <int HD, bool FP4, bool TOKENS>
+__global__ __launch_bounds__(TOKENS ? 512 : 1024) void qk_norm_rope_write_kernel(QkWriteArgs a) {
+    constexpr int LANES = HD / 8, HALF = HD / 2, ROWS = kWave / LANES, T = TOKENS ? ROWS : 1, HL = LANES / 2;
+    // (cos, sin) of [query, key], of both where their offsets agree; channel d at (d % 8) * HL + d / 8, so
+    // that the lanes of a row read beside each other
+    __shared__ double2 cs[2][T][HALF + 8];
+    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, waves = blockDim.x / kWave;
+    const int sub = lane / LANES, j = lane % LANES;
+    const uint32_t t0 = blockIdx.x * T, t = TOKENS ? t0 + sub : t0;
+    const bool on = t < a.S, lo = j < HL;
+    const int first = a.q_out != nullptr ? 0 : a.Hq, heads = a.Hq + 2 * a.Hkv;
+    const bf16_t* const src = a.qkv + (int64_t)(on ? t : t0) * a.qkv_sn + 8 * j;
+    const int step = TOKENS ? waves : waves * ROWS;
+    int h = first + (TOKENS ? wave : wave * ROWS + sub);
+    auto request = [&](int head) { return *reinterpret_cast<const uint4*>(src + (int64_t)min(head, heads - 1) * HD); };
+    uint4 next[2] = {request(h), request(h + step)};
+    uint4 qw = make_uint4(0, 0, 0, 0), kw = qw;
+    if (a.q_w != nullptr) qw = reinterpret_cast<const uint4*>(a.q_w)[j];
+    if (a.k_w != nullptr) kw = reinterpret_cast<const uint4*>(a.k_w)[j];
     uint32_t base = a.base;
     if (a.d_kv_len != nullptr) {
         const uint32_t L = a.d_kv_len[0];
@@ -75,106 +126,118 @@ __global__ __launch_bounds__(256) void qk_norm_rope_write_kernel(QkWriteArgs a) 
         base = L - a.S;
     }
     const uint32_t row = base + t;
-    const bf16_t* const src = a.qkv + (int64_t)t * a.qkv_sn;
+    const int same = a.pos != nullptr || a.q_off == a.k_off;
     if (a.rotate) {
-        for (int i = threadIdx.x; i < HD; i += 256) {
-            const int d = i % HALF, is_k = i / HALF;
+        for (int i = threadIdx.x; i < (same ? 1 : 2) * T * HALF; i += blockDim.x) {
+            const int at = i % HALF, d = at % HL * 8 + at / HL, tt = i / HALF % T, is_k = i / HALF / T;
             double p;
-            if (a.pos != nullptr) p = (double)a.pos[(d < a.cum0 ? 0 : d < a.cum1 ? 1 : 2) * a.pos_stride + t];
-            else p = (double)row + (double)(is_k ? a.k_off : a.q_off);
+            if (a.pos != nullptr)
+                p = (double)a.pos[(d < a.cum0 ? 0 : d < a.cum1 ? 1 : 2) * a.pos_stride + min(t0 + tt, a.S - 1)];
+            else p = (double)(base + t0 + tt) + (double)(is_k ? a.k_off : a.q_off);
             const double turn = p * a.turns[d];
             double s, c;
             sincospi(2.0 * (turn - rint(turn)), &s, &c);
-            cs[is_k][d] = make_double2(c, s);
+            cs[is_k][tt][at] = make_double2(c, s);
         }
         __syncthreads();
     }
-    const KvFp4Layout lay(KvFp4Layout::rows(a.max_rows), a.Hkv, HD);
-    const int j = threadIdx.x % LANES;
-    const bool lo = j < LANES / 2;
-    const int heads = a.Hq + 2 * a.Hkv;
-    const int first = a.q_out != nullptr ? 0 : a.Hq;
-    // whole waves walk the heads together: lanes exchange halves inside a head
-    for (int h0 = first + threadIdx.x / kWave * (kWave / LANES); h0 < heads; h0 += 256 / LANES) {
-        const int h = h0 + threadIdx.x % kWave / LANES;
-        const bool on = h < heads;
-        uint4 raw = make_uint4(0, 0, 0, 0);
-        if (on) raw = *reinterpret_cast<const uint4*>(src + (int64_t)h * HD + 8 * j);
-        const bool is_q = h < a.Hq, is_k = !is_q && h < a.Hq + a.Hkv;
-        const bf16_t* const w = is_q ? a.q_w : a.k_w;
-        if constexpr (FP4) {
-            if (__any(is_k)) {
-                float f[8];
-                unpack8(raw, f);
-                double x[8];
+    float2 csq[8];
+    if (a.rotate) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) x[e] = (double)f[e];
-                if (a.k_w != nullptr) norm8<double, LANES>(x, reinterpret_cast<const uint4*>(a.k_w)[j], (double)a.eps);
-                if (a.rotate) turn8<double>(x, &cs[1][8 * (j % (LANES / 2))], LANES / 2, lo);
+        for (int e = 0; e < 8; ++e) {
+            const double2 v = cs[0][TOKENS ? sub : 0][e * HL + j % HL];
+            csq[e] = make_float2((float)v.x, lo ? -(float)v.y : (float)v.y);
+        }
+    }
+    const KvFp4Layout lay(KvFp4Layout::rows(a.max_rows), a.Hkv, HD);
+    for (; __any(h < heads); h += step) {
+        const uint4 raw = next[0];
+        next[0] = next[1];
+        next[1] = request(h + 2 * step);
+        const bool is_q = h < a.Hq, is_k = !is_q && h < a.Hq + a.Hkv, is_v = !is_q && !is_k && h < heads;
+        if (__any(is_q)) {
+            float x[8];
+            unpack8(raw, x);
+            if (a.q_w != nullptr) norm8<float, LANES>(x, qw, a.eps);
+            if (a.rotate) turn8<float, LANES>(x, [&](int e) { return csq[e]; });
+            if (is_q && on)
+                *reinterpret_cast<uint4*>(a.q_out + (int64_t)t * a.q_sn + (int64_t)h * a.q_sh + 8 * j) = pack8(x);
+        }
+        if (__any(is_k)) {
+            using Y = std::conditional_t<FP4, double, float>;
+            float x[8];
+            unpack8(raw, x);
+            Y y[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[e] = (Y)x[e];
+            if (a.k_w != nullptr) norm8<Y, LANES>(y, kw, (Y)a.eps);
+            if (a.rotate) {
+                int at = j % HL;
+                asm volatile("" : "+v"(at));   // read here: held over the loop, they would cost 32 registers
+                turn8<Y, LANES>(y, [&](int e) {
+                    const double2 v = cs[same ? 0 : 1][TOKENS ? sub : 0][e * HL + at];
+                    return make_double2(v.x, lo ? -v.y : v.y);
+                });
+            }
+            const int kh = h - a.Hq;
+            if constexpr (FP4) {
                 uint64_t top = 0;
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    top = max(top, (uint64_t)(__double_as_longlong(x[e]) & 0x7fffffffffffffffll));
+                for (int e = 0; e < 8; ++e) top = max(top, (uint64_t)(__double_as_longlong(y[e]) & 0x7fffffffffffffffll));
                 top = max(top, (uint64_t)__shfl_xor((unsigned long long)top, 1, kWave));
                 top = max(top, (uint64_t)__shfl_xor((unsigned long long)top, 2, kWave));
-                const uint32_t byte = fp4_scale_byte(top);
-                const uint32_t word = fp4_encode8(x, byte);
-                if (is_k) {
-                    const int kh = h - a.Hq;
+                const uint32_t byte = fp4_scale_byte(top), word = fp4_encode8(y, byte);
+                if (is_k && on) {
                     *reinterpret_cast<uint32_t*>(a.cache + lay.k(kh) + lay.k_word(row, j)) = word;
                     if (j % 4 == 0) a.cache[lay.ks(kh) + lay.k_scale(row, j)] = (uint8_t)byte;
                 }
+            } else if (is_k && on) {
+                *reinterpret_cast<uint4*>(a.k_cache + (int64_t)row * a.k_sn + (int64_t)kh * a.k_sh + 8 * j) = pack8(y);
             }
         }
-        float x[8];
-        unpack8(raw, x);
-        if (FP4 ? __any(on && !is_q && !is_k) : false) {
-            uint32_t top = 0;
+        if (__any(is_v)) {
+            const int vh = h - a.Hq - a.Hkv;
+            if constexpr (FP4) {
+                float x[8];
+                unpack8(raw, x);
+                uint32_t top = 0;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
-            top = max(top, (uint32_t)__shfl_xor((int)top, 1, kWave));
-            top = max(top, (uint32_t)__shfl_xor((int)top, 2, kWave));
-            const uint32_t byte = fp4_scale_byte(top);
-            if (on && !is_q && !is_k) {
-                const int vh = h - a.Hq - a.Hkv;
-                *reinterpret_cast<uint32_t*>(a.cache + lay.v(vh) + lay.v_word(row, j)) = fp4_encode8(x, byte);
-                if (j % 4 == 0) a.cache[lay.vs(vh) + lay.v_scale(row, j)] = (uint8_t)byte;
+                for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
+                top = max(top, (uint32_t)__shfl_xor((int)top, 1, kWave));
+                top = max(top, (uint32_t)__shfl_xor((int)top, 2, kWave));
+                const uint32_t byte = fp4_scale_byte(top), word = fp4_encode8(x, byte);
+                if (is_v && on) {
+                    *reinterpret_cast<uint32_t*>(a.cache + lay.v(vh) + lay.v_word(row, j)) = word;
+                    if (j % 4 == 0) a.cache[lay.vs(vh) + lay.v_scale(row, j)] = (uint8_t)byte;
+                }
+            } else if (is_v && on) {
+                *reinterpret_cast<uint4*>(a.v_cache + (int64_t)row * a.v_sn + (int64_t)vh * a.v_sh + 8 * j) = raw;
             }
-        }
-        // queries, and keys of a bf16 cache
-        float y[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = x[e];
-        if (w != nullptr) norm8<float, LANES>(y, reinterpret_cast<const uint4*>(w)[j], a.eps);
-        if (a.rotate) turn8<float>(y, &cs[is_q ? 0 : 1][8 * (j % (LANES / 2))], LANES / 2, lo);
-        if (!on) continue;
-        if (is_q) {
-            *reinterpret_cast<uint4*>(a.q_out + (int64_t)t * a.q_sn + (int64_t)h * a.q_sh + 8 * j) = pack8(y);
-        } else if (!FP4) {
-            if (is_k)
-                *reinterpret_cast<uint4*>(a.k_cache + (int64_t)row * a.k_sn + (int64_t)(h - a.Hq) * a.k_sh + 8 * j) = pack8(y);
-            else
-                *reinterpret_cast<uint4*>(a.v_cache + (int64_t)row * a.v_sn + (int64_t)(h - a.Hq - a.Hkv) * a.v_sh + 8 * j) = raw;
         }
     }
 }
 
-// One lane for 8 channels of a row.
+// One lane for 8 channels of a row. Workgroups of the first half of the grid read keys, row after row;
+// the others values, 8 rows of an octet beside each other as they lie.
 template <int HD>
-__global__ __launch_bounds__(256) void kv_fp4_read_kernel(const uint8_t* cache, KvFp4Layout lay, uint32_t first, int64_t octets,
-                                                          uint4* k_out, uint4* v_out) {
-    const int64_t i = blockIdx.x * 256ll + threadIdx.x;
-    if (i >= octets) return;
-    const int j = (int)(i % (HD / 8)), h = (int)(i / (HD / 8) % lay.Hkv);
-    const size_t row = first + (size_t)(i / (HD / 8) / lay.Hkv);
-    if (k_out != nullptr) {
-        const uint32_t w = *reinterpret_cast<const uint32_t*>(cache + lay.k(h) + lay.k_word(row, j));
-        k_out[i] = __builtin_bit_cast(uint4, fp4_unpack8(w, fp4_scale(cache[lay.ks(h) + lay.k_scale(row, j)])));
+__global__ __launch_bounds__(256) void kv_fp4_read_kernel(const uint8_t* cache, KvFp4Layout lay, uint32_t first, uint32_t rows,
+                                                          uint32_t per, uint4* k_out, uint4* v_out) {
+    constexpr int J = HD / 8;
+    const bool values = blockIdx.x >= per;
+    uint4* const out = values ? v_out : k_out;
+    if (out == nullptr) return;
+    const int64_t i = (blockIdx.x - (values ? per : 0)) * 256ll + threadIdx.x;
+    int64_t row, h;
+    int j;
+    if (!values) {
+        j = (int)(i % J), h = i / J % lay.Hkv, row = first + i / J / lay.Hkv;
+    } else {
+        j = (int)(i / 8 % J), h = i / 8 / J % lay.Hkv, row = (first / 8 + i / 8 / J / lay.Hkv) * 8 + i % 8;
     }
-    if (v_out != nullptr) {
-        const uint32_t w = *reinterpret_cast<const uint32_t*>(cache + lay.v(h) + lay.v_word(row, j));
-        v_out[i] = __builtin_bit_cast(uint4, fp4_unpack8(w, fp4_scale(cache[lay.vs(h) + lay.v_scale(row, j)])));
-    }
+    if (row < first || row >= (int64_t)first + rows) return;
+    const uint32_t w = *reinterpret_cast<const uint32_t*>(cache + (values ? lay.v((int)h) + lay.v_word(row, j) : lay.k((int)h) + lay.k_word(row, j)));
+    const uint32_t byte = cache[values ? lay.vs((int)h) + lay.v_scale(row, j) : lay.ks((int)h) + lay.k_scale(row, j)];
+    out[((row - first) * lay.Hkv + h) * J + j] = __builtin_bit_cast(uint4, fp4_unpack8(w, fp4_scale(byte)));
 }
 
 static bool qk_aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -243,11 +306,27 @@ static int qk_write(const char* who, bool fp4, const efm_attention_ctx* ctx, con
         a.turns[d] = rotate && d < hd / 2 ? exp(-2.0 * d / (double)hd * log((double)ctx->rope_theta)) /
                                                 (double)ctx->rope_scale / 6.283185307179586476925
                                           : 0.0;
-    const dim3 grid(seq_len), block(256);
-    if (hd == 128 && fp4) hipLaunchKernelGGL((qk_norm_rope_write_kernel<128, true>), grid, block, 0, stream, a);
-    else if (hd == 128) hipLaunchKernelGGL((qk_norm_rope_write_kernel<128, false>), grid, block, 0, stream, a);
-    else if (fp4) hipLaunchKernelGGL((qk_norm_rope_write_kernel<64, true>), grid, block, 0, stream, a);
-    else hipLaunchKernelGGL((qk_norm_rope_write_kernel<64, false>), grid, block, 0, stream, a);
+    // A token a workgroup spreads few tokens over the chip; once its waves would fill the chip (16 a CU
+    // by the FP4 kernel's registers, 24 by the bf16 one's), tokens together do less apiece. Measured (us,
+    // one / together): 28/4 heads of 128, FP4: 64 tokens 4.5 / 5.7, 512 7.4 / 6.6, 1024 13.1 / 8.0, 4096
+    // 37 / 16; bf16: 64 3.4 / 4.6, 512 4.6 / 5.2, 1024 9.1 / 6.6, 4096 25.2 / 14.4. 14/2 heads of 64, 2000
+    // tokens: FP4 8.6 / 5.6, bf16 5.4 / 4.7.
+    auto launch = [&](auto hdc, auto fc) {
+        constexpr int HD = decltype(hdc)::value, ROWS = kWave * 8 / HD;
+        constexpr bool F = decltype(fc)::value;
+        const int64_t heads = (q_out ? Hq : 0) + 2 * Hkv, waves = std::min<int64_t>(16, (heads + ROWS - 1) / ROWS);
+        if (seq_len * waves >= (F ? 4096 : 6144))
+            hipLaunchKernelGGL((qk_norm_rope_write_kernel<HD, F, true>), dim3((seq_len + ROWS - 1) / ROWS),
+                               dim3(kWave * (unsigned)std::min<int64_t>(8, heads)), 0, stream, a);
+        else
+            hipLaunchKernelGGL((qk_norm_rope_write_kernel<HD, F, false>), dim3(seq_len), dim3(kWave * (unsigned)waves), 0,
+                               stream, a);
+    };
+    using std::integral_constant;
+    if (hd == 128 && fp4) launch(integral_constant<int, 128>{}, std::true_type{});
+    else if (hd == 128) launch(integral_constant<int, 128>{}, std::false_type{});
+    else if (fp4) launch(integral_constant<int, 64>{}, std::true_type{});
+    else launch(integral_constant<int, 64>{}, std::false_type{});
     return check_launch(who);
 }
 
@@ -290,14 +369,16 @@ extern "C" int efm_kv_fp4_read(const efm_attention_ctx* ctx, const void* cache, 
         return set_error(EFM_ERR_INVALID_ARGUMENT, "kv_fp4_read: rows %u + %u do not fit max_rows %u", first, rows, max_rows);
     if (rows == 0) return EFM_OK;
     const KvFp4Layout lay(KvFp4Layout::rows(max_rows), (int)ctx->num_kv_heads, (int)ctx->head_dim);
-    const int64_t octets = (int64_t)rows * ctx->num_kv_heads * (ctx->head_dim / 8);
-    if (octets > (1ll << 38)) return set_error(EFM_ERR_UNSUPPORTED, "kv_fp4_read: too many rows");
-    const dim3 grid((unsigned)((octets + 255) / 256));
-    if (ctx->head_dim == 128)
-        hipLaunchKernelGGL(kv_fp4_read_kernel<128>, grid, dim3(256), 0, stream, static_cast<const uint8_t*>(cache), lay, first,
-                           octets, static_cast<uint4*>(k_out), static_cast<uint4*>(v_out));
-    else
-        hipLaunchKernelGGL(kv_fp4_read_kernel<64>, grid, dim3(256), 0, stream, static_cast<const uint8_t*>(cache), lay, first,
-                           octets, static_cast<uint4*>(k_out), static_cast<uint4*>(v_out));
+    // lanes for keys, and for values' whole blocks of 8 rows, the larger count
+    const int64_t lanes = ((int64_t)rows + 14) / 8 * 8 * ctx->num_kv_heads * (ctx->head_dim / 8);
+    if (lanes > (1ll << 38)) return set_error(EFM_ERR_UNSUPPORTED, "kv_fp4_read: too many rows");
+    const uint32_t per = (uint32_t)((lanes + 255) / 256);
+    auto launch = [&](auto hdc) {
+        hipLaunchKernelGGL(kv_fp4_read_kernel<decltype(hdc)::value>, dim3(2 * per), dim3(256), 0, stream,
+                           static_cast<const uint8_t*>(cache), lay, first, rows, per, static_cast<uint4*>(k_out),
+                           static_cast<uint4*>(v_out));
+    };
+    if (ctx->head_dim == 128) launch(std::integral_constant<int, 128>{});
+    else launch(std::integral_constant<int, 64>{});
     return check_launch("kv_fp4_read");
 }
