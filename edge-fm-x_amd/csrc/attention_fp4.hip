@@ -386,9 +386,9 @@ __global__ __launch_bounds__(256) void kv_fp4_merge_kernel(KvFp4Args a) {
 // a quarter of the stage's operands each, the codes of the next stage unpacked into LDS in the order
 // in which the lanes take them, while the present stage is multiplied: unpacking costs a row an eighth
 // of what it does above, and is hidden behind the matrix cores' other work.
-template <int HD>
+// Heads of 128; the keys are not split, since there are rows enough.
 __global__ __launch_bounds__(256, 2) void kv_fp4_rows_kernel(KvFp4Args a) {
-    constexpr int W = HD / 32, MT = HD / 16, NQ = 2;
+    constexpr int HD = 128, W = HD / 32, MT = HD / 16, NQ = 2;
     constexpr int FRAGS = 2 * W + MT;                // 1 KB operands of a 32-key tile: keys [2][W], values [MT]
     __shared__ uint4 frag[2][2][FRAGS][kWave];       // [buffer][tile of the stage]
     const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), l = lane % 16, g = lane / 16;
@@ -396,7 +396,7 @@ __global__ __launch_bounds__(256, 2) void kv_fp4_rows_kernel(KvFp4Args a) {
     // are resident at once, two to a CU, the second to arrive at a CU is the lighter the heavier its first.
     int rank = blockIdx.x;
     if ((int)gridDim.x > a.cus && (int)gridDim.x <= 2 * a.cus && rank >= a.cus) rank = (int)gridDim.x - 1 - (rank - a.cus);
-    const int r0 = ((int)(gridDim.x / a.Hkv) - 1 - rank / a.Hkv) * (64 * NQ), kvh = rank % a.Hkv, split = blockIdx.z;
+    const int r0 = ((int)(gridDim.x / a.Hkv) - 1 - rank / a.Hkv) * (64 * NQ), kvh = rank % a.Hkv;
     const KvFp4Layout lay(a.T, a.Hkv, HD);
     const int L = (int)a.kv_len;
     int sees[NQ];
@@ -419,32 +419,26 @@ __global__ __launch_bounds__(256, 2) void kv_fp4_rows_kernel(KvFp4Args a) {
     const int any_sees = a.causal ? L - (int)a.S + last + 1 : L;
     const int wave_sees = w0 >= a.rows ? 0 : a.causal ? L - (int)a.S + min(w0 + 16 * NQ - 1, a.rows - 1) / a.G + 1 : L;
     const int all_see = w0 + 16 * NQ > a.rows ? 0 : a.causal ? L - (int)a.S + w0 / a.G + 1 : L;
-    const int stage0 = split * a.split_tiles / 2, stage_end = min((any_sees + 63) / 64, (split + 1) * a.split_tiles / 2);
+    const int stages = (any_sees + 63) / 64;
 
     // this wave's part of a stage: tile wave / 2, operand wave % 2 of the keys, bytes (HD / 64) (wave % 2) on of
     // the values' words
     const int part = wave % 2;
-    const int oct = HD == 128 ? l : l % 8, oshift = (HD == 128 ? 0 : 16 * (l / 8)) + part * (HD / 8);
+    const int oshift = part * (HD / 8);
     const int kr = (wave / 2) * 32 + 8 * (l / 4) + 4 * part + l % 4;
     const uint8_t* const kc = a.cache + lay.k(kvh) + kr * (HD / 2) + g * (HD / 8);
-    const uint8_t* const vc = a.cache + lay.v(kvh) + (((wave / 2) * 4 + g) * (HD / 8) + oct) * 32;
+    const uint8_t* const vc = a.cache + lay.v(kvh) + (((wave / 2) * 4 + g) * (HD / 8) + l) * 32;
     const uint8_t* const ksc = a.cache + lay.ks(kvh) + kr * W;
-    const uint8_t* const vsc = a.cache + lay.vs(kvh) + (((wave / 2) * 4 + g) * W + oct / 4) * 8;
+    const uint8_t* const vsc = a.cache + lay.vs(kvh) + (((wave / 2) * 4 + g) * W + l / 4) * 8;
     const int tile_max = (int)(a.T / 32) - 1;   // the cache's last tile; a stage may end past it
     uint32_t ck[W], cks, cv[8], cvs[2];
     bool saw_nan = false;
     auto load = [&](int st) {
         const int t = min(2 * st + wave / 2, tile_max) - wave / 2;   // the bases are at the wave's tile of stage 0
         const int ko = t * (32 * HD / 2), sof = t * (32 * W);
-        if constexpr (HD == 128) {
-            const uint4 u = *reinterpret_cast<const uint4*>(kc + ko);
-            ck[0] = u.x, ck[1] = u.y, ck[2] = u.z, ck[3] = u.w;
-            cks = *reinterpret_cast<const uint32_t*>(ksc + sof);
-        } else {
-            const uint2 u = *reinterpret_cast<const uint2*>(kc + ko);
-            ck[0] = u.x, ck[1] = u.y;
-            cks = *reinterpret_cast<const uint16_t*>(ksc + sof);
-        }
+        const uint4 c = *reinterpret_cast<const uint4*>(kc + ko);
+        ck[0] = c.x, ck[1] = c.y, ck[2] = c.z, ck[3] = c.w;
+        cks = *reinterpret_cast<const uint32_t*>(ksc + sof);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const uint4 u = *reinterpret_cast<const uint4*>(vc + ko + 16 * i);
@@ -501,16 +495,14 @@ __global__ __launch_bounds__(256, 2) void kv_fp4_rows_kernel(KvFp4Args a) {
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
     };
-    if (stage0 < stage_end) {
-        load(stage0);
-        unpack(stage0, 0);
-        load(min(stage0 + 1, stage_end - 1));
-    }
-    for (int st = stage0; st < stage_end; ++st) {
-        const int b = (st - stage0) & 1;
+    load(0);   // every row sees a key
+    unpack(0, 0);
+    load(min(1, stages - 1));
+    for (int st = 0; st < stages; ++st) {
+        const int b = st & 1;
         meet();   // this stage is in LDS, and the other buffer is read out
-        if (st + 1 < stage_end) unpack(st + 1, 1 - b);
-        load(min(st + 2, stage_end - 1));
+        if (st + 1 < stages) unpack(st + 1, 1 - b);
+        load(min(st + 2, stages - 1));
         if (st * 64 >= wave_sees) continue;
         f32x4_t s[NQ][2][2];
 #pragma unroll
@@ -548,7 +540,7 @@ __global__ __launch_bounds__(256, 2) void kv_fp4_rows_kernel(KvFp4Args a) {
     if (lane == 0) flag[wave] = wave_saw;
     meet();
     if (flag[0] | flag[1] | flag[2] | flag[3])
-        for (int k = stage0 * 64; k < min(wave_sees, stage_end * 64); ++k)
+        for (int k = 0; k < wave_sees; ++k)
             kv_fp4_put_nan<HD, NQ>(a.cache + lay.vs(kvh), lay, k, g, sees, o);
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
@@ -557,23 +549,14 @@ __global__ __launch_bounds__(256, 2) void kv_fp4_rows_kernel(KvFp4Args a) {
         if (gr >= a.rows) continue;
         const float inv = den == 0.f ? 0.f : 1.f / den;
         const int tk = gr / a.G, h = kvh * a.G + gr % a.G;
-        const int64_t at = ((int64_t)split * a.Hkv + kvh) * a.rows + gr;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const int op = 4 * g + r, d = HD == 128 ? 8 * op : 8 * (op % 8) + 4 * (op / 8);
-            if (a.splits == 1) {
-                bf16_t* const dst = a.o + ((int64_t)tk * a.Hq + h) * HD + d;
+            bf16_t* const dst = a.o + ((int64_t)tk * a.Hq + h) * HD + 8 * (4 * g + r);
 #pragma unroll
-                for (int i = 0; i < MT; i += 4)
-                    *reinterpret_cast<uint2*>(dst + i) = make_uint2(pack_bf16x2(o[n][i][r] * inv, o[n][i + 1][r] * inv),
-                                                                   pack_bf16x2(o[n][i + 2][r] * inv, o[n][i + 3][r] * inv));
-            } else if (stage_end > stage0) {
-#pragma unroll
-                for (int i = 0; i < MT; i += 4)
-                    *reinterpret_cast<float4*>(a.o_part + at * HD + d + i) = make_float4(o[n][i][r], o[n][i + 1][r], o[n][i + 2][r], o[n][i + 3][r]);
-            }
+            for (int i = 0; i < MT; i += 4)
+                *reinterpret_cast<uint2*>(dst + i) = make_uint2(pack_bf16x2(o[n][i][r] * inv, o[n][i + 1][r] * inv),
+                                                               pack_bf16x2(o[n][i + 2][r] * inv, o[n][i + 3][r] * inv));
         }
-        if (a.splits > 1 && g == 0) *reinterpret_cast<float2*>(a.ml_part + at * 2) = make_float2(m[n] * a.scale, den);
     }
 }
 
@@ -593,7 +576,7 @@ struct KvFp4Plan {
 // 58 / 62, 1500 behind 2000 - / 89 / 106, 6000 of 16/2 heads - / 190 / 165.
 static KvFp4Plan kv_fp4_plan(const efm_attention_ctx* c, uint32_t S, uint32_t kv_len, bool causal) {
     const int64_t Hkv = c->num_kv_heads, rows = (int64_t)S * (c->num_qo_heads / Hkv), cus = prefill_cus();
-    const int tiles = (int)((kv_len + 31) / 32);
+    const int tiles = (int)(((int64_t)kv_len + 31) / 32);
     auto blocks_of = [&](int n) { return (rows + n - 1) / n * Hkv; };
     KvFp4Plan p = {};
     // The shared kernel's 128-row workgroups pay where they fill the CUs several times, or just twice and
@@ -622,6 +605,15 @@ static KvFp4Plan kv_fp4_plan(const efm_attention_ctx* c, uint32_t S, uint32_t kv
     return p;
 }
 
+// Bytes that hold the partial results of every call of up to S rows behind up to kv_len keys. A call's
+// own need goes up and down with its sizes; splits <= min(tiles, CUs / blocks of 16 rows) bounds it.
+static size_t kv_fp4_workspace(const efm_attention_ctx* c, uint32_t S, uint32_t kv_len) {
+    const int64_t tiles = ((int64_t)kv_len + 31) / 32, cus = prefill_cus();
+    if (tiles <= 8) return 0;
+    const int64_t rows = std::min(std::min(tiles, cus) * S * (int64_t)c->num_qo_heads, 16 * cus);
+    return rows * (c->head_dim + 2) * sizeof(float);
+}
+
 static int kv_fp4_attention(const char* who, const efm_attention_ctx* ctx, const void* q, const void* cache, uint32_t max_rows,
                             void* o, uint32_t S, uint32_t kv_len, const uint32_t* d_kv_len, uint32_t max_kv_len, int causal,
                             void* workspace, size_t workspace_bytes, hipStream_t stream) {
@@ -638,6 +630,8 @@ static int kv_fp4_attention(const char* who, const efm_attention_ctx* ctx, const
     if (((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(cache) | reinterpret_cast<uintptr_t>(o)) & 15u) != 0)
         return set_error(EFM_ERR_INVALID_ARGUMENT, "%s: pointers must be 16-byte aligned", who);
     if (S == 0) return EFM_OK;
+    if (ctx->num_qo_heads > (1u << 16) || (uint64_t)S * ctx->num_qo_heads > (1ull << 30))
+        return set_error(EFM_ERR_UNSUPPORTED, "%s: %u rows of %u query heads", who, S, ctx->num_qo_heads);
     const int hd = (int)ctx->head_dim;
     const KvFp4Plan p = kv_fp4_plan(ctx, S, bound, causal != 0);
     if (p.total() > 0 && (workspace == nullptr || workspace_bytes < p.total()))
@@ -673,7 +667,7 @@ static int kv_fp4_attention(const char* who, const efm_attention_ctx* ctx, const
     const int64_t all = (int64_t)a.Hkv * a.rows;
     auto launch = [&](auto hdc) {
         constexpr int HD = decltype(hdc)::value;
-        if (p.shared) hipLaunchKernelGGL(kv_fp4_rows_kernel<128>, grid, dim3(256), 0, stream, a);
+        if (p.shared) hipLaunchKernelGGL(kv_fp4_rows_kernel, grid, dim3(256), 0, stream, a);
         else if (p.nq == 2) hipLaunchKernelGGL((kv_fp4_attn_kernel<HD, 4, 2>), grid, dim3(256), 0, stream, a);
         else if (p.nw == 4) hipLaunchKernelGGL((kv_fp4_attn_kernel<HD, 4, 1>), grid, dim3(256), 0, stream, a);
         else hipLaunchKernelGGL((kv_fp4_attn_kernel<HD, 8, 1>), grid, dim3(512), 0, stream, a);
@@ -693,7 +687,7 @@ using namespace efm;
 
 extern "C" size_t efm_attention_decode_kv_fp4_workspace_bytes(const efm_attention_ctx* ctx, uint32_t max_kv_len) {
     if (validate_attention_ctx(ctx, "attention_decode_kv_fp4_workspace_bytes") != EFM_OK) return 0;
-    return kv_fp4_plan(ctx, 1, max_kv_len, false).total();
+    return kv_fp4_workspace(ctx, 1, max_kv_len);
 }
 
 extern "C" int efm_attention_decode_kv_fp4(const efm_attention_ctx* ctx, const void* q, const void* cache, uint32_t max_rows,
@@ -706,7 +700,7 @@ extern "C" int efm_attention_decode_kv_fp4(const efm_attention_ctx* ctx, const v
 extern "C" size_t efm_attention_prefill_kv_fp4_workspace_bytes(const efm_attention_ctx* ctx, uint32_t qo_len,
                                                                uint32_t kv_len) {
     if (validate_attention_ctx(ctx, "attention_prefill_kv_fp4_workspace_bytes") != EFM_OK) return 0;
-    return kv_fp4_plan(ctx, qo_len, kv_len, true).total();   // calls that `causal` sends elsewhere need none
+    return kv_fp4_workspace(ctx, qo_len, kv_len);
 }
 
 extern "C" int efm_attention_prefill_kv_fp4(const efm_attention_ctx* ctx, const void* q, const void* cache, uint32_t max_rows,

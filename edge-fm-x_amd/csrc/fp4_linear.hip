@@ -546,7 +546,8 @@ static void w4_launch_few(const W4Args& a, int cus, hipStream_t stream) {
     auto each = [&](auto ntc) {
         go(ntc, integral_constant<int, 1>{}, std::true_type{});
         go(ntc, integral_constant<int, 2>{}, std::true_type{});
-        go(ntc, integral_constant<int, 1>{}, std::false_type{});
+        // x past LDS has 40 blocks and more: two under way, but for SwiGLU's 16 waves with two tiles each
+        if constexpr (EPI == W4_SWIGLU) go(ntc, integral_constant<int, 1>{}, std::false_type{});
         go(ntc, integral_constant<int, 2>{}, std::false_type{});
     };
     if constexpr (EPI != W4_SWIGLU) each(integral_constant<int, 1>{});

@@ -302,10 +302,10 @@ static int qk_write(const char* who, bool fp4, const efm_attention_ctx* ctx, con
     a.q_off = ctx->q_rope_pos_offset;
     a.k_off = ctx->k_rope_pos_offset;
     a.eps = eps;
-    for (int d = 0; d < kMaxHalfDim; ++d)
-        a.turns[d] = rotate && d < hd / 2 ? exp(-2.0 * d / (double)hd * log((double)ctx->rope_theta)) /
-                                                (double)ctx->rope_scale / 6.283185307179586476925
-                                          : 0.0;
+    if (rotate) {
+        const double l = log((double)ctx->rope_theta), scale = ctx->rope_scale;
+        for (int d = 0; d < hd / 2; ++d) a.turns[d] = exp(-2.0 * d / (double)hd * l) / scale / 6.283185307179586476925;
+    }
     // A token a workgroup spreads few tokens over the chip; once its waves would fill the chip (16 a CU
     // by the FP4 kernel's registers, 24 by the bf16 one's), tokens together do less apiece. Measured (us,
     // one / together): 28/4 heads of 128, FP4: 64 tokens 4.5 / 5.7, 512 7.4 / 6.6, 1024 13.1 / 8.0, 4096
@@ -353,7 +353,7 @@ extern "C" int efm_qk_norm_rope_write_kv_fp4(const efm_attention_ctx* ctx, const
 }
 
 extern "C" size_t efm_kv_fp4_bytes(const efm_attention_ctx* ctx, uint32_t max_rows) {
-    if (validate_attention_ctx(ctx, "kv_fp4_bytes") != EFM_OK) return 0;
+    if (validate_attention_ctx(ctx, "kv_fp4_bytes") != EFM_OK || ctx->num_qo_heads > (1u << 16) || max_rows > (1u << 24)) return 0;
     return KvFp4Layout(KvFp4Layout::rows(max_rows), (int)ctx->num_kv_heads, (int)ctx->head_dim).bytes();
 }
 
@@ -365,6 +365,8 @@ extern "C" int efm_kv_fp4_read(const efm_attention_ctx* ctx, const void* cache, 
     if (!qk_aligned(cache) || !qk_aligned(k_out) || !qk_aligned(v_out))
         return set_error(EFM_ERR_INVALID_ARGUMENT, "kv_fp4_read: pointers must be 16-byte aligned");
     if (max_rows > (1u << 24)) return set_error(EFM_ERR_UNSUPPORTED, "kv_fp4_read: max_rows %u too large", max_rows);
+    if (ctx->num_qo_heads > (1u << 16))
+        return set_error(EFM_ERR_UNSUPPORTED, "kv_fp4_read: %u query heads", ctx->num_qo_heads);
     if (first > max_rows || rows > max_rows - first)
         return set_error(EFM_ERR_INVALID_ARGUMENT, "kv_fp4_read: rows %u + %u do not fit max_rows %u", first, rows, max_rows);
     if (rows == 0) return EFM_OK;

@@ -558,8 +558,9 @@ int efm_kv_fp4_read(const efm_attention_ctx* ctx, const void* cache, uint32_t ma
  * attended rows is min(*d_kv_len, max_kv_len) when d_kv_len != NULL, else kv_len; none: o is
  * zero. fp32 softmax, P rounded to bf16 for the PV product. Rows past the attended ones are
  * never part of the result, whatever they hold. workspace:
- * efm_attention_decode_kv_fp4_workspace_bytes(ctx, max_kv_len or kv_len) bytes (0: none), no
- * initial contents required; calls that share one must be stream-ordered. */
+ * efm_attention_decode_kv_fp4_workspace_bytes(ctx, max_kv_len or kv_len) bytes (0: none), which
+ * every call with no more keys fits in, 16-byte aligned, no initial contents required; calls
+ * that share one must be stream-ordered. */
 size_t efm_attention_decode_kv_fp4_workspace_bytes(const efm_attention_ctx* ctx, uint32_t max_kv_len);
 int efm_attention_decode_kv_fp4(const efm_attention_ctx* ctx, const void* q, const void* cache, uint32_t max_rows, void* o,
                                 uint32_t kv_len, const uint32_t* d_kv_len, uint32_t max_kv_len, void* workspace,
@@ -568,7 +569,8 @@ int efm_attention_decode_kv_fp4(const efm_attention_ctx* ctx, const void* q, con
 /* efm_attention_prefill over an FP4 cache whose first kv_len rows include the queries' own:
  * q [qo_len, Hq, hd] (ctx->q_stride_*), o [qo_len, Hq * hd] contiguous, kv_len >= qo_len; when
  * causal, query i sees keys j <= i + (kv_len - qo_len). pos_encoding must be EFM_POS_NONE.
- * workspace: efm_attention_prefill_kv_fp4_workspace_bytes bytes (0: none), as above. */
+ * workspace: efm_attention_prefill_kv_fp4_workspace_bytes bytes (0: none), which every call
+ * with no more queries and keys fits in, as above. */
 size_t efm_attention_prefill_kv_fp4_workspace_bytes(const efm_attention_ctx* ctx, uint32_t qo_len, uint32_t kv_len);
 int efm_attention_prefill_kv_fp4(const efm_attention_ctx* ctx, const void* q, const void* cache, uint32_t max_rows,
                                  void* o, uint32_t qo_len, uint32_t kv_len, int32_t causal, void* workspace,

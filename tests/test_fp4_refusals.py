@@ -129,3 +129,23 @@ def test_rows_refusals(kw, want):
     assert _rows(**kw) == want
     assert C.load().efm_attention_prefill_kv_fp4_workspace_bytes(_ctx(10, 2, rope=False), 4, 64) == 0
     assert C.load().efm_attention_decode_kv_fp4_workspace_bytes(_ctx(rope=False), 4096) > 64
+
+
+def test_workspaces_serve_every_smaller_call():
+    """The bytes never fall as rows or keys grow; none for a few tiles of keys."""
+    lib = C.load()
+    for ctx in (_ctx(rope=False), _ctx(28, 4, rope=False), _ctx(14, 2, hd=64, rope=False)):
+        lens = [1, 200, 257, 900, 4000, 8192, 8193, 8300, 40000, 1 << 24, (1 << 32) - 1]
+        one = [lib.efm_attention_decode_kv_fp4_workspace_bytes(ctx, n) for n in lens]
+        assert one == sorted(one) and one[0] == 0
+        for rows in (1, 2, 40, 600, 5000):
+            many = [lib.efm_attention_prefill_kv_fp4_workspace_bytes(ctx, rows, n) for n in lens]
+            more = [lib.efm_attention_prefill_kv_fp4_workspace_bytes(ctx, rows + 1, n) for n in lens]
+            assert many == sorted(many) and all(a <= b for a, b in zip(many, more))
+
+
+def test_more_heads_than_an_index_holds():
+    big = _ctx(1 << 17, 1 << 17, rope=False)
+    assert _decode(ctx=big) == UNSUP and _rows(ctx=big) == UNSUP
+    assert _rows(ctx=_ctx(1 << 15, 1 << 15, rope=False), n=1 << 16, kv=1 << 16, room=1 << 16) == UNSUP
+    assert C.load().efm_kv_fp4_bytes(big, 64) == 0 and C.load().efm_kv_fp4_bytes(_ctx(), 1 << 25) == 0

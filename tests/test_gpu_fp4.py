@@ -137,6 +137,63 @@ def test_swiglu(gpu, m, hidden, inter):
     _within(y, silu * up, tol + (HALF + 2.0 ** -20) * ((silu * up).abs() + tol), f"{m} {hidden} {inter}")
 
 
+# sizes that between them take every shape of workgroup, with widths and lengths that end inside its tiles
+WIDE = [(7, 32, 50), (5, 32, 4177), (5, 1664, 4303), (17, 32, 4481), (19, 1568, 8650), (19, 5184, 4250), (17, 928, 34530),
+        (35, 672, 15219), (5, 32, 16530), (97, 160, 41515), (33, 1824, 64960), (71, 1088, 57690), (3, 8224, 70), (4, 6176, 65530),
+        (4, 1056, 65601), (2, 32, 65537)]
+
+
+def _columns(g, n):
+    return torch.cat([torch.arange(min(n, 150)), torch.randint(0, n, (200,), generator=g), torch.arange(max(0, n - 150), n)])
+
+
+def _weights_on_device(seed, out, k):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    half = torch.randint(0, 256, (out, k // 2), generator=g, dtype=torch.uint8, device="cuda")
+    return half, torch.randint(117, 123, (out, k // 32), generator=g, dtype=torch.uint8, device="cuda")
+
+
+def _values_of(half, byte, rows):
+    half, byte = half[rows.cuda()].cpu(), byte[rows.cuda()].cpu()
+    return R.values(torch.stack([half & 15, half >> 4], 2).flatten(1), byte)
+
+
+@pytest.mark.parametrize("m,k,out", WIDE)
+@pytest.mark.parametrize("f32", [False, True])
+def test_linear_every_shape(gpu, m, k, out, f32):
+    """Against 64 bits in the first and last columns and 200 others, equal to a second call in all."""
+    g = _gen(m + k + out)
+    half, byte = _weights_on_device(m + k, out, k)
+    packed, x = _pack(half, byte), _bf(g, m, k)
+    y = _linear(x.cuda(), packed, k, out, None, f32)
+    at = _columns(g, out)
+    ref, tol = _product(x.double(), _values_of(half, byte, at))
+    _within(y[:, at.cuda()], ref, tol if f32 else tol + HALF * (ref.abs() + tol), f"{m} x {k} -> {out}")
+    assert not y.isnan().any() and torch.equal(y, _linear(x.cuda(), packed, k, out, None, f32))
+
+
+@pytest.mark.parametrize("m,hidden,inter", [(5, 32, 16), (5, 544, 16), (17, 32, 2144), (18, 1504, 4160), (18, 5024, 2160),
+                                            (42, 992, 8272), (35, 672, 7936), (5, 32, 8288), (33, 32, 43248), (33, 1088, 56288),
+                                            (72, 1120, 28112), (4, 4192, 80), (4, 8224, 48), (2, 2080, 33040)])
+def test_swiglu_every_shape(gpu, m, hidden, inter):
+    g = _gen(m + hidden + inter)
+    half, byte = _weights_on_device(m + hidden, 2 * inter, hidden)
+    packed, x = _pack(half, byte), _bf(g, m, hidden)
+    xd, ys = x.cuda(), []
+    for _ in range(2):
+        ys.append(torch.full((m, inter), math.nan, dtype=torch.bfloat16, device="cuda"))
+        C.call("efm_fused_gate_up_swiglu_fp4", m, hidden, inter, ptr(xd), ptr(packed), ptr(ys[-1]), None, 0, stream())
+    torch.cuda.synchronize()
+    at = _columns(g, inter)
+    up, eu = _product(x.double(), _values_of(half, byte, at))
+    gate, eg = _product(x.double(), _values_of(half, byte, at + inter))
+    silu = gate * torch.sigmoid(gate)
+    du, dg = eu + HALF * (up.abs() + eu), eg + HALF * (gate.abs() + eg)
+    tol = 1.1 * dg * (up.abs() + du) + silu.abs() * du   # |silu'| < 1.1
+    _within(ys[0][:, at.cuda()], silu * up, tol + (HALF + 2.0 ** -20) * ((silu * up).abs() + tol), f"{m} {hidden} {inter}")
+    assert not ys[0].isnan().any() and torch.equal(*ys)
+
+
 @pytest.mark.parametrize("m", [1, 20, 200])
 def test_linear_nan_stays_in_its_place(gpu, m):
     """A NaN group reaches its own output column alone, a NaN row of x its own row; rows and columns that pad the tiles
@@ -431,6 +488,69 @@ def test_rows_head_layouts(gpu, hq, hkv, hd, n, kv):
     ctx = C.make_attention_ctx(hq, hkv, hd, rope=False)
     ref, tol = R.attention(q.double(), R.rounded(k), R.rounded(v), True)
     _within(_rows(ctx, q.cuda(), _fill(ctx, k, v, kv), kv, n, kv), ref, tol)
+
+
+# Many blocks of 128 rows: workgroups that share the unpacked keys
+SHARED = [(64, 64, 1000, 1501, True), (64, 64, 1000, 1000, False), (96, 96, 900, 900, True), (256, 32, 340, 340, True),
+          (320, 320, 130, 333, True), (320, 320, 130, 131, False), (224, 32, 366, 397, True), (640, 640, 2, 77, True),
+          (640, 640, 2, 2, True), (648, 648, 65, 65, True)]
+
+
+@pytest.mark.parametrize("hq,hkv,n,kv,causal", SHARED)
+def test_rows_of_many_blocks(gpu, hq, hkv, n, kv, causal):
+    """Rows past the end hold NaN groups; strided queries; every third head is checked, and a second call's equality."""
+    g = _gen(hq + n + kv)
+    k, v, q = _bf(g, kv, hkv, 128), _bf(g, kv, hkv, 128), _bf(g, n, hq, 128)
+    k[..., 5] *= 6
+    room = kv + 100
+    wide = torch.full((n, hq, 136), math.nan, dtype=torch.bfloat16, device="cuda")
+    wide[..., :128] = q.cuda()
+    ctx = C.make_attention_ctx(hq, hkv, 128, rope=False, q_stride_n=hq * 136, q_stride_h=136)
+    cache = _fill(ctx, k, v, room)
+    o = _rows(ctx, wide, cache, room, n, kv, causal)
+    kvh = torch.arange(0, hkv, 3)
+    qh = (kvh[:, None] * (hq // hkv) + torch.arange(hq // hkv)).flatten()
+    ref, tol = R.attention(q[:, qh].double(), R.rounded(k[:, kvh]), R.rounded(v[:, kvh]), causal)
+    _within(o[:, qh.cuda()], ref, tol)
+    assert not o.isnan().any() and torch.equal(o, _rows(ctx, wide, cache, room, n, kv, causal))
+
+
+@pytest.mark.parametrize("what", ["key", "value"])
+def test_nan_groups_of_many_blocks(gpu, what):
+    hq = hkv = 320
+    n, kv, at = 130, 300, 221
+    q, k, v = _qkv(n, n, kv, hq, hkv, 128)
+    (k if what == "key" else v)[at, 7, 40] = math.nan
+    ctx = C.make_attention_ctx(hq, hkv, 128, rope=False)
+    heads = torch.tensor([0, 6, 7, 8, 319])
+    o = _rows(ctx, q.cuda(), _fill(ctx, k, v, kv), kv, n, kv)
+    ref, tol = R.attention(q[:, heads].double(), R.rounded(k[:, heads]).nan_to_num(0), R.rounded(v[:, heads]).nan_to_num(0), True)
+    sees = torch.arange(n) + kv - n >= at
+    if what == "key":
+        ref[sees, 2] = math.nan
+    else:
+        ref[sees, 2, 32:64] = math.nan
+    _within(o[:, heads.cuda()], ref, tol, what)
+    others = torch.arange(hq) != 7
+    assert not o[:, others.cuda()].isnan().any()
+
+
+def test_a_workspace_serves_fewer_rows_and_keys(gpu):
+    """One workspace of the largest call's bytes is enough for every smaller call."""
+    lib, ctx = C.load(), C.make_attention_ctx(28, 4, 128, rope=False)
+    kv = 8300
+    q, k, v = _qkv(3, 40, kv, 28, 4, 128)
+    cache, q = _fill(ctx, k, v, kv), q.cuda()
+    ws = _buf(lib.efm_attention_prefill_kv_fp4_workspace_bytes(ctx, 40, kv))
+    wd = _buf(lib.efm_attention_decode_kv_fp4_workspace_bytes(ctx, kv))
+    for n in (40, 17, 5, 1):
+        for L in (8300, 8192, 4096, 1000, 600, 300, 40):
+            o = torch.empty(n, 28, 128, dtype=torch.bfloat16, device="cuda")
+            C.call("efm_attention_prefill_kv_fp4", ctx, ptr(q), ptr(cache), kv, ptr(o), n, L, 1, ptr(ws), ws.numel(), stream())
+            assert torch.equal(o, _rows(ctx, q, cache, kv, n, L))
+            if n == 1:
+                C.call("efm_attention_decode_kv_fp4", ctx, ptr(q), ptr(cache), kv, ptr(o), L, None, 0, ptr(wd), wd.numel(), stream())
+                assert torch.equal(o, _decode(ctx, q, cache, kv, L))
 
 
 @pytest.mark.parametrize("n", [1, 21, 600])
