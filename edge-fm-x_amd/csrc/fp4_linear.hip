@@ -467,6 +467,14 @@ __global__ __launch_bounds__(64 * WM * WN * KG, w4_tile_waves(TM, TN, D, WM, WN,
         part(sl + 2, c0, c1);
         part(sl + 3, c1, c1);
     }
+    const int ct0 = (nb * WN + wn) * NO;   // first column tile of y
+    float bias[NO][4] = {};                // all requested at once
+    if (EPI != W4_SWIGLU && a.bias != nullptr) {
+#pragma unroll
+        for (int j = 0; j < NO; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) bias[j][e] = bf16_to_f32(a.bias[min((int64_t)(ct0 + j) * 16 + 4 * g + e, a.N - 1)]);
+    }
     landed();
     tie_x(0);
     attn_pipe::vm_wait<0>();
@@ -490,7 +498,6 @@ __global__ __launch_bounds__(64 * WM * WN * KG, w4_tile_waves(TM, TN, D, WM, WN,
 #pragma unroll
                 for (int j = 0; j < TN; ++j) acc[i][j] += sums[at(gr, i, j)];
     }
-    const int ct0 = (nb * WN + wn) * NO;   // first column tile of y
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
         const int64_t row = m0 + (wm * TM + i) * 16 + l;
@@ -502,7 +509,7 @@ __global__ __launch_bounds__(64 * WM * WN * KG, w4_tile_waves(TM, TN, D, WM, WN,
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 if constexpr (EPI == W4_SWIGLU) v[e] = silu_f32(round_bf16(acc[i][j + NO][e])) * round_bf16(acc[i][j][e]);
-                else v[e] = acc[i][j][e] + (a.bias != nullptr && col + e < a.N ? bf16_to_f32(a.bias[col + e]) : 0.f);
+                else v[e] = acc[i][j][e] + bias[j][e];
             }
             w4_store4<EPI == W4_F32>(a.y, row * a.N + col, v, a.N - col);
         }
@@ -565,19 +572,21 @@ struct W4Form {
 };
 constexpr W4Form kW4Forms[] = {
     // few rows: each wave a part of K and rings of its own
-    {1, 1, 1, 1, 8, 2, 0.246f, 0.241f, 2.40f, 0.68f, 0.42f},
-    {1, 2, 1, 1, 4, 3, 0.241f, 0.156f, 2.82f, 0.37f, 0.19f},
-    {1, 2, 1, 1, 8, 1, 0.251f, 0.337f, 2.38f, 1.59f, 0.25f},
-    {2, 2, 1, 1, 2, 4, 0.273f, 0.128f, 3.26f, 0.23f, 0.68f},
-    {2, 2, 1, 1, 4, 2, 0.285f, 0.252f, 3.47f, 0.65f, 0.61f},
-    {2, 2, 1, 1, 8, 1, 0.100f, 0.488f, 3.40f, 1.71f, 0.35f},
-    {2, 4, 1, 1, 2, 3, 0.345f, 0.203f, 4.93f, 0.17f, 0.92f},
+    {1, 1, 1, 1, 8, 2, 0.197f, 0.247f, 2.71f, 0.37f, 0.38f},
+    {1, 2, 1, 1, 4, 3, 0.237f, 0.154f, 2.29f, 0.53f, 0.26f},
+    {1, 2, 1, 1, 8, 1, 0.253f, 0.319f, 1.80f, 1.76f, 0.21f},
+    {2, 2, 1, 1, 2, 4, 0.290f, 0.120f, 1.87f, 0.64f, 0.51f},
+    {2, 2, 1, 1, 4, 2, 0.304f, 0.234f, 2.13f, 1.07f, 0.45f},
+    {2, 2, 1, 1, 8, 1, 0.333f, 0.453f, 2.13f, 2.07f, 0.26f},
+    {2, 4, 1, 1, 2, 3, 0.379f, 0.157f, 1.62f, 1.47f, 0.19f},
     // four waves beside each other share x; two such groups, or one
-    {2, 2, 1, 4, 2, 2, 0.319f, 0.313f, 3.99f, 0.93f, 0.44f},
-    {2, 2, 1, 4, 1, 4, 0.250f, 0.147f, 3.48f, 0.42f, 0.05f},
-    {4, 2, 1, 4, 1, 3, 0.286f, 0.266f, 5.13f, 0.36f, 0.66f},
-    {4, 4, 1, 4, 1, 2, 0.436f, 0.387f, 6.00f, 2.28f, 0.36f},
-    {6, 4, 1, 4, 1, 2, 0.593f, 0.438f, 6.00f, 5.06f, 0.00f},
+    {2, 2, 1, 4, 2, 2, 0.320f, 0.290f, 2.62f, 1.04f, 0.25f},
+    {2, 2, 1, 4, 1, 4, 0.284f, 0.125f, 1.50f, 0.95f, 0.00f},
+    {4, 2, 1, 4, 1, 3, 0.290f, 0.252f, 3.21f, 0.62f, 0.51f},
+    {6, 2, 1, 4, 1, 2, 0.332f, 0.350f, 3.84f, 0.93f, 0.63f},
+    {8, 2, 1, 4, 1, 2, 0.382f, 0.447f, 4.53f, 1.23f, 0.64f},
+    {4, 4, 1, 4, 1, 2, 0.420f, 0.393f, 4.26f, 2.01f, 0.45f},
+    {6, 4, 1, 4, 1, 2, 0.519f, 0.518f, 4.77f, 2.72f, 0.37f},
 };
 constexpr int kW4FormCount = sizeof(kW4Forms) / sizeof(kW4Forms[0]);
 
