@@ -701,3 +701,140 @@ def test_same_stream_order_on_a_side_stream(gpu):
     s.synchronize()
     ref, tol = R.attention(q.double(), R.rounded(k), R.rounded(v), False)
     _within(o, ref, tol)
+
+
+def test_layer_step_in_a_graph(gpu):
+    """A decode step of a layer captured once and replayed for several rows, the workspaces shared by its operators: bit
+    for bit the eager step, cache included."""
+    g = _gen(21)
+    lib = C.load()
+    hidden, hq, hkv, hd, inter, room = 512, 8, 2, 128, 768, 1300
+    width = (hq + 2 * hkv) * hd
+    packed = {n: _pack(*_weights_on_device(i, o, k)) for i, (n, o, k) in
+              enumerate((("qkv", width, hidden), ("o", hidden, hq * hd), ("gu", 2 * inter, hidden), ("down", hidden, inter)))}
+    qw, kw, bias = ((1 + _bf(g, n, std=0.2)).cuda() for n in (hd, hd, width))
+    rope, ctx = C.make_attention_ctx(hq, hkv, hd), C.make_attention_ctx(hq, hkv, hd, rope=False)
+    start = 1200
+    prompt = _bf(g, start, width).cuda()
+    ws = _buf(lib.efm_attention_decode_kv_fp4_workspace_bytes(ctx, room))
+
+    def state():
+        cache = _buf(lib.efm_kv_fp4_bytes(ctx, room), 0xff)
+        _write(rope, True, prompt, qw, kw, None, [cache], room, start, 0)
+        return dict(cache=cache, x=torch.empty(1, hidden, dtype=torch.bfloat16, device="cuda"), n=torch.tensor([start], dtype=torch.int32, device="cuda"),
+                    qkv=torch.empty(1, width, dtype=torch.bfloat16, device="cuda"), q=torch.empty(1, hq, hd, dtype=torch.bfloat16, device="cuda"),
+                    att=torch.empty(1, hq * hd, dtype=torch.bfloat16, device="cuda"), out=torch.empty(1, hidden, dtype=torch.bfloat16, device="cuda"),
+                    mid=torch.empty(1, inter, dtype=torch.bfloat16, device="cuda"), y=torch.empty(1, hidden, dtype=torch.float32, device="cuda"))
+
+    def step(t, on):
+        lin = lambda k, n, x, w, b, y, dt: C.call("efm_linear_fp4", 1, k, n, ptr(x), ptr(w), ptr(b), ptr(y), dt, None, 0, on)
+        lin(hidden, width, t["x"], packed["qkv"], bias, t["qkv"], C.EFM_DTYPE_BF16)
+        _write(rope, True, t["qkv"], qw, kw, t["q"], [t["cache"]], room, 1, 0, d_len=t["n"], on=on)
+        C.call("efm_attention_decode_kv_fp4", ctx, ptr(t["q"]), ptr(t["cache"]), room, ptr(t["att"]), 0, ptr(t["n"]), room, ptr(ws), ws.numel(), on)
+        lin(hq * hd, hidden, t["att"], packed["o"], None, t["out"], C.EFM_DTYPE_BF16)
+        C.call("efm_fused_gate_up_swiglu_fp4", 1, hidden, inter, ptr(t["out"]), ptr(packed["gu"]), ptr(t["mid"]), None, 0, on)
+        lin(inter, hidden, t["mid"], packed["down"], None, t["y"], C.EFM_DTYPE_F32)
+
+    eager, captured = state(), state()
+    s, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=s, capture_error_mode="thread_local"):
+        step(captured, s.cuda_stream)
+    for rep in range(4):
+        x = _bf(g, 1, hidden)
+        for t in (eager, captured):
+            t["x"].copy_(x)
+            t["n"] += 1
+        ws.fill_(0xff)
+        step(eager, stream())
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.isfinite(eager["y"]).all()
+        for name in eager:
+            assert torch.equal(eager[name], captured[name]), (rep, name)
+
+
+def test_prompt_in_a_graph(gpu):
+    """Write and attention of a prompt's rows behind others, captured and replayed with other rows."""
+    g = _gen(22)
+    hq, hkv, hd, base, n = 12, 2, 128, 500, 70
+    room = base + n
+    rope, ctx = C.make_attention_ctx(hq, hkv, hd), C.make_attention_ctx(hq, hkv, hd, rope=False)
+    cache = _buf(C.load().efm_kv_fp4_bytes(ctx, room), 0xff)
+    w = (1 + _bf(g, hd, std=0.2)).cuda()
+    _write(rope, True, _bf(g, base, (hq + 2 * hkv) * hd).cuda(), w, w, None, [cache], room, base, 0)
+    qkv = torch.empty(n, (hq + 2 * hkv) * hd, dtype=torch.bfloat16, device="cuda")
+    q, o = (torch.empty(n, hq, hd, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    ws = _buf(C.load().efm_attention_prefill_kv_fp4_workspace_bytes(ctx, n, room))
+
+    def both(on):
+        _write(rope, True, qkv, w, w, q, [cache], room, n, base, on=on)
+        C.call("efm_attention_prefill_kv_fp4", ctx, ptr(q), ptr(cache), room, ptr(o), n, room, 1, ptr(ws), ws.numel(), on)
+
+    s, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=s, capture_error_mode="thread_local"):
+        both(s.cuda_stream)
+    for rep in range(3):
+        qkv.copy_(_bf(g, *qkv.shape))
+        ws.fill_(0xff)
+        graph.replay()
+        torch.randn(1 << 18, device="cuda").sum()
+        torch.cuda.synchronize()
+        got = o.clone()
+        o.fill_(math.nan)
+        both(stream())
+        torch.cuda.synchronize()
+        assert torch.isfinite(o).all() and torch.equal(got, o), f"replay {rep}"
+
+
+def test_two_streams_at_once(gpu):
+    """Calls on two streams, each with a workspace of its own, do not disturb each other."""
+    hq, hkv, hd, kv = 28, 4, 128, 6000
+    ctx = C.make_attention_ctx(hq, hkv, hd, rope=False)
+    sets = []
+    for seed in (1, 2):
+        q, k, v = _qkv(seed, 1, kv, hq, hkv, hd)
+        sets.append([q.cuda(), _fill(ctx, k, v, kv), _buf(C.load().efm_attention_decode_kv_fp4_workspace_bytes(ctx, kv)),
+                     torch.empty(20, 1, hq, hd, dtype=torch.bfloat16, device="cuda"), torch.cuda.Stream()])
+    torch.cuda.synchronize()
+    for i in range(20):
+        for q, cache, ws, o, s in sets:
+            C.call("efm_attention_decode_kv_fp4", ctx, ptr(q), ptr(cache), kv, ptr(o[i]), kv, None, 0, ptr(ws), ws.numel(), s.cuda_stream)
+    torch.cuda.synchronize()
+    for q, cache, ws, o, s in sets:
+        alone = _decode(ctx, q, cache, kv, kv)
+        assert all(torch.equal(x, alone) for x in o)
+
+
+def test_cache_past_32_bits(gpu):
+    """The largest cache, 9 GB of 2^24 rows: zeros but for rows at both ends whose scores outweigh the rest."""
+    hq, hkv, hd, room, n = 28, 4, 128, 1 << 24, 24
+    g = _gen(31)
+    ctx = C.make_attention_ctx(hq, hkv, hd, rope=False)
+    cache = torch.zeros(C.load().efm_kv_fp4_bytes(ctx, room), dtype=torch.uint8, device="cuda")
+    q, k, v = _bf(g, 1, hq, hd), _bf(g, 2 * n, hkv, hd), _bf(g, 2 * n, hkv, hd)
+    k[::5] = q.view(hkv, hq // hkv, hd)[:, 0] * 2.5   # scores of 28 for a head of each group
+    rows = torch.cat([torch.zeros(2 * n, hq * hd, dtype=torch.bfloat16), k.flatten(1), v.flatten(1)], 1).cuda()
+    _write(ctx, True, rows[:n].contiguous(), None, None, None, [cache], room, n, 0)
+    _write(ctx, True, rows[n:].contiguous(), None, None, None, [cache], room, n, room - n)
+    kk, vv = R.rounded(k), R.rounded(v)
+    for at, part in ((0, slice(0, n)), (room - n, slice(n, 2 * n))):
+        a, b = _read(ctx, cache, room, at, n, hkv, hd)
+        assert torch.equal(a, kk[part]) and torch.equal(b, vv[part])
+    o = _decode(ctx, q.cuda(), cache, room, room)
+    rep = lambda t: t.repeat_interleave(hq // hkv, 1)
+    s = (q.double() * rep(kk)).sum(-1) / math.sqrt(hd)                       # [rows, heads]
+    mag = (q.double() * rep(kk)).abs().sum(-1).amax(0) / math.sqrt(hd)
+    top = s.amax(0).clamp(min=0)
+    w = (s - top).exp()
+    den = w.sum(0) + (room - 2 * n) * (-top).exp()
+    ref = (w[..., None] * rep(vv)).sum(0) / den[:, None]
+    # as for shorter lengths: output and weights to bf16, scores in fp32; and a sum's chain, 2^19 tiles over 2^8 workgroups at
+    # least and their partial sums: under 2^13 additions of 2^-23
+    d = (hd / 32 + 40) * 2.0 ** -23 * mag[:, None]
+    share = (w[..., None] * rep(vv).abs()).sum(0) / den[:, None]
+    tol = HALF * ref.abs() + share * (HALF + 2 * d + 2.0 ** -18 + 2.0 ** -10)
+    _within(o[0], ref, tol)
+    assert (ref[:: hq // hkv].abs().amax(-1) > 0.1).all()
