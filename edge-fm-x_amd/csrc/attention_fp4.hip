@@ -60,25 +60,24 @@ struct KvFp4Tile {
     uint32_t k[2][W], ks[2], v[8], vs[2];
 };
 
-// The softmax step of NT tiles of 32 keys for the lane's row: s, its products with keys key0 .. key0 + 7
-// of each tile, to weights; m, sum and the outputs so far follow a maximum larger by 2^kKvFp4Lazy in
-// weights, which is rare past a row's first keys: weights of up to that and their sums are as exact in
-// bf16 and fp32 as those of up to 1. pf: the weights as second operands of the second product.
+// The first half of the softmax step of NT tiles of 32 keys for the lane's row: masks s, its products with
+// keys key0 .. key0 + 7 of each tile, and returns what their exponents are relative to. m, sum and the
+// outputs so far follow a maximum larger by 2^kKvFp4Lazy in weights, which is rare past a row's first
+// keys: weights of up to that and their sums are as exact in bf16 and fp32 as those of up to 1.
 template <int MT, int NT>
-__device__ __forceinline__ void kv_fp4_softmax(const f32x4_t (*s)[2], int key0, bool masked, int sees, float scale, float& m,
-                                               float& sum, f32x4_t* o, bf16x8_t* pf) {
+__device__ __forceinline__ float kv_fp4_maximum(f32x4_t (*s)[2], int key0, bool masked, int sees, float scale, float& m, float& sum,
+                                                f32x4_t* o) {
     // v_maximum3_f32 takes three operands as they are; a NaN among them leaves m, and makes the row's sum NaN
     auto larger = [](float x, float y) { return __builtin_elementwise_maximum(x, y); };
-    float p[NT][8], tops[NT];
+    float tops[NT];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) p[t][i] = s[t][i / 4][i % 4];
         if (masked) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) p[t][i] = key0 + 32 * t + i < sees ? p[t][i] : -INFINITY;
+            for (int i = 0; i < 8; ++i) s[t][i / 4][i % 4] = key0 + 32 * t + i < sees ? s[t][i / 4][i % 4] : -INFINITY;
         }
-        tops[t] = larger(larger(larger(larger(p[t][0], p[t][1]), p[t][2]), larger(larger(p[t][3], p[t][4]), p[t][5])), larger(p[t][6], p[t][7]));
+        const f32x4_t x = s[t][0], y = s[t][1];
+        tops[t] = larger(larger(larger(larger(x[0], x[1]), x[2]), larger(larger(x[3], y[0]), y[1])), larger(y[2], y[3]));
     }
     float top = NT == 1 ? tops[0] : larger(tops[0], tops[NT - 1]);
     top = larger(m, over_groups(top, larger));
@@ -89,13 +88,21 @@ __device__ __forceinline__ void kv_fp4_softmax(const f32x4_t (*s)[2], int key0, 
         for (int i = 0; i < MT; ++i) o[i] *= alpha;
         m = top;
     }
-    const float ref = m == -INFINITY ? 0.f : m * scale;
+    return m == -INFINITY ? 0.f : m * scale;
+}
+
+// The whole step; pf: the weights as second operands of the second product.
+template <int MT, int NT>
+__device__ __forceinline__ void kv_fp4_softmax(f32x4_t (*s)[2], int key0, bool masked, int sees, float scale, float& m, float& sum,
+                                               f32x4_t* o, bf16x8_t* pf) {
+    const float ref = kv_fp4_maximum<MT, NT>(s, key0, masked, sees, scale, m, sum, o);
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
+        float p[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) p[t][i] = __builtin_amdgcn_exp2f(fmaf(p[t][i], scale, -ref));
-        sum += ((p[t][0] + p[t][1]) + (p[t][2] + p[t][3])) + ((p[t][4] + p[t][5]) + (p[t][6] + p[t][7]));
-        pf[t] = __builtin_bit_cast(bf16x8_t, pack8(p[t]));
+        for (int i = 0; i < 8; ++i) p[i] = __builtin_amdgcn_exp2f(fmaf(s[t][i / 4][i % 4], scale, -ref));
+        sum += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+        pf[t] = __builtin_bit_cast(bf16x8_t, pack8(p));
     }
 }
 
@@ -384,18 +391,24 @@ __global__ __launch_bounds__(256) void kv_fp4_merge_kernel(KvFp4Args a) {
 
 // Many rows: four waves with 32 rows each share the keys. 64 keys (a stage) at a time the waves make
 // a quarter of the stage's operands each, the codes of the next stage unpacked into LDS in the order
-// in which the lanes take them, while the present stage is multiplied: unpacking costs a row an eighth
-// of what it does above, and is hidden behind the matrix cores' other work.
+// in which the lanes take them: unpacking costs a row an eighth of what it does above. A wave's own
+// instructions alternate: unpacking goes out between the first products, the second tile's exponentials
+// between the first tile's second products, and a wave at its products goes before the other on its SIMD,
+// which so falls to its softmax (4096 rows of 28/4 heads: 150 us one after the other, 143 alternating, 122 with
+// the priority). 4096 rows 990 TFLOP/s, 8192 rows 1110; fewer rows are bound by workgroups that see more
+// keys than others.
 // Heads of 128; the keys are not split, since there are rows enough.
 __global__ __launch_bounds__(256, 2) void kv_fp4_rows_kernel(KvFp4Args a) {
     constexpr int HD = 128, W = HD / 32, MT = HD / 16, NQ = 2;
     constexpr int FRAGS = 2 * W + MT;                // 1 KB operands of a 32-key tile: keys [2][W], values [MT]
+    constexpr int AHEAD = 4;
     __shared__ uint4 frag[2][2][FRAGS][kWave];       // [buffer][tile of the stage]
     const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), l = lane % 16, g = lane / 16;
-    // Row blocks from the last, which see the most keys, the KV heads side by side. Where all workgroups
-    // are resident at once, two to a CU, the second to arrive at a CU is the lighter the heavier its first.
+    // Row blocks from the last, which see the most keys, the KV heads side by side. The second workgroup to
+    // arrive at a CU is the lighter the heavier its first (2500 rows of 28/4 heads 70 us, 75 in plain order).
     int rank = blockIdx.x;
-    if ((int)gridDim.x > a.cus && (int)gridDim.x <= 2 * a.cus && rank >= a.cus) rank = (int)gridDim.x - 1 - (rank - a.cus);
+    const int resident = min((int)gridDim.x, 2 * a.cus);
+    if (rank >= a.cus && rank < resident) rank = a.cus + resident - 1 - rank;
     const int r0 = ((int)(gridDim.x / a.Hkv) - 1 - rank / a.Hkv) * (64 * NQ), kvh = rank % a.Hkv;
     const KvFp4Layout lay(a.T, a.Hkv, HD);
     const int L = (int)a.kv_len;
@@ -447,11 +460,9 @@ __global__ __launch_bounds__(256, 2) void kv_fp4_rows_kernel(KvFp4Args a) {
         const uint2 u = *reinterpret_cast<const uint2*>(vsc + sof);
         cvs[0] = u.x, cvs[1] = u.y;
     };
-    // unpack the codes at hand, of stage st, into a buffer; values past the end and NaN groups as zeros
-    auto unpack = [&](int st, int b) {
-        uint4 (*const f)[kWave] = frag[b][wave / 2];
-#pragma unroll
-        for (int w = 0; w < W; ++w) f[part * W + w][lane] = __builtin_bit_cast(uint4, fp4_unpack8(ck[w], fp4_scale_at(cks, w)));
+    // The codes at hand, of stage st, are unpacked into a buffer in 24 pieces, which go out between the
+    // matrix instructions. Before that, values past the end and NaN groups are made zeros.
+    auto clean = [&](int st) {
         const int key0 = (2 * st + wave / 2) * 32 + 8 * g;
         const uint32_t ff = ((cvs[0] & 0x7f7f7f7fu) + 0x01010101u) & cvs[0], fg = ((cvs[1] & 0x7f7f7f7fu) + 0x01010101u) & cvs[1];
         if (st * 64 + 64 > L || __any(((ff | fg) & 0x80808080u) != 0)) {
@@ -466,20 +477,27 @@ __global__ __launch_bounds__(256, 2) void kv_fp4_rows_kernel(KvFp4Args a) {
                 }
             }
         }
-        [&]<int... B>(std::integer_sequence<int, B...>) {
-            ([&] {
-                uint32_t e[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) e[i] = fp4_pair<B>(cv[i] >> oshift, fp4_scale_at(cvs[i / 4], i % 4));
-                uint4 lo, hi;
-                lo.x = __builtin_amdgcn_perm(e[1], e[0], 0x05040100), hi.x = __builtin_amdgcn_perm(e[1], e[0], 0x07060302);
-                lo.y = __builtin_amdgcn_perm(e[3], e[2], 0x05040100), hi.y = __builtin_amdgcn_perm(e[3], e[2], 0x07060302);
-                lo.z = __builtin_amdgcn_perm(e[5], e[4], 0x05040100), hi.z = __builtin_amdgcn_perm(e[5], e[4], 0x07060302);
-                lo.w = __builtin_amdgcn_perm(e[7], e[6], 0x05040100), hi.w = __builtin_amdgcn_perm(e[7], e[6], 0x07060302);
-                f[2 * W + part * (MT / 2) + 2 * B][lane] = lo;
-                f[2 * W + part * (MT / 2) + 2 * B + 1][lane] = hi;
-            }(), ...);
-        }(std::make_integer_sequence<int, MT / 4>{});
+    };
+    constexpr int PIECES = W + 2 * 10;
+    uint32_t e[8];
+    auto unpack = [&](auto pc, int b) {
+        constexpr int P = decltype(pc)::value, V = P - W, B = V / 10, I = V % 10;
+        uint4 (*const f)[kWave] = frag[b][wave / 2];
+        if constexpr (P < W) {
+            f[part * W + P][lane] = __builtin_bit_cast(uint4, fp4_unpack8(ck[P], fp4_scale_at(cks, P)));
+        } else if constexpr (I < 8) {
+            e[I] = fp4_pair<B>(cv[I] >> oshift, fp4_scale_at(cvs[I / 4], I % 4));
+        } else {
+            constexpr uint32_t half = I == 8 ? 0x05040100 : 0x07060302;
+            f[2 * W + part * (MT / 2) + 2 * B + I - 8][lane] =
+                make_uint4(__builtin_amdgcn_perm(e[1], e[0], half), __builtin_amdgcn_perm(e[3], e[2], half),
+                           __builtin_amdgcn_perm(e[5], e[4], half), __builtin_amdgcn_perm(e[7], e[6], half));
+        }
+    };
+    // f(0) to f(n - 1)
+    auto each = [](auto nc, auto&& f) {
+        [&]<int... I>(std::integer_sequence<int, I...>) { (f(std::integral_constant<int, I>{}), ...); }
+        (std::make_integer_sequence<int, decltype(nc)::value>{});
     };
 
     f32x4_t o[NQ][MT];
@@ -495,43 +513,74 @@ __global__ __launch_bounds__(256, 2) void kv_fp4_rows_kernel(KvFp4Args a) {
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
     };
+    using std::integral_constant;
     load(0);   // every row sees a key
-    unpack(0, 0);
+    clean(0);
+    each(integral_constant<int, PIECES>{}, [&](auto pc) { unpack(pc, 0); });
     load(min(1, stages - 1));
     for (int st = 0; st < stages; ++st) {
         const int b = st & 1;
         meet();   // this stage is in LDS, and the other buffer is read out
-        if (st + 1 < stages) unpack(st + 1, 1 - b);
-        load(min(st + 2, stages - 1));
-        if (st * 64 >= wave_sees) continue;
+        // the stage's operands in the order of their use: keys of both tiles, values of both; AHEAD reads under way
+        bf16x8_t ring[AHEAD];
+        auto read = [&](auto fc) {
+            constexpr int F = decltype(fc)::value, T = F < 4 * W ? F / (2 * W) : (F - 4 * W) / MT, X = F < 4 * W ? F % (2 * W) : 2 * W + (F - 4 * W) % MT;
+            if constexpr (F < 2 * FRAGS) ring[F % AHEAD] = __builtin_bit_cast(bf16x8_t, frag[b][T][X][lane]);
+        };
+        each(integral_constant<int, AHEAD>{}, read);
+        clean(st + 1);   // past the last stage: the last one once more, into a buffer that nothing reads
         f32x4_t s[NQ][2][2];
+        __builtin_amdgcn_s_setprio(1);
+        each(integral_constant<int, 4 * W>{}, [&](auto fc) {
+            constexpr int F = decltype(fc)::value, T = F / (2 * W), I = F / W % 2;
 #pragma unroll
-        for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-#pragma unroll
-                for (int n = 0; n < NQ; ++n) s[n][tt][i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int w = 0; w < W; ++w) {
-                    const bf16x8_t kf = __builtin_bit_cast(bf16x8_t, frag[b][tt][i * W + w][lane]);
-#pragma unroll
-                    for (int n = 0; n < NQ; ++n)
-                        s[n][tt][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[n][w], s[n][tt][i], 0, 0, 0);
-                }
+            for (int n = 0; n < NQ; ++n) {
+                s[n][T][I] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ring[F % AHEAD], qf[n][F % W], F % W == 0 ? f32x4_t{0.f, 0.f, 0.f, 0.f} : s[n][T][I], 0, 0, 0);
+                if (n == 1) read(integral_constant<int, F + AHEAD>{});
+                constexpr int P0 = F * PIECES / (4 * W), P1 = (F + 1) * PIECES / (4 * W), PM = (P0 + P1) / 2;
+                if (n == 0) each(integral_constant<int, PM - P0>{}, [&](auto pc) { unpack(integral_constant<int, P0 + decltype(pc)::value>{}, 1 - b); });
+                else each(integral_constant<int, P1 - PM>{}, [&](auto pc) { unpack(integral_constant<int, PM + decltype(pc)::value>{}, 1 - b); });
+                __builtin_amdgcn_sched_barrier(0);
             }
+        });
+        __builtin_amdgcn_s_setprio(0);
+        load(min(st + 2, stages - 1));
         bf16x8_t pf[NQ][2];
+        float ref[NQ];
 #pragma unroll
         for (int n = 0; n < NQ; ++n)
-            kv_fp4_softmax<MT, 2>(s[n], st * 64 + 8 * g, st * 64 + 64 > all_see, sees[n], a.scale, m[n], sum[n], o[n], pf[n]);
+            ref[n] = kv_fp4_maximum<MT, 2>(s[n], st * 64 + 8 * g, st * 64 + 64 > all_see, sees[n], a.scale, m[n], sum[n], o[n]);
+        uint4 pw[NQ];
+        // weights E and E + 1 of a row's tile
+        auto weigh = [&](int n, int t, auto ec) {
+            constexpr int E = decltype(ec)::value;
+            const float x = __builtin_amdgcn_exp2f(fmaf(s[n][t][E / 4][E % 4], a.scale, -ref[n]));
+            const float y = __builtin_amdgcn_exp2f(fmaf(s[n][t][E / 4][E % 4 + 1], a.scale, -ref[n]));
+            sum[n] += x + y;
+            reinterpret_cast<uint32_t*>(&pw[n])[E / 2] = pack_bf16x2(x, y);
+        };
 #pragma unroll
-        for (int tt = 0; tt < 2; ++tt)
+        for (int n = 0; n < NQ; ++n) {
+            each(integral_constant<int, 4>{}, [&](auto ec) { weigh(n, 0, integral_constant<int, 2 * decltype(ec)::value>{}); });
+            pf[n][0] = __builtin_bit_cast(bf16x8_t, pw[n]);
+        }
+        __builtin_amdgcn_s_setprio(1);
+        each(integral_constant<int, 2 * MT>{}, [&](auto fc) {
+            constexpr int F = decltype(fc)::value, T = F / MT, I = F % MT;
 #pragma unroll
-            for (int i = 0; i < MT; ++i) {
-                const bf16x8_t vf = __builtin_bit_cast(bf16x8_t, frag[b][tt][2 * W + i][lane]);
-#pragma unroll
-                for (int n = 0; n < NQ; ++n)
-                    o[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[n][tt], o[n][i], 0, 0, 0);
+            for (int n = 0; n < NQ; ++n) {
+                o[n][I] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ring[(4 * W + F) % AHEAD], pf[n][T], o[n][I], 0, 0, 0);
+                if (n == 1) read(integral_constant<int, 4 * W + F + AHEAD>{});
+                // the second tile's weights, beside the first tile's products
+                if (T == 0 && n == 1) weigh(F / 4, 1, integral_constant<int, 2 * (F % 4)>{});
+                __builtin_amdgcn_sched_barrier(0);
             }
+            if constexpr (T == 0 && I == MT - 1) {
+#pragma unroll
+                for (int n = 0; n < NQ; ++n) pf[n][1] = __builtin_bit_cast(bf16x8_t, pw[n]);
+            }
+        });
+        __builtin_amdgcn_s_setprio(0);
     }
     // NaN groups of values reach the outputs of the rows that see them
     meet();
@@ -572,18 +621,19 @@ struct KvFp4Plan {
 // keys of 28/4 heads 7.2 in workgroups of four waves, 7.4 of eight; 32771 keys 11.9 with up to 512
 // workgroups, 10.9 with 256. Rows, kv_fp4_attn_kernel with 16 and with 32 rows a workgroup and
 // kv_fp4_rows_kernel: 37 rows behind 8000 of 12/2 heads 13 / 16 / 20, 512 behind 512 of 28/4 heads 22 / 17 /
-// 29, 4096 of 28/4 heads - / 163 / 144, 8192 - / 583 / 489, 2048 behind 2048 - / 121 / 113, 2048 alone - /
-// 58 / 62, 1500 behind 2000 - / 89 / 106, 6000 of 16/2 heads - / 190 / 165.
+// 29, 1500 behind 2000 - / 89 / 99, 2048 alone - / 55 / 54, 2048 behind 2048 - / 127 / 113, 2500 alone - / 73 /
+// 70, 2500 behind 2500 - / 174 / 162, 3000 - / 96 / 85, 4096 - / 161 / 120; of 12/2 heads 5000 - / 103 / 126, 6000
+// - / 142 / 153, 6000 behind 6000 - / 390 / 374, 7000 - / 188 / 188, 10000 - / 364 / 283.
 static KvFp4Plan kv_fp4_plan(const efm_attention_ctx* c, uint32_t S, uint32_t kv_len, bool causal) {
     const int64_t Hkv = c->num_kv_heads, rows = (int64_t)S * (c->num_qo_heads / Hkv), cus = prefill_cus();
     const int tiles = (int)(((int64_t)kv_len + 31) / 32);
     auto blocks_of = [&](int n) { return (rows + n - 1) / n * Hkv; };
     KvFp4Plan p = {};
-    // The shared kernel's 128-row workgroups pay where they fill the CUs several times, or just twice and
-    // differ little in their keys.
+    // The shared kernel's 128-row workgroups pay where they fill the CUs' places (two each) and more, or
+    // fill them and differ little in their keys.
     const int64_t shared = blocks_of(128);
     p.shared = c->head_dim == 128 && S > 1 &&
-               (2 * shared >= 5 * cus || (4 * shared >= 7 * cus && shared <= 2 * cus && (!causal || kv_len >= S + S / 2)));
+               (2 * shared >= 5 * cus || (4 * shared >= 7 * cus && (!causal || kv_len >= S + S / 2)));
     p.nq = blocks_of(16) >= 2 * cus ? 2 : 1;
     p.nw = p.nq == 2 ? 4 : 8;
     const int64_t blocks = p.shared ? shared : blocks_of(16 * p.nq);
