@@ -11,7 +11,7 @@
 //
 // Bound by memory once there are many tokens: 4096 tokens of 28/4 heads of 128 into a bf16 cache read
 // and write 76 MB in 14.4 us (5.2 TB/s, a copy's rate), into an FP4 cache 70 MB in 16 us. A token by itself
-// takes 3.1 us (bf16) and 4.3 us (FP4), of which an empty launch is 2: the rest is one chain of a load,
+// takes 3.1 us (bf16) and 3.9 us (FP4), of which an empty launch is 2: the rest is one chain of a load,
 // the angle's sine and cosine in 64 bits, the norm's sum, and the store. Reading 4096 such rows of an FP4
 // cache back (8.4 MB written) takes 5 us.
 #include "fp4.hpp"
@@ -44,30 +44,39 @@ struct QkWriteArgs {
     double turns[kMaxHalfDim];   // theta^(-2 d / hd) / rope_scale / (2 pi)
 };
 
-// Sum over the LANES lanes of a row, alike in all of them.
-template <int LANES>
-__device__ __forceinline__ float row_sum(float v) {
-    v += dpp_f32<0xB1>(v);
-    v += dpp_f32<0x4E>(v);
-    v += dpp_f32<0x141>(v);
-    return LANES == 16 ? v + dpp_f32<0x140>(v) : v;
+// A value of 4 or 8 bytes from another lane of the row.
+template <int CTRL, typename T>
+__device__ __forceinline__ T dpp(T v) {
+    auto move = [](uint32_t w) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)w, CTRL, 0xf, 0xf, false); };
+    if constexpr (sizeof(T) == 4) {
+        return __builtin_bit_cast(T, move(__builtin_bit_cast(uint32_t, v)));
+    } else {
+        const uint64_t u = __builtin_bit_cast(uint64_t, v);
+        return __builtin_bit_cast(T, (uint64_t)move((uint32_t)(u >> 32)) << 32 | move((uint32_t)u));
+    }
 }
 
-template <int LANES>
-__device__ __forceinline__ double row_sum(double v) {
-#pragma unroll
-    for (int m = 1; m < LANES; m *= 2) v += __shfl_xor(v, m, kWave);
-    return v;
+// Sum over the LANES lanes of a row, alike in all of them.
+template <int LANES, typename T>
+__device__ __forceinline__ T row_sum(T v) {
+    v += dpp<0xB1>(v);
+    v += dpp<0x4E>(v);
+    v += dpp<0x141>(v);
+    return LANES == 16 ? v + dpp<0x140>(v) : v;
+}
+
+// The largest of four lanes, which hold a group of 32 channels.
+template <typename T>
+__device__ __forceinline__ T group_max(T v) {
+    v = max(v, dpp<0xB1>(v));
+    return max(v, dpp<0x4E>(v));
 }
 
 // The value of the lane that holds the other half of this lane's pairs, LANES / 2 away.
-template <int LANES>
-__device__ __forceinline__ float row_other(float v) {
-    return LANES == 16 ? dpp_f32<0x128>(v) : dpp_f32<0x141>(dpp_f32<0x1B>(v));
+template <int LANES, typename T>
+__device__ __forceinline__ T row_other(T v) {
+    return LANES == 16 ? dpp<0x128>(v) : dpp<0x141>(dpp<0x1B>(v));
 }
-
-template <int LANES>
-__device__ __forceinline__ double row_other(double v) { return __shfl_xor(v, LANES / 2, kWave); }
 
 __device__ __forceinline__ float inv_sqrt(float v) { return rsqrtf(v); }
 __device__ __forceinline__ double inv_sqrt(double v) { return 1.0 / sqrt(v); }
@@ -184,9 +193,7 @@ __global__ __launch_bounds__(TOKENS ? 512 : 1024) void qk_norm_rope_write_kernel
                 uint64_t top = 0;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) top = max(top, (uint64_t)(__double_as_longlong(y[e]) & 0x7fffffffffffffffll));
-                top = max(top, (uint64_t)__shfl_xor((unsigned long long)top, 1, kWave));
-                top = max(top, (uint64_t)__shfl_xor((unsigned long long)top, 2, kWave));
-                const uint32_t byte = fp4_scale_byte(top), word = fp4_encode8(y, byte);
+                const uint32_t byte = fp4_scale_byte(group_max(top)), word = fp4_encode8(y, byte);
                 if (is_k && on) {
                     *reinterpret_cast<uint32_t*>(a.cache + lay.k(kh) + lay.k_word(row, j)) = word;
                     if (j % 4 == 0) a.cache[lay.ks(kh) + lay.k_scale(row, j)] = (uint8_t)byte;
@@ -203,9 +210,7 @@ __global__ __launch_bounds__(TOKENS ? 512 : 1024) void qk_norm_rope_write_kernel
                 uint32_t top = 0;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
-                top = max(top, (uint32_t)__shfl_xor((int)top, 1, kWave));
-                top = max(top, (uint32_t)__shfl_xor((int)top, 2, kWave));
-                const uint32_t byte = fp4_scale_byte(top), word = fp4_encode8(x, byte);
+                const uint32_t byte = fp4_scale_byte(group_max(top)), word = fp4_encode8(x, byte);
                 if (is_v && on) {
                     *reinterpret_cast<uint32_t*>(a.cache + lay.v(vh) + lay.v_word(row, j)) = word;
                     if (j % 4 == 0) a.cache[lay.vs(vh) + lay.v_scale(row, j)] = (uint8_t)byte;
