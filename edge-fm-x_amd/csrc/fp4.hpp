@@ -1,14 +1,15 @@
 // FP4 values with shared scales (the OCP microscaling format): groups of 32 values along a
 // row share a scale 2^(b - 127), b one byte (255: the group is NaN), and a value is one of
 // 0, 0.5, 1, 1.5, 2, 3, 4, 6 times the scale, with a sign in bit 3 of its 4-bit code. A value
-// has two significant bits, so value times scale is exact in bf16: every kernel here feeds
-// the bf16 matrix cores what is stored, no scale meets an accumulator, and kernels that read
+// has two significant bits, so value times scale is exact in bf16 (subnormals included; 2^128 and
+// more is infinite there): every kernel here feeds the bf16 matrix cores what is stored, no scale meets an accumulator, and kernels that read
 // the same codes see the same numbers. gfx950 turns two codes and a scale into two bf16 in one
 // instruction of the full VALU rate (v_cvt_scalef32_pk_bf16_fp4; a scale of exponent 255 gives
 // NaN for every code).
 //
 // Quantisation: the scale is the least power of two with max |x| <= 7 * scale, at least
-// 2^-125 (so that no value needs a bf16 subnormal), and a value is rounded to the nearest of
+// 2^-125 (so that no value needs a bf16 subnormal) and at most 2^125 (so that none is infinite;
+// larger groups are NaN), and a value is rounded to the nearest of
 // the grid, of two as near to the one with the even code. Up to 7 the nearest is at most half
 // a step of the grid away. Scaling by a power of two is exact, so for bf16 inputs the codes
 // are defined bit for bit.
@@ -22,7 +23,7 @@ typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
 constexpr int kFp4Group = 32;
 constexpr uint32_t kFp4ScaleNan = 255;
-constexpr int kFp4MinExp = -125;
+constexpr int kFp4MinExp = -125, kFp4MaxExp = 125;
 
 // The scale as fp32 (byte 0 comes out as 0, which the conversion reads as 2^-127).
 __device__ __forceinline__ float fp4_scale(uint32_t byte) { return __uint_as_float(byte << 23); }
@@ -51,9 +52,8 @@ __device__ __forceinline__ int fp4_exp(int E, bool over_1_75) { return max(E - 2
 
 // Scale byte for the largest magnitude of a group, given as its fp32 bits (sign cleared).
 __device__ __forceinline__ uint32_t fp4_scale_byte(uint32_t abs_bits) {
-    const int E = (int)(abs_bits >> 23) - 127;
-    if (E == 128) return kFp4ScaleNan;
-    return (uint32_t)(fp4_exp(E, (abs_bits & 0x7fffffu) > 0x600000u) + 127);
+    const int e = fp4_exp((int)(abs_bits >> 23) - 127, (abs_bits & 0x7fffffu) > 0x600000u);
+    return e > kFp4MaxExp ? kFp4ScaleNan : (uint32_t)(e + 127);
 }
 
 // Two codes of values already divided by the scale, in the low byte: v_cvt_scalef32_pk_fp4_f32
@@ -93,12 +93,11 @@ __device__ __forceinline__ uint32_t fp4_encode8(const double* x, uint32_t byte) 
     return w;
 }
 
-// Scale byte for the largest magnitude of a group in 64 bits; beyond the format's largest
-// scale the group is NaN.
+// The same for a magnitude in 64 bits.
 __device__ __forceinline__ uint32_t fp4_scale_byte(uint64_t abs_bits) {
     const int E = (int)(abs_bits >> 52) - 1023;
     const int e = fp4_exp(E, (abs_bits & 0xfffffffffffffull) > 0xc000000000000ull);
-    return e > 127 ? kFp4ScaleNan : (uint32_t)(e + 127);
+    return e > kFp4MaxExp ? kFp4ScaleNan : (uint32_t)(e + 127);
 }
 
 // Geometry of an FP4 cache of one layer for Hkv heads of HD channels and T rows (a multiple of

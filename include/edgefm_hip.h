@@ -483,10 +483,11 @@ int efm_decode_norm_lm_head_top1(int32_t hidden, int64_t vocab, float eps, const
  * The format is the OCP microscaling FP4 (E2M1 elements, E8M0 scales): groups of 32
  * consecutive values share a scale 2^(b - 127) held in a byte b (255: the group is NaN); an
  * element is a 4-bit code, sign in bit 3, magnitude 0, 0.5, 1, 1.5, 2, 3, 4, 6 for codes 0 to
- * 7. An element's value (magnitude times scale) is exact in bf16. Quantisation takes the
- * least scale with max |x| <= 7 * scale (at least 2^-125) and rounds x / scale to the nearest
- * magnitude, of two as near to the one with the even code, so that the error is at most half
- * a step of the grid; a group that holds a NaN or an infinity is stored as NaN.
+ * 7. An element's value (magnitude times scale) is exact in bf16; one of 2^128 and more
+ * (bytes 253 and 254) is infinite there. Quantisation takes the least scale with
+ * max |x| <= 7 * scale, from 2^-125 to 2^125, and rounds x / scale to the nearest magnitude, of
+ * two as near to the one with the even code, so that the error is at most half a step of the
+ * grid; a group that holds a NaN, an infinity or a magnitude past 7 * 2^125 is stored as NaN.
  * ---------------------------------------------------------------------------------- */
 
 /* Weights in the interchange form: codes [out, in / 2], element 2 i of a row in the low half

@@ -10,7 +10,7 @@ def quantize(x):
     """(codes uint8, scale bytes uint8) of x [..., 32 g], by search over the format's scales and magnitudes."""
     x = x.double().cpu().unflatten(-1, (-1, 32))
     top = x.abs().amax(-1)
-    exps = torch.arange(-125, 128)
+    exps = torch.arange(-125, 126)
     fits = top.unsqueeze(-1) <= 7 * torch.exp2(exps.double())
     at = fits.to(torch.int8).argmax(-1)   # the least scale that fits
     bad = ~torch.isfinite(top) | ~fits.any(-1)

@@ -197,6 +197,26 @@ def test_swiglu_every_shape(gpu, m, hidden, inter):
 
 
 @pytest.mark.parametrize("m", [1, 20, 200])
+@pytest.mark.parametrize("low,high,power", [(0, 4, 120), (250, 255, -120)])
+def test_linear_smallest_and_largest_scales(gpu, m, low, high, power):
+    """Scales at both ends of the format, where values are subnormal in bf16, or close to its largest and, from 2^128 on,
+    infinite, with rows of x that bring the products back."""
+    g = _gen(m)
+    k, out = 256, 40
+    code = torch.randint(0, 16, (out, k), generator=g).to(torch.uint8)
+    code = torch.where((code & 7) > 5, code & 13, code) if low else code
+    byte = torch.randint(low, high, (out, k // 32), generator=g).to(torch.uint8)
+    x = _bf(g, m, k) * 2.0 ** power
+    y = _linear(x.cuda(), _pack(R.halves(code), byte), k, out, None, True).cpu()
+    w = R.values(code, byte)
+    w[w.abs() >= 2.0 ** 128] *= math.inf
+    ref, tol = _product(x.double(), w)
+    assert torch.equal(y.isnan(), ref.isnan()) and torch.equal(y[ref.isinf()].double(), ref[ref.isinf()])
+    assert (ref[ref.isfinite()].abs() > 2.0 ** -30).any()
+    _within(y[ref.isfinite()], ref[ref.isfinite()], tol[ref.isfinite()])
+
+
+@pytest.mark.parametrize("m", [1, 20, 200])
 def test_linear_nan_stays_in_its_place(gpu, m):
     """A NaN group reaches its own output column alone, a NaN row of x its own row; rows and columns that pad the tiles
     reach nothing."""
@@ -379,6 +399,25 @@ def test_write_without_queries_and_read_of_one_side(gpu):
     C.call("efm_kv_fp4_read", ctx, ptr(cache), 9, 5, 4, None, ptr(v), stream())
     torch.cuda.synchronize()
     assert torch.equal(k.cpu().double(), R.rounded(x[5:, 14:16])) and torch.equal(v.cpu().double(), R.rounded(x[5:, 16:]))
+
+
+@pytest.mark.parametrize("n,kv", [(1, 70), (40, 100), (600, 900)])
+def test_the_largest_values_reach_the_rows_that_see_them(gpu, n, kv):
+    """Values up to 7 * 2^125 are stored as finite ones, larger as NaN: neither reaches a row before their key."""
+    hq, hkv, hd = 12, 2, 128
+    q, k, v = _qkv(n, n, kv, hq, hkv, hd)
+    at = kv - max(1, n // 2)
+    v[at, 0, 3], v[at, 1, 70] = 7 * 2.0 ** 125, torch.finfo(torch.bfloat16).max
+    ctx = C.make_attention_ctx(hq, hkv, hd, rope=False)
+    cache = _fill(ctx, k, v, kv)
+    got = _read(ctx, cache, kv, at, 1, hkv, hd)[1]
+    assert got[0, 0, 3] == 6 * 2.0 ** 125 and got[0, 1].isnan().sum() == 32
+    o = _rows(ctx, q.cuda(), cache, kv, n, kv).cpu()
+    before = torch.arange(n) + kv - n < at
+    assert torch.isfinite(o[before]).all() and o[~before, hq // 2:, 64:96].isnan().all()
+    rv = R.rounded(v)
+    ref, tol = R.attention(q.double(), R.rounded(k), rv.nan_to_num(0), True)
+    _within(o[before], ref[before], tol[before])
 
 
 def test_write_fp4_groups_that_are_not_finite(gpu):
