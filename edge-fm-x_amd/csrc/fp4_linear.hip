@@ -231,9 +231,10 @@ __global__ __launch_bounds__(1024) void fp4_linear_kernel(W4Args a) {
     }
 }
 
-// Many rows of x: WM x (4 / WM) waves, each 16 TM rows of x by 16 TN weight rows. x, 64 columns (a
-// slab) at a time, and the codes and scales, 128 columns (a block) at a time, go straight into
-// rings of D and R places in LDS, D - 1 slabs ahead. In LDS the 16-byte chunk c of a row r of x
+// Five rows of x and more: KG groups, each with a part of K, of WN waves that share 16 TM rows of x and take
+// 16 TN weight rows each; a group of one wave meets no barrier. x, 64 columns (a slab) at a time, and the
+// codes and scales, 128 columns (a block) at a time, go straight into rings of D and R places in LDS,
+// D - 1 slabs ahead. In LDS the 16-byte chunk c of a row r of x
 // sits at c ^ (r / 2 % 8), so that sixteen rows' reads meet all banks. The weights are the first
 // operand: a lane ends with four consecutive columns of a row of y.
 constexpr int w4_swz(int r) { return (r >> 1) & 7; }
@@ -253,25 +254,26 @@ __device__ __forceinline__ void w4_read32(uint32_t& dst, uint32_t addr) {
 }
 
 // LDS of a group: D slabs of x, (D + 1) / 2 blocks of codes and scales.
-constexpr int w4_tile_lds(int tm, int tn, int d, int wm, int wn) {
-    return d * 2048 * tm * wm + (d + 1) / 2 * (1024 * wn * tn + 256 * wm * wn);
+constexpr int kW4Ring = 3;
+constexpr int w4_tile_lds(int tm, int tn, int wn) {
+    return kW4Ring * 2048 * tm + (kW4Ring + 1) / 2 * (1024 * wn * tn + 256 * wn);
 }
 // Waves a SIMD to compile for: two while two workgroups of four waves fit LDS.
-constexpr int w4_tile_waves(int tm, int tn, int d, int wm, int wn, int kg) {
-    return wm * wn * kg > 4 ? wm * wn * kg / 4 : w4_tile_lds(tm, tn, d, wm, wn) * kg <= 80 * 1024 && tm * tn <= 16 ? 2 : 1;
+constexpr int w4_tile_waves(int tm, int tn, int wn, int kg) {
+    return wn * kg > 4 ? wn * kg / 4 : w4_tile_lds(tm, tn, wn) * kg <= 80 * 1024 && tm * tn <= 16 ? 2 : 1;
 }
 
-template <int TM, int TN, int D, int WM, int WN, int KG, int EPI>
-__global__ __launch_bounds__(64 * WM * WN * KG, w4_tile_waves(TM, TN, D, WM, WN, KG)) void fp4_linear_tile_kernel(W4Args a, int mt, int nt) {
-    constexpr int NW = WM * WN, BM = 16 * TM * WM;      // waves of a group
+template <int TM, int TN, int WN, int KG, int EPI>
+__global__ __launch_bounds__(64 * WN * KG, w4_tile_waves(TM, TN, WN, KG)) void fp4_linear_tile_kernel(W4Args a, int mt, int nt) {
+    constexpr int D = kW4Ring, NW = WN, BM = 16 * TM;   // NW: waves of a group
     constexpr int XS = BM * 128, WS = WN * TN * 1024;   // bytes of a slab of x, of a block of codes
-    constexpr int LX = XS / 1024 / NW, LW = TN / WM;    // 1 KB loads of x a wave and slab; tiles whose codes a wave fetches
+    constexpr int LX = XS / 1024 / NW, LW = TN;         // 1 KB loads of x a wave and slab; tiles whose codes a wave fetches
     constexpr int NO = EPI == W4_SWIGLU ? TN / 2 : TN;  // column tiles of y a wave
     constexpr int R = (D + 1) / 2;                      // blocks of codes in their ring
     constexpr int W0 = D * XS, S0 = W0 + R * WS;
     // loads that may be under way behind the barrier of an even and of an odd slab
     constexpr int AHEAD0 = (D - 2) * LX + (D - 1) / 2 * (LW + 1), AHEAD1 = (D - 2) * LX + (D - 2) / 2 * (LW + 1);
-    static_assert(D >= 3 && XS % (1024 * NW) == 0 && TN % WM == 0 && LW <= 4 && AHEAD0 < 64, "the waits below count these loads");
+    static_assert(D >= 3 && XS % (1024 * NW) == 0 && LW <= 4 && AHEAD0 < 64, "the waits below count these loads");
     constexpr int SS = 256 * NW, GS = S0 + R * SS;       // scales of a block; LDS of a group
     static_assert(KG == 1 || (KG - 1) * NW * TM * TN * 1024 <= KG * GS, "the groups' sums fit where their rings were");
     __shared__ __align__(1024) unsigned char smem_all[KG * GS];
@@ -282,7 +284,7 @@ __global__ __launch_bounds__(64 * WM * WN * KG, w4_tile_waves(TM, TN, D, WM, WN,
     const int64_t m0 = (int64_t)(t % mt) * BM;
     const int nb = t / mt;
     const int wave4 = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), wave = wave4 % NW, grp = wave4 / NW, lane = threadIdx.x % kWave;
-    const int l = lane % 16, g = lane / 16, wm = wave % WM, wn = wave / WM;
+    const int l = lane % 16, g = lane / 16;
     const int half = a.w.tiles / 2;
     // the group's blocks and slabs: a KG-th of K
     const int gb = (a.w.blocks + KG - 1) / KG, blk0 = grp * gb, sl0 = 2 * blk0;
@@ -321,9 +323,9 @@ __global__ __launch_bounds__(64 * WM * WN * KG, w4_tile_waves(TM, TN, D, WM, WN,
     const uint32_t lds = (uint32_t)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) unsigned char*)smem);
     uint32_t xa[2];
 #pragma unroll
-    for (int q = 0; q < 2; ++q) xa[q] = lds + (uint32_t)((wm * TM * 16 + l) * 128 + (((q * 4 + g) ^ w4_swz(l)) << 4));
-    const uint32_t wa = lds + (uint32_t)(W0 + wn * TN * 1024 + lane * 16);
-    const uint32_t sa = lds + (uint32_t)(S0 + wn * TN / LW * 256 + l * 4);   // tile j: its loader's place, 64 (j % LW) on
+    for (int q = 0; q < 2; ++q) xa[q] = lds + (uint32_t)(l * 128 + (((q * 4 + g) ^ w4_swz(l)) << 4));
+    const uint32_t wa = lds + (uint32_t)(W0 + wave * TN * 1024 + lane * 16);
+    const uint32_t sa = lds + (uint32_t)(S0 + wave * 256 + l * 4);   // tile j: its loader's place, 64 (j % LW) on
 
     f32x4_t acc[TM][TN];
 #pragma unroll
@@ -467,7 +469,7 @@ __global__ __launch_bounds__(64 * WM * WN * KG, w4_tile_waves(TM, TN, D, WM, WN,
         part(sl + 2, c0, c1);
         part(sl + 3, c1, c1);
     }
-    const int ct0 = (nb * WN + wn) * NO;   // first column tile of y
+    const int ct0 = (nb * WN + wave) * NO;   // first column tile of y
     float bias[NO][4] = {};                // all requested at once
     if (EPI != W4_SWIGLU && a.bias != nullptr) {
 #pragma unroll
@@ -500,7 +502,7 @@ __global__ __launch_bounds__(64 * WM * WN * KG, w4_tile_waves(TM, TN, D, WM, WN,
     }
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
-        const int64_t row = m0 + (wm * TM + i) * 16 + l;
+        const int64_t row = m0 + i * 16 + l;
         if (row >= a.M) continue;
 #pragma unroll
         for (int j = 0; j < NO; ++j) {
@@ -565,28 +567,30 @@ static void w4_launch_few(const W4Args& a, int cus, hipStream_t stream) {
 // rows over the projections of the models' dimensions on 256 CUs: fixed + per_group * x + slabs *
 // max(alone * rounds, full * x), x the workgroups that the busiest CU has (their mean and its ceiling,
 // weighted), rounds = x / resident, slabs those that one group of waves walks. The form that it picks
-// is 0.9 % off the best of them over the sweeps.
+// is 0.7 % off the best of them over the sweeps.
 struct W4Form {
-    int tm, tn, wm, wn, kg, resident;
+    int tm, tn, wn, kg, resident;
     float alone, full, fixed, per_group, mean;
 };
 constexpr W4Form kW4Forms[] = {
     // few rows: each wave a part of K and rings of its own
-    {1, 1, 1, 1, 8, 2, 0.197f, 0.247f, 2.71f, 0.37f, 0.38f},
-    {1, 2, 1, 1, 4, 3, 0.237f, 0.154f, 2.29f, 0.53f, 0.26f},
-    {1, 2, 1, 1, 8, 1, 0.253f, 0.319f, 1.80f, 1.76f, 0.21f},
-    {2, 2, 1, 1, 2, 4, 0.290f, 0.120f, 1.87f, 0.64f, 0.51f},
-    {2, 2, 1, 1, 4, 2, 0.304f, 0.234f, 2.13f, 1.07f, 0.45f},
-    {2, 2, 1, 1, 8, 1, 0.333f, 0.453f, 2.13f, 2.07f, 0.26f},
-    {2, 4, 1, 1, 2, 3, 0.379f, 0.157f, 1.62f, 1.47f, 0.19f},
-    // four waves beside each other share x; two such groups, or one
-    {2, 2, 1, 4, 2, 2, 0.320f, 0.290f, 2.62f, 1.04f, 0.25f},
-    {2, 2, 1, 4, 1, 4, 0.284f, 0.125f, 1.50f, 0.95f, 0.00f},
-    {4, 2, 1, 4, 1, 3, 0.290f, 0.252f, 3.21f, 0.62f, 0.51f},
-    {6, 2, 1, 4, 1, 2, 0.332f, 0.350f, 3.84f, 0.93f, 0.63f},
-    {8, 2, 1, 4, 1, 2, 0.382f, 0.447f, 4.53f, 1.23f, 0.64f},
-    {4, 4, 1, 4, 1, 2, 0.420f, 0.393f, 4.26f, 2.01f, 0.45f},
-    {6, 4, 1, 4, 1, 2, 0.519f, 0.518f, 4.77f, 2.72f, 0.37f},
+    {1, 1, 1, 8, 2, 0.197f, 0.247f, 2.71f, 0.37f, 0.38f},
+    {1, 2, 1, 2, 4, 0.259f, 0.069f, 1.66f, 0.41f, 0.00f},
+    {1, 2, 1, 4, 3, 0.238f, 0.153f, 2.29f, 0.54f, 0.25f},
+    {1, 2, 1, 8, 1, 0.100f, 0.318f, 1.89f, 1.67f, 0.20f},
+    {2, 2, 1, 2, 4, 0.288f, 0.119f, 1.87f, 0.65f, 0.49f},
+    {2, 2, 1, 4, 2, 0.304f, 0.235f, 2.14f, 1.07f, 0.45f},
+    {2, 2, 1, 8, 1, 0.333f, 0.453f, 2.13f, 2.07f, 0.26f},
+    {2, 4, 1, 2, 3, 0.394f, 0.159f, 1.50f, 1.45f, 0.19f},
+    // two or four waves beside each other share x, in groups that split K or alone
+    {2, 2, 2, 4, 1, 0.331f, 0.390f, 1.50f, 2.30f, 0.15f},
+    {2, 2, 4, 2, 2, 0.327f, 0.289f, 2.51f, 1.07f, 0.24f},
+    {2, 2, 4, 1, 4, 0.284f, 0.125f, 1.50f, 0.95f, 0.00f},
+    {4, 2, 4, 1, 3, 0.290f, 0.252f, 3.21f, 0.62f, 0.51f},
+    {6, 2, 4, 1, 2, 0.332f, 0.350f, 3.84f, 0.93f, 0.63f},
+    {8, 2, 4, 1, 2, 0.382f, 0.447f, 4.53f, 1.23f, 0.64f},
+    {4, 4, 4, 1, 2, 0.420f, 0.393f, 4.26f, 2.01f, 0.45f},
+    {6, 4, 4, 1, 2, 0.519f, 0.518f, 4.77f, 2.72f, 0.37f},
 };
 constexpr int kW4FormCount = sizeof(kW4Forms) / sizeof(kW4Forms[0]);
 
@@ -595,7 +599,7 @@ struct W4Tiles {
 };
 
 static W4Tiles w4_tiles_of(const W4Form& f, const W4Args& a, bool swiglu) {
-    const int cols = 16 * f.wn * (swiglu ? f.tn / 2 : f.tn), rows = 16 * f.wm * f.tm;
+    const int cols = 16 * f.wn * (swiglu ? f.tn / 2 : f.tn), rows = 16 * f.tm;
     return W4Tiles{(a.M + rows - 1) / rows, (a.N + cols - 1) / cols};
 }
 
@@ -629,8 +633,8 @@ static int w4_launch(const char* who, const W4Args& a, hipStream_t stream) {
         constexpr W4Form f = kW4Forms[decltype(ic)::value];
         if constexpr (EPI != W4_SWIGLU || f.tn % 2 == 0) {
             if (pick == decltype(ic)::value)
-                hipLaunchKernelGGL((fp4_linear_tile_kernel<f.tm, f.tn, 3, f.wm, f.wn, f.kg, EPI>), grid,
-                                   dim3(kWave * f.wm * f.wn * f.kg), 0, stream, a, (int)t.mt, (int)t.nt);
+                hipLaunchKernelGGL((fp4_linear_tile_kernel<f.tm, f.tn, f.wn, f.kg, EPI>), grid,
+                                   dim3(kWave * f.wn * f.kg), 0, stream, a, (int)t.mt, (int)t.nt);
         }
     };
     [&]<int... I>(std::integer_sequence<int, I...>) { (go(std::integral_constant<int, I>{}), ...); }

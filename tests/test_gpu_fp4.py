@@ -140,7 +140,8 @@ def test_swiglu(gpu, m, hidden, inter):
 # sizes that between them take every shape of workgroup, with widths and lengths that end inside its tiles
 WIDE = [(7, 32, 50), (5, 32, 4177), (5, 1664, 4303), (17, 32, 4481), (19, 1568, 8650), (19, 5184, 4250), (17, 928, 34530),
         (35, 672, 15219), (5, 32, 16530), (97, 160, 41515), (33, 1824, 64960), (71, 1088, 57690), (6, 544, 50), (5, 288, 17), (3001, 672, 270),
-        (65, 32, 53179), (723, 32, 57850), (3, 8224, 70), (4, 6176, 65530),
+        (65, 32, 53179), (723, 32, 57850), (5, 864, 4460), (17, 800, 4351), (17, 1440, 8410),
+        (17, 704, 20401), (3, 8224, 70), (4, 6176, 65530),
         (4, 1056, 65601), (2, 32, 65537)]
 
 
@@ -176,6 +177,7 @@ def test_linear_every_shape(gpu, m, k, out, f32):
 @pytest.mark.parametrize("m,hidden,inter", [(5, 32, 16), (5, 544, 16), (17, 32, 2144), (18, 1504, 4160), (18, 5024, 2160),
                                             (42, 992, 8272), (35, 672, 7936), (5, 32, 8288), (33, 32, 43248), (33, 1088, 56288),
                                             (72, 1120, 28112), (5, 1568, 16), (1667, 672, 288), (66, 32, 25200), (871, 32, 22256),
+                                            (5, 800, 16), (21, 800, 2144), (17, 832, 7216), (17, 672, 9392),
                                             (4, 4192, 80), (4, 8224, 48), (2, 2080, 33040)])
 def test_swiglu_every_shape(gpu, m, hidden, inter):
     g = _gen(m + hidden + inter)
