@@ -287,7 +287,7 @@ def _y_tol(y, x, w, eps):
 
 
 @pytest.mark.parametrize("hq,hkv,hd", HEADS)
-@pytest.mark.parametrize("S,base", [(1, 0), (1, 63), (5, 3), (33, 31), (130, 1000000)])
+@pytest.mark.parametrize("S,base", [(1, 0), (1, 63), (5, 3), (33, 31), (130, 1000000), (2051, 13)])
 @pytest.mark.parametrize("norm", [True, False])
 @pytest.mark.parametrize("fp4", [False, True])
 def test_write(gpu, hq, hkv, hd, S, base, norm, fp4):
@@ -328,12 +328,13 @@ def test_write(gpu, hq, hkv, hd, S, base, norm, fp4):
     _within(q_out, q, _y_tol(q, x[:, :hq], qw, 1e-6), "queries")
 
 
+@pytest.mark.parametrize("S", [37, 2051])
 @pytest.mark.parametrize("fp4", [False, True])
-def test_write_mrope_offsets_strides_and_in_place(gpu, fp4):
+def test_write_mrope_offsets_strides_and_in_place(gpu, fp4, S):
     """M-RoPE ids with sections; without ids, offsets of queries and keys that differ; a strided bf16 cache; the queries
     written over their own columns."""
     g = _gen(9)
-    hq, hkv, hd, S, base, room = 16, 2, 128, 37, 11, 64
+    hq, hkv, hd, base, room = 16, 2, 128, 11, S + 27
     width = (hq + 2 * hkv) * hd
     qkv, qw, kw = _bf(g, S, width), 1 + _bf(g, hd, std=0.2), 1 + _bf(g, hd, std=0.2)
     x = qkv.double().view(S, -1, hd)
@@ -386,6 +387,46 @@ def test_write_at_a_device_length(gpu, fp4, length):
         outs.append([q] + dst)
     for a, b in zip(*outs):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("fp4", [False, True])
+@pytest.mark.parametrize("length", [1601, 1602, 1700, 1701])
+def test_write_many_rows_at_a_device_length(gpu, fp4, length):
+    """1602 rows, equal to blocks of 89 by the host's base; too short or long a length writes nothing."""
+    g = _gen(2)
+    hq, hkv, hd, S, room = 12, 2, 128, 1602, 1700
+    ctx = C.make_attention_ctx(hq, hkv, hd)
+    qkv, w = _bf(g, S, (hq + 2 * hkv) * hd).cuda(), (1 + _bf(g, hd, std=0.2)).cuda()
+    d_len = torch.tensor([length], dtype=torch.int32, device="cuda")
+    outs = []
+    for by_device in (True, False):
+        q = torch.full((S, hq, hd), 7.0, dtype=torch.bfloat16, device="cuda")
+        dst = [_buf(C.load().efm_kv_fp4_bytes(ctx, room), 0x11)] if fp4 else \
+            [torch.full((room, hkv, hd), 7.0, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+        if by_device:
+            _write(ctx, fp4, qkv, w, w, q, dst, room, S, 0, d_len=d_len)
+        elif S <= length <= room:
+            for i in range(0, S, 89):
+                _write(ctx, fp4, qkv[i:i + 89], w, w, q[i:i + 89], dst, room, 89, length - S + i)
+        torch.cuda.synchronize()
+        outs.append([q] + dst)
+    for a, b in zip(*outs):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("n", [40, 4200])
+def test_write_without_queries_in_many_rows(gpu, n):
+    """Keys and values alone, wide enough for rows together; nothing but the cache changes."""
+    g = _gen(n)
+    hq, hkv, hd = 14, 2, 64
+    ctx = C.make_attention_ctx(hq, hkv, hd)
+    qkv, w = _bf(g, n, 18 * 64), 1 + _bf(g, hd, std=0.2)
+    cache, dev = _buf(C.load().efm_kv_fp4_bytes(ctx, n)), qkv.cuda()
+    _write(ctx, True, dev, None, w.cuda(), None, [cache], n, n, 0)
+    k, v = _read(ctx, cache, n, 0, n, hkv, hd)
+    x = qkv.double().view(n, 18, 64)
+    assert torch.equal(k, R.rounded(R.norm_rope(x[:, 14:16], w, 1e-6, _positions(0, n, 32), 1e6)))
+    assert torch.equal(v, R.rounded(x[:, 16:])) and torch.equal(dev.cpu(), qkv)
 
 
 def test_write_without_queries_and_read_of_one_side(gpu):
