@@ -222,27 +222,22 @@ __global__ __launch_bounds__(TOKENS ? 512 : 1024) void qk_norm_rope_write_kernel
     }
 }
 
-// One lane for 8 channels of a row. Workgroups of the first half of the grid read keys, row after row;
-// the others values, 8 rows of an octet beside each other as they lie.
+// One lane for 8 channels of a row of head blockIdx.y: keys (blockIdx.z == 0) row after row, values 8 rows
+// of an octet beside each other as they lie.
 template <int HD>
 __global__ __launch_bounds__(256) void kv_fp4_read_kernel(const uint8_t* cache, KvFp4Layout lay, uint32_t first, uint32_t rows,
-                                                          uint32_t per, uint4* k_out, uint4* v_out) {
-    constexpr int J = HD / 8;
-    const bool values = blockIdx.x >= per;
+                                                          uint4* k_out, uint4* v_out) {
+    constexpr uint32_t J = HD / 8;
+    const bool values = blockIdx.z == 1;
     uint4* const out = values ? v_out : k_out;
     if (out == nullptr) return;
-    const int64_t i = (blockIdx.x - (values ? per : 0)) * 256ll + threadIdx.x;
-    int64_t row, h;
-    int j;
-    if (!values) {
-        j = (int)(i % J), h = i / J % lay.Hkv, row = first + i / J / lay.Hkv;
-    } else {
-        j = (int)(i / 8 % J), h = i / 8 / J % lay.Hkv, row = (first / 8 + i / 8 / J / lay.Hkv) * 8 + i % 8;
-    }
-    if (row < first || row >= (int64_t)first + rows) return;
-    const uint32_t w = *reinterpret_cast<const uint32_t*>(cache + (values ? lay.v((int)h) + lay.v_word(row, j) : lay.k((int)h) + lay.k_word(row, j)));
-    const uint32_t byte = cache[values ? lay.vs((int)h) + lay.v_scale(row, j) : lay.ks((int)h) + lay.k_scale(row, j)];
-    out[((row - first) * lay.Hkv + h) * J + j] = __builtin_bit_cast(uint4, fp4_unpack8(w, fp4_scale(byte)));
+    const uint32_t i = blockIdx.x * 256 + threadIdx.x;   // rows <= 2^24
+    const int h = blockIdx.y, j = (int)(values ? i / 8 % J : i % J);
+    const uint32_t row = values ? (first / 8 + i / 8 / J) * 8 + i % 8 : first + i / J;
+    if (row < first || row >= first + rows) return;
+    const uint32_t w = *reinterpret_cast<const uint32_t*>(cache + (values ? lay.v(h) + lay.v_word(row, j) : lay.k(h) + lay.k_word(row, j)));
+    const uint32_t byte = cache[values ? lay.vs(h) + lay.v_scale(row, j) : lay.ks(h) + lay.k_scale(row, j)];
+    out[((int64_t)(row - first) * lay.Hkv + h) * J + j] = __builtin_bit_cast(uint4, fp4_unpack8(w, fp4_scale(byte)));
 }
 
 static bool qk_aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -316,6 +311,8 @@ static int qk_write(const char* who, bool fp4, const efm_attention_ctx* ctx, con
     // one / together): 28/4 heads of 128, FP4: 64 tokens 4.5 / 5.7, 512 7.4 / 6.6, 1024 13.1 / 8.0, 4096
     // 37 / 16; bf16: 64 3.4 / 4.6, 512 4.6 / 5.2, 1024 9.1 / 6.6, 4096 25.2 / 14.4. 14/2 heads of 64, 2000
     // tokens: FP4 8.6 / 5.6, bf16 5.4 / 4.7.
+    // Eight waves for tokens together: 4096 of 28/4 heads into a bf16 cache 14.5, with six 15.5, twelve 16.1;
+    // 1344 of 16/2 heads 6.0, with five 6.4, ten 6.2.
     auto launch = [&](auto hdc, auto fc) {
         constexpr int HD = decltype(hdc)::value, ROWS = kWave * 8 / HD;
         constexpr bool F = decltype(fc)::value;
@@ -370,19 +367,17 @@ extern "C" int efm_kv_fp4_read(const efm_attention_ctx* ctx, const void* cache, 
     if (!qk_aligned(cache) || !qk_aligned(k_out) || !qk_aligned(v_out))
         return set_error(EFM_ERR_INVALID_ARGUMENT, "kv_fp4_read: pointers must be 16-byte aligned");
     if (max_rows > (1u << 24)) return set_error(EFM_ERR_UNSUPPORTED, "kv_fp4_read: max_rows %u too large", max_rows);
-    if (ctx->num_qo_heads > (1u << 16))
+    if (ctx->num_qo_heads >= (1u << 16))
         return set_error(EFM_ERR_UNSUPPORTED, "kv_fp4_read: %u query heads", ctx->num_qo_heads);
     if (first > max_rows || rows > max_rows - first)
         return set_error(EFM_ERR_INVALID_ARGUMENT, "kv_fp4_read: rows %u + %u do not fit max_rows %u", first, rows, max_rows);
     if (rows == 0) return EFM_OK;
     const KvFp4Layout lay(KvFp4Layout::rows(max_rows), (int)ctx->num_kv_heads, (int)ctx->head_dim);
-    // lanes for keys, and for values' whole blocks of 8 rows, the larger count
-    const int64_t lanes = ((int64_t)rows + 14) / 8 * 8 * ctx->num_kv_heads * (ctx->head_dim / 8);
-    if (lanes > (1ll << 38)) return set_error(EFM_ERR_UNSUPPORTED, "kv_fp4_read: too many rows");
-    const uint32_t per = (uint32_t)((lanes + 255) / 256);
+    // a head's lanes for values' whole blocks of 8 rows; keys take no more
+    const uint32_t lanes = (rows + 14) / 8 * 8 * (ctx->head_dim / 8);
     auto launch = [&](auto hdc) {
-        hipLaunchKernelGGL(kv_fp4_read_kernel<decltype(hdc)::value>, dim3(2 * per), dim3(256), 0, stream,
-                           static_cast<const uint8_t*>(cache), lay, first, rows, per, static_cast<uint4*>(k_out),
+        hipLaunchKernelGGL(kv_fp4_read_kernel<decltype(hdc)::value>, dim3((lanes + 255) / 256, ctx->num_kv_heads, 2), dim3(256), 0,
+                           stream, static_cast<const uint8_t*>(cache), lay, first, rows, static_cast<uint4*>(k_out),
                            static_cast<uint4*>(v_out));
     };
     if (ctx->head_dim == 128) launch(std::integral_constant<int, 128>{});
