@@ -98,6 +98,8 @@ template <typename T, int LANES, typename CS>
 __device__ __forceinline__ void turn8(T* x, CS cs) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
+        // 64-bit pairs one after another: all eight at once would cost 20 registers, and with them waves
+        if constexpr (sizeof(T) == 8) __builtin_amdgcn_sched_barrier(0);
         const T o = row_other<LANES>(x[e]);
         const auto v = cs(e);
         x[e] = x[e] * (T)v.x + o * (T)v.y;
@@ -127,7 +129,7 @@ __global__ __launch_bounds__(TOKENS ? 512 : 1024) void qk_norm_rope_write_kernel
     uint4 next[2] = {request(h), request(h + step)};
     uint4 qw = make_uint4(0, 0, 0, 0), kw = qw;
     if (a.q_w != nullptr) qw = reinterpret_cast<const uint4*>(a.q_w)[j];
-    if (a.k_w != nullptr) kw = reinterpret_cast<const uint4*>(a.k_w)[j];
+    if (!FP4 && a.k_w != nullptr) kw = reinterpret_cast<const uint4*>(a.k_w)[j];
     uint32_t base = a.base;
     if (a.d_kv_len != nullptr) {
         const uint32_t L = a.d_kv_len[0];
@@ -179,7 +181,7 @@ __global__ __launch_bounds__(TOKENS ? 512 : 1024) void qk_norm_rope_write_kernel
             Y y[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) y[e] = (Y)x[e];
-            if (a.k_w != nullptr) norm8<Y, LANES>(y, kw, (Y)a.eps);
+            if (a.k_w != nullptr) norm8<Y, LANES>(y, FP4 ? reinterpret_cast<const uint4*>(a.k_w)[j] : kw, (Y)a.eps);
             if (a.rotate) {
                 int at = j % HL;
                 asm volatile("" : "+v"(at));   // read here: held over the loop, they would cost 32 registers
