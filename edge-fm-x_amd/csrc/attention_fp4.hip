@@ -8,9 +8,9 @@
 // product O^T = V^T P^T takes from it as its second operand: P never moves between lanes. The
 // codes become bf16 in registers, exactly.
 // A workgroup's waves take every NW-th tile of its split of the keys, each with the running
-// maximum and sum of its own softmax; their outputs meet in LDS. Where the keys are split over
-// workgroups too, those write unnormalised outputs with (maximum, sum), and a second kernel joins
-// them.
+// maximum and sum of its own softmax; their outputs meet in LDS (many rows: a kernel of its own,
+// below). Where the keys are split over workgroups too, those write unnormalised outputs with
+// (maximum, sum), and a second kernel joins them.
 #include "fp4.hpp"
 
 #include <algorithm>
