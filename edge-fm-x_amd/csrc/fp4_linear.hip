@@ -127,10 +127,12 @@ __global__ __launch_bounds__(1024) void fp4_linear_kernel(W4Args a) {
         wp[j] = a.w.codes + (size_t)tile * a.w.blocks * 1024 + lane * 16;
         sp[j] = a.w.scales + (size_t)tile * a.w.blocks * 64 + l * 4;
     }
-    // not in LDS: rows past the last are asked for past the buffer's end, and come as zeros
+    // not in LDS: rows past the last, and columns past the last row's, are asked for past the buffer's end and
+    // come as zeros. All of the offset is in the lane's register, since a scalar offset is outside the check
+    // of that end.
     const __amdgpu_buffer_rsrc_t xb =
         __builtin_amdgcn_make_buffer_rsrc(const_cast<bf16_t*>(a.x), (short)0, (int)(a.M * a.K * 2), 0x00020000);
-    const int xo = l < a.M ? (int)(l * a.K + 8 * g) * 2 : -1;
+    const uint32_t xo = l < a.M ? (uint32_t)(l * a.K + 8 * g) * 2 : 0x80000000u;
     // in LDS, behind the sums: row r at r * (K + 8) values, so that the rows' reads meet different banks
     unsigned char* const xl = reinterpret_cast<unsigned char*>(red) + (size_t)KW * NT * 1024;
     const unsigned char* const xr = xl + (l < a.M ? l : 0) * (a.K * 2 + 16) + 16 * g;
@@ -157,7 +159,7 @@ __global__ __launch_bounds__(1024) void fp4_linear_kernel(W4Args a) {
         }
         if constexpr (!XLDS) {
 #pragma unroll
-            for (int q = 0; q < 4; ++q) x[st][q] = __builtin_amdgcn_raw_buffer_load_b128(xb, xo, (b * kW4Cols + 32 * q) * 2, 0);
+            for (int q = 0; q < 4; ++q) x[st][q] = __builtin_amdgcn_raw_buffer_load_b128(xb, (int)(xo + (b * kW4Cols + 32 * q) * 2), 0, 0);
         }
     };
     auto multiply = [&](int st, int b) {
@@ -239,10 +241,11 @@ __global__ __launch_bounds__(1024) void fp4_linear_kernel(W4Args a) {
 // operand: a lane ends with four consecutive columns of a row of y.
 constexpr int w4_swz(int r) { return (r >> 1) & 7; }
 
-// 16 bytes a lane from base + lane_off + off into consecutive places at dst; zeros past `bytes`.
-__device__ __forceinline__ void w4_dma16(const void* base, uint32_t bytes, uint32_t lane_off, uint32_t off, void* dst) {
+// 16 bytes a lane from base + off, off a lane's own, into consecutive places at dst; zeros past `bytes`. The
+// scalar offset of the load stays 0: it is outside the check of that end.
+__device__ __forceinline__ void w4_dma16(const void* base, uint32_t bytes, uint32_t off, void* dst) {
     const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0, (int)bytes, 0x00020000);
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)dst, 16, (int)lane_off, (int)off, 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)dst, 16, (int)off, 0, 0, 0);
 }
 // 4 bytes a lane.
 __device__ __forceinline__ void w4_dma4(const void* src, void* dst) {
@@ -311,12 +314,12 @@ __global__ __launch_bounds__(64 * WN * KG, w4_tile_waves(TM, TN, WN, KG)) void f
     }
     // loads past the end repeat the last slab and block into places that nothing reads
     auto load_x = [&](int slab, int i) {
-        w4_dma16(xbase, xbytes, xv[i], (uint32_t)min(sl0 + slab, all_slabs - 1) * 128, smem + slab % D * XS + (i * NW + wave) * 1024);
+        w4_dma16(xbase, xbytes, xv[i] + (uint32_t)min(sl0 + slab, all_slabs - 1) * 128, smem + slab % D * XS + (i * NW + wave) * 1024);
     };
     auto load_w = [&](int b, int i) {
         const size_t at = (size_t)min(blk0 + b, a.w.blocks - 1);
         if (i < LW)
-            w4_dma16(wp[i < LW ? i : 0] + at * 1024, 1024, lane * 16, 0, smem + W0 + b % R * WS + (wave * LW + i) * 1024);
+            w4_dma16(wp[i < LW ? i : 0] + at * 1024, 1024, lane * 16, smem + W0 + b % R * WS + (wave * LW + i) * 1024);
         else
             w4_dma4(sp + at * 64, smem + S0 + b % R * SS + wave * 256);
     };

@@ -101,6 +101,15 @@ def _product(x, w):
     return x @ w.T, (k / 32 + 32 + 64) * 2.0 ** -23 * (x.abs() @ w.abs().T)
 
 
+def _swiglu(x, w):
+    """(bf16(silu(bf16(gate)) * bf16(up)) in 64 bits, its bound): both products' errors through the activation."""
+    (up, gate), (eu, eg) = (t.chunk(2, 1) for t in _product(x.double(), w))
+    silu = gate * torch.sigmoid(gate)
+    du, dg = eu + HALF * (up.abs() + eu), eg + HALF * (gate.abs() + eg)
+    tol = 1.1 * dg * (up.abs() + du) + silu.abs() * du   # |silu'| < 1.1
+    return silu * up, tol + (HALF + 2.0 ** -20) * ((silu * up).abs() + tol)
+
+
 SHAPES = [(1, 32, 1), (1, 896, 1152), (1, 160, 17), (1, 18944, 100), (2, 96, 33), (5, 4864, 896), (16, 1536, 300), (17, 544, 48),
           (31, 992, 130), (33, 288, 64), (64, 2048, 272), (100, 160, 4608), (129, 896, 257), (300, 1536, 640), (1000, 512, 384)]
 
@@ -196,6 +205,35 @@ def test_swiglu_every_shape(gpu, m, hidden, inter):
     tol = 1.1 * dg * (up.abs() + du) + silu.abs() * du   # |silu'| < 1.1
     _within(ys[0][:, at.cuda()], silu * up, tol + (HALF + 2.0 ** -20) * ((silu * up).abs() + tol), f"{m} {hidden} {inter}")
     assert not ys[0].isnan().any() and torch.equal(*ys)
+
+
+def _ahead_of_nan(x):
+    """x in a larger buffer that holds NaN behind it."""
+    wide = torch.full((x.numel() + 512,), math.nan, dtype=torch.bfloat16, device="cuda")
+    wide[:x.numel()] = x.flatten().cuda()
+    return wide[:x.numel()].view(x.shape)
+
+
+@pytest.mark.parametrize("m,k,out", [(1, 24608, 17), (1, 24672, 40), (1, 24736, 130), (2, 24608, 33), (5, 160, 50), (17, 544, 48),
+                                     (100, 672, 300), (500, 416, 1024)])
+def test_linear_whose_last_columns_end_inside_a_load(gpu, m, k, out):
+    """Lengths of K that end inside the last block or slab, one row of x past LDS among them: what lies behind x stays out."""
+    g = _gen(m + k + out)
+    code, byte = _weights(g, out, k)
+    x = _bf(g, m, k)
+    y = _linear(_ahead_of_nan(x), _pack(R.halves(code), byte), k, out, None, True)
+    _within(y, *_product(x.double(), R.values(code, byte)), f"{m} x {k} -> {out}")
+
+
+@pytest.mark.parametrize("m,hidden,inter", [(1, 16416, 16), (1, 16480, 48), (1, 16928, 48), (3, 5472, 32), (40, 160, 80)])
+def test_swiglu_whose_last_columns_end_inside_a_load(gpu, m, hidden, inter):
+    g = _gen(m + hidden + inter)
+    code, byte = _weights(g, 2 * inter, hidden)
+    x, packed = _bf(g, m, hidden), _pack(R.halves(code), byte)
+    y, xd = torch.full((m, inter), math.nan, dtype=torch.bfloat16, device="cuda"), _ahead_of_nan(x)
+    C.call("efm_fused_gate_up_swiglu_fp4", m, hidden, inter, ptr(xd), ptr(packed), ptr(y), None, 0, stream())
+    torch.cuda.synchronize()
+    _within(y, *_swiglu(x, R.values(code, byte)), f"{m} {hidden} {inter}")
 
 
 @pytest.mark.parametrize("m", [1, 20, 200])
