@@ -537,7 +537,9 @@ constexpr int kW4FewRows = 4;
 
 // Waves of a workgroup: 16 while it is alone on its CU, else 8, and no more than blocks of K. One tile
 // of weight rows each (SwiGLU: one of up and one of gate), two where there are thousands (152064 x
-// 3584: 46 us, 60 with one). Two blocks under way where a wave has three or more to go.
+// 3584: 46 us, 60 with one). Two blocks under way where a wave has three or more to go, and always where
+// x is outside LDS, from 48 blocks on; SwiGLU's sums of two tiles a wave put x outside from 32 on, where
+// 16 waves have one under way.
 template <int EPI>
 static void w4_launch_few(const W4Args& a, int cus, hipStream_t stream) {
     const int half = EPI == W4_SWIGLU ? 2 : 1;
@@ -545,9 +547,9 @@ static void w4_launch_few(const W4Args& a, int cus, hipStream_t stream) {
     const int nt = wide ? 2 : half, groups = (a.w.tiles / half + (wide ? 1 : 0)) / (wide ? 2 : 1);
     int kw = groups <= 2 * cus ? 16 : 8;
     while (kw > 1 && kw / 2 >= a.w.blocks) kw /= 2;
-    const bool two = a.w.blocks >= 3 * kw;
     const size_t sums = (size_t)kw * nt * 1024, x = (size_t)a.M * (a.K * 2 + 16);
     const bool xlds = sums + x <= 64 * 1024;
+    const bool two = a.w.blocks >= 3 * kw || (EPI != W4_SWIGLU && !xlds);
     auto go = [&](auto ntc, auto pc, auto xc) {
         constexpr int NT = decltype(ntc)::value, P = decltype(pc)::value;
         if (nt != NT || two != (P == 2) || xlds != decltype(xc)::value) return;
@@ -558,7 +560,6 @@ static void w4_launch_few(const W4Args& a, int cus, hipStream_t stream) {
     auto each = [&](auto ntc) {
         go(ntc, integral_constant<int, 1>{}, std::true_type{});
         go(ntc, integral_constant<int, 2>{}, std::true_type{});
-        // x past LDS has 40 blocks and more: two under way, but for SwiGLU's 16 waves with two tiles each
         if constexpr (EPI == W4_SWIGLU) go(ntc, integral_constant<int, 1>{}, std::false_type{});
         go(ntc, integral_constant<int, 2>{}, std::false_type{});
     };

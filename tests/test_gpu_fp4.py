@@ -236,6 +236,26 @@ def test_swiglu_whose_last_columns_end_inside_a_load(gpu, m, hidden, inter):
     _within(y, *_swiglu(x, R.values(code, byte)), f"{m} {hidden} {inter}")
 
 
+@pytest.mark.parametrize("m,k", [(m, k) for m, last in ((1, 24544), (2, 12256), (3, 8160), (4, 6112)) for k in (last, last + 32)])
+def test_linear_where_x_leaves_lds(gpu, m, k):
+    """The longest rows of x that LDS holds, and the next."""
+    g = _gen(m + k)
+    code, byte = _weights(g, 50, k)
+    x = _bf(g, m, k)
+    _within(_linear(x.cuda(), _pack(R.halves(code), byte), k, 50, None, True), *_product(x.double(), R.values(code, byte)))
+
+
+@pytest.mark.parametrize("m,hidden", [(m, k) for m, last in ((1, 16352), (4, 4064)) for k in (last, last + 32)])
+def test_swiglu_where_x_leaves_lds(gpu, m, hidden):
+    g = _gen(m + hidden)
+    code, byte = _weights(g, 96, hidden)
+    x, packed = _bf(g, m, hidden), _pack(R.halves(code), byte)
+    y, xd = torch.full((m, 48), math.nan, dtype=torch.bfloat16, device="cuda"), x.cuda()
+    C.call("efm_fused_gate_up_swiglu_fp4", m, hidden, 48, ptr(xd), ptr(packed), ptr(y), None, 0, stream())
+    torch.cuda.synchronize()
+    _within(y, *_swiglu(x, R.values(code, byte)))
+
+
 @pytest.mark.parametrize("m", [1, 20, 200])
 @pytest.mark.parametrize("low,high,power", [(0, 4, 120), (250, 255, -120)])
 def test_linear_smallest_and_largest_scales(gpu, m, low, high, power):
