@@ -224,17 +224,17 @@ __global__ __launch_bounds__(TOKENS ? 512 : 1024) void qk_norm_rope_write_kernel
     }
 }
 
-// One lane for 8 channels of a row of head blockIdx.y: keys (blockIdx.z == 0) row after row, values 8 rows
+// One lane for 8 channels of a row of head head0 + blockIdx.y: keys (blockIdx.z == 0) row after row, values 8 rows
 // of an octet beside each other as they lie.
 template <int HD>
-__global__ __launch_bounds__(256) void kv_fp4_read_kernel(const uint8_t* cache, KvFp4Layout lay, uint32_t first, uint32_t rows,
-                                                          uint4* k_out, uint4* v_out) {
+__global__ __launch_bounds__(256) void kv_fp4_read_kernel(const uint8_t* cache, KvFp4Layout lay, int head0, uint32_t first,
+                                                          uint32_t rows, uint4* k_out, uint4* v_out) {
     constexpr uint32_t J = HD / 8;
     const bool values = blockIdx.z == 1;
     uint4* const out = values ? v_out : k_out;
     if (out == nullptr) return;
     const uint32_t i = blockIdx.x * 256 + threadIdx.x;   // rows <= 2^24
-    const int h = blockIdx.y, j = (int)(values ? i / 8 % J : i % J);
+    const int h = head0 + blockIdx.y, j = (int)(values ? i / 8 % J : i % J);
     const uint32_t row = values ? (first / 8 + i / 8 / J) * 8 + i % 8 : first + i / J;
     if (row < first || row >= first + rows) return;
     const uint32_t w = *reinterpret_cast<const uint32_t*>(cache + (values ? lay.v(h) + lay.v_word(row, j) : lay.k(h) + lay.k_word(row, j)));
@@ -369,7 +369,7 @@ extern "C" int efm_kv_fp4_read(const efm_attention_ctx* ctx, const void* cache, 
     if (!qk_aligned(cache) || !qk_aligned(k_out) || !qk_aligned(v_out))
         return set_error(EFM_ERR_INVALID_ARGUMENT, "kv_fp4_read: pointers must be 16-byte aligned");
     if (max_rows > (1u << 24)) return set_error(EFM_ERR_UNSUPPORTED, "kv_fp4_read: max_rows %u too large", max_rows);
-    if (ctx->num_qo_heads >= (1u << 16))
+    if (ctx->num_qo_heads > (1u << 16))
         return set_error(EFM_ERR_UNSUPPORTED, "kv_fp4_read: %u query heads", ctx->num_qo_heads);
     if (first > max_rows || rows > max_rows - first)
         return set_error(EFM_ERR_INVALID_ARGUMENT, "kv_fp4_read: rows %u + %u do not fit max_rows %u", first, rows, max_rows);
@@ -377,10 +377,13 @@ extern "C" int efm_kv_fp4_read(const efm_attention_ctx* ctx, const void* cache, 
     const KvFp4Layout lay(KvFp4Layout::rows(max_rows), (int)ctx->num_kv_heads, (int)ctx->head_dim);
     // a head's lanes for values' whole blocks of 8 rows; keys take no more
     const uint32_t lanes = (rows + 14) / 8 * 8 * (ctx->head_dim / 8);
+    const uint32_t grid_heads = 65535;   // a grid holds one head less than a cache may have
     auto launch = [&](auto hdc) {
-        hipLaunchKernelGGL(kv_fp4_read_kernel<decltype(hdc)::value>, dim3((lanes + 255) / 256, ctx->num_kv_heads, 2), dim3(256), 0,
-                           stream, static_cast<const uint8_t*>(cache), lay, first, rows, static_cast<uint4*>(k_out),
-                           static_cast<uint4*>(v_out));
+        for (uint32_t h = 0; h < ctx->num_kv_heads; h += grid_heads)
+            hipLaunchKernelGGL(kv_fp4_read_kernel<decltype(hdc)::value>,
+                               dim3((lanes + 255) / 256, std::min(ctx->num_kv_heads - h, grid_heads), 2), dim3(256), 0, stream,
+                               static_cast<const uint8_t*>(cache), lay, (int)h, first, rows, static_cast<uint4*>(k_out),
+                               static_cast<uint4*>(v_out));
     };
     if (ctx->head_dim == 128) launch(std::integral_constant<int, 128>{});
     else launch(std::integral_constant<int, 64>{});

@@ -149,3 +149,14 @@ def test_more_heads_than_an_index_holds():
     assert _decode(ctx=big) == UNSUP and _rows(ctx=big) == UNSUP
     assert _rows(ctx=_ctx(1 << 15, 1 << 15, rope=False), n=1 << 16, kv=1 << 16, room=1 << 16) == UNSUP
     assert C.load().efm_kv_fp4_bytes(big, 64) == 0 and C.load().efm_kv_fp4_bytes(_ctx(), 1 << 25) == 0
+
+
+def test_every_operator_of_the_cache_takes_the_same_heads():
+    most, more = _ctx(1 << 16, 1 << 16, hd=64, rope=False), _ctx(1 << 17, 1 << 17, hd=64, rope=False)
+    read = lambda c: _rc("efm_kv_fp4_read", c, P, 64, 0, 0, P, P, None)  # noqa: E731
+    write = lambda c: _write(True, ctx=c, seq=0)  # noqa: E731
+    rows = lambda c: _rows(ctx=c, n=0)  # noqa: E731
+    for call in (read, write, rows):
+        assert call(most) == C.EFM_OK
+    assert read(more) == UNSUP and write(more) == UNSUP
+    assert C.load().efm_kv_fp4_bytes(most, 64) > 0 and C.load().efm_kv_fp4_bytes(more, 64) == 0

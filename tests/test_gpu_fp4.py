@@ -502,6 +502,23 @@ def test_write_without_queries_and_read_of_one_side(gpu):
     assert torch.equal(k.cpu().double(), R.rounded(x[5:, 14:16])) and torch.equal(v.cpu().double(), R.rounded(x[5:, 16:]))
 
 
+@pytest.mark.parametrize("heads", [65535, 65536])
+def test_the_most_heads(gpu, heads):
+    """Written, read back and attended: a row of one key is its value."""
+    g = _gen(heads)
+    ctx = C.make_attention_ctx(heads, heads, 64, rope=False)
+    qkv = _bf(g, 2, 3 * heads * 64)
+    x = qkv.view(2, 3 * heads, 64)
+    cache, q = _buf(C.load().efm_kv_fp4_bytes(ctx, 3), 0xff), torch.empty(2, heads, 64, dtype=torch.bfloat16, device="cuda")
+    _write(ctx, True, qkv.cuda(), None, None, q, [cache], 3, 2, 0)
+    k, v = _read(ctx, cache, 3, 0, 2, heads, 64)
+    at = torch.cat([torch.arange(40), torch.randint(0, heads, (500,), generator=g), torch.arange(heads - 40, heads)])
+    assert torch.equal(q.cpu(), x[:, :heads])
+    assert torch.equal(k[:, at], R.rounded(x[:, heads + at])) and torch.equal(v[:, at], R.rounded(x[:, 2 * heads + at]))
+    assert torch.equal(_decode(ctx, q[:1], cache, 3, 1).cpu().double(), v[:1])
+    assert torch.equal(_rows(ctx, q, cache, 3, 2, 2)[0].cpu().double(), v[0])
+
+
 @pytest.mark.parametrize("n,kv", [(1, 70), (40, 100), (600, 900)])
 def test_the_largest_values_reach_the_rows_that_see_them(gpu, n, kv):
     """Values up to 7 * 2^125 are stored as finite ones, larger as NaN: neither reaches a row before their key."""
