@@ -23,6 +23,8 @@ typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
 constexpr int kFp4Group = 32;
 constexpr uint32_t kFp4ScaleNan = 255;
+// A grid's threads stay below 2^32: past that the runtime starts the remainder alone, without an error.
+constexpr int64_t kGridThreads = 0xffffffffll;
 constexpr int kFp4MinExp = -125, kFp4MaxExp = 125;
 
 // The scale as fp32 (byte 0 comes out as 0, which the conversion reads as 2^-127).

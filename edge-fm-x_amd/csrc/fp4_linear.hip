@@ -57,21 +57,21 @@ __global__ __launch_bounds__(256) void fp4_quantize_kernel(const uint4* w, uint3
 __global__ __launch_bounds__(256) void fp4_pack_kernel(const uint8_t* codes, const uint8_t* scales, uint4* out_codes,
                                                        uint32_t* out_scales, int64_t in, int64_t out, int blocks,
                                                        int64_t total) {
-    const int64_t t = blockIdx.x * 4ll + threadIdx.x / kWave;
-    if (t >= total) return;
     const int lane = threadIdx.x % kWave, g = lane / 16;
-    const int64_t row = t / blocks * kW4Rows + lane % 16, col = t % blocks * kW4Cols;
-    uint32_t w[4] = {0, 0, 0, 0}, s = 0;
-    if (row < out) {
+    for (int64_t t = blockIdx.x * 4ll + threadIdx.x / kWave; t < total; t += gridDim.x * 4ll) {
+        const int64_t row = t / blocks * kW4Rows + lane % 16, col = t % blocks * kW4Cols;
+        uint32_t w[4] = {0, 0, 0, 0}, s = 0;
+        if (row < out) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if (col + 32 * i >= in) break;
-            w[i] = *reinterpret_cast<const uint32_t*>(codes + (row * in + col + 32 * i + 8 * g) / 2);
-            s |= (uint32_t)scales[(row * in + col) / 32 + i] << (8 * i);
+            for (int i = 0; i < 4; ++i) {
+                if (col + 32 * i >= in) break;
+                w[i] = *reinterpret_cast<const uint32_t*>(codes + (row * in + col + 32 * i + 8 * g) / 2);
+                s |= (uint32_t)scales[(row * in + col) / 32 + i] << (8 * i);
+            }
         }
+        out_codes[t * 64 + lane] = make_uint4(w[0], w[1], w[2], w[3]);
+        if (lane < 16) out_scales[t * 16 + lane] = s;
     }
-    out_codes[t * 64 + lane] = make_uint4(w[0], w[1], w[2], w[3]);
-    if (lane < 16) out_scales[t * 16 + lane] = s;
 }
 
 enum { W4_BF16 = 0, W4_F32 = 1, W4_SWIGLU = 2 };
@@ -676,7 +676,7 @@ extern "C" int efm_fp4_pack(int64_t in_features, int64_t out_features, const uin
         return set_error(EFM_ERR_INVALID_ARGUMENT, "fp4_pack: codes and packed must be 16-byte aligned");
     const int64_t total = (int64_t)w4_tiles(out_features) * w4_blocks(in_features);
     uint8_t* p = static_cast<uint8_t*>(packed);
-    hipLaunchKernelGGL(fp4_pack_kernel, dim3((unsigned)((total + 3) / 4)), dim3(256), 0, stream, codes, scales,
+    hipLaunchKernelGGL(fp4_pack_kernel, dim3((unsigned)std::min(kGridThreads / 256, (total + 3) / 4)), dim3(256), 0, stream, codes, scales,
                        reinterpret_cast<uint4*>(p), reinterpret_cast<uint32_t*>(p + w4_code_bytes(in_features, out_features)),
                        in_features, out_features, w4_blocks(in_features), total);
     return check_launch("fp4_pack");

@@ -77,6 +77,44 @@ def test_quantize_equals_the_definition(gpu):
     assert torch.equal(codes.cpu(), R.halves(code))
 
 
+def test_quantize_many_groups(gpu):
+    """More values than a pass of the grid takes: the parts by themselves give the same."""
+    g = torch.Generator(device="cuda").manual_seed(2)
+    w = torch.randn(8200, 4128, generator=g, device="cuda").bfloat16()
+    codes, scales = _quantize(w)
+    for lo, hi in ((0, 2000), (2000, 6000), (6000, 8200)):
+        c, s = _quantize(w[lo:hi].contiguous())
+        assert torch.equal(codes[lo:hi], c) and torch.equal(scales[lo:hi], s)
+    at = torch.tensor([0, 4063, 4064, 8199])   # the grid's first pass ends in row 4064
+    code, byte = R.quantize(w[at.cuda()])
+    assert torch.equal(scales.cpu()[at], byte) and torch.equal(codes.cpu()[at], R.halves(code))
+
+
+@pytest.mark.parametrize("k,out", [(1 << 20, (1 << 17) + 24)])
+def test_pack_past_32_bits_of_threads(gpu, k, out):
+    """The first, a middle and the last tile of 73 GB of weights, equal to the packing of their rows alone."""
+    lib = C.load()
+    if torch.cuda.mem_get_info()[0] < 200 << 30:
+        pytest.skip("needs 160 GB")
+    torch.cuda.empty_cache()
+    codes, scales = (torch.empty(out, k // n, dtype=torch.uint8, device="cuda") for n in (2, 32))
+    packed = torch.empty(lib.efm_fp4_packed_bytes(k, out), dtype=torch.uint8, device="cuda")
+    tiles, of_tile = -(-out // 16), k * 8
+    rows = {t: slice(16 * t, min(16 * t + 16, out)) for t in (0, tiles // 2, tiles - 1)}
+    for t, at in rows.items():
+        half, byte = _weights_on_device(t, at.stop - at.start, k)
+        codes[at], scales[at] = half, byte
+        packed[t * of_tile:(t + 1) * of_tile] = 0xff
+    C.call("efm_fp4_pack", k, out, ptr(codes), ptr(scales), ptr(packed), stream())
+    torch.cuda.synchronize()
+    for t, at in rows.items():
+        alone, s0 = _pack(codes[at], scales[at]), tiles * of_tile + t * of_tile // 16
+        assert torch.equal(packed[t * of_tile:(t + 1) * of_tile], alone[:of_tile]), t
+        assert torch.equal(packed[s0:s0 + of_tile // 16], alone[of_tile:]), t
+    del codes, scales, packed
+    torch.cuda.empty_cache()
+
+
 def _linear(x, packed, k, out, bias=None, f32=False, fill_ws=0xff):
     m = x.shape[0]
     y = torch.full((m, out), math.nan, dtype=torch.float32 if f32 else torch.bfloat16, device="cuda")
