@@ -684,6 +684,11 @@ static int kv_fp4_attention(const char* who, const efm_attention_ctx* ctx, const
         return set_error(EFM_ERR_UNSUPPORTED, "%s: %u rows of %u query heads", who, S, ctx->num_qo_heads);
     const int hd = (int)ctx->head_dim;
     const KvFp4Plan p = kv_fp4_plan(ctx, S, bound, causal != 0);
+    const int64_t rows = (int64_t)S * (ctx->num_qo_heads / ctx->num_kv_heads), block = p.shared ? 128 : 16 * p.nq;
+    const int64_t groups = (rows + block - 1) / block * ctx->num_kv_heads;
+    const int threads = kWave * (p.shared ? 4 : p.nw);
+    if (groups * threads > kGridThreads)
+        return set_error(EFM_ERR_UNSUPPORTED, "%s: %u rows of %u query heads", who, S, ctx->num_qo_heads);
     if (p.total() > 0 && (workspace == nullptr || workspace_bytes < p.total()))
         return set_error(EFM_ERR_WORKSPACE, "%s: workspace of %zu bytes required", who, p.total());
     if (p.total() > 0 && (reinterpret_cast<uintptr_t>(workspace) & 15u) != 0)
@@ -706,21 +711,20 @@ static int kv_fp4_attention(const char* who, const efm_attention_ctx* ctx, const
     a.Hkv = (int)ctx->num_kv_heads;
     a.G = a.Hq / a.Hkv;
     a.causal = causal != 0;
-    a.rows = (int)S * a.G;
+    a.rows = (int)rows;
     a.split_tiles = p.split_tiles;
     a.splits = p.splits;
     a.tiles = (int)((bound + 31) / 32);
     a.cus = prefill_cus();
     a.scale = 1.4426950408889634f / sqrtf((float)hd);
-    const int block = p.shared ? 128 : 16 * p.nq;
-    const dim3 grid((unsigned)((a.rows + block - 1) / block * a.Hkv), 1, p.splits);
+    const dim3 grid((unsigned)groups, 1, p.splits);
     const int64_t all = (int64_t)a.Hkv * a.rows;
     auto launch = [&](auto hdc) {
         constexpr int HD = decltype(hdc)::value;
-        if (p.shared) hipLaunchKernelGGL(kv_fp4_rows_kernel, grid, dim3(256), 0, stream, a);
-        else if (p.nq == 2) hipLaunchKernelGGL((kv_fp4_attn_kernel<HD, 4, 2>), grid, dim3(256), 0, stream, a);
-        else if (p.nw == 4) hipLaunchKernelGGL((kv_fp4_attn_kernel<HD, 4, 1>), grid, dim3(256), 0, stream, a);
-        else hipLaunchKernelGGL((kv_fp4_attn_kernel<HD, 8, 1>), grid, dim3(512), 0, stream, a);
+        if (p.shared) hipLaunchKernelGGL(kv_fp4_rows_kernel, grid, dim3(threads), 0, stream, a);
+        else if (p.nq == 2) hipLaunchKernelGGL((kv_fp4_attn_kernel<HD, 4, 2>), grid, dim3(threads), 0, stream, a);
+        else if (p.nw == 4) hipLaunchKernelGGL((kv_fp4_attn_kernel<HD, 4, 1>), grid, dim3(threads), 0, stream, a);
+        else hipLaunchKernelGGL((kv_fp4_attn_kernel<HD, 8, 1>), grid, dim3(threads), 0, stream, a);
         if (p.splits > 1 && p.splits <= kWave && all >= 256)
             hipLaunchKernelGGL((kv_fp4_merge_kernel<HD, kWave>), dim3((unsigned)((all + 3) / 4)), dim3(256), 0, stream, a);
         else if (p.splits > 1)

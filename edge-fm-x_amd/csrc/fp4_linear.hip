@@ -631,7 +631,8 @@ static int w4_launch(const char* who, const W4Args& a, hipStream_t stream) {
     }
     const int pick = w4_pick(a, EPI == W4_SWIGLU, cus);
     const W4Tiles t = w4_tiles_of(kW4Forms[pick], a, EPI == W4_SWIGLU);
-    if (t.mt * t.nt > 0x7ffffff0) return set_error(EFM_ERR_UNSUPPORTED, "%s: too many tiles", who);
+    if ((t.mt * t.nt + 7) / 8 * 8 * (kWave * kW4Forms[pick].wn * kW4Forms[pick].kg) > kGridThreads)
+        return set_error(EFM_ERR_UNSUPPORTED, "%s: too many tiles", who);
     const dim3 grid((unsigned)((t.mt * t.nt + 7) / 8 * 8));
     auto go = [&](auto ic) {
         constexpr W4Form f = kW4Forms[decltype(ic)::value];

@@ -160,3 +160,10 @@ def test_every_operator_of_the_cache_takes_the_same_heads():
         assert call(most) == C.EFM_OK
     assert read(more) == UNSUP and write(more) == UNSUP
     assert C.load().efm_kv_fp4_bytes(most, 64) > 0 and C.load().efm_kv_fp4_bytes(more, 64) == 0
+
+
+def test_more_threads_than_a_grid_holds():
+    assert _rows(ctx=_ctx(512, 64, hd=64, rope=False), n=1 << 20, kv=1 << 20, room=1 << 20) == UNSUP
+    assert "rows of 512 query heads" in C.load().efm_last_error().decode()
+    assert _rc("efm_linear_fp4", 1 << 20, 32, 1 << 24, P, P, None, P, 2, None, 0, None) == UNSUP
+    assert "too many tiles" in C.load().efm_last_error().decode()
