@@ -22,7 +22,7 @@ namespace efm {
 int validate_attention_ctx(const efm_attention_ctx* c, const char* who);
 int prefill_cus();
 
-constexpr int kKvFp4MaxSplits = 512;
+constexpr int kKvFp4MaxSplits = 256;   // threads of a workgroup that joins them
 constexpr float kKvFp4Lazy = 8.f;
 
 struct KvFp4Args {
@@ -320,8 +320,8 @@ __global__ __launch_bounds__(NW * kWave, NQ == 1 ? (HD == 128 ? 3 : 4) : NQ == 2
 // splits: a wave each; a decode step's few rows have many: a workgroup each.
 template <int HD, int NT>
 __global__ __launch_bounds__(256) void kv_fp4_merge_kernel(KvFp4Args a) {
-    constexpr int C = HD / 4, P = NT / C, CH = 8, K = NT == 256 ? kKvFp4MaxSplits / 256 : 1, RW = 256 / NT;
-    __shared__ float wt[RW][K * NT], red_max[4], red_sum[4];
+    constexpr int C = HD / 4, P = NT / C, CH = 8, RW = 256 / NT;   // at most NT splits
+    __shared__ float wt[RW][NT], red_max[4], red_sum[4];
     __shared__ float4 part[RW][P][C];
     const int64_t all = (int64_t)a.Hkv * a.rows;
     const int rw = threadIdx.x / NT, tid = threadIdx.x % NT, c = tid % C, lane_p = tid / C;
@@ -336,30 +336,17 @@ __global__ __launch_bounds__(256) void kv_fp4_merge_kernel(KvFp4Args a) {
             x[k] = s0 + k * P < a.splits ? *reinterpret_cast<const float4*>(op + (int64_t)(s0 + k * P) * all * HD) : make_float4(0.f, 0.f, 0.f, 0.f);
     };
     request(lane_p);
-    float ms[K], ls[K], M = -INFINITY;
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-        const int s = k * NT + tid;
-        const float2 ml = s < a.splits ? *reinterpret_cast<const float2*>(a.ml_part + ((int64_t)s * all + rr) * 2) : make_float2(-INFINITY, 0.f);
-        ms[k] = ml.x, ls[k] = ml.y;
-        M = fmaxf(M, ml.x);
-    }
-    M = wave_max_uniform(M);
+    const float2 ml = tid < a.splits ? *reinterpret_cast<const float2*>(a.ml_part + ((int64_t)tid * all + rr) * 2) : make_float2(-INFINITY, 0.f);
+    float M = wave_max_uniform(ml.x);
     if constexpr (NT == 256) {
         if (tid % kWave == 0) red_max[tid / kWave] = M;
         __syncthreads();
         M = fmaxf(fmaxf(red_max[0], red_max[1]), fmaxf(red_max[2], red_max[3]));
     }
-    float den = 0.f;
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-        const int s = k * NT + tid;
-        const bool used = ls[k] != 0.f || ms[k] != -INFINITY;
-        const float f = M == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ms[k] - M);
-        if (s < a.splits) wt[rw][s] = used ? f : -1.f;
-        if (used) den += f * ls[k];
-    }
-    den = wave_total(den);
+    const bool used = ml.y != 0.f || ml.x != -INFINITY;
+    const float f = M == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ml.x - M);
+    if (tid < a.splits) wt[rw][tid] = used ? f : -1.f;
+    float den = wave_total(used ? f * ml.y : 0.f);
     if constexpr (NT == 256) {
         if (tid % kWave == 0) red_sum[tid / kWave] = den;
     }
@@ -370,9 +357,9 @@ __global__ __launch_bounds__(256) void kv_fp4_merge_kernel(KvFp4Args a) {
         if (s0 != lane_p) request(s0);
 #pragma unroll
         for (int k = 0; k < CH; ++k) {
-            const float f = s0 + k * P < a.splits ? wt[rw][s0 + k * P] : -1.f;
-            if (f < 0.f) continue;
-            t.x += f * x[k].x, t.y += f * x[k].y, t.z += f * x[k].z, t.w += f * x[k].w;
+            const float w = s0 + k * P < a.splits ? wt[rw][s0 + k * P] : -1.f;
+            if (w < 0.f) continue;
+            t.x += w * x[k].x, t.y += w * x[k].y, t.z += w * x[k].z, t.w += w * x[k].w;
         }
     }
     part[rw][lane_p][c] = t;
@@ -646,7 +633,6 @@ static KvFp4Plan kv_fp4_plan(const efm_attention_ctx* c, uint32_t S, uint32_t kv
     }
     const int64_t want = std::max<int64_t>(1, cus / blocks);   // one workgroup a CU where keys are split
     p.split_tiles = std::max({least, (int)((tiles + want - 1) / want), (tiles + kKvFp4MaxSplits - 1) / kKvFp4MaxSplits});
-    p.split_tiles += p.split_tiles % 2;   // whole stages
     p.splits = std::max(1, (tiles + p.split_tiles - 1) / p.split_tiles);
     if (p.splits > 1) {
         p.o_bytes = (size_t)p.splits * Hkv * rows * c->head_dim * sizeof(float);

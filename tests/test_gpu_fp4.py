@@ -654,6 +654,21 @@ def test_decode_long(gpu):
     _within(_decode(ctx, q.cuda(), cache, 65536, 0, d_len, 65536), ref, tol)
 
 
+@pytest.mark.parametrize("kv", [8161, 16400, 65536, 70001])
+def test_decode_of_one_kv_head(gpu, kv):
+    """Up to as many splits as a joining workgroup has threads, the last ones short or, by a smaller length on the device,
+    without keys."""
+    q, k, v = _qkv(kv, 1, kv, 7, 1, 128)
+    ctx = C.make_attention_ctx(7, 1, 128, rope=False)
+    cache = _fill(ctx, k, v, kv + 3)
+    ref, tol = R.attention(q.double(), R.rounded(k), R.rounded(v), False)
+    _within(_decode(ctx, q.cuda(), cache, kv + 3, kv), ref, tol)
+    n = kv // 3
+    d_len = torch.tensor([n], dtype=torch.int32, device="cuda")
+    ref, tol = R.attention(q.double(), R.rounded(k[:n]), R.rounded(v[:n]), False)
+    _within(_decode(ctx, q.cuda(), cache, kv + 3, 0, d_len, kv), ref, tol)
+
+
 def test_decode_length_beyond_the_bound(gpu):
     """*d_kv_len past max_kv_len attends max_kv_len rows."""
     q, k, v = _qkv(8, 1, 200, 12, 2, 128)
