@@ -622,6 +622,11 @@ static int w4_pick(const W4Args& a, bool swiglu, int cus) {
     return best;
 }
 
+// Steps of 64 columns that a wave of the form walks: groups of waves take whole blocks of two.
+static int w4_steps(const W4Form& f, int64_t K, int blocks) {
+    return f.kg > 1 ? 2 * ((blocks + f.kg - 1) / f.kg) : (int)((K + 63) / 64);
+}
+
 template <int EPI>
 static int w4_launch(const char* who, const W4Args& a, hipStream_t stream) {
     const int cus = prefill_cus();
@@ -709,6 +714,20 @@ extern "C" int efm_linear_fp4(int64_t m, int64_t in_features, int64_t out_featur
     const W4Args a{static_cast<const bf16_t*>(x), w4_weights(in_features, out_features, w_packed),
                    static_cast<const bf16_t*>(bias), y, m, out_features, in_features};
     return out_dtype == EFM_DTYPE_F32 ? w4_launch<W4_F32>("linear_fp4", a, stream) : w4_launch<W4_BF16>("linear_fp4", a, stream);
+}
+
+extern "C" int32_t efm_testing_fp4_linear_form(int64_t m, int64_t in_features, int64_t out_features, int32_t swiglu,
+                                               int32_t* forms, int32_t* steps) {
+    const bool s = swiglu != 0;
+    if (w4_check("testing_fp4_linear_form", in_features, s ? 2 * out_features : out_features) != EFM_OK || m <= kW4FewRows ||
+        forms == nullptr || steps == nullptr)
+        return -1;
+    const W4Args a{nullptr, w4_weights(in_features, s ? 2 * out_features : out_features, nullptr), nullptr, nullptr, m, out_features,
+                   in_features};
+    const int pick = w4_pick(a, s, prefill_cus());
+    *forms = (int32_t)std::count_if(kW4Forms, kW4Forms + kW4FormCount, [&](const W4Form& f) { return !s || f.tn % 2 == 0; });
+    *steps = w4_steps(kW4Forms[pick], in_features, a.w.blocks);
+    return pick;
 }
 
 extern "C" size_t efm_fused_gate_up_swiglu_fp4_workspace_bytes(int64_t m, int64_t hidden, int64_t inter) {

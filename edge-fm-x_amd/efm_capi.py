@@ -148,6 +148,7 @@ SIGNATURES = {
                                                  c_void_p, c_void_p, c_void_p]),
     "efm_decode_norm_lm_head_top1": (c_int32, [c_int32, c_int64, c_float, c_void_p, c_void_p, c_void_p, c_void_p,
                                                c_void_p, c_void_p, c_size_t, c_void_p]),
+    "efm_testing_fp4_linear_form": (c_int32, [c_int64, c_int64, c_int64, c_int32, POINTER(c_int32), POINTER(c_int32)]),
     "efm_fp4_packed_bytes": (c_size_t, [c_int64, c_int64]),
     "efm_fp4_quantize": (c_int32, [c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p]),
     "efm_fp4_pack": (c_int32, [c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p]),

@@ -94,6 +94,13 @@ int efm_init(void);
 #define EFM_KNOB_COUNT 6
 int efm_testing_set_kernel_path(int32_t knob, int32_t value);
 
+/* Test hook: which of its *forms kernels a call of efm_linear_fp4 (swiglu: of
+ * efm_fused_gate_up_swiglu_fp4 with inter = out_features) of five rows and more takes on the
+ * current device (without one: on 256 CUs), and how many steps of 64 columns a wave of it walks.
+ * -1: bad shape, or fewer rows. */
+int32_t efm_testing_fp4_linear_form(int64_t m, int64_t in_features, int64_t out_features, int32_t swiglu, int32_t* forms,
+                                    int32_t* steps);
+
 /* ------------------------------------------------------------------------------------
  * Attention.  Mirrors edge_fm::AttentionOpContext (src/operators/attention_op.h:20-39).
  * Strides are in elements; 0 means contiguous ([n, heads, head_dim] NHD layout).

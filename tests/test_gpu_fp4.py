@@ -9,6 +9,7 @@ import torch
 
 import _fp4_ref as R
 import efm_capi as C
+from _fp4_sizes import LINEAR_LONG, SWIGLU_LONG
 from _util import ptr, stream
 
 pytestmark = pytest.mark.gpu
@@ -242,6 +243,30 @@ def test_swiglu_every_shape(gpu, m, hidden, inter):
     du, dg = eu + HALF * (up.abs() + eu), eg + HALF * (gate.abs() + eg)
     tol = 1.1 * dg * (up.abs() + du) + silu.abs() * du   # |silu'| < 1.1
     _within(ys[0][:, at.cuda()], silu * up, tol + (HALF + 2.0 ** -20) * ((silu * up).abs() + tol), f"{m} {hidden} {inter}")
+    assert not ys[0].isnan().any() and torch.equal(*ys)
+
+
+@pytest.mark.parametrize("m,k,out", LINEAR_LONG)
+def test_linear_every_shape_over_long_k(gpu, m, k, out):
+    g = _gen(m + k + out)
+    half, byte = _weights_on_device(m + k, out, k)
+    packed, x = _pack(half, byte), _bf(g, m, k)
+    y, at = _linear(x.cuda(), packed, k, out, None, True), _columns(g, out).unique()
+    _within(y[:, at.cuda()], *_product(x.double(), _values_of(half, byte, at)), f"{m} x {k} -> {out}")
+    assert not y.isnan().any() and torch.equal(y, _linear(x.cuda(), packed, k, out, None, True))
+
+
+@pytest.mark.parametrize("m,hidden,inter", SWIGLU_LONG)
+def test_swiglu_every_shape_over_long_k(gpu, m, hidden, inter):
+    g = _gen(m + hidden + inter)
+    half, byte = _weights_on_device(m + hidden, 2 * inter, hidden)
+    packed, x = _pack(half, byte), _bf(g, m, hidden)
+    xd, at, ys = x.cuda(), _columns(g, inter).unique(), []
+    for _ in range(2):
+        ys.append(torch.full((m, inter), math.nan, dtype=torch.bfloat16, device="cuda"))
+        C.call("efm_fused_gate_up_swiglu_fp4", m, hidden, inter, ptr(xd), ptr(packed), ptr(ys[-1]), None, 0, stream())
+    torch.cuda.synchronize()
+    _within(ys[0][:, at.cuda()], *_swiglu(x, _values_of(half, byte, torch.cat([at, at + inter]))), f"{m} {hidden} {inter}")
     assert not ys[0].isnan().any() and torch.equal(*ys)
 
 
