@@ -920,6 +920,37 @@ def test_layer_step_and_prompt(gpu):
         check_linear(_linear(mid, packed["down"], inter, hidden), mid, "down")
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("n", [1, 3, 1100])
+def test_queries_at_a_device_length_and_the_activation(gpu, n, hd):
+    """Queries of rows that end at the device's length, and what the down projection is given, against 64 bits: the outputs
+    of a layer that its attention and its down projection take as they are."""
+    g = _gen(n + hd)
+    hidden, hq, hkv, inter, room, length = 512, 8, 2, 1024, 1400, 1331
+    width = (hq + 2 * hkv) * hd
+    code, byte = _weights(g, 2 * inter, hidden)
+    qkv, x, qw, kw = _bf(g, n, width), _bf(g, n, hidden), 1 + _bf(g, hd, std=0.2), 1 + _bf(g, hd, std=0.2)
+    ctx = C.make_attention_ctx(hq, hkv, hd)
+    d_len = torch.tensor([length], dtype=torch.int32, device="cuda")
+    pos = _positions(length - n, n, hd // 2)
+    heads = qkv.double().view(n, -1, hd)
+    ref = R.norm_rope(heads[:, :hq], qw, 1e-6, pos, 1e6)
+    tol = _y_tol(ref, heads[:, :hq], qw, 1e-6)
+    dev = [t.cuda() for t in (qkv, qw, kw)]
+    for fp4 in (True, False):
+        dst = [_buf(C.load().efm_kv_fp4_bytes(ctx, room))] if fp4 else \
+            [torch.zeros(room, hkv, hd, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+        q = torch.full((n, hq, hd), math.nan, dtype=torch.bfloat16, device="cuda")
+        _write(ctx, fp4, *dev, q, dst, room, n, 0, d_len=d_len)
+        torch.cuda.synchronize()
+        _within(q, ref, tol, "queries")
+    packed, xd = _pack(R.halves(code), byte), x.cuda()
+    mid = torch.full((n, inter), math.nan, dtype=torch.bfloat16, device="cuda")
+    C.call("efm_fused_gate_up_swiglu_fp4", n, hidden, inter, ptr(xd), ptr(packed), ptr(mid), None, 0, stream())
+    torch.cuda.synchronize()
+    _within(mid, *_swiglu(x, R.values(code, byte)), "activation")
+
+
 def test_same_stream_order_on_a_side_stream(gpu):
     """Write, read and attention queued on a side stream follow each other without host waits."""
     hq, hkv, hd, kv = 12, 2, 128, 400
