@@ -23,6 +23,7 @@
 namespace efm {
 
 int validate_attention_ctx(const efm_attention_ctx* c, const char* who);
+int prefill_cus();
 
 struct QkWriteArgs {
     const bf16_t* qkv;       // [S, qkv_sn]: q at 0, k at Hq*hd, v at (Hq+Hkv)*hd
@@ -308,18 +309,19 @@ static int qk_write(const char* who, bool fp4, const efm_attention_ctx* ctx, con
         const double l = log((double)ctx->rope_theta), scale = ctx->rope_scale;
         for (int d = 0; d < hd / 2; ++d) a.turns[d] = exp(-2.0 * d / (double)hd * l) / scale / 6.283185307179586476925;
     }
-    // A token a workgroup spreads few tokens over the chip; once its waves would fill the chip (16 a CU
-    // by the FP4 kernel's registers, 24 by the bf16 one's), tokens together do less apiece. Measured (us,
-    // one / together): 28/4 heads of 128, FP4: 64 tokens 4.5 / 5.7, 512 7.4 / 6.6, 1024 13.1 / 8.0, 4096
-    // 37 / 16; bf16: 64 3.4 / 4.6, 512 4.6 / 5.2, 1024 9.1 / 6.6, 4096 25.2 / 14.4. 14/2 heads of 64, 2000
-    // tokens: FP4 8.6 / 5.6, bf16 5.4 / 4.7.
+    // A token a workgroup spreads few tokens over the chip; from ten of its waves a CU on (bf16: 24), tokens
+    // together do less apiece. Measured (us, one / together; FP4 with the rows read back, 2 to 2.5 of it):
+    // 28/4 heads of 128, FP4: 64 tokens 6.3 / 7.4, 256 6.8 / 7.7, 284 8.2 / 7.7, 512 9.0 / 8.1, 1024 14.4 /
+    // 9.9; bf16: 64 3.4 / 4.6, 512 4.6 / 5.2, 682 6.2 / 5.7, 1024 9.2 / 6.6, 4096 25.8 / 14.5. 12/2 heads, FP4:
+    // 500 tokens 6.8 / 6.8, 1024 7.7 / 7.3; bf16: 1300 5.1 / 5.4, 1536 5.5 / 5.7, 2000 7.2 / 6.3. 14/2 heads of
+    // 64, FP4: 700 tokens 6.8 / 6.8, 2000 10.2 / 7.4; bf16: 1500 4.9 / 4.5, 2000 5.4 / 4.7, 2500 7.0 / 5.8.
     // Eight waves for tokens together: 4096 of 28/4 heads into a bf16 cache 14.5, with six 15.5, twelve 16.1;
     // 1344 of 16/2 heads 6.0, with five 6.4, ten 6.2.
     auto launch = [&](auto hdc, auto fc) {
         constexpr int HD = decltype(hdc)::value, ROWS = kWave * 8 / HD;
         constexpr bool F = decltype(fc)::value;
         const int64_t heads = (q_out ? Hq : 0) + 2 * Hkv, waves = std::min<int64_t>(16, (heads + ROWS - 1) / ROWS);
-        if (seq_len * waves >= (F ? 4096 : 6144))
+        if (seq_len * waves >= (F ? 10 : 24) * (int64_t)prefill_cus())
             hipLaunchKernelGGL((qk_norm_rope_write_kernel<HD, F, true>), dim3((seq_len + ROWS - 1) / ROWS),
                                dim3(kWave * (unsigned)std::min<int64_t>(8, heads)), 0, stream, a);
         else
