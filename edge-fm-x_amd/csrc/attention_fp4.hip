@@ -606,21 +606,23 @@ struct KvFp4Plan {
 // Measured on 256 CUs (us). One row: 200 keys of 14/2 heads 3.8 in one workgroup a head, 6.3 split; 500
 // keys of 12/2 heads 5.4 and 6.6; 700 keys of 12/2 heads 6.8 and 6.6, of 14/2 heads of 64 5.5 and 6.3; 2000
 // keys of 28/4 heads 7.2 in workgroups of four waves, 7.4 of eight; 32771 keys 11.9 with up to 512
-// workgroups, 10.9 with 256. Rows, kv_fp4_attn_kernel with 16 and with 32 rows a workgroup and
-// kv_fp4_rows_kernel: 37 rows behind 8000 of 12/2 heads 13 / 16 / 20, 512 behind 512 of 28/4 heads 22 / 17 /
-// 29, 1500 behind 2000 - / 89 / 99, 2048 alone - / 55 / 54, 2048 behind 2048 - / 127 / 113, 2500 alone - / 73 /
-// 70, 2500 behind 2500 - / 174 / 162, 3000 - / 96 / 85, 4096 - / 161 / 120; of 12/2 heads 5000 - / 103 / 126, 6000
-// - / 142 / 153, 6000 behind 6000 - / 390 / 374, 7000 - / 188 / 188, 10000 - / 364 / 283.
+// workgroups, 10.9 with 256. Rows, kv_fp4_attn_kernel with 16 and with 32 rows a workgroup: 37 rows behind 8000 of
+// 12/2 heads 13 / 16, 512 behind 512 of 28/4 heads 22 / 17. kv_fp4_attn_kernel with 32 and kv_fp4_rows_kernel, by the
+// latter's workgroups: behind as many rows, 28/4 heads, 372 of them 87 / 95, 396 101 / 100, 416 107 / 105, 448
+// 117 / 104, 484 138 / 120, and behind 8000 416 303 / 272; 16/2 heads 376 140 / 159, 414 172 / 176, 448 190 / 176; 12/2
+// heads 404 217 / 226, 442 244 / 246, 516 346 / 323. Alone, 28/4 heads, 448 51 / 52, 484 58 / 60, 548 70.7 / 69.2,
+// 640 92 / 83; 12/2 heads 564 142 / 152, 640 178 / 181; 10000 rows of them 364 / 283. 13/8 of the CUs
+// lies between the head layouts' borders: 396 workgroups of 28/4 heads behind 4000 keys take 172 instead of 160.
 static KvFp4Plan kv_fp4_plan(const efm_attention_ctx* c, uint32_t S, uint32_t kv_len, bool causal) {
     const int64_t Hkv = c->num_kv_heads, rows = (int64_t)S * (c->num_qo_heads / Hkv), cus = prefill_cus();
     const int tiles = (int)(((int64_t)kv_len + 31) / 32);
     auto blocks_of = [&](int n) { return (rows + n - 1) / n * Hkv; };
     KvFp4Plan p = {};
-    // The shared kernel's 128-row workgroups pay where they fill the CUs' places (two each) and more, or
+    // The shared kernel's 128-row workgroups pay where they fill the CUs' places (two each) and more, or nearly
     // fill them and differ little in their keys.
     const int64_t shared = blocks_of(128);
     p.shared = c->head_dim == 128 && S > 1 &&
-               (2 * shared >= 5 * cus || (4 * shared >= 7 * cus && (!causal || kv_len >= S + S / 2)));
+               (2 * shared >= 5 * cus || (8 * shared >= 13 * cus && (!causal || kv_len >= S + S / 2)));
     p.nq = blocks_of(16) >= 2 * cus ? 2 : 1;
     p.nw = p.nq == 2 ? 4 : 8;
     const int64_t blocks = p.shared ? shared : blocks_of(16 * p.nq);
