@@ -40,7 +40,7 @@ struct QkWriteArgs {
     int64_t pos_stride;
     uint32_t max_rows, S, base;
     int Hq, Hkv, rotate, cum0, cum1;
-    uint32_t q_off, k_off;
+    int q_off, k_off;   // as in the other operators: 2^31 and more are below zero
     float eps;
     double turns[kMaxHalfDim];   // theta^(-2 d / hd) / rope_scale / (2 pi)
 };
@@ -302,8 +302,8 @@ static int qk_write(const char* who, bool fp4, const efm_attention_ctx* ctx, con
     a.rotate = rotate;
     a.cum0 = s0;
     a.cum1 = s0 + s1;
-    a.q_off = ctx->q_rope_pos_offset;
-    a.k_off = ctx->k_rope_pos_offset;
+    a.q_off = (int)ctx->q_rope_pos_offset;
+    a.k_off = (int)ctx->k_rope_pos_offset;
     a.eps = eps;
     if (rotate) {
         const double l = log((double)ctx->rope_theta), scale = ctx->rope_scale;

@@ -534,7 +534,7 @@ int efm_fused_gate_up_swiglu_fp4(int64_t m, int64_t hidden, int64_t inter, const
  * seq_len - 1 (strides ctx->k_stride_* and ctx->kv_stride_*), base = *d_kv_len - seq_len when
  * d_kv_len is not NULL (device-resident, graph-stable; a length outside [seq_len, max_rows]
  * writes nothing, q_out included). The token's position is its cache row plus
- * ctx->q_rope_pos_offset (keys: k_rope_pos_offset), or with position_ids
+ * ctx->q_rope_pos_offset (keys: k_rope_pos_offset; 2^32 - n shifts back by n), or with position_ids
  * [3, position_stride] (M-RoPE; sections sum to hd/2) the id of the pair's section.
  * Rows behind the last one written are left as they are. Stands beside
  * efm_prefill_rope_write_kv for models that normalise queries and keys. */

@@ -486,6 +486,29 @@ def test_write_mrope_offsets_strides_and_in_place(gpu, fp4, S):
             assert torch.equal(kv[base:base + S, :, 1].cpu(), qkv.view(S, -1, hd)[:, hq + hkv:])
 
 
+@pytest.mark.parametrize("S", [3, 1500])
+@pytest.mark.parametrize("fp4", [False, True])
+def test_write_at_offsets_below_zero(gpu, fp4, S):
+    """Positions that lie before the cache rows, the first of them below zero."""
+    g = _gen(S)
+    hq, hkv, hd, base = 12, 2, 128, 40
+    qkv, w = _bf(g, S, (hq + 2 * hkv) * hd), 1 + _bf(g, hd, std=0.2)
+    x, room = qkv.double().view(S, -1, hd), base + S
+    ctx = C.make_attention_ctx(hq, hkv, hd, q_rope_pos_offset=2 ** 32 - 41, k_rope_pos_offset=2 ** 32 - 7)
+    q = torch.empty(S, hq, hd, dtype=torch.bfloat16, device="cuda")
+    dst = [_buf(C.load().efm_kv_fp4_bytes(ctx, room))] if fp4 else \
+        [torch.empty(room, hkv, hd, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    _write(ctx, fp4, qkv.cuda(), w.cuda(), w.cuda(), q, dst, room, S, base)
+    torch.cuda.synchronize()
+    ref = R.norm_rope(x[:, :hq], w, 1e-6, _positions(base, S, 64, -41), 1e6)
+    _within(q, ref, _y_tol(ref, x[:, :hq], w, 1e-6), "queries")
+    k = R.norm_rope(x[:, hq:hq + hkv], w, 1e-6, _positions(base, S, 64, -7), 1e6)
+    if fp4:
+        assert torch.equal(_read(ctx, dst[0], room, base, S, hkv, hd)[0], R.rounded(k))
+    else:
+        _within(dst[0][base:], k, _y_tol(k, x[:, hq:hq + hkv], w, 1e-6), "keys")
+
+
 @pytest.mark.parametrize("fp4", [False, True])
 @pytest.mark.parametrize("length", [0, 2, 3, 50, 64, 65])
 def test_write_at_a_device_length(gpu, fp4, length):
