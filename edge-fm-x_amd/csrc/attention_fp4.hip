@@ -6,7 +6,9 @@
 // with the keys as the first operand. A lane then holds, for one row, 8 consecutive keys of a
 // 32-key tile (the keys of the two 16-key operands are interleaved so), which is what the second
 // product O^T = V^T P^T takes from it as its second operand: P never moves between lanes. The
-// codes become bf16 in registers, exactly.
+// codes become bf16 in registers, exactly. P is rounded to bf16 there, the type of the matrix cores'
+// products (a relative 2^-9 a weight: outputs move by 0.0013 to 0.0016 of their size before their own
+// rounding to bf16, which moves them by 0.0017); maxima, sums and outputs stay in fp32, the sums over P unrounded.
 // A workgroup's waves take every NW-th tile of its split of the keys, each with the running
 // maximum and sum of its own softmax; their outputs meet in LDS (many rows: a kernel of its own,
 // below). Where the keys are split over workgroups too, those write unnormalised outputs with
@@ -382,7 +384,7 @@ __global__ __launch_bounds__(256) void kv_fp4_merge_kernel(KvFp4Args a) {
 // instructions alternate: unpacking goes out between the first products, the second tile's exponentials
 // between the first tile's second products, and a wave at its products goes before the other on its SIMD,
 // which so falls to its softmax (4096 rows of 28/4 heads: 150 us one after the other, 143 alternating, 122 with
-// the priority). 4096 rows 990 TFLOP/s, 8192 rows 1110; fewer rows are bound by workgroups that see more
+// the priority). 4096 rows 970 TFLOP/s, 8192 rows 1090; fewer rows are bound by workgroups that see more
 // keys than others.
 // Heads of 128; the keys are not split, since there are rows enough.
 __global__ __launch_bounds__(256, 2) void kv_fp4_rows_kernel(KvFp4Args a) {

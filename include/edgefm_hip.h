@@ -510,7 +510,8 @@ int efm_fp4_pack(int64_t in_features, int64_t out_features, const uint8_t* codes
 
 /* efm_linear with packed FP4 weights: y[m, out] = x[m, in] . W^T (+ bias[out]), x and bias
  * bf16, fp32 accumulate, y bf16 or fp32. Any m; few rows are bound by the weights' bytes, a
- * quarter of bf16's. workspace: efm_linear_fp4_workspace_bytes (0: none is used), no initial
+ * quarter of bf16's. x and w_packed must be 16-byte aligned, here and below.
+ * workspace: efm_linear_fp4_workspace_bytes (0: none is used), no initial
  * contents required; calls that share one must be stream-ordered. Deterministic. */
 size_t efm_linear_fp4_workspace_bytes(int64_t m, int64_t in_features, int64_t out_features);
 int efm_linear_fp4(int64_t m, int64_t in_features, int64_t out_features, const void* x, const void* w_packed,
