@@ -855,6 +855,28 @@ def test_nan_groups_reach_the_rows_that_see_them(gpu, hd, n, kv):
             _within(_decode(ctx, q.cuda(), _fill(ctx, kk, vv, kv + 9), kv + 9, kv), ref, tol, what + ", decode")
 
 
+@pytest.mark.parametrize("hq,hkv,hd", [(12, 2, 128), (14, 2, 64), (320, 320, 128)])
+@pytest.mark.parametrize("n,kv", [(1, 700), (40, 300), (130, 333)])
+def test_queries_that_are_not_finite(gpu, hq, hkv, hd, n, kv):
+    """A NaN or an infinity in a query makes NaN of its own row and head alone."""
+    q, k, v = _qkv(n, n, kv, hq, hkv, hd)
+    heads = torch.tensor([0, 1, hq // 2, hq - 1])
+    ctx = C.make_attention_ctx(hq, hkv, hd, rope=False)
+    kvh = heads // (hq // hkv)
+    ref, tol = R.attention(q[:, heads].double(), R.rounded(k[:, kvh]), R.rounded(v[:, kvh]), True)
+    for bad in (math.nan, math.inf):
+        x = q.clone()
+        x[n // 2, 1, 7] = bad
+        want = ref.clone()
+        want[n // 2, 1] = math.nan
+        cache = _fill(ctx, k, v, kv)
+        o = _rows(ctx, x.cuda(), cache, kv, n, kv)
+        _within(o[:, heads.cuda()], want, tol, str(bad))
+        assert int(o.isnan().sum()) == hd
+        if n == 1:
+            assert torch.equal(_decode(ctx, x.cuda(), cache, kv, kv).isnan(), o.isnan())
+
+
 @pytest.mark.parametrize("n", [1, 50, 600])
 def test_large_scores(gpu, n):
     """Scores of thousands: one key takes all the weight, whichever wave or split holds it."""
