@@ -36,6 +36,8 @@ EFM_LAYOUT_UP_GATE = 1
 
 EFM_ATTENTION_DECODE_NOALLOC_SCRATCH_BYTES = 2359296
 
+EFM_DRAFT_TREE_MAX_NODES = 1024
+
 EFM_KNOB_DECODE_REGISTER = 0
 EFM_KNOB_PREFILL_REGISTER = 1
 EFM_KNOB_PREFILL_SHAPE = 2
@@ -173,6 +175,18 @@ SIGNATURES = {
     "efm_attention_prefill_kv_fp4_workspace_bytes": (c_size_t, [POINTER(AttentionCtx), c_uint32, c_uint32]),
     "efm_attention_prefill_kv_fp4": (c_int32, [POINTER(AttentionCtx), c_void_p, c_void_p, c_uint32, c_void_p, c_uint32,
                                                c_uint32, c_int32, c_void_p, c_size_t, c_void_p]),
+    "efm_draft_tree_plan": (c_int32, [c_uint32, c_void_p, c_uint32, c_void_p, c_int32, c_void_p, c_void_p, c_int32,
+                                      c_void_p]),
+    "efm_attention_tree_workspace_bytes": (c_size_t, [POINTER(AttentionCtx), c_uint32, c_uint32]),
+    "efm_attention_tree": (c_int32, [POINTER(AttentionCtx), c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_uint32,
+                                     c_uint32, c_void_p, c_uint32, c_void_p, c_size_t, c_void_p]),
+    "efm_sampler_filtered_workspace_bytes": (c_size_t, [c_int64, c_int64]),
+    "efm_sampler_filtered": (c_int32, [c_int64, c_int64, c_void_p, c_int32, c_int64, c_float, c_int32, c_float, c_float,
+                                       c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "efm_draft_tree_accept": (c_int32, [c_uint32, c_void_p, c_void_p, c_void_p, c_void_p, c_uint32, c_void_p, c_void_p,
+                                        c_void_p, c_void_p]),
+    "efm_draft_tree_move_kv": (c_int32, [POINTER(AttentionCtx), c_uint32, c_int64, c_void_p, c_void_p, c_uint32,
+                                         c_uint32, c_void_p, c_void_p]),
 }
 
 

@@ -585,6 +585,89 @@ int efm_attention_prefill_kv_fp4(const efm_attention_ctx* ctx, const void* q, co
                                  void* o, uint32_t qo_len, uint32_t kv_len, int32_t causal, void* workspace,
                                  size_t workspace_bytes, hipStream_t stream);
 
+/* ------------------------------------------------------------------------------------
+ * Speculative decoding: one step that checks a tree of drafted tokens. No counterpart in the
+ * reference, whose decode step takes one token.
+ *
+ * A step of n nodes over a cache of c rows: efm_draft_tree_plan (once); in every layer
+ * efm_qk_norm_rope_write_kv with the planned positions puts the nodes' rows into cache rows c ..
+ * c + n - 1, and efm_attention_tree attends; efm_sampler_filtered (or efm_sampler_greedy) draws a
+ * token from each node's logits; efm_draft_tree_accept walks from node 0 down the nodes whose
+ * tokens were drawn, and efm_draft_tree_move_kv puts their rows together. The accepted tokens are
+ * distributed as if they had been drawn one by one. Lengths stay on the device, and every call can
+ * be captured.
+ *
+ * The tree: parents[i] is the node before node i, -1 for a root, and parents[i] < i. Node 0 is the
+ * last token of the text, whose row the cache does not hold yet. A node whose parent is neither -1
+ * nor an earlier node is unused (padding), and so are its descendants. d_kv_len counts cache rows
+ * with the nodes' among them, as in efm_qk_norm_rope_write_kv.
+ * ---------------------------------------------------------------------------------- */
+#define EFM_DRAFT_TREE_MAX_NODES 1024
+
+/* Ancestor masks and positions. mask [nodes, ceil(nodes / 64)] 64-bit words: bit j of row i is set
+ * where node j is node i or one of its ancestors; an unused node's row is empty. positions
+ * [3, position_stride]: three equal rows (for M-RoPE) of kv_len - nodes + depth + pos_offset, depth 0
+ * for roots and unused nodes. Either output may be NULL. The rows are *d_kv_len when d_kv_len is
+ * not NULL (below nodes: every node is unused, at position pos_offset), else kv_len >= nodes. */
+int efm_draft_tree_plan(uint32_t nodes, const int32_t* parents, uint32_t kv_len, const uint32_t* d_kv_len,
+                        int32_t pos_offset, uint64_t* mask, int32_t* positions, int32_t position_stride,
+                        hipStream_t stream);
+
+/* Attention of the nodes: q [nodes, Hq, hd] (ctx->q_stride_*), k, v the cache, whose first L rows
+ * (L = *d_kv_len when d_kv_len is not NULL, else kv_len) end with the nodes' own; o [nodes, Hq * hd]
+ * contiguous. Node i sees rows j < L - nodes, and row L - nodes + c where bit c of its row of mask
+ * (as efm_draft_tree_plan lays it out; any bits may be set, those past the nodes are not looked at)
+ * is set. fp32 softmax, P rounded to bf16 for the PV product, sm_scale = 1/sqrt(hd); a node that
+ * sees no row gets zeros. Keys and values that a node does not see take no part in its output,
+ * whatever they hold; a value seen that is not finite leaves its channel not finite. pos_encoding
+ * must be EFM_POS_NONE: the cache holds keys as they are multiplied. A device length outside
+ * [nodes, max_kv_len] gives zeros. workspace: efm_attention_tree_workspace_bytes(ctx, nodes,
+ * max_kv_len or kv_len) bytes (0: none), which every call with no more nodes and rows fits in,
+ * 16-byte aligned, no initial contents required; calls that share one must be stream-ordered. Up to
+ * EFM_DRAFT_TREE_MAX_NODES nodes. Stands beside efm_attention_decode and efm_attention_prefill. */
+size_t efm_attention_tree_workspace_bytes(const efm_attention_ctx* ctx, uint32_t nodes, uint32_t max_kv_len);
+int efm_attention_tree(const efm_attention_ctx* ctx, const void* q, const void* k, const void* v, const uint64_t* mask,
+                       void* o, uint32_t nodes, uint32_t kv_len, const uint32_t* d_kv_len, uint32_t max_kv_len,
+                       void* workspace, size_t workspace_bytes, hipStream_t stream);
+
+/* A token for each row of logits (fp32 or bf16, EFM_DTYPE_*; rows logits_stride elements apart, 0:
+ * vocab), from the row's random number u in [0, 1): m = max l (a NaN counts as -inf),
+ * w_i = rint(2^44 exp((l_i - m) / T)) in 64 bits; K = the first top_k ids in the order of logits
+ * (largest first, of equal ones the lowest id; all when top_k <= 0), of these the ones with
+ * w_i >= min_p 2^44; N = K's ids in that order up to the first at which their mass reaches
+ * max(1, ceil(top_p W)), W the mass of K (all of K when top_p >= 1); the token is the smallest id
+ * of N whose inclusive mass, in the order of ids, exceeds floor(u M), M the mass of N. A row
+ * without mass (all -inf or NaN) gives -1. u outside [0, 1) or NaN is taken as the nearest end (0).
+ * temperature >= 1e-6 (smaller means greedy: use efm_sampler_greedy), top_p > 0, min_p <= 1 (not
+ * above 0: off), 1 <= vocab < 2^20. The same inputs give the same token, whatever the other rows
+ * are. workspace: efm_sampler_filtered_workspace_bytes(rows, vocab) bytes (0: none), 16-byte
+ * aligned, no initial contents required; calls that share one must be stream-ordered. Stands beside
+ * efm_sampler_top_p, which draws its own random number for one row. */
+size_t efm_sampler_filtered_workspace_bytes(int64_t rows, int64_t vocab);
+int efm_sampler_filtered(int64_t rows, int64_t vocab, const void* logits, int32_t logits_dtype, int64_t logits_stride,
+                         float temperature, int32_t top_k, float top_p, float min_p, const float* uniforms,
+                         int32_t* token_out, void* workspace, size_t workspace_bytes, hipStream_t stream);
+
+/* The walk: from node 0, the child of lowest index whose draft_tokens entry equals the node's
+ * target_tokens entry is accepted, and so on; tokens below 0 match nothing. With c rows before the
+ * tree (c = *d_kv_len - nodes) and a nodes accepted (node 0 among them, a >= 1): commit
+ * [nodes + 2] = {c, a, the a nodes, -1 ...}; tokens_out [nodes] (may be NULL) = target_tokens of those
+ * nodes, then -1: the a tokens that the step emits, the last of which is the next step's node 0;
+ * *d_kv_len_out (may be d_kv_len) = c + a + next_nodes, next_nodes the size of the next step's tree
+ * (0: the rows of the text so far). *d_kv_len below nodes: nothing is accepted (commit {0, 0, -1
+ * ...}) and *d_kv_len_out = *d_kv_len. Stands beside efm_finalize_decode_token_indexed. */
+int efm_draft_tree_accept(uint32_t nodes, const int32_t* parents, const int32_t* draft_tokens,
+                          const int32_t* target_tokens, const uint32_t* d_kv_len, uint32_t next_nodes,
+                          uint32_t* d_kv_len_out, int32_t* commit, int32_t* tokens_out, hipStream_t stream);
+
+/* Moves cache rows commit[0] + path[i] to commit[0] + i, path = commit[2 .. 2 + commit[1]), of K and V of
+ * `layers` layers, layer_stride elements apart (multiple of 8), with the head layout and strides
+ * of ctx (k_stride_*, kv_stride_*). path must rise; where it does not, or leaves the tree, the move
+ * ends. All other rows are left as they are; commit[0] + nodes past max_rows moves nothing. Stands
+ * beside efm_copy_decode_kv_cache_slots. */
+int efm_draft_tree_move_kv(const efm_attention_ctx* ctx, uint32_t layers, int64_t layer_stride, void* k_cache, void* v_cache,
+                           uint32_t max_rows, uint32_t nodes, const int32_t* commit, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,559 @@
+"""GPU tests of a speculative decoding step's operators against plain 64-bit forms (_draft_tree_ref).
+
+Tolerances of the attention are derived there; everything else has to be equal."""
+import math
+
+import pytest
+import torch
+
+import _draft_tree_ref as R
+import efm_capi as C
+from _util import ptr, stream
+
+pytestmark = pytest.mark.gpu
+
+HEADS = [pytest.param(14, 2, 64, id="0p5b"), pytest.param(12, 2, 128, id="1p5b"), pytest.param(28, 4, 128, id="7b")]
+
+
+def _gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def _bf(g, *size, std=1.0):
+    return (torch.randn(*size, generator=g) * std).to(torch.bfloat16)
+
+
+def _i32(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+def _buf(nbytes, fill=0xff):
+    return torch.full((max(int(nbytes), 256),), fill, dtype=torch.uint8, device="cuda")
+
+
+# ---------------------------------------------------------------- plan
+
+def _plan(parents, rows, device_len=True, off=0, stride=None, want=(True, True)):
+    n = len(parents)
+    stride = stride or n
+    par, d = _i32(parents), _i32([rows])
+    mask = torch.full((n, -(-n // 64)), 0x5a, dtype=torch.int64, device="cuda")
+    pos = torch.full((3, stride), -7, dtype=torch.int32, device="cuda")
+    C.call("efm_draft_tree_plan", n, ptr(par), 0 if device_len else rows, ptr(d) if device_len else None, off,
+           ptr(mask) if want[0] else None, ptr(pos) if want[1] else None, stride, stream())
+    torch.cuda.synchronize()
+    return mask.cpu(), pos.cpu()
+
+
+def _check_plan(parents, rows, off=0, **kw):
+    n = len(parents)
+    mask, pos = _plan(parents, rows, off=off, **kw)
+    assert torch.equal(mask, R.words(R.bits(parents)))
+    want = torch.tensor([rows - n + max(len(x) - 1, 0) + off for x in R.lines(parents)], dtype=torch.int32)
+    assert torch.equal(pos[:, :n], want.expand(3, -1))
+    assert (pos[:, n:] == -7).all()
+
+
+@pytest.mark.parametrize("n", [1, 2, 3, 63, 64, 65, 127, 128, 500, 1000, 1024])
+@pytest.mark.parametrize("shape", ["chain", "star", "random", "near", "forest"])
+def test_plan(gpu, n, shape):
+    g = _gen(n)
+    parents = dict(chain=list(range(-1, n - 1)), star=[-1] + [0] * (n - 1), random=R.random_tree(n, g),
+                   near=R.random_tree(n, g, reach=3), forest=R.random_tree(n, g, roots=min(n, 5)))[shape]
+    _check_plan(parents, 3000 + n, off=-17)
+
+
+@pytest.mark.parametrize("device_len", [False, True])
+def test_plan_unused_nodes(gpu, device_len):
+    """Parents that are neither -1 nor earlier nodes, and their descendants; rows right at the nodes' number."""
+    parents = [-1, 0, -2, 2, 3, 5, 9, 1, 2 ** 31 - 1, -2 ** 31, 9, 7, 8, 3]
+    _check_plan(parents, len(parents), device_len=device_len, stride=20)
+    chain = [-5] + list(range(700))
+    _check_plan(chain, 5000, device_len=device_len)
+
+
+def test_plan_single_outputs_and_short_lengths(gpu):
+    parents = [-1, 0, 0, 1]
+    mask, pos = _plan(parents, 104, want=(True, False))
+    assert torch.equal(mask, R.words(R.bits(parents))) and (pos == -7).all()
+    mask, pos = _plan(parents, 104, want=(False, True))
+    assert (mask == 0x5a).all() and pos[0].tolist() == [100, 101, 101, 102]
+    mask, pos = _plan(parents, 3, off=11)   # fewer rows than nodes: every node is unused
+    assert (mask == 0).all() and (pos == 11).all()
+
+
+# ---------------------------------------------------------------- attention
+
+class _Attn:
+    """Inputs of a call, on the host; `call` runs it with the layout asked for."""
+
+    def __init__(self, g, hq, hkv, hd, n, prefix, mask=None):
+        self.hq, self.hkv, self.hd, self.n, self.rows = hq, hkv, hd, n, prefix + n
+        self.q, self.k, self.v = _bf(g, n, hq, hd), _bf(g, self.rows, hkv, hd), _bf(g, self.rows, hkv, hd)
+        self.k[..., 3] *= 5
+        self.mask = mask if mask is not None else R.bits(R.random_tree(n, g))
+
+    def ref(self):
+        return R.attention(self.q.double().cuda(), self.k.double().cuda(), self.v.double().cuda(), self.mask)
+
+    def call(self, device_len=True, bound=None, ws=None, words=None):
+        n, hq, hkv, hd = self.n, self.hq, self.hkv, self.hd
+        bound = bound or (self.rows + 50 if device_len else self.rows)
+        c = C.make_attention_ctx(hq, hkv, hd, rope=False)
+        k = torch.full((bound, hkv, hd), math.nan, dtype=torch.bfloat16, device="cuda")   # rows past the end: NaN
+        v = torch.full_like(k, math.nan)
+        k[:self.rows], v[:self.rows] = self.k.cuda(), self.v.cuda()
+        q, mask, d = self.q.cuda(), (R.words(self.mask) if words is None else words).cuda(), _i32([self.rows])
+        o = torch.full((n + 1, hq * hd), 7.0, dtype=torch.bfloat16, device="cuda")
+        size = C.load().efm_attention_tree_workspace_bytes(c, n, bound)
+        ws = _buf(size) if ws is None else ws
+        C.call("efm_attention_tree", c, ptr(q), ptr(k), ptr(v), ptr(mask), ptr(o), n, 0 if device_len else self.rows,
+               ptr(d) if device_len else None, bound if device_len else 0, ptr(ws), ws.numel(), stream())
+        torch.cuda.synchronize()
+        assert (o[n] == 7).all()   # the row behind the last is left as it was
+        return o[:n].view(n, hq, hd)
+
+
+def _close(got, ref, tol, what=""):
+    got, ref, tol = got.double().cpu(), ref.cpu(), tol.cpu()
+    assert torch.equal(torch.isfinite(got), torch.isfinite(ref)), f"{what}: not finite in other places"
+    ok = torch.isfinite(ref)
+    err = (got - ref).abs()[ok]
+    assert bool((err <= tol[ok]).all()), f"{what}: worst {float((err - tol[ok]).max())} past its tolerance"
+
+
+@pytest.mark.parametrize("hq,hkv,hd", HEADS)
+@pytest.mark.parametrize("n,prefix", [(1, 0), (1, 1), (1, 700), (2, 31), (5, 300), (7, 33), (16, 2003), (31, 64), (33, 8001), (64, 0),
+                                      (65, 127), (70, 1000), (130, 63), (250, 3900), (600, 17)])
+def test_attention(gpu, hq, hkv, hd, n, prefix):
+    a = _Attn(_gen(n + prefix), hq, hkv, hd, n, prefix)
+    ref, tol = a.ref()
+    _close(a.call(), ref, tol, "device length")
+    _close(a.call(device_len=False), ref, tol, "host length")
+
+
+@pytest.mark.parametrize("hq,hkv,hd", [(1, 1, 128), (8, 8, 64), (4, 2, 128), (6, 2, 64), (8, 2, 128), (12, 2, 64), (16, 2, 128), (64, 8, 128),
+                                       (14, 14, 128), (9, 3, 128)])
+@pytest.mark.parametrize("n,prefix", [(3, 95), (40, 1500)])
+def test_attention_head_layouts(gpu, hq, hkv, hd, n, prefix):
+    a = _Attn(_gen(hq), hq, hkv, hd, n, prefix)
+    _close(a.call(), *a.ref())
+
+
+def test_attention_largest_tree(gpu):
+    a = _Attn(_gen(4), 12, 2, 128, 1024, 100)
+    _close(a.call(), *a.ref())
+
+
+@pytest.mark.parametrize("hq,hkv,hd", HEADS)
+@pytest.mark.parametrize("prefix", [0, 5, 1000])
+def test_attention_any_mask(gpu, hq, hkv, hd, prefix):
+    """Masks that are no tree's: random bits, later nodes seen, rows without a bit (zeros without a prefix), all bits; and
+    bits past the nodes in the mask's words, which are not looked at."""
+    g = _gen(prefix)
+    n = 75
+    m = torch.rand(n, n, generator=g) < 0.3
+    m[3], m[74], m[10], m[40, :64], m[41, 64:] = False, False, True, False, False
+    a = _Attn(g, hq, hkv, hd, n, prefix, mask=m)
+    ref, tol = a.ref()
+    got = a.call()
+    _close(got, ref, tol)
+    if prefix == 0:
+        assert (got[3] == 0).all() and (got[74] == 0).all()
+    words = R.words(m)
+    words[:, 1] |= -1 << (n - 64)
+    assert torch.equal(a.call(words=words), got)
+
+
+@pytest.mark.parametrize("hq,hkv,hd", HEADS)
+@pytest.mark.parametrize("prefix", [0, 3, 700])
+def test_attention_not_finite_where_masked(gpu, hq, hkv, hd, prefix):
+    """A node's key and value hold NaN or infinities: the nodes that do not see it are as without it, and those that do
+    are not finite in the channels of a value, or everywhere for a NaN key."""
+    g = _gen(7)
+    n = 40
+    parents = R.random_tree(n, g)
+    clean = _Attn(g, hq, hkv, hd, n, prefix, mask=R.bits(parents))
+    ref, tol = clean.ref()
+    a = _Attn(g, hq, hkv, hd, n, prefix, mask=clean.mask)
+    a.q, a.k, a.v = clean.q.clone(), clean.k.clone(), clean.v.clone()
+    bad = {5: math.nan, 17: math.inf, 29: -math.inf, 39: math.nan}
+    sees = torch.zeros(n, hd, dtype=torch.bool)
+    for node, x in bad.items():
+        a.v[prefix + node, :, 1:hd:node] = x
+        sees[:, 1:hd:node] |= clean.mask[:, node, None]
+    for node in (11, 38):
+        a.k[prefix + node] = math.nan
+        sees |= clean.mask[:, node, None]
+    got = a.call().double().cpu()
+    for h in range(hq):
+        assert not torch.isfinite(got[:, h][sees]).any()
+        ok = ~sees
+        assert bool(((got[:, h] - ref[:, h].cpu()).abs()[ok] <= tol[:, h].cpu()[ok]).all())
+
+
+def test_attention_prefix_not_finite(gpu):
+    """Every node sees the rows before the tree: an infinite value there reaches its channel of every node."""
+    a = _Attn(_gen(9), 12, 2, 128, 9, 500)
+    ref, tol = a.ref()
+    a.v[100, 1, 7] = math.inf
+    got = a.call().double().cpu()
+    assert not torch.isfinite(got[:, 6:, 7]).any()
+    got[:, 6:, 7], ref, tol = 0, ref.cpu(), tol.cpu()
+    ref[:, 6:, 7] = 0
+    _close(got, ref, tol)
+
+
+def test_attention_score_extremes(gpu):
+    """Scores far apart, and equal ones: large keys, and keys of zeros."""
+    a = _Attn(_gen(10), 12, 2, 128, 20, 3000)
+    a.k[:1000] *= 30
+    a.k[1000:2000] = 0
+    a.q[3] = 0
+    _close(a.call(), *a.ref())
+
+
+def test_attention_minus_infinity_scores(gpu):
+    """All of a row's visible scores are -inf: zeros, as in the other attention operators."""
+    a = _Attn(_gen(11), 4, 2, 128, 3, 0, mask=torch.eye(3, dtype=torch.bool))
+    a.q[1], a.k[1] = 1, 0
+    a.k[1, :, 0] = -math.inf
+    got = a.call()
+    assert (got[1] == 0).all() and torch.isfinite(got).all()
+
+
+@pytest.mark.parametrize("hq,hkv,hd", HEADS)
+def test_attention_strides(gpu, hq, hkv, hd):
+    """Queries inside a fused q/k/v buffer; a cache with the heads outermost; a cache with wide rows."""
+    g = _gen(12)
+    n, prefix = 21, 1111
+    a = _Attn(g, hq, hkv, hd, n, prefix)
+    ref, tol = a.ref()
+    rows, bound, width = a.rows, a.rows + 9, (hq + 2 * hkv) * hd
+    fused = torch.full((n, width), math.nan, dtype=torch.bfloat16, device="cuda")
+    fused[:, :hq * hd] = a.q.cuda().flatten(1)
+    mask, d = R.words(a.mask).cuda(), _i32([rows])
+    for layout in ("heads", "wide"):
+        if layout == "heads":
+            k = torch.full((hkv, bound, hd), math.nan, dtype=torch.bfloat16, device="cuda")
+            v = torch.full((hkv, bound + 3, hd), math.nan, dtype=torch.bfloat16, device="cuda")
+            k[:, :rows], v[:, :rows] = a.k.cuda().transpose(0, 1), a.v.cuda().transpose(0, 1)
+            st = dict(k_stride_n=hd, k_stride_h=bound * hd, kv_stride_n=hd, kv_stride_h=(bound + 3) * hd)
+        else:
+            k = torch.full((bound, hkv * hd + 24), math.nan, dtype=torch.bfloat16, device="cuda")
+            v = torch.full((bound, hkv * hd + 8), math.nan, dtype=torch.bfloat16, device="cuda")
+            k[:rows, :hkv * hd], v[:rows, :hkv * hd] = a.k.cuda().flatten(1), a.v.cuda().flatten(1)
+            st = dict(k_stride_n=hkv * hd + 24, kv_stride_n=hkv * hd + 8)
+        c = C.make_attention_ctx(hq, hkv, hd, rope=False, q_stride_n=width, **st)
+        o = torch.empty(n, hq, hd, dtype=torch.bfloat16, device="cuda")
+        ws = _buf(C.load().efm_attention_tree_workspace_bytes(c, n, bound))
+        C.call("efm_attention_tree", c, ptr(fused), ptr(k), ptr(v), ptr(mask), ptr(o), n, 0, ptr(d), bound, ptr(ws), ws.numel(), stream())
+        torch.cuda.synchronize()
+        _close(o, ref, tol, layout)
+
+
+def test_attention_cache_past_32_bits(gpu):
+    """Rows more than 2^32 elements from the cache's start."""
+    if torch.cuda.mem_get_info()[0] < 60 << 30:
+        pytest.skip("needs 60 GB")
+    hq, hkv, hd, n, prefix, stride = 12, 2, 128, 10, 2300, 1 << 22
+    a = _Attn(_gen(13), hq, hkv, hd, n, prefix)
+    rows = a.rows
+    # one buffer: K, and V 1024 elements on in each row
+    both = torch.empty((rows - 1) * stride + 1024 + hkv * hd, dtype=torch.bfloat16, device="cuda")
+    kd, vd = both.as_strided((rows, hkv, hd), (stride, hd, 1)), both[1024:].as_strided((rows, hkv, hd), (stride, hd, 1))
+    kd.copy_(a.k), vd.copy_(a.v)
+    c = C.make_attention_ctx(hq, hkv, hd, rope=False, k_stride_n=stride, kv_stride_n=stride)
+    q, mask, o = a.q.cuda(), R.words(a.mask).cuda(), torch.empty(n, hq, hd, dtype=torch.bfloat16, device="cuda")
+    ws = _buf(C.load().efm_attention_tree_workspace_bytes(c, n, rows))
+    C.call("efm_attention_tree", c, ptr(q), ptr(kd), ptr(vd), ptr(mask), ptr(o), n, rows, None, 0, ptr(ws), ws.numel(), stream())
+    torch.cuda.synchronize()
+    _close(o, *a.ref())
+    # the move of rows that far
+    commit = _i32([prefix, 3, 0, 4, 9] + [-1] * (n - 3))
+    C.call("efm_draft_tree_move_kv", c, 1, 0, ptr(kd), ptr(vd), rows, n, ptr(commit), stream())
+    torch.cuda.synchronize()
+    assert torch.equal(kd[prefix + 1].cpu(), a.k[prefix + 4]) and torch.equal(vd[prefix + 2].cpu(), a.v[prefix + 9])
+    assert torch.equal(kd[prefix + 3:].cpu(), a.k[prefix + 3:]) and torch.equal(vd[:prefix + 1].cpu(), a.v[:prefix + 1])
+
+
+@pytest.mark.parametrize("length", [0, 6, 1001, 2 ** 31, 2 ** 32 - 1])
+def test_attention_device_length_out_of_range(gpu, length):
+    """Lengths below the nodes' number and past the bound: zeros."""
+    a = _Attn(_gen(14), 12, 2, 128, 7, 900)
+    bound = 1000
+    c = C.make_attention_ctx(12, 2, 128, rope=False)
+    k = torch.zeros(bound, 2, 128, dtype=torch.bfloat16, device="cuda")
+    q, mask = a.q.cuda(), R.words(a.mask).cuda()
+    d = torch.tensor([length - (1 << 32) if length >= 1 << 31 else length], dtype=torch.int32, device="cuda")
+    o = torch.full((7, 12 * 128), 5.0, dtype=torch.bfloat16, device="cuda")
+    ws = _buf(C.load().efm_attention_tree_workspace_bytes(c, 7, bound))
+    C.call("efm_attention_tree", c, ptr(q), ptr(k), ptr(k), ptr(mask), ptr(o), 7, 0, ptr(d), bound, ptr(ws), ws.numel(), stream())
+    torch.cuda.synchronize()
+    assert (o == 0).all()
+
+
+def test_attention_one_workspace_serves_smaller_calls(gpu):
+    """The largest call's workspace, filled with NaN, under calls of fewer nodes and rows."""
+    c = C.make_attention_ctx(28, 4, 128, rope=False)
+    ws = _buf(C.load().efm_attention_tree_workspace_bytes(c, 64, 9000))
+    for n, prefix in ((64, 8936), (1, 8999), (2, 8000), (9, 5000), (17, 8983), (40, 300), (64, 1000)):
+        a = _Attn(_gen(n), 28, 4, 128, n, prefix)
+        _close(a.call(ws=ws, bound=n + prefix), *a.ref(), f"{n} nodes behind {prefix}")
+
+
+def test_attention_repeats(gpu):
+    a = _Attn(_gen(15), 28, 4, 128, 33, 9000)
+    first = a.call()
+    for _ in range(3):
+        assert torch.equal(a.call(), first)
+
+
+def test_attention_chain_is_causal_prefill(gpu):
+    """A chain of nodes sees what the rows of a causal prompt see."""
+    n, prefix = 45, 2000
+    a = _Attn(_gen(16), 28, 4, 128, n, prefix, mask=torch.ones(n, n, dtype=torch.bool).tril())
+    got = a.call()
+    c = C.make_attention_ctx(28, 4, 128, rope=False)
+    q, k, v = a.q.cuda(), a.k.cuda(), a.v.cuda()
+    o = torch.empty(n, 28, 128, dtype=torch.bfloat16, device="cuda")
+    C.call("efm_attention_prefill", c, ptr(q), ptr(k), ptr(v), ptr(o), n, n + prefix, 1, stream())
+    torch.cuda.synchronize()
+    ref, tol = a.ref()
+    _close(got, ref, tol)
+    assert bool(((got.double() - o.double()).abs() <= 2 * tol + 2.0 ** -8 * 3 * ref.abs()).all())
+
+
+# ---------------------------------------------------------------- sampling
+
+def _sample(x, u, t=1.0, k=0, p=1.0, min_p=0.0, stride=0, vocab=None, rows=None, data=None):
+    rows, vocab = rows or x.shape[0], vocab or x.shape[1]
+    out = torch.full((rows + 1,), -77, dtype=torch.int32, device="cuda")
+    ws = _buf(C.load().efm_sampler_filtered_workspace_bytes(rows, vocab))
+    dt = C.EFM_DTYPE_BF16 if x.dtype == torch.bfloat16 else C.EFM_DTYPE_F32
+    C.call("efm_sampler_filtered", rows, vocab, data or ptr(x), dt, stride, t, k, p, min_p, ptr(u), ptr(out), ptr(ws), ws.numel(), stream())
+    torch.cuda.synchronize()
+    assert int(out[rows]) == -77
+    return out[:rows]
+
+
+def _logits(seed, rows, vocab, dtype=torch.float32):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    x = 2.5 * torch.randn(rows, vocab, generator=g, device="cuda")
+    x.scatter_(1, torch.randint(0, vocab, (rows, 12), generator=g, device="cuda"),
+               7 + 3 * torch.rand(rows, 12, generator=g, device="cuda"))
+    return x.to(dtype), torch.rand(rows, generator=g, device="cuda")
+
+
+FILTERS = [dict(), dict(t=0.5), dict(k=1), dict(k=50), dict(k=1000), dict(p=0.9), dict(p=0.3, t=1.4), dict(min_p=0.05), dict(min_p=1.0),
+           dict(k=40, p=0.95), dict(k=300, min_p=0.01), dict(p=0.999, min_p=0.002), dict(k=64, p=0.8, min_p=0.1, t=0.7), dict(p=1e-9),
+           dict(t=1e-6), dict(t=1e6), dict(t=1e6, p=0.5), dict(t=1e6, k=700, p=0.5), dict(k=2 ** 31 - 1, p=0.99)]
+
+
+@pytest.mark.parametrize("f", FILTERS, ids=str)
+@pytest.mark.parametrize("rows,vocab,dtype", [(1, 151936, torch.float32), (5, 8192, torch.float32), (3, 151936, torch.bfloat16),
+                                              (70, 3001, torch.float32), (40, 1000, torch.bfloat16)])
+def test_sampler(gpu, f, rows, vocab, dtype):
+    x, u = _logits(rows + vocab, rows, vocab, dtype)
+    assert torch.equal(_sample(x, u, **f), R.sample(x, u, **f))
+
+
+@pytest.mark.parametrize("f", [dict(), dict(k=50, p=0.9), dict(p=0.95), dict(min_p=0.03)], ids=str)
+@pytest.mark.parametrize("rows,vocab", [(1, 1), (4, 2), (3, 63), (2, 65), (9, 1023), (9, 1025), (2, 32768), (2, 32769), (2, (1 << 20) - 1),
+                                        (260, 40000), (600, 700)])
+def test_sampler_sizes(gpu, f, rows, vocab):
+    for dtype in (torch.float32, torch.bfloat16):
+        x, u = _logits(vocab, rows, vocab, dtype)
+        assert torch.equal(_sample(x, u, **f), R.sample(x, u, **f))
+
+
+@pytest.mark.parametrize("f", [dict(k=7), dict(k=700), dict(p=0.5), dict(k=900, p=0.6), dict(p=0.999), dict()], ids=str)
+@pytest.mark.parametrize("values", [1, 2, 5])
+@pytest.mark.parametrize("vocab", [3000, 151936])
+def test_sampler_ties(gpu, f, values, vocab):
+    """Few different logits, both zeros among them: ties go to the lowest ids."""
+    g = torch.Generator(device="cuda").manual_seed(values)
+    table = torch.tensor([0.0, -0.0, 1.0, -1.5, -40.0], device="cuda")
+    x = table[torch.randint(0, values, (6, vocab), generator=g, device="cuda")]
+    u = torch.rand(6, generator=g, device="cuda")
+    assert torch.equal(_sample(x, u, **f), R.sample(x, u, **f))
+
+
+@pytest.mark.parametrize("f", [dict(), dict(k=20), dict(p=0.9), dict(min_p=0.1), dict(k=30, p=0.7, min_p=0.01)], ids=str)
+@pytest.mark.parametrize("vocab", [2000, 100000])
+def test_sampler_rows_that_are_not_finite(gpu, f, vocab):
+    """NaN and infinities among the logits; rows with one finite logit, one +inf, several, and none (-1)."""
+    x, u = _logits(3, 9, vocab)
+    x[0, ::3], x[1, 1::2] = math.nan, -math.inf
+    x[2], x[3] = -math.inf, math.nan
+    x[4] = -math.inf
+    x[4, vocab - 7] = -1e30
+    x[5, 1234], x[6, 100:1500:9] = math.inf, math.inf
+    x[7, 5], x[7, 6] = 3.4e38, -3.4e38
+    x[8, vocab // 2:] = torch.finfo(torch.float32).min
+    got = _sample(x, u, **f)
+    assert torch.equal(got, R.sample(x, u, **f))
+    assert got[2] == -1 and got[3] == -1 and got[4] == vocab - 7 and got[5] == 1234
+
+
+def test_sampler_random_numbers_at_the_ends(gpu):
+    x, _ = _logits(4, 8, 5000)
+    x[:] = x[0]
+    u = torch.tensor([0.0, 1 - 2.0 ** -24, 1.0, 5.0, math.inf, -1.0, math.nan, 2.0 ** -140], device="cuda")
+    for f in (dict(), dict(k=9), dict(p=0.5)):
+        got = _sample(x, u, **f)
+        assert torch.equal(got, R.sample(x, u, **f))
+        first, last = int(got[0]), int(got[1])
+        assert got.tolist() == [first, last, last, last, last, first, first, first] and first <= last
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("vocab", [8192, 60001])
+def test_sampler_strides_and_offsets(gpu, dtype, vocab):
+    """Padded rows whose padding would win, and rows that start at any element."""
+    for pad, shift in ((1, 0), (64, 1), (7, 3), (0, 5)):
+        x, u = _logits(pad, 5, vocab, dtype)
+        flat = torch.full((shift + 5 * (vocab + pad) + 8,), 1e4, dtype=dtype, device="cuda")
+        flat[shift:shift + 5 * (vocab + pad)].view(5, -1)[:, :vocab] = x
+        got = _sample(x, u, t=0.8, k=60, p=0.95, stride=vocab + pad, data=flat.data_ptr() + shift * flat.element_size())
+        assert torch.equal(got, R.sample(x, u, t=0.8, k=60, p=0.95)), (pad, shift)
+
+
+def test_sampler_row_offsets_past_32_bits(gpu):
+    rows, vocab, stride = 3, 5000, 1 << 31
+    if torch.cuda.mem_get_info()[0] < 30 << 30:
+        pytest.skip("needs 30 GB")
+    x, u = _logits(6, rows, vocab)
+    flat = torch.empty(2 * stride + vocab, device="cuda")
+    for r in range(rows):
+        flat[r * stride:r * stride + vocab] = x[r]
+    for f in (dict(p=0.9), dict(k=40), dict(min_p=0.05)):
+        assert torch.equal(_sample(x, u, stride=stride, data=flat.data_ptr(), **f), R.sample(x, u, **f))
+
+
+def test_sampler_rows_do_not_meet(gpu):
+    """A row's token is the same alone and among others, and with a workspace that held other calls."""
+    x, u = _logits(8, 90, 151936)
+    for f in (dict(k=50, p=0.9), dict(p=0.95, t=1.3), dict(min_p=0.02)):
+        all_rows = _sample(x, u, **f)
+        for r in (0, 41, 89):
+            assert torch.equal(_sample(x[r:r + 1], u[r:r + 1], **f), all_rows[r:r + 1])
+
+
+def test_sampler_draws_the_distribution(gpu):
+    """Evenly spaced random numbers draw each id as often as its probability says, to one draw."""
+    vocab, rows = 50, 4096
+    x, _ = _logits(9, 1, vocab)
+    u = (torch.arange(rows, device="cuda") + 0.5) / rows
+    got = _sample(x.expand(rows, -1).contiguous(), u, t=0.9)
+    p = torch.softmax(x[0].double() / 0.9, -1)
+    count = torch.bincount(got.long(), minlength=vocab)
+    assert bool(((count - p * rows).abs() <= 1.01).all())
+
+
+# ---------------------------------------------------------------- accept and move
+
+def _accept(parents, draft, target, rows, next_nodes=0, in_place=False):
+    n = len(parents)
+    args = [_i32(x) for x in (parents, draft, target)]
+    d = _i32([rows])
+    out = d if in_place else _i32([-9])
+    commit, tokens = torch.full((n + 3,), -77, dtype=torch.int32, device="cuda"), torch.full((n + 1,), -77, dtype=torch.int32, device="cuda")
+    C.call("efm_draft_tree_accept", n, *[ptr(x) for x in args], ptr(d), next_nodes, ptr(out), ptr(commit), ptr(tokens), stream())
+    torch.cuda.synchronize()
+    assert int(commit[n + 2]) == -77 and int(tokens[n]) == -77
+    return commit[:n + 2].tolist(), tokens[:n].tolist(), int(out[0])
+
+
+def _check_accept(parents, draft, target, rows, **kw):
+    n = len(parents)
+    path = R.accept(parents, draft, target)
+    commit, tokens, length = _accept(parents, draft, target, rows, **kw)
+    fill = [-1] * (n - len(path))
+    assert commit == [rows - n, len(path)] + path + fill
+    assert tokens == [target[p] for p in path] + fill
+    assert length == rows - n + len(path) + kw.get("next_nodes", 0)
+    return path
+
+
+@pytest.mark.parametrize("n", [1, 2, 5, 64, 65, 300, 1024])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_accept(gpu, n, in_place):
+    for seed in range(4):
+        g = _gen(seed)
+        parents = R.random_tree(n, g, reach=(None, 4, 30, 2)[seed])
+        draft = torch.randint(0, 3, (n,), generator=g).tolist()   # few tokens: siblings often agree, the lowest index wins
+        target = torch.randint(0, 3, (n,), generator=g).tolist()
+        _check_accept(parents, draft, target, 500 + n, next_nodes=seed * 7, in_place=in_place)
+
+
+def test_accept_whole_chain(gpu):
+    n = 1024
+    assert len(_check_accept(list(range(-1, n - 1)), list(range(n)), list(range(1, n + 1)), n)) == n
+
+
+def test_accept_unused_nodes_and_missing_tokens(gpu):
+    parents = [-1, 0, 0, -2, 2, 4, 9, 5, -1]
+    # node 1 has no token (-1) and neither has node 0's row: they do not match; node 2 is accepted, then 4, 5
+    assert _check_accept(parents, [9, -1, 3, 3, 4, 5, 6, 7, 3], [-1] * 9, 100) == [0]
+    assert _check_accept(parents, [9, -1, 3, 3, 4, 5, 6, 7, 3], [3, 1, 4, 4, 5, 8, 6, 7, 3], 100) == [0, 2, 4, 5]
+    # fewer rows than nodes: nothing
+    commit, tokens, length = _accept(parents, [0] * 9, [0] * 9, 8, next_nodes=5)
+    assert commit == [0, 0] + [-1] * 9 and tokens == [-1] * 9 and length == 8
+
+
+@pytest.mark.parametrize("hq,hkv,hd", HEADS)
+@pytest.mark.parametrize("path", [[0], [0, 1, 2], [0, 3, 4, 9], [0, 2, 3, 5, 6, 7, 8, 9, 10, 11, 13, 14, 18, 19], list(range(20)), [5, 19], []],
+                         ids=str)
+def test_move(gpu, hq, hkv, hd, path):
+    g = _gen(len(path))
+    layers, rows, n, base = 3, 70, 20, 41
+    cache = _bf(g, layers, 2, rows, hkv * hd)
+    dev = cache.cuda()
+    c = C.make_attention_ctx(hq, hkv, hd, rope=False)
+    commit = _i32([base, len(path)] + path + [-1] * (n - len(path)))
+    C.call("efm_draft_tree_move_kv", c, layers, 2 * rows * hkv * hd, ptr(dev[0, 0]), ptr(dev[0, 1]), rows, n, ptr(commit), stream())
+    torch.cuda.synchronize()
+    want = cache.clone()
+    for i, p in enumerate(path):
+        want[:, :, base + i] = cache[:, :, base + p]
+    assert torch.equal(dev.cpu(), want)
+
+
+def test_move_with_the_heads_outermost(gpu):
+    hkv, hd, layers, rows, n = 4, 64, 2, 50, 8
+    k, v = _bf(_gen(1), layers, hkv, rows, hd).cuda(), _bf(_gen(2), layers, hkv, rows, hd).cuda()
+    k0, v0 = k.clone(), v.clone()
+    c = C.make_attention_ctx(8, hkv, hd, rope=False, k_stride_n=hd, k_stride_h=rows * hd, kv_stride_n=hd, kv_stride_h=rows * hd)
+    commit = _i32([rows - n, 3, 0, 2, 7] + [-1] * 5)
+    C.call("efm_draft_tree_move_kv", c, layers, hkv * rows * hd, ptr(k), ptr(v), rows, n, ptr(commit), stream())
+    torch.cuda.synchronize()
+    for i, p in enumerate((0, 2, 7)):
+        k0[:, :, rows - n + i], v0[:, :, rows - n + i] = k0[:, :, rows - n + p].clone(), v0[:, :, rows - n + p].clone()
+    assert torch.equal(k, k0) and torch.equal(v, v0)
+
+
+@pytest.mark.parametrize("commit", [[43, 3, 0, 2, 3], [-1, 3, 0, 2, 3], [10, -4, 0, 2, 3], [2 ** 31 - 1, 3, 0, 2, 3]], ids=str)
+def test_move_that_would_leave_the_cache(gpu, commit):
+    """A base past the cache (here 43 + 8 of 50 rows) and a negative count move nothing."""
+    k = _bf(_gen(3), 50, 256).cuda()
+    v, k0 = k.clone(), k.clone()
+    c = C.make_attention_ctx(12, 2, 128, rope=False)
+    d = _i32(commit + [-1] * 5)
+    C.call("efm_draft_tree_move_kv", c, 1, 0, ptr(k), ptr(v), 50, 8, ptr(d), stream())
+    torch.cuda.synchronize()
+    assert torch.equal(k, k0) and torch.equal(v, k0)
+
+
+@pytest.mark.parametrize("path,moved", [([0, 3, 2, 6], 2), ([0, 3, 8, 9], 2), ([0, 4, -1, 5], 2), ([0, 4, 4, 5], 2), ([0, 2, 5, 7, 1, 1, 1, 1, 7], 4)], ids=str)
+def test_move_of_a_path_that_does_not_rise(gpu, path, moved):
+    """The move ends where the path falls, repeats itself or leaves the tree's 8 nodes."""
+    k = _bf(_gen(4), 50, 256).cuda()
+    v, want = k.clone(), k.clone()
+    for i, p in enumerate(path[:moved]):
+        want[20 + i] = k[20 + p]
+    c = C.make_attention_ctx(12, 2, 128, rope=False)
+    d = _i32([20, len(path)] + path + [-1] * 8)
+    C.call("efm_draft_tree_move_kv", c, 1, 0, ptr(k), ptr(v), 50, 8, ptr(d), stream())
+    torch.cuda.synchronize()
+    assert torch.equal(k, want) and torch.equal(v, want)
