@@ -72,7 +72,8 @@ def _sample(rows=2, vocab=100, x=P, dt=C.EFM_DTYPE_F32, stride=0, t=1.0, k=0, p=
     (dict(t=0.0), BAD), (dict(t=1e-7), BAD), (dict(t=math.inf), BAD), (dict(t=math.nan), BAD), (dict(t=-1.0), BAD),
     (dict(p=0.0), BAD), (dict(p=math.nan), BAD), (dict(p=-0.5), BAD), (dict(mp=1.5), BAD), (dict(mp=math.nan), BAD),
     (dict(x=None), BAD), (dict(u=None), BAD), (dict(out=None), BAD), (dict(x=ODD), BAD), (dict(x=4097, dt=C.EFM_DTYPE_BF16), BAD),
-    (dict(u=ODD), BAD), (dict(out=ODD), BAD), (dict(rows=0), C.EFM_OK), (dict(rows=(1 << 20) + 1), UNSUP),
+    (dict(u=ODD), BAD), (dict(out=ODD), BAD), (dict(rows=0), C.EFM_OK), (dict(rows=65536), UNSUP),
+    (dict(vocab=151936), WS), (dict(vocab=151936, ws=P, nbytes=1000), WS), (dict(vocab=151936, ws=4104, nbytes=1 << 40), BAD),
 ])
 def test_sampler_refusals(kw, want):
     assert _sample(**kw) == want

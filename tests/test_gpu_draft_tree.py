@@ -326,10 +326,10 @@ def test_attention_chain_is_causal_prefill(gpu):
 
 # ---------------------------------------------------------------- sampling
 
-def _sample(x, u, t=1.0, k=0, p=1.0, min_p=0.0, stride=0, vocab=None, rows=None, data=None):
+def _sample(x, u, t=1.0, k=0, p=1.0, min_p=0.0, stride=0, vocab=None, rows=None, data=None, ws=None):
     rows, vocab = rows or x.shape[0], vocab or x.shape[1]
     out = torch.full((rows + 1,), -77, dtype=torch.int32, device="cuda")
-    ws = _buf(C.load().efm_sampler_filtered_workspace_bytes(rows, vocab))
+    ws = _buf(C.load().efm_sampler_filtered_workspace_bytes(rows, vocab), 0) if ws is None else ws
     dt = C.EFM_DTYPE_BF16 if x.dtype == torch.bfloat16 else C.EFM_DTYPE_F32
     C.call("efm_sampler_filtered", rows, vocab, data or ptr(x), dt, stride, t, k, p, min_p, ptr(u), ptr(out), ptr(ws), ws.numel(), stream())
     torch.cuda.synchronize()
@@ -360,7 +360,7 @@ def test_sampler(gpu, f, rows, vocab, dtype):
 
 @pytest.mark.parametrize("f", [dict(), dict(k=50, p=0.9), dict(p=0.95), dict(min_p=0.03)], ids=str)
 @pytest.mark.parametrize("rows,vocab", [(1, 1), (4, 2), (3, 63), (2, 65), (9, 1023), (9, 1025), (2, 32768), (2, 32769), (2, (1 << 20) - 1),
-                                        (260, 40000), (600, 700)])
+                                        (260, 40000), (600, 700), (1100, 15000), (3, 14336), (3, 14337), (1500, 20000)])
 def test_sampler_sizes(gpu, f, rows, vocab):
     for dtype in (torch.float32, torch.bfloat16):
         x, u = _logits(vocab, rows, vocab, dtype)
@@ -438,6 +438,18 @@ def test_sampler_rows_do_not_meet(gpu):
         all_rows = _sample(x, u, **f)
         for r in (0, 41, 89):
             assert torch.equal(_sample(x[r:r + 1], u[r:r + 1], **f), all_rows[r:r + 1])
+
+
+def test_sampler_workspace_serves_calls_of_any_size(gpu):
+    """One workspace under calls of other sizes, filters and types, overflowing lists among them."""
+    ws = _buf(C.load().efm_sampler_filtered_workspace_bytes(64, 1 << 19), 0)
+    for i in range(3):
+        for rows, vocab, f in ((64, 20000, dict(p=0.9)), (1, 151936, dict(k=50)), (7, 500000, dict(p=0.99, t=1.5)), (33, 151936, dict(k=900, p=0.9)),
+                               (2, 40000, dict()), (5, 30000, dict(t=1e6, p=0.5)), (5, 30000, dict(t=1e6, k=9)), (64, 15000, dict(min_p=0.1))):
+            x, u = _logits(i, rows, vocab, (torch.float32, torch.bfloat16)[i % 2])
+            if i == 2:
+                x[:, ::2] = 1.0
+            assert torch.equal(_sample(x, u, ws=ws, **f), R.sample(x, u, **f)), (rows, vocab, f)
 
 
 def test_sampler_draws_the_distribution(gpu):
