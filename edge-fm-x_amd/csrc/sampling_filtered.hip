@@ -16,16 +16,16 @@
 //
 // What bounds it: few rows by the launches and the chain of a row's last workgroup, many rows by the
 // logits' bytes and the 64-bit exponentials. A large vocabulary is cut into blocks of a workgroup each:
-//   no top-k, no top-p   1. block maxima  2. block masses; the row's last workgroup finds the block
+//   no top-k, no top-p   1. block maxima  2. masses of tiles; the row's last workgroup finds the tile
 //                        that holds r and the id within it
-//   top-p                1. block maxima  2. histogram of masses by logit  3. masses of the ids that
-//                        are surely in N by block, and a list of the ids of the bin in which N ends;
-//                        the last workgroup orders that list and goes on as above
+//   top-p                1. block maxima  2. histogram of masses by logit  3. masses by tile of the ids
+//                        that are surely in N, and a list of the ids of the bin in which N ends; the
+//                        last workgroup finds N's end in that list and goes on as above
 //   top-k                1. block maxima and a histogram of counts by logit  2. a list of the ids that
-//                        may be in K; the last workgroup orders it and draws
-// A list that does not fit (thousands of equal logits) sends the row's last workgroup through the
-// row itself, digit by digit: filt_select below, which is also what the small vocabularies run on, a
-// workgroup a row with the row in LDS.
+//                        may be in K; the last workgroup finds the ends of K and N in it and draws
+// A small vocabulary goes through the same steps in one launch, a workgroup a row. Where the list's
+// masses do not fit in LDS, or the list not in its place (thousands of equal logits), the last
+// workgroup works from the list in memory or from the row itself.
 #include "common.hpp"
 
 #include <algorithm>
@@ -40,12 +40,12 @@ constexpr int kFiltWaves = kFiltThreads / kWave;
 constexpr int kFiltMaxVocab = 1 << 20;
 constexpr double kFiltOne = 17592186044416.0;   // 2^44
 constexpr int kFiltBlocks = 128;                 // of a row, at most
+constexpr int kFiltTiles = 1024;                 // of a row: passes of a workgroup's loads, 1024 logits or more each
 constexpr int kFiltMassBins = 1024, kFiltBinsPerOctave = 22;   // masses from 2^0 to below 2^-46
 constexpr int kFiltCountBins = 4096, kFiltCountShift = 20;     // sign, exponent and three bits of the logit
-constexpr int kFiltMaxTiles = kFiltThreads;      // a block's passes of a workgroup's loads, 1024 logits or more each
 constexpr int kFiltList = 4096;
-constexpr int kFiltSort = 1024;
-constexpr int kFiltLdsVocab = 14336;             // rows that a workgroup holds in LDS
+constexpr int kFiltHeld = 1024;                  // entries of a list that a workgroup holds with their masses
+constexpr int kFiltOneVocab = 16384;             // rows of one launch
 
 // One row's part of the workspace. hist, counter and count are zero between calls.
 struct FiltRow {
@@ -56,8 +56,8 @@ struct FiltRow {
     uint32_t counter, count;
     uint32_t pad[2];
     float bmax[kFiltBlocks];
-    unsigned long long bmass[kFiltBlocks];
-    unsigned long long list[kFiltList];   // ~key << 32 | id: ascending in the sampler's order
+    unsigned long long tile[kFiltTiles];
+    unsigned long long list[kFiltList];   // key << 32 | id
 };
 static_assert(sizeof(FiltRow) % 16 == 0, "rows of the workspace stay aligned");
 
@@ -116,52 +116,74 @@ __device__ __forceinline__ float filt_logit(uint32_t key) { return __uint_as_flo
 
 __device__ __forceinline__ float filt_clean(float l) { return l == l ? l : -INFINITY; }
 
-// f(id, logit) for the logits of [first, end) of a row: 16 bytes a thread, four under way.
+// A row's logits [first, end), first a multiple of a tile: f(tile of the range, first id, the thread's
+// E logits, how many of them there are), by all threads together; 16 bytes a thread, four under way.
 template <bool BF16, typename F>
-__device__ __forceinline__ void filt_each(const void* row, int first, int end, F f) {
-    constexpr int E = BF16 ? 8 : 4, U = 4;
-    const int tid = threadIdx.x;
-    int done = first;
-    if ((reinterpret_cast<uintptr_t>(row) & 15) == 0) {   // first is a multiple of 8
-        const int whole = (end - first) / E;
-        const uint4* const p = reinterpret_cast<const uint4*>(static_cast<const char*>(row) + (int64_t)first * (BF16 ? 2 : 4));
-        for (int v0 = tid; v0 < whole; v0 += U * kFiltThreads) {
-            uint4 x[U];
+__device__ __forceinline__ void filt_tiles(const void* row, int first, int end, F f) {
+    constexpr int E = BF16 ? 8 : 4, U = 4, TILE = E * kFiltThreads;
+    const bool aligned = (reinterpret_cast<uintptr_t>(row) & 15) == 0;
+    for (int t0 = 0; first + t0 * TILE < end; t0 += U) {
+        uint4 x[U];
 #pragma unroll
-            for (int j = 0; j < U; ++j)
-                if (v0 + j * kFiltThreads < whole) x[j] = p[v0 + j * kFiltThreads];
-#pragma unroll
-            for (int j = 0; j < U; ++j) {
-                const int v = v0 + j * kFiltThreads;
-                if (v >= whole) break;
-                const int i = first + v * E;
-                const uint32_t w[4] = {x[j].x, x[j].y, x[j].z, x[j].w};
+        for (int j = 0; j < U; ++j) {
+            const int i = first + (t0 + j) * TILE + (int)threadIdx.x * E;
+            if (aligned && i + E <= end) {
+                x[j] = *reinterpret_cast<const uint4*>(static_cast<const char*>(row) + (int64_t)i * (BF16 ? 2 : 4));
+            } else {
+                uint32_t w[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     if constexpr (BF16) {
-                        f(i + 2 * e, filt_clean(lo_f32(w[e])));
-                        f(i + 2 * e + 1, filt_clean(hi_f32(w[e])));
+                        const uint16_t* const p = static_cast<const uint16_t*>(row);
+                        const uint32_t lo = i + 2 * e < end ? p[i + 2 * e] : 0xff80u, hi = i + 2 * e + 1 < end ? p[i + 2 * e + 1] : 0xff80u;
+                        w[e] = lo | hi << 16;
                     } else {
-                        f(i + e, filt_clean(__uint_as_float(w[e])));
+                        w[e] = i + e < end ? static_cast<const uint32_t*>(row)[i + e] : 0xff800000u;
                     }
                 }
+                x[j] = make_uint4(w[0], w[1], w[2], w[3]);
             }
         }
-        done = first + whole * E;
-    }
-    for (int i = done + tid; i < end; i += kFiltThreads) {
-        if constexpr (BF16) f(i, filt_clean(bf16_to_f32(static_cast<const uint16_t*>(row)[i])));
-        else f(i, filt_clean(static_cast<const float*>(row)[i]));
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+            const int i = first + (t0 + j) * TILE + (int)threadIdx.x * E;
+            if (first + (t0 + j) * TILE >= end) break;
+            float l[E];
+            const uint32_t w[4] = {x[j].x, x[j].y, x[j].z, x[j].w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if constexpr (BF16) l[2 * e] = filt_clean(lo_f32(w[e])), l[2 * e + 1] = filt_clean(hi_f32(w[e]));
+                else l[e] = filt_clean(__uint_as_float(w[e]));
+            }
+            f(t0 + j, i, l, min(max(end - i, 0), E));
+        }
     }
 }
 
-__device__ __forceinline__ uint64_t filt_wave_scan(uint64_t v, int lane) {
-#pragma unroll
-    for (int off = 1; off < kWave; off <<= 1) {
-        const uint64_t o = __shfl_up(v, off, kWave);
-        if (lane >= off) v += o;
-    }
+// A 64-bit value moved across lanes, 0 where the source is none.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t filt_dpp(uint64_t v) {
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, ROWS, 0xf, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), CTRL, ROWS, 0xf, false);
+    return (uint64_t)hi << 32 | lo;
+}
+
+// Inclusive sums over the lanes of a wave: shifts by 1, 2, 4 and 8 within 16 lanes, then the ends of
+// the rows of 16.
+__device__ __forceinline__ uint64_t filt_wave_scan(uint64_t v) {
+    v += filt_dpp<0x111, 0xf>(v);
+    v += filt_dpp<0x112, 0xf>(v);
+    v += filt_dpp<0x114, 0xf>(v);
+    v += filt_dpp<0x118, 0xf>(v);
+    v += filt_dpp<0x142, 0xa>(v);
+    v += filt_dpp<0x143, 0xc>(v);
     return v;
+}
+
+// Their last, in every lane.
+__device__ __forceinline__ uint64_t filt_last_lane(uint64_t v) {
+    return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), 63) << 32 |
+           (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, 63);
 }
 
 struct FiltShared {
@@ -169,13 +191,14 @@ struct FiltShared {
     unsigned long long sel[2];
     unsigned long long bins[kFiltThreads];
     float redf[kFiltWaves];
-    uint32_t flag;
+    uint32_t range[kFiltWaves][3];
+    uint32_t flag, found[2];
 };
 
 // Sum of the values of the threads before this one, and of all.
 __device__ __forceinline__ uint64_t filt_scan(uint64_t v, FiltShared& s, uint64_t* total) {
     const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-    const uint64_t incl = filt_wave_scan(v, lane);
+    const uint64_t incl = filt_wave_scan(v);
     __syncthreads();
     if (lane == kWave - 1) s.red[wave] = incl;
     __syncthreads();
@@ -187,6 +210,12 @@ __device__ __forceinline__ uint64_t filt_scan(uint64_t v, FiltShared& s, uint64_
     }
     *total = all;
     return before + incl - v;
+}
+
+__device__ __forceinline__ uint64_t filt_sum(uint64_t v, FiltShared& s) {
+    uint64_t all;
+    filt_scan(v, s, &all);
+    return all;
 }
 
 // The thread whose `own` units hold unit `rank` (from 0), in the order of threads, and the units
@@ -201,7 +230,7 @@ __device__ __forceinline__ int filt_find(uint64_t own, uint64_t rank, FiltShared
 }
 
 __device__ __forceinline__ float filt_max(float m, FiltShared& s) {
-    m = wave_max(m);
+    m = wave_max_uniform(m);
     if (threadIdx.x % kWave == 0) s.redf[threadIdx.x / kWave] = m;
     __syncthreads();
     m = s.redf[0];
@@ -229,112 +258,274 @@ __device__ __forceinline__ uint64_t filt_need(float top_p, uint64_t W) {
     return need < 1 ? 1 : need > W ? W : need;
 }
 
-// The whole choice over any source of (id, logit), each(f), by histograms of eight bits at a time.
+// The entry that holds unit `rank` of the weights of a source of (id, key, weight), each(f): in the
+// sampler's order, or by id alone. The range of the keys (of equal keys: of the ids) that may hold it is
+// cut into 256 bins until one entry is left. rank is below the sum of the weights.
 template <typename Each>
-__device__ int filt_select(const FiltArgs& a, float m, float u, FiltShared& s, Each each) {
-    const int tid = threadIdx.x;
-    uint64_t before;
-    // The bins of `digit` of what take(i, k) takes, and the one that holds unit `rank` of `weight`.
-    auto pass = [&](auto take, auto digit, auto weight, uint64_t& rank) {
-        __syncthreads();
+__device__ __forceinline__ FiltCut filt_pick(bool by_id, uint64_t rank, FiltShared& s, Each each) {
+    const int tid = threadIdx.x, wave = tid / kWave;
+    uint32_t lo = 0, hi = ~0u, tie = 0;   // of ~key, or of the ids with ~key = tie
+    bool ids = by_id;
+    for (;;) {
+        uint32_t n = 0, least = ~0u, most = 0, key = 0, id = 0;
+        auto active = [&](int i, uint32_t k, uint64_t w) {
+            const uint32_t v = ids ? (uint32_t)i : ~k;
+            return w != 0 && v >= lo && v <= hi && (!ids || by_id || ~k == tie);
+        };
+        each([&](int i, uint32_t k, uint64_t w) {
+            if (!active(i, k, w)) return;
+            const uint32_t v = ids ? (uint32_t)i : ~k;
+            ++n, least = min(least, v), most = max(most, v), key = k, id = (uint32_t)i;
+        });
+        const bool mine = n != 0;
+#pragma unroll
+        for (int off = 32; off >= 1; off >>= 1) {
+            n += __shfl_xor(n, off, kWave);
+            least = min(least, (uint32_t)__shfl_xor((int)least, off, kWave));
+            most = max(most, (uint32_t)__shfl_xor((int)most, off, kWave));
+        }
+        if (tid % kWave == 0) s.range[wave][0] = n, s.range[wave][1] = least, s.range[wave][2] = most;
         s.bins[tid] = 0;
         __syncthreads();
-        each([&](int i, float l) {
-            const uint32_t k = filt_key(l);
-            if (!take(i, k)) return;
-            const uint64_t w = weight(l);
-            if (w != 0) atomicAdd(&s.bins[digit(i, k)], (unsigned long long)w);
+        n = 0;
+#pragma unroll
+        for (int w = 0; w < kFiltWaves; ++w) n += s.range[w][0], least = min(least, s.range[w][1]), most = max(most, s.range[w][2]);
+        if (n == 1) {
+            if (mine) s.found[0] = key, s.found[1] = id;
+            __syncthreads();
+            return FiltCut{s.found[0], (int)s.found[1]};
+        }
+        if (least == most) {   // equal keys: by id
+            ids = true, tie = least, lo = 0, hi = ~0u;
+            __syncthreads();
+            continue;
+        }
+        const int bits = 32 - __builtin_clz(most - least), shift = max(bits - 8, 0);
+        each([&](int i, uint32_t k, uint64_t w) {
+            if (active(i, k, w)) atomicAdd(&s.bins[((ids ? (uint32_t)i : ~k) - least) >> shift], (unsigned long long)w);
         });
         __syncthreads();
-        const int bin = filt_find(s.bins[tid], rank, s, &before);
+        uint64_t before;
+        const uint32_t bin = (uint32_t)filt_find(s.bins[tid], rank, s, &before);
         rank -= before;
-        return (uint32_t)bin;
-    };
-    auto by_id = [&](auto take, auto weight, uint64_t rank) {
-        uint32_t top = 0;
-        for (int shift = 16; shift >= 0; shift -= 8) {
-            const uint32_t bin = pass([&](int i, uint32_t k) { return take(i, k) && (uint32_t)i >> shift >> 8 == top; },
-                                      [&](int i, uint32_t) { return (uint32_t)i >> shift & 255; }, weight, rank);
-            top = top << 8 | bin;
-        }
-        return (int)top;
-    };
-    auto cut_at = [&](const FiltCut& kept, auto weight, uint64_t rank) {
-        uint32_t prefix = 0, mask = 0;
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            const uint32_t bin = pass([&](int i, uint32_t k) { return (k & mask) == prefix && kept.keeps(k, i); },
-                                      [&](int, uint32_t k) { return 255 - (k >> shift & 255); }, weight, rank);
-            prefix |= (255 - bin) << shift;
-            mask |= 255u << shift;
-        }
-        return FiltCut{prefix, by_id([&](int i, uint32_t k) { return k == prefix && kept.keeps(k, i); }, weight, rank)};
-    };
-    auto mass = [&](float l) { return filt_mass(a, l, m); };
-    auto total = [&](const FiltCut& kept) {
-        uint64_t sum = 0, all;
-        each([&](int i, float l) { sum += kept.keeps(filt_key(l), i) ? mass(l) : 0ull; });
-        filt_scan(sum, s, &all);
-        return all;
-    };
-    FiltCut kept{0u, a.V};
-    if (a.top_k < a.V) kept = cut_at(kept, [](float) { return 1ull; }, (uint64_t)a.top_k - 1);
-    uint64_t M = total(kept);
-    if (a.top_p < 1.0f) {
-        kept = cut_at(kept, mass, filt_need(a.top_p, M) - 1);
-        M = total(kept);
+        lo = least + (bin << shift), hi = lo + ((1u << shift) - 1);
+        __syncthreads();
     }
-    return by_id([&](int i, uint32_t k) { return kept.keeps(k, i); }, mass, filt_draw(u, M));
 }
 
-// Sorts v[0, N), N a power of two, ascending.
-__device__ __forceinline__ void filt_sort(unsigned long long* v, int N) {
-    for (int k = 2; k <= N; k *= 2)
-        for (int j = k / 2; j > 0; j /= 2) {
-            __syncthreads();
-            for (int t = threadIdx.x; t < N / 2; t += kFiltThreads) {
-                const int lo = (t & ~(j - 1)) * 2 | (t & (j - 1)), hi = lo | j;
-                const unsigned long long x = v[lo], y = v[hi];
-                if ((x > y) == ((lo & k) == 0)) v[lo] = y, v[hi] = x;
+// K, N and the draw over a source of (id, key, mass), each(f).
+template <typename Each>
+__device__ __forceinline__ int filt_choose(const FiltArgs& a, float u, FiltShared& s, Each each) {
+    FiltCut kept{0u, a.V};
+    if (a.top_k < a.V)
+        kept = filt_pick(false, (uint64_t)a.top_k - 1, s, [&](auto f) { each([&](int i, uint32_t k, uint64_t) { f(i, k, 1ull); }); });
+    auto left = [&](auto f) { each([&](int i, uint32_t k, uint64_t w) { f(i, k, kept.keeps(k, i) ? w : 0ull); }); };
+    auto total = [&]() {
+        uint64_t sum = 0;
+        left([&](int, uint32_t, uint64_t w) { sum += w; });
+        return filt_sum(sum, s);
+    };
+    uint64_t M = total();
+    if (a.top_p < 1.0f) {
+        kept = filt_pick(false, filt_need(a.top_p, M) - 1, s, left);
+        M = total();
+    }
+    return filt_pick(true, filt_draw(u, M), s, left).id;
+}
+
+// The same over the row itself: for what fits nowhere.
+template <bool BF16>
+__device__ __noinline__ int filt_choose_row(const FiltArgs& a, const void* row, float m, float u, FiltShared& s) {
+    return filt_choose(a, u, s, [&](auto f) {
+        filt_tiles<BF16>(row, 0, a.V, [&](int, int i, const auto& l, int n) {
+            constexpr int E = BF16 ? 8 : 4;
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                if (e < n) f(i + e, filt_key(l[e]), filt_mass(a, l[e], m));
+        });
+    });
+}
+
+constexpr int kFiltPer = kFiltCountBins / kFiltThreads;
+// A thread's 16 bins of a count histogram in LDS lie side by side, with a word between the threads'.
+__device__ __forceinline__ int filt_slot(int bin) { return bin + bin / kFiltPer; }
+constexpr int kFiltSlots = kFiltCountBins + kFiltThreads;
+
+// The bin that holds the top_k-th logit; the thread has the counts of bins high, high - 1, ... .
+__device__ __forceinline__ int filt_count_cut(const FiltArgs& a, const uint32_t (&c)[kFiltPer], int high, FiltShared& s) {
+    uint32_t own = 0;
+#pragma unroll
+    for (int i = 0; i < kFiltPer; ++i) own += c[i];
+    uint64_t all, excl = filt_scan(own, s, &all);
+    const uint64_t rank = (uint64_t)a.top_k - 1;
+    if (excl <= rank && rank - excl < own) {
+        int at = 0;
+#pragma unroll
+        for (int i = 0; i < kFiltPer; ++i) {
+            if (excl <= rank) at = high - i;
+            excl += c[i];
+        }
+        s.sel[0] = at;
+    }
+    __syncthreads();
+    return (int)s.sel[0];
+}
+
+// The bin in which N ends; the thread has the masses of four bins. *above: the mass of the bins before
+// it, *W: of all.
+__device__ __forceinline__ int filt_mass_cut(const FiltArgs& a, const uint64_t (&h)[4], FiltShared& s, uint64_t* above, uint64_t* W) {
+    uint64_t excl = filt_scan(h[0] + h[1] + h[2] + h[3], s, W);
+    const uint64_t rank = filt_need(a.top_p, *W) - 1;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (excl <= rank && rank - excl < h[i]) s.sel[0] = threadIdx.x * 4 + i, s.sel[1] = excl;
+        excl += h[i];
+    }
+    __syncthreads();
+    *above = s.sel[1];
+    return (int)s.sel[0];
+}
+
+// Shared memory of the last step: the list with its masses, and the tiles' masses.
+struct FiltLast {
+    unsigned long long list[kFiltHeld];
+    unsigned long long mass[kFiltHeld];
+    unsigned long long tile[kFiltTiles];
+    uint32_t count, base;
+};
+
+// A block's part of the last step: top-k: ids of bins >= bin are listed; top-p: masses of bins < bin by
+// tile, ids of `bin` are listed; neither: masses by tile. Tiles count from the block's first.
+template <bool BF16, int MODE>
+__device__ __forceinline__ void filt_gather(const FiltArgs& a, const void* row, int first, int end, float m, int bin, FiltLast& z) {
+    constexpr int E = BF16 ? 8 : 4;
+    auto enlist = [&](int i, float l) {
+        const uint32_t at = atomicAdd(&z.count, 1u);
+        if (at < kFiltHeld) z.list[at] = (unsigned long long)filt_key(l) << 32 | (uint32_t)i;
+    };
+    filt_tiles<BF16>(row, first, end, [&](int t, int i, const float (&l)[E], int n) {
+        uint64_t y = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            if constexpr (MODE == kFiltTopK) {
+                if (e < n && (int)(filt_key(l[e]) >> kFiltCountShift) >= bin) enlist(i + e, l[e]);
+            } else if constexpr (MODE == kFiltTopP) {
+                const int b = filt_bin(a, l[e], m);
+                if (b < bin) y += filt_mass(a, l[e], m);
+                else if (b == bin && e < n) enlist(i + e, l[e]);
+            } else {
+                y += filt_mass(a, l[e], m);   // there is none past the end: -inf
             }
         }
+        if (MODE != kFiltTopK && __any(y != 0)) {
+            y = filt_last_lane(filt_wave_scan(y));
+            if (threadIdx.x % kWave == 0) atomicAdd(&z.tile[t], (unsigned long long)y);
+        }
+    });
+}
+
+// The choice from a row's list (`count` entries, in z or in `list`) and its tiles' masses (in z.tile).
+template <bool BF16, int MODE>
+__device__ __forceinline__ int filt_last(const FiltArgs& a, const void* row, float m, float u, uint64_t above, uint64_t W, uint32_t count,
+                                         const unsigned long long* list, FiltShared& s, FiltLast& z) {
+    const int tid = threadIdx.x;
+    if (m == -INFINITY) return -1;
+    if (count > (list != nullptr && MODE == kFiltTopK ? kFiltList : kFiltHeld)) return filt_choose_row<BF16>(a, row, m, u, s);
+    if (MODE == kFiltTopK && count > kFiltHeld)
+        return filt_choose(a, u, s, [&](auto f) {
+            for (uint32_t i = tid; i < count; i += kFiltThreads) {
+                const unsigned long long x = __hip_atomic_load(&list[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                f((int)(uint32_t)x, (uint32_t)(x >> 32), filt_mass(a, filt_logit((uint32_t)(x >> 32)), m));
+            }
+        });
+    for (uint32_t i = tid; i < count; i += kFiltThreads) {
+        const unsigned long long x = list != nullptr ? __hip_atomic_load(&list[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : z.list[i];
+        z.list[i] = x;
+        z.mass[i] = filt_mass(a, filt_logit((uint32_t)(x >> 32)), m);
+    }
     __syncthreads();
+    auto each = [&](auto f) {
+        for (uint32_t i = tid; i < count; i += kFiltThreads) f((int)(uint32_t)z.list[i], (uint32_t)(z.list[i] >> 32), (uint64_t)z.mass[i]);
+    };
+    if constexpr (MODE == kFiltTopK) return filt_choose(a, u, s, each);
+    constexpr int E = BF16 ? 8 : 4, TILE = E * kFiltThreads;
+    FiltCut kept{0u, a.V};
+    if constexpr (MODE == kFiltTopP) {
+        kept = filt_pick(false, filt_need(a.top_p, W) - 1 - above, s, each);
+        each([&](int i, uint32_t k, uint64_t w) {
+            if (w != 0 && kept.keeps(k, i)) atomicAdd(&z.tile[i / TILE], (unsigned long long)w);
+        });
+        __syncthreads();
+    }
+    uint64_t own = 0, M, h[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) own += h[i] = z.tile[tid * 4 + i];
+    uint64_t excl = filt_scan(own, s, &M);
+    const uint64_t r = filt_draw(u, M);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (excl <= r && r - excl < h[i]) s.sel[0] = tid * 4 + i, s.sel[1] = excl;
+        excl += h[i];
+    }
+    __syncthreads();
+    const int t = (int)s.sel[0];
+    const uint64_t rest = r - s.sel[1];
+    filt_tiles<BF16>(row, t * TILE, min(t * TILE + TILE, a.V), [&](int, int i, const float (&l)[E], int) {
+        uint64_t y[E], sum = 0, all;
+#pragma unroll
+        for (int e = 0; e < E; ++e) sum += y[e] = kept.keeps(filt_key(l[e]), i + e) ? filt_mass(a, l[e], m) : 0ull;
+        uint64_t at = filt_scan(sum, s, &all);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            if (at <= rest && rest - at < y[e]) s.found[0] = i + e;
+            at += y[e];
+        }
+    });
+    __syncthreads();
+    return (int)s.found[0];
+}
+
+template <bool BF16>
+__device__ __forceinline__ const char* filt_row(const FiltArgs& a, unsigned r) {
+    return static_cast<const char*>(a.logits) + (int64_t)r * a.stride * (BF16 ? 2 : 4);
 }
 
 // 1. Block maxima; top-k: a histogram of counts, of which a block adds the bins that its own first
 // top_k logits reach (lower ones cannot be among the row's).
 template <bool BF16, int MODE>
 __global__ __launch_bounds__(kFiltThreads) void filt_max_kernel(FiltArgs a) {
+    constexpr int E = BF16 ? 8 : 4;
     __shared__ FiltShared s;
-    __shared__ uint32_t bins[MODE == kFiltTopK ? kFiltCountBins : 1];
-    constexpr int PER = kFiltCountBins / kFiltThreads;
+    __shared__ uint32_t bins[MODE == kFiltTopK ? kFiltSlots : 1];
     const int tid = threadIdx.x, block = blockIdx.x;
     FiltRow& w = a.ws[blockIdx.y];
-    const char* const row = static_cast<const char*>(a.logits) + (int64_t)blockIdx.y * a.stride * (BF16 ? 2 : 4);
     const int first = block * a.chunk, end = min(first + a.chunk, a.V);
     if constexpr (MODE == kFiltTopK) {
-        for (int i = tid; i < kFiltCountBins; i += kFiltThreads) bins[i] = 0;
+        for (int i = tid; i < kFiltSlots; i += kFiltThreads) bins[i] = 0;
         __syncthreads();
     }
     float m = -INFINITY;
-    filt_each<BF16>(row, first, end, [&](int, float l) {
-        m = fmaxf(m, l);
-        if constexpr (MODE == kFiltTopK) atomicAdd(&bins[filt_key(l) >> kFiltCountShift], 1u);
+    filt_tiles<BF16>(filt_row<BF16>(a, blockIdx.y), first, end, [&](int, int, const float (&l)[E], int n) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            m = fmaxf(m, l[e]);
+            if (MODE == kFiltTopK && e < n) atomicAdd(&bins[filt_slot(filt_key(l[e]) >> kFiltCountShift)], 1u);
+        }
     });
     m = filt_max(m, s);   // the counts are whole behind its barrier
     if (tid == 0) w.bmax[block] = m;
     if constexpr (MODE == kFiltTopK) {
-        const int high = kFiltCountBins - 1 - tid * PER;   // the thread's bins, from the highest
-        uint32_t own = 0;
+        const int high = kFiltCountBins - 1 - tid * kFiltPer;   // the thread's bins, from the highest
+        uint32_t c[kFiltPer], own = 0;
 #pragma unroll
-        for (int i = 0; i < PER; ++i) own += bins[high - i];
+        for (int i = 0; i < kFiltPer; ++i) own += c[i] = bins[filt_slot(high - i)];
         uint64_t all;
         uint64_t above = filt_scan(own, s, &all);
 #pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const uint32_t c = bins[high - i];
-            if (c != 0 && above < (uint64_t)a.top_k)
-                __hip_atomic_fetch_add(&w.hist.count[high - i], c, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            above += c;
+        for (int i = 0; i < kFiltPer; ++i) {
+            if (c[i] != 0 && above < (uint64_t)a.top_k)
+                __hip_atomic_fetch_add(&w.hist.count[high - i], c[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            above += c[i];
         }
     }
 }
@@ -344,6 +535,18 @@ __device__ __forceinline__ float filt_row_max(const FiltArgs& a, const FiltRow& 
     return filt_max(threadIdx.x < a.blocks ? w.bmax[threadIdx.x] : -INFINITY, s);
 }
 
+template <bool BF16>
+__device__ __forceinline__ void filt_mass_bins(const FiltArgs& a, const void* row, int first, int end, float m, unsigned long long* bins) {
+    constexpr int E = BF16 ? 8 : 4;
+    filt_tiles<BF16>(row, first, end, [&](int, int, const float (&l)[E], int) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const uint64_t x = filt_mass(a, l[e], m);
+            if (x != 0) atomicAdd(&bins[filt_bin(a, l[e], m)], (unsigned long long)x);
+        }
+    });
+}
+
 // 2. top-p: masses by bin.
 template <bool BF16>
 __global__ __launch_bounds__(kFiltThreads) void filt_mass_kernel(FiltArgs a) {
@@ -351,14 +554,9 @@ __global__ __launch_bounds__(kFiltThreads) void filt_mass_kernel(FiltArgs a) {
     __shared__ unsigned long long bins[kFiltMassBins];
     const int tid = threadIdx.x, first = blockIdx.x * a.chunk, end = min(first + a.chunk, a.V);
     FiltRow& w = a.ws[blockIdx.y];
-    const char* const row = static_cast<const char*>(a.logits) + (int64_t)blockIdx.y * a.stride * (BF16 ? 2 : 4);
     for (int i = tid; i < kFiltMassBins; i += kFiltThreads) bins[i] = 0;
     const float m = filt_row_max(a, w, s);
-    __syncthreads();
-    filt_each<BF16>(row, first, end, [&](int, float l) {
-        const uint64_t x = filt_mass(a, l, m);
-        if (x != 0) atomicAdd(&bins[filt_bin(a, l, m)], (unsigned long long)x);
-    });
+    filt_mass_bins<BF16>(a, filt_row<BF16>(a, blockIdx.y), first, end, m, bins);
     __syncthreads();
     for (int i = tid; i < kFiltMassBins; i += kFiltThreads)
         if (bins[i] != 0) __hip_atomic_fetch_add(&w.hist.mass[i], bins[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -368,99 +566,51 @@ __global__ __launch_bounds__(kFiltThreads) void filt_mass_kernel(FiltArgs a) {
 // stores that have returned before the block counts in, and agent-scope loads.
 template <bool BF16, int MODE>
 __global__ __launch_bounds__(kFiltThreads) void filt_draw_kernel(FiltArgs a) {
+    constexpr int TILE = (BF16 ? 8 : 4) * kFiltThreads;
     __shared__ FiltShared s;
-    __shared__ unsigned long long buf[kFiltSort];   // the block's part of the list, then the row's list
-    __shared__ unsigned long long sums[kFiltBlocks];
-    __shared__ uint32_t s_count, s_base;
-    const int tid = threadIdx.x, block = blockIdx.x;
+    __shared__ FiltLast z;
+    const int tid = threadIdx.x;
     FiltRow& w = a.ws[blockIdx.y];
-    const char* const row = static_cast<const char*>(a.logits) + (int64_t)blockIdx.y * a.stride * (BF16 ? 2 : 4);
-    const int first = block * a.chunk, end = min(first + a.chunk, a.V);
-    if (tid == 0) s_count = 0;
-    const float m = filt_row_max(a, w, s);
+    const char* const row = filt_row<BF16>(a, blockIdx.y);
+    const int first = blockIdx.x * a.chunk, end = min(first + a.chunk, a.V), tiles = (end - first + TILE - 1) / TILE;
+    if (tid == 0) z.count = 0;
+    if constexpr (MODE != kFiltTopK)
+        for (int i = tid; i < tiles; i += kFiltThreads) z.tile[i] = 0;
     // where K or N ends: the bin, and what lies above it
     int bin = 0;
     uint64_t above = 0, W = 0;
+    uint32_t c[kFiltPer];
+    uint64_t h[4];
+    const int high = kFiltCountBins - 1 - tid * kFiltPer;
     if constexpr (MODE == kFiltTopK) {
-        constexpr int PER = kFiltCountBins / kFiltThreads;
-        const int high = kFiltCountBins - 1 - tid * PER;
-        uint32_t c[PER], own = 0;
 #pragma unroll
-        for (int i = 0; i < PER; i += 4) {
+        for (int i = 0; i < kFiltPer; i += 4) {
             const uint4 x = *reinterpret_cast<const uint4*>(&w.hist.count[high - i - 3]);
             c[i] = x.w, c[i + 1] = x.z, c[i + 2] = x.y, c[i + 3] = x.x;
         }
-#pragma unroll
-        for (int i = 0; i < PER; ++i) own += c[i];
-        uint64_t all, excl = filt_scan(own, s, &all);
-        const uint64_t rank = (uint64_t)a.top_k - 1;
-        if (excl <= rank && rank - excl < own) {
-            int at = 0;
-#pragma unroll
-            for (int i = 0; i < PER; ++i) {
-                if (excl <= rank) at = high - i;
-                excl += c[i];
-            }
-            s.sel[0] = at;
-        }
-        __syncthreads();
-        bin = (int)s.sel[0];
     }
     if constexpr (MODE == kFiltTopP) {
-        constexpr int PER = kFiltMassBins / kFiltThreads;
-        uint64_t h[PER], own = 0;
 #pragma unroll
-        for (int i = 0; i < PER; ++i) own += h[i] = w.hist.mass[tid * PER + i];
-        uint64_t excl = filt_scan(own, s, &W);
-        const uint64_t rank = filt_need(a.top_p, W) - 1;
-        if (excl <= rank && rank - excl < own) {
-#pragma unroll
-            for (int i = 0; i < PER; ++i) {
-                if (excl <= rank) s.sel[0] = tid * PER + i, s.sel[1] = excl;
-                excl += h[i];
-            }
-        }
-        __syncthreads();
-        bin = (int)s.sel[0], above = s.sel[1];
+        for (int i = 0; i < 4; ++i) h[i] = w.hist.mass[tid * 4 + i];
     }
-    __syncthreads();
-    uint64_t mine = 0;
-    auto enlist = [&](int i, uint32_t key) {
-        const unsigned long long x = (unsigned long long)~key << 32 | (uint32_t)i;
-        const uint32_t at = atomicAdd(&s_count, 1u);
-        if (at < kFiltSort) buf[at] = x;
-    };
-    if (m > -INFINITY)
-        filt_each<BF16>(row, first, end, [&](int i, float l) {
-            if constexpr (MODE == kFiltTopK) {
-                const uint32_t k = filt_key(l);
-                if ((int)(k >> kFiltCountShift) >= bin) enlist(i, k);
-            } else if constexpr (MODE == kFiltTopP) {
-                const int b = filt_bin(a, l, m);
-                if (b < bin) mine += filt_mass(a, l, m);
-                else if (b == bin) enlist(i, filt_key(l));
-            } else {
-                mine += filt_mass(a, l, m);
-            }
-        });
-    if constexpr (MODE != kFiltTopK) {
-        uint64_t all;
-        filt_scan(mine, s, &all);
-        mine = all;
-    }
+    const float m = filt_row_max(a, w, s);
+    if constexpr (MODE == kFiltTopK) bin = filt_count_cut(a, c, high, s);
+    if constexpr (MODE == kFiltTopP) bin = filt_mass_cut(a, h, s, &above, &W);
+    if (m > -INFINITY) filt_gather<BF16, MODE>(a, row, first, end, m, bin, z);
     __syncthreads();
     if constexpr (MODE != kFiltAll) {
-        const uint32_t n = s_count;
-        if (tid == 0 && n != 0) {
-            // a block whose part does not fit makes the row's list overflow
-            s_base = __hip_atomic_fetch_add(&w.count, n <= kFiltSort ? n : (uint32_t)kFiltList + 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        }
+        const uint32_t n = z.count;
+        // a block whose part does not fit makes the row's list overflow
+        if (tid == 0 && n != 0)
+            z.base = __hip_atomic_fetch_add(&w.count, n <= kFiltHeld ? n : (uint32_t)kFiltList + 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         __syncthreads();
-        if (n <= kFiltSort)
+        if (n <= kFiltHeld)
             for (uint32_t i = tid; i < n; i += kFiltThreads)
-                if (s_base + i < kFiltList) __hip_atomic_store(&w.list[s_base + i], buf[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                if (z.base + i < kFiltList) __hip_atomic_store(&w.list[z.base + i], z.list[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
-    if (MODE != kFiltTopK && tid == 0) __hip_atomic_store(&w.bmass[block], mine, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if constexpr (MODE != kFiltTopK)
+        for (int i = tid; i < tiles; i += kFiltThreads)
+            __hip_atomic_store(&w.tile[first / TILE + i], z.tile[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     if (tid == 0)
@@ -471,201 +621,99 @@ __global__ __launch_bounds__(kFiltThreads) void filt_draw_kernel(FiltArgs a) {
     // ---- the row's last workgroup
     const float u = a.u[blockIdx.y];
     const uint32_t count = MODE == kFiltAll ? 0u : __hip_atomic_load(&w.count, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if constexpr (MODE != kFiltTopK) {
+        const int all = (a.V + TILE - 1) / TILE;
+#pragma unroll
+        for (int i = 0; i < kFiltTiles / kFiltThreads; ++i) {
+            const int t = i * kFiltThreads + tid;
+            z.tile[t] = t < all ? __hip_atomic_load(&w.tile[t], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0ull;
+        }
+    }
     __syncthreads();
     if (tid == 0) w.counter = 0, w.count = 0;
     if constexpr (MODE == kFiltTopK)
         for (int i = tid; i < kFiltCountBins; i += kFiltThreads) w.hist.count[i] = 0;
     if constexpr (MODE == kFiltTopP)
         for (int i = tid; i < kFiltMassBins; i += kFiltThreads) w.hist.mass[i] = 0;
-    if (m == -INFINITY) {
-        if (tid == 0) a.out[blockIdx.y] = -1;
-        return;
-    }
-    if (count > kFiltSort) {
-        int token;
-        if (MODE == kFiltTopK && count <= kFiltList)
-            token = filt_select(a, m, u, s, [&](auto f) {
-                for (uint32_t i = tid; i < count; i += kFiltThreads) {
-                    const unsigned long long x = __hip_atomic_load(&w.list[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                    f((int)(uint32_t)x, filt_logit(~(uint32_t)(x >> 32)));
-                }
-            });
-        else
-            token = filt_select(a, m, u, s, [&](auto f) { filt_each<BF16>(row, 0, a.V, f); });
-        if (tid == 0) a.out[blockIdx.y] = token;
-        return;
-    }
-    // the list in the sampler's order; a thread has PER neighbours of it
-    constexpr int PER = kFiltSort / kFiltThreads;
-    uint64_t x[PER];
-    uint64_t mass[PER];
-    int N = 0;
-    if constexpr (MODE != kFiltAll) {
-        N = 2;
-        while (N < (int)count) N *= 2;
-        for (int i = tid; i < N; i += kFiltThreads)
-            buf[i] = i < (int)count ? __hip_atomic_load(&w.list[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : ~0ull;
-        filt_sort(buf, N);
-        uint64_t own = 0;
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const int at = tid * PER + i;
-            x[i] = at < N ? buf[at] : ~0ull;
-            mass[i] = 0;
-            if (at < (int)count && (MODE == kFiltTopP || at < a.top_k)) mass[i] = filt_mass(a, filt_logit(~(uint32_t)(x[i] >> 32)), m);
-            own += mass[i];
-        }
-        if (MODE == kFiltTopP || a.top_p < 1.0f) {
-            uint64_t all, before = filt_scan(own, s, &all);
-            const uint64_t need = MODE == kFiltTopP ? filt_need(a.top_p, W) - above : filt_need(a.top_p, all);
-#pragma unroll
-            for (int i = 0; i < PER; ++i) {
-                const uint64_t y = mass[i];
-                if (before >= need) mass[i] = 0;
-                before += y;
-            }
-        }
-    }
-    if constexpr (MODE == kFiltTopK) {
-        // the draw, in the order of ids: masses join their ids
-        __syncthreads();
-        uint64_t own = 0, M;
-#pragma unroll
-        for (int i = 0; i < PER; ++i) own += mass[i];
-        filt_scan(own, s, &M);
-        const uint64_t r = filt_draw(u, M);
-        // ids of kept ones with their places, sorted by id
-        __shared__ unsigned long long masses[kFiltSort];
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const int at = tid * PER + i;
-            if (at < N) buf[at] = mass[i] != 0 ? (x[i] & 0xffffffffull) << 32 | (uint32_t)at : ~0ull, masses[at] = mass[i];
-        }
-        filt_sort(buf, N);
-        own = 0;
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const int at = tid * PER + i;
-            x[i] = at < N ? buf[at] : ~0ull;
-            mass[i] = x[i] != ~0ull ? masses[(uint32_t)x[i]] : 0ull;
-            own += mass[i];
-        }
-        uint64_t excl = filt_scan(own, s, &M);
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            if (excl <= r && r - excl < mass[i]) a.out[blockIdx.y] = (int32_t)(x[i] >> 32);
-            excl += mass[i];
-        }
-    } else {
-        // masses of the blocks, and of the list's kept ids in theirs
-        FiltCut kept{0u, a.V};
-        __syncthreads();
-        if (tid < kFiltBlocks)
-            sums[tid] = tid < a.blocks ? __hip_atomic_load(&w.bmass[tid], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0ull;
-        __syncthreads();
-        if constexpr (MODE == kFiltTopP) {
-            // the last that is kept: its successor is not
-            unsigned long long last = 0;
-#pragma unroll
-            for (int i = 0; i < PER; ++i)
-                if (mass[i] != 0) {
-                    atomicAdd(&sums[(uint32_t)x[i] / (uint32_t)a.chunk], (unsigned long long)mass[i]);
-                    last = x[i];   // neighbours ascend
-                }
-            if (tid == 0) s.sel[0] = 0;
-            __syncthreads();
-            if (last != 0) atomicMax(&s.sel[0], last);
-            __syncthreads();
-            last = s.sel[0];
-            kept = FiltCut{~(uint32_t)(last >> 32), (int)(uint32_t)last};
-            __syncthreads();
-        }
-        uint64_t before, M;
-        const uint64_t own = tid < kFiltBlocks ? sums[tid] : 0ull;
-        filt_scan(own, s, &M);
-        uint64_t r = filt_draw(u, M);
-        const int b = filt_find(own, r, s, &before);
-        r -= before;
-        // the block's tiles of 256 vectors, then the id
-        constexpr int TILE = kFiltThreads * (BF16 ? 8 : 4);
-        const int b0 = b * a.chunk, b1 = min(b0 + a.chunk, a.V);
-        auto weigh = [&](int i, float l) { return kept.keeps(filt_key(l), i) ? filt_mass(a, l, m) : 0ull; };
-        __syncthreads();
-        s.bins[tid] = 0;
-        __syncthreads();
-        filt_each<BF16>(row, b0, b1, [&](int i, float l) {
-            const uint64_t y = weigh(i, l);
-            if (y != 0) atomicAdd(&s.bins[(i - b0) / TILE], (unsigned long long)y);
-        });
-        __syncthreads();
-        const int t = filt_find(s.bins[tid], r, s, &before);
-        r -= before;
-        const int t0 = b0 + t * TILE;
-        constexpr int E = TILE / kFiltThreads;
-        uint64_t y[E], sum = 0;
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const int i = t0 + tid * E + e;
-            y[e] = 0;
-            if (i < b1) {
-                float l;
-                if constexpr (BF16) l = bf16_to_f32(reinterpret_cast<const uint16_t*>(row)[i]);
-                else l = reinterpret_cast<const float*>(row)[i];
-                y[e] = weigh(i, filt_clean(l));
-            }
-            sum += y[e];
-        }
-        uint64_t excl = filt_scan(sum, s, &M);
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            if (excl <= r && r - excl < y[e]) a.out[blockIdx.y] = t0 + tid * E + e;
-            excl += y[e];
-        }
-    }
+    const int token = filt_last<BF16, MODE>(a, row, m, u, above, W, count, w.list, s, z);
+    if (tid == 0) a.out[blockIdx.y] = token;
 }
 
-// Small vocabularies: a workgroup a row, the row in LDS.
-template <bool BF16>
-__global__ __launch_bounds__(kFiltThreads) void filt_row_kernel(FiltArgs a) {
+// Small vocabularies: all steps in one launch, a workgroup a row.
+template <bool BF16, int MODE>
+__global__ __launch_bounds__(kFiltThreads) void filt_one_kernel(FiltArgs a) {
+    constexpr int E = BF16 ? 8 : 4;
     __shared__ FiltShared s;
-    extern __shared__ float held[];
+    __shared__ FiltLast z;
+    __shared__ uint32_t counts[MODE == kFiltTopK ? kFiltSlots : 1];
+    __shared__ unsigned long long masses[MODE == kFiltTopP ? kFiltMassBins : 1];
     const int tid = threadIdx.x;
-    const char* const row = static_cast<const char*>(a.logits) + (int64_t)blockIdx.x * a.stride * (BF16 ? 2 : 4);
+    const char* const row = filt_row<BF16>(a, blockIdx.x);
+    if (tid == 0) z.count = 0;
+    for (int i = tid; i < kFiltTiles; i += kFiltThreads) z.tile[i] = 0;
+    if constexpr (MODE == kFiltTopK) {
+        for (int i = tid; i < kFiltSlots; i += kFiltThreads) counts[i] = 0;
+        __syncthreads();
+    }
+    if constexpr (MODE == kFiltTopP)
+        for (int i = tid; i < kFiltMassBins; i += kFiltThreads) masses[i] = 0;
     float m = -INFINITY;
-    filt_each<BF16>(row, 0, a.V, [&](int i, float l) { m = fmaxf(m, l), held[i] = l; });
+    filt_tiles<BF16>(row, 0, a.V, [&](int, int, const float (&l)[E], int n) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            m = fmaxf(m, l[e]);
+            if (MODE == kFiltTopK && e < n) atomicAdd(&counts[filt_slot(filt_key(l[e]) >> kFiltCountShift)], 1u);
+        }
+    });
     m = filt_max(m, s);
-    int token = -1;
-    if (m > -INFINITY)
-        token = filt_select(a, m, a.u[blockIdx.x], s, [&](auto f) {
-            for (int i = tid; i < a.V; i += kFiltThreads) f(i, held[i]);
-        });
+    int bin = 0;
+    uint64_t above = 0, W = 0;
+    if constexpr (MODE == kFiltTopK) {
+        const int high = kFiltCountBins - 1 - tid * kFiltPer;
+        uint32_t c[kFiltPer];
+#pragma unroll
+        for (int i = 0; i < kFiltPer; ++i) c[i] = counts[filt_slot(high - i)];
+        bin = filt_count_cut(a, c, high, s);
+    }
+    if constexpr (MODE == kFiltTopP) {
+        filt_mass_bins<BF16>(a, row, 0, a.V, m, masses);
+        __syncthreads();
+        uint64_t h[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) h[i] = masses[tid * 4 + i];
+        bin = filt_mass_cut(a, h, s, &above, &W);
+    }
+    if (m > -INFINITY) filt_gather<BF16, MODE>(a, row, 0, a.V, m, bin, z);
+    __syncthreads();
+    const int token = filt_last<BF16, MODE>(a, row, m, a.u[blockIdx.x], above, W, z.count, nullptr, s, z);
     if (tid == 0) a.out[blockIdx.x] = token;
 }
 
-// Blocks of a row: some four workgroups a CU in all, blocks of whole passes of a workgroup's loads.
+// Blocks of a row: some four workgroups a CU in all, blocks of whole tiles.
 static void filt_split(int64_t rows, int64_t vocab, int* blocks, int* chunk) {
     const int64_t want = std::min<int64_t>(kFiltBlocks, std::max<int64_t>(1, (4 * prefill_cus() + rows - 1) / rows));
-    int64_t c = std::min<int64_t>((vocab + want - 1) / want, kFiltMaxTiles * kFiltThreads * 4 - 2047);
-    c = (c + 2047) / 2048 * 2048;
+    const int64_t c = ((vocab + want - 1) / want + 2047) / 2048 * 2048;
     *chunk = (int)c;
     *blocks = (int)((vocab + c - 1) / c);
 }
 
 template <bool BF16>
 static void filt_launch(const FiltArgs& a, int64_t rows, hipStream_t stream) {
-    const dim3 t(kFiltThreads);
+    const dim3 t(kFiltThreads), grid(a.blocks, (unsigned)rows), one((unsigned)rows);
+    const bool k = a.top_k < a.V, p = a.top_p < 1.0f;
     if (a.ws == nullptr) {
-        hipLaunchKernelGGL(filt_row_kernel<BF16>, dim3((unsigned)rows), t, (unsigned)a.V * sizeof(float), stream, a);
+        if (k) hipLaunchKernelGGL((filt_one_kernel<BF16, kFiltTopK>), one, t, 0, stream, a);
+        else if (p) hipLaunchKernelGGL((filt_one_kernel<BF16, kFiltTopP>), one, t, 0, stream, a);
+        else hipLaunchKernelGGL((filt_one_kernel<BF16, kFiltAll>), one, t, 0, stream, a);
         return;
     }
-    const dim3 grid(a.blocks, (unsigned)rows);
-    if (a.top_k < a.V) {
+    if (k) {
         hipLaunchKernelGGL((filt_max_kernel<BF16, kFiltTopK>), grid, t, 0, stream, a);
         hipLaunchKernelGGL((filt_draw_kernel<BF16, kFiltTopK>), grid, t, 0, stream, a);
         return;
     }
     hipLaunchKernelGGL((filt_max_kernel<BF16, kFiltAll>), grid, t, 0, stream, a);
-    if (a.top_p < 1.0f) {
+    if (p) {
         hipLaunchKernelGGL(filt_mass_kernel<BF16>, grid, t, 0, stream, a);
         hipLaunchKernelGGL((filt_draw_kernel<BF16, kFiltTopP>), grid, t, 0, stream, a);
     } else {
@@ -678,7 +726,7 @@ static void filt_launch(const FiltArgs& a, int64_t rows, hipStream_t stream) {
 using namespace efm;
 
 extern "C" size_t efm_sampler_filtered_workspace_bytes(int64_t rows, int64_t vocab) {
-    return rows <= 0 || vocab <= kFiltLdsVocab ? 0 : (size_t)rows * sizeof(FiltRow);
+    return rows <= 0 || vocab <= kFiltOneVocab ? 0 : (size_t)rows * sizeof(FiltRow);
 }
 
 extern "C" int efm_sampler_filtered(int64_t rows, int64_t vocab, const void* logits, int32_t logits_dtype, int64_t logits_stride,

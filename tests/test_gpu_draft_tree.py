@@ -360,7 +360,7 @@ def test_sampler(gpu, f, rows, vocab, dtype):
 
 @pytest.mark.parametrize("f", [dict(), dict(k=50, p=0.9), dict(p=0.95), dict(min_p=0.03)], ids=str)
 @pytest.mark.parametrize("rows,vocab", [(1, 1), (4, 2), (3, 63), (2, 65), (9, 1023), (9, 1025), (2, 32768), (2, 32769), (2, (1 << 20) - 1),
-                                        (260, 40000), (600, 700), (1100, 15000), (3, 14336), (3, 14337), (1500, 20000)])
+                                        (260, 40000), (600, 700), (1100, 15000), (3, 16384), (3, 16385), (1500, 20000)])
 def test_sampler_sizes(gpu, f, rows, vocab):
     for dtype in (torch.float32, torch.bfloat16):
         x, u = _logits(vocab, rows, vocab, dtype)
