@@ -117,7 +117,8 @@ __device__ __forceinline__ float filt_logit(uint32_t key) { return __uint_as_flo
 __device__ __forceinline__ float filt_clean(float l) { return l == l ? l : -INFINITY; }
 
 // A row's logits [first, end), first a multiple of a tile: f(tile of the range, first id, the thread's
-// E logits, how many of them there are), by all threads together; 16 bytes a thread, four under way.
+// E logits as they are (-inf past the end), how many of them there are), by all threads together; 16
+// bytes a thread, four under way.
 template <bool BF16, typename F>
 __device__ __forceinline__ void filt_tiles(const void* row, int first, int end, F f) {
     constexpr int E = BF16 ? 8 : 4, U = 4, TILE = E * kFiltThreads;
@@ -152,8 +153,8 @@ __device__ __forceinline__ void filt_tiles(const void* row, int first, int end, 
             const uint32_t w[4] = {x[j].x, x[j].y, x[j].z, x[j].w};
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                if constexpr (BF16) l[2 * e] = filt_clean(lo_f32(w[e])), l[2 * e + 1] = filt_clean(hi_f32(w[e]));
-                else l[e] = filt_clean(__uint_as_float(w[e]));
+                if constexpr (BF16) l[2 * e] = lo_f32(w[e]), l[2 * e + 1] = hi_f32(w[e]);
+                else l[e] = __uint_as_float(w[e]);
             }
             f(t0 + j, i, l, min(max(end - i, 0), E));
         }
@@ -189,10 +190,10 @@ __device__ __forceinline__ uint64_t filt_last_lane(uint64_t v) {
 struct FiltShared {
     unsigned long long red[kFiltWaves];
     unsigned long long sel[2];
-    unsigned long long bins[kFiltThreads];
+    unsigned long long bins[2][kFiltThreads];
+    uint32_t counts[2][kFiltThreads];
     float redf[kFiltWaves];
-    uint32_t range[kFiltWaves][3];
-    uint32_t flag, found[2];
+    uint32_t flag, found[3];
 };
 
 // Sum of the values of the threads before this one, and of all.
@@ -216,17 +217,6 @@ __device__ __forceinline__ uint64_t filt_sum(uint64_t v, FiltShared& s) {
     uint64_t all;
     filt_scan(v, s, &all);
     return all;
-}
-
-// The thread whose `own` units hold unit `rank` (from 0), in the order of threads, and the units
-// before it; rank is below the total.
-__device__ __forceinline__ int filt_find(uint64_t own, uint64_t rank, FiltShared& s, uint64_t* before) {
-    uint64_t all;
-    const uint64_t excl = filt_scan(own, s, &all);
-    if (excl <= rank && rank - excl < own) s.sel[0] = threadIdx.x, s.sel[1] = excl;
-    __syncthreads();
-    *before = s.sel[1];
-    return (int)s.sel[0];
 }
 
 __device__ __forceinline__ float filt_max(float m, FiltShared& s) {
@@ -259,66 +249,59 @@ __device__ __forceinline__ uint64_t filt_need(float top_p, uint64_t W) {
 }
 
 // The entry that holds unit `rank` of the weights of a source of (id, key, weight), each(f): in the
-// sampler's order, or by id alone. The range of the keys (of equal keys: of the ids) that may hold it is
-// cut into 256 bins until one entry is left. rank is below the sum of the weights.
+// sampler's order (keys of [low, high]), or by id alone (ids of [low, high]). The range that may hold
+// it is cut into 256 bins until one entry is left, four times for keys and three for the ids of equal
+// keys at most. rank is below the sum of the weights; were it not (a workspace that was not zeroed),
+// the entry is any.
 template <typename Each>
-__device__ __forceinline__ FiltCut filt_pick(bool by_id, uint64_t rank, FiltShared& s, Each each) {
-    const int tid = threadIdx.x, wave = tid / kWave;
-    uint32_t lo = 0, hi = ~0u, tie = 0;   // of ~key, or of the ids with ~key = tie
+__device__ __forceinline__ FiltCut filt_pick(bool by_id, uint32_t low, uint32_t high, uint64_t rank, const FiltArgs& a, FiltShared& s, Each each) {
+    const int tid = threadIdx.x;
     bool ids = by_id;
-    for (;;) {
-        uint32_t n = 0, least = ~0u, most = 0, key = 0, id = 0;
+    uint32_t lo = by_id ? low : ~high, hi = by_id ? high : ~low, tie = 0;   // of ~key, or of the ids with ~key = tie
+    __syncthreads();
+    s.bins[0][tid] = 0, s.counts[0][tid] = 0;
+    __syncthreads();
+    for (int step = 0; step < 8; ++step) {
+        const int b = step & 1, bits = 32 - __builtin_clz(hi - lo | 1u), shift = max(bits - 8, 0);
+        auto value = [&](int i, uint32_t k) { return ids ? (uint32_t)i : ~k; };
         auto active = [&](int i, uint32_t k, uint64_t w) {
-            const uint32_t v = ids ? (uint32_t)i : ~k;
-            return w != 0 && v >= lo && v <= hi && (!ids || by_id || ~k == tie);
+            return w != 0 && value(i, k) >= lo && value(i, k) <= hi && (!ids || by_id || ~k == tie);
         };
         each([&](int i, uint32_t k, uint64_t w) {
             if (!active(i, k, w)) return;
-            const uint32_t v = ids ? (uint32_t)i : ~k;
-            ++n, least = min(least, v), most = max(most, v), key = k, id = (uint32_t)i;
+            const uint32_t bin = (value(i, k) - lo) >> shift;
+            atomicAdd(&s.bins[b][bin], (unsigned long long)w);
+            atomicAdd(&s.counts[b][bin], 1u);
         });
-        const bool mine = n != 0;
-#pragma unroll
-        for (int off = 32; off >= 1; off >>= 1) {
-            n += __shfl_xor(n, off, kWave);
-            least = min(least, (uint32_t)__shfl_xor((int)least, off, kWave));
-            most = max(most, (uint32_t)__shfl_xor((int)most, off, kWave));
-        }
-        if (tid % kWave == 0) s.range[wave][0] = n, s.range[wave][1] = least, s.range[wave][2] = most;
-        s.bins[tid] = 0;
+        s.bins[1 - b][tid] = 0, s.counts[1 - b][tid] = 0;
         __syncthreads();
-        n = 0;
-#pragma unroll
-        for (int w = 0; w < kFiltWaves; ++w) n += s.range[w][0], least = min(least, s.range[w][1]), most = max(most, s.range[w][2]);
-        if (n == 1) {
-            if (mine) s.found[0] = key, s.found[1] = id;
+        uint64_t all;
+        const uint64_t own = s.bins[b][tid], excl = filt_scan(own, s, &all);
+        if (excl <= rank && rank - excl < own) s.sel[0] = tid, s.sel[1] = excl, s.found[2] = s.counts[b][tid];
+        __syncthreads();
+        rank -= s.sel[1];
+        lo += ((uint32_t)s.sel[0] & (kFiltThreads - 1)) << shift, hi = min(hi, lo + ((1u << shift) - 1));
+        if (s.found[2] == 1) {
+            each([&](int i, uint32_t k, uint64_t w) {
+                if (active(i, k, w)) s.found[0] = k, s.found[1] = (uint32_t)i;
+            });
             __syncthreads();
             return FiltCut{s.found[0], (int)s.found[1]};
         }
-        if (least == most) {   // equal keys: by id
-            ids = true, tie = least, lo = 0, hi = ~0u;
-            __syncthreads();
-            continue;
+        if (shift == 0) {   // equal keys: by id
+            if (ids) break;
+            ids = true, tie = lo, lo = 0, hi = (uint32_t)a.V - 1;
         }
-        const int bits = 32 - __builtin_clz(most - least), shift = max(bits - 8, 0);
-        each([&](int i, uint32_t k, uint64_t w) {
-            if (active(i, k, w)) atomicAdd(&s.bins[((ids ? (uint32_t)i : ~k) - least) >> shift], (unsigned long long)w);
-        });
-        __syncthreads();
-        uint64_t before;
-        const uint32_t bin = (uint32_t)filt_find(s.bins[tid], rank, s, &before);
-        rank -= before;
-        lo = least + (bin << shift), hi = lo + ((1u << shift) - 1);
-        __syncthreads();
     }
+    return FiltCut{~0u, 0};
 }
 
-// K, N and the draw over a source of (id, key, mass), each(f).
+// K, N and the draw over a source of `count` entries (id, key, mass), each(f), keys of [low, high].
 template <typename Each>
-__device__ __forceinline__ int filt_choose(const FiltArgs& a, float u, FiltShared& s, Each each) {
+__device__ __forceinline__ int filt_choose(const FiltArgs& a, uint32_t low, uint32_t high, uint32_t count, float u, FiltShared& s, Each each) {
     FiltCut kept{0u, a.V};
-    if (a.top_k < a.V)
-        kept = filt_pick(false, (uint64_t)a.top_k - 1, s, [&](auto f) { each([&](int i, uint32_t k, uint64_t) { f(i, k, 1ull); }); });
+    if ((uint32_t)a.top_k < count)
+        kept = filt_pick(false, low, high, (uint64_t)a.top_k - 1, a, s, [&](auto f) { each([&](int i, uint32_t k, uint64_t) { f(i, k, 1ull); }); });
     auto left = [&](auto f) { each([&](int i, uint32_t k, uint64_t w) { f(i, k, kept.keeps(k, i) ? w : 0ull); }); };
     auto total = [&]() {
         uint64_t sum = 0;
@@ -327,23 +310,28 @@ __device__ __forceinline__ int filt_choose(const FiltArgs& a, float u, FiltShare
     };
     uint64_t M = total();
     if (a.top_p < 1.0f) {
-        kept = filt_pick(false, filt_need(a.top_p, M) - 1, s, left);
+        kept = filt_pick(false, low, high, filt_need(a.top_p, M) - 1, a, s, left);
         M = total();
     }
-    return filt_pick(true, filt_draw(u, M), s, left).id;
+    return filt_pick(true, 0, (uint32_t)a.V - 1, filt_draw(u, M), a, s, left).id;
 }
 
 // The same over the row itself: for what fits nowhere.
 template <bool BF16>
 __device__ __noinline__ int filt_choose_row(const FiltArgs& a, const void* row, float m, float u, FiltShared& s) {
-    return filt_choose(a, u, s, [&](auto f) {
+    return filt_choose(a, 0u, ~0u, (uint32_t)a.V, u, s, [&](auto f) {
         filt_tiles<BF16>(row, 0, a.V, [&](int, int i, const auto& l, int n) {
             constexpr int E = BF16 ? 8 : 4;
 #pragma unroll
             for (int e = 0; e < E; ++e)
-                if (e < n) f(i + e, filt_key(l[e]), filt_mass(a, l[e], m));
+                if (e < n) f(i + e, filt_key(filt_clean(l[e])), filt_mass(a, filt_clean(l[e]), m));
         });
     });
+}
+
+// The least logit of a bin of counts.
+__device__ __forceinline__ float filt_bin_logit(int bin) {
+    return bin <= (int)(0x007fffffu >> kFiltCountShift) ? -INFINITY : filt_logit((uint32_t)bin << kFiltCountShift);
 }
 
 constexpr int kFiltPer = kFiltCountBins / kFiltThreads;
@@ -395,7 +383,8 @@ struct FiltLast {
 };
 
 // A block's part of the last step: top-k: ids of bins >= bin are listed; top-p: masses of bins < bin by
-// tile, ids of `bin` are listed; neither: masses by tile. Tiles count from the block's first.
+// tile, ids of `bin` are listed; neither: masses by tile. Tiles count from the block's first. Most logits
+// are below what any of that takes: one comparison each, and a NaN goes the careful way.
 template <bool BF16, int MODE>
 __device__ __forceinline__ void filt_gather(const FiltArgs& a, const void* row, int first, int end, float m, int bin, FiltLast& z) {
     constexpr int E = BF16 ? 8 : 4;
@@ -403,18 +392,26 @@ __device__ __forceinline__ void filt_gather(const FiltArgs& a, const void* row, 
         const uint32_t at = atomicAdd(&z.count, 1u);
         if (at < kFiltHeld) z.list[at] = (unsigned long long)filt_key(l) << 32 | (uint32_t)i;
     };
+    const float least = filt_bin_logit(bin), past = bin < kFiltMassBins - 1 ? (float)(bin + 1) : INFINITY;
     filt_tiles<BF16>(row, first, end, [&](int t, int i, const float (&l)[E], int n) {
-        uint64_t y = 0;
+        bool some = false;
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            if constexpr (MODE == kFiltTopK) {
-                if (e < n && (int)(filt_key(l[e]) >> kFiltCountShift) >= bin) enlist(i + e, l[e]);
-            } else if constexpr (MODE == kFiltTopP) {
-                const int b = filt_bin(a, l[e], m);
-                if (b < bin) y += filt_mass(a, l[e], m);
-                else if (b == bin && e < n) enlist(i + e, l[e]);
-            } else {
-                y += filt_mass(a, l[e], m);   // there is none past the end: -inf
+        for (int e = 0; e < E; ++e)
+            some |= MODE == kFiltTopK ? l[e] >= least : MODE == kFiltTopP ? !((m - l[e]) * a.to_bin >= past) : !((l[e] - m) * a.to_log2f <= a.low);
+        uint64_t y = 0;
+        if (some) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const float x = filt_clean(l[e]);
+                if constexpr (MODE == kFiltTopK) {
+                    if (e < n && x >= least) enlist(i + e, x);
+                } else if constexpr (MODE == kFiltTopP) {
+                    const int b = filt_bin(a, x, m);
+                    if (b < bin) y += filt_mass(a, x, m);
+                    else if (b == bin && e < n) enlist(i + e, x);
+                } else {
+                    y += filt_mass(a, x, m);   // there is none past the end: -inf
+                }
             }
         }
         if (MODE != kFiltTopK && __any(y != 0)) {
@@ -426,13 +423,14 @@ __device__ __forceinline__ void filt_gather(const FiltArgs& a, const void* row, 
 
 // The choice from a row's list (`count` entries, in z or in `list`) and its tiles' masses (in z.tile).
 template <bool BF16, int MODE>
-__device__ __forceinline__ int filt_last(const FiltArgs& a, const void* row, float m, float u, uint64_t above, uint64_t W, uint32_t count,
-                                         const unsigned long long* list, FiltShared& s, FiltLast& z) {
+__device__ __forceinline__ int filt_last(const FiltArgs& a, const void* row, float m, float u, int bin, uint64_t above, uint64_t W,
+                                         uint32_t count, const unsigned long long* list, FiltShared& s, FiltLast& z) {
     const int tid = threadIdx.x;
+    const uint32_t high = filt_key(m), low = filt_key(filt_bin_logit(bin));   // the keys of top-k's list
     if (m == -INFINITY) return -1;
     if (count > (list != nullptr && MODE == kFiltTopK ? kFiltList : kFiltHeld)) return filt_choose_row<BF16>(a, row, m, u, s);
     if (MODE == kFiltTopK && count > kFiltHeld)
-        return filt_choose(a, u, s, [&](auto f) {
+        return filt_choose(a, low, high, count, u, s, [&](auto f) {
             for (uint32_t i = tid; i < count; i += kFiltThreads) {
                 const unsigned long long x = __hip_atomic_load(&list[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
                 f((int)(uint32_t)x, (uint32_t)(x >> 32), filt_mass(a, filt_logit((uint32_t)(x >> 32)), m));
@@ -447,13 +445,13 @@ __device__ __forceinline__ int filt_last(const FiltArgs& a, const void* row, flo
     auto each = [&](auto f) {
         for (uint32_t i = tid; i < count; i += kFiltThreads) f((int)(uint32_t)z.list[i], (uint32_t)(z.list[i] >> 32), (uint64_t)z.mass[i]);
     };
-    if constexpr (MODE == kFiltTopK) return filt_choose(a, u, s, each);
+    if constexpr (MODE == kFiltTopK) return filt_choose(a, low, high, count, u, s, each);
     constexpr int E = BF16 ? 8 : 4, TILE = E * kFiltThreads;
     FiltCut kept{0u, a.V};
     if constexpr (MODE == kFiltTopP) {
-        kept = filt_pick(false, filt_need(a.top_p, W) - 1 - above, s, each);
+        kept = filt_pick(false, 0u, high, filt_need(a.top_p, W) - 1 - above, a, s, each);
         each([&](int i, uint32_t k, uint64_t w) {
-            if (w != 0 && kept.keeps(k, i)) atomicAdd(&z.tile[i / TILE], (unsigned long long)w);
+            if (w != 0 && kept.keeps(k, i) && i < a.V) atomicAdd(&z.tile[i / TILE], (unsigned long long)w);
         });
         __syncthreads();
     }
@@ -468,12 +466,12 @@ __device__ __forceinline__ int filt_last(const FiltArgs& a, const void* row, flo
         excl += h[i];
     }
     __syncthreads();
-    const int t = (int)s.sel[0];
+    const int t = (int)min((uint32_t)s.sel[0], (uint32_t)(a.V - 1) / TILE);
     const uint64_t rest = r - s.sel[1];
     filt_tiles<BF16>(row, t * TILE, min(t * TILE + TILE, a.V), [&](int, int i, const float (&l)[E], int) {
         uint64_t y[E], sum = 0, all;
 #pragma unroll
-        for (int e = 0; e < E; ++e) sum += y[e] = kept.keeps(filt_key(l[e]), i + e) ? filt_mass(a, l[e], m) : 0ull;
+        for (int e = 0; e < E; ++e) sum += y[e] = kept.keeps(filt_key(filt_clean(l[e])), i + e) ? filt_mass(a, filt_clean(l[e]), m) : 0ull;
         uint64_t at = filt_scan(sum, s, &all);
 #pragma unroll
         for (int e = 0; e < E; ++e) {
@@ -508,8 +506,8 @@ __global__ __launch_bounds__(kFiltThreads) void filt_max_kernel(FiltArgs a) {
     filt_tiles<BF16>(filt_row<BF16>(a, blockIdx.y), first, end, [&](int, int, const float (&l)[E], int n) {
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            m = fmaxf(m, l[e]);
-            if (MODE == kFiltTopK && e < n) atomicAdd(&bins[filt_slot(filt_key(l[e]) >> kFiltCountShift)], 1u);
+            m = fmaxf(m, l[e]);   // not a NaN
+            if (MODE == kFiltTopK && e < n) atomicAdd(&bins[filt_slot(filt_key(filt_clean(l[e])) >> kFiltCountShift)], 1u);
         }
     });
     m = filt_max(m, s);   // the counts are whole behind its barrier
@@ -541,7 +539,7 @@ __device__ __forceinline__ void filt_mass_bins(const FiltArgs& a, const void* ro
     filt_tiles<BF16>(row, first, end, [&](int, int, const float (&l)[E], int) {
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            const uint64_t x = filt_mass(a, l[e], m);
+            const uint64_t x = filt_mass(a, filt_clean(l[e]), m);
             if (x != 0) atomicAdd(&bins[filt_bin(a, l[e], m)], (unsigned long long)x);
         }
     });
@@ -635,7 +633,7 @@ __global__ __launch_bounds__(kFiltThreads) void filt_draw_kernel(FiltArgs a) {
         for (int i = tid; i < kFiltCountBins; i += kFiltThreads) w.hist.count[i] = 0;
     if constexpr (MODE == kFiltTopP)
         for (int i = tid; i < kFiltMassBins; i += kFiltThreads) w.hist.mass[i] = 0;
-    const int token = filt_last<BF16, MODE>(a, row, m, u, above, W, count, w.list, s, z);
+    const int token = filt_last<BF16, MODE>(a, row, m, u, bin, above, W, count, w.list, s, z);
     if (tid == 0) a.out[blockIdx.y] = token;
 }
 
@@ -662,7 +660,7 @@ __global__ __launch_bounds__(kFiltThreads) void filt_one_kernel(FiltArgs a) {
 #pragma unroll
         for (int e = 0; e < E; ++e) {
             m = fmaxf(m, l[e]);
-            if (MODE == kFiltTopK && e < n) atomicAdd(&counts[filt_slot(filt_key(l[e]) >> kFiltCountShift)], 1u);
+            if (MODE == kFiltTopK && e < n) atomicAdd(&counts[filt_slot(filt_key(filt_clean(l[e])) >> kFiltCountShift)], 1u);
         }
     });
     m = filt_max(m, s);
@@ -685,13 +683,13 @@ __global__ __launch_bounds__(kFiltThreads) void filt_one_kernel(FiltArgs a) {
     }
     if (m > -INFINITY) filt_gather<BF16, MODE>(a, row, 0, a.V, m, bin, z);
     __syncthreads();
-    const int token = filt_last<BF16, MODE>(a, row, m, a.u[blockIdx.x], above, W, z.count, nullptr, s, z);
+    const int token = filt_last<BF16, MODE>(a, row, m, a.u[blockIdx.x], bin, above, W, z.count, nullptr, s, z);
     if (tid == 0) a.out[blockIdx.x] = token;
 }
 
 // Blocks of a row: some four workgroups a CU in all, blocks of whole tiles.
 static void filt_split(int64_t rows, int64_t vocab, int* blocks, int* chunk) {
-    const int64_t want = std::min<int64_t>(kFiltBlocks, std::max<int64_t>(1, (4 * prefill_cus() + rows - 1) / rows));
+    const int64_t want = std::min<int64_t>(kFiltBlocks, std::max<int64_t>(1, 4 * prefill_cus() / rows));
     const int64_t c = ((vocab + want - 1) / want + 2047) / 2048 * 2048;
     *chunk = (int)c;
     *blocks = (int)((vocab + c - 1) / c);
