@@ -15,17 +15,19 @@
 // some 2^-44 an id. V < 2^20 keeps every sum below 2^64.
 //
 // What bounds it: few rows by the launches and the chain of a row's last workgroup, many rows by the
-// logits' bytes and the 64-bit exponentials. A large vocabulary is cut into blocks of a workgroup each:
-//   no top-k, no top-p   1. block maxima  2. masses of tiles; the row's last workgroup finds the tile
+// logits' bytes and the 64-bit exponentials. The steps:
+//   no top-k, no top-p   1. the maximum  2. masses by tile (a pass of a workgroup's loads); the tile
 //                        that holds r and the id within it
-//   top-p                1. block maxima  2. histogram of masses by logit  3. masses by tile of the ids
-//                        that are surely in N, and a list of the ids of the bin in which N ends; the
-//                        last workgroup finds N's end in that list and goes on as above
-//   top-k                1. block maxima and a histogram of counts by logit  2. a list of the ids that
-//                        may be in K; the last workgroup finds the ends of K and N in it and draws
-// A small vocabulary goes through the same steps in one launch, a workgroup a row. Where the list's
-// masses do not fit in LDS, or the list not in its place (thousands of equal logits), the last
-// workgroup works from the list in memory or from the row itself.
+//   top-p                1. the maximum  2. a histogram of masses by logit  3. masses by tile of the
+//                        ids that are surely in N, and a list of the ids of the bin in which N ends;
+//                        N's end in that list, then the tile as above
+//   top-k                1. the maxima of runs of 32 logits: the top_k-th largest of those bounds the
+//                        top_k-th logit from below  2. a list of the ids above the bound; the ends of
+//                        K and N in it, and the draw
+// Few rows of a large vocabulary are cut into blocks of a workgroup each, a launch a step, and what
+// follows the last step's pass is done by the row's last workgroup to arrive. Small vocabularies and
+// many rows take one launch, a workgroup a row. Where the list does not fit (thousands of equal logits)
+// the choice is made from the row itself.
 #include "common.hpp"
 
 #include <algorithm>
@@ -35,29 +37,27 @@ namespace efm {
 
 int prefill_cus();
 
-constexpr int kFiltThreads = 256;
-constexpr int kFiltWaves = kFiltThreads / kWave;
+constexpr int kFiltThreads = 256;                // of a block of a row
 constexpr int kFiltMaxVocab = 1 << 20;
 constexpr double kFiltOne = 17592186044416.0;   // 2^44
 constexpr int kFiltBlocks = 128;                 // of a row, at most
-constexpr int kFiltTiles = 1024;                 // of a row: passes of a workgroup's loads, 1024 logits or more each
+constexpr int kFiltTiles = 1024;                 // of a row: 1024 logits or more each
 constexpr int kFiltMassBins = 1024, kFiltBinsPerOctave = 22;   // masses from 2^0 to below 2^-46
-constexpr int kFiltCountBins = 4096, kFiltCountShift = 20;     // sign, exponent and three bits of the logit
+constexpr int kFiltRuns = 8192;                  // runs of logits whose maxima are kept
+constexpr int kFiltRunBins = 1024;
 constexpr int kFiltList = 4096;
 constexpr int kFiltHeld = 1024;                  // entries of a list that a workgroup holds with their masses
-constexpr int kFiltOneVocab = 16384;             // rows of one launch
+constexpr int kFiltOneVocab = 16384;             // vocabularies of one launch
 
-// One row's part of the workspace. hist, counter and count are zero between calls.
+// One row's part of the workspace. mass_bins, counter and count are zero between calls.
 struct FiltRow {
-    union {
-        unsigned long long mass[kFiltMassBins];
-        uint32_t count[kFiltCountBins];
-    } hist;
+    unsigned long long mass_bins[kFiltMassBins];
     uint32_t counter, count;
     uint32_t pad[2];
     float bmax[kFiltBlocks];
     unsigned long long tile[kFiltTiles];
     unsigned long long list[kFiltList];   // key << 32 | id
+    float run[kFiltRuns];
 };
 static_assert(sizeof(FiltRow) % 16 == 0, "rows of the workspace stay aligned");
 
@@ -74,6 +74,7 @@ struct FiltArgs {
     int32_t* out;
     FiltRow* ws;
     int blocks, chunk;    // of a row; logits of a block
+    int run_lanes, runs;  // neighbouring threads that share a run; runs of a row
 };
 
 enum { kFiltAll, kFiltTopP, kFiltTopK };
@@ -116,12 +117,14 @@ __device__ __forceinline__ float filt_logit(uint32_t key) { return __uint_as_flo
 
 __device__ __forceinline__ float filt_clean(float l) { return l == l ? l : -INFINITY; }
 
+constexpr int kFiltBatch = 4;   // 16-byte loads of a thread under way
+
 // A row's logits [first, end), first a multiple of a tile: f(tile of the range, first id, the thread's
-// E logits as they are (-inf past the end), how many of them there are), by all threads together; 16
-// bytes a thread, four under way.
-template <bool BF16, typename F>
-__device__ __forceinline__ void filt_tiles(const void* row, int first, int end, F f) {
-    constexpr int E = BF16 ? 8 : 4, U = 4, TILE = E * kFiltThreads;
+// E logits as they are (-inf past the end), how many of them there are), by all threads together;
+// after each batch g(batch).
+template <int NT, bool BF16, typename F, typename G>
+__device__ __forceinline__ void filt_tiles(const void* row, int first, int end, F f, G g) {
+    constexpr int E = BF16 ? 8 : 4, U = kFiltBatch, TILE = E * NT;
     const bool aligned = (reinterpret_cast<uintptr_t>(row) & 15) == 0;
     for (int t0 = 0; first + t0 * TILE < end; t0 += U) {
         uint4 x[U];
@@ -158,7 +161,12 @@ __device__ __forceinline__ void filt_tiles(const void* row, int first, int end, 
             }
             f(t0 + j, i, l, min(max(end - i, 0), E));
         }
+        g(t0 / U);
     }
+}
+template <int NT, bool BF16, typename F>
+__device__ __forceinline__ void filt_tiles(const void* row, int first, int end, F f) {
+    filt_tiles<NT, BF16>(row, first, end, f, [](int) {});
 }
 
 // A 64-bit value moved across lanes, 0 where the source is none.
@@ -187,17 +195,19 @@ __device__ __forceinline__ uint64_t filt_last_lane(uint64_t v) {
            (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, 63);
 }
 
+template <int NT>
 struct FiltShared {
-    unsigned long long red[kFiltWaves];
+    unsigned long long red[NT / kWave];
     unsigned long long sel[2];
-    unsigned long long bins[2][kFiltThreads];
-    uint32_t counts[2][kFiltThreads];
-    float redf[kFiltWaves];
+    unsigned long long bins[2][256];
+    uint32_t counts[2][256];
+    float redf[2][NT / kWave];
     uint32_t flag, found[3];
 };
 
 // Sum of the values of the threads before this one, and of all.
-__device__ __forceinline__ uint64_t filt_scan(uint64_t v, FiltShared& s, uint64_t* total) {
+template <int NT>
+__device__ __forceinline__ uint64_t filt_scan(uint64_t v, FiltShared<NT>& s, uint64_t* total) {
     const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
     const uint64_t incl = filt_wave_scan(v);
     __syncthreads();
@@ -205,7 +215,7 @@ __device__ __forceinline__ uint64_t filt_scan(uint64_t v, FiltShared& s, uint64_
     __syncthreads();
     uint64_t before = 0, all = 0;
 #pragma unroll
-    for (int w = 0; w < kFiltWaves; ++w) {
+    for (int w = 0; w < NT / kWave; ++w) {
         if (w < wave) before += s.red[w];
         all += s.red[w];
     }
@@ -213,19 +223,25 @@ __device__ __forceinline__ uint64_t filt_scan(uint64_t v, FiltShared& s, uint64_
     return before + incl - v;
 }
 
-__device__ __forceinline__ uint64_t filt_sum(uint64_t v, FiltShared& s) {
+template <int NT>
+__device__ __forceinline__ uint64_t filt_sum(uint64_t v, FiltShared<NT>& s) {
     uint64_t all;
-    filt_scan(v, s, &all);
+    filt_scan<NT>(v, s, &all);
     return all;
 }
 
-__device__ __forceinline__ float filt_max(float m, FiltShared& s) {
+// The largest m and the smallest *least of the workgroup.
+template <int NT>
+__device__ __forceinline__ float filt_max(float m, float* least, FiltShared<NT>& s) {
     m = wave_max_uniform(m);
-    if (threadIdx.x % kWave == 0) s.redf[threadIdx.x / kWave] = m;
+    const float n = wave_max_uniform(-*least);
+    if (threadIdx.x % kWave == 0) s.redf[0][threadIdx.x / kWave] = m, s.redf[1][threadIdx.x / kWave] = n;
     __syncthreads();
-    m = s.redf[0];
+    m = s.redf[0][0];
+    float z = s.redf[1][0];
 #pragma unroll
-    for (int w = 1; w < kFiltWaves; ++w) m = fmaxf(m, s.redf[w]);
+    for (int w = 1; w < NT / kWave; ++w) m = fmaxf(m, s.redf[0][w]), z = fmaxf(z, s.redf[1][w]);
+    *least = -z;
     return m;
 }
 
@@ -253,13 +269,14 @@ __device__ __forceinline__ uint64_t filt_need(float top_p, uint64_t W) {
 // it is cut into 256 bins until one entry is left, four times for keys and three for the ids of equal
 // keys at most. rank is below the sum of the weights; were it not (a workspace that was not zeroed),
 // the entry is any.
-template <typename Each>
-__device__ __forceinline__ FiltCut filt_pick(bool by_id, uint32_t low, uint32_t high, uint64_t rank, const FiltArgs& a, FiltShared& s, Each each) {
+template <int NT, typename Each>
+__device__ __forceinline__ FiltCut filt_pick(bool by_id, uint32_t low, uint32_t high, uint64_t rank, const FiltArgs& a, FiltShared<NT>& s,
+                                             Each each) {
     const int tid = threadIdx.x;
     bool ids = by_id;
     uint32_t lo = by_id ? low : ~high, hi = by_id ? high : ~low, tie = 0;   // of ~key, or of the ids with ~key = tie
     __syncthreads();
-    s.bins[0][tid] = 0, s.counts[0][tid] = 0;
+    if (tid < 256) s.bins[0][tid] = 0, s.counts[0][tid] = 0;
     __syncthreads();
     for (int step = 0; step < 8; ++step) {
         const int b = step & 1, bits = 32 - __builtin_clz(hi - lo | 1u), shift = max(bits - 8, 0);
@@ -273,14 +290,14 @@ __device__ __forceinline__ FiltCut filt_pick(bool by_id, uint32_t low, uint32_t 
             atomicAdd(&s.bins[b][bin], (unsigned long long)w);
             atomicAdd(&s.counts[b][bin], 1u);
         });
-        s.bins[1 - b][tid] = 0, s.counts[1 - b][tid] = 0;
+        if (tid < 256) s.bins[1 - b][tid] = 0, s.counts[1 - b][tid] = 0;
         __syncthreads();
         uint64_t all;
-        const uint64_t own = s.bins[b][tid], excl = filt_scan(own, s, &all);
+        const uint64_t own = tid < 256 ? s.bins[b][tid] : 0ull, excl = filt_scan<NT>(own, s, &all);
         if (excl <= rank && rank - excl < own) s.sel[0] = tid, s.sel[1] = excl, s.found[2] = s.counts[b][tid];
         __syncthreads();
         rank -= s.sel[1];
-        lo += ((uint32_t)s.sel[0] & (kFiltThreads - 1)) << shift, hi = min(hi, lo + ((1u << shift) - 1));
+        lo += ((uint32_t)s.sel[0] & 255u) << shift, hi = min(hi, lo + ((1u << shift) - 1));
         if (s.found[2] == 1) {
             each([&](int i, uint32_t k, uint64_t w) {
                 if (active(i, k, w)) s.found[0] = k, s.found[1] = (uint32_t)i;
@@ -297,30 +314,32 @@ __device__ __forceinline__ FiltCut filt_pick(bool by_id, uint32_t low, uint32_t 
 }
 
 // K, N and the draw over a source of `count` entries (id, key, mass), each(f), keys of [low, high].
-template <typename Each>
-__device__ __forceinline__ int filt_choose(const FiltArgs& a, uint32_t low, uint32_t high, uint32_t count, float u, FiltShared& s, Each each) {
+template <int NT, typename Each>
+__device__ __forceinline__ int filt_choose(const FiltArgs& a, uint32_t low, uint32_t high, uint32_t count, float u, FiltShared<NT>& s,
+                                           Each each) {
     FiltCut kept{0u, a.V};
     if ((uint32_t)a.top_k < count)
-        kept = filt_pick(false, low, high, (uint64_t)a.top_k - 1, a, s, [&](auto f) { each([&](int i, uint32_t k, uint64_t) { f(i, k, 1ull); }); });
+        kept = filt_pick<NT>(false, low, high, (uint64_t)a.top_k - 1, a, s,
+                             [&](auto f) { each([&](int i, uint32_t k, uint64_t) { f(i, k, 1ull); }); });
     auto left = [&](auto f) { each([&](int i, uint32_t k, uint64_t w) { f(i, k, kept.keeps(k, i) ? w : 0ull); }); };
     auto total = [&]() {
         uint64_t sum = 0;
         left([&](int, uint32_t, uint64_t w) { sum += w; });
-        return filt_sum(sum, s);
+        return filt_sum<NT>(sum, s);
     };
     uint64_t M = total();
     if (a.top_p < 1.0f) {
-        kept = filt_pick(false, low, high, filt_need(a.top_p, M) - 1, a, s, left);
+        kept = filt_pick<NT>(false, low, high, filt_need(a.top_p, M) - 1, a, s, left);
         M = total();
     }
-    return filt_pick(true, 0, (uint32_t)a.V - 1, filt_draw(u, M), a, s, left).id;
+    return filt_pick<NT>(true, 0, (uint32_t)a.V - 1, filt_draw(u, M), a, s, left).id;
 }
 
 // The same over the row itself: for what fits nowhere.
-template <bool BF16>
-__device__ __noinline__ int filt_choose_row(const FiltArgs& a, const void* row, float m, float u, FiltShared& s) {
-    return filt_choose(a, 0u, ~0u, (uint32_t)a.V, u, s, [&](auto f) {
-        filt_tiles<BF16>(row, 0, a.V, [&](int, int i, const auto& l, int n) {
+template <int NT, bool BF16>
+__device__ __noinline__ int filt_choose_row(const FiltArgs& a, const void* row, float m, float u, FiltShared<NT>& s) {
+    return filt_choose<NT>(a, 0u, ~0u, (uint32_t)a.V, u, s, [&](auto f) {
+        filt_tiles<NT, BF16>(row, 0, a.V, [&](int, int i, const auto& l, int n) {
             constexpr int E = BF16 ? 8 : 4;
 #pragma unroll
             for (int e = 0; e < E; ++e)
@@ -329,44 +348,66 @@ __device__ __noinline__ int filt_choose_row(const FiltArgs& a, const void* row, 
     });
 }
 
-// The least logit of a bin of counts.
-__device__ __forceinline__ float filt_bin_logit(int bin) {
-    return bin <= (int)(0x007fffffu >> kFiltCountShift) ? -INFINITY : filt_logit((uint32_t)bin << kFiltCountShift);
-}
+// Top-k: what a logit has to reach to be listed. Logits fall into bins of equal width from the row's
+// maximum down to the smallest maximum of a run (-inf apart: it has no mass), and those of the bins down
+// to the one at which the runs are top_k are listed.
+struct FiltBound {
+    float m, width, past;   // listed unless (m - l) width >= past
+    __device__ __forceinline__ bool takes(float l) const { return !((m - l) * width >= past); }
+};
 
-constexpr int kFiltPer = kFiltCountBins / kFiltThreads;
-// A thread's 16 bins of a count histogram in LDS lie side by side, with a word between the threads'.
-__device__ __forceinline__ int filt_slot(int bin) { return bin + bin / kFiltPer; }
-constexpr int kFiltSlots = kFiltCountBins + kFiltThreads;
-
-// The bin that holds the top_k-th logit; the thread has the counts of bins high, high - 1, ... .
-__device__ __forceinline__ int filt_count_cut(const FiltArgs& a, const uint32_t (&c)[kFiltPer], int high, FiltShared& s) {
-    uint32_t own = 0;
+// From the maxima of the row's runs; *m: the row's maximum.
+template <int NT>
+__device__ __forceinline__ FiltBound filt_bound(const FiltArgs& a, const float* run, uint32_t* bins, FiltShared<NT>& s) {
+    constexpr int PER = kFiltRunBins / NT, HELD = kFiltRuns / NT;
+    const int tid = threadIdx.x;
+    float x[HELD], m = -INFINITY, least = INFINITY;
 #pragma unroll
-    for (int i = 0; i < kFiltPer; ++i) own += c[i];
-    uint64_t all, excl = filt_scan(own, s, &all);
+    for (int i = 0; i < HELD; ++i) {
+        const int r = i * NT + tid;
+        x[i] = -INFINITY;
+        if (i * NT < a.runs && r < a.runs) x[i] = run[r];
+        m = fmaxf(m, x[i]);
+        least = x[i] > -INFINITY ? fminf(least, x[i]) : least;
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) bins[i * NT + tid] = 0;
+    m = filt_max<NT>(m, &least, s);
+    const float width = (float)(kFiltRunBins - 1) / (m - least);
+    // few runs for so large a top_k, equal runs or infinite ones: all but -inf is listed
+    if (a.top_k > a.runs || !(width < INFINITY) || !(width > 0.f)) return FiltBound{m, 1.f, INFINITY};
+    FiltBound b{m, width, INFINITY};
+#pragma unroll
+    for (int i = 0; i < HELD; ++i)
+        if (i * NT < a.runs && i * NT + tid < a.runs) atomicAdd(&bins[(int)fminf((m - x[i]) * width, kFiltRunBins - 1)], 1u);
+    __syncthreads();
+    uint32_t own = 0, c[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) own += c[i] = bins[tid * PER + i];
+    uint64_t all, excl = filt_scan<NT>(own, s, &all);
     const uint64_t rank = (uint64_t)a.top_k - 1;
-    if (excl <= rank && rank - excl < own) {
-        int at = 0;
 #pragma unroll
-        for (int i = 0; i < kFiltPer; ++i) {
-            if (excl <= rank) at = high - i;
-            excl += c[i];
-        }
-        s.sel[0] = at;
+    for (int i = 0; i < PER; ++i) {
+        if (excl <= rank && rank - excl < c[i]) s.sel[0] = tid * PER + i;
+        excl += c[i];
     }
     __syncthreads();
-    return (int)s.sel[0];
+    if ((int)s.sel[0] < kFiltRunBins - 1) b.past = (float)((int)s.sel[0] + 1);
+    return b;
 }
 
-// The bin in which N ends; the thread has the masses of four bins. *above: the mass of the bins before
-// it, *W: of all.
-__device__ __forceinline__ int filt_mass_cut(const FiltArgs& a, const uint64_t (&h)[4], FiltShared& s, uint64_t* above, uint64_t* W) {
-    uint64_t excl = filt_scan(h[0] + h[1] + h[2] + h[3], s, W);
+// Top-p: the bin in which N ends. *above: the mass of the bins before it, *W: of all.
+template <int NT>
+__device__ __forceinline__ int filt_mass_cut(const FiltArgs& a, const unsigned long long* bins, FiltShared<NT>& s, uint64_t* above, uint64_t* W) {
+    constexpr int PER = kFiltMassBins / NT;
+    uint64_t h[PER], own = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) own += h[i] = bins[threadIdx.x * PER + i];
+    uint64_t excl = filt_scan<NT>(own, s, W);
     const uint64_t rank = filt_need(a.top_p, *W) - 1;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if (excl <= rank && rank - excl < h[i]) s.sel[0] = threadIdx.x * 4 + i, s.sel[1] = excl;
+    for (int i = 0; i < PER; ++i) {
+        if (excl <= rank && rank - excl < h[i]) s.sel[0] = threadIdx.x * PER + i, s.sel[1] = excl;
         excl += h[i];
     }
     __syncthreads();
@@ -382,29 +423,65 @@ struct FiltLast {
     uint32_t count, base;
 };
 
-// A block's part of the last step: top-k: ids of bins >= bin are listed; top-p: masses of bins < bin by
-// tile, ids of `bin` are listed; neither: masses by tile. Tiles count from the block's first. Most logits
-// are below what any of that takes: one comparison each, and a NaN goes the careful way.
-template <bool BF16, int MODE>
-__device__ __forceinline__ void filt_gather(const FiltArgs& a, const void* row, int first, int end, float m, int bin, FiltLast& z) {
+// The maximum of [first, end) and, for top-k, of its runs: those of a batch of a thread's loads, or of
+// run_lanes threads'. `runs` is where the range's begin.
+template <int NT, bool BF16, int MODE>
+__device__ __forceinline__ float filt_maxima(const FiltArgs& a, const void* row, int first, int end, float* runs) {
+    constexpr int E = BF16 ? 8 : 4;
+    float m = -INFINITY, x = -INFINITY;
+    filt_tiles<NT, BF16>(
+        row, first, end,
+        [&](int, int, const float (&l)[E], int) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) x = fmaxf(x, l[e]);   // not a NaN
+        },
+        [&](int batch) {
+            m = fmaxf(m, x);
+            if constexpr (MODE == kFiltTopK) {
+                for (int off = 1; off < a.run_lanes; off *= 2) x = fmaxf(x, __shfl_xor(x, off, kWave));
+                if (((int)threadIdx.x & (a.run_lanes - 1)) == 0) runs[(batch * NT + (int)threadIdx.x) / a.run_lanes] = x;
+            }
+            x = -INFINITY;
+        });
+    return m;
+}
+
+template <int NT, bool BF16>
+__device__ __forceinline__ void filt_mass_bins(const FiltArgs& a, const void* row, int first, int end, float m, unsigned long long* bins) {
+    constexpr int E = BF16 ? 8 : 4;
+    filt_tiles<NT, BF16>(row, first, end, [&](int, int, const float (&l)[E], int) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const uint64_t x = filt_mass(a, filt_clean(l[e]), m);
+            if (x != 0) atomicAdd(&bins[filt_bin(a, l[e], m)], (unsigned long long)x);
+        }
+    });
+}
+
+// The last step's pass: top-k: ids within the bound are listed; top-p: masses of bins < bin by tile, ids
+// of `bin` are listed; neither: masses by tile. Tiles count from the range's first. Most logits are below
+// what any of that takes: one comparison each, and a NaN goes the careful way.
+template <int NT, bool BF16, int MODE>
+__device__ __forceinline__ void filt_gather(const FiltArgs& a, const void* row, int first, int end, float m, int bin, const FiltBound& bound,
+                                            FiltLast& z) {
     constexpr int E = BF16 ? 8 : 4;
     auto enlist = [&](int i, float l) {
         const uint32_t at = atomicAdd(&z.count, 1u);
         if (at < kFiltHeld) z.list[at] = (unsigned long long)filt_key(l) << 32 | (uint32_t)i;
     };
-    const float least = filt_bin_logit(bin), past = bin < kFiltMassBins - 1 ? (float)(bin + 1) : INFINITY;
-    filt_tiles<BF16>(row, first, end, [&](int t, int i, const float (&l)[E], int n) {
+    const float past = bin < kFiltMassBins - 1 ? (float)(bin + 1) : INFINITY;
+    filt_tiles<NT, BF16>(row, first, end, [&](int t, int i, const float (&l)[E], int n) {
         bool some = false;
 #pragma unroll
         for (int e = 0; e < E; ++e)
-            some |= MODE == kFiltTopK ? l[e] >= least : MODE == kFiltTopP ? !((m - l[e]) * a.to_bin >= past) : !((l[e] - m) * a.to_log2f <= a.low);
+            some |= MODE == kFiltTopK ? bound.takes(l[e]) : MODE == kFiltTopP ? !((m - l[e]) * a.to_bin >= past) : !((l[e] - m) * a.to_log2f <= a.low);
         uint64_t y = 0;
         if (some) {
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 const float x = filt_clean(l[e]);
                 if constexpr (MODE == kFiltTopK) {
-                    if (e < n && x >= least) enlist(i + e, x);
+                    if (e < n && bound.takes(x)) enlist(i + e, x);
                 } else if constexpr (MODE == kFiltTopP) {
                     const int b = filt_bin(a, x, m);
                     if (b < bin) y += filt_mass(a, x, m);
@@ -422,57 +499,66 @@ __device__ __forceinline__ void filt_gather(const FiltArgs& a, const void* row, 
 }
 
 // The choice from a row's list (`count` entries, in z or in `list`) and its tiles' masses (in z.tile).
-template <bool BF16, int MODE>
-__device__ __forceinline__ int filt_last(const FiltArgs& a, const void* row, float m, float u, int bin, uint64_t above, uint64_t W,
-                                         uint32_t count, const unsigned long long* list, FiltShared& s, FiltLast& z) {
+template <int NT, bool BF16, int MODE>
+__device__ __forceinline__ int filt_last(const FiltArgs& a, const void* row, float m, float u, uint64_t above, uint64_t W, uint32_t count,
+                                         const unsigned long long* list, FiltShared<NT>& s, FiltLast& z) {
     const int tid = threadIdx.x;
-    const uint32_t high = filt_key(m), low = filt_key(filt_bin_logit(bin));   // the keys of top-k's list
+    const uint32_t high = filt_key(m);
     if (m == -INFINITY) return -1;
-    if (count > (list != nullptr && MODE == kFiltTopK ? kFiltList : kFiltHeld)) return filt_choose_row<BF16>(a, row, m, u, s);
+    if (count > (list != nullptr && MODE == kFiltTopK ? kFiltList : kFiltHeld)) return filt_choose_row<NT, BF16>(a, row, m, u, s);
     if (MODE == kFiltTopK && count > kFiltHeld)
-        return filt_choose(a, low, high, count, u, s, [&](auto f) {
-            for (uint32_t i = tid; i < count; i += kFiltThreads) {
+        return filt_choose<NT>(a, 0u, high, count, u, s, [&](auto f) {
+            for (uint32_t i = tid; i < count; i += NT) {
                 const unsigned long long x = __hip_atomic_load(&list[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
                 f((int)(uint32_t)x, (uint32_t)(x >> 32), filt_mass(a, filt_logit((uint32_t)(x >> 32)), m));
             }
         });
-    for (uint32_t i = tid; i < count; i += kFiltThreads) {
+    uint32_t low = ~0u;
+    for (uint32_t i = tid; i < count; i += NT) {
         const unsigned long long x = list != nullptr ? __hip_atomic_load(&list[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : z.list[i];
         z.list[i] = x;
         z.mass[i] = filt_mass(a, filt_logit((uint32_t)(x >> 32)), m);
+        low = min(low, (uint32_t)(x >> 32));
     }
-    __syncthreads();
     auto each = [&](auto f) {
-        for (uint32_t i = tid; i < count; i += kFiltThreads) f((int)(uint32_t)z.list[i], (uint32_t)(z.list[i] >> 32), (uint64_t)z.mass[i]);
+        for (uint32_t i = tid; i < count; i += NT) f((int)(uint32_t)z.list[i], (uint32_t)(z.list[i] >> 32), (uint64_t)z.mass[i]);
     };
-    if constexpr (MODE == kFiltTopK) return filt_choose(a, low, high, count, u, s, each);
-    constexpr int E = BF16 ? 8 : 4, TILE = E * kFiltThreads;
+    if constexpr (MODE != kFiltAll) {   // the least key listed
+#pragma unroll
+        for (int off = 32; off >= 1; off >>= 1) low = min(low, (uint32_t)__shfl_xor((int)low, off, kWave));
+        if (tid % kWave == 0) s.counts[0][tid / kWave] = low;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < NT / kWave; ++w) low = min(low, s.counts[0][w]);
+    }
+    if constexpr (MODE == kFiltTopK) return filt_choose<NT>(a, low, high, count, u, s, each);
+    constexpr int E = BF16 ? 8 : 4, TILE = E * NT, PER = kFiltTiles / NT;
     FiltCut kept{0u, a.V};
     if constexpr (MODE == kFiltTopP) {
-        kept = filt_pick(false, 0u, high, filt_need(a.top_p, W) - 1 - above, a, s, each);
+        kept = filt_pick<NT>(false, low, high, filt_need(a.top_p, W) - 1 - above, a, s, each);
         each([&](int i, uint32_t k, uint64_t w) {
             if (w != 0 && kept.keeps(k, i) && i < a.V) atomicAdd(&z.tile[i / TILE], (unsigned long long)w);
         });
         __syncthreads();
     }
-    uint64_t own = 0, M, h[4];
+    uint64_t own = 0, M, h[PER];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) own += h[i] = z.tile[tid * 4 + i];
-    uint64_t excl = filt_scan(own, s, &M);
+    for (int i = 0; i < PER; ++i) own += h[i] = z.tile[tid * PER + i];
+    uint64_t excl = filt_scan<NT>(own, s, &M);
     const uint64_t r = filt_draw(u, M);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if (excl <= r && r - excl < h[i]) s.sel[0] = tid * 4 + i, s.sel[1] = excl;
+    for (int i = 0; i < PER; ++i) {
+        if (excl <= r && r - excl < h[i]) s.sel[0] = tid * PER + i, s.sel[1] = excl;
         excl += h[i];
     }
     __syncthreads();
     const int t = (int)min((uint32_t)s.sel[0], (uint32_t)(a.V - 1) / TILE);
     const uint64_t rest = r - s.sel[1];
-    filt_tiles<BF16>(row, t * TILE, min(t * TILE + TILE, a.V), [&](int, int i, const float (&l)[E], int) {
+    filt_tiles<NT, BF16>(row, t * TILE, min(t * TILE + TILE, a.V), [&](int, int i, const float (&l)[E], int) {
         uint64_t y[E], sum = 0, all;
 #pragma unroll
         for (int e = 0; e < E; ++e) sum += y[e] = kept.keeps(filt_key(filt_clean(l[e])), i + e) ? filt_mass(a, filt_clean(l[e]), m) : 0ull;
-        uint64_t at = filt_scan(sum, s, &all);
+        uint64_t at = filt_scan<NT>(sum, s, &all);
 #pragma unroll
         for (int e = 0; e < E; ++e) {
             if (at <= rest && rest - at < y[e]) s.found[0] = i + e;
@@ -488,113 +574,80 @@ __device__ __forceinline__ const char* filt_row(const FiltArgs& a, unsigned r) {
     return static_cast<const char*>(a.logits) + (int64_t)r * a.stride * (BF16 ? 2 : 4);
 }
 
-// 1. Block maxima; top-k: a histogram of counts, of which a block adds the bins that its own first
-// top_k logits reach (lower ones cannot be among the row's).
+// Runs of [0, logits) of a row that threads of NT go through from its start.
+template <int NT, bool BF16>
+__host__ __device__ constexpr int filt_runs(int logits, int run_lanes) {
+    constexpr int BATCH = kFiltBatch * (BF16 ? 8 : 4) * NT;
+    return (logits + BATCH - 1) / BATCH * (NT / run_lanes);
+}
+
+// 1. Block maxima, and those of runs.
 template <bool BF16, int MODE>
 __global__ __launch_bounds__(kFiltThreads) void filt_max_kernel(FiltArgs a) {
-    constexpr int E = BF16 ? 8 : 4;
-    __shared__ FiltShared s;
-    __shared__ uint32_t bins[MODE == kFiltTopK ? kFiltSlots : 1];
-    const int tid = threadIdx.x, block = blockIdx.x;
+    __shared__ FiltShared<kFiltThreads> s;
     FiltRow& w = a.ws[blockIdx.y];
-    const int first = block * a.chunk, end = min(first + a.chunk, a.V);
-    if constexpr (MODE == kFiltTopK) {
-        for (int i = tid; i < kFiltSlots; i += kFiltThreads) bins[i] = 0;
-        __syncthreads();
-    }
-    float m = -INFINITY;
-    filt_tiles<BF16>(filt_row<BF16>(a, blockIdx.y), first, end, [&](int, int, const float (&l)[E], int n) {
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            m = fmaxf(m, l[e]);   // not a NaN
-            if (MODE == kFiltTopK && e < n) atomicAdd(&bins[filt_slot(filt_key(filt_clean(l[e])) >> kFiltCountShift)], 1u);
-        }
-    });
-    m = filt_max(m, s);   // the counts are whole behind its barrier
-    if (tid == 0) w.bmax[block] = m;
-    if constexpr (MODE == kFiltTopK) {
-        const int high = kFiltCountBins - 1 - tid * kFiltPer;   // the thread's bins, from the highest
-        uint32_t c[kFiltPer], own = 0;
-#pragma unroll
-        for (int i = 0; i < kFiltPer; ++i) own += c[i] = bins[filt_slot(high - i)];
-        uint64_t all;
-        uint64_t above = filt_scan(own, s, &all);
-#pragma unroll
-        for (int i = 0; i < kFiltPer; ++i) {
-            if (c[i] != 0 && above < (uint64_t)a.top_k)
-                __hip_atomic_fetch_add(&w.hist.count[high - i], c[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            above += c[i];
-        }
+    const int first = blockIdx.x * a.chunk, end = min(first + a.chunk, a.V);
+    float* const runs = w.run + blockIdx.x * filt_runs<kFiltThreads, BF16>(a.chunk, a.run_lanes);
+    float m = filt_maxima<kFiltThreads, BF16, MODE>(a, filt_row<BF16>(a, blockIdx.y), first, end, runs);
+    if constexpr (MODE == kFiltTopK) {   // the last block may end early
+        const int done = filt_runs<kFiltThreads, BF16>(end - first, a.run_lanes), all = filt_runs<kFiltThreads, BF16>(a.chunk, a.run_lanes);
+        for (int i = done + (int)threadIdx.x; i < all; i += kFiltThreads) runs[i] = -INFINITY;
+    } else {
+        float least = 0.f;
+        m = filt_max<kFiltThreads>(m, &least, s);
+        if (threadIdx.x == 0) w.bmax[blockIdx.x] = m;
     }
 }
 
 // The row's maximum, from its blocks'.
-__device__ __forceinline__ float filt_row_max(const FiltArgs& a, const FiltRow& w, FiltShared& s) {
-    return filt_max(threadIdx.x < a.blocks ? w.bmax[threadIdx.x] : -INFINITY, s);
-}
-
-template <bool BF16>
-__device__ __forceinline__ void filt_mass_bins(const FiltArgs& a, const void* row, int first, int end, float m, unsigned long long* bins) {
-    constexpr int E = BF16 ? 8 : 4;
-    filt_tiles<BF16>(row, first, end, [&](int, int, const float (&l)[E], int) {
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const uint64_t x = filt_mass(a, filt_clean(l[e]), m);
-            if (x != 0) atomicAdd(&bins[filt_bin(a, l[e], m)], (unsigned long long)x);
-        }
-    });
+__device__ __forceinline__ float filt_row_max(const FiltArgs& a, const FiltRow& w, FiltShared<kFiltThreads>& s) {
+    float least = 0.f;
+    return filt_max<kFiltThreads>(threadIdx.x < a.blocks ? w.bmax[threadIdx.x] : -INFINITY, &least, s);
 }
 
 // 2. top-p: masses by bin.
 template <bool BF16>
 __global__ __launch_bounds__(kFiltThreads) void filt_mass_kernel(FiltArgs a) {
-    __shared__ FiltShared s;
+    __shared__ FiltShared<kFiltThreads> s;
     __shared__ unsigned long long bins[kFiltMassBins];
     const int tid = threadIdx.x, first = blockIdx.x * a.chunk, end = min(first + a.chunk, a.V);
     FiltRow& w = a.ws[blockIdx.y];
     for (int i = tid; i < kFiltMassBins; i += kFiltThreads) bins[i] = 0;
     const float m = filt_row_max(a, w, s);
-    filt_mass_bins<BF16>(a, filt_row<BF16>(a, blockIdx.y), first, end, m, bins);
+    filt_mass_bins<kFiltThreads, BF16>(a, filt_row<BF16>(a, blockIdx.y), first, end, m, bins);
     __syncthreads();
     for (int i = tid; i < kFiltMassBins; i += kFiltThreads)
-        if (bins[i] != 0) __hip_atomic_fetch_add(&w.hist.mass[i], bins[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (bins[i] != 0) __hip_atomic_fetch_add(&w.mass_bins[i], bins[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
 // The last step: see the top. What a row's blocks hand to its last workgroup goes through agent-scope
 // stores that have returned before the block counts in, and agent-scope loads.
 template <bool BF16, int MODE>
 __global__ __launch_bounds__(kFiltThreads) void filt_draw_kernel(FiltArgs a) {
-    constexpr int TILE = (BF16 ? 8 : 4) * kFiltThreads;
-    __shared__ FiltShared s;
+    constexpr int NT = kFiltThreads, TILE = (BF16 ? 8 : 4) * NT;
+    __shared__ FiltShared<NT> s;
     __shared__ FiltLast z;
+    __shared__ uint32_t run_bins[MODE == kFiltTopK ? kFiltRunBins : 1];
     const int tid = threadIdx.x;
     FiltRow& w = a.ws[blockIdx.y];
     const char* const row = filt_row<BF16>(a, blockIdx.y);
     const int first = blockIdx.x * a.chunk, end = min(first + a.chunk, a.V), tiles = (end - first + TILE - 1) / TILE;
     if (tid == 0) z.count = 0;
     if constexpr (MODE != kFiltTopK)
-        for (int i = tid; i < tiles; i += kFiltThreads) z.tile[i] = 0;
-    // where K or N ends: the bin, and what lies above it
+        for (int i = tid; i < tiles; i += NT) z.tile[i] = 0;
     int bin = 0;
     uint64_t above = 0, W = 0;
-    uint32_t c[kFiltPer];
-    uint64_t h[4];
-    const int high = kFiltCountBins - 1 - tid * kFiltPer;
+    FiltBound bound{0.f, 0.f, 0.f};
+    float m;
     if constexpr (MODE == kFiltTopK) {
-#pragma unroll
-        for (int i = 0; i < kFiltPer; i += 4) {
-            const uint4 x = *reinterpret_cast<const uint4*>(&w.hist.count[high - i - 3]);
-            c[i] = x.w, c[i + 1] = x.z, c[i + 2] = x.y, c[i + 3] = x.x;
-        }
+        bound = filt_bound<NT>(a, w.run, run_bins, s);
+        m = bound.m;
+    } else {
+        m = filt_row_max(a, w, s);
     }
-    if constexpr (MODE == kFiltTopP) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) h[i] = w.hist.mass[tid * 4 + i];
-    }
-    const float m = filt_row_max(a, w, s);
-    if constexpr (MODE == kFiltTopK) bin = filt_count_cut(a, c, high, s);
-    if constexpr (MODE == kFiltTopP) bin = filt_mass_cut(a, h, s, &above, &W);
-    if (m > -INFINITY) filt_gather<BF16, MODE>(a, row, first, end, m, bin, z);
+    if constexpr (MODE == kFiltTopP) bin = filt_mass_cut<NT>(a, w.mass_bins, s, &above, &W);
+    __syncthreads();
+    if (m > -INFINITY) filt_gather<NT, BF16, MODE>(a, row, first, end, m, bin, bound, z);
     __syncthreads();
     if constexpr (MODE != kFiltAll) {
         const uint32_t n = z.count;
@@ -603,11 +656,11 @@ __global__ __launch_bounds__(kFiltThreads) void filt_draw_kernel(FiltArgs a) {
             z.base = __hip_atomic_fetch_add(&w.count, n <= kFiltHeld ? n : (uint32_t)kFiltList + 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         __syncthreads();
         if (n <= kFiltHeld)
-            for (uint32_t i = tid; i < n; i += kFiltThreads)
+            for (uint32_t i = tid; i < n; i += NT)
                 if (z.base + i < kFiltList) __hip_atomic_store(&w.list[z.base + i], z.list[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     if constexpr (MODE != kFiltTopK)
-        for (int i = tid; i < tiles; i += kFiltThreads)
+        for (int i = tid; i < tiles; i += NT)
             __hip_atomic_store(&w.tile[first / TILE + i], z.tile[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
@@ -622,70 +675,58 @@ __global__ __launch_bounds__(kFiltThreads) void filt_draw_kernel(FiltArgs a) {
     if constexpr (MODE != kFiltTopK) {
         const int all = (a.V + TILE - 1) / TILE;
 #pragma unroll
-        for (int i = 0; i < kFiltTiles / kFiltThreads; ++i) {
-            const int t = i * kFiltThreads + tid;
+        for (int i = 0; i < kFiltTiles / NT; ++i) {
+            const int t = i * NT + tid;
             z.tile[t] = t < all ? __hip_atomic_load(&w.tile[t], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0ull;
         }
     }
     __syncthreads();
     if (tid == 0) w.counter = 0, w.count = 0;
-    if constexpr (MODE == kFiltTopK)
-        for (int i = tid; i < kFiltCountBins; i += kFiltThreads) w.hist.count[i] = 0;
     if constexpr (MODE == kFiltTopP)
-        for (int i = tid; i < kFiltMassBins; i += kFiltThreads) w.hist.mass[i] = 0;
-    const int token = filt_last<BF16, MODE>(a, row, m, u, bin, above, W, count, w.list, s, z);
+        for (int i = tid; i < kFiltMassBins; i += NT) w.mass_bins[i] = 0;
+    const int token = filt_last<NT, BF16, MODE>(a, row, m, u, above, W, count, w.list, s, z);
     if (tid == 0) a.out[blockIdx.y] = token;
 }
 
-// Small vocabularies: all steps in one launch, a workgroup a row.
-template <bool BF16, int MODE>
-__global__ __launch_bounds__(kFiltThreads) void filt_one_kernel(FiltArgs a) {
-    constexpr int E = BF16 ? 8 : 4;
-    __shared__ FiltShared s;
+// All steps in one launch, a workgroup a row.
+template <int NT, bool BF16, int MODE>
+__global__ __launch_bounds__(NT) void filt_one_kernel(FiltArgs a) {
+    __shared__ FiltShared<NT> s;
     __shared__ FiltLast z;
-    __shared__ uint32_t counts[MODE == kFiltTopK ? kFiltSlots : 1];
+    __shared__ uint32_t run_bins[MODE == kFiltTopK ? kFiltRunBins : 1];
+    __shared__ float runs[MODE == kFiltTopK ? kFiltRuns : 1];
     __shared__ unsigned long long masses[MODE == kFiltTopP ? kFiltMassBins : 1];
     const int tid = threadIdx.x;
     const char* const row = filt_row<BF16>(a, blockIdx.x);
     if (tid == 0) z.count = 0;
-    for (int i = tid; i < kFiltTiles; i += kFiltThreads) z.tile[i] = 0;
-    if constexpr (MODE == kFiltTopK) {
-        for (int i = tid; i < kFiltSlots; i += kFiltThreads) counts[i] = 0;
-        __syncthreads();
-    }
+    for (int i = tid; i < kFiltTiles; i += NT) z.tile[i] = 0;
     if constexpr (MODE == kFiltTopP)
-        for (int i = tid; i < kFiltMassBins; i += kFiltThreads) masses[i] = 0;
-    float m = -INFINITY;
-    filt_tiles<BF16>(row, 0, a.V, [&](int, int, const float (&l)[E], int n) {
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            m = fmaxf(m, l[e]);
-            if (MODE == kFiltTopK && e < n) atomicAdd(&counts[filt_slot(filt_key(filt_clean(l[e])) >> kFiltCountShift)], 1u);
-        }
-    });
-    m = filt_max(m, s);
+        for (int i = tid; i < kFiltMassBins; i += NT) masses[i] = 0;
+    float m = filt_maxima<NT, BF16, MODE>(a, row, 0, a.V, runs), least = 0.f;
     int bin = 0;
     uint64_t above = 0, W = 0;
+    FiltBound bound{0.f, 0.f, 0.f};
     if constexpr (MODE == kFiltTopK) {
-        const int high = kFiltCountBins - 1 - tid * kFiltPer;
-        uint32_t c[kFiltPer];
-#pragma unroll
-        for (int i = 0; i < kFiltPer; ++i) c[i] = counts[filt_slot(high - i)];
-        bin = filt_count_cut(a, c, high, s);
+        __syncthreads();
+        bound = filt_bound<NT>(a, runs, run_bins, s);
+        m = bound.m;
+    } else {
+        m = filt_max<NT>(m, &least, s);
     }
     if constexpr (MODE == kFiltTopP) {
-        filt_mass_bins<BF16>(a, row, 0, a.V, m, masses);
+        filt_mass_bins<NT, BF16>(a, row, 0, a.V, m, masses);
         __syncthreads();
-        uint64_t h[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) h[i] = masses[tid * 4 + i];
-        bin = filt_mass_cut(a, h, s, &above, &W);
+        bin = filt_mass_cut<NT>(a, masses, s, &above, &W);
     }
-    if (m > -INFINITY) filt_gather<BF16, MODE>(a, row, 0, a.V, m, bin, z);
     __syncthreads();
-    const int token = filt_last<BF16, MODE>(a, row, m, a.u[blockIdx.x], bin, above, W, z.count, nullptr, s, z);
+    if (m > -INFINITY) filt_gather<NT, BF16, MODE>(a, row, 0, a.V, m, bin, bound, z);
+    __syncthreads();
+    const int token = filt_last<NT, BF16, MODE>(a, row, m, a.u[blockIdx.x], above, W, z.count, nullptr, s, z);
     if (tid == 0) a.out[blockIdx.x] = token;
 }
+
+// A workgroup a row: small vocabularies, and rows enough to fill the chip.
+static bool filt_one(int64_t rows, int64_t vocab) { return vocab <= kFiltOneVocab || rows >= prefill_cus() / 2; }
 
 // Blocks of a row: some four workgroups a CU in all, blocks of whole tiles.
 static void filt_split(int64_t rows, int64_t vocab, int* blocks, int* chunk) {
@@ -695,23 +736,34 @@ static void filt_split(int64_t rows, int64_t vocab, int* blocks, int* chunk) {
     *blocks = (int)((vocab + c - 1) / c);
 }
 
+template <int NT, bool BF16>
+static void filt_launch_one(FiltArgs a, int64_t rows, hipStream_t stream) {
+    for (a.run_lanes = 1; filt_runs<NT, BF16>(a.V, a.run_lanes) > kFiltRuns; a.run_lanes *= 2) {}
+    a.runs = filt_runs<NT, BF16>(a.V, a.run_lanes);
+    const dim3 grid((unsigned)rows), t(NT);
+    if (a.top_k < a.V) hipLaunchKernelGGL((filt_one_kernel<NT, BF16, kFiltTopK>), grid, t, 0, stream, a);
+    else if (a.top_p < 1.0f) hipLaunchKernelGGL((filt_one_kernel<NT, BF16, kFiltTopP>), grid, t, 0, stream, a);
+    else hipLaunchKernelGGL((filt_one_kernel<NT, BF16, kFiltAll>), grid, t, 0, stream, a);
+}
+
 template <bool BF16>
-static void filt_launch(const FiltArgs& a, int64_t rows, hipStream_t stream) {
-    const dim3 t(kFiltThreads), grid(a.blocks, (unsigned)rows), one((unsigned)rows);
-    const bool k = a.top_k < a.V, p = a.top_p < 1.0f;
+static void filt_launch(FiltArgs a, int64_t rows, hipStream_t stream) {
     if (a.ws == nullptr) {
-        if (k) hipLaunchKernelGGL((filt_one_kernel<BF16, kFiltTopK>), one, t, 0, stream, a);
-        else if (p) hipLaunchKernelGGL((filt_one_kernel<BF16, kFiltTopP>), one, t, 0, stream, a);
-        else hipLaunchKernelGGL((filt_one_kernel<BF16, kFiltAll>), one, t, 0, stream, a);
+        if (a.V <= kFiltOneVocab) filt_launch_one<256, BF16>(a, rows, stream);
+        else filt_launch_one<1024, BF16>(a, rows, stream);
         return;
     }
-    if (k) {
+    filt_split(rows, a.V, &a.blocks, &a.chunk);
+    for (a.run_lanes = 1; a.blocks * filt_runs<kFiltThreads, BF16>(a.chunk, a.run_lanes) > kFiltRuns; a.run_lanes *= 2) {}
+    a.runs = a.blocks * filt_runs<kFiltThreads, BF16>(a.chunk, a.run_lanes);
+    const dim3 t(kFiltThreads), grid(a.blocks, (unsigned)rows);
+    if (a.top_k < a.V) {
         hipLaunchKernelGGL((filt_max_kernel<BF16, kFiltTopK>), grid, t, 0, stream, a);
         hipLaunchKernelGGL((filt_draw_kernel<BF16, kFiltTopK>), grid, t, 0, stream, a);
         return;
     }
     hipLaunchKernelGGL((filt_max_kernel<BF16, kFiltAll>), grid, t, 0, stream, a);
-    if (p) {
+    if (a.top_p < 1.0f) {
         hipLaunchKernelGGL(filt_mass_kernel<BF16>, grid, t, 0, stream, a);
         hipLaunchKernelGGL((filt_draw_kernel<BF16, kFiltTopP>), grid, t, 0, stream, a);
     } else {
@@ -724,7 +776,7 @@ static void filt_launch(const FiltArgs& a, int64_t rows, hipStream_t stream) {
 using namespace efm;
 
 extern "C" size_t efm_sampler_filtered_workspace_bytes(int64_t rows, int64_t vocab) {
-    return rows <= 0 || vocab <= kFiltOneVocab ? 0 : (size_t)rows * sizeof(FiltRow);
+    return rows <= 0 || filt_one(rows, vocab) ? 0 : (size_t)rows * sizeof(FiltRow);
 }
 
 extern "C" int efm_sampler_filtered(int64_t rows, int64_t vocab, const void* logits, int32_t logits_dtype, int64_t logits_stride,
@@ -767,7 +819,7 @@ extern "C" int efm_sampler_filtered(int64_t rows, int64_t vocab, const void* log
     a.u = uniforms;
     a.out = token_out;
     a.ws = need > 0 ? static_cast<FiltRow*>(workspace) : nullptr;
-    filt_split(rows, vocab, &a.blocks, &a.chunk);
+    a.blocks = a.chunk = a.run_lanes = a.runs = 0;
     if (logits_dtype == EFM_DTYPE_BF16) filt_launch<true>(a, rows, stream);
     else filt_launch<false>(a, rows, stream);
     return check_launch("sampler_filtered");

@@ -360,7 +360,7 @@ def test_sampler(gpu, f, rows, vocab, dtype):
 
 @pytest.mark.parametrize("f", [dict(), dict(k=50, p=0.9), dict(p=0.95), dict(min_p=0.03)], ids=str)
 @pytest.mark.parametrize("rows,vocab", [(1, 1), (4, 2), (3, 63), (2, 65), (9, 1023), (9, 1025), (2, 32768), (2, 32769), (2, (1 << 20) - 1),
-                                        (260, 40000), (600, 700), (1100, 15000), (3, 16384), (3, 16385), (1500, 20000)])
+                                        (260, 40000), (600, 700), (1100, 15000), (3, 16384), (3, 16385), (1500, 20000), (127, 50000), (128, 50000)])
 def test_sampler_sizes(gpu, f, rows, vocab):
     for dtype in (torch.float32, torch.bfloat16):
         x, u = _logits(vocab, rows, vocab, dtype)
@@ -394,6 +394,18 @@ def test_sampler_rows_that_are_not_finite(gpu, f, vocab):
     got = _sample(x, u, **f)
     assert torch.equal(got, R.sample(x, u, **f))
     assert got[2] == -1 and got[3] == -1 and got[4] == vocab - 7 and got[5] == 1234
+
+
+@pytest.mark.parametrize("f", [dict(k=20), dict(k=3000), dict(k=50, p=0.9), dict(p=0.9), dict(min_p=0.02), dict()], ids=str)
+@pytest.mark.parametrize("rows,vocab", [(3, 10000), (2, 151936), (140, 30000)])
+def test_sampler_masked_rows(gpu, f, rows, vocab):
+    """Rows with -inf for all but some ids, as a grammar leaves them: in one run, every 1000th, and all below zero."""
+    x, u = _logits(5, rows, vocab)
+    keep = torch.zeros(rows, vocab, dtype=torch.bool, device="cuda")
+    keep[0, 64:90], keep[1:, 13::1000] = True, True
+    x = torch.where(keep, x, -math.inf)
+    x[1:] -= 60
+    assert torch.equal(_sample(x, u, **f), R.sample(x, u, **f))
 
 
 def test_sampler_random_numbers_at_the_ends(gpu):
