@@ -38,6 +38,7 @@ namespace efm {
 int prefill_cus();
 
 constexpr int kFiltThreads = 256;                // of a block of a row
+constexpr int kFiltListThreads = 512;
 constexpr int kFiltMaxVocab = 1 << 20;
 constexpr double kFiltOne = 17592186044416.0;   // 2^44
 constexpr int kFiltBlocks = 128;                 // of a row, at most
@@ -45,8 +46,7 @@ constexpr int kFiltTiles = 1024;                 // of a row: 1024 logits or mor
 constexpr int kFiltMassBins = 1024, kFiltBinsPerOctave = 22;   // masses from 2^0 to below 2^-46
 constexpr int kFiltRuns = 8192;                  // runs of logits whose maxima are kept
 constexpr int kFiltRunBins = 1024;
-constexpr int kFiltList = 4096;
-constexpr int kFiltHeld = 1024;                  // entries of a list that a workgroup holds with their masses
+constexpr int kFiltHeld = 1024, kFiltHeldK = 2048;   // entries of a list that a workgroup holds with their masses; top-k
 constexpr int kFiltOneVocab = 16384;             // vocabularies of one launch
 
 // One row's part of the workspace. mass_bins, counter and count are zero between calls.
@@ -56,7 +56,7 @@ struct FiltRow {
     uint32_t pad[2];
     float bmax[kFiltBlocks];
     unsigned long long tile[kFiltTiles];
-    unsigned long long list[kFiltList];   // key << 32 | id
+    unsigned long long list[kFiltHeld];   // key << 32 | id
     float run[kFiltRuns];
 };
 static_assert(sizeof(FiltRow) % 16 == 0, "rows of the workspace stay aligned");
@@ -119,6 +119,40 @@ __device__ __forceinline__ float filt_clean(float l) { return l == l ? l : -INFI
 
 constexpr int kFiltBatch = 4;   // 16-byte loads of a thread under way
 
+template <bool BF16>
+__device__ __forceinline__ uint4 filt_raw(const void* row, bool aligned, int i, int end) {
+    constexpr int E = BF16 ? 8 : 4;
+    if (aligned && i + E <= end) return *reinterpret_cast<const uint4*>(static_cast<const char*>(row) + (int64_t)i * (BF16 ? 2 : 4));
+    uint32_t w[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        if constexpr (BF16) {
+            const uint16_t* const p = static_cast<const uint16_t*>(row);
+            const uint32_t lo = i + 2 * e < end ? p[i + 2 * e] : 0xff80u, hi = i + 2 * e + 1 < end ? p[i + 2 * e + 1] : 0xff80u;
+            w[e] = lo | hi << 16;
+        } else {
+            w[e] = i + e < end ? static_cast<const uint32_t*>(row)[i + e] : 0xff800000u;
+        }
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+template <bool BF16>
+__device__ __forceinline__ void filt_unpack(const uint4& x, float* l) {
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        if constexpr (BF16) l[2 * e] = lo_f32(w[e]), l[2 * e + 1] = hi_f32(w[e]);
+        else l[e] = __uint_as_float(w[e]);
+    }
+}
+
+// Logits i to i + E - 1 of a row that ends at `end`, -inf past it.
+template <bool BF16>
+__device__ __forceinline__ void filt_load(const void* row, int i, int end, float* l) {
+    filt_unpack<BF16>(filt_raw<BF16>(row, (reinterpret_cast<uintptr_t>(row) & 15) == 0, i, end), l);
+}
+
 // A row's logits [first, end), first a multiple of a tile: f(tile of the range, first id, the thread's
 // E logits as they are (-inf past the end), how many of them there are), by all threads together;
 // after each batch g(batch).
@@ -131,34 +165,14 @@ __device__ __forceinline__ void filt_tiles(const void* row, int first, int end, 
 #pragma unroll
         for (int j = 0; j < U; ++j) {
             const int i = first + (t0 + j) * TILE + (int)threadIdx.x * E;
-            if (aligned && i + E <= end) {
-                x[j] = *reinterpret_cast<const uint4*>(static_cast<const char*>(row) + (int64_t)i * (BF16 ? 2 : 4));
-            } else {
-                uint32_t w[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    if constexpr (BF16) {
-                        const uint16_t* const p = static_cast<const uint16_t*>(row);
-                        const uint32_t lo = i + 2 * e < end ? p[i + 2 * e] : 0xff80u, hi = i + 2 * e + 1 < end ? p[i + 2 * e + 1] : 0xff80u;
-                        w[e] = lo | hi << 16;
-                    } else {
-                        w[e] = i + e < end ? static_cast<const uint32_t*>(row)[i + e] : 0xff800000u;
-                    }
-                }
-                x[j] = make_uint4(w[0], w[1], w[2], w[3]);
-            }
+            x[j] = filt_raw<BF16>(row, aligned, i, end);
         }
 #pragma unroll
         for (int j = 0; j < U; ++j) {
             const int i = first + (t0 + j) * TILE + (int)threadIdx.x * E;
             if (first + (t0 + j) * TILE >= end) break;
             float l[E];
-            const uint32_t w[4] = {x[j].x, x[j].y, x[j].z, x[j].w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                if constexpr (BF16) l[2 * e] = lo_f32(w[e]), l[2 * e + 1] = hi_f32(w[e]);
-                else l[e] = __uint_as_float(w[e]);
-            }
+            filt_unpack<BF16>(x[j], l);
             f(t0 + j, i, l, min(max(end - i, 0), E));
         }
         g(t0 / U);
@@ -356,9 +370,9 @@ struct FiltBound {
     __device__ __forceinline__ bool takes(float l) const { return !((m - l) * width >= past); }
 };
 
-// From the maxima of the row's runs; *m: the row's maximum.
-template <int NT>
-__device__ __forceinline__ FiltBound filt_bound(const FiltArgs& a, const float* run, uint32_t* bins, FiltShared<NT>& s) {
+// From the maxima of the row's runs; pick(run) for the runs that hold such logits.
+template <int NT, typename Pick>
+__device__ __forceinline__ FiltBound filt_bound(const FiltArgs& a, const float* run, uint32_t* bins, FiltShared<NT>& s, Pick pick) {
     constexpr int PER = kFiltRunBins / NT, HELD = kFiltRuns / NT;
     const int tid = threadIdx.x;
     float x[HELD], m = -INFINITY, least = INFINITY;
@@ -373,26 +387,33 @@ __device__ __forceinline__ FiltBound filt_bound(const FiltArgs& a, const float* 
 #pragma unroll
     for (int i = 0; i < PER; ++i) bins[i * NT + tid] = 0;
     m = filt_max<NT>(m, &least, s);
-    const float width = (float)(kFiltRunBins - 1) / (m - least);
     // few runs for so large a top_k, equal runs or infinite ones: all but -inf is listed
-    if (a.top_k > a.runs || !(width < INFINITY) || !(width > 0.f)) return FiltBound{m, 1.f, INFINITY};
-    FiltBound b{m, width, INFINITY};
+    FiltBound b{m, (float)(kFiltRunBins - 1) / (m - least), INFINITY};
+    if (a.top_k >= a.V) {   // min-p alone: what has mass that counts
+        b.width = a.to_log2f, b.past = -a.low;
+    } else if (a.top_k > a.runs || !(b.width < INFINITY) || !(b.width > 0.f)) {
+        b.width = 1.f;
+    } else {
+#pragma unroll
+        for (int i = 0; i < HELD; ++i)
+            if (i * NT < a.runs && i * NT + tid < a.runs) atomicAdd(&bins[(int)fminf((m - x[i]) * b.width, kFiltRunBins - 1)], 1u);
+        __syncthreads();
+        uint32_t own = 0, c[PER];
+#pragma unroll
+        for (int i = 0; i < PER; ++i) own += c[i] = bins[tid * PER + i];
+        uint64_t all, excl = filt_scan<NT>(own, s, &all);
+        const uint64_t rank = (uint64_t)a.top_k - 1;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            if (excl <= rank && rank - excl < c[i]) s.sel[0] = tid * PER + i;
+            excl += c[i];
+        }
+        __syncthreads();
+        if ((int)s.sel[0] < kFiltRunBins - 1) b.past = (float)((int)s.sel[0] + 1);
+    }
 #pragma unroll
     for (int i = 0; i < HELD; ++i)
-        if (i * NT < a.runs && i * NT + tid < a.runs) atomicAdd(&bins[(int)fminf((m - x[i]) * width, kFiltRunBins - 1)], 1u);
-    __syncthreads();
-    uint32_t own = 0, c[PER];
-#pragma unroll
-    for (int i = 0; i < PER; ++i) own += c[i] = bins[tid * PER + i];
-    uint64_t all, excl = filt_scan<NT>(own, s, &all);
-    const uint64_t rank = (uint64_t)a.top_k - 1;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-        if (excl <= rank && rank - excl < c[i]) s.sel[0] = tid * PER + i;
-        excl += c[i];
-    }
-    __syncthreads();
-    if ((int)s.sel[0] < kFiltRunBins - 1) b.past = (float)((int)s.sel[0] + 1);
+        if (i * NT < a.runs && x[i] > -INFINITY && b.takes(x[i])) pick(i * NT + tid);
     return b;
 }
 
@@ -416,9 +437,11 @@ __device__ __forceinline__ int filt_mass_cut(const FiltArgs& a, const unsigned l
 }
 
 // Shared memory of the last step: the list with its masses, and the tiles' masses.
+template <int H>
 struct FiltLast {
-    unsigned long long list[kFiltHeld];
-    unsigned long long mass[kFiltHeld];
+    static constexpr int kHeld = H;
+    unsigned long long list[H];
+    unsigned long long mass[H];
     unsigned long long tile[kFiltTiles];
     uint32_t count, base;
 };
@@ -461,13 +484,13 @@ __device__ __forceinline__ void filt_mass_bins(const FiltArgs& a, const void* ro
 // The last step's pass: top-k: ids within the bound are listed; top-p: masses of bins < bin by tile, ids
 // of `bin` are listed; neither: masses by tile. Tiles count from the range's first. Most logits are below
 // what any of that takes: one comparison each, and a NaN goes the careful way.
-template <int NT, bool BF16, int MODE>
+template <int NT, bool BF16, int MODE, typename Last>
 __device__ __forceinline__ void filt_gather(const FiltArgs& a, const void* row, int first, int end, float m, int bin, const FiltBound& bound,
-                                            FiltLast& z) {
+                                            Last& z) {
     constexpr int E = BF16 ? 8 : 4;
     auto enlist = [&](int i, float l) {
         const uint32_t at = atomicAdd(&z.count, 1u);
-        if (at < kFiltHeld) z.list[at] = (unsigned long long)filt_key(l) << 32 | (uint32_t)i;
+        if (at < Last::kHeld) z.list[at] = (unsigned long long)filt_key(l) << 32 | (uint32_t)i;
     };
     const float past = bin < kFiltMassBins - 1 ? (float)(bin + 1) : INFINITY;
     filt_tiles<NT, BF16>(row, first, end, [&](int t, int i, const float (&l)[E], int n) {
@@ -499,20 +522,13 @@ __device__ __forceinline__ void filt_gather(const FiltArgs& a, const void* row, 
 }
 
 // The choice from a row's list (`count` entries, in z or in `list`) and its tiles' masses (in z.tile).
-template <int NT, bool BF16, int MODE>
+template <int NT, bool BF16, int MODE, typename Last>
 __device__ __forceinline__ int filt_last(const FiltArgs& a, const void* row, float m, float u, uint64_t above, uint64_t W, uint32_t count,
-                                         const unsigned long long* list, FiltShared<NT>& s, FiltLast& z) {
+                                         const unsigned long long* list, FiltShared<NT>& s, Last& z) {
     const int tid = threadIdx.x;
     const uint32_t high = filt_key(m);
     if (m == -INFINITY) return -1;
-    if (count > (list != nullptr && MODE == kFiltTopK ? kFiltList : kFiltHeld)) return filt_choose_row<NT, BF16>(a, row, m, u, s);
-    if (MODE == kFiltTopK && count > kFiltHeld)
-        return filt_choose<NT>(a, 0u, high, count, u, s, [&](auto f) {
-            for (uint32_t i = tid; i < count; i += NT) {
-                const unsigned long long x = __hip_atomic_load(&list[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                f((int)(uint32_t)x, (uint32_t)(x >> 32), filt_mass(a, filt_logit((uint32_t)(x >> 32)), m));
-            }
-        });
+    if (count > Last::kHeld) return filt_choose_row<NT, BF16>(a, row, m, u, s);
     uint32_t low = ~0u;
     for (uint32_t i = tid; i < count; i += NT) {
         const unsigned long long x = list != nullptr ? __hip_atomic_load(&list[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : z.list[i];
@@ -589,7 +605,7 @@ __global__ __launch_bounds__(kFiltThreads) void filt_max_kernel(FiltArgs a) {
     const int first = blockIdx.x * a.chunk, end = min(first + a.chunk, a.V);
     float* const runs = w.run + blockIdx.x * filt_runs<kFiltThreads, BF16>(a.chunk, a.run_lanes);
     float m = filt_maxima<kFiltThreads, BF16, MODE>(a, filt_row<BF16>(a, blockIdx.y), first, end, runs);
-    if constexpr (MODE == kFiltTopK) {   // the last block may end early
+    if constexpr (MODE == kFiltTopK) {   // the last block may end before its runs do
         const int done = filt_runs<kFiltThreads, BF16>(end - first, a.run_lanes), all = filt_runs<kFiltThreads, BF16>(a.chunk, a.run_lanes);
         for (int i = done + (int)threadIdx.x; i < all; i += kFiltThreads) runs[i] = -INFINITY;
     } else {
@@ -626,25 +642,17 @@ template <bool BF16, int MODE>
 __global__ __launch_bounds__(kFiltThreads) void filt_draw_kernel(FiltArgs a) {
     constexpr int NT = kFiltThreads, TILE = (BF16 ? 8 : 4) * NT;
     __shared__ FiltShared<NT> s;
-    __shared__ FiltLast z;
-    __shared__ uint32_t run_bins[MODE == kFiltTopK ? kFiltRunBins : 1];
+    __shared__ FiltLast<kFiltHeld> z;
     const int tid = threadIdx.x;
     FiltRow& w = a.ws[blockIdx.y];
     const char* const row = filt_row<BF16>(a, blockIdx.y);
     const int first = blockIdx.x * a.chunk, end = min(first + a.chunk, a.V), tiles = (end - first + TILE - 1) / TILE;
     if (tid == 0) z.count = 0;
-    if constexpr (MODE != kFiltTopK)
-        for (int i = tid; i < tiles; i += NT) z.tile[i] = 0;
+    for (int i = tid; i < tiles; i += NT) z.tile[i] = 0;
     int bin = 0;
     uint64_t above = 0, W = 0;
-    FiltBound bound{0.f, 0.f, 0.f};
-    float m;
-    if constexpr (MODE == kFiltTopK) {
-        bound = filt_bound<NT>(a, w.run, run_bins, s);
-        m = bound.m;
-    } else {
-        m = filt_row_max(a, w, s);
-    }
+    const FiltBound bound{0.f, 0.f, 0.f};
+    const float m = filt_row_max(a, w, s);
     if constexpr (MODE == kFiltTopP) bin = filt_mass_cut<NT>(a, w.mass_bins, s, &above, &W);
     __syncthreads();
     if (m > -INFINITY) filt_gather<NT, BF16, MODE>(a, row, first, end, m, bin, bound, z);
@@ -653,15 +661,14 @@ __global__ __launch_bounds__(kFiltThreads) void filt_draw_kernel(FiltArgs a) {
         const uint32_t n = z.count;
         // a block whose part does not fit makes the row's list overflow
         if (tid == 0 && n != 0)
-            z.base = __hip_atomic_fetch_add(&w.count, n <= kFiltHeld ? n : (uint32_t)kFiltList + 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            z.base = __hip_atomic_fetch_add(&w.count, n <= kFiltHeld ? n : (uint32_t)kFiltHeld + 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         __syncthreads();
         if (n <= kFiltHeld)
             for (uint32_t i = tid; i < n; i += NT)
-                if (z.base + i < kFiltList) __hip_atomic_store(&w.list[z.base + i], z.list[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                if (z.base + i < kFiltHeld) __hip_atomic_store(&w.list[z.base + i], z.list[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
-    if constexpr (MODE != kFiltTopK)
-        for (int i = tid; i < tiles; i += NT)
-            __hip_atomic_store(&w.tile[first / TILE + i], z.tile[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    for (int i = tid; i < tiles; i += NT)
+        __hip_atomic_store(&w.tile[first / TILE + i], z.tile[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     if (tid == 0)
@@ -672,13 +679,11 @@ __global__ __launch_bounds__(kFiltThreads) void filt_draw_kernel(FiltArgs a) {
     // ---- the row's last workgroup
     const float u = a.u[blockIdx.y];
     const uint32_t count = MODE == kFiltAll ? 0u : __hip_atomic_load(&w.count, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    if constexpr (MODE != kFiltTopK) {
-        const int all = (a.V + TILE - 1) / TILE;
+    const int all = (a.V + TILE - 1) / TILE;
 #pragma unroll
-        for (int i = 0; i < kFiltTiles / NT; ++i) {
-            const int t = i * NT + tid;
-            z.tile[t] = t < all ? __hip_atomic_load(&w.tile[t], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0ull;
-        }
+    for (int i = 0; i < kFiltTiles / NT; ++i) {
+        const int t = i * NT + tid;
+        z.tile[t] = t < all ? __hip_atomic_load(&w.tile[t], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0ull;
     }
     __syncthreads();
     if (tid == 0) w.counter = 0, w.count = 0;
@@ -688,11 +693,67 @@ __global__ __launch_bounds__(kFiltThreads) void filt_draw_kernel(FiltArgs a) {
     if (tid == 0) a.out[blockIdx.y] = token;
 }
 
+// Top-k, or min-p alone, after the maxima: a workgroup a row. Only runs whose maximum is within the bound
+// hold logits to be listed, some top_k of them, so that the row is read once in all.
+template <int NT, bool BF16>
+__global__ __launch_bounds__(NT) void filt_list_kernel(FiltArgs a) {
+    constexpr int E = BF16 ? 8 : 4, TILE = E * kFiltThreads;
+    __shared__ FiltShared<NT> s;
+    __shared__ FiltLast<kFiltHeldK> z;
+    __shared__ uint32_t run_bins[kFiltRunBins];
+    __shared__ uint32_t picked[kFiltHeldK];
+    __shared__ uint32_t n_picked;
+    const int tid = threadIdx.x;
+    const FiltRow& w = a.ws[blockIdx.x];
+    const char* const row = filt_row<BF16>(a, blockIdx.x);
+    const float u = a.u[blockIdx.x];
+    if (tid == 0) z.count = 0, n_picked = 0;
+    const FiltBound bound = filt_bound<NT>(a, w.run, run_bins, s, [&](int r) {
+        const uint32_t at = atomicAdd(&n_picked, 1u);
+        if (at < kFiltHeldK) picked[at] = r;
+    });
+    __syncthreads();
+    const int lanes = a.run_lanes, lg = __builtin_ctz(lanes), vg = lg + __builtin_ctz(kFiltBatch);   // vectors of a run: 2^vg
+    const int per_block = filt_runs<kFiltThreads, BF16>(a.chunk, lanes);
+    const uint32_t n = n_picked;
+    if (n <= kFiltHeldK) {
+        for (int i = tid; i < (int)n << vg; i += NT) {
+            const int r = (int)picked[i >> vg], v = i & ((1 << vg) - 1), in = (r % per_block) << lg;
+            const int first = r / per_block * a.chunk, end = min(first + a.chunk, a.V);
+            const int at = first + (in / kFiltThreads * kFiltBatch + (v >> lg)) * TILE + (in % kFiltThreads + (v & (lanes - 1))) * E;
+            float l[E];
+            filt_load<BF16>(row, at, end, l);
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const float x = filt_clean(l[e]);
+                if (at + e < end && bound.takes(x)) {
+                    const uint32_t to = atomicAdd(&z.count, 1u);
+                    if (to < kFiltHeldK) z.list[to] = (unsigned long long)filt_key(x) << 32 | (uint32_t)(at + e);
+                }
+            }
+        }
+    }
+    __syncthreads();
+    const uint32_t count = n <= kFiltHeldK ? z.count : kFiltHeldK + 1;
+    int token;
+    if (count > kFiltHeldK && a.top_k >= a.V && a.top_p >= 1.0f && bound.m > -INFINITY) {
+        // min-p that keeps many: by tiles
+        for (int i = tid; i < kFiltTiles; i += NT) z.tile[i] = 0;
+        __syncthreads();
+        filt_gather<NT, BF16, kFiltAll>(a, row, 0, a.V, bound.m, 0, bound, z);
+        __syncthreads();
+        token = filt_last<NT, BF16, kFiltAll>(a, row, bound.m, u, 0, 0, 0, nullptr, s, z);
+    } else {
+        token = filt_last<NT, BF16, kFiltTopK>(a, row, bound.m, u, 0, 0, count, nullptr, s, z);
+    }
+    if (tid == 0) a.out[blockIdx.x] = token;
+}
+
 // All steps in one launch, a workgroup a row.
 template <int NT, bool BF16, int MODE>
 __global__ __launch_bounds__(NT) void filt_one_kernel(FiltArgs a) {
     __shared__ FiltShared<NT> s;
-    __shared__ FiltLast z;
+    __shared__ FiltLast<MODE == kFiltTopK ? kFiltHeldK : kFiltHeld> z;
     __shared__ uint32_t run_bins[MODE == kFiltTopK ? kFiltRunBins : 1];
     __shared__ float runs[MODE == kFiltTopK ? kFiltRuns : 1];
     __shared__ unsigned long long masses[MODE == kFiltTopP ? kFiltMassBins : 1];
@@ -708,7 +769,7 @@ __global__ __launch_bounds__(NT) void filt_one_kernel(FiltArgs a) {
     FiltBound bound{0.f, 0.f, 0.f};
     if constexpr (MODE == kFiltTopK) {
         __syncthreads();
-        bound = filt_bound<NT>(a, runs, run_bins, s);
+        bound = filt_bound<NT>(a, runs, run_bins, s, [](int) {});
         m = bound.m;
     } else {
         m = filt_max<NT>(m, &least, s);
@@ -725,8 +786,8 @@ __global__ __launch_bounds__(NT) void filt_one_kernel(FiltArgs a) {
     if (tid == 0) a.out[blockIdx.x] = token;
 }
 
-// A workgroup a row: small vocabularies, and rows enough to fill the chip.
-static bool filt_one(int64_t rows, int64_t vocab) { return vocab <= kFiltOneVocab || rows >= prefill_cus() / 2; }
+// One launch: small vocabularies, and rows enough to fill the chip where all of a row is looked at again.
+static bool filt_one(int64_t rows, int64_t vocab, bool again) { return vocab <= kFiltOneVocab || (again && rows >= prefill_cus() / 2); }
 
 // Blocks of a row: some four workgroups a CU in all, blocks of whole tiles.
 static void filt_split(int64_t rows, int64_t vocab, int* blocks, int* chunk) {
@@ -748,7 +809,8 @@ static void filt_launch_one(FiltArgs a, int64_t rows, hipStream_t stream) {
 
 template <bool BF16>
 static void filt_launch(FiltArgs a, int64_t rows, hipStream_t stream) {
-    if (a.ws == nullptr) {
+    const bool list = a.top_k < a.V || (a.top_p >= 1.0f && a.min_mass > 1);
+    if (filt_one(rows, a.V, !list)) {
         if (a.V <= kFiltOneVocab) filt_launch_one<256, BF16>(a, rows, stream);
         else filt_launch_one<1024, BF16>(a, rows, stream);
         return;
@@ -757,9 +819,9 @@ static void filt_launch(FiltArgs a, int64_t rows, hipStream_t stream) {
     for (a.run_lanes = 1; a.blocks * filt_runs<kFiltThreads, BF16>(a.chunk, a.run_lanes) > kFiltRuns; a.run_lanes *= 2) {}
     a.runs = a.blocks * filt_runs<kFiltThreads, BF16>(a.chunk, a.run_lanes);
     const dim3 t(kFiltThreads), grid(a.blocks, (unsigned)rows);
-    if (a.top_k < a.V) {
+    if (list) {
         hipLaunchKernelGGL((filt_max_kernel<BF16, kFiltTopK>), grid, t, 0, stream, a);
-        hipLaunchKernelGGL((filt_draw_kernel<BF16, kFiltTopK>), grid, t, 0, stream, a);
+        hipLaunchKernelGGL((filt_list_kernel<kFiltListThreads, BF16>), dim3((unsigned)rows), dim3(kFiltListThreads), 0, stream, a);
         return;
     }
     hipLaunchKernelGGL((filt_max_kernel<BF16, kFiltAll>), grid, t, 0, stream, a);
@@ -776,7 +838,7 @@ static void filt_launch(FiltArgs a, int64_t rows, hipStream_t stream) {
 using namespace efm;
 
 extern "C" size_t efm_sampler_filtered_workspace_bytes(int64_t rows, int64_t vocab) {
-    return rows <= 0 || filt_one(rows, vocab) ? 0 : (size_t)rows * sizeof(FiltRow);
+    return rows <= 0 || vocab <= kFiltOneVocab ? 0 : (size_t)rows * sizeof(FiltRow);
 }
 
 extern "C" int efm_sampler_filtered(int64_t rows, int64_t vocab, const void* logits, int32_t logits_dtype, int64_t logits_stride,
