@@ -22,8 +22,9 @@
 //                        ids that are surely in N, and a list of the ids of the bin in which N ends;
 //                        N's end in that list, then the tile as above
 //   top-k                1. the maxima of runs of 32 logits: the top_k-th largest of those bounds the
-//                        top_k-th logit from below  2. a list of the ids above the bound; the ends of
-//                        K and N in it, and the draw
+//                        top_k-th logit from below  2. a list of the ids above the bound, from the runs
+//                        that reach it; the ends of K and N in it, and the draw
+// Top-p's third step is done so too where few runs reach N's end, and min-p's second.
 // Few rows of a large vocabulary are cut into blocks of a workgroup each, a launch a step, and what
 // follows the last step's pass is done by the row's last workgroup to arrive. Small vocabularies and
 // many rows take one launch, a workgroup a row. Where the list does not fit (thousands of equal logits)
@@ -44,7 +45,7 @@ constexpr double kFiltOne = 17592186044416.0;   // 2^44
 constexpr int kFiltBlocks = 128;                 // of a row, at most
 constexpr int kFiltTiles = 1024;                 // of a row: 1024 logits or more each
 constexpr int kFiltMassBins = 1024, kFiltBinsPerOctave = 22;   // masses from 2^0 to below 2^-46
-constexpr int kFiltRuns = 8192;                  // runs of logits whose maxima are kept
+constexpr int kFiltRuns = 5120;                  // runs of neighbouring logits whose maxima are kept, at most
 constexpr int kFiltRunBins = 1024;
 constexpr int kFiltHeld = 1024, kFiltHeldK = 2048;   // entries of a list that a workgroup holds with their masses; top-k
 constexpr int kFiltOneVocab = 16384;             // vocabularies of one launch
@@ -74,7 +75,7 @@ struct FiltArgs {
     int32_t* out;
     FiltRow* ws;
     int blocks, chunk;    // of a row; logits of a block
-    int run_lanes, runs;  // neighbouring threads that share a run; runs of a row
+    int run_lanes, runs;  // 16-byte loads of a run; runs of a row
 };
 
 enum { kFiltAll, kFiltTopP, kFiltTopK };
@@ -154,10 +155,9 @@ __device__ __forceinline__ void filt_load(const void* row, int i, int end, float
 }
 
 // A row's logits [first, end), first a multiple of a tile: f(tile of the range, first id, the thread's
-// E logits as they are (-inf past the end), how many of them there are), by all threads together;
-// after each batch g(batch).
-template <int NT, bool BF16, typename F, typename G>
-__device__ __forceinline__ void filt_tiles(const void* row, int first, int end, F f, G g) {
+// E logits as they are (-inf past the end), how many of them there are), by all threads together.
+template <int NT, bool BF16, typename F>
+__device__ __forceinline__ void filt_tiles(const void* row, int first, int end, F f) {
     constexpr int E = BF16 ? 8 : 4, U = kFiltBatch, TILE = E * NT;
     const bool aligned = (reinterpret_cast<uintptr_t>(row) & 15) == 0;
     for (int t0 = 0; first + t0 * TILE < end; t0 += U) {
@@ -175,12 +175,7 @@ __device__ __forceinline__ void filt_tiles(const void* row, int first, int end, 
             filt_unpack<BF16>(x[j], l);
             f(t0 + j, i, l, min(max(end - i, 0), E));
         }
-        g(t0 / U);
     }
-}
-template <int NT, bool BF16, typename F>
-__device__ __forceinline__ void filt_tiles(const void* row, int first, int end, F f) {
-    filt_tiles<NT, BF16>(row, first, end, f, [](int) {});
 }
 
 // A 64-bit value moved across lanes, 0 where the source is none.
@@ -349,6 +344,55 @@ __device__ __forceinline__ int filt_choose(const FiltArgs& a, uint32_t low, uint
     return filt_pick<NT>(true, 0, (uint32_t)a.V - 1, filt_draw(u, M), a, s, left).id;
 }
 
+// The same where every thread has an entry at most (x: ~key << 32 | id, and its mass), by ranks: the
+// entries before one are counted, it moves to that place, and K, N and the draw are prefix sums. W: the
+// mass that top_p is of (0: K's). order and mass are LDS of NT entries each.
+template <int NT>
+__device__ __forceinline__ int filt_choose_held(const FiltArgs& a, uint32_t count, unsigned long long x, uint64_t w, uint64_t W, float u,
+                                                unsigned long long* order, unsigned long long* mass, FiltShared<NT>& s) {
+    const int tid = threadIdx.x;
+    const bool on = tid < (int)count;
+    const int pairs = ((int)count + 1) / 2;
+    // places: of entries y(j), two a read, those below mine
+    auto place = [&](unsigned long long mine) {
+        int n = 0;
+        for (int j = 0; j < pairs; ++j) {
+            const ulonglong2 y = reinterpret_cast<const ulonglong2*>(order)[j];
+            n += (y.x < mine) + (y.y < mine);
+        }
+        return n;
+    };
+    __syncthreads();
+    order[tid] = on ? x : ~0ull;
+    __syncthreads();
+    int at = tid / kWave * kWave < (int)count ? place(x) : 0;
+    __syncthreads();
+    if (on) order[at] = x, mass[at] = w;
+    __syncthreads();
+    x = on ? order[tid] : ~0ull;
+    w = on && tid < a.top_k ? mass[tid] : 0ull;
+    if (a.top_p < 1.0f) {
+        uint64_t all;
+        const uint64_t before = filt_scan<NT>(w, s, &all);
+        if (before >= filt_need(a.top_p, W != 0 ? W : all)) w = 0;
+    }
+    // by id: what has mass comes first, in the order of ids
+    const unsigned long long id = w != 0 ? x & 0xffffffffull : ~0ull;
+    __syncthreads();
+    order[tid] = id;
+    __syncthreads();
+    at = tid / kWave * kWave < (int)count && w != 0 ? place(id) : NT - 1;
+    mass[tid] = 0;
+    __syncthreads();
+    if (w != 0) order[at] = id, mass[at] = w;
+    __syncthreads();
+    uint64_t M;
+    const uint64_t own = mass[tid], excl = filt_scan<NT>(own, s, &M), r = filt_draw(u, M);
+    if (excl <= r && r - excl < own) s.found[0] = (uint32_t)order[tid];
+    __syncthreads();
+    return (int)s.found[0];
+}
+
 // The same over the row itself: for what fits nowhere.
 template <int NT, bool BF16>
 __device__ __noinline__ int filt_choose_row(const FiltArgs& a, const void* row, float m, float u, FiltShared<NT>& s) {
@@ -377,15 +421,15 @@ __device__ __forceinline__ FiltBound filt_bound(const FiltArgs& a, const float* 
     const int tid = threadIdx.x;
     float x[HELD], m = -INFINITY, least = INFINITY;
 #pragma unroll
+    for (int i = 0; i < HELD; ++i) x[i] = run[min(i * NT + tid, a.runs - 1)];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) bins[i * NT + tid] = 0;
+#pragma unroll
     for (int i = 0; i < HELD; ++i) {
-        const int r = i * NT + tid;
-        x[i] = -INFINITY;
-        if (i * NT < a.runs && r < a.runs) x[i] = run[r];
+        x[i] = i * NT + tid < a.runs ? x[i] : -INFINITY;
         m = fmaxf(m, x[i]);
         least = x[i] > -INFINITY ? fminf(least, x[i]) : least;
     }
-#pragma unroll
-    for (int i = 0; i < PER; ++i) bins[i * NT + tid] = 0;
     m = filt_max<NT>(m, &least, s);
     // few runs for so large a top_k, equal runs or infinite ones: all but -inf is listed
     FiltBound b{m, (float)(kFiltRunBins - 1) / (m - least), INFINITY};
@@ -446,26 +490,28 @@ struct FiltLast {
     uint32_t count, base;
 };
 
-// The maximum of [first, end) and, for top-k, of its runs: those of a batch of a thread's loads, or of
-// run_lanes threads'. `runs` is where the range's begin.
-template <int NT, bool BF16, int MODE>
+// The maximum of [first, end) and, where runs is not null, those of the row's runs in it.
+template <int NT, bool BF16>
 __device__ __forceinline__ float filt_maxima(const FiltArgs& a, const void* row, int first, int end, float* runs) {
     constexpr int E = BF16 ? 8 : 4;
-    float m = -INFINITY, x = -INFINITY;
-    filt_tiles<NT, BF16>(
-        row, first, end,
-        [&](int, int, const float (&l)[E], int) {
+    float m = -INFINITY;
+    const int lanes = a.run_lanes, lg = __builtin_ctz(lanes);
+    filt_tiles<NT, BF16>(row, first, end, [&](int, int i, const float (&l)[E], int) {
+        float x = l[0];
 #pragma unroll
-            for (int e = 0; e < E; ++e) x = fmaxf(x, l[e]);   // not a NaN
-        },
-        [&](int batch) {
-            m = fmaxf(m, x);
-            if constexpr (MODE == kFiltTopK) {
-                for (int off = 1; off < a.run_lanes; off *= 2) x = fmaxf(x, __shfl_xor(x, off, kWave));
-                if (((int)threadIdx.x & (a.run_lanes - 1)) == 0) runs[(batch * NT + (int)threadIdx.x) / a.run_lanes] = x;
-            }
-            x = -INFINITY;
-        });
+        for (int e = 1; e < E; ++e) x = fmaxf(x, l[e]);
+        x = fmaxf(x, -INFINITY);   // not a NaN
+        m = fmaxf(m, x);
+        if (runs == nullptr) return;
+        if (lanes >= 2) x = fmaxf(x, dpp_f32<0xB1>(x));
+        if (lanes >= 4) x = fmaxf(x, dpp_f32<0x4E>(x));
+        if (lanes >= 8) x = fmaxf(x, dpp_f32<0x141>(x));
+        if (lanes >= 16) x = fmaxf(x, dpp_f32<0x140>(x));
+        if (lanes >= 32) x = fmaxf(x, __shfl_xor(x, 16, kWave));
+        if (lanes >= 64) x = fmaxf(x, __shfl_xor(x, 32, kWave));
+        const int r = (i / E) >> lg;
+        if ((threadIdx.x & (lanes - 1)) == 0 && r < a.runs) runs[r] = x;
+    });
     return m;
 }
 
@@ -529,6 +575,16 @@ __device__ __forceinline__ int filt_last(const FiltArgs& a, const void* row, flo
     const uint32_t high = filt_key(m);
     if (m == -INFINITY) return -1;
     if (count > Last::kHeld) return filt_choose_row<NT, BF16>(a, row, m, u, s);
+    if (MODE == kFiltTopK && count <= NT) {
+        unsigned long long x = ~0ull;
+        uint64_t mass = 0;
+        if (tid < (int)count) {
+            x = z.list[tid];
+            mass = filt_mass(a, filt_logit((uint32_t)(x >> 32)), m);
+            x = (unsigned long long)~(uint32_t)(x >> 32) << 32 | (uint32_t)x;
+        }
+        return filt_choose_held<NT>(a, count, x, mass, W, u, z.list, z.mass, s);
+    }
     uint32_t low = ~0u;
     for (uint32_t i = tid; i < count; i += NT) {
         const unsigned long long x = list != nullptr ? __hip_atomic_load(&list[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : z.list[i];
@@ -590,29 +646,15 @@ __device__ __forceinline__ const char* filt_row(const FiltArgs& a, unsigned r) {
     return static_cast<const char*>(a.logits) + (int64_t)r * a.stride * (BF16 ? 2 : 4);
 }
 
-// Runs of [0, logits) of a row that threads of NT go through from its start.
-template <int NT, bool BF16>
-__host__ __device__ constexpr int filt_runs(int logits, int run_lanes) {
-    constexpr int BATCH = kFiltBatch * (BF16 ? 8 : 4) * NT;
-    return (logits + BATCH - 1) / BATCH * (NT / run_lanes);
-}
-
 // 1. Block maxima, and those of runs.
-template <bool BF16, int MODE>
+template <bool BF16>
 __global__ __launch_bounds__(kFiltThreads) void filt_max_kernel(FiltArgs a) {
     __shared__ FiltShared<kFiltThreads> s;
     FiltRow& w = a.ws[blockIdx.y];
     const int first = blockIdx.x * a.chunk, end = min(first + a.chunk, a.V);
-    float* const runs = w.run + blockIdx.x * filt_runs<kFiltThreads, BF16>(a.chunk, a.run_lanes);
-    float m = filt_maxima<kFiltThreads, BF16, MODE>(a, filt_row<BF16>(a, blockIdx.y), first, end, runs);
-    if constexpr (MODE == kFiltTopK) {   // the last block may end before its runs do
-        const int done = filt_runs<kFiltThreads, BF16>(end - first, a.run_lanes), all = filt_runs<kFiltThreads, BF16>(a.chunk, a.run_lanes);
-        for (int i = done + (int)threadIdx.x; i < all; i += kFiltThreads) runs[i] = -INFINITY;
-    } else {
-        float least = 0.f;
-        m = filt_max<kFiltThreads>(m, &least, s);
-        if (threadIdx.x == 0) w.bmax[blockIdx.x] = m;
-    }
+    float m = filt_maxima<kFiltThreads, BF16>(a, filt_row<BF16>(a, blockIdx.y), first, end, a.runs > 0 ? w.run : nullptr), least = 0.f;
+    m = filt_max<kFiltThreads>(m, &least, s);
+    if (threadIdx.x == 0) w.bmax[blockIdx.x] = m;
 }
 
 // The row's maximum, from its blocks'.
@@ -697,7 +739,7 @@ __global__ __launch_bounds__(kFiltThreads) void filt_draw_kernel(FiltArgs a) {
 // hold logits to be listed, some top_k of them, so that the row is read once in all.
 template <int NT, bool BF16>
 __global__ __launch_bounds__(NT) void filt_list_kernel(FiltArgs a) {
-    constexpr int E = BF16 ? 8 : 4, TILE = E * kFiltThreads;
+    constexpr int E = BF16 ? 8 : 4;
     __shared__ FiltShared<NT> s;
     __shared__ FiltLast<kFiltHeldK> z;
     __shared__ uint32_t run_bins[kFiltRunBins];
@@ -713,14 +755,11 @@ __global__ __launch_bounds__(NT) void filt_list_kernel(FiltArgs a) {
         if (at < kFiltHeldK) picked[at] = r;
     });
     __syncthreads();
-    const int lanes = a.run_lanes, lg = __builtin_ctz(lanes), vg = lg + __builtin_ctz(kFiltBatch);   // vectors of a run: 2^vg
-    const int per_block = filt_runs<kFiltThreads, BF16>(a.chunk, lanes);
+    const int lg = __builtin_ctz(a.run_lanes);
     const uint32_t n = n_picked;
     if (n <= kFiltHeldK) {
-        for (int i = tid; i < (int)n << vg; i += NT) {
-            const int r = (int)picked[i >> vg], v = i & ((1 << vg) - 1), in = (r % per_block) << lg;
-            const int first = r / per_block * a.chunk, end = min(first + a.chunk, a.V);
-            const int at = first + (in / kFiltThreads * kFiltBatch + (v >> lg)) * TILE + (in % kFiltThreads + (v & (lanes - 1))) * E;
+        for (int i = tid; i < (int)n << lg; i += NT) {
+            const int at = (((int)picked[i >> lg] << lg) + (i & (a.run_lanes - 1))) * E, end = a.V;
             float l[E];
             filt_load<BF16>(row, at, end, l);
 #pragma unroll
@@ -763,7 +802,7 @@ __global__ __launch_bounds__(NT) void filt_one_kernel(FiltArgs a) {
     for (int i = tid; i < kFiltTiles; i += NT) z.tile[i] = 0;
     if constexpr (MODE == kFiltTopP)
         for (int i = tid; i < kFiltMassBins; i += NT) masses[i] = 0;
-    float m = filt_maxima<NT, BF16, MODE>(a, row, 0, a.V, runs), least = 0.f;
+    float m = filt_maxima<NT, BF16>(a, row, 0, a.V, MODE == kFiltTopK ? runs : nullptr), least = 0.f;
     int bin = 0;
     uint64_t above = 0, W = 0;
     FiltBound bound{0.f, 0.f, 0.f};
@@ -798,9 +837,7 @@ static void filt_split(int64_t rows, int64_t vocab, int* blocks, int* chunk) {
 }
 
 template <int NT, bool BF16>
-static void filt_launch_one(FiltArgs a, int64_t rows, hipStream_t stream) {
-    for (a.run_lanes = 1; filt_runs<NT, BF16>(a.V, a.run_lanes) > kFiltRuns; a.run_lanes *= 2) {}
-    a.runs = filt_runs<NT, BF16>(a.V, a.run_lanes);
+static void filt_launch_one(const FiltArgs& a, int64_t rows, hipStream_t stream) {
     const dim3 grid((unsigned)rows), t(NT);
     if (a.top_k < a.V) hipLaunchKernelGGL((filt_one_kernel<NT, BF16, kFiltTopK>), grid, t, 0, stream, a);
     else if (a.top_p < 1.0f) hipLaunchKernelGGL((filt_one_kernel<NT, BF16, kFiltTopP>), grid, t, 0, stream, a);
@@ -809,6 +846,9 @@ static void filt_launch_one(FiltArgs a, int64_t rows, hipStream_t stream) {
 
 template <bool BF16>
 static void filt_launch(FiltArgs a, int64_t rows, hipStream_t stream) {
+    const int vectors = (a.V + (BF16 ? 7 : 3)) / (BF16 ? 8 : 4);
+    while ((vectors + a.run_lanes - 1) / a.run_lanes > kFiltRuns) a.run_lanes *= 2;
+    a.runs = (vectors + a.run_lanes - 1) / a.run_lanes;
     const bool list = a.top_k < a.V || (a.top_p >= 1.0f && a.min_mass > 1);
     if (filt_one(rows, a.V, !list)) {
         if (a.V <= kFiltOneVocab) filt_launch_one<256, BF16>(a, rows, stream);
@@ -816,16 +856,12 @@ static void filt_launch(FiltArgs a, int64_t rows, hipStream_t stream) {
         return;
     }
     filt_split(rows, a.V, &a.blocks, &a.chunk);
-    for (a.run_lanes = 1; a.blocks * filt_runs<kFiltThreads, BF16>(a.chunk, a.run_lanes) > kFiltRuns; a.run_lanes *= 2) {}
-    a.runs = a.blocks * filt_runs<kFiltThreads, BF16>(a.chunk, a.run_lanes);
     const dim3 t(kFiltThreads), grid(a.blocks, (unsigned)rows);
+    if (!list) a.runs = 0;
+    hipLaunchKernelGGL(filt_max_kernel<BF16>, grid, t, 0, stream, a);
     if (list) {
-        hipLaunchKernelGGL((filt_max_kernel<BF16, kFiltTopK>), grid, t, 0, stream, a);
         hipLaunchKernelGGL((filt_list_kernel<kFiltListThreads, BF16>), dim3((unsigned)rows), dim3(kFiltListThreads), 0, stream, a);
-        return;
-    }
-    hipLaunchKernelGGL((filt_max_kernel<BF16, kFiltAll>), grid, t, 0, stream, a);
-    if (a.top_p < 1.0f) {
+    } else if (a.top_p < 1.0f) {
         hipLaunchKernelGGL(filt_mass_kernel<BF16>, grid, t, 0, stream, a);
         hipLaunchKernelGGL((filt_draw_kernel<BF16, kFiltTopP>), grid, t, 0, stream, a);
     } else {
@@ -881,7 +917,8 @@ extern "C" int efm_sampler_filtered(int64_t rows, int64_t vocab, const void* log
     a.u = uniforms;
     a.out = token_out;
     a.ws = need > 0 ? static_cast<FiltRow*>(workspace) : nullptr;
-    a.blocks = a.chunk = a.run_lanes = a.runs = 0;
+    a.blocks = a.chunk = a.runs = 0;
+    a.run_lanes = 1;
     if (logits_dtype == EFM_DTYPE_BF16) filt_launch<true>(a, rows, stream);
     else filt_launch<false>(a, rows, stream);
     return check_launch("sampler_filtered");
