@@ -47,10 +47,11 @@ constexpr int kFiltTiles = 1024;                 // of a row: 1024 logits or mor
 constexpr int kFiltMassBins = 1024, kFiltBinsPerOctave = 22;   // masses from 2^0 to below 2^-46
 constexpr int kFiltRuns = 5120;                  // runs of neighbouring logits whose maxima are kept, at most
 constexpr int kFiltRunBins = 1024;
+constexpr int kFiltFewRuns = 512;                // that one workgroup goes through
 constexpr int kFiltHeld = 1024, kFiltHeldK = 2048;   // entries of a list that a workgroup holds with their masses; top-k
 constexpr int kFiltOneVocab = 16384;             // vocabularies of one launch
 
-// One row's part of the workspace. mass_bins, counter and count are zero between calls.
+// One row's part of the workspace.
 struct FiltRow {
     unsigned long long mass_bins[kFiltMassBins];
     uint32_t counter, count;
@@ -80,27 +81,32 @@ struct FiltArgs {
 
 enum { kFiltAll, kFiltTopP, kFiltTopK };
 
-// w of a logit, m the row's largest. 2^t, t = (l - m) log2(e) / T, as 2^n 2^f with the series of
-// exp(f ln 2), |f| <= 1/2: the term after the last is below 2^-52. Adding 2^52 rounds to an integer.
+// w of a logit, m the row's largest. 2^t, t = (l - m) log2(e) / T, is 2^n 2^f with the series of
+// exp(f ln 2), |f| <= 1/2: the term after the last is below 2^-52. Adding 1.5 2^52 rounds t to an integer,
+// and a last step to p 2^(n + 44) + 2^52 leaves w in the low bits. Without branches, so that a thread's
+// logits go through side by side (33 rows of 151936: 14.9 -> 9.5 us for the masses by bin).
 __device__ __forceinline__ uint64_t filt_mass(const FiltArgs& a, float l, float m) {
-    if (l != m && !((l - m) * a.to_log2f > a.low)) return 0;
     const double t = l == m ? 0.0 : ((double)l - (double)m) * a.to_log2;
-    const double n = __builtin_rint(t), f = (t - n) * 0.69314718055994530942;
-    double p = 1.0 / 479001600.0;
-    p = __builtin_fma(p, f, 1.0 / 39916800.0);
-    p = __builtin_fma(p, f, 1.0 / 3628800.0);
-    p = __builtin_fma(p, f, 1.0 / 362880.0);
-    p = __builtin_fma(p, f, 1.0 / 40320.0);
-    p = __builtin_fma(p, f, 1.0 / 5040.0);
-    p = __builtin_fma(p, f, 1.0 / 720.0);
-    p = __builtin_fma(p, f, 1.0 / 120.0);
-    p = __builtin_fma(p, f, 1.0 / 24.0);
-    p = __builtin_fma(p, f, 1.0 / 6.0);
-    p = __builtin_fma(p, f, 0.5);
+    const double near = t + 6755399441055744.0, f = t - (near - 6755399441055744.0);
+    constexpr double c = 0.69314718055994530942, c2 = c * c / 2, c3 = c2 * c / 3, c4 = c3 * c / 4, c5 = c4 * c / 5, c6 = c5 * c / 6,
+                     c7 = c6 * c / 7, c8 = c7 * c / 8, c9 = c8 * c / 9, c10 = c9 * c / 10, c11 = c10 * c / 11, c12 = c11 * c / 12;
+    double p = c12;
+    p = __builtin_fma(p, f, c11);
+    p = __builtin_fma(p, f, c10);
+    p = __builtin_fma(p, f, c9);
+    p = __builtin_fma(p, f, c8);
+    p = __builtin_fma(p, f, c7);
+    p = __builtin_fma(p, f, c6);
+    p = __builtin_fma(p, f, c5);
+    p = __builtin_fma(p, f, c4);
+    p = __builtin_fma(p, f, c3);
+    p = __builtin_fma(p, f, c2);
+    p = __builtin_fma(p, f, c);
     p = __builtin_fma(p, f, 1.0);
-    p = __builtin_fma(p, f, 1.0);
-    const uint64_t w = __builtin_bit_cast(uint64_t, __builtin_ldexp(p, (int)n + 44) + 4503599627370496.0) & 0xfffffffffffffull;
-    return w >= a.min_mass ? w : 0;
+    const double scale = __builtin_bit_cast(double, (uint64_t)((uint32_t)__builtin_bit_cast(uint64_t, near) + 44u + 1023u) << 52);
+    const uint64_t w = __builtin_bit_cast(uint64_t, __builtin_fma(p, scale, 4503599627370496.0)) & 0xfffffffffffffull;
+    // fp32 decides what is far below (no 2^n is made of those); the largest is there even where it is infinite
+    return (l == m || (l - m) * a.to_log2f > a.low) && w >= a.min_mass ? w : 0;
 }
 
 // Bin of a mass histogram, 0 for the largest logit; it rises as the logit falls.
@@ -146,12 +152,6 @@ __device__ __forceinline__ void filt_unpack(const uint4& x, float* l) {
         if constexpr (BF16) l[2 * e] = lo_f32(w[e]), l[2 * e + 1] = hi_f32(w[e]);
         else l[e] = __uint_as_float(w[e]);
     }
-}
-
-// Logits i to i + E - 1 of a row that ends at `end`, -inf past it.
-template <bool BF16>
-__device__ __forceinline__ void filt_load(const void* row, int i, int end, float* l) {
-    filt_unpack<BF16>(filt_raw<BF16>(row, (reinterpret_cast<uintptr_t>(row) & 15) == 0, i, end), l);
 }
 
 // A row's logits [first, end), first a multiple of a tile: f(tile of the range, first id, the thread's
@@ -276,8 +276,7 @@ __device__ __forceinline__ uint64_t filt_need(float top_p, uint64_t W) {
 // The entry that holds unit `rank` of the weights of a source of (id, key, weight), each(f): in the
 // sampler's order (keys of [low, high]), or by id alone (ids of [low, high]). The range that may hold
 // it is cut into 256 bins until one entry is left, four times for keys and three for the ids of equal
-// keys at most. rank is below the sum of the weights; were it not (a workspace that was not zeroed),
-// the entry is any.
+// keys at most. rank is below the sum of the weights.
 template <int NT, typename Each>
 __device__ __forceinline__ FiltCut filt_pick(bool by_id, uint32_t low, uint32_t high, uint64_t rank, const FiltArgs& a, FiltShared<NT>& s,
                                              Each each) {
@@ -322,9 +321,10 @@ __device__ __forceinline__ FiltCut filt_pick(bool by_id, uint32_t low, uint32_t 
     return FiltCut{~0u, 0};
 }
 
-// K, N and the draw over a source of `count` entries (id, key, mass), each(f), keys of [low, high].
+// K, N and the draw over a source of `count` entries (id, key, mass), each(f), keys of [low, high]. W: the
+// mass that top_p is of (0: K's).
 template <int NT, typename Each>
-__device__ __forceinline__ int filt_choose(const FiltArgs& a, uint32_t low, uint32_t high, uint32_t count, float u, FiltShared<NT>& s,
+__device__ __forceinline__ int filt_choose(const FiltArgs& a, uint32_t low, uint32_t high, uint32_t count, uint64_t W, float u, FiltShared<NT>& s,
                                            Each each) {
     FiltCut kept{0u, a.V};
     if ((uint32_t)a.top_k < count)
@@ -338,57 +338,64 @@ __device__ __forceinline__ int filt_choose(const FiltArgs& a, uint32_t low, uint
     };
     uint64_t M = total();
     if (a.top_p < 1.0f) {
-        kept = filt_pick<NT>(false, low, high, filt_need(a.top_p, M) - 1, a, s, left);
+        kept = filt_pick<NT>(false, low, high, filt_need(a.top_p, W != 0 ? W : M) - 1, a, s, left);
         M = total();
     }
     return filt_pick<NT>(true, 0, (uint32_t)a.V - 1, filt_draw(u, M), a, s, left).id;
 }
 
-// The same where every thread has an entry at most (x: ~key << 32 | id, and its mass), by ranks: the
-// entries before one are counted, it moves to that place, and K, N and the draw are prefix sums. W: the
-// mass that top_p is of (0: K's). order and mass are LDS of NT entries each.
+// The same where every thread has an entry at most, by ranks: entries move to their places in the order
+// of ids, their places by key are counted (so that of equal keys the lowest id comes first), and K, N and
+// the draw are prefix sums. W: the mass that top_p is of (0: K's). keys, ids and mass are LDS of NT
+// entries each.
 template <int NT>
-__device__ __forceinline__ int filt_choose_held(const FiltArgs& a, uint32_t count, unsigned long long x, uint64_t w, uint64_t W, float u,
-                                                unsigned long long* order, unsigned long long* mass, FiltShared<NT>& s) {
-    const int tid = threadIdx.x;
+__device__ __forceinline__ int filt_choose_held(const FiltArgs& a, uint32_t count, uint32_t key, uint32_t id, uint64_t w, uint64_t W, float u,
+                                                uint32_t* keys, uint32_t* ids, unsigned long long* mass, FiltShared<NT>& s) {
+    const int tid = threadIdx.x, n16 = ((int)count + 15) & ~15, wave0 = tid / kWave * kWave;
     const bool on = tid < (int)count;
-    const int pairs = ((int)count + 1) / 2;
-    // places: of entries y(j), two a read, those below mine
-    auto place = [&](unsigned long long mine) {
+    // how many of v[j0, j1) are below mine; 16 at a time, those past the last are the largest there are
+    auto below = [&](const uint32_t* v, int j0, int j1, uint32_t mine) {
         int n = 0;
-        for (int j = 0; j < pairs; ++j) {
-            const ulonglong2 y = reinterpret_cast<const ulonglong2*>(order)[j];
-            n += (y.x < mine) + (y.y < mine);
+        for (int j = j0; j < j1; j += 16) {
+            uint4 y[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) y[i] = reinterpret_cast<const uint4*>(v + j)[i];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) n += (y[i].x < mine) + (y[i].y < mine) + (y[i].z < mine) + (y[i].w < mine);
         }
         return n;
     };
     __syncthreads();
-    order[tid] = on ? x : ~0ull;
+    ids[tid] = on ? id : ~0u;
+    keys[tid] = ~0u;
     __syncthreads();
-    int at = tid / kWave * kWave < (int)count ? place(x) : 0;
+    int at = wave0 < (int)count ? below(ids, 0, n16, id) : 0;
     __syncthreads();
-    if (on) order[at] = x, mass[at] = w;
+    if (on) ids[at] = id, keys[at] = ~key, mass[at] = w;   // ~key: below 2^32 - 1, no key is 0
     __syncthreads();
-    x = on ? order[tid] : ~0ull;
-    w = on && tid < a.top_k ? mass[tid] : 0ull;
-    if (a.top_p < 1.0f) {
-        uint64_t all;
-        const uint64_t before = filt_scan<NT>(w, s, &all);
-        if (before >= filt_need(a.top_p, W != 0 ? W : all)) w = 0;
+    id = ids[tid], key = keys[tid], w = on ? mass[tid] : 0ull;
+    if (a.top_k < (int)count || a.top_p < 1.0f) {
+        if (wave0 < (int)count) {
+            // equal keys of lower ids count too: those of the waves before, and of the lanes before
+            at = below(keys, 0, wave0, key + 1) + below(keys, wave0, n16, key);
+            for (int j = 0; j < kWave; ++j) at += (uint32_t)__builtin_amdgcn_readlane((int)key, j) == key && j < tid % kWave;
+        }
+        __syncthreads();
+        if (on) mass[at] = w;
+        __syncthreads();
+        if (a.top_p < 1.0f) {
+            uint64_t all;
+            const uint64_t x = on && tid < a.top_k ? mass[tid] : 0ull, before = filt_scan<NT>(x, s, &all);
+            if (on) mass[tid] = tid < a.top_k && before < filt_need(a.top_p, W != 0 ? W : all);
+        } else if (on) {
+            mass[tid] = tid < a.top_k;
+        }
+        __syncthreads();
+        if (on && mass[at] == 0) w = 0;
     }
-    // by id: what has mass comes first, in the order of ids
-    const unsigned long long id = w != 0 ? x & 0xffffffffull : ~0ull;
-    __syncthreads();
-    order[tid] = id;
-    __syncthreads();
-    at = tid / kWave * kWave < (int)count && w != 0 ? place(id) : NT - 1;
-    mass[tid] = 0;
-    __syncthreads();
-    if (w != 0) order[at] = id, mass[at] = w;
-    __syncthreads();
     uint64_t M;
-    const uint64_t own = mass[tid], excl = filt_scan<NT>(own, s, &M), r = filt_draw(u, M);
-    if (excl <= r && r - excl < own) s.found[0] = (uint32_t)order[tid];
+    const uint64_t excl = filt_scan<NT>(w, s, &M), r = filt_draw(u, M);
+    if (excl <= r && r - excl < w) s.found[0] = id;
     __syncthreads();
     return (int)s.found[0];
 }
@@ -396,7 +403,7 @@ __device__ __forceinline__ int filt_choose_held(const FiltArgs& a, uint32_t coun
 // The same over the row itself: for what fits nowhere.
 template <int NT, bool BF16>
 __device__ __noinline__ int filt_choose_row(const FiltArgs& a, const void* row, float m, float u, FiltShared<NT>& s) {
-    return filt_choose<NT>(a, 0u, ~0u, (uint32_t)a.V, u, s, [&](auto f) {
+    return filt_choose<NT>(a, 0u, ~0u, (uint32_t)a.V, 0, u, s, [&](auto f) {
         filt_tiles<NT, BF16>(row, 0, a.V, [&](int, int i, const auto& l, int n) {
             constexpr int E = BF16 ? 8 : 4;
 #pragma unroll
@@ -519,11 +526,12 @@ template <int NT, bool BF16>
 __device__ __forceinline__ void filt_mass_bins(const FiltArgs& a, const void* row, int first, int end, float m, unsigned long long* bins) {
     constexpr int E = BF16 ? 8 : 4;
     filt_tiles<NT, BF16>(row, first, end, [&](int, int, const float (&l)[E], int) {
+        uint64_t x[E];
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const uint64_t x = filt_mass(a, filt_clean(l[e]), m);
-            if (x != 0) atomicAdd(&bins[filt_bin(a, l[e], m)], (unsigned long long)x);
-        }
+        for (int e = 0; e < E; ++e) x[e] = filt_mass(a, filt_clean(l[e]), m);
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            if (x[e] != 0) atomicAdd(&bins[filt_bin(a, l[e], m)], (unsigned long long)x[e]);
     });
 }
 
@@ -567,6 +575,38 @@ __device__ __forceinline__ void filt_gather(const FiltArgs& a, const void* row, 
     });
 }
 
+// Lists the logits within the bound of n picked runs.
+template <int NT, bool BF16, typename Last>
+__device__ __forceinline__ void filt_list_runs(const FiltArgs& a, const void* row, const uint32_t* picked, int n, const FiltBound& bound, Last& z) {
+    constexpr int E = BF16 ? 8 : 4;
+    const int lg = __builtin_ctz(a.run_lanes), all = n << lg;
+    const bool aligned = (reinterpret_cast<uintptr_t>(row) & 15) == 0;
+    for (int i0 = threadIdx.x; i0 < all; i0 += 4 * NT) {
+        uint4 x[4];
+        int at[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int i = min(i0 + j * NT, all - 1);
+            at[j] = (((int)picked[i >> lg] << lg) + (i & (a.run_lanes - 1))) * E;
+            if (i0 + j * NT < all) x[j] = filt_raw<BF16>(row, aligned, at[j], a.V);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (i0 + j * NT >= all) break;
+            float l[E];
+            filt_unpack<BF16>(x[j], l);
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const float y = filt_clean(l[e]);
+                if (at[j] + e < a.V && bound.takes(y)) {
+                    const uint32_t to = atomicAdd(&z.count, 1u);
+                    if (to < Last::kHeld) z.list[to] = (unsigned long long)filt_key(y) << 32 | (uint32_t)(at[j] + e);
+                }
+            }
+        }
+    }
+}
+
 // The choice from a row's list (`count` entries, in z or in `list`) and its tiles' masses (in z.tile).
 template <int NT, bool BF16, int MODE, typename Last>
 __device__ __forceinline__ int filt_last(const FiltArgs& a, const void* row, float m, float u, uint64_t above, uint64_t W, uint32_t count,
@@ -576,14 +616,10 @@ __device__ __forceinline__ int filt_last(const FiltArgs& a, const void* row, flo
     if (m == -INFINITY) return -1;
     if (count > Last::kHeld) return filt_choose_row<NT, BF16>(a, row, m, u, s);
     if (MODE == kFiltTopK && count <= NT) {
-        unsigned long long x = ~0ull;
-        uint64_t mass = 0;
-        if (tid < (int)count) {
-            x = z.list[tid];
-            mass = filt_mass(a, filt_logit((uint32_t)(x >> 32)), m);
-            x = (unsigned long long)~(uint32_t)(x >> 32) << 32 | (uint32_t)x;
-        }
-        return filt_choose_held<NT>(a, count, x, mass, W, u, z.list, z.mass, s);
+        const unsigned long long x = tid < (int)count ? z.list[tid] : 0ull;
+        const uint64_t mass = tid < (int)count ? filt_mass(a, filt_logit((uint32_t)(x >> 32)), m) : 0ull;
+        uint32_t* const keys = reinterpret_cast<uint32_t*>(z.list);
+        return filt_choose_held<NT>(a, count, (uint32_t)(x >> 32), (uint32_t)x, mass, W, u, keys, keys + NT, z.mass, s);
     }
     uint32_t low = ~0u;
     for (uint32_t i = tid; i < count; i += NT) {
@@ -603,7 +639,7 @@ __device__ __forceinline__ int filt_last(const FiltArgs& a, const void* row, flo
 #pragma unroll
         for (int w = 0; w < NT / kWave; ++w) low = min(low, s.counts[0][w]);
     }
-    if constexpr (MODE == kFiltTopK) return filt_choose<NT>(a, low, high, count, u, s, each);
+    if constexpr (MODE == kFiltTopK) return filt_choose<NT>(a, low, high, count, W, u, s, each);
     constexpr int E = BF16 ? 8 : 4, TILE = E * NT, PER = kFiltTiles / NT;
     FiltCut kept{0u, a.V};
     if constexpr (MODE == kFiltTopP) {
@@ -655,6 +691,10 @@ __global__ __launch_bounds__(kFiltThreads) void filt_max_kernel(FiltArgs a) {
     float m = filt_maxima<kFiltThreads, BF16>(a, filt_row<BF16>(a, blockIdx.y), first, end, a.runs > 0 ? w.run : nullptr), least = 0.f;
     m = filt_max<kFiltThreads>(m, &least, s);
     if (threadIdx.x == 0) w.bmax[blockIdx.x] = m;
+    if (blockIdx.x == 0) {   // what the next steps add to
+        for (int i = threadIdx.x; i < kFiltMassBins; i += kFiltThreads) w.mass_bins[i] = 0;
+        if (threadIdx.x == 0) w.counter = 0, w.count = 0;
+    }
 }
 
 // The row's maximum, from its blocks'.
@@ -685,17 +725,53 @@ __global__ __launch_bounds__(kFiltThreads) void filt_draw_kernel(FiltArgs a) {
     constexpr int NT = kFiltThreads, TILE = (BF16 ? 8 : 4) * NT;
     __shared__ FiltShared<NT> s;
     __shared__ FiltLast<kFiltHeld> z;
+    __shared__ uint32_t picked[MODE == kFiltTopP ? kFiltFewRuns : 1];
+    __shared__ uint32_t n_picked;
     const int tid = threadIdx.x;
     FiltRow& w = a.ws[blockIdx.y];
     const char* const row = filt_row<BF16>(a, blockIdx.y);
     const int first = blockIdx.x * a.chunk, end = min(first + a.chunk, a.V), tiles = (end - first + TILE - 1) / TILE;
-    if (tid == 0) z.count = 0;
+    if (tid == 0) z.count = 0, n_picked = 0;
     for (int i = tid; i < tiles; i += NT) z.tile[i] = 0;
     int bin = 0;
     uint64_t above = 0, W = 0;
     const FiltBound bound{0.f, 0.f, 0.f};
     const float m = filt_row_max(a, w, s);
-    if constexpr (MODE == kFiltTopP) bin = filt_mass_cut<NT>(a, w.mass_bins, s, &above, &W);
+    if constexpr (MODE == kFiltTopP) {
+        float x[kFiltRuns / NT];
+#pragma unroll
+        for (int i = 0; i < kFiltRuns / NT; ++i) x[i] = w.run[min(i * NT + tid, a.runs - 1)];
+        bin = filt_mass_cut<NT>(a, w.mass_bins, s, &above, &W);
+        // the runs that reach N's end
+        const FiltBound reach{m, a.to_bin, bin < kFiltMassBins - 1 ? (float)(bin + 1) : INFINITY};
+        uint32_t mine = 0;
+#pragma unroll
+        for (int i = 0; i < kFiltRuns / NT; ++i) mine += i * NT + tid < a.runs && x[i] > -INFINITY && reach.takes(x[i]);
+        const uint64_t few = filt_sum<NT>(mine, s);
+        if (few <= kFiltFewRuns) {   // the first block has them all
+            if (blockIdx.x != 0) return;
+#pragma unroll
+            for (int i = 0; i < kFiltRuns / NT; ++i)
+                if (i * NT + tid < a.runs && x[i] > -INFINITY && reach.takes(x[i])) picked[atomicAdd(&n_picked, 1u)] = i * NT + tid;
+            __syncthreads();
+            filt_list_runs<NT, BF16>(a, row, picked, (int)n_picked, reach, z);
+            __syncthreads();
+            int token;
+            if (z.count <= kFiltHeld) {
+                token = filt_last<NT, BF16, kFiltTopK>(a, row, m, a.u[blockIdx.y], 0, W, z.count, nullptr, s, z);
+            } else {
+                __syncthreads();
+                if (tid == 0) z.count = 0;
+                for (int i = tid; i < kFiltTiles; i += NT) z.tile[i] = 0;
+                __syncthreads();
+                filt_gather<NT, BF16, kFiltTopP>(a, row, 0, a.V, m, bin, bound, z);
+                __syncthreads();
+                token = filt_last<NT, BF16, kFiltTopP>(a, row, m, a.u[blockIdx.y], above, W, z.count, nullptr, s, z);
+            }
+            if (tid == 0) a.out[blockIdx.y] = token;
+            return;
+        }
+    }
     __syncthreads();
     if (m > -INFINITY) filt_gather<NT, BF16, MODE>(a, row, first, end, m, bin, bound, z);
     __syncthreads();
@@ -728,9 +804,6 @@ __global__ __launch_bounds__(kFiltThreads) void filt_draw_kernel(FiltArgs a) {
         z.tile[t] = t < all ? __hip_atomic_load(&w.tile[t], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0ull;
     }
     __syncthreads();
-    if (tid == 0) w.counter = 0, w.count = 0;
-    if constexpr (MODE == kFiltTopP)
-        for (int i = tid; i < kFiltMassBins; i += NT) w.mass_bins[i] = 0;
     const int token = filt_last<NT, BF16, MODE>(a, row, m, u, above, W, count, w.list, s, z);
     if (tid == 0) a.out[blockIdx.y] = token;
 }
@@ -755,23 +828,8 @@ __global__ __launch_bounds__(NT) void filt_list_kernel(FiltArgs a) {
         if (at < kFiltHeldK) picked[at] = r;
     });
     __syncthreads();
-    const int lg = __builtin_ctz(a.run_lanes);
     const uint32_t n = n_picked;
-    if (n <= kFiltHeldK) {
-        for (int i = tid; i < (int)n << lg; i += NT) {
-            const int at = (((int)picked[i >> lg] << lg) + (i & (a.run_lanes - 1))) * E, end = a.V;
-            float l[E];
-            filt_load<BF16>(row, at, end, l);
-#pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const float x = filt_clean(l[e]);
-                if (at + e < end && bound.takes(x)) {
-                    const uint32_t to = atomicAdd(&z.count, 1u);
-                    if (to < kFiltHeldK) z.list[to] = (unsigned long long)filt_key(x) << 32 | (uint32_t)(at + e);
-                }
-            }
-        }
-    }
+    if (n <= kFiltHeldK) filt_list_runs<NT, BF16>(a, row, picked, (int)n, bound, z);
     __syncthreads();
     const uint32_t count = n <= kFiltHeldK ? z.count : kFiltHeldK + 1;
     int token;
@@ -857,7 +915,7 @@ static void filt_launch(FiltArgs a, int64_t rows, hipStream_t stream) {
     }
     filt_split(rows, a.V, &a.blocks, &a.chunk);
     const dim3 t(kFiltThreads), grid(a.blocks, (unsigned)rows);
-    if (!list) a.runs = 0;
+    if (!list && a.top_p >= 1.0f) a.runs = 0;
     hipLaunchKernelGGL(filt_max_kernel<BF16>, grid, t, 0, stream, a);
     if (list) {
         hipLaunchKernelGGL((filt_list_kernel<kFiltListThreads, BF16>), dim3((unsigned)rows), dim3(kFiltListThreads), 0, stream, a);

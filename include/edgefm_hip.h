@@ -641,8 +641,7 @@ int efm_attention_tree(const efm_attention_ctx* ctx, const void* q, const void* 
  * temperature >= 1e-6 (smaller means greedy: use efm_sampler_greedy), top_p > 0, min_p <= 1 (not
  * above 0: off), 1 <= vocab < 2^20. The same inputs give the same token, whatever the other rows
  * are. workspace: efm_sampler_filtered_workspace_bytes(rows, vocab) bytes (0: none), 16-byte
- * aligned, zero-filled before its first use; every call leaves it zeroed again where it has to be,
- * for calls of any size. Calls that share one must be stream-ordered. Stands beside
+ * aligned, no initial contents required; calls that share one must be stream-ordered. Stands beside
  * efm_sampler_top_p, which draws its own random number for one row. */
 size_t efm_sampler_filtered_workspace_bytes(int64_t rows, int64_t vocab);
 int efm_sampler_filtered(int64_t rows, int64_t vocab, const void* logits, int32_t logits_dtype, int64_t logits_stride,

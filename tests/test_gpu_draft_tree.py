@@ -329,7 +329,7 @@ def test_attention_chain_is_causal_prefill(gpu):
 def _sample(x, u, t=1.0, k=0, p=1.0, min_p=0.0, stride=0, vocab=None, rows=None, data=None, ws=None):
     rows, vocab = rows or x.shape[0], vocab or x.shape[1]
     out = torch.full((rows + 1,), -77, dtype=torch.int32, device="cuda")
-    ws = _buf(C.load().efm_sampler_filtered_workspace_bytes(rows, vocab), 0) if ws is None else ws
+    ws = _buf(C.load().efm_sampler_filtered_workspace_bytes(rows, vocab)) if ws is None else ws
     dt = C.EFM_DTYPE_BF16 if x.dtype == torch.bfloat16 else C.EFM_DTYPE_F32
     C.call("efm_sampler_filtered", rows, vocab, data or ptr(x), dt, stride, t, k, p, min_p, ptr(u), ptr(out), ptr(ws), ws.numel(), stream())
     torch.cuda.synchronize()
@@ -454,7 +454,7 @@ def test_sampler_rows_do_not_meet(gpu):
 
 def test_sampler_workspace_serves_calls_of_any_size(gpu):
     """One workspace under calls of other sizes, filters and types, overflowing lists among them."""
-    ws = _buf(C.load().efm_sampler_filtered_workspace_bytes(64, 1 << 19), 0)
+    ws = _buf(C.load().efm_sampler_filtered_workspace_bytes(64, 1 << 19))
     for i in range(3):
         for rows, vocab, f in ((64, 20000, dict(p=0.9)), (1, 151936, dict(k=50)), (7, 500000, dict(p=0.99, t=1.5)), (33, 151936, dict(k=900, p=0.9)),
                                (2, 40000, dict()), (5, 30000, dict(t=1e6, p=0.5)), (5, 30000, dict(t=1e6, k=9)), (64, 15000, dict(min_p=0.1))):
