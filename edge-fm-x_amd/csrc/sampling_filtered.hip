@@ -106,7 +106,8 @@ __device__ __forceinline__ uint64_t filt_mass(const FiltArgs& a, float l, float 
     const double scale = __builtin_bit_cast(double, (uint64_t)((uint32_t)__builtin_bit_cast(uint64_t, near) + 44u + 1023u) << 52);
     const uint64_t w = __builtin_bit_cast(uint64_t, __builtin_fma(p, scale, 4503599627370496.0)) & 0xfffffffffffffull;
     // fp32 decides what is far below (no 2^n is made of those); the largest is there even where it is infinite
-    return (l == m || (l - m) * a.to_log2f > a.low) && w >= a.min_mass ? w : 0;
+    const bool counts = (l == m) | ((l - m) * a.to_log2f > a.low);
+    return (counts & (w >= a.min_mass)) ? w : 0;
 }
 
 // Bin of a mass histogram, 0 for the largest logit; it rises as the logit falls.
@@ -344,58 +345,58 @@ __device__ __forceinline__ int filt_choose(const FiltArgs& a, uint32_t low, uint
     return filt_pick<NT>(true, 0, (uint32_t)a.V - 1, filt_draw(u, M), a, s, left).id;
 }
 
-// The same where every thread has an entry at most, by ranks: entries move to their places in the order
-// of ids, their places by key are counted (so that of equal keys the lowest id comes first), and K, N and
-// the draw are prefix sums. W: the mass that top_p is of (0: K's). keys, ids and mass are LDS of NT
-// entries each.
+// The same where every thread has an entry at most (x: ~key << 32 | id, and its mass w), by ranks: the
+// entries before one are counted, it moves to that place, and K, N and the draw are prefix sums. W: the
+// mass that top_p is of (0: K's). order and mass are LDS of NT entries each.
 template <int NT>
-__device__ __forceinline__ int filt_choose_held(const FiltArgs& a, uint32_t count, uint32_t key, uint32_t id, uint64_t w, uint64_t W, float u,
-                                                uint32_t* keys, uint32_t* ids, unsigned long long* mass, FiltShared<NT>& s) {
-    const int tid = threadIdx.x, n16 = ((int)count + 15) & ~15, wave0 = tid / kWave * kWave;
-    const bool on = tid < (int)count;
-    // how many of v[j0, j1) are below mine; 16 at a time, those past the last are the largest there are
-    auto below = [&](const uint32_t* v, int j0, int j1, uint32_t mine) {
-        int n = 0;
-        for (int j = j0; j < j1; j += 16) {
-            uint4 y[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) y[i] = reinterpret_cast<const uint4*>(v + j)[i];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) n += (y[i].x < mine) + (y[i].y < mine) + (y[i].z < mine) + (y[i].w < mine);
-        }
-        return n;
-    };
+__device__ __forceinline__ int filt_choose_held(const FiltArgs& a, uint32_t count, unsigned long long x, uint64_t w, uint64_t W, float u,
+                                                unsigned long long* order, unsigned long long* mass, FiltShared<NT>& s) {
+    const int tid = threadIdx.x, wave0 = tid / kWave * kWave;
+    uint32_t* const ids = reinterpret_cast<uint32_t*>(order);
     __syncthreads();
-    ids[tid] = on ? id : ~0u;
-    keys[tid] = ~0u;
+    order[tid] = x;   // ~0 for threads without one
     __syncthreads();
-    int at = wave0 < (int)count ? below(ids, 0, n16, id) : 0;
-    __syncthreads();
-    if (on) ids[at] = id, keys[at] = ~key, mass[at] = w;   // ~key: below 2^32 - 1, no key is 0
-    __syncthreads();
-    id = ids[tid], key = keys[tid], w = on ? mass[tid] : 0ull;
     if (a.top_k < (int)count || a.top_p < 1.0f) {
-        if (wave0 < (int)count) {
-            // equal keys of lower ids count too: those of the waves before, and of the lanes before
-            at = below(keys, 0, wave0, key + 1) + below(keys, wave0, n16, key);
-            for (int j = 0; j < kWave; ++j) at += (uint32_t)__builtin_amdgcn_readlane((int)key, j) == key && j < tid % kWave;
-        }
+        int at = 0;
+        if (wave0 < (int)count)
+            for (int j = 0; j < (int)count; j += 16) {
+                ulonglong2 y[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) y[i] = reinterpret_cast<const ulonglong2*>(order + j)[i];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) at += (y[i].x < x) + (y[i].y < x);
+            }
         __syncthreads();
-        if (on) mass[at] = w;
+        if (tid < (int)count) order[at] = x, mass[at] = w;
         __syncthreads();
+        x = order[tid];
+        w = tid < (int)count && tid < a.top_k ? mass[tid] : 0ull;
         if (a.top_p < 1.0f) {
             uint64_t all;
-            const uint64_t x = on && tid < a.top_k ? mass[tid] : 0ull, before = filt_scan<NT>(x, s, &all);
-            if (on) mass[tid] = tid < a.top_k && before < filt_need(a.top_p, W != 0 ? W : all);
-        } else if (on) {
-            mass[tid] = tid < a.top_k;
+            const uint64_t before = filt_scan<NT>(w, s, &all);
+            if (before >= filt_need(a.top_p, W != 0 ? W : all)) w = 0;
         }
-        __syncthreads();
-        if (on && mass[at] == 0) w = 0;
     }
+    // what has mass, in the order of ids
+    const uint32_t id = w != 0 ? (uint32_t)x : ~0u;
+    __syncthreads();
+    ids[tid] = id;
+    mass[tid] = 0;
+    __syncthreads();
+    int at = 0;
+    if (wave0 < (int)count)
+        for (int j = 0; j < (int)count; j += 16) {
+            uint4 y[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) y[i] = reinterpret_cast<const uint4*>(ids + j)[i];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) at += (y[i].x < id) + (y[i].y < id) + (y[i].z < id) + (y[i].w < id);
+        }
+    if (w != 0) ids[NT + at] = id, mass[at] = w;
+    __syncthreads();
     uint64_t M;
-    const uint64_t excl = filt_scan<NT>(w, s, &M), r = filt_draw(u, M);
-    if (excl <= r && r - excl < w) s.found[0] = id;
+    const uint64_t own = mass[tid], excl = filt_scan<NT>(own, s, &M), r = filt_draw(u, M);
+    if (excl <= r && r - excl < own) s.found[0] = ids[NT + tid];
     __syncthreads();
     return (int)s.found[0];
 }
@@ -527,11 +528,12 @@ __device__ __forceinline__ void filt_mass_bins(const FiltArgs& a, const void* ro
     constexpr int E = BF16 ? 8 : 4;
     filt_tiles<NT, BF16>(row, first, end, [&](int, int, const float (&l)[E], int) {
         uint64_t x[E];
+        uint64_t any = 0;
 #pragma unroll
-        for (int e = 0; e < E; ++e) x[e] = filt_mass(a, filt_clean(l[e]), m);
+        for (int e = 0; e < E; ++e) any |= x[e] = filt_mass(a, filt_clean(l[e]), m);
+        if (any == 0) return;
 #pragma unroll
-        for (int e = 0; e < E; ++e)
-            if (x[e] != 0) atomicAdd(&bins[filt_bin(a, l[e], m)], (unsigned long long)x[e]);
+        for (int e = 0; e < E; ++e) atomicAdd(&bins[filt_bin(a, filt_clean(l[e]), m)], (unsigned long long)x[e]);
     });
 }
 
@@ -547,28 +549,57 @@ __device__ __forceinline__ void filt_gather(const FiltArgs& a, const void* row, 
         if (at < Last::kHeld) z.list[at] = (unsigned long long)filt_key(l) << 32 | (uint32_t)i;
     };
     const float past = bin < kFiltMassBins - 1 ? (float)(bin + 1) : INFINITY;
+    if constexpr (MODE == kFiltTopP) {
+        // What is above the bin is listed too at first, if it fits: its masses then take full waves.
+        filt_tiles<NT, BF16>(row, first, end, [&](int, int i, const float (&l)[E], int n) {
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                if (e < n && !((m - l[e]) * a.to_bin >= past)) enlist(i + e, filt_clean(l[e]));
+        });
+        __syncthreads();
+        const uint32_t listed = z.count;
+        __syncthreads();
+        if (threadIdx.x == 0) z.count = 0;
+        unsigned long long x[Last::kHeld / NT];
+#pragma unroll
+        for (int j = 0; j < Last::kHeld / NT; ++j) x[j] = z.list[j * NT + threadIdx.x];
+        __syncthreads();
+        if (listed <= Last::kHeld) {
+#pragma unroll
+            for (int j = 0; j < Last::kHeld / NT; ++j) {
+                if (j * NT + threadIdx.x >= listed) break;
+                const float l = filt_logit((uint32_t)(x[j] >> 32));
+                if (filt_bin(a, l, m) == bin) z.list[atomicAdd(&z.count, 1u)] = x[j];
+                else atomicAdd(&z.tile[((int)(uint32_t)x[j] - first) / (E * NT)], (unsigned long long)filt_mass(a, l, m));
+            }
+            return;
+        }
+    }
     filt_tiles<NT, BF16>(row, first, end, [&](int t, int i, const float (&l)[E], int n) {
         bool some = false;
 #pragma unroll
         for (int e = 0; e < E; ++e)
             some |= MODE == kFiltTopK ? bound.takes(l[e]) : MODE == kFiltTopP ? !((m - l[e]) * a.to_bin >= past) : !((l[e] - m) * a.to_log2f <= a.low);
-        uint64_t y = 0;
-        if (some) {
+        if (MODE == kFiltTopK && some) {
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
+            for (int e = 0; e < E; ++e)
+                if (e < n && bound.takes(l[e])) enlist(i + e, filt_clean(l[e]));
+        }
+        if constexpr (MODE != kFiltTopK) {
+            if (!__any(some)) return;
+            uint64_t y = 0;
+#pragma unroll
+            for (int e = 0; e < E; ++e) {   // there is none past the end: -inf
                 const float x = filt_clean(l[e]);
-                if constexpr (MODE == kFiltTopK) {
-                    if (e < n && bound.takes(x)) enlist(i + e, x);
-                } else if constexpr (MODE == kFiltTopP) {
+                const uint64_t w = filt_mass(a, x, m);
+                if constexpr (MODE == kFiltTopP) {
                     const int b = filt_bin(a, x, m);
-                    if (b < bin) y += filt_mass(a, x, m);
-                    else if (b == bin && e < n) enlist(i + e, x);
+                    y += b < bin ? w : 0ull;
+                    if (b == bin && e < n) enlist(i + e, x);
                 } else {
-                    y += filt_mass(a, x, m);   // there is none past the end: -inf
+                    y += w;
                 }
             }
-        }
-        if (MODE != kFiltTopK && __any(y != 0)) {
             y = filt_last_lane(filt_wave_scan(y));
             if (threadIdx.x % kWave == 0) atomicAdd(&z.tile[t], (unsigned long long)y);
         }
@@ -616,10 +647,10 @@ __device__ __forceinline__ int filt_last(const FiltArgs& a, const void* row, flo
     if (m == -INFINITY) return -1;
     if (count > Last::kHeld) return filt_choose_row<NT, BF16>(a, row, m, u, s);
     if (MODE == kFiltTopK && count <= NT) {
-        const unsigned long long x = tid < (int)count ? z.list[tid] : 0ull;
+        unsigned long long x = tid < (int)count ? z.list[tid] : 0ull;
         const uint64_t mass = tid < (int)count ? filt_mass(a, filt_logit((uint32_t)(x >> 32)), m) : 0ull;
-        uint32_t* const keys = reinterpret_cast<uint32_t*>(z.list);
-        return filt_choose_held<NT>(a, count, (uint32_t)(x >> 32), (uint32_t)x, mass, W, u, keys, keys + NT, z.mass, s);
+        x = tid < (int)count ? (unsigned long long)~(uint32_t)(x >> 32) << 32 | (uint32_t)x : ~0ull;
+        return filt_choose_held<NT>(a, count, x, mass, W, u, z.list, z.mass, s);
     }
     uint32_t low = ~0u;
     for (uint32_t i = tid; i < count; i += NT) {
