@@ -69,6 +69,20 @@ __device__ __forceinline__ uint32_t finite_pair(uint32_t w) {
     return w;
 }
 
+// Channels 4 c to 4 c + 3 of a row: the output, or what a split hands on. some: the split has keys.
+template <int HD>
+__device__ __forceinline__ void tree_store(const TreeArgs& a, int kvh, int split, int row, int c, float m, float l, const float4& acc, bool some) {
+    if (a.splits == 1) {
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        *reinterpret_cast<uint2*>(a.o + ((int64_t)(row / a.G) * a.Hq + kvh * a.G + row % a.G) * HD + c * 4) =
+            make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+        return;
+    }
+    const int64_t at = ((int64_t)split * a.Hkv + kvh) * a.rows + row;
+    if (some) *reinterpret_cast<float4*>(a.o_part + at * HD + c * 4) = acc;
+    if (c == 0) *reinterpret_cast<float2*>(a.ml_part + at * 2) = make_float2(m, l);
+}
+
 template <int HD, int KW>
 __global__ __launch_bounds__(KW * kWave, 2) void tree_attn_kernel(TreeArgs a) {
     typedef SplitTile<HD> T;
@@ -346,15 +360,285 @@ __global__ __launch_bounds__(KW * kWave, 2) void tree_attn_kernel(TreeArgs a) {
             acc.z += x * y.z;
             acc.w += x * y.w;
         }
-        if (a.splits == 1) {
-            const float inv = l == 0.f ? 0.f : 1.f / l;
-            *reinterpret_cast<uint2*>(a.o + ((int64_t)(gr / a.G) * a.Hq + kvh * a.G + gr % a.G) * HD + c * 4) =
-                make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
-        } else {
-            const int64_t at = ((int64_t)split * a.Hkv + kvh) * a.rows + gr;
-            if (tile_end > split * a.split_tiles) *reinterpret_cast<float4*>(a.o_part + at * HD + c * 4) = acc;
-            if (c == 0) *reinterpret_cast<float2*>(a.ml_part + at * 2) = make_float2(m, l);
+        tree_store<HD>(a, kvh, split, gr, c, m, l, acc, tile_end > split * a.split_tiles);
+    }
+}
+
+// Many rows: a workgroup takes 128 rows, 32 a wave, and two groups of four waves take every other tile of
+// 64 keys. A group's tiles go through a ring of two in LDS that its waves read in common; the next tile is
+// requested before a tile is multiplied. Two waves a SIMD, one from each group, so that one's softmax runs
+// beside the other's products.
+template <int HD>
+__global__ __launch_bounds__(512, 2) void tree_rows_kernel(TreeArgs a) {
+    typedef SplitTile<HD> T;
+    constexpr int KT = 64, KS = HD / 16, DT = HD / 32, CPR = HD / 4;
+    constexpr int TILE = KT * T::kRow, STAGE = 2 * TILE, RING = 2 * STAGE;   // bytes: keys or values; both; a group's ring
+    constexpr int NL = TILE / 1024 / 4;                                      // loads of a wave: keys, and as many of values
+    typedef short s4_t __attribute__((ext_vector_type(4)));
+    static_assert(4 * 32 * HD * 4 <= RING, "the outputs fit in the rings");
+    __shared__ __align__(1024) unsigned char smem[2 * RING];
+    __shared__ float ml[2][2][128];
+    __shared__ int s_odd[2];
+
+    const int tid = threadIdx.x;
+    const int wave = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave, grp = wave / 4, wg = wave % 4;
+    const int ql = lane % 32, hh = lane / 32;
+    const int xcd = blockIdx.x % 8, rest = blockIdx.x / 8;
+    const int unit = rest / a.blocks * 8 + xcd, block = rest % a.blocks;
+    if (unit >= a.Hkv * a.splits) return;
+    const int kvh = unit % a.Hkv, split = unit / a.Hkv;
+    const int r0 = block * 128, row = min(r0 + wg * 32 + ql, a.rows - 1), node = row / a.G, head = kvh * a.G + row % a.G;
+    const bool idle = r0 + wg * 32 >= a.rows;   // a wave without rows helps to load
+
+    const int L = tree_len(a), before = L - a.n;
+    const int t0 = split * a.split_tiles, tile_end = min((L + KT - 1) / KT, t0 + a.split_tiles);
+    const int steps = tile_end > t0 ? (tile_end - t0 + 1) / 2 : 0;
+    if (tid < 2) s_odd[tid] = -1;
+
+    const char* const kbase = reinterpret_cast<const char*>(a.k + kvh * a.k_sh);
+    const char* const vbase = reinterpret_cast<const char*>(a.v + kvh * a.v_sh);
+    unsigned char* const ring = smem + grp * RING;
+    const int pr = lane / T::kChunks, pc = lane % T::kChunks;
+    auto issue = [&](int t, int slot) {
+        const int k0 = t * KT;
+        const bool whole = k0 + KT <= L;
+        unsigned char* const dst = ring + slot * STAGE + wg * 1024;
+#pragma unroll
+        for (int i = 0; i < 2 * NL; ++i) {
+            const bool is_v = i >= NL;
+            const int rr = ((i % NL) * 4 + wg) * T::kRows + pr;
+            const int c = pc ^ (is_v ? T::v_swz(rr) : T::k_swz(rr));
+            const int r = whole ? rr : min(rr, L - 1 - k0);   // rows past the end read the last row
+            const int sn = is_v ? a.v_sn : a.k_sn;
+            const char* const src = (is_v ? vbase : kbase) + (int64_t)k0 * sn * 2 + (uint32_t)((r * sn + c * 8) * 2);
+            __builtin_amdgcn_global_load_lds(static_cast<const void*>(src),
+                                             (__attribute__((address_space(3))) void*)(dst + (is_v ? TILE : 0) + (i % NL) * 4096), 16, 0, 0);
         }
+    };
+    bf16x8_t qf[KS];
+    {
+        const bf16_t* qp = a.q + node * a.q_sn + head * a.q_sh;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            Pack8 x;
+            x.u = *reinterpret_cast<const uint4*>(qp + ks * 16 + hh * 8);
+            qf[ks] = x.v;
+        }
+    }
+    if (t0 + grp < tile_end) issue(t0 + grp, 0);
+    f32x16_t oacc[DT];
+#pragma unroll
+    for (int tt = 0; tt < DT; ++tt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) oacc[tt][e] = 0.f;
+    float m_run = -INFINITY, l_run = 0.f;
+    const uint64_t* const bits_row = a.mask + (int64_t)node * a.words;
+    const uint32_t lds = (uint32_t)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) unsigned char*)ring);
+    uint32_t koff[KS], voff[DT];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) koff[ks] = lds + (uint32_t)(ql * T::kRow + (((ks * 2 + hh) ^ T::k_swz(ql)) << 4));
+    {
+        const int g = lane >> 4, j = lane & 15, rr = (g >> 1) * 4 + (j >> 2);
+#pragma unroll
+        for (int tt = 0; tt < DT; ++tt) {
+            const int d = tt * 32 + 16 * (g & 1) + 4 * (j & 3);
+            voff[tt] = lds + (uint32_t)(TILE + rr * T::kRow + (((d >> 3) ^ T::v_swz(rr)) << 4) + ((d & 7) << 1));
+        }
+    }
+    const float lazy = kTreeLazy / a.scale;
+    auto meet = [] {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+    for (int st = 0; st < steps; ++st) {
+        const int t = t0 + 2 * st + grp, kb0 = t * KT;
+        const bool on = t < tile_end, masked = kb0 + KT > before;
+        // whether either group's tile is of the tree's rows: the same in every wave
+        const bool clean = (t0 + 2 * st + 1) * KT + KT > before;
+        uint64_t bits = ~0ull;
+        if (on && masked) {
+            bits = tree_window<KT>(bits_row, a.words, kb0 - before);
+            if (L - kb0 < 64) bits &= (1ull << (L - kb0)) - 1;
+            asm volatile("" : "+v"(bits));
+        }
+        attn_pipe::vm_wait<0>();
+        meet();   // the tile is there, and the other slot is read out
+        unsigned char* const stage = ring + (st & 1) * STAGE;
+        if (clean) {
+            // values that are not finite are made zeros, and added below where they are seen
+            bool odd = false;
+            if (on && masked) {
+                uint4* const vp = reinterpret_cast<uint4*>(stage + TILE);
+#pragma unroll
+                for (int i = 0; i < NL; ++i) {
+                    const uint4 x = vp[(i * 4 + wg) * 64 + lane];
+                    const uint4 y = make_uint4(finite_pair(x.x), finite_pair(x.y), finite_pair(x.z), finite_pair(x.w));
+                    if (x.x != y.x || x.y != y.y || x.z != y.z || x.w != y.w) {
+                        odd = true;
+                        vp[(i * 4 + wg) * 64 + lane] = y;
+                    }
+                }
+            }
+            if (__any(odd) && lane == 0) s_odd[grp] = st;
+            meet();
+        }
+        if (t + 2 < tile_end) issue(t + 2, (st + 1) & 1);
+        if (!on || idle) continue;
+        const uint32_t at = (uint32_t)((st & 1) * STAGE);
+        // S^T; element e of s[h]: key kb0 + 32 h + 8 (e / 4) + 4 hh + e % 4 of the lane's row
+        f32x16_t s[2];
+        bf16x8_t kf[2][KS];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                if (h == 0) attn_pipe::read_b128<0>(kf[h][ks], koff[ks] + at);
+                else attn_pipe::read_b128<32 * T::kRow>(kf[h][ks], koff[ks] + at);
+            }
+        asm volatile("s_waitcnt lgkmcnt(%0)" ::"n"(KS) : "memory");
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(kf[0][ks]));
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[0][e] = 0.f, s[1][e] = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) s[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[0][ks], qf[ks], s[0], 0, 0, 0);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(kf[1][ks]));
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) s[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[1][ks], qf[ks], s[1], 0, 0, 0);
+        s4_t vf[4][DT][2];
+        auto read_v = [&](auto kbc) {
+            constexpr int kb = decltype(kbc)::value;
+#pragma unroll
+            for (int tt = 0; tt < DT; ++tt) {
+                attn_pipe::read_tr16<(kb * 16) * T::kRow>(vf[kb][tt][0], voff[tt] + at);
+                attn_pipe::read_tr16<(kb * 16 + 8) * T::kRow>(vf[kb][tt][1], voff[tt] + at);
+            }
+        };
+        read_v(std::integral_constant<int, 0>{});
+        read_v(std::integral_constant<int, 1>{});
+        if (masked) {
+            const uint64_t mine = bits >> (4 * hh);
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    s[h][e] = (mine >> (32 * h + 8 * (e / 4) + e % 4) & 1) ? s[h][e] : -INFINITY;
+        }
+        float top = fmaxf(s[0][0], s[1][0]);
+#pragma unroll
+        for (int e = 1; e < 16; ++e) top = fmaxf(fmaxf(top, s[0][e]), s[1][e]);
+        {
+            const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+            top = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
+        }
+        if (__any(top > m_run + lazy)) {   // -inf: whatever is seen first
+            const float m_new = fmaxf(m_run, top);
+            const float alpha = m_run == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m_run - m_new) * a.scale);
+            l_run *= alpha;
+#pragma unroll
+            for (int tt = 0; tt < DT; ++tt)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) oacc[tt][e] *= alpha;
+            m_run = m_new;
+        }
+        const float ref = m_run == -INFINITY ? 0.f : m_run * a.scale;
+        Pack8 pb[4];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            float p[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) p[e] = __builtin_amdgcn_exp2f(fmaf(s[h][e], a.scale, -ref));
+            pb[2 * h].u = pack8(&p[0]);
+            pb[2 * h + 1].u = pack8(&p[8]);
+        }
+        float psum = 0.f;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            psum = add_bf16_pair(pb[b].u.x, psum);
+            psum = add_bf16_pair(pb[b].u.y, psum);
+            psum = add_bf16_pair(pb[b].u.z, psum);
+            psum = add_bf16_pair(pb[b].u.w, psum);
+        }
+        {
+            const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(psum), __float_as_uint(psum), false, false);
+            l_run += __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
+        }
+        auto pv = [&](int kb) {
+#pragma unroll
+            for (int tt = 0; tt < DT; ++tt) {
+                asm volatile("" : "+v"(vf[kb][tt][0]), "+v"(vf[kb][tt][1]));
+                union {
+                    s4_t h[2];
+                    bf16x8_t v;
+                } vv;
+                vv.h[0] = vf[kb][tt][0];
+                vv.h[1] = vf[kb][tt][1];
+                oacc[tt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vv.v, pb[kb].v, oacc[tt], 0, 0, 0);
+            }
+        };
+        // a block's reads go out once the block two before has landed
+        asm volatile("s_waitcnt lgkmcnt(%0)" ::"n"(2 * DT) : "memory");
+        pv(0);
+        read_v(std::integral_constant<int, 2>{});
+        asm volatile("s_waitcnt lgkmcnt(%0)" ::"n"(2 * DT) : "memory");
+        pv(1);
+        read_v(std::integral_constant<int, 3>{});
+        asm volatile("s_waitcnt lgkmcnt(%0)" ::"n"(2 * DT) : "memory");
+        pv(2);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        pv(3);
+        if (clean && s_odd[grp] == st) {
+            const int keys = min(KT, L - kb0);
+            for (int j = 0; j < keys; ++j) {
+                const bf16_t* const vr = reinterpret_cast<const bf16_t*>(vbase) + (int64_t)(kb0 + j) * a.v_sn;
+                const bool seen = bits >> j & 1;
+#pragma unroll
+                for (int tt = 0; tt < DT; ++tt)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const uint32_t x = vr[tt * 32 + (e / 4) * 8 + hh * 4 + e % 4];
+                        if (seen && (x & 0x7f80u) == 0x7f80u) oacc[tt][e] += bf16_to_f32(x);
+                    }
+            }
+        }
+    }
+    // the groups' outputs meet in LDS (float4 chunk c of row r at c ^ (r & 15))
+    meet();
+    {
+        float4* const part = reinterpret_cast<float4*>(smem + (grp * 4 + wg) * 32 * HD * 4);
+#pragma unroll
+        for (int tt = 0; tt < DT; ++tt)
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                part[ql * CPR + ((tt * 8 + g * 2 + hh) ^ (ql & 15))] =
+                    make_float4(oacc[tt][g * 4], oacc[tt][g * 4 + 1], oacc[tt][g * 4 + 2], oacc[tt][g * 4 + 3]);
+        if (hh == 0) {
+            ml[0][grp][wg * 32 + ql] = m_run * a.scale;
+            ml[1][grp][wg * 32 + ql] = l_run;
+        }
+    }
+    __syncthreads();
+    for (int idx = tid; idx < 128 * CPR; idx += 512) {
+        const int r = idx / CPR, c = idx % CPR, gr = r0 + r;
+        if (gr >= a.rows) break;
+        const float m = fmaxf(ml[0][0][r], ml[0][1][r]);
+        float l = 0.f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+            if (ml[0][g][r] == -INFINITY && ml[1][g][r] == 0.f) continue;   // it saw nothing of the row
+            const float x = __builtin_amdgcn_exp2f(ml[0][g][r] - m);
+            const float4 y = reinterpret_cast<const float4*>(smem + (g * 4 + r / 32) * 32 * HD * 4)[r % 32 * CPR + (c ^ (r & 15))];
+            l += x * ml[1][g][r];
+            acc.x += x * y.x;
+            acc.y += x * y.y;
+            acc.z += x * y.z;
+            acc.w += x * y.w;
+        }
+        tree_store<HD>(a, kvh, split, gr, c, m, l, acc, tile_end > t0);
     }
 }
 
@@ -415,20 +699,23 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a) {
 }
 
 struct TreePlan {
-    int waves, blocks, splits, split_tiles;
+    bool many;   // tree_rows_kernel
+    int blocks, splits, split_tiles;
     size_t o_bytes, ml_bytes;
     size_t total() const { return o_bytes + ml_bytes; }
 };
 
 static TreePlan tree_plan(const efm_attention_ctx* c, uint32_t n, uint32_t kv_len) {
-    const int hd = (int)c->head_dim, Hkv = (int)c->num_kv_heads, keys = hd == 128 ? 32 : 64;
+    const int hd = (int)c->head_dim, Hkv = (int)c->num_kv_heads;
     const int64_t rows = (int64_t)n * (c->num_qo_heads / c->num_kv_heads), cus = prefill_cus();
-    const int64_t tiles = ((int64_t)kv_len + keys - 1) / keys;
     TreePlan p = {};
-    p.waves = 4;
-    p.blocks = (int)((rows + 31) / 32);
-    const int64_t want = std::max<int64_t>(1, 2 * cus / ((int64_t)p.blocks * Hkv));
-    p.split_tiles = (int)std::max<int64_t>({2 * p.waves, (tiles + want - 1) / want, (tiles + kTreeMaxSplits - 1) / kTreeMaxSplits});
+    p.many = rows > 64;
+    const int keys = p.many || hd == 64 ? 64 : 32, waves = 4;
+    const int64_t tiles = ((int64_t)kv_len + keys - 1) / keys;
+    p.blocks = (int)(p.many ? (rows + 127) / 128 : (rows + 31) / 32);
+    // workgroups: one a CU of the large ones, two of the small
+    const int64_t want = std::max<int64_t>(1, (p.many ? 1 : 2) * cus / ((int64_t)p.blocks * Hkv));
+    p.split_tiles = (int)std::max<int64_t>({p.many ? 4 : 2 * waves, (tiles + want - 1) / want, (tiles + kTreeMaxSplits - 1) / kTreeMaxSplits});
     p.splits = (int)std::max<int64_t>(1, (tiles + p.split_tiles - 1) / p.split_tiles);
     if (p.splits > 1) {
         p.o_bytes = (size_t)p.splits * Hkv * rows * hd * sizeof(float);
@@ -440,10 +727,10 @@ static TreePlan tree_plan(const efm_attention_ctx* c, uint32_t n, uint32_t kv_le
 // Bytes that hold the partial results of every call of up to n nodes over up to kv_len rows: a call's
 // own need goes up and down with its sizes, and splits <= min(tiles, workgroups wanted / row blocks).
 static size_t tree_workspace(const efm_attention_ctx* c, uint32_t n, uint32_t kv_len) {
-    const int64_t keys = c->head_dim == 128 ? 32 : 64, tiles = ((int64_t)kv_len + keys - 1) / keys, cus = prefill_cus();
-    if (tiles <= 8) return 0;
-    const int64_t splits = std::min<int64_t>(std::min<int64_t>(tiles, kTreeMaxSplits), 2 * cus);
-    const int64_t rows = std::min(splits * n * (int64_t)c->num_qo_heads, 32 * 2 * cus);
+    const int64_t tiles = ((int64_t)kv_len + 31) / 32, cus = prefill_cus();
+    if (kv_len <= 256) return 0;
+    const int64_t splits = std::min<int64_t>(tiles, kTreeMaxSplits);
+    const int64_t rows = std::min(splits * n * (int64_t)c->num_qo_heads, 128 * cus);   // workgroups' rows: 128 a CU, or twice 32
     return (size_t)rows * (c->head_dim + 2) * sizeof(float);
 }
 
@@ -516,10 +803,12 @@ extern "C" int efm_attention_tree(const efm_attention_ctx* ctx, const void* q, c
     const int64_t units = ((int64_t)Hkv * p.splits + 7) / 8 * 8, all = (int64_t)Hkv * a.rows;
     const dim3 grid((unsigned)(units * p.blocks)), joins((unsigned)((all + 3) / 4));
     if (hd == 128) {
-        hipLaunchKernelGGL((tree_attn_kernel<128, 4>), grid, dim3(256), 0, stream, a);
+        if (p.many) hipLaunchKernelGGL(tree_rows_kernel<128>, grid, dim3(512), 0, stream, a);
+        else hipLaunchKernelGGL((tree_attn_kernel<128, 4>), grid, dim3(256), 0, stream, a);
         if (p.splits > 1) hipLaunchKernelGGL(tree_merge_kernel<128>, joins, dim3(256), 0, stream, a);
     } else {
-        hipLaunchKernelGGL((tree_attn_kernel<64, 4>), grid, dim3(256), 0, stream, a);
+        if (p.many) hipLaunchKernelGGL(tree_rows_kernel<64>, grid, dim3(512), 0, stream, a);
+        else hipLaunchKernelGGL((tree_attn_kernel<64, 4>), grid, dim3(256), 0, stream, a);
         if (p.splits > 1) hipLaunchKernelGGL(tree_merge_kernel<64>, joins, dim3(256), 0, stream, a);
     }
     return check_launch("attention_tree");
