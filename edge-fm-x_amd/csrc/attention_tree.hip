@@ -364,21 +364,20 @@ __global__ __launch_bounds__(KW * kWave, 2) void tree_attn_kernel(TreeArgs a) {
     }
 }
 
-// Many rows: a workgroup takes 128 rows, 32 a wave, and two groups of four waves take every other tile of
-// 64 keys. A group's tiles go through a ring of two in LDS that its waves read in common; the next tile is
-// requested before a tile is multiplied. Two waves a SIMD, one from each group, so that one's softmax runs
-// beside the other's products.
+// Many rows: a workgroup takes 128 rows. Tiles of 64 keys go through a ring in LDS that its eight waves
+// read in common; a wave takes 32 rows and one half of a tile's keys. Two waves a SIMD, so that one's
+// softmax runs beside the other's products, and a ring of S tiles, S - 1 of them under way.
 template <int HD>
 __global__ __launch_bounds__(512, 2) void tree_rows_kernel(TreeArgs a) {
     typedef SplitTile<HD> T;
-    constexpr int KT = 64, KS = HD / 16, DT = HD / 32, CPR = HD / 4;
-    constexpr int TILE = KT * T::kRow, STAGE = 2 * TILE, RING = 2 * STAGE;   // bytes: keys or values; both; a group's ring
-    constexpr int NL = TILE / 1024 / 4;                                      // loads of a wave: keys, and as many of values
+    constexpr int KT = 64, KS = HD / 16, DT = HD / 32, CPR = HD / 4, S = HD == 128 ? 4 : 6;
+    constexpr int TILE = KT * T::kRow, STAGE = 2 * TILE;   // bytes: keys or values; both
+    constexpr int NL = TILE / 1024 / 8;                    // loads of a wave: keys, and as many of values
     typedef short s4_t __attribute__((ext_vector_type(4)));
-    static_assert(4 * 32 * HD * 4 <= RING, "the outputs fit in the rings");
-    __shared__ __align__(1024) unsigned char smem[2 * RING];
+    constexpr int SMEM = S * STAGE > 8 * 32 * HD * 4 ? S * STAGE : 8 * 32 * HD * 4;   // the ring, later the outputs
+    __shared__ __align__(1024) unsigned char smem[SMEM];
     __shared__ float ml[2][2][128];
-    __shared__ int s_odd[2];
+    __shared__ int s_odd;
 
     const int tid = threadIdx.x;
     const int wave = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave, grp = wave / 4, wg = wave % 4;
@@ -391,28 +390,26 @@ __global__ __launch_bounds__(512, 2) void tree_rows_kernel(TreeArgs a) {
     const bool idle = r0 + wg * 32 >= a.rows;   // a wave without rows helps to load
 
     const int L = tree_len(a), before = L - a.n;
-    const int t0 = split * a.split_tiles, tile_end = min((L + KT - 1) / KT, t0 + a.split_tiles);
-    const int steps = tile_end > t0 ? (tile_end - t0 + 1) / 2 : 0;
-    if (tid < 2) s_odd[tid] = -1;
+    const int t0 = split * a.split_tiles, tile_end = min((L + KT - 1) / KT, t0 + a.split_tiles), tiles = max(tile_end - t0, 0);
+    if (tid == 0) s_odd = -1;
 
     const char* const kbase = reinterpret_cast<const char*>(a.k + kvh * a.k_sh);
     const char* const vbase = reinterpret_cast<const char*>(a.v + kvh * a.v_sh);
-    unsigned char* const ring = smem + grp * RING;
     const int pr = lane / T::kChunks, pc = lane % T::kChunks;
     auto issue = [&](int t, int slot) {
         const int k0 = t * KT;
         const bool whole = k0 + KT <= L;
-        unsigned char* const dst = ring + slot * STAGE + wg * 1024;
+        unsigned char* const dst = smem + slot * STAGE + wave * 1024;
 #pragma unroll
         for (int i = 0; i < 2 * NL; ++i) {
             const bool is_v = i >= NL;
-            const int rr = ((i % NL) * 4 + wg) * T::kRows + pr;
+            const int rr = ((i % NL) * 8 + wave) * T::kRows + pr;
             const int c = pc ^ (is_v ? T::v_swz(rr) : T::k_swz(rr));
             const int r = whole ? rr : min(rr, L - 1 - k0);   // rows past the end read the last row
             const int sn = is_v ? a.v_sn : a.k_sn;
             const char* const src = (is_v ? vbase : kbase) + (int64_t)k0 * sn * 2 + (uint32_t)((r * sn + c * 8) * 2);
             __builtin_amdgcn_global_load_lds(static_cast<const void*>(src),
-                                             (__attribute__((address_space(3))) void*)(dst + (is_v ? TILE : 0) + (i % NL) * 4096), 16, 0, 0);
+                                             (__attribute__((address_space(3))) void*)(dst + (is_v ? TILE : 0) + (i % NL) * 8192), 16, 0, 0);
         }
     };
     bf16x8_t qf[KS];
@@ -425,24 +422,25 @@ __global__ __launch_bounds__(512, 2) void tree_rows_kernel(TreeArgs a) {
             qf[ks] = x.v;
         }
     }
-    if (t0 + grp < tile_end) issue(t0 + grp, 0);
+    for (int i = 0; i < S - 1; ++i)
+        if (i < tiles) issue(t0 + i, i);
     f32x16_t oacc[DT];
 #pragma unroll
     for (int tt = 0; tt < DT; ++tt)
 #pragma unroll
         for (int e = 0; e < 16; ++e) oacc[tt][e] = 0.f;
-    float m_run = -INFINITY, l_run = 0.f;
+    float m_run = -INFINITY, l_part = 0.f;
     const uint64_t* const bits_row = a.mask + (int64_t)node * a.words;
-    const uint32_t lds = (uint32_t)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) unsigned char*)ring);
+    const uint32_t lds = (uint32_t)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) unsigned char*)smem);
     uint32_t koff[KS], voff[DT];
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) koff[ks] = lds + (uint32_t)(ql * T::kRow + (((ks * 2 + hh) ^ T::k_swz(ql)) << 4));
+    for (int ks = 0; ks < KS; ++ks) koff[ks] = lds + (uint32_t)((grp * 32 + ql) * T::kRow + (((ks * 2 + hh) ^ T::k_swz(ql)) << 4));
     {
         const int g = lane >> 4, j = lane & 15, rr = (g >> 1) * 4 + (j >> 2);
 #pragma unroll
         for (int tt = 0; tt < DT; ++tt) {
             const int d = tt * 32 + 16 * (g & 1) + 4 * (j & 3);
-            voff[tt] = lds + (uint32_t)(TILE + rr * T::kRow + (((d >> 3) ^ T::v_swz(rr)) << 4) + ((d & 7) << 1));
+            voff[tt] = lds + (uint32_t)(TILE + (grp * 32 + rr) * T::kRow + (((d >> 3) ^ T::v_swz(rr)) << 4) + ((d & 7) << 1));
         }
     }
     const float lazy = kTreeLazy / a.scale;
@@ -451,64 +449,50 @@ __global__ __launch_bounds__(512, 2) void tree_rows_kernel(TreeArgs a) {
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
     };
-    for (int st = 0; st < steps; ++st) {
-        const int t = t0 + 2 * st + grp, kb0 = t * KT;
-        const bool on = t < tile_end, masked = kb0 + KT > before;
-        // whether either group's tile is of the tree's rows: the same in every wave
-        const bool clean = (t0 + 2 * st + 1) * KT + KT > before;
+    for (int st = 0; st < tiles; ++st) {
+        const int k0 = (t0 + st) * KT, kb0 = k0 + grp * 32;
+        const bool masked = k0 + KT > before;   // the tile has rows of the tree: the same in every wave
+        const uint32_t slot = (uint32_t)(st % S);
         uint64_t bits = ~0ull;
-        if (on && masked) {
-            bits = tree_window<KT>(bits_row, a.words, kb0 - before);
-            if (L - kb0 < 64) bits &= (1ull << (L - kb0)) - 1;
+        if (masked) {
+            bits = tree_window<32>(bits_row, a.words, kb0 - before);
+            bits &= L - kb0 >= 32 ? 0xffffffffull : L - kb0 > 0 ? (1ull << (L - kb0)) - 1 : 0ull;
             asm volatile("" : "+v"(bits));
         }
-        attn_pipe::vm_wait<0>();
-        meet();   // the tile is there, and the other slot is read out
-        unsigned char* const stage = ring + (st & 1) * STAGE;
-        if (clean) {
+        switch (min(S - 2, tiles - 1 - st)) {   // tiles that may be under way
+            case 0: attn_pipe::vm_wait<0>(); break;
+            case 1: attn_pipe::vm_wait<2 * NL>(); break;
+            case 2: attn_pipe::vm_wait<4 * NL>(); break;
+            case 3: attn_pipe::vm_wait<6 * NL>(); break;
+            default: attn_pipe::vm_wait<8 * NL>(); break;
+        }
+        meet();   // the tile is there, and the slot of the one before is read out
+        unsigned char* const stage = smem + slot * STAGE;
+        if (masked) {
             // values that are not finite are made zeros, and added below where they are seen
             bool odd = false;
-            if (on && masked) {
-                uint4* const vp = reinterpret_cast<uint4*>(stage + TILE);
+            uint4* const vp = reinterpret_cast<uint4*>(stage + TILE);
 #pragma unroll
-                for (int i = 0; i < NL; ++i) {
-                    const uint4 x = vp[(i * 4 + wg) * 64 + lane];
-                    const uint4 y = make_uint4(finite_pair(x.x), finite_pair(x.y), finite_pair(x.z), finite_pair(x.w));
-                    if (x.x != y.x || x.y != y.y || x.z != y.z || x.w != y.w) {
-                        odd = true;
-                        vp[(i * 4 + wg) * 64 + lane] = y;
-                    }
+            for (int i = 0; i < NL; ++i) {
+                const uint4 x = vp[(i * 8 + wave) * 64 + lane];
+                const uint4 y = make_uint4(finite_pair(x.x), finite_pair(x.y), finite_pair(x.z), finite_pair(x.w));
+                if (x.x != y.x || x.y != y.y || x.z != y.z || x.w != y.w) {
+                    odd = true;
+                    vp[(i * 8 + wave) * 64 + lane] = y;
                 }
             }
-            if (__any(odd) && lane == 0) s_odd[grp] = st;
+            if (__any(odd) && lane == 0) s_odd = st;
             meet();
         }
-        if (t + 2 < tile_end) issue(t + 2, (st + 1) & 1);
-        if (!on || idle) continue;
-        const uint32_t at = (uint32_t)((st & 1) * STAGE);
-        // S^T; element e of s[h]: key kb0 + 32 h + 8 (e / 4) + 4 hh + e % 4 of the lane's row
-        f32x16_t s[2];
-        bf16x8_t kf[2][KS];
+        if (st + S - 1 < tiles) issue(t0 + st + S - 1, (st + S - 1) % S);
+        if (idle || kb0 >= L) continue;
+        const uint32_t at = slot * STAGE;
+        // S^T; element e: key kb0 + 8 (e / 4) + 4 hh + e % 4 of the lane's row
+        f32x16_t s;
+        bf16x8_t kf[KS];
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                if (h == 0) attn_pipe::read_b128<0>(kf[h][ks], koff[ks] + at);
-                else attn_pipe::read_b128<32 * T::kRow>(kf[h][ks], koff[ks] + at);
-            }
-        asm volatile("s_waitcnt lgkmcnt(%0)" ::"n"(KS) : "memory");
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(kf[0][ks]));
-#pragma unroll
-        for (int e = 0; e < 16; ++e) s[0][e] = 0.f, s[1][e] = 0.f;
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) s[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[0][ks], qf[ks], s[0], 0, 0, 0);
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(kf[1][ks]));
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) s[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[1][ks], qf[ks], s[1], 0, 0, 0);
-        s4_t vf[4][DT][2];
+        for (int ks = 0; ks < KS; ++ks) attn_pipe::read_b128<0>(kf[ks], koff[ks] + at);
+        s4_t vf[2][DT][2];
         auto read_v = [&](auto kbc) {
             constexpr int kb = decltype(kbc)::value;
 #pragma unroll
@@ -517,19 +501,28 @@ __global__ __launch_bounds__(512, 2) void tree_rows_kernel(TreeArgs a) {
                 attn_pipe::read_tr16<(kb * 16 + 8) * T::kRow>(vf[kb][tt][1], voff[tt] + at);
             }
         };
+        asm volatile("s_waitcnt lgkmcnt(%0)" ::"n"(KS / 2) : "memory");
+#pragma unroll
+        for (int ks = 0; ks < KS / 2; ++ks) asm volatile("" : "+v"(kf[ks]));
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[e] = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < KS / 2; ++ks) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[ks], qf[ks], s, 0, 0, 0);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+        for (int ks = KS / 2; ks < KS; ++ks) asm volatile("" : "+v"(kf[ks]));
+#pragma unroll
+        for (int ks = KS / 2; ks < KS; ++ks) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[ks], qf[ks], s, 0, 0, 0);
         read_v(std::integral_constant<int, 0>{});
         read_v(std::integral_constant<int, 1>{});
         if (masked) {
-            const uint64_t mine = bits >> (4 * hh);
+            const uint32_t mine = (uint32_t)bits >> (4 * hh);
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int e = 0; e < 16; ++e)
-                    s[h][e] = (mine >> (32 * h + 8 * (e / 4) + e % 4) & 1) ? s[h][e] : -INFINITY;
+            for (int e = 0; e < 16; ++e) s[e] = (mine >> (8 * (e / 4) + e % 4) & 1) ? s[e] : -INFINITY;
         }
-        float top = fmaxf(s[0][0], s[1][0]);
+        float top = s[0];
 #pragma unroll
-        for (int e = 1; e < 16; ++e) top = fmaxf(fmaxf(top, s[0][e]), s[1][e]);
+        for (int e = 1; e < 16; ++e) top = fmaxf(top, s[e]);
         {
             const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
             top = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
@@ -537,7 +530,7 @@ __global__ __launch_bounds__(512, 2) void tree_rows_kernel(TreeArgs a) {
         if (__any(top > m_run + lazy)) {   // -inf: whatever is seen first
             const float m_new = fmaxf(m_run, top);
             const float alpha = m_run == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m_run - m_new) * a.scale);
-            l_run *= alpha;
+            l_part *= alpha;
 #pragma unroll
             for (int tt = 0; tt < DT; ++tt)
 #pragma unroll
@@ -545,27 +538,23 @@ __global__ __launch_bounds__(512, 2) void tree_rows_kernel(TreeArgs a) {
             m_run = m_new;
         }
         const float ref = m_run == -INFINITY ? 0.f : m_run * a.scale;
-        Pack8 pb[4];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        Pack8 pb[2];
+        {
             float p[16];
 #pragma unroll
-            for (int e = 0; e < 16; ++e) p[e] = __builtin_amdgcn_exp2f(fmaf(s[h][e], a.scale, -ref));
-            pb[2 * h].u = pack8(&p[0]);
-            pb[2 * h + 1].u = pack8(&p[8]);
+            for (int e = 0; e < 16; ++e) p[e] = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale, -ref));
+            pb[0].u = pack8(&p[0]);
+            pb[1].u = pack8(&p[8]);
         }
         float psum = 0.f;
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
+        for (int b = 0; b < 2; ++b) {
             psum = add_bf16_pair(pb[b].u.x, psum);
             psum = add_bf16_pair(pb[b].u.y, psum);
             psum = add_bf16_pair(pb[b].u.z, psum);
             psum = add_bf16_pair(pb[b].u.w, psum);
         }
-        {
-            const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(psum), __float_as_uint(psum), false, false);
-            l_run += __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
-        }
+        l_part += psum;   // of the lane's half of the keys
         auto pv = [&](int kb) {
 #pragma unroll
             for (int tt = 0; tt < DT; ++tt) {
@@ -579,19 +568,12 @@ __global__ __launch_bounds__(512, 2) void tree_rows_kernel(TreeArgs a) {
                 oacc[tt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vv.v, pb[kb].v, oacc[tt], 0, 0, 0);
             }
         };
-        // a block's reads go out once the block two before has landed
         asm volatile("s_waitcnt lgkmcnt(%0)" ::"n"(2 * DT) : "memory");
         pv(0);
-        read_v(std::integral_constant<int, 2>{});
-        asm volatile("s_waitcnt lgkmcnt(%0)" ::"n"(2 * DT) : "memory");
-        pv(1);
-        read_v(std::integral_constant<int, 3>{});
-        asm volatile("s_waitcnt lgkmcnt(%0)" ::"n"(2 * DT) : "memory");
-        pv(2);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        pv(3);
-        if (clean && s_odd[grp] == st) {
-            const int keys = min(KT, L - kb0);
+        pv(1);
+        if (masked && s_odd == st) {
+            const int keys = min(32, L - kb0);
             for (int j = 0; j < keys; ++j) {
                 const bf16_t* const vr = reinterpret_cast<const bf16_t*>(vbase) + (int64_t)(kb0 + j) * a.v_sn;
                 const bool seen = bits >> j & 1;
@@ -604,6 +586,11 @@ __global__ __launch_bounds__(512, 2) void tree_rows_kernel(TreeArgs a) {
                     }
             }
         }
+    }
+    float l_run;
+    {
+        const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(l_part), __float_as_uint(l_part), false, false);
+        l_run = __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
     }
     // the groups' outputs meet in LDS (float4 chunk c of row r at c ^ (r & 15))
     meet();
@@ -638,7 +625,7 @@ __global__ __launch_bounds__(512, 2) void tree_rows_kernel(TreeArgs a) {
             acc.z += x * y.z;
             acc.w += x * y.w;
         }
-        tree_store<HD>(a, kvh, split, gr, c, m, l, acc, tile_end > t0);
+        tree_store<HD>(a, kvh, split, gr, c, m, l, acc, tiles > 0);
     }
 }
 
