@@ -17,6 +17,7 @@
 
 #include <algorithm>
 #include <type_traits>
+#include <utility>
 
 namespace efm {
 
@@ -83,14 +84,78 @@ __device__ __forceinline__ void tree_store(const TreeArgs& a, int kvh, int split
     if (c == 0) *reinterpret_cast<float2*>(a.ml_part + at * 2) = make_float2(m, l);
 }
 
-template <int HD, int KW>
-__global__ __launch_bounds__(KW * kWave, 2) void tree_attn_kernel(TreeArgs a) {
+// Adds what is not finite of channels 4 c to 4 c + 3 of the values of keys [j0, j1) that a row sees.
+__device__ __forceinline__ void tree_not_finite(const TreeArgs& a, const char* vbase, int row, int c, int before, int j0, int j1, float4& acc) {
+    const uint64_t* const bits = a.mask + (int64_t)(row / a.G) * a.words;
+#pragma unroll 1
+    for (int j = j0; j < j1; ++j) {
+        const int at = j - before;
+        if (at >= 0 && !(bits[at / 64] >> at % 64 & 1)) continue;
+        const uint2 x = *reinterpret_cast<const uint2*>(vbase + ((int64_t)j * a.v_sn + c * 4) * 2);
+        acc.x += (x.x & 0x7f80u) == 0x7f80u ? lo_f32(x.x) : 0.f;
+        acc.y += (x.x & 0x7f800000u) == 0x7f800000u ? hi_f32(x.x) : 0.f;
+        acc.z += (x.y & 0x7f80u) == 0x7f80u ? lo_f32(x.y) : 0.f;
+        acc.w += (x.y & 0x7f800000u) == 0x7f800000u ? hi_f32(x.y) : 0.f;
+    }
+}
+
+// Joins the outputs of P parts of a workgroup, part(p, row, chunk), with the rows' maxima at ml[p * R + row] and sums at
+// ml[(P + p) * R + row]; N chunks of four channels a thread. A part that saw nothing of a row has none in it.
+template <int HD, int P, int N, typename Part, typename Last>
+__device__ __forceinline__ void tree_join(const TreeArgs& a, int tid, int threads, int kvh, int split, int r0, bool some, Part part,
+                                          const float* ml, int R, Last last) {
+    constexpr int CPR = HD / 4;
+    const int c = tid % CPR, step = threads / CPR;
+    // a row's weights once, the outputs of two rows under way
+#pragma unroll 2
+    for (int i = 0; i < N; ++i) {
+        const int r = tid / CPR + i * step, gr = r0 + r;
+        float mp[P], lp[P], m = -INFINITY, l = 0.f;
+        float4 y[P], acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int p = 0; p < P; ++p) mp[p] = ml[p * R + r], lp[p] = ml[(P + p) * R + r], y[p] = part(p, r, c);
+#pragma unroll
+        for (int p = 0; p < P; ++p) m = fmaxf(m, mp[p]);
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+            const bool used = mp[p] != -INFINITY || lp[p] != 0.f;
+            const float x = used ? __builtin_amdgcn_exp2f(mp[p] - m) : 0.f;
+            l += used ? x * lp[p] : 0.f;
+            acc.x += used ? x * y[p].x : 0.f;
+            acc.y += used ? x * y[p].y : 0.f;
+            acc.z += used ? x * y[p].z : 0.f;
+            acc.w += used ? x * y[p].w : 0.f;
+        }
+        if (gr < a.rows) {
+            last(gr, c, acc);
+            tree_store<HD>(a, kvh, split, gr, c, m, l, acc, some);
+        }
+    }
+}
+
+// f(0) to f(N - 1), the index a constant.
+template <int N, typename F>
+__device__ __forceinline__ void tree_each(F f) {
+    [&]<int... I>(std::integer_sequence<int, I...>) { (f(std::integral_constant<int, I>{}), ...); }
+    (std::make_integer_sequence<int, N>{});
+}
+
+// NB x 32 rows a workgroup of four waves, a wave a SIMD. A wave's tiles (8 KB of keys and 8 KB of values) go
+// through two slots each of its own in LDS, requested two tiles ahead. A wave issues in order, so what is to
+// run beside the matrix instructions stands between them: the first row block's exponentials between the
+// second's first products, the second's between the first's second products, and the next tile's keys are
+// read from LDS meanwhile.
+template <int HD, int NB>
+__global__ __launch_bounds__(256, 1) void tree_attn_kernel(TreeArgs a) {
     typedef SplitTile<HD> T;
-    constexpr int KT = T::kKeys, NH = KT / 32, KS = HD / 16, DT = HD / 32, NL = T::kLoads, KB = KT / 16;
-    constexpr int SLOT = 2 * T::kBytes, CPR = HD / 4;
+    constexpr int KW = 4, KT = T::kKeys, NH = KT / 32, KS = HD / 16, DT = HD / 32, NL = T::kLoads, KB = KT / 16;
+    constexpr int SLOT = T::kBytes, RING = 4 * SLOT, CPR = HD / 4;   // a wave's: keys 0, keys 1, values 0, values 1
+    constexpr int NM = NH * KS, NE = NH * 16 / NM;                   // matrix instructions of a product; weights between two
+    static_assert(NM == KB * DT && NM == 8 && NB * 32 * HD * 4 <= RING, "tile geometry");
     typedef short s4_t __attribute__((ext_vector_type(4)));
-    __shared__ __align__(1024) unsigned char smem[KW * SLOT];
-    __shared__ float ml[2][KW][32];
+    __shared__ __align__(1024) unsigned char smem[KW * RING];
+    __shared__ float ml[2][KW][NB * 32];
+    __shared__ int s_odd[KW];
 
     const int tid = threadIdx.x;
     const int wave = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave;
@@ -99,101 +164,139 @@ __global__ __launch_bounds__(KW * kWave, 2) void tree_attn_kernel(TreeArgs a) {
     const int xcd = blockIdx.x % 8, rest = blockIdx.x / 8;
     const int unit = rest / a.blocks * 8 + xcd, block = rest % a.blocks;
     if (unit >= a.Hkv * a.splits) return;
-    const int kvh = unit % a.Hkv, split = unit / a.Hkv;
-    const int r0 = block * 32, row = r0 + ql, node = min(row, a.rows - 1) / a.G, head = kvh * a.G + min(row, a.rows - 1) % a.G;
+    const int kvh = unit % a.Hkv, split = unit / a.Hkv, r0 = block * NB * 32;
 
     const int L = tree_len(a), before = L - a.n;   // rows before the tree
-    const int tiles = (L + KT - 1) / KT;
-    const int tile_end = min(tiles, (split + 1) * a.split_tiles);
-    int t = split * a.split_tiles + wave;
-
+    const int t0 = split * a.split_tiles, tile_end = min((L + KT - 1) / KT, t0 + a.split_tiles);
     const char* const kbase = reinterpret_cast<const char*>(a.k + kvh * a.k_sh);
     const char* const vbase = reinterpret_cast<const char*>(a.v + kvh * a.v_sh);
-    unsigned char* const kslot = smem + wave * SLOT;
-    unsigned char* const vslot = kslot + T::kBytes;
+    unsigned char* const ring = smem + wave * RING;
     const int pr = lane / T::kChunks, pc = lane % T::kChunks;
     auto issue = [&](const char* base, int sn, int k0, unsigned char* slot, auto is_v) {
-        const char* const t0 = base + (int64_t)k0 * sn * 2;
+        const char* const tile = base + (int64_t)k0 * sn * 2;
         const bool whole = k0 + KT <= L;
 #pragma unroll
         for (int i = 0; i < NL; ++i) {
             const int rr = i * T::kRows + pr;
             const int c = pc ^ (decltype(is_v)::value ? T::v_swz(rr) : T::k_swz(rr));
             const int r = whole ? rr : min(rr, L - 1 - k0);   // rows past the end read the last row
-            __builtin_amdgcn_global_load_lds(static_cast<const void*>(t0 + (uint32_t)((r * sn + c * 8) * 2)),
+            __builtin_amdgcn_global_load_lds(static_cast<const void*>(tile + (uint32_t)((r * sn + c * 8) * 2)),
                                              (__attribute__((address_space(3))) void*)(slot + i * 1024), 16, 0, 0);
         }
     };
-    auto issue_k = [&](int tt) { issue(kbase, a.k_sn, tt * KT, kslot, std::false_type{}); };
-    auto issue_v = [&](int tt) { issue(vbase, a.v_sn, tt * KT, vslot, std::true_type{}); };
+    auto issue_k = [&](int t, int b) { issue(kbase, a.k_sn, t * KT, ring + b * SLOT, std::false_type{}); };
+    auto issue_v = [&](int t, int b) { issue(vbase, a.v_sn, t * KT, ring + (2 + b) * SLOT, std::true_type{}); };
 
     // Q, the second operand: d = 16 ks + 8 hh + e
-    bf16x8_t qf[KS];
-    {
+    bf16x8_t qf[NB][KS];
+    const uint64_t* bits_row[NB];
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+        const int row = min(r0 + n * 32 + ql, a.rows - 1), node = row / a.G, head = kvh * a.G + row % a.G;
         const bf16_t* qp = a.q + node * a.q_sn + head * a.q_sh;
+        bits_row[n] = a.mask + (int64_t)node * a.words;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
             Pack8 x;
             x.u = *reinterpret_cast<const uint4*>(qp + ks * 16 + hh * 8);
-            qf[ks] = x.v;
+            qf[n][ks] = x.v;
         }
     }
-    if (t < tile_end) {
-        issue_k(t);
-        issue_v(t);
-    }
-    f32x16_t oacc[DT];
+    int t = t0 + wave;
+    if (t < tile_end) issue_k(t, 0), issue_v(t, 0);
+    if (t + KW < tile_end) issue_k(t + KW, 1), issue_v(t + KW, 1);
+    // Q has landed here: a first use in the loop would wait for every load under way, each time
 #pragma unroll
-    for (int tt = 0; tt < DT; ++tt)
+    for (int n = 0; n < NB; ++n)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) oacc[tt][e] = 0.f;
-    float m_run = -INFINITY, l_run = 0.f;
-    const uint64_t* const bits_row = a.mask + (int64_t)node * a.words;
+        for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(qf[n][ks]));
 
-    const uint32_t lk = (uint32_t)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) unsigned char*)kslot);
+    f32x16_t o[NB][DT];
+    float m_run[NB], l_part[NB];   // the largest score so far; the sum over the lane's half of the keys
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+        m_run[n] = -INFINITY, l_part[n] = 0.f;
+#pragma unroll
+        for (int i = 0; i < DT; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[n][i][e] = 0.f;
+    }
+    const uint32_t lds = (uint32_t)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) unsigned char*)ring);
     uint32_t ka[KS], va[DT];
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) ka[ks] = lk + (uint32_t)(ql * T::kRow + (((ks * 2 + hh) ^ T::k_swz(ql)) << 4));
+    for (int ks = 0; ks < KS; ++ks) ka[ks] = lds + (uint32_t)(ql * T::kRow + (((ks * 2 + hh) ^ T::k_swz(ql)) << 4));
     {
         const int g = lane >> 4, j = lane & 15, rr = (g >> 1) * 4 + (j >> 2);
 #pragma unroll
-        for (int tt = 0; tt < DT; ++tt) {
-            const int d = tt * 32 + 16 * (g & 1) + 4 * (j & 3);
-            va[tt] = lk + (uint32_t)(T::kBytes + rr * T::kRow + (((d >> 3) ^ T::v_swz(rr)) << 4) + ((d & 7) << 1));
+        for (int i = 0; i < DT; ++i) {
+            const int d = i * 32 + 16 * (g & 1) + 4 * (j & 3);
+            va[i] = lds + (uint32_t)(2 * SLOT + rr * T::kRow + (((d >> 3) ^ T::v_swz(rr)) << 4) + ((d & 7) << 1));
         }
     }
     const float lazy = kTreeLazy / a.scale;
-    for (; t < tile_end; t += KW) {
-        const bool more = t + KW < tile_end;
-        const int kb0 = t * KT;
-        const bool masked = kb0 + KT > before;
-        uint64_t bits = ~0ull;
-        if (masked) {   // requested before the waits below
-            bits = tree_window<KT>(bits_row, a.words, kb0 - before);
-            if (L - kb0 < 64) bits &= (1ull << (L - kb0)) - 1;
-            asm volatile("" : "+v"(bits));
-            attn_pipe::vm_wait<0>();
-        } else {
-            attn_pipe::vm_wait<NL>();   // K has landed; V may be under way
-        }
-        asm volatile("" ::: "memory");
-        bf16x8_t kf[NH][KS];
+    bf16x8_t kf[NH][KS];
+    auto read_k = [&](int b) {
+        const uint32_t at = (uint32_t)(b * SLOT);
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
-            attn_pipe::read_b128<0>(kf[0][ks], ka[ks]);
-            if constexpr (NH == 2) attn_pipe::read_b128<32 * T::kRow>(kf[1][ks], ka[ks]);
+            attn_pipe::read_b128<0>(kf[0][ks], ka[ks] + at);
+            if constexpr (NH == 2) attn_pipe::read_b128<32 * T::kRow>(kf[1][ks], ka[ks] + at);
         }
+    };
+    if (t < tile_end) {
+        if (t + KW < tile_end) attn_pipe::vm_wait<3 * NL>();
+        else attn_pipe::vm_wait<NL>();
+        read_k(0);
+    }
+    bool odd = false;
+    for (int b = 0; t < tile_end; t += KW, b ^= 1) {
+        const bool one = t + KW < tile_end, two = t + 2 * KW < tile_end;   // tiles to come
+        const int kb0 = t * KT;
+        const bool masked = kb0 + KT > before;
+        uint64_t bits[NB];
+#pragma unroll
+        for (int n = 0; n < NB; ++n) bits[n] = ~0ull;
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 #pragma unroll
         for (int h = 0; h < NH; ++h)
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(kf[h][ks]));
-        // Values that a row does not see take no part in its output whatever they are: a zero weight
-        // times an infinity would be a NaN. V of the tree's rows and of rows past the end is made
-        // finite here, and what was not is added below where it is seen.
-        bool odd = false;
+        if (two) issue_k(t + 2 * KW, b);
+        // S^T; element e of s[n][h]: key kb0 + 32 h + 8 (e / 4) + 4 hh + e % 4 of row block n
+        f32x16_t s[NB][NH];
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+            for (int h = 0; h < NH; ++h)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s[n][h][e] = 0.f;
+        auto qk = [&](auto nc, auto ic) {
+            constexpr int N = decltype(nc)::value, H = decltype(ic)::value % NH, K = decltype(ic)::value / NH;
+            s[N][H] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[H][K], qf[N][K], s[N][H], 0, 0, 0);
+        };
+        using std::integral_constant;
+        tree_each<NM>([&](auto i) { qk(integral_constant<int, 0>{}, i); });
         if (masked) {
-            uint4* const vp = reinterpret_cast<uint4*>(vslot);
+#pragma unroll
+            for (int n = 0; n < NB; ++n) {
+                bits[n] = tree_window<KT>(bits_row[n], a.words, kb0 - before);
+                if (L - kb0 < 64) bits[n] &= (1ull << (L - kb0)) - 1;
+                asm volatile("" : "+v"(bits[n]));
+            }
+            attn_pipe::vm_wait<0>();
+        } else if (two) {
+            attn_pipe::vm_wait<3 * NL>();
+        } else if (one) {
+            attn_pipe::vm_wait<2 * NL>();
+        } else {
+            attn_pipe::vm_wait<0>();
+        }
+        asm volatile("" ::: "memory");
+        // Values that a row does not see take no part in its output whatever they are: a zero weight times an
+        // infinity would be a NaN. V of the tree's rows and of rows past the end is made finite here, and what
+        // was not is added at the end where it is seen.
+        if (masked) {
+            uint4* const vp = reinterpret_cast<uint4*>(ring + (2 + b) * SLOT);
 #pragma unroll
             for (int i = 0; i < NL; ++i) {
                 const uint4 x = vp[i * 64 + lane];
@@ -205,163 +308,129 @@ __global__ __launch_bounds__(KW * kWave, 2) void tree_attn_kernel(TreeArgs a) {
             }
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         }
-        if (more) issue_k(t + KW);
-        // S^T - m; element e of s[h]: key kb0 + 32 h + 8 (e / 4) + 4 hh + e % 4 of the lane's row
-        const float start = m_run == -INFINITY ? 0.f : -m_run;
-        f32x16_t s[NH];
-#pragma unroll
-        for (int h = 0; h < NH; ++h) {
-#pragma unroll
-            for (int e = 0; e < 16; ++e) s[h][e] = start;
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) s[h] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[h][ks], qf[ks], s[h], 0, 0, 0);
-        }
-        if (!masked) {
-            if (more) attn_pipe::vm_wait<NL>();
-            else attn_pipe::vm_wait<0>();
-        }
-        asm volatile("" ::: "memory");
         s4_t vf[KB][DT][2];
+        {
+            const uint32_t at = (uint32_t)(b * SLOT);
+            tree_each<KB>([&](auto kc) {
+                constexpr int K = decltype(kc)::value;
 #pragma unroll
-        for (int tt = 0; tt < DT; ++tt) {
-            attn_pipe::read_tr16<0>(vf[0][tt][0], va[tt]);
-            attn_pipe::read_tr16<8 * T::kRow>(vf[0][tt][1], va[tt]);
-            attn_pipe::read_tr16<16 * T::kRow>(vf[1][tt][0], va[tt]);
-            attn_pipe::read_tr16<24 * T::kRow>(vf[1][tt][1], va[tt]);
-            if constexpr (KB == 4) {
-                attn_pipe::read_tr16<32 * T::kRow>(vf[KB - 2][tt][0], va[tt]);
-                attn_pipe::read_tr16<40 * T::kRow>(vf[KB - 2][tt][1], va[tt]);
-                attn_pipe::read_tr16<48 * T::kRow>(vf[KB - 1][tt][0], va[tt]);
-                attn_pipe::read_tr16<56 * T::kRow>(vf[KB - 1][tt][1], va[tt]);
-            }
+                for (int i = 0; i < DT; ++i) {
+                    attn_pipe::read_tr16<16 * K * T::kRow>(vf[K][i][0], va[i] + at);
+                    attn_pipe::read_tr16<(16 * K + 8) * T::kRow>(vf[K][i][1], va[i] + at);
+                }
+            });
         }
-        if (masked) {
-            const uint64_t mine = bits >> (4 * hh);
+        float ref[NB];
+        // masks the scores of row block n, and follows its maximum where it is exceeded by 2^kTreeLazy in weights
+        auto maximum = [&](auto nc) {
+            constexpr int N = decltype(nc)::value;
+            if (masked) {
+                const uint64_t mine = bits[N] >> (4 * hh);
+#pragma unroll
+                for (int h = 0; h < NH; ++h)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        s[N][h][e] = (mine >> (32 * h + 8 * (e / 4) + e % 4) & 1) ? s[N][h][e] : -INFINITY;
+            }
+            float top = s[N][0][0];
 #pragma unroll
             for (int h = 0; h < NH; ++h)
 #pragma unroll
-                for (int e = 0; e < 16; ++e)
-                    s[h][e] = (mine >> (32 * h + 8 * (e / 4) + e % 4) & 1) ? s[h][e] : -INFINITY;
-        }
-        float top = s[0][0];
-#pragma unroll
-        for (int h = 0; h < NH; ++h)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) top = fmaxf(top, s[h][e]);
-        {
+                for (int e = 0; e < 16; ++e) top = fmaxf(top, s[N][h][e]);
             const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
             top = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
-        }
-        if (__any((m_run == -INFINITY && top > -INFINITY) || top > lazy)) {
-            // a row may see none of its wave's first tiles: its maximum stays -inf, its weights are 0
-            const float m_new = fmaxf(m_run, top - start);
-            const float alpha = m_run == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m_run - m_new) * a.scale);
-            const float shift = m_new == -INFINITY ? 0.f : m_new + start;
-            l_run *= alpha;
+            if (__any(top > m_run[N] + lazy)) {   // from -inf: whatever is seen first
+                const float m_new = fmaxf(m_run[N], top);
+                const float alpha = m_run[N] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m_run[N] - m_new) * a.scale);
+                l_part[N] *= alpha;
 #pragma unroll
-            for (int tt = 0; tt < DT; ++tt)
+                for (int i = 0; i < DT; ++i)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) oacc[tt][e] *= alpha;
+                    for (int e = 0; e < 16; ++e) o[N][i][e] *= alpha;
+                m_run[N] = m_new;
+            }
+            ref[N] = m_run[N] == -INFINITY ? 0.f : m_run[N] * a.scale;
+        };
+        uint32_t pw[NB][NH * 8];   // weights, two a word
+        auto weigh = [&](auto nc, auto ic) {   // NE of them
+            constexpr int N = decltype(nc)::value, I = decltype(ic)::value;
 #pragma unroll
-            for (int h = 0; h < NH; ++h)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) s[h][e] -= shift;
-            m_run = m_new;
-        }
-        Pack8 pb[KB];
-#pragma unroll
-        for (int h = 0; h < NH; ++h) {
-            float p[16];
-#pragma unroll
-            for (int e = 0; e < 16; ++e) p[e] = __builtin_amdgcn_exp2f(s[h][e] * a.scale);
-            pb[2 * h].u = pack8(&p[0]);
-            pb[2 * h + 1].u = pack8(&p[8]);
-        }
-        float psum = 0.f;
-#pragma unroll
-        for (int b = 0; b < KB; ++b) {
-            psum = add_bf16_pair(pb[b].u.x, psum);
-            psum = add_bf16_pair(pb[b].u.y, psum);
-            psum = add_bf16_pair(pb[b].u.z, psum);
-            psum = add_bf16_pair(pb[b].u.w, psum);
-        }
-        {
-            const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(psum), __float_as_uint(psum), false, false);
-            l_run += __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
-        }
+            for (int j = 0; j < NE; j += 2) {
+                constexpr int E0 = I * NE;
+                const int e = E0 + j;
+                const float x = __builtin_amdgcn_exp2f(fmaf(s[N][e / 16][e % 16], a.scale, -ref[N]));
+                const float y = __builtin_amdgcn_exp2f(fmaf(s[N][e / 16][e % 16 + 1], a.scale, -ref[N]));
+                pw[N][e / 2] = pack_bf16x2(x, y);
+                l_part[N] = add_bf16_pair(pw[N][e / 2], l_part[N]);
+            }
+        };
+        auto pv = [&](auto nc, auto ic) {
+            constexpr int N = decltype(nc)::value, K = decltype(ic)::value / DT, I = decltype(ic)::value % DT;
+            union {
+                s4_t h[2];
+                bf16x8_t v;
+            } vv;
+            vv.h[0] = vf[K][I][0];
+            vv.h[1] = vf[K][I][1];
+            Pack8 p;
+            p.u = make_uint4(pw[N][4 * K], pw[N][4 * K + 1], pw[N][4 * K + 2], pw[N][4 * K + 3]);
+            o[N][I] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vv.v, p.v, o[N][I], 0, 0, 0);
+        };
+        maximum(integral_constant<int, 0>{});
+        tree_each<NM>([&](auto i) {
+            if constexpr (NB == 2) qk(integral_constant<int, NB - 1>{}, i);
+            weigh(integral_constant<int, 0>{}, i);
+            if constexpr (NB == 2) __builtin_amdgcn_sched_barrier(0);
+        });
+        if constexpr (NB == 2) maximum(integral_constant<int, NB - 1>{});
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-            for (int tt = 0; tt < DT; ++tt) asm volatile("" : "+v"(vf[kb][tt][0]), "+v"(vf[kb][tt][1]));
-        if (more) issue_v(t + KW);
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-            for (int tt = 0; tt < DT; ++tt) {
-                union {
-                    s4_t h[2];
-                    bf16x8_t v;
-                } vv;
-                vv.h[0] = vf[kb][tt][0];
-                vv.h[1] = vf[kb][tt][1];
-                oacc[tt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vv.v, pb[kb].v, oacc[tt], 0, 0, 0);
-            }
-        if (__any(odd)) {
-            // the values that were not finite, from memory: rows that see the key add them
-            const int keys = min(KT, L - kb0);
-            for (int j = 0; j < keys; ++j) {
-                const bf16_t* const vr = reinterpret_cast<const bf16_t*>(vbase) + (int64_t)(kb0 + j) * a.v_sn;
-                const bool seen = bits >> j & 1;
-#pragma unroll
-                for (int tt = 0; tt < DT; ++tt)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        const int d = tt * 32 + (e / 4) * 8 + hh * 4 + e % 4;
-                        const uint32_t x = vr[d];
-                        if (seen && (x & 0x7f80u) == 0x7f80u) oacc[tt][e] += bf16_to_f32(x);
-                    }
-            }
+            for (int i = 0; i < DT; ++i) asm volatile("" : "+v"(vf[kb][i][0]), "+v"(vf[kb][i][1]));
+        if (two) issue_v(t + 2 * KW, b);
+        if (one) {   // the next tile's keys
+            if (masked) attn_pipe::vm_wait<0>();
+            else if (two) attn_pipe::vm_wait<3 * NL>();
+            else attn_pipe::vm_wait<NL>();
+            asm volatile("" ::: "memory");
+            read_k(b ^ 1);
         }
+        tree_each<NM>([&](auto i) {
+            pv(integral_constant<int, 0>{}, i);
+            if constexpr (NB == 2) {
+                weigh(integral_constant<int, NB - 1>{}, i);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        });
+        if constexpr (NB == 2) tree_each<NM>([&](auto i) { pv(integral_constant<int, NB - 1>{}, i); });
     }
 
     // the waves' outputs meet in LDS (float4 chunk c of row r at c ^ (r & 15))
-    {
-        float4* const part = reinterpret_cast<float4*>(kslot);
 #pragma unroll
-        for (int tt = 0; tt < DT; ++tt)
+    for (int n = 0; n < NB; ++n) {
+        float4* const part = reinterpret_cast<float4*>(ring) + n * 32 * CPR;
+#pragma unroll
+        for (int i = 0; i < DT; ++i)
 #pragma unroll
             for (int g = 0; g < 4; ++g)
-                part[ql * CPR + ((tt * 8 + g * 2 + hh) ^ (ql & 15))] =
-                    make_float4(oacc[tt][g * 4], oacc[tt][g * 4 + 1], oacc[tt][g * 4 + 2], oacc[tt][g * 4 + 3]);
+                part[ql * CPR + ((i * 8 + g * 2 + hh) ^ (ql & 15))] =
+                    make_float4(o[n][i][g * 4], o[n][i][g * 4 + 1], o[n][i][g * 4 + 2], o[n][i][g * 4 + 3]);
+        const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(l_part[n]), __float_as_uint(l_part[n]), false, false);
         if (hh == 0) {
-            ml[0][wave][ql] = m_run * a.scale;
-            ml[1][wave][ql] = l_run;
+            ml[0][wave][n * 32 + ql] = m_run[n] * a.scale;
+            ml[1][wave][n * 32 + ql] = __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
         }
     }
+    odd = __any(odd);
+    if (lane == 0) s_odd[wave] = odd;
     __syncthreads();
-    for (int idx = tid; idx < 32 * CPR; idx += KW * kWave) {
-        const int r = idx / CPR, c = idx % CPR, gr = r0 + r;
-        if (gr >= a.rows) continue;
-        float m = ml[0][0][r];
-#pragma unroll
-        for (int w = 1; w < KW; ++w) m = fmaxf(m, ml[0][w][r]);
-        float l = 0.f;
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-        for (int w = 0; w < KW; ++w) {
-            // a wave that saw nothing of the row has no part in it
-            if (ml[0][w][r] == -INFINITY && ml[1][w][r] == 0.f) continue;
-            const float x = __builtin_amdgcn_exp2f(ml[0][w][r] - m);
-            const float4 y = reinterpret_cast<const float4*>(smem + w * SLOT)[r * CPR + (c ^ (r & 15))];
-            l += x * ml[1][w][r];
-            acc.x += x * y.x;
-            acc.y += x * y.y;
-            acc.z += x * y.z;
-            acc.w += x * y.w;
-        }
-        tree_store<HD>(a, kvh, split, gr, c, m, l, acc, tile_end > split * a.split_tiles);
-    }
+    odd = (s_odd[0] | s_odd[1] | s_odd[2] | s_odd[3]) != 0;
+    tree_join<HD, KW, NB * 32 * CPR / 256>(a, tid, 256, kvh, split, r0, tile_end > t0, [&](int w, int r, int c) {
+        return reinterpret_cast<const float4*>(smem + w * RING)[r * CPR + (c ^ (r & 15))];
+    }, &ml[0][0][0], NB * 32, [&](int gr, int c, float4& acc) {
+        if (odd) tree_not_finite(a, vbase, gr, c, before, max(before / KT, t0) * KT, min(L, tile_end * KT), acc);
+    });
 }
 
 // Many rows: a workgroup takes 128 rows. Tiles of 64 keys go through a ring in LDS that its eight waves
@@ -391,7 +460,7 @@ __global__ __launch_bounds__(512, 2) void tree_rows_kernel(TreeArgs a) {
 
     const int L = tree_len(a), before = L - a.n;
     const int t0 = split * a.split_tiles, tile_end = min((L + KT - 1) / KT, t0 + a.split_tiles), tiles = max(tile_end - t0, 0);
-    if (tid == 0) s_odd = -1;
+    if (tid == 0) s_odd = 0;
 
     const char* const kbase = reinterpret_cast<const char*>(a.k + kvh * a.k_sh);
     const char* const vbase = reinterpret_cast<const char*>(a.v + kvh * a.v_sh);
@@ -424,6 +493,9 @@ __global__ __launch_bounds__(512, 2) void tree_rows_kernel(TreeArgs a) {
     }
     for (int i = 0; i < S - 1; ++i)
         if (i < tiles) issue(t0 + i, i);
+    // Q has landed here: a first use in the loop would wait for every load under way, each time
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(qf[ks]));
     f32x16_t oacc[DT];
 #pragma unroll
     for (int tt = 0; tt < DT; ++tt)
@@ -469,7 +541,7 @@ __global__ __launch_bounds__(512, 2) void tree_rows_kernel(TreeArgs a) {
         meet();   // the tile is there, and the slot of the one before is read out
         unsigned char* const stage = smem + slot * STAGE;
         if (masked) {
-            // values that are not finite are made zeros, and added below where they are seen
+            // values that are not finite are made zeros, and added at the end where they are seen
             bool odd = false;
             uint4* const vp = reinterpret_cast<uint4*>(stage + TILE);
 #pragma unroll
@@ -481,7 +553,7 @@ __global__ __launch_bounds__(512, 2) void tree_rows_kernel(TreeArgs a) {
                     vp[(i * 8 + wave) * 64 + lane] = y;
                 }
             }
-            if (__any(odd) && lane == 0) s_odd = st;
+            if (__any(odd) && lane == 0) s_odd = 1;
             meet();
         }
         if (st + S - 1 < tiles) issue(t0 + st + S - 1, (st + S - 1) % S);
@@ -572,20 +644,6 @@ __global__ __launch_bounds__(512, 2) void tree_rows_kernel(TreeArgs a) {
         pv(0);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         pv(1);
-        if (masked && s_odd == st) {
-            const int keys = min(32, L - kb0);
-            for (int j = 0; j < keys; ++j) {
-                const bf16_t* const vr = reinterpret_cast<const bf16_t*>(vbase) + (int64_t)(kb0 + j) * a.v_sn;
-                const bool seen = bits >> j & 1;
-#pragma unroll
-                for (int tt = 0; tt < DT; ++tt)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        const uint32_t x = vr[tt * 32 + (e / 4) * 8 + hh * 4 + e % 4];
-                        if (seen && (x & 0x7f80u) == 0x7f80u) oacc[tt][e] += bf16_to_f32(x);
-                    }
-            }
-        }
     }
     float l_run;
     {
@@ -608,25 +666,12 @@ __global__ __launch_bounds__(512, 2) void tree_rows_kernel(TreeArgs a) {
         }
     }
     __syncthreads();
-    for (int idx = tid; idx < 128 * CPR; idx += 512) {
-        const int r = idx / CPR, c = idx % CPR, gr = r0 + r;
-        if (gr >= a.rows) break;
-        const float m = fmaxf(ml[0][0][r], ml[0][1][r]);
-        float l = 0.f;
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-        for (int g = 0; g < 2; ++g) {
-            if (ml[0][g][r] == -INFINITY && ml[1][g][r] == 0.f) continue;   // it saw nothing of the row
-            const float x = __builtin_amdgcn_exp2f(ml[0][g][r] - m);
-            const float4 y = reinterpret_cast<const float4*>(smem + (g * 4 + r / 32) * 32 * HD * 4)[r % 32 * CPR + (c ^ (r & 15))];
-            l += x * ml[1][g][r];
-            acc.x += x * y.x;
-            acc.y += x * y.y;
-            acc.z += x * y.z;
-            acc.w += x * y.w;
-        }
-        tree_store<HD>(a, kvh, split, gr, c, m, l, acc, tiles > 0);
-    }
+    const bool odd = s_odd != 0;
+    tree_join<HD, 2, 128 * CPR / 512>(a, tid, 512, kvh, split, r0, tiles > 0, [&](int g, int r, int c) {
+        return reinterpret_cast<const float4*>(smem + (g * 4 + r / 32) * 32 * HD * 4)[r % 32 * CPR + (c ^ (r & 15))];
+    }, &ml[0][0][0], 128, [&](int gr, int c, float4& acc) {
+        if (odd) tree_not_finite(a, vbase, gr, c, before, max(before / KT, t0) * KT, min(L, tile_end * KT), acc);
+    });
 }
 
 // Joins the splits of a row: a wave a row, HD / 4 lanes across its channels, the rest over the splits.
@@ -686,7 +731,7 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a) {
 }
 
 struct TreePlan {
-    bool many;   // tree_rows_kernel
+    int nb;   // row blocks of 32 of a workgroup
     int blocks, splits, split_tiles;
     size_t o_bytes, ml_bytes;
     size_t total() const { return o_bytes + ml_bytes; }
@@ -696,13 +741,13 @@ static TreePlan tree_plan(const efm_attention_ctx* c, uint32_t n, uint32_t kv_le
     const int hd = (int)c->head_dim, Hkv = (int)c->num_kv_heads;
     const int64_t rows = (int64_t)n * (c->num_qo_heads / c->num_kv_heads), cus = prefill_cus();
     TreePlan p = {};
-    p.many = rows > 64;
-    const int keys = p.many || hd == 64 ? 64 : 32, waves = 4;
+    p.nb = rows > 64 ? 4 : rows > 32 ? 2 : 1;
+    const int keys = hd == 128 && p.nb < 4 ? 32 : 64;
     const int64_t tiles = ((int64_t)kv_len + keys - 1) / keys;
-    p.blocks = (int)(p.many ? (rows + 127) / 128 : (rows + 31) / 32);
-    // workgroups: one a CU of the large ones, two of the small
-    const int64_t want = std::max<int64_t>(1, (p.many ? 1 : 2) * cus / ((int64_t)p.blocks * Hkv));
-    p.split_tiles = (int)std::max<int64_t>({p.many ? 4 : 2 * waves, (tiles + want - 1) / want, (tiles + kTreeMaxSplits - 1) / kTreeMaxSplits});
+    p.blocks = (int)((rows + 32 * p.nb - 1) / (32 * p.nb));
+    const int64_t want = std::max<int64_t>(1, cus / ((int64_t)p.blocks * Hkv));   // a workgroup a CU
+    p.split_tiles = (int)std::max<int64_t>({4, (tiles + want - 1) / want, (tiles + kTreeMaxSplits - 1) / kTreeMaxSplits});
+    if (p.nb < 4) p.split_tiles = (p.split_tiles + 3) / 4 * 4;   // as many for each wave
     p.splits = (int)std::max<int64_t>(1, (tiles + p.split_tiles - 1) / p.split_tiles);
     if (p.splits > 1) {
         p.o_bytes = (size_t)p.splits * Hkv * rows * hd * sizeof(float);
@@ -715,9 +760,9 @@ static TreePlan tree_plan(const efm_attention_ctx* c, uint32_t n, uint32_t kv_le
 // own need goes up and down with its sizes, and splits <= min(tiles, workgroups wanted / row blocks).
 static size_t tree_workspace(const efm_attention_ctx* c, uint32_t n, uint32_t kv_len) {
     const int64_t tiles = ((int64_t)kv_len + 31) / 32, cus = prefill_cus();
-    if (kv_len <= 256) return 0;
+    if (kv_len <= 128) return 0;
     const int64_t splits = std::min<int64_t>(tiles, kTreeMaxSplits);
-    const int64_t rows = std::min(splits * n * (int64_t)c->num_qo_heads, 128 * cus);   // workgroups' rows: 128 a CU, or twice 32
+    const int64_t rows = std::min(splits * n * (int64_t)c->num_qo_heads, 128 * cus);   // 128 rows a workgroup at most
     return (size_t)rows * (c->head_dim + 2) * sizeof(float);
 }
 
@@ -789,14 +834,14 @@ extern "C" int efm_attention_tree(const efm_attention_ctx* ctx, const void* q, c
     a.scale = 1.4426950408889634f / sqrtf((float)hd);
     const int64_t units = ((int64_t)Hkv * p.splits + 7) / 8 * 8, all = (int64_t)Hkv * a.rows;
     const dim3 grid((unsigned)(units * p.blocks)), joins((unsigned)((all + 3) / 4));
-    if (hd == 128) {
-        if (p.many) hipLaunchKernelGGL(tree_rows_kernel<128>, grid, dim3(512), 0, stream, a);
-        else hipLaunchKernelGGL((tree_attn_kernel<128, 4>), grid, dim3(256), 0, stream, a);
-        if (p.splits > 1) hipLaunchKernelGGL(tree_merge_kernel<128>, joins, dim3(256), 0, stream, a);
-    } else {
-        if (p.many) hipLaunchKernelGGL(tree_rows_kernel<64>, grid, dim3(512), 0, stream, a);
-        else hipLaunchKernelGGL((tree_attn_kernel<64, 4>), grid, dim3(256), 0, stream, a);
-        if (p.splits > 1) hipLaunchKernelGGL(tree_merge_kernel<64>, joins, dim3(256), 0, stream, a);
-    }
+    auto launch = [&](auto hdc) {
+        constexpr int HD = decltype(hdc)::value;
+        if (p.nb == 4) hipLaunchKernelGGL(tree_rows_kernel<HD>, grid, dim3(512), 0, stream, a);
+        else if (p.nb == 2) hipLaunchKernelGGL((tree_attn_kernel<HD, 2>), grid, dim3(256), 0, stream, a);
+        else hipLaunchKernelGGL((tree_attn_kernel<HD, 1>), grid, dim3(256), 0, stream, a);
+        if (p.splits > 1) hipLaunchKernelGGL(tree_merge_kernel<HD>, joins, dim3(256), 0, stream, a);
+    };
+    if (hd == 128) launch(std::integral_constant<int, 128>{});
+    else launch(std::integral_constant<int, 64>{});
     return check_launch("attention_tree");
 }
