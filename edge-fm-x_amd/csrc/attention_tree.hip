@@ -37,6 +37,7 @@ struct TreeArgs {
     float* ml_part;   // [splits][Hkv][rows][2]
     const uint32_t* d_kv_len;
     uint32_t kv_len, max_kv_len;
+    int bound;                        // rows that the cache holds
     int n, words, Hq, Hkv, G, rows;   // rows: n * G
     int64_t q_sn, q_sh, k_sh, v_sh;
     int k_sn, v_sn;
@@ -433,18 +434,19 @@ __global__ __launch_bounds__(256, 1) void tree_attn_kernel(TreeArgs a) {
     });
 }
 
-// Many rows: a workgroup takes 128 rows. Tiles of 64 keys go through a ring in LDS that its eight waves
-// read in common; a wave takes 32 rows and one half of a tile's keys. Two waves a SIMD, so that one's
-// softmax runs beside the other's products, and a ring of S tiles, S - 1 of them under way.
+// Many rows: a workgroup takes 128 rows, 32 a wave, and two groups of four waves take every other tile of
+// 64 keys. A group's tiles go through a ring of two in LDS that its waves read in common; the next tile is
+// requested before a tile is multiplied. Two waves a SIMD, one from each group, so that one's softmax runs
+// beside the other's products.
 template <int HD>
 __global__ __launch_bounds__(512, 2) void tree_rows_kernel(TreeArgs a) {
     typedef SplitTile<HD> T;
-    constexpr int KT = 64, KS = HD / 16, DT = HD / 32, CPR = HD / 4, S = HD == 128 ? 4 : 6;
-    constexpr int TILE = KT * T::kRow, STAGE = 2 * TILE;   // bytes: keys or values; both
-    constexpr int NL = TILE / 1024 / 8;                    // loads of a wave: keys, and as many of values
+    constexpr int KT = 64, KS = HD / 16, DT = HD / 32, CPR = HD / 4;
+    constexpr int TILE = KT * T::kRow, STAGE = 2 * TILE, RING = 2 * STAGE;   // bytes: keys or values; both; a group's ring
+    constexpr int NL = TILE / 1024 / 4;                                      // loads of a wave: keys, and as many of values
     typedef short s4_t __attribute__((ext_vector_type(4)));
-    constexpr int SMEM = S * STAGE > 8 * 32 * HD * 4 ? S * STAGE : 8 * 32 * HD * 4;   // the ring, later the outputs
-    __shared__ __align__(1024) unsigned char smem[SMEM];
+    static_assert(4 * 32 * HD * 4 <= RING, "the outputs fit in the rings");
+    __shared__ __align__(1024) unsigned char smem[2 * RING];
     __shared__ float ml[2][2][128];
     __shared__ int s_odd;
 
@@ -458,27 +460,41 @@ __global__ __launch_bounds__(512, 2) void tree_rows_kernel(TreeArgs a) {
     const int r0 = block * 128, row = min(r0 + wg * 32 + ql, a.rows - 1), node = row / a.G, head = kvh * a.G + row % a.G;
     const bool idle = r0 + wg * 32 >= a.rows;   // a wave without rows helps to load
 
-    const int L = tree_len(a), before = L - a.n;
-    const int t0 = split * a.split_tiles, tile_end = min((L + KT - 1) / KT, t0 + a.split_tiles), tiles = max(tile_end - t0, 0);
-    if (tid == 0) s_odd = 0;
-
     const char* const kbase = reinterpret_cast<const char*>(a.k + kvh * a.k_sh);
     const char* const vbase = reinterpret_cast<const char*>(a.v + kvh * a.v_sh);
-    const int pr = lane / T::kChunks, pc = lane % T::kChunks;
+    unsigned char* const ring = smem + grp * RING;
+    // Loads of a wave: rows (4 i + wg) kRows + pr of a tile, the chunk that belongs at its place, which is the same
+    // in all of them: one offset a lane serves.
+    const int pr = lane / T::kChunks, pc = lane % T::kChunks, row0 = wg * T::kRows + pr;
+    static_assert(4 * T::kRows % 16 == 0, "the swizzles repeat after 16 rows");
+    const uint32_t koff0 = (uint32_t)(row0 * a.k_sn * 2 + ((pc ^ T::k_swz(row0)) << 4));
+    const uint32_t voff0 = (uint32_t)(row0 * a.v_sn * 2 + ((pc ^ T::v_swz(row0)) << 4));
+    const int bound = a.bound, t0 = split * a.split_tiles;
     auto issue = [&](int t, int slot) {
         const int k0 = t * KT;
-        const bool whole = k0 + KT <= L;
-        unsigned char* const dst = smem + slot * STAGE + wave * 1024;
+        unsigned char* const dst = ring + slot * STAGE + wg * 1024;
+        if (k0 + KT <= bound) {
+            const char* const kt = kbase + (int64_t)k0 * a.k_sn * 2;
+            const char* const vt = vbase + (int64_t)k0 * a.v_sn * 2;
 #pragma unroll
-        for (int i = 0; i < 2 * NL; ++i) {
+            for (int i = 0; i < NL; ++i)
+                __builtin_amdgcn_global_load_lds(static_cast<const void*>(kt + (int64_t)i * 4 * T::kRows * a.k_sn * 2 + koff0),
+                                                 (__attribute__((address_space(3))) void*)(dst + i * 4096), 16, 0, 0);
+#pragma unroll
+            for (int i = 0; i < NL; ++i)
+                __builtin_amdgcn_global_load_lds(static_cast<const void*>(vt + (int64_t)i * 4 * T::kRows * a.v_sn * 2 + voff0),
+                                                 (__attribute__((address_space(3))) void*)(dst + TILE + i * 4096), 16, 0, 0);
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i < 2 * NL; ++i) {   // rows past the end read the last row
             const bool is_v = i >= NL;
-            const int rr = ((i % NL) * 8 + wave) * T::kRows + pr;
+            const int rr = (i % NL) * 4 * T::kRows + row0, r = min(rr, bound - 1 - k0);
             const int c = pc ^ (is_v ? T::v_swz(rr) : T::k_swz(rr));
-            const int r = whole ? rr : min(rr, L - 1 - k0);   // rows past the end read the last row
             const int sn = is_v ? a.v_sn : a.k_sn;
             const char* const src = (is_v ? vbase : kbase) + (int64_t)k0 * sn * 2 + (uint32_t)((r * sn + c * 8) * 2);
             __builtin_amdgcn_global_load_lds(static_cast<const void*>(src),
-                                             (__attribute__((address_space(3))) void*)(dst + (is_v ? TILE : 0) + (i % NL) * 8192), 16, 0, 0);
+                                             (__attribute__((address_space(3))) void*)(dst + (is_v ? TILE : 0) + (i % NL) * 4096), 16, 0, 0);
         }
     };
     bf16x8_t qf[KS];
@@ -491,8 +507,12 @@ __global__ __launch_bounds__(512, 2) void tree_rows_kernel(TreeArgs a) {
             qf[ks] = x.v;
         }
     }
-    for (int i = 0; i < S - 1; ++i)
-        if (i < tiles) issue(t0 + i, i);
+    // The first tile is requested before the length is known: the cache holds `bound` rows.
+    if (t0 + grp < min((bound + KT - 1) / KT, t0 + a.split_tiles)) issue(t0 + grp, 0);
+    const int L = tree_len(a), before = L - a.n;   // rows before the tree
+    const int tile_end = min((L + KT - 1) / KT, t0 + a.split_tiles);
+    const int steps = tile_end > t0 ? (tile_end - t0 + 1) / 2 : 0;
+    if (tid == 0) s_odd = 0;
     // Q has landed here: a first use in the loop would wait for every load under way, each time
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(qf[ks]));
@@ -501,18 +521,18 @@ __global__ __launch_bounds__(512, 2) void tree_rows_kernel(TreeArgs a) {
     for (int tt = 0; tt < DT; ++tt)
 #pragma unroll
         for (int e = 0; e < 16; ++e) oacc[tt][e] = 0.f;
-    float m_run = -INFINITY, l_part = 0.f;
+    float m_run = -INFINITY, l_part = 0.f;   // the largest score so far; the sum over the lane's half of the keys
     const uint64_t* const bits_row = a.mask + (int64_t)node * a.words;
-    const uint32_t lds = (uint32_t)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) unsigned char*)smem);
+    const uint32_t lds = (uint32_t)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) unsigned char*)ring);
     uint32_t koff[KS], voff[DT];
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) koff[ks] = lds + (uint32_t)((grp * 32 + ql) * T::kRow + (((ks * 2 + hh) ^ T::k_swz(ql)) << 4));
+    for (int ks = 0; ks < KS; ++ks) koff[ks] = lds + (uint32_t)(ql * T::kRow + (((ks * 2 + hh) ^ T::k_swz(ql)) << 4));
     {
         const int g = lane >> 4, j = lane & 15, rr = (g >> 1) * 4 + (j >> 2);
 #pragma unroll
         for (int tt = 0; tt < DT; ++tt) {
             const int d = tt * 32 + 16 * (g & 1) + 4 * (j & 3);
-            voff[tt] = lds + (uint32_t)(TILE + (grp * 32 + rr) * T::kRow + (((d >> 3) ^ T::v_swz(rr)) << 4) + ((d & 7) << 1));
+            voff[tt] = lds + (uint32_t)(TILE + rr * T::kRow + (((d >> 3) ^ T::v_swz(rr)) << 4) + ((d & 7) << 1));
         }
     }
     const float lazy = kTreeLazy / a.scale;
@@ -521,50 +541,64 @@ __global__ __launch_bounds__(512, 2) void tree_rows_kernel(TreeArgs a) {
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
     };
-    for (int st = 0; st < tiles; ++st) {
-        const int k0 = (t0 + st) * KT, kb0 = k0 + grp * 32;
-        const bool masked = k0 + KT > before;   // the tile has rows of the tree: the same in every wave
-        const uint32_t slot = (uint32_t)(st % S);
+    for (int st = 0; st < steps; ++st) {
+        const int t = t0 + 2 * st + grp, kb0 = t * KT;
+        const bool on = t < tile_end, masked = kb0 + KT > before;
+        // whether either group's tile is of the tree's rows: the same in every wave
+        const bool clean = (t0 + 2 * st + 1) * KT + KT > before;
         uint64_t bits = ~0ull;
-        if (masked) {
-            bits = tree_window<32>(bits_row, a.words, kb0 - before);
-            bits &= L - kb0 >= 32 ? 0xffffffffull : L - kb0 > 0 ? (1ull << (L - kb0)) - 1 : 0ull;
+        if (on && masked) {
+            bits = tree_window<KT>(bits_row, a.words, kb0 - before);
+            if (L - kb0 < 64) bits &= (1ull << (L - kb0)) - 1;
             asm volatile("" : "+v"(bits));
         }
-        switch (min(S - 2, tiles - 1 - st)) {   // tiles that may be under way
-            case 0: attn_pipe::vm_wait<0>(); break;
-            case 1: attn_pipe::vm_wait<2 * NL>(); break;
-            case 2: attn_pipe::vm_wait<4 * NL>(); break;
-            case 3: attn_pipe::vm_wait<6 * NL>(); break;
-            default: attn_pipe::vm_wait<8 * NL>(); break;
-        }
-        meet();   // the tile is there, and the slot of the one before is read out
-        unsigned char* const stage = smem + slot * STAGE;
-        if (masked) {
+        attn_pipe::vm_wait<0>();
+        meet();   // the tile is there, and the other slot is read out
+        unsigned char* const stage = ring + (st & 1) * STAGE;
+        if (clean) {
             // values that are not finite are made zeros, and added at the end where they are seen
             bool odd = false;
-            uint4* const vp = reinterpret_cast<uint4*>(stage + TILE);
+            if (on && masked) {
+                uint4* const vp = reinterpret_cast<uint4*>(stage + TILE);
 #pragma unroll
-            for (int i = 0; i < NL; ++i) {
-                const uint4 x = vp[(i * 8 + wave) * 64 + lane];
-                const uint4 y = make_uint4(finite_pair(x.x), finite_pair(x.y), finite_pair(x.z), finite_pair(x.w));
-                if (x.x != y.x || x.y != y.y || x.z != y.z || x.w != y.w) {
-                    odd = true;
-                    vp[(i * 8 + wave) * 64 + lane] = y;
+                for (int i = 0; i < NL; ++i) {
+                    const uint4 x = vp[(i * 4 + wg) * 64 + lane];
+                    const uint4 y = make_uint4(finite_pair(x.x), finite_pair(x.y), finite_pair(x.z), finite_pair(x.w));
+                    if (x.x != y.x || x.y != y.y || x.z != y.z || x.w != y.w) {
+                        odd = true;
+                        vp[(i * 4 + wg) * 64 + lane] = y;
+                    }
                 }
             }
             if (__any(odd) && lane == 0) s_odd = 1;
             meet();
         }
-        if (st + S - 1 < tiles) issue(t0 + st + S - 1, (st + S - 1) % S);
-        if (idle || kb0 >= L) continue;
-        const uint32_t at = slot * STAGE;
-        // S^T; element e: key kb0 + 8 (e / 4) + 4 hh + e % 4 of the lane's row
-        f32x16_t s;
-        bf16x8_t kf[KS];
+        if (t + 2 < tile_end) issue(t + 2, (st + 1) & 1);
+        if (!on || idle) continue;
+        const uint32_t at = (uint32_t)((st & 1) * STAGE);
+        // S^T; element e of s[h]: key kb0 + 32 h + 8 (e / 4) + 4 hh + e % 4 of the lane's row
+        f32x16_t s[2];
+        bf16x8_t kf[2][KS];
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) attn_pipe::read_b128<0>(kf[ks], koff[ks] + at);
-        s4_t vf[2][DT][2];
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                if (h == 0) attn_pipe::read_b128<0>(kf[h][ks], koff[ks] + at);
+                else attn_pipe::read_b128<32 * T::kRow>(kf[h][ks], koff[ks] + at);
+            }
+        asm volatile("s_waitcnt lgkmcnt(%0)" ::"n"(KS) : "memory");
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(kf[0][ks]));
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[0][e] = 0.f, s[1][e] = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) s[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[0][ks], qf[ks], s[0], 0, 0, 0);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(kf[1][ks]));
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) s[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[1][ks], qf[ks], s[1], 0, 0, 0);
+        s4_t vf[4][DT][2];
         auto read_v = [&](auto kbc) {
             constexpr int kb = decltype(kbc)::value;
 #pragma unroll
@@ -573,28 +607,19 @@ __global__ __launch_bounds__(512, 2) void tree_rows_kernel(TreeArgs a) {
                 attn_pipe::read_tr16<(kb * 16 + 8) * T::kRow>(vf[kb][tt][1], voff[tt] + at);
             }
         };
-        asm volatile("s_waitcnt lgkmcnt(%0)" ::"n"(KS / 2) : "memory");
-#pragma unroll
-        for (int ks = 0; ks < KS / 2; ++ks) asm volatile("" : "+v"(kf[ks]));
-#pragma unroll
-        for (int e = 0; e < 16; ++e) s[e] = 0.f;
-#pragma unroll
-        for (int ks = 0; ks < KS / 2; ++ks) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[ks], qf[ks], s, 0, 0, 0);
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-#pragma unroll
-        for (int ks = KS / 2; ks < KS; ++ks) asm volatile("" : "+v"(kf[ks]));
-#pragma unroll
-        for (int ks = KS / 2; ks < KS; ++ks) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[ks], qf[ks], s, 0, 0, 0);
         read_v(std::integral_constant<int, 0>{});
         read_v(std::integral_constant<int, 1>{});
         if (masked) {
-            const uint32_t mine = (uint32_t)bits >> (4 * hh);
+            const uint64_t mine = bits >> (4 * hh);
 #pragma unroll
-            for (int e = 0; e < 16; ++e) s[e] = (mine >> (8 * (e / 4) + e % 4) & 1) ? s[e] : -INFINITY;
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    s[h][e] = (mine >> (32 * h + 8 * (e / 4) + e % 4) & 1) ? s[h][e] : -INFINITY;
         }
-        float top = s[0];
+        float top = fmaxf(s[0][0], s[1][0]);
 #pragma unroll
-        for (int e = 1; e < 16; ++e) top = fmaxf(top, s[e]);
+        for (int e = 1; e < 16; ++e) top = fmaxf(fmaxf(top, s[0][e]), s[1][e]);
         {
             const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
             top = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
@@ -610,23 +635,22 @@ __global__ __launch_bounds__(512, 2) void tree_rows_kernel(TreeArgs a) {
             m_run = m_new;
         }
         const float ref = m_run == -INFINITY ? 0.f : m_run * a.scale;
-        Pack8 pb[2];
-        {
+        Pack8 pb[4];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
             float p[16];
 #pragma unroll
-            for (int e = 0; e < 16; ++e) p[e] = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale, -ref));
-            pb[0].u = pack8(&p[0]);
-            pb[1].u = pack8(&p[8]);
+            for (int e = 0; e < 16; ++e) p[e] = __builtin_amdgcn_exp2f(fmaf(s[h][e], a.scale, -ref));
+            pb[2 * h].u = pack8(&p[0]);
+            pb[2 * h + 1].u = pack8(&p[8]);
         }
-        float psum = 0.f;
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
-            psum = add_bf16_pair(pb[b].u.x, psum);
-            psum = add_bf16_pair(pb[b].u.y, psum);
-            psum = add_bf16_pair(pb[b].u.z, psum);
-            psum = add_bf16_pair(pb[b].u.w, psum);
+        for (int b = 0; b < 4; ++b) {
+            l_part = add_bf16_pair(pb[b].u.x, l_part);
+            l_part = add_bf16_pair(pb[b].u.y, l_part);
+            l_part = add_bf16_pair(pb[b].u.z, l_part);
+            l_part = add_bf16_pair(pb[b].u.w, l_part);
         }
-        l_part += psum;   // of the lane's half of the keys
         auto pv = [&](int kb) {
 #pragma unroll
             for (int tt = 0; tt < DT; ++tt) {
@@ -640,16 +664,19 @@ __global__ __launch_bounds__(512, 2) void tree_rows_kernel(TreeArgs a) {
                 oacc[tt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vv.v, pb[kb].v, oacc[tt], 0, 0, 0);
             }
         };
+        // a block's reads go out once the block two before has landed
         asm volatile("s_waitcnt lgkmcnt(%0)" ::"n"(2 * DT) : "memory");
         pv(0);
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        read_v(std::integral_constant<int, 2>{});
+        asm volatile("s_waitcnt lgkmcnt(%0)" ::"n"(2 * DT) : "memory");
         pv(1);
+        read_v(std::integral_constant<int, 3>{});
+        asm volatile("s_waitcnt lgkmcnt(%0)" ::"n"(2 * DT) : "memory");
+        pv(2);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        pv(3);
     }
-    float l_run;
-    {
-        const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(l_part), __float_as_uint(l_part), false, false);
-        l_run = __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
-    }
+    attn_pipe::vm_wait<0>();   // a tile past the length
     // the groups' outputs meet in LDS (float4 chunk c of row r at c ^ (r & 15))
     meet();
     {
@@ -660,70 +687,87 @@ __global__ __launch_bounds__(512, 2) void tree_rows_kernel(TreeArgs a) {
             for (int g = 0; g < 4; ++g)
                 part[ql * CPR + ((tt * 8 + g * 2 + hh) ^ (ql & 15))] =
                     make_float4(oacc[tt][g * 4], oacc[tt][g * 4 + 1], oacc[tt][g * 4 + 2], oacc[tt][g * 4 + 3]);
+        const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(l_part), __float_as_uint(l_part), false, false);
         if (hh == 0) {
             ml[0][grp][wg * 32 + ql] = m_run * a.scale;
-            ml[1][grp][wg * 32 + ql] = l_run;
+            ml[1][grp][wg * 32 + ql] = __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
         }
     }
     __syncthreads();
     const bool odd = s_odd != 0;
-    tree_join<HD, 2, 128 * CPR / 512>(a, tid, 512, kvh, split, r0, tiles > 0, [&](int g, int r, int c) {
+    tree_join<HD, 2, 128 * CPR / 512>(a, tid, 512, kvh, split, r0, tile_end > t0, [&](int g, int r, int c) {
         return reinterpret_cast<const float4*>(smem + (g * 4 + r / 32) * 32 * HD * 4)[r % 32 * CPR + (c ^ (r & 15))];
     }, &ml[0][0][0], 128, [&](int gr, int c, float4& acc) {
         if (odd) tree_not_finite(a, vbase, gr, c, before, max(before / KT, t0) * KT, min(L, tile_end * KT), acc);
     });
 }
 
-// Joins the splits of a row: a wave a row, HD / 4 lanes across its channels, the rest over the splits.
-template <int HD>
+// Joins the splits of a row: TPR threads a row, HD / 4 across its channels and P over the splits. The first
+// outputs are requested before it is known which splits have any.
+template <int HD, int TPR>
 __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a) {
-    constexpr int C = HD / 4, P = kWave / C, CH = 8;
-    __shared__ float wt[4][kTreeMaxSplits];
+    constexpr int C = HD / 4, P = TPR / C, CH = 4, RW = 256 / TPR;
+    __shared__ float wt[RW][kTreeMaxSplits];
+    __shared__ float4 parts[RW][P][C];
+    __shared__ float red[2][4];
     const int64_t all = (int64_t)a.Hkv * a.rows;
-    const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave, c = lane % C, part = lane / C;
-    const int64_t r = (int64_t)blockIdx.x * 4 + wave, rr = min(r, all - 1);
-    float M = -INFINITY;
-    float2 mine[kTreeMaxSplits / kWave];
+    const int rw = threadIdx.x / TPR, tid = threadIdx.x % TPR, c = tid % C, part = tid / C;
+    const int64_t r = (int64_t)blockIdx.x * RW + rw, rr = min(r, all - 1);
+    const float* const op = a.o_part + rr * HD + c * 4;
+    float4 x[CH];
+    auto request = [&](int s0) {
 #pragma unroll
-    for (int i = 0; i < kTreeMaxSplits / kWave; ++i) {
-        const int s = i * kWave + lane;
-        mine[i] = s < a.splits ? *reinterpret_cast<const float2*>(a.ml_part + ((int64_t)s * all + rr) * 2) : make_float2(-INFINITY, 0.f);
+        for (int k = 0; k < CH; ++k) x[k] = *reinterpret_cast<const float4*>(op + (int64_t)min(s0 + k * P, a.splits - 1) * all * HD);
+    };
+    request(part);
+    constexpr int N = kTreeMaxSplits / TPR;
+    float2 mine[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) mine[i] = *reinterpret_cast<const float2*>(a.ml_part + ((int64_t)min(i * TPR + tid, a.splits - 1) * all + rr) * 2);
+    float M = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        if (i * TPR + tid >= a.splits) mine[i] = make_float2(-INFINITY, 0.f);
         M = fmaxf(M, mine[i].x);
     }
     M = wave_max_uniform(M);
+    if constexpr (TPR == 256) {
+        if (tid % kWave == 0) red[0][tid / kWave] = M;
+        __syncthreads();
+        M = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+    }
     float den = 0.f;
 #pragma unroll
-    for (int i = 0; i < kTreeMaxSplits / kWave; ++i) {
+    for (int i = 0; i < N; ++i) {
         const bool used = mine[i].x != -INFINITY || mine[i].y != 0.f;   // the others may have no output
         const float f = used ? __builtin_amdgcn_exp2f(mine[i].x - M) : 0.f;
         den += used ? f * mine[i].y : 0.f;
-        wt[wave][i * kWave + lane] = used ? f : -1.f;
+        wt[rw][i * TPR + tid] = used ? f : -1.f;
     }
     den = wave_total(den);
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_wave_barrier();
+    if constexpr (TPR == 256) {
+        if (tid % kWave == 0) red[1][tid / kWave] = den;
+    }
+    __syncthreads();
+    if constexpr (TPR == 256) den = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
     float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
-    const float* const op = a.o_part + rr * HD + c * 4;
     for (int s0 = part; s0 < a.splits; s0 += CH * P) {
-        float4 x[CH];
-        float w[CH];
+        if (s0 != part) request(s0);
 #pragma unroll
         for (int k = 0; k < CH; ++k) {
-            const int s = s0 + k * P;
-            w[k] = s < a.splits ? wt[wave][s] : -1.f;
-            if (!(w[k] < 0.f)) x[k] = *reinterpret_cast<const float4*>(op + (int64_t)s * all * HD);
+            const float w = s0 + k * P < a.splits ? wt[rw][s0 + k * P] : -1.f;
+            const bool on = !(w < 0.f);
+            t.x += on ? w * x[k].x : 0.f, t.y += on ? w * x[k].y : 0.f, t.z += on ? w * x[k].z : 0.f, t.w += on ? w * x[k].w : 0.f;
         }
-#pragma unroll
-        for (int k = 0; k < CH; ++k)
-            if (!(w[k] < 0.f)) t.x += w[k] * x[k].x, t.y += w[k] * x[k].y, t.z += w[k] * x[k].z, t.w += w[k] * x[k].w;
     }
-    // the parts of a channel are C lanes apart
-#pragma unroll
-    for (int off = C; off < kWave; off *= 2) {
-        t.x += __shfl_xor(t.x, off, kWave), t.y += __shfl_xor(t.y, off, kWave);
-        t.z += __shfl_xor(t.z, off, kWave), t.w += __shfl_xor(t.w, off, kWave);
-    }
+    parts[rw][part][c] = t;
+    __syncthreads();
     if (part > 0 || r >= all) return;
+#pragma unroll
+    for (int p = 1; p < P; ++p) {
+        const float4 y = parts[rw][p][c];
+        t.x += y.x, t.y += y.y, t.z += y.z, t.w += y.w;
+    }
     const float inv = den == 0.f ? 0.f : 1.f / den;
     const int kvh = (int)(r / a.rows), gr = (int)(r % a.rows);
     *reinterpret_cast<uint2*>(a.o + ((int64_t)(gr / a.G) * a.Hq + kvh * a.G + gr % a.G) * HD + c * 4) =
@@ -816,6 +860,7 @@ extern "C" int efm_attention_tree(const efm_attention_ctx* ctx, const void* q, c
     a.d_kv_len = d_kv_len;
     a.kv_len = kv_len;
     a.max_kv_len = max_kv_len;
+    a.bound = (int)bound;
     a.n = (int)nodes;
     a.words = ((int)nodes + 63) / 64;
     a.Hq = Hq;
@@ -833,13 +878,14 @@ extern "C" int efm_attention_tree(const efm_attention_ctx* ctx, const void* q, c
     a.split_tiles = p.split_tiles;
     a.scale = 1.4426950408889634f / sqrtf((float)hd);
     const int64_t units = ((int64_t)Hkv * p.splits + 7) / 8 * 8, all = (int64_t)Hkv * a.rows;
-    const dim3 grid((unsigned)(units * p.blocks)), joins((unsigned)((all + 3) / 4));
+    const dim3 grid((unsigned)(units * p.blocks));
     auto launch = [&](auto hdc) {
         constexpr int HD = decltype(hdc)::value;
         if (p.nb == 4) hipLaunchKernelGGL(tree_rows_kernel<HD>, grid, dim3(512), 0, stream, a);
         else if (p.nb == 2) hipLaunchKernelGGL((tree_attn_kernel<HD, 2>), grid, dim3(256), 0, stream, a);
         else hipLaunchKernelGGL((tree_attn_kernel<HD, 1>), grid, dim3(256), 0, stream, a);
-        if (p.splits > 1) hipLaunchKernelGGL(tree_merge_kernel<HD>, joins, dim3(256), 0, stream, a);
+        if (p.splits > 8) hipLaunchKernelGGL((tree_merge_kernel<HD, 256>), dim3((unsigned)all), dim3(256), 0, stream, a);
+        else if (p.splits > 1) hipLaunchKernelGGL((tree_merge_kernel<HD, 64>), dim3((unsigned)((all + 3) / 4)), dim3(256), 0, stream, a);
     };
     if (hd == 128) launch(std::integral_constant<int, 128>{});
     else launch(std::integral_constant<int, 64>{});

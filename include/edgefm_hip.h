@@ -614,8 +614,8 @@ int efm_draft_tree_plan(uint32_t nodes, const int32_t* parents, uint32_t kv_len,
                         hipStream_t stream);
 
 /* Attention of the nodes: q [nodes, Hq, hd] (ctx->q_stride_*), k, v the cache, whose first L rows
- * (L = *d_kv_len when d_kv_len is not NULL, else kv_len) end with the nodes' own; o [nodes, Hq * hd]
- * contiguous. Node i sees rows j < L - nodes, and row L - nodes + c where bit c of its row of mask
+ * (L = *d_kv_len when d_kv_len is not NULL; then k, v must hold max_kv_len rows, which may be read
+ * before the length is known; else kv_len) end with the nodes' own; o [nodes, Hq * hd] contiguous. Node i sees rows j < L - nodes, and row L - nodes + c where bit c of its row of mask
  * (as efm_draft_tree_plan lays it out; any bits may be set, those past the nodes are not looked at)
  * is set. fp32 softmax, P rounded to bf16 for the PV product, sm_scale = 1/sqrt(hd); a node that
  * sees no row gets zeros. Keys and values that a node does not see take no part in its output,
