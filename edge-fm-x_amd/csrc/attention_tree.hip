@@ -1,17 +1,19 @@
-// Attention of a tree of drafted tokens over a bf16 cache that holds their own keys in its last rows
-// (gfx950, bf16 in, fp32 softmax). Node i sees the L - n rows before the tree and, of the tree's n
-// rows, those with a bit in its mask.
+// Attention of a tree of drafted tokens over a bf16 cache that holds their own keys in its last rows (gfx950, bf16 in,
+// fp32 softmax). Node i sees the L - n rows before the tree and, of the tree's n rows, those with a bit in its mask.
 //
-// The query rows of the heads that share a KV head are flattened (row r: node r / G, head r % G) and
-// taken 32 at a time; S^T = K Q^T and O^T = V^T P^T go to the 32 x 32 x 16 matrix instructions with
-// the keys as the first operand, so that a lane holds one row's scores and P enters the second
-// product from the registers that it was made in (layouts in attn_split.hpp and attn_pipe.hpp). A
-// workgroup's waves take every KW-th tile of its split of the keys, each through LDS of its own.
-// Where the keys are split over workgroups too, those write unnormalised outputs with (maximum,
-// sum), and a second kernel joins them.
+// The query rows of the heads that share a KV head are flattened (row r: node r / G, head r % G) and taken 32 a wave;
+// S^T = K Q^T and O^T = V^T P^T go to the 32 x 32 x 16 matrix instructions with the keys as the first operand, so that
+// a lane holds one row's scores and P enters the second product from the registers that it was made in (layouts in
+// attn_split.hpp and attn_pipe.hpp). The keys are split over waves and workgroups; parts carry unnormalised outputs
+// with (maximum, sum) and are joined in LDS, and a second kernel joins those of different workgroups.
 //
-// P is rounded to bf16 for the second product, and the sums are over the rounded P, so that the
-// weights of a row add up to one; maxima, sums and outputs stay in fp32.
+// P is rounded to bf16 for the second product, and the sums are over the rounded P, so that the weights of a row add up
+// to one; maxima, sums and outputs stay in fp32.
+//
+// A short context is bound by latencies: a launch, a length and a tile that come from memory, the join. A long one reads
+// the cache at a part of the memory's rate, since each of a wave's steps waits for its tile, and the parts that the splits
+// write and the second launch weigh as much as a third of it (33 nodes at 32000 rows of 4 heads of 128: 66 MB in 22 us,
+// the join 5 us).
 #include "attn_split.hpp"
 #include "common.hpp"
 
@@ -25,6 +27,7 @@ int validate_attention_ctx(const efm_attention_ctx* c, const char* who);
 int prefill_cus();
 
 constexpr int kTreeMaxSplits = 256;
+constexpr int kTreeMany = 16000, kTreeLeast = 8, kTreeManyLeast = 4;   // tree_plan
 constexpr float kTreeLazy = 8.f;   // a maximum is followed once it is exceeded by 2^8 in weights
 
 struct TreeArgs {
@@ -52,17 +55,22 @@ __device__ __forceinline__ int tree_len(const TreeArgs& a) {
     return L >= (uint32_t)a.n && L <= a.max_kv_len ? (int)L : 0;
 }
 
-// Bit i: the node sees key k0 + i, for the KT keys from k0; c0: k0's place in the tree (negative in
-// the rows before it).
-template <int KT>
-__device__ __forceinline__ uint64_t tree_window(const uint64_t* row, int words, int c0) {
-    if (c0 <= -KT) return ~0ull;
-    if (c0 < 0) return row[0] << -c0 | ((1ull << -c0) - 1);
-    const int w = c0 / 64, sh = c0 % 64;
-    uint64_t bits = w < words ? row[w] >> sh : 0ull;
-    if (sh != 0 && w + 1 < words) bits |= row[w + 1] << (64 - sh);
-    return bits;
-}
+// The 64 bits of a node's mask from key c0 of the tree on, which may be before it: bit i says that the node sees key
+// c0 + i. request() may come long before get(), which waits for it.
+struct TreeBits {
+    uint64_t lo, hi;
+    __device__ __forceinline__ void request(const uint64_t* row, int words, int c0) {
+        const int w = max(c0, 0) / 64;
+        lo = row[min(w, words - 1)], hi = row[min(w + 1, words - 1)];
+    }
+    __device__ __forceinline__ uint64_t get(int words, int c0) const {
+        if (c0 <= -64) return ~0ull;
+        if (c0 < 0) return lo << -c0 | ((1ull << -c0) - 1);
+        const int w = c0 / 64, sh = c0 % 64;
+        const uint64_t a = w < words ? lo >> sh : 0ull, b = w + 1 < words ? hi << 1 << (63 - sh) : 0ull;
+        return a | b;
+    }
+};
 
 // A bf16 pair with zeros in the place of infinities and NaN.
 __device__ __forceinline__ uint32_t finite_pair(uint32_t w) {
@@ -83,6 +91,16 @@ __device__ __forceinline__ void tree_store(const TreeArgs& a, int kvh, int split
     const int64_t at = ((int64_t)split * a.Hkv + kvh) * a.rows + row;
     if (some) *reinterpret_cast<float4*>(a.o_part + at * HD + c * 4) = acc;
     if (c == 0) *reinterpret_cast<float2*>(a.ml_part + at * 2) = make_float2(m, l);
+}
+
+// What a workgroup works at. Workgroups go to the 8 XCDs in turn: an XCD takes an eighth of all workgroups, the row
+// blocks of a (split, head) side by side, which share the tiles in its L2. (Whole pairs to the XCDs in turn leave some of
+// them idle where the pairs are few or no multiple of 8: 1000 nodes at 2000 rows 53 -> 191 us.)
+__device__ __forceinline__ bool tree_place(const TreeArgs& a, int& kvh, int& split, int& block) {
+    const int all = a.Hkv * a.splits * a.blocks, xcd = blockIdx.x % 8, at = xcd * all / 8 + (int)(blockIdx.x / 8);
+    if (at >= (xcd + 1) * all / 8) return false;
+    block = at % a.blocks, kvh = at / a.blocks % a.Hkv, split = at / a.blocks / a.Hkv;
+    return true;
 }
 
 // Adds what is not finite of channels 4 c to 4 c + 3 of the values of keys [j0, j1) that a row sees.
@@ -141,163 +159,125 @@ __device__ __forceinline__ void tree_each(F f) {
     (std::make_integer_sequence<int, N>{});
 }
 
-// NB x 32 rows a workgroup of four waves, a wave a SIMD. A wave's tiles (8 KB of keys and 8 KB of values) go
-// through two slots each of its own in LDS, requested two tiles ahead. A wave issues in order, so what is to
-// run beside the matrix instructions stands between them: the first row block's exponentials between the
-// second's first products, the second's between the first's second products, and the next tile's keys are
-// read from LDS meanwhile.
-template <int HD, int NB>
-__global__ __launch_bounds__(256, 1) void tree_attn_kernel(TreeArgs a) {
+// Few rows: 32 a workgroup, whose waves take every KW-th tile of 8 KB of keys and 8 KB of values, each through a
+// slot of its own in LDS that is requested again as soon as it is read out, so that no wave waits for another
+// before the end. Two workgroups share a CU: one's products run while the other's tiles arrive. (Two slots a wave and
+// loads two tiles ahead, one workgroup a CU: 11.4 -> 12.3 us for 24 nodes at 2003 rows, 28 -> 61 us for 250 at 3900.)
+template <int HD>
+__global__ __launch_bounds__(256, 2) void tree_few_kernel(TreeArgs a) {
     typedef SplitTile<HD> T;
     constexpr int KW = 4, KT = T::kKeys, NH = KT / 32, KS = HD / 16, DT = HD / 32, NL = T::kLoads, KB = KT / 16;
-    constexpr int SLOT = T::kBytes, RING = 4 * SLOT, CPR = HD / 4;   // a wave's: keys 0, keys 1, values 0, values 1
-    constexpr int NM = NH * KS, NE = NH * 16 / NM;                   // matrix instructions of a product; weights between two
-    static_assert(NM == KB * DT && NM == 8 && NB * 32 * HD * 4 <= RING, "tile geometry");
+    constexpr int SLOT = 2 * T::kBytes, CPR = HD / 4;
     typedef short s4_t __attribute__((ext_vector_type(4)));
-    __shared__ __align__(1024) unsigned char smem[KW * RING];
-    __shared__ float ml[2][KW][NB * 32];
+    __shared__ __align__(1024) unsigned char smem[KW * SLOT];
+    __shared__ float ml[2][KW][32];
     __shared__ int s_odd[KW];
+    static_assert(32 * HD * 4 <= SLOT && 32 * CPR % (KW * kWave) == 0, "a wave's outputs fit in its slot");
 
     const int tid = threadIdx.x;
     const int wave = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave;
     const int ql = lane % 32, hh = lane / 32;
-    // the row blocks of a (head, split) are 8 workgroups apart: on one XCD, whose L2 they share
-    const int xcd = blockIdx.x % 8, rest = blockIdx.x / 8;
-    const int unit = rest / a.blocks * 8 + xcd, block = rest % a.blocks;
-    if (unit >= a.Hkv * a.splits) return;
-    const int kvh = unit % a.Hkv, split = unit / a.Hkv, r0 = block * NB * 32;
+    int kvh, split, block;
+    if (!tree_place(a, kvh, split, block)) return;
+    const int r0 = block * 32, row = min(r0 + ql, a.rows - 1), node = row / a.G, head = kvh * a.G + row % a.G;
+    const int bound = a.bound, t0 = split * a.split_tiles;
+    int t = t0 + wave;
 
-    const int L = tree_len(a), before = L - a.n;   // rows before the tree
-    const int t0 = split * a.split_tiles, tile_end = min((L + KT - 1) / KT, t0 + a.split_tiles);
     const char* const kbase = reinterpret_cast<const char*>(a.k + kvh * a.k_sh);
     const char* const vbase = reinterpret_cast<const char*>(a.v + kvh * a.v_sh);
-    unsigned char* const ring = smem + wave * RING;
+    unsigned char* const kslot = smem + wave * SLOT;
+    unsigned char* const vslot = kslot + T::kBytes;
     const int pr = lane / T::kChunks, pc = lane % T::kChunks;
     auto issue = [&](const char* base, int sn, int k0, unsigned char* slot, auto is_v) {
         const char* const tile = base + (int64_t)k0 * sn * 2;
-        const bool whole = k0 + KT <= L;
+        const bool whole = k0 + KT <= bound;
 #pragma unroll
         for (int i = 0; i < NL; ++i) {
             const int rr = i * T::kRows + pr;
             const int c = pc ^ (decltype(is_v)::value ? T::v_swz(rr) : T::k_swz(rr));
-            const int r = whole ? rr : min(rr, L - 1 - k0);   // rows past the end read the last row
+            const int r = whole ? rr : min(rr, bound - 1 - k0);   // rows past the end read the last row
             __builtin_amdgcn_global_load_lds(static_cast<const void*>(tile + (uint32_t)((r * sn + c * 8) * 2)),
                                              (__attribute__((address_space(3))) void*)(slot + i * 1024), 16, 0, 0);
         }
     };
-    auto issue_k = [&](int t, int b) { issue(kbase, a.k_sn, t * KT, ring + b * SLOT, std::false_type{}); };
-    auto issue_v = [&](int t, int b) { issue(vbase, a.v_sn, t * KT, ring + (2 + b) * SLOT, std::true_type{}); };
+    auto issue_k = [&](int tt) { issue(kbase, a.k_sn, tt * KT, kslot, std::false_type{}); };
+    auto issue_v = [&](int tt) { issue(vbase, a.v_sn, tt * KT, vslot, std::true_type{}); };
 
     // Q, the second operand: d = 16 ks + 8 hh + e
-    bf16x8_t qf[NB][KS];
-    const uint64_t* bits_row[NB];
-#pragma unroll
-    for (int n = 0; n < NB; ++n) {
-        const int row = min(r0 + n * 32 + ql, a.rows - 1), node = row / a.G, head = kvh * a.G + row % a.G;
+    bf16x8_t qf[KS];
+    {
         const bf16_t* qp = a.q + node * a.q_sn + head * a.q_sh;
-        bits_row[n] = a.mask + (int64_t)node * a.words;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
             Pack8 x;
             x.u = *reinterpret_cast<const uint4*>(qp + ks * 16 + hh * 8);
-            qf[n][ks] = x.v;
+            qf[ks] = x.v;
         }
     }
-    int t = t0 + wave;
-    if (t < tile_end) issue_k(t, 0), issue_v(t, 0);
-    if (t + KW < tile_end) issue_k(t + KW, 1), issue_v(t + KW, 1);
+    // the first tile is requested before the length is known: the cache holds `bound` rows
+    if (t < min((bound + KT - 1) / KT, t0 + a.split_tiles)) {
+        issue_k(t);
+        issue_v(t);
+    }
+    const int L = tree_len(a), before = L - a.n;   // rows before the tree
+    const int tile_end = min((L + KT - 1) / KT, t0 + a.split_tiles);
     // Q has landed here: a first use in the loop would wait for every load under way, each time
 #pragma unroll
-    for (int n = 0; n < NB; ++n)
+    for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(qf[ks]));
+    f32x16_t oacc[DT];
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(qf[n][ks]));
+    for (int tt = 0; tt < DT; ++tt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) oacc[tt][e] = 0.f;
+    float m_run = -INFINITY, l_part = 0.f;   // the largest score so far; the sum over the lane's half of the keys
+    bool odd = false;
+    const uint64_t* const bits_row = a.mask + (int64_t)node * a.words;
 
-    f32x16_t o[NB][DT];
-    float m_run[NB], l_part[NB];   // the largest score so far; the sum over the lane's half of the keys
-#pragma unroll
-    for (int n = 0; n < NB; ++n) {
-        m_run[n] = -INFINITY, l_part[n] = 0.f;
-#pragma unroll
-        for (int i = 0; i < DT; ++i)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) o[n][i][e] = 0.f;
-    }
-    const uint32_t lds = (uint32_t)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) unsigned char*)ring);
+    const uint32_t lk = (uint32_t)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) unsigned char*)kslot);
     uint32_t ka[KS], va[DT];
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) ka[ks] = lds + (uint32_t)(ql * T::kRow + (((ks * 2 + hh) ^ T::k_swz(ql)) << 4));
+    for (int ks = 0; ks < KS; ++ks) ka[ks] = lk + (uint32_t)(ql * T::kRow + (((ks * 2 + hh) ^ T::k_swz(ql)) << 4));
     {
         const int g = lane >> 4, j = lane & 15, rr = (g >> 1) * 4 + (j >> 2);
 #pragma unroll
-        for (int i = 0; i < DT; ++i) {
-            const int d = i * 32 + 16 * (g & 1) + 4 * (j & 3);
-            va[i] = lds + (uint32_t)(2 * SLOT + rr * T::kRow + (((d >> 3) ^ T::v_swz(rr)) << 4) + ((d & 7) << 1));
+        for (int tt = 0; tt < DT; ++tt) {
+            const int d = tt * 32 + 16 * (g & 1) + 4 * (j & 3);
+            va[tt] = lk + (uint32_t)(T::kBytes + rr * T::kRow + (((d >> 3) ^ T::v_swz(rr)) << 4) + ((d & 7) << 1));
         }
     }
     const float lazy = kTreeLazy / a.scale;
-    bf16x8_t kf[NH][KS];
-    auto read_k = [&](int b) {
-        const uint32_t at = (uint32_t)(b * SLOT);
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-            attn_pipe::read_b128<0>(kf[0][ks], ka[ks] + at);
-            if constexpr (NH == 2) attn_pipe::read_b128<32 * T::kRow>(kf[1][ks], ka[ks] + at);
-        }
-    };
-    if (t < tile_end) {
-        if (t + KW < tile_end) attn_pipe::vm_wait<3 * NL>();
-        else attn_pipe::vm_wait<NL>();
-        read_k(0);
-    }
-    bool odd = false;
-    for (int b = 0; t < tile_end; t += KW, b ^= 1) {
-        const bool one = t + KW < tile_end, two = t + 2 * KW < tile_end;   // tiles to come
+    for (; t < tile_end; t += KW) {
+        const bool more = t + KW < tile_end;
         const int kb0 = t * KT;
         const bool masked = kb0 + KT > before;
-        uint64_t bits[NB];
+        uint64_t bits = ~0ull;
+        if (masked) {   // requested before the waits below
+            TreeBits window;
+            window.request(bits_row, a.words, kb0 - before);
+            bits = window.get(a.words, kb0 - before);
+            if (L - kb0 < 64) bits &= (1ull << (L - kb0)) - 1;
+            asm volatile("" : "+v"(bits));
+            attn_pipe::vm_wait<0>();
+        } else {
+            attn_pipe::vm_wait<NL>();   // K has landed; V may be under way
+        }
+        asm volatile("" ::: "memory");
+        bf16x8_t kf[NH][KS];
 #pragma unroll
-        for (int n = 0; n < NB; ++n) bits[n] = ~0ull;
+        for (int ks = 0; ks < KS; ++ks) {
+            attn_pipe::read_b128<0>(kf[0][ks], ka[ks]);
+            if constexpr (NH == 2) attn_pipe::read_b128<32 * T::kRow>(kf[1][ks], ka[ks]);
+        }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 #pragma unroll
         for (int h = 0; h < NH; ++h)
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(kf[h][ks]));
-        if (two) issue_k(t + 2 * KW, b);
-        // S^T; element e of s[n][h]: key kb0 + 32 h + 8 (e / 4) + 4 hh + e % 4 of row block n
-        f32x16_t s[NB][NH];
-#pragma unroll
-        for (int n = 0; n < NB; ++n)
-#pragma unroll
-            for (int h = 0; h < NH; ++h)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) s[n][h][e] = 0.f;
-        auto qk = [&](auto nc, auto ic) {
-            constexpr int N = decltype(nc)::value, H = decltype(ic)::value % NH, K = decltype(ic)::value / NH;
-            s[N][H] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[H][K], qf[N][K], s[N][H], 0, 0, 0);
-        };
-        using std::integral_constant;
-        tree_each<NM>([&](auto i) { qk(integral_constant<int, 0>{}, i); });
+        // Values that a row does not see take no part in its output whatever they are: a zero weight
+        // times an infinity would be a NaN. V of the tree's rows and of rows past the end is made
+        // finite here, and what was not is added at the end where it is seen.
         if (masked) {
-#pragma unroll
-            for (int n = 0; n < NB; ++n) {
-                bits[n] = tree_window<KT>(bits_row[n], a.words, kb0 - before);
-                if (L - kb0 < 64) bits[n] &= (1ull << (L - kb0)) - 1;
-                asm volatile("" : "+v"(bits[n]));
-            }
-            attn_pipe::vm_wait<0>();
-        } else if (two) {
-            attn_pipe::vm_wait<3 * NL>();
-        } else if (one) {
-            attn_pipe::vm_wait<2 * NL>();
-        } else {
-            attn_pipe::vm_wait<0>();
-        }
-        asm volatile("" ::: "memory");
-        // Values that a row does not see take no part in its output whatever they are: a zero weight times an
-        // infinity would be a NaN. V of the tree's rows and of rows past the end is made finite here, and what
-        // was not is added at the end where it is seen.
-        if (masked) {
-            uint4* const vp = reinterpret_cast<uint4*>(ring + (2 + b) * SLOT);
+            uint4* const vp = reinterpret_cast<uint4*>(vslot);
 #pragma unroll
             for (int i = 0; i < NL; ++i) {
                 const uint4 x = vp[i * 64 + lane];
@@ -309,127 +289,125 @@ __global__ __launch_bounds__(256, 1) void tree_attn_kernel(TreeArgs a) {
             }
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         }
-        s4_t vf[KB][DT][2];
-        {
-            const uint32_t at = (uint32_t)(b * SLOT);
-            tree_each<KB>([&](auto kc) {
-                constexpr int K = decltype(kc)::value;
+        if (more) issue_k(t + KW);
+        // S^T; element e of s[h]: key kb0 + 32 h + 8 (e / 4) + 4 hh + e % 4 of the lane's row
+        f32x16_t s[NH];
 #pragma unroll
-                for (int i = 0; i < DT; ++i) {
-                    attn_pipe::read_tr16<16 * K * T::kRow>(vf[K][i][0], va[i] + at);
-                    attn_pipe::read_tr16<(16 * K + 8) * T::kRow>(vf[K][i][1], va[i] + at);
-                }
-            });
+        for (int h = 0; h < NH; ++h) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[h][e] = 0.f;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) s[h] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[h][ks], qf[ks], s[h], 0, 0, 0);
         }
-        float ref[NB];
-        // masks the scores of row block n, and follows its maximum where it is exceeded by 2^kTreeLazy in weights
-        auto maximum = [&](auto nc) {
-            constexpr int N = decltype(nc)::value;
-            if (masked) {
-                const uint64_t mine = bits[N] >> (4 * hh);
+        if (!masked) {
+            if (more) attn_pipe::vm_wait<NL>();
+            else attn_pipe::vm_wait<0>();
+        }
+        asm volatile("" ::: "memory");
+        s4_t vf[KB][DT][2];
 #pragma unroll
-                for (int h = 0; h < NH; ++h)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e)
-                        s[N][h][e] = (mine >> (32 * h + 8 * (e / 4) + e % 4) & 1) ? s[N][h][e] : -INFINITY;
+        for (int tt = 0; tt < DT; ++tt) {
+            attn_pipe::read_tr16<0>(vf[0][tt][0], va[tt]);
+            attn_pipe::read_tr16<8 * T::kRow>(vf[0][tt][1], va[tt]);
+            attn_pipe::read_tr16<16 * T::kRow>(vf[1][tt][0], va[tt]);
+            attn_pipe::read_tr16<24 * T::kRow>(vf[1][tt][1], va[tt]);
+            if constexpr (KB == 4) {
+                attn_pipe::read_tr16<32 * T::kRow>(vf[KB - 2][tt][0], va[tt]);
+                attn_pipe::read_tr16<40 * T::kRow>(vf[KB - 2][tt][1], va[tt]);
+                attn_pipe::read_tr16<48 * T::kRow>(vf[KB - 1][tt][0], va[tt]);
+                attn_pipe::read_tr16<56 * T::kRow>(vf[KB - 1][tt][1], va[tt]);
             }
-            float top = s[N][0][0];
+        }
+        if (masked) {
+            const uint64_t mine = bits >> (4 * hh);
 #pragma unroll
             for (int h = 0; h < NH; ++h)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) top = fmaxf(top, s[N][h][e]);
+                for (int e = 0; e < 16; ++e)
+                    s[h][e] = (mine >> (32 * h + 8 * (e / 4) + e % 4) & 1) ? s[h][e] : -INFINITY;
+        }
+        float top = s[0][0];
+#pragma unroll
+        for (int h = 0; h < NH; ++h)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) top = fmaxf(top, s[h][e]);
+        {
             const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
             top = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
-            if (__any(top > m_run[N] + lazy)) {   // from -inf: whatever is seen first
-                const float m_new = fmaxf(m_run[N], top);
-                const float alpha = m_run[N] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m_run[N] - m_new) * a.scale);
-                l_part[N] *= alpha;
+        }
+        if (__any(top > m_run + lazy)) {   // from -inf: whatever is seen first
+            const float m_new = fmaxf(m_run, top);
+            const float alpha = m_run == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m_run - m_new) * a.scale);
+            l_part *= alpha;
 #pragma unroll
-                for (int i = 0; i < DT; ++i)
+            for (int tt = 0; tt < DT; ++tt)
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) o[N][i][e] *= alpha;
-                m_run[N] = m_new;
-            }
-            ref[N] = m_run[N] == -INFINITY ? 0.f : m_run[N] * a.scale;
-        };
-        uint32_t pw[NB][NH * 8];   // weights, two a word
-        auto weigh = [&](auto nc, auto ic) {   // NE of them
-            constexpr int N = decltype(nc)::value, I = decltype(ic)::value;
+                for (int e = 0; e < 16; ++e) oacc[tt][e] *= alpha;
+            m_run = m_new;
+        }
+        const float ref = m_run == -INFINITY ? 0.f : m_run * a.scale;
+        Pack8 pb[KB];
 #pragma unroll
-            for (int j = 0; j < NE; j += 2) {
-                constexpr int E0 = I * NE;
-                const int e = E0 + j;
-                const float x = __builtin_amdgcn_exp2f(fmaf(s[N][e / 16][e % 16], a.scale, -ref[N]));
-                const float y = __builtin_amdgcn_exp2f(fmaf(s[N][e / 16][e % 16 + 1], a.scale, -ref[N]));
-                pw[N][e / 2] = pack_bf16x2(x, y);
-                l_part[N] = add_bf16_pair(pw[N][e / 2], l_part[N]);
-            }
-        };
-        auto pv = [&](auto nc, auto ic) {
-            constexpr int N = decltype(nc)::value, K = decltype(ic)::value / DT, I = decltype(ic)::value % DT;
-            union {
-                s4_t h[2];
-                bf16x8_t v;
-            } vv;
-            vv.h[0] = vf[K][I][0];
-            vv.h[1] = vf[K][I][1];
-            Pack8 p;
-            p.u = make_uint4(pw[N][4 * K], pw[N][4 * K + 1], pw[N][4 * K + 2], pw[N][4 * K + 3]);
-            o[N][I] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vv.v, p.v, o[N][I], 0, 0, 0);
-        };
-        maximum(integral_constant<int, 0>{});
-        tree_each<NM>([&](auto i) {
-            if constexpr (NB == 2) qk(integral_constant<int, NB - 1>{}, i);
-            weigh(integral_constant<int, 0>{}, i);
-            if constexpr (NB == 2) __builtin_amdgcn_sched_barrier(0);
-        });
-        if constexpr (NB == 2) maximum(integral_constant<int, NB - 1>{});
+        for (int h = 0; h < NH; ++h) {
+            float p[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) p[e] = __builtin_amdgcn_exp2f(fmaf(s[h][e], a.scale, -ref));
+            pb[2 * h].u = pack8(&p[0]);
+            pb[2 * h + 1].u = pack8(&p[8]);
+        }
+#pragma unroll
+        for (int b = 0; b < KB; ++b) {
+            l_part = add_bf16_pair(pb[b].u.x, l_part);
+            l_part = add_bf16_pair(pb[b].u.y, l_part);
+            l_part = add_bf16_pair(pb[b].u.z, l_part);
+            l_part = add_bf16_pair(pb[b].u.w, l_part);
+        }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-            for (int i = 0; i < DT; ++i) asm volatile("" : "+v"(vf[kb][i][0]), "+v"(vf[kb][i][1]));
-        if (two) issue_v(t + 2 * KW, b);
-        if (one) {   // the next tile's keys
-            if (masked) attn_pipe::vm_wait<0>();
-            else if (two) attn_pipe::vm_wait<3 * NL>();
-            else attn_pipe::vm_wait<NL>();
-            asm volatile("" ::: "memory");
-            read_k(b ^ 1);
-        }
-        tree_each<NM>([&](auto i) {
-            pv(integral_constant<int, 0>{}, i);
-            if constexpr (NB == 2) {
-                weigh(integral_constant<int, NB - 1>{}, i);
-                __builtin_amdgcn_sched_barrier(0);
+            for (int tt = 0; tt < DT; ++tt) asm volatile("" : "+v"(vf[kb][tt][0]), "+v"(vf[kb][tt][1]));
+        if (more) issue_v(t + KW);
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int tt = 0; tt < DT; ++tt) {
+                union {
+                    s4_t h[2];
+                    bf16x8_t v;
+                } vv;
+                vv.h[0] = vf[kb][tt][0];
+                vv.h[1] = vf[kb][tt][1];
+                oacc[tt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vv.v, pb[kb].v, oacc[tt], 0, 0, 0);
             }
-        });
-        if constexpr (NB == 2) tree_each<NM>([&](auto i) { pv(integral_constant<int, NB - 1>{}, i); });
     }
+    attn_pipe::vm_wait<0>();   // a tile past the length
+    asm volatile("" ::: "memory");
 
     // the waves' outputs meet in LDS (float4 chunk c of row r at c ^ (r & 15))
+    {
+        float4* const part = reinterpret_cast<float4*>(kslot);
 #pragma unroll
-    for (int n = 0; n < NB; ++n) {
-        float4* const part = reinterpret_cast<float4*>(ring) + n * 32 * CPR;
-#pragma unroll
-        for (int i = 0; i < DT; ++i)
+        for (int tt = 0; tt < DT; ++tt)
 #pragma unroll
             for (int g = 0; g < 4; ++g)
-                part[ql * CPR + ((i * 8 + g * 2 + hh) ^ (ql & 15))] =
-                    make_float4(o[n][i][g * 4], o[n][i][g * 4 + 1], o[n][i][g * 4 + 2], o[n][i][g * 4 + 3]);
-        const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(l_part[n]), __float_as_uint(l_part[n]), false, false);
+                part[ql * CPR + ((tt * 8 + g * 2 + hh) ^ (ql & 15))] =
+                    make_float4(oacc[tt][g * 4], oacc[tt][g * 4 + 1], oacc[tt][g * 4 + 2], oacc[tt][g * 4 + 3]);
+        const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(l_part), __float_as_uint(l_part), false, false);
         if (hh == 0) {
-            ml[0][wave][n * 32 + ql] = m_run[n] * a.scale;
-            ml[1][wave][n * 32 + ql] = __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
+            ml[0][wave][ql] = m_run * a.scale;
+            ml[1][wave][ql] = __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
         }
+        odd = __any(odd);
+        if (lane == 0) s_odd[wave] = odd;
     }
-    odd = __any(odd);
-    if (lane == 0) s_odd[wave] = odd;
     __syncthreads();
-    odd = (s_odd[0] | s_odd[1] | s_odd[2] | s_odd[3]) != 0;
-    tree_join<HD, KW, NB * 32 * CPR / 256>(a, tid, 256, kvh, split, r0, tile_end > t0, [&](int w, int r, int c) {
-        return reinterpret_cast<const float4*>(smem + w * RING)[r * CPR + (c ^ (r & 15))];
-    }, &ml[0][0][0], NB * 32, [&](int gr, int c, float4& acc) {
+    odd = false;
+#pragma unroll
+    for (int w = 0; w < KW; ++w) odd |= s_odd[w] != 0;
+    tree_join<HD, KW, 32 * CPR / (KW * kWave)>(a, tid, KW * kWave, kvh, split, r0, tile_end > t0, [&](int w, int r, int c) {
+        return reinterpret_cast<const float4*>(smem + w * SLOT)[r * CPR + (c ^ (r & 15))];
+    }, &ml[0][0][0], 32, [&](int gr, int c, float4& acc) {
         if (odd) tree_not_finite(a, vbase, gr, c, before, max(before / KT, t0) * KT, min(L, tile_end * KT), acc);
     });
 }
@@ -453,10 +431,8 @@ __global__ __launch_bounds__(512, 2) void tree_rows_kernel(TreeArgs a) {
     const int tid = threadIdx.x;
     const int wave = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave, grp = wave / 4, wg = wave % 4;
     const int ql = lane % 32, hh = lane / 32;
-    const int xcd = blockIdx.x % 8, rest = blockIdx.x / 8;
-    const int unit = rest / a.blocks * 8 + xcd, block = rest % a.blocks;
-    if (unit >= a.Hkv * a.splits) return;
-    const int kvh = unit % a.Hkv, split = unit / a.Hkv;
+    int kvh, split, block;
+    if (!tree_place(a, kvh, split, block)) return;
     const int r0 = block * 128, row = min(r0 + wg * 32 + ql, a.rows - 1), node = row / a.G, head = kvh * a.G + row % a.G;
     const bool idle = r0 + wg * 32 >= a.rows;   // a wave without rows helps to load
 
@@ -541,18 +517,19 @@ __global__ __launch_bounds__(512, 2) void tree_rows_kernel(TreeArgs a) {
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
     };
+    TreeBits window = {};
+    if (steps > 0 && (t0 + grp) * KT + KT > before) window.request(bits_row, a.words, (t0 + grp) * KT - before);
     for (int st = 0; st < steps; ++st) {
         const int t = t0 + 2 * st + grp, kb0 = t * KT;
         const bool on = t < tile_end, masked = kb0 + KT > before;
         // whether either group's tile is of the tree's rows: the same in every wave
         const bool clean = (t0 + 2 * st + 1) * KT + KT > before;
+        attn_pipe::vm_wait<0>();
         uint64_t bits = ~0ull;
         if (on && masked) {
-            bits = tree_window<KT>(bits_row, a.words, kb0 - before);
+            bits = window.get(a.words, kb0 - before);
             if (L - kb0 < 64) bits &= (1ull << (L - kb0)) - 1;
-            asm volatile("" : "+v"(bits));
         }
-        attn_pipe::vm_wait<0>();
         meet();   // the tile is there, and the other slot is read out
         unsigned char* const stage = ring + (st & 1) * STAGE;
         if (clean) {
@@ -573,7 +550,10 @@ __global__ __launch_bounds__(512, 2) void tree_rows_kernel(TreeArgs a) {
             if (__any(odd) && lane == 0) s_odd = 1;
             meet();
         }
-        if (t + 2 < tile_end) issue(t + 2, (st + 1) & 1);
+        if (t + 2 < tile_end) {
+            issue(t + 2, (st + 1) & 1);
+            if (kb0 + 3 * KT > before) window.request(bits_row, a.words, kb0 + 2 * KT - before);
+        }
         if (!on || idle) continue;
         const uint32_t at = (uint32_t)((st & 1) * STAGE);
         // S^T; element e of s[h]: key kb0 + 32 h + 8 (e / 4) + 4 hh + e % 4 of the lane's row
@@ -775,23 +755,30 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a) {
 }
 
 struct TreePlan {
-    int nb;   // row blocks of 32 of a workgroup
+    bool many;   // tree_rows_kernel
     int blocks, splits, split_tiles;
     size_t o_bytes, ml_bytes;
     size_t total() const { return o_bytes + ml_bytes; }
 };
 
+// tree_few_kernel or tree_rows_kernel: the first starts and joins faster, the second reads a tile for four times as many
+// rows. With the tiles of 8 KB that blocks of 32 rows visit, both measured in us:
+//   630 (24 nodes, 2000 rows) 11.5 | 14.8     8000 (33, 8000) 18.5 | 22.7     11000 (100, 4000) 23.4 | 26.3
+//   16000 (250, 3900) 28.2 | 27.4             16000 (33, 16000) 27.0 | 24.1   32000 (33, 32000) 40.3 | 32.3
+// A workgroup a CU, or two where a row block has fewer than four splits, whose join is cheap (250 nodes at 3900 rows
+// 39 -> 28 us; 24 nodes at 32000, 25 splits instead of 51, 25 -> 20 us); a split of two tiles a wave at least.
 static TreePlan tree_plan(const efm_attention_ctx* c, uint32_t n, uint32_t kv_len) {
     const int hd = (int)c->head_dim, Hkv = (int)c->num_kv_heads;
     const int64_t rows = (int64_t)n * (c->num_qo_heads / c->num_kv_heads), cus = prefill_cus();
     TreePlan p = {};
-    p.nb = rows > 64 ? 4 : rows > 32 ? 2 : 1;
-    const int keys = hd == 128 && p.nb < 4 ? 32 : 64;
+    const int few = hd == 128 ? 32 : 64;   // keys of 8 KB
+    p.many = (rows + 31) / 32 * Hkv * (((int64_t)kv_len + few - 1) / few) >= kTreeMany;
+    const int keys = p.many ? 64 : few;
     const int64_t tiles = ((int64_t)kv_len + keys - 1) / keys;
-    p.blocks = (int)((rows + 32 * p.nb - 1) / (32 * p.nb));
-    const int64_t want = std::max<int64_t>(1, cus / ((int64_t)p.blocks * Hkv));   // a workgroup a CU
-    p.split_tiles = (int)std::max<int64_t>({4, (tiles + want - 1) / want, (tiles + kTreeMaxSplits - 1) / kTreeMaxSplits});
-    if (p.nb < 4) p.split_tiles = (p.split_tiles + 3) / 4 * 4;   // as many for each wave
+    p.blocks = (int)((rows + (p.many ? 127 : 31)) / (p.many ? 128 : 32));
+    const int64_t pairs = (int64_t)p.blocks * Hkv, each = !p.many && cus / pairs < 4 ? 2 : 1;
+    const int64_t want = std::max<int64_t>(1, each * cus / pairs);
+    p.split_tiles = (int)std::max<int64_t>({p.many ? kTreeManyLeast : kTreeLeast, (tiles + want - 1) / want, (tiles + kTreeMaxSplits - 1) / kTreeMaxSplits});
     p.splits = (int)std::max<int64_t>(1, (tiles + p.split_tiles - 1) / p.split_tiles);
     if (p.splits > 1) {
         p.o_bytes = (size_t)p.splits * Hkv * rows * hd * sizeof(float);
@@ -877,13 +864,12 @@ extern "C" int efm_attention_tree(const efm_attention_ctx* ctx, const void* q, c
     a.splits = p.splits;
     a.split_tiles = p.split_tiles;
     a.scale = 1.4426950408889634f / sqrtf((float)hd);
-    const int64_t units = ((int64_t)Hkv * p.splits + 7) / 8 * 8, all = (int64_t)Hkv * a.rows;
-    const dim3 grid((unsigned)(units * p.blocks));
+    const int64_t all = (int64_t)Hkv * a.rows;
+    const dim3 grid((unsigned)(((int64_t)Hkv * p.splits * p.blocks + 7) / 8 * 8));
     auto launch = [&](auto hdc) {
         constexpr int HD = decltype(hdc)::value;
-        if (p.nb == 4) hipLaunchKernelGGL(tree_rows_kernel<HD>, grid, dim3(512), 0, stream, a);
-        else if (p.nb == 2) hipLaunchKernelGGL((tree_attn_kernel<HD, 2>), grid, dim3(256), 0, stream, a);
-        else hipLaunchKernelGGL((tree_attn_kernel<HD, 1>), grid, dim3(256), 0, stream, a);
+        if (p.many) hipLaunchKernelGGL(tree_rows_kernel<HD>, grid, dim3(512), 0, stream, a);
+        else hipLaunchKernelGGL(tree_few_kernel<HD>, grid, dim3(256), 0, stream, a);
         if (p.splits > 8) hipLaunchKernelGGL((tree_merge_kernel<HD, 256>), dim3((unsigned)all), dim3(256), 0, stream, a);
         else if (p.splits > 1) hipLaunchKernelGGL((tree_merge_kernel<HD, 64>), dim3((unsigned)((all + 3) / 4)), dim3(256), 0, stream, a);
     };
