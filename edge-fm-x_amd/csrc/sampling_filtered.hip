@@ -24,11 +24,13 @@
 //   top-k                1. the maxima of runs of 32 logits: the top_k-th largest of those bounds the
 //                        top_k-th logit from below  2. a list of the ids above the bound, from the runs
 //                        that reach it; the ends of K and N in it, and the draw
-// Top-p's third step is done so too where few runs reach N's end, and min-p's second.
-// Few rows of a large vocabulary are cut into blocks of a workgroup each, a launch a step, and what
-// follows the last step's pass is done by the row's last workgroup to arrive. Small vocabularies and
-// many rows take one launch, a workgroup a row. Where the list does not fit (thousands of equal logits)
-// the choice is made from the row itself.
+// Top-p's third step is done so too where few runs reach N's end.
+// Rows of a large vocabulary are cut into blocks of a workgroup each, a launch a step, and what follows
+// the last step's pass is done by the row's last workgroup to arrive. Small vocabularies take one
+// launch, a workgroup a row. A list that does not fit in LDS is read from the workspace (top-p of flat
+// rows, where thousands of ids have the mass at which N ends: 33 rows of 151936 55 us, peaked ones 29),
+// and where it does not fit there either, or top_k is in the thousands, the choice is made from the row
+// itself, some ten passes of a workgroup (top_k = 5000 of 151936: 340 us).
 #include "common.hpp"
 
 #include <algorithm>
@@ -49,6 +51,7 @@ constexpr int kFiltRuns = 5120;                  // runs of neighbouring logits 
 constexpr int kFiltRunBins = 1024;
 constexpr int kFiltFewRuns = 512;                // that one workgroup goes through
 constexpr int kFiltHeld = 1024, kFiltHeldK = 2048;   // entries of a list that a workgroup holds with their masses; top-k
+constexpr int kFiltLong = 8192;                  // entries of a row's list in the workspace
 constexpr int kFiltOneVocab = 16384;             // vocabularies of one launch
 
 // One row's part of the workspace.
@@ -58,7 +61,7 @@ struct FiltRow {
     uint32_t pad[2];
     float bmax[kFiltBlocks];
     unsigned long long tile[kFiltTiles];
-    unsigned long long list[kFiltHeld];   // key << 32 | id
+    unsigned long long list[kFiltLong];   // key << 32 | id
     float run[kFiltRuns];
 };
 static_assert(sizeof(FiltRow) % 16 == 0, "rows of the workspace stay aligned");
@@ -84,7 +87,7 @@ enum { kFiltAll, kFiltTopP, kFiltTopK };
 // w of a logit, m the row's largest. 2^t, t = (l - m) log2(e) / T, is 2^n 2^f with the series of
 // exp(f ln 2), |f| <= 1/2: the term after the last is below 2^-52. Adding 1.5 2^52 rounds t to an integer,
 // and a last step to p 2^(n + 44) + 2^52 leaves w in the low bits. Without branches, so that a thread's
-// logits go through side by side (33 rows of 151936: 14.9 -> 9.5 us for the masses by bin).
+// logits go through side by side (33 rows of 151936: 15.1 -> 11.9 us for the masses by bin).
 __device__ __forceinline__ uint64_t filt_mass(const FiltArgs& a, float l, float m) {
     const double t = l == m ? 0.0 : ((double)l - (double)m) * a.to_log2;
     const double near = t + 6755399441055744.0, f = t - (near - 6755399441055744.0);
@@ -274,11 +277,11 @@ __device__ __forceinline__ uint64_t filt_need(float top_p, uint64_t W) {
     return need < 1 ? 1 : need > W ? W : need;
 }
 
-// The entry that holds unit `rank` of the weights of a source of (id, key, weight), each(f): in the
-// sampler's order (keys of [low, high]), or by id alone (ids of [low, high]). The range that may hold
-// it is cut into 256 bins until one entry is left, four times for keys and three for the ids of equal
-// keys at most. rank is below the sum of the weights.
-template <int NT, typename Each>
+// The entry that holds unit `rank` of the weights of a source, each(f): f(id, key, whether it is one, weight()) by whole
+// waves where ROW; in the sampler's order (keys of [low, high]), or by id alone (ids of [low, high]). The range that may
+// hold it is cut into 256 bins until one entry is left, four times for keys and three for the ids of equal keys at most;
+// weights outside it are not asked for. rank is below the sum of the weights.
+template <int NT, bool ROW, typename Each>
 __device__ __forceinline__ FiltCut filt_pick(bool by_id, uint32_t low, uint32_t high, uint64_t rank, const FiltArgs& a, FiltShared<NT>& s,
                                              Each each) {
     const int tid = threadIdx.x;
@@ -287,17 +290,31 @@ __device__ __forceinline__ FiltCut filt_pick(bool by_id, uint32_t low, uint32_t 
     __syncthreads();
     if (tid < 256) s.bins[0][tid] = 0, s.counts[0][tid] = 0;
     __syncthreads();
+#pragma unroll 1
     for (int step = 0; step < 8; ++step) {
         const int b = step & 1, bits = 32 - __builtin_clz(hi - lo | 1u), shift = max(bits - 8, 0);
         auto value = [&](int i, uint32_t k) { return ids ? (uint32_t)i : ~k; };
-        auto active = [&](int i, uint32_t k, uint64_t w) {
-            return w != 0 && value(i, k) >= lo && value(i, k) <= hi && (!ids || by_id || ~k == tie);
-        };
-        each([&](int i, uint32_t k, uint64_t w) {
-            if (!active(i, k, w)) return;
+        auto active = [&](int i, uint32_t k) { return value(i, k) >= lo && value(i, k) <= hi && (!ids || by_id || ~k == tie); };
+        each([&](int i, uint32_t k, bool in, auto weight) {
+            uint64_t w = 0;
+            if (in && active(i, k)) w = weight();
             const uint32_t bin = (value(i, k) - lo) >> shift;
-            atomicAdd(&s.bins[b][bin], (unsigned long long)w);
-            atomicAdd(&s.counts[b][bin], 1u);
+            if constexpr (ROW) {   // a wave whose entries share a bin, as equal logits do, adds once
+                const uint64_t lanes = __ballot(w != 0);
+                if (lanes == 0) return;
+                const uint32_t bin0 = (uint32_t)__builtin_amdgcn_readlane((int)bin, __builtin_ctzll(lanes));
+                if (__ballot(w != 0 && bin != bin0) == 0) {
+                    w = filt_last_lane(filt_wave_scan(w));
+                    if (tid % kWave == 0) {
+                        atomicAdd(&s.bins[b][bin0 & 255u], (unsigned long long)w);
+                        atomicAdd(&s.counts[b][bin0 & 255u], (uint32_t)__builtin_popcountll(lanes));
+                    }
+                    return;
+                }
+            }
+            if (w == 0) return;
+            atomicAdd(&s.bins[b][bin & 255u], (unsigned long long)w);
+            atomicAdd(&s.counts[b][bin & 255u], 1u);
         });
         if (tid < 256) s.bins[1 - b][tid] = 0, s.counts[1 - b][tid] = 0;
         __syncthreads();
@@ -308,8 +325,8 @@ __device__ __forceinline__ FiltCut filt_pick(bool by_id, uint32_t low, uint32_t 
         rank -= s.sel[1];
         lo += ((uint32_t)s.sel[0] & 255u) << shift, hi = min(hi, lo + ((1u << shift) - 1));
         if (s.found[2] == 1) {
-            each([&](int i, uint32_t k, uint64_t w) {
-                if (active(i, k, w)) s.found[0] = k, s.found[1] = (uint32_t)i;
+            each([&](int i, uint32_t k, bool in, auto weight) {
+                if (in && active(i, k) && weight() != 0) s.found[0] = k, s.found[1] = (uint32_t)i;
             });
             __syncthreads();
             return FiltCut{s.found[0], (int)s.found[1]};
@@ -322,27 +339,27 @@ __device__ __forceinline__ FiltCut filt_pick(bool by_id, uint32_t low, uint32_t 
     return FiltCut{~0u, 0};
 }
 
-// K, N and the draw over a source of `count` entries (id, key, mass), each(f), keys of [low, high]. W: the
+// K, N and the draw over a list, each(f): f(id, key, mass), `count` entries with keys of [low, high]. W: the
 // mass that top_p is of (0: K's).
 template <int NT, typename Each>
 __device__ __forceinline__ int filt_choose(const FiltArgs& a, uint32_t low, uint32_t high, uint32_t count, uint64_t W, float u, FiltShared<NT>& s,
                                            Each each) {
     FiltCut kept{0u, a.V};
     if ((uint32_t)a.top_k < count)
-        kept = filt_pick<NT>(false, low, high, (uint64_t)a.top_k - 1, a, s,
-                             [&](auto f) { each([&](int i, uint32_t k, uint64_t) { f(i, k, 1ull); }); });
-    auto left = [&](auto f) { each([&](int i, uint32_t k, uint64_t w) { f(i, k, kept.keeps(k, i) ? w : 0ull); }); };
+        kept = filt_pick<NT, false>(false, low, high, (uint64_t)a.top_k - 1, a, s,
+                                    [&](auto f) { each([&](int i, uint32_t k, uint64_t) { f(i, k, true, [] { return (uint64_t)1; }); }); });
+    auto left = [&](auto f) { each([&](int i, uint32_t k, uint64_t w) { f(i, k, kept.keeps(k, i), [=] { return w; }); }); };
     auto total = [&]() {
         uint64_t sum = 0;
-        left([&](int, uint32_t, uint64_t w) { sum += w; });
+        each([&](int i, uint32_t k, uint64_t w) { sum += kept.keeps(k, i) ? w : 0ull; });
         return filt_sum<NT>(sum, s);
     };
     uint64_t M = total();
     if (a.top_p < 1.0f) {
-        kept = filt_pick<NT>(false, low, high, filt_need(a.top_p, W != 0 ? W : M) - 1, a, s, left);
+        kept = filt_pick<NT, false>(false, low, high, filt_need(a.top_p, W != 0 ? W : M) - 1, a, s, left);
         M = total();
     }
-    return filt_pick<NT>(true, 0, (uint32_t)a.V - 1, filt_draw(u, M), a, s, left).id;
+    return filt_pick<NT, false>(true, 0, (uint32_t)a.V - 1, filt_draw(u, M), a, s, left).id;
 }
 
 // The same where every thread has an entry at most (x: ~key << 32 | id, and its mass w), by ranks: the
@@ -401,17 +418,105 @@ __device__ __forceinline__ int filt_choose_held(const FiltArgs& a, uint32_t coun
     return (int)s.found[0];
 }
 
-// The same over the row itself: for what fits nowhere.
+// Keys that a bin's logits can have, with 2^-20 of each of the terms to spare.
+__device__ __forceinline__ void filt_bin_keys(const FiltArgs& a, float m, int bin, uint32_t* from, uint32_t* to) {
+    *from = 0u, *to = filt_key(m);
+    if (!(m < INFINITY)) return;
+    const double spare = 0x1p-20 * __builtin_fabs((double)m), one = 1.0 / (double)a.to_bin;
+    if (bin < kFiltMassBins - 1) *from = filt_key((float)((double)m - (bin + 1) * one * (1.0 + 0x1p-20) - spare));
+    *to = min(*to, filt_key((float)((double)m - bin * one * (1.0 - 0x1p-20) + spare)));
+}
+
+// The draw from the masses by tile, in `tile`, of what the cut keeps.
 template <int NT, bool BF16>
-__device__ __noinline__ int filt_choose_row(const FiltArgs& a, const void* row, float m, float u, FiltShared<NT>& s) {
-    return filt_choose<NT>(a, 0u, ~0u, (uint32_t)a.V, 0, u, s, [&](auto f) {
-        filt_tiles<NT, BF16>(row, 0, a.V, [&](int, int i, const auto& l, int n) {
-            constexpr int E = BF16 ? 8 : 4;
+__device__ __forceinline__ int filt_tile_draw(const FiltArgs& a, const void* row, float m, float u, const FiltCut& kept, const unsigned long long* tile,
+                                              FiltShared<NT>& s) {
+    constexpr int E = BF16 ? 8 : 4, TILE = E * NT, PER = kFiltTiles / NT;
+    const int tid = threadIdx.x;
+    uint64_t own = 0, M, h[PER];
 #pragma unroll
-            for (int e = 0; e < E; ++e)
-                if (e < n) f(i + e, filt_key(filt_clean(l[e])), filt_mass(a, filt_clean(l[e]), m));
-        });
+    for (int i = 0; i < PER; ++i) own += h[i] = tile[tid * PER + i];
+    uint64_t excl = filt_scan<NT>(own, s, &M);
+    const uint64_t r = filt_draw(u, M);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        if (excl <= r && r - excl < h[i]) s.sel[0] = tid * PER + i, s.sel[1] = excl;
+        excl += h[i];
+    }
+    __syncthreads();
+    const int t = (int)min((uint32_t)s.sel[0], (uint32_t)(a.V - 1) / TILE);
+    const uint64_t rest = r - s.sel[1];
+    filt_tiles<NT, BF16>(row, t * TILE, min(t * TILE + TILE, a.V), [&](int, int i, const float (&l)[E], int) {
+        uint64_t y[E], sum = 0, all;
+#pragma unroll
+        for (int e = 0; e < E; ++e) sum += y[e] = kept.keeps(filt_key(filt_clean(l[e])), i + e) ? filt_mass(a, filt_clean(l[e]), m) : 0ull;
+        uint64_t at = filt_scan<NT>(sum, s, &all);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            if (at <= rest && rest - at < y[e]) s.found[0] = i + e;
+            at += y[e];
+        }
     });
+    __syncthreads();
+    return (int)s.found[0];
+}
+
+// The choice where the list does not fit, from the row itself, a pass a step of filt_pick. bin < 0: from the start;
+// otherwise N ends in that bin of masses, `above` is the mass of the bins before it and `tile` theirs by tile.
+template <int NT, bool BF16>
+__device__ __forceinline__ int filt_choose_row(const FiltArgs& a, const void* row, float m, float u, int bin, uint64_t above, uint64_t W,
+                                               unsigned long long* tile, FiltShared<NT>& s) {
+    constexpr int E = BF16 ? 8 : 4;
+    FiltCut kept{0u, a.V};
+    uint64_t sum = 0;
+    bool tiles = false;   // the pass adds masses by tile
+    auto pass = [&](auto f) {
+        filt_tiles<NT, BF16>(row, 0, a.V, [&](int t, int i, const float (&l)[E], int n) {
+            uint64_t y = 0;
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const float x = filt_clean(l[e]);
+                const uint32_t k = filt_key(x);
+                y += f(i + e, k, x, e < n && kept.keeps(k, i + e) && (bin < 0 || filt_bin(a, x, m) == bin));
+            }
+            if (!tiles) return;
+            y = filt_last_lane(filt_wave_scan(y));
+            if (threadIdx.x % kWave == 0 && y != 0) atomicAdd(&tile[t], (unsigned long long)y);
+        });
+    };
+    auto masses = [&](auto f) {
+        pass([&](int i, uint32_t k, float x, bool in) {
+            f(i, k, in, [&] { return filt_mass(a, x, m); });
+            return 0ull;
+        });
+    };
+    const uint32_t high = filt_key(m);
+    if (bin >= 0) {
+        uint32_t from, to;
+        filt_bin_keys(a, m, bin, &from, &to);
+        kept = filt_pick<NT, true>(false, from, to, filt_need(a.top_p, W) - 1 - above, a, s, masses);
+    } else {
+        for (int i = threadIdx.x; i < kFiltTiles; i += NT) tile[i] = 0;
+        if (a.top_k < a.V)
+            kept = filt_pick<NT, true>(false, 0u, high, (uint64_t)a.top_k - 1, a, s, [&](auto f) {
+                pass([&](int i, uint32_t k, float, bool in) {
+                    f(i, k, in, [] { return (uint64_t)1; });
+                    return 0ull;
+                });
+            });
+        if (a.top_p < 1.0f) {
+            pass([&](int, uint32_t, float x, bool in) {
+                if (in) sum += filt_mass(a, x, m);
+                return 0ull;
+            });
+            W = filt_sum<NT>(sum, s);
+            kept = filt_pick<NT, true>(false, kept.key, high, filt_need(a.top_p, W) - 1, a, s, masses);
+        }
+    }
+    tiles = true;
+    pass([&](int, uint32_t, float x, bool in) { return in ? filt_mass(a, x, m) : (uint64_t)0; });
+    __syncthreads();
+    return filt_tile_draw<NT, BF16>(a, row, m, u, kept, tile, s);
 }
 
 // Top-k: what a logit has to reach to be listed. Logits fall into bins of equal width from the row's
@@ -441,9 +546,7 @@ __device__ __forceinline__ FiltBound filt_bound(const FiltArgs& a, const float* 
     m = filt_max<NT>(m, &least, s);
     // few runs for so large a top_k, equal runs or infinite ones: all but -inf is listed
     FiltBound b{m, (float)(kFiltRunBins - 1) / (m - least), INFINITY};
-    if (a.top_k >= a.V) {   // min-p alone: what has mass that counts
-        b.width = a.to_log2f, b.past = -a.low;
-    } else if (a.top_k > a.runs || !(b.width < INFINITY) || !(b.width > 0.f)) {
+    if (a.top_k > a.runs || !(b.width < INFINITY) || !(b.width > 0.f)) {
         b.width = 1.f;
     } else {
 #pragma unroll
@@ -640,12 +743,35 @@ __device__ __forceinline__ void filt_list_runs(const FiltArgs& a, const void* ro
 
 // The choice from a row's list (`count` entries, in z or in `list`) and its tiles' masses (in z.tile).
 template <int NT, bool BF16, int MODE, typename Last>
-__device__ __forceinline__ int filt_last(const FiltArgs& a, const void* row, float m, float u, uint64_t above, uint64_t W, uint32_t count,
+__device__ __forceinline__ int filt_last(const FiltArgs& a, const void* row, float m, float u, int bin, uint64_t above, uint64_t W, uint32_t count,
                                          const unsigned long long* list, FiltShared<NT>& s, Last& z) {
     const int tid = threadIdx.x;
     const uint32_t high = filt_key(m);
     if (m == -INFINITY) return -1;
-    if (count > Last::kHeld) return filt_choose_row<NT, BF16>(a, row, m, u, s);
+    if (MODE == kFiltTopP && list != nullptr && count > Last::kHeld && count <= kFiltLong) {
+        // from the list in the workspace; masses of what is in question only
+        auto each = [&](auto f) {
+            constexpr int U = 8;
+            for (uint32_t i0 = tid; i0 < count; i0 += U * NT) {
+                unsigned long long x[U];
+#pragma unroll
+                for (int j = 0; j < U; ++j) x[j] = __hip_atomic_load(&list[min(i0 + j * NT, count - 1)], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+#pragma unroll
+                for (int j = 0; j < U; ++j)
+                    if (i0 + j * NT < count)
+                        f((int)(uint32_t)x[j], (uint32_t)(x[j] >> 32), true, [&] { return filt_mass(a, filt_logit((uint32_t)(x[j] >> 32)), m); });
+            }
+        };
+        uint32_t from, to;
+        filt_bin_keys(a, m, bin, &from, &to);
+        const FiltCut kept = filt_pick<NT, false>(false, from, to, filt_need(a.top_p, W) - 1 - above, a, s, each);
+        each([&](int i, uint32_t k, bool, auto weight) {
+            if (kept.keeps(k, i) && i < a.V) atomicAdd(&z.tile[i / ((BF16 ? 8 : 4) * NT)], (unsigned long long)weight());
+        });
+        __syncthreads();
+        return filt_tile_draw<NT, BF16>(a, row, m, u, kept, z.tile, s);
+    }
+    if (MODE != kFiltAll && count > Last::kHeld) return filt_choose_row<NT, BF16>(a, row, m, u, MODE == kFiltTopP ? bin : -1, above, W, z.tile, s);
     if (MODE == kFiltTopK && count <= NT) {
         unsigned long long x = tid < (int)count ? z.list[tid] : 0ull;
         const uint64_t mass = tid < (int)count ? filt_mass(a, filt_logit((uint32_t)(x >> 32)), m) : 0ull;
@@ -671,41 +797,18 @@ __device__ __forceinline__ int filt_last(const FiltArgs& a, const void* row, flo
         for (int w = 0; w < NT / kWave; ++w) low = min(low, s.counts[0][w]);
     }
     if constexpr (MODE == kFiltTopK) return filt_choose<NT>(a, low, high, count, W, u, s, each);
-    constexpr int E = BF16 ? 8 : 4, TILE = E * NT, PER = kFiltTiles / NT;
+    constexpr int TILE = (BF16 ? 8 : 4) * NT;
     FiltCut kept{0u, a.V};
     if constexpr (MODE == kFiltTopP) {
-        kept = filt_pick<NT>(false, low, high, filt_need(a.top_p, W) - 1 - above, a, s, each);
+        kept = filt_pick<NT, false>(false, low, high, filt_need(a.top_p, W) - 1 - above, a, s, [&](auto f) {
+            each([&](int i, uint32_t k, uint64_t w) { f(i, k, true, [=] { return w; }); });
+        });
         each([&](int i, uint32_t k, uint64_t w) {
             if (w != 0 && kept.keeps(k, i) && i < a.V) atomicAdd(&z.tile[i / TILE], (unsigned long long)w);
         });
         __syncthreads();
     }
-    uint64_t own = 0, M, h[PER];
-#pragma unroll
-    for (int i = 0; i < PER; ++i) own += h[i] = z.tile[tid * PER + i];
-    uint64_t excl = filt_scan<NT>(own, s, &M);
-    const uint64_t r = filt_draw(u, M);
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-        if (excl <= r && r - excl < h[i]) s.sel[0] = tid * PER + i, s.sel[1] = excl;
-        excl += h[i];
-    }
-    __syncthreads();
-    const int t = (int)min((uint32_t)s.sel[0], (uint32_t)(a.V - 1) / TILE);
-    const uint64_t rest = r - s.sel[1];
-    filt_tiles<NT, BF16>(row, t * TILE, min(t * TILE + TILE, a.V), [&](int, int i, const float (&l)[E], int) {
-        uint64_t y[E], sum = 0, all;
-#pragma unroll
-        for (int e = 0; e < E; ++e) sum += y[e] = kept.keeps(filt_key(filt_clean(l[e])), i + e) ? filt_mass(a, filt_clean(l[e]), m) : 0ull;
-        uint64_t at = filt_scan<NT>(sum, s, &all);
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            if (at <= rest && rest - at < y[e]) s.found[0] = i + e;
-            at += y[e];
-        }
-    });
-    __syncthreads();
-    return (int)s.found[0];
+    return filt_tile_draw<NT, BF16>(a, row, m, u, kept, z.tile, s);
 }
 
 template <bool BF16>
@@ -789,7 +892,7 @@ __global__ __launch_bounds__(kFiltThreads) void filt_draw_kernel(FiltArgs a) {
             __syncthreads();
             int token;
             if (z.count <= kFiltHeld) {
-                token = filt_last<NT, BF16, kFiltTopK>(a, row, m, a.u[blockIdx.y], 0, W, z.count, nullptr, s, z);
+                token = filt_last<NT, BF16, kFiltTopK>(a, row, m, a.u[blockIdx.y], bin, 0, W, z.count, nullptr, s, z);
             } else {
                 __syncthreads();
                 if (tid == 0) z.count = 0;
@@ -797,7 +900,7 @@ __global__ __launch_bounds__(kFiltThreads) void filt_draw_kernel(FiltArgs a) {
                 __syncthreads();
                 filt_gather<NT, BF16, kFiltTopP>(a, row, 0, a.V, m, bin, bound, z);
                 __syncthreads();
-                token = filt_last<NT, BF16, kFiltTopP>(a, row, m, a.u[blockIdx.y], above, W, z.count, nullptr, s, z);
+                token = filt_last<NT, BF16, kFiltTopP>(a, row, m, a.u[blockIdx.y], bin, above, W, z.count, nullptr, s, z);
             }
             if (tid == 0) a.out[blockIdx.y] = token;
             return;
@@ -810,11 +913,11 @@ __global__ __launch_bounds__(kFiltThreads) void filt_draw_kernel(FiltArgs a) {
         const uint32_t n = z.count;
         // a block whose part does not fit makes the row's list overflow
         if (tid == 0 && n != 0)
-            z.base = __hip_atomic_fetch_add(&w.count, n <= kFiltHeld ? n : (uint32_t)kFiltHeld + 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            z.base = __hip_atomic_fetch_add(&w.count, n <= kFiltHeld ? n : (uint32_t)kFiltLong + 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         __syncthreads();
         if (n <= kFiltHeld)
             for (uint32_t i = tid; i < n; i += NT)
-                if (z.base + i < kFiltHeld) __hip_atomic_store(&w.list[z.base + i], z.list[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                if (z.base + i < kFiltLong) __hip_atomic_store(&w.list[z.base + i], z.list[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     for (int i = tid; i < tiles; i += NT)
         __hip_atomic_store(&w.tile[first / TILE + i], z.tile[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -835,11 +938,11 @@ __global__ __launch_bounds__(kFiltThreads) void filt_draw_kernel(FiltArgs a) {
         z.tile[t] = t < all ? __hip_atomic_load(&w.tile[t], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0ull;
     }
     __syncthreads();
-    const int token = filt_last<NT, BF16, MODE>(a, row, m, u, above, W, count, w.list, s, z);
+    const int token = filt_last<NT, BF16, MODE>(a, row, m, u, bin, above, W, count, w.list, s, z);
     if (tid == 0) a.out[blockIdx.y] = token;
 }
 
-// Top-k, or min-p alone, after the maxima: a workgroup a row. Only runs whose maximum is within the bound
+// Top-k, after the maxima: a workgroup a row. Only runs whose maximum is within the bound
 // hold logits to be listed, some top_k of them, so that the row is read once in all.
 template <int NT, bool BF16>
 __global__ __launch_bounds__(NT) void filt_list_kernel(FiltArgs a) {
@@ -863,17 +966,7 @@ __global__ __launch_bounds__(NT) void filt_list_kernel(FiltArgs a) {
     if (n <= kFiltHeldK) filt_list_runs<NT, BF16>(a, row, picked, (int)n, bound, z);
     __syncthreads();
     const uint32_t count = n <= kFiltHeldK ? z.count : kFiltHeldK + 1;
-    int token;
-    if (count > kFiltHeldK && a.top_k >= a.V && a.top_p >= 1.0f && bound.m > -INFINITY) {
-        // min-p that keeps many: by tiles
-        for (int i = tid; i < kFiltTiles; i += NT) z.tile[i] = 0;
-        __syncthreads();
-        filt_gather<NT, BF16, kFiltAll>(a, row, 0, a.V, bound.m, 0, bound, z);
-        __syncthreads();
-        token = filt_last<NT, BF16, kFiltAll>(a, row, bound.m, u, 0, 0, 0, nullptr, s, z);
-    } else {
-        token = filt_last<NT, BF16, kFiltTopK>(a, row, bound.m, u, 0, 0, count, nullptr, s, z);
-    }
+    const int token = filt_last<NT, BF16, kFiltTopK>(a, row, bound.m, u, 0, 0, 0, count, nullptr, s, z);
     if (tid == 0) a.out[blockIdx.x] = token;
 }
 
@@ -910,12 +1003,9 @@ __global__ __launch_bounds__(NT) void filt_one_kernel(FiltArgs a) {
     __syncthreads();
     if (m > -INFINITY) filt_gather<NT, BF16, MODE>(a, row, 0, a.V, m, bin, bound, z);
     __syncthreads();
-    const int token = filt_last<NT, BF16, MODE>(a, row, m, a.u[blockIdx.x], above, W, z.count, nullptr, s, z);
+    const int token = filt_last<NT, BF16, MODE>(a, row, m, a.u[blockIdx.x], bin, above, W, z.count, nullptr, s, z);
     if (tid == 0) a.out[blockIdx.x] = token;
 }
-
-// One launch: small vocabularies, and rows enough to fill the chip where all of a row is looked at again.
-static bool filt_one(int64_t rows, int64_t vocab, bool again) { return vocab <= kFiltOneVocab || (again && rows >= prefill_cus() / 2); }
 
 // Blocks of a row: some four workgroups a CU in all, blocks of whole tiles.
 static void filt_split(int64_t rows, int64_t vocab, int* blocks, int* chunk) {
@@ -925,6 +1015,8 @@ static void filt_split(int64_t rows, int64_t vocab, int* blocks, int* chunk) {
     *blocks = (int)((vocab + c - 1) / c);
 }
 
+// NT: a row of 16384 and top-p take 44 us with 256 threads and 32 with 512, a row of 2048 12.7 and 14.0; rows beyond the
+// CUs share them (1000 rows of 8192: 67 and 91).
 template <int NT, bool BF16>
 static void filt_launch_one(const FiltArgs& a, int64_t rows, hipStream_t stream) {
     const dim3 grid((unsigned)rows), t(NT);
@@ -938,12 +1030,12 @@ static void filt_launch(FiltArgs a, int64_t rows, hipStream_t stream) {
     const int vectors = (a.V + (BF16 ? 7 : 3)) / (BF16 ? 8 : 4);
     while ((vectors + a.run_lanes - 1) / a.run_lanes > kFiltRuns) a.run_lanes *= 2;
     a.runs = (vectors + a.run_lanes - 1) / a.run_lanes;
-    const bool list = a.top_k < a.V || (a.top_p >= 1.0f && a.min_mass > 1);
-    if (filt_one(rows, a.V, !list)) {
-        if (a.V <= kFiltOneVocab) filt_launch_one<256, BF16>(a, rows, stream);
-        else filt_launch_one<1024, BF16>(a, rows, stream);
+    if (a.V <= kFiltOneVocab) {
+        if (a.V > kFiltOneVocab / 4 && rows <= prefill_cus()) filt_launch_one<512, BF16>(a, rows, stream);
+        else filt_launch_one<256, BF16>(a, rows, stream);
         return;
     }
+    const bool list = a.top_k < a.V;
     filt_split(rows, a.V, &a.blocks, &a.chunk);
     const dim3 t(kFiltThreads), grid(a.blocks, (unsigned)rows);
     if (!list && a.top_p >= 1.0f) a.runs = 0;

@@ -379,6 +379,19 @@ def test_sampler_ties(gpu, f, values, vocab):
     assert torch.equal(_sample(x, u, **f), R.sample(x, u, **f))
 
 
+@pytest.mark.parametrize("f", [dict(p=0.9), dict(p=0.5, t=3.0), dict(p=0.999), dict(k=5000), dict(k=2500, p=0.7), dict(k=9000, p=0.99, min_p=0.02),
+                               dict(min_p=0.3), dict(p=0.8, min_p=0.2)], ids=str)
+@pytest.mark.parametrize("shift", [0.0, 1e4, -1e4])
+@pytest.mark.parametrize("rows,vocab", [(1, 151936), (4, 16000), (7, 4097), (257, 16000)])
+def test_sampler_flat_rows(gpu, f, shift, rows, vocab):
+    """Thousands of ids of nearly the same mass at the place where the choice ends; logits far from zero."""
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    x = 0.6 * torch.randn(rows, vocab, generator=g, device="cuda") + shift
+    u = torch.rand(rows, generator=g, device="cuda")
+    for y in (x, x.bfloat16()):
+        assert torch.equal(_sample(y, u, **f), R.sample(y, u, **f))
+
+
 @pytest.mark.parametrize("f", [dict(), dict(k=20), dict(p=0.9), dict(min_p=0.1), dict(k=30, p=0.7, min_p=0.01)], ids=str)
 @pytest.mark.parametrize("vocab", [2000, 100000])
 def test_sampler_rows_that_are_not_finite(gpu, f, vocab):
