@@ -18,9 +18,9 @@ constexpr int kTreeMax = EFM_DRAFT_TREE_MAX_NODES;
 __global__ __launch_bounds__(kTreeMax) void draft_tree_plan_kernel(int n, const int32_t* parents, uint32_t kv_len,
                                                                    const uint32_t* d_kv_len, int32_t pos_offset, uint64_t* mask,
                                                                    int32_t* positions, int32_t position_stride) {
-    __shared__ uint64_t s_set[kTreeMax];
-    __shared__ int s_up[kTreeMax];
-    __shared__ int s_depth[kTreeMax];   // ancestors in the set; unused nodes: negative
+    __shared__ uint64_t s_set[2][kTreeMax];   // of this round and the last, so that a round has one barrier
+    __shared__ int s_up[2][kTreeMax];
+    __shared__ int s_depth[2][kTreeMax];   // ancestors in the set; unused nodes: negative
     const int i = threadIdx.x, word = blockIdx.x, words = gridDim.x;
     constexpr int kUnused = -(1 << 20);   // stays negative however many are added up
     const uint32_t len = d_kv_len != nullptr ? d_kv_len[0] : kv_len;
@@ -28,13 +28,13 @@ __global__ __launch_bounds__(kTreeMax) void draft_tree_plan_kernel(int n, const 
     const bool ok = p >= -1 && p < i && len >= (uint32_t)n;
     uint64_t set = i / 64 == word ? 1ull << (i % 64) : 0ull;
     int up = ok ? p : -1, depth = !ok ? kUnused : p >= 0 ? 1 : 0;
-    while (__syncthreads_or(up >= 0)) {
-        s_set[i] = set, s_up[i] = up, s_depth[i] = depth;
-        __syncthreads();
+    for (int b = 0;; b ^= 1) {
+        s_set[b][i] = set, s_up[b][i] = up, s_depth[b][i] = depth;
+        if (!__syncthreads_or(up >= 0)) break;
         if (up >= 0) {
-            set |= s_set[up];
-            depth = max(depth + s_depth[up], kUnused);
-            up = s_up[up];
+            set |= s_set[b][up];
+            depth = max(depth + s_depth[b][up], kUnused);
+            up = s_up[b][up];
         }
     }
     if (i >= n) return;
@@ -83,38 +83,44 @@ __global__ __launch_bounds__(kTreeMax) void draft_tree_accept_kernel(int n, cons
     if (tokens != nullptr) tokens[i] = on ? s_target[s_path[i]] : -1;
 }
 
-// Row base + path[i] of every layer's K and V goes to row base + i. A thread moves the same 16 bytes
-// of all rows, in order; path[i] >= i and the path rises, so that no row is written before it is read.
-// A path that does not rise so ends there.
-__global__ __launch_bounds__(256) void draft_tree_move_kernel(uint16_t* k, uint16_t* v, int64_t layer_stride, int64_t k_sn, int64_t k_sh,
-                                                              int64_t v_sn, int64_t v_sh, int hd, int chunks, uint32_t max_rows, int n,
-                                                              const int32_t* commit) {
+// Row base + path[i] of every layer's K and V goes to row base + i. A thread moves the same 16 bytes of all rows, in
+// order; path[i] >= i and the path rises, so that no row is written before it is read. A path that does not rise so ends
+// there. A wave holds 64 of the path's nodes, and its loads of 8 rows go out together: what bounds it is the chain of
+// launch, path, rows and stores (28 layers of 4 heads of 128: 6.2 -> 3.9 us, 2.4 at best; a workgroup that does nearly nothing takes 2.0).
+__global__ __launch_bounds__(kWave) void draft_tree_move_kernel(uint16_t* k, uint16_t* v, int64_t layer_stride, int64_t k_sn, int64_t k_sh,
+                                                                int64_t v_sn, int64_t v_sh, int hd, int chunks, uint32_t max_rows, int n,
+                                                                const int32_t* commit) {
+    typedef uint32_t vec_t __attribute__((ext_vector_type(4)));
     constexpr int B = 8;   // rows under way
-    const int c = blockIdx.x * 256 + threadIdx.x;
+    const int lane = threadIdx.x, c = min((int)(blockIdx.x * kWave) + lane, chunks - 1);   // the last chunk again past the end
+    int path = lane < n ? commit[2 + lane] : 0;
     const uint32_t base = (uint32_t)commit[0];
-    const int count = min(commit[1], n);
-    if (c >= chunks || (uint64_t)base + (uint64_t)n > max_rows) return;
+    int count = min(commit[1], n);
+    if ((uint64_t)base + (uint64_t)n > max_rows) return;
     const bool is_v = blockIdx.z != 0;
     const int64_t sn = is_v ? v_sn : k_sn;
     const int head = c * 8 / hd;
     uint16_t* const at = (is_v ? v : k) + (int64_t)blockIdx.y * layer_stride + (int64_t)base * sn + head * (is_v ? v_sh : k_sh) + c * 8 % hd;
     int last = -1;
-    for (int i0 = 0; i0 < count; i0 += B) {
-        uint4 x[B];
-        int from[B];
+    for (int g = 0; g < count; g += kWave) {
+        if (g > 0) path = g + lane < n ? commit[2 + g + lane] : 0;
+        int before = __shfl_up(path, 1, kWave);
+        before = lane == 0 ? last : before;
+        const uint64_t ends = __ballot(!(path > before && path < n));
+        if (ends != 0) count = min(count, g + __builtin_ctzll(ends));
+        last = __builtin_amdgcn_readlane(path, kWave - 1);
+        const int rows = min(count - g, kWave);
+        for (int i0 = 0; i0 < rows; i0 += B) {
+            vec_t x[B];
 #pragma unroll
-        for (int j = 0; j < B; ++j) {
-            from[j] = -1;
-            if (i0 + j < count && last < n) {
-                const int p = commit[2 + i0 + j];
-                if (p > last && p < n) from[j] = p, last = p;
-                else last = n;
-            }
-            if (from[j] > i0 + j) x[j] = *reinterpret_cast<const uint4*>(at + (int64_t)from[j] * sn);
+            for (int j = 0; j < B; ++j) x[j] = *reinterpret_cast<const vec_t*>(at + (int64_t)__builtin_amdgcn_readlane(path, min(i0 + j, rows - 1)) * sn);
+#pragma unroll
+            for (int j = 0; j < B; ++j) asm volatile("" : "+v"(x[j]));   // all of them before the first store
+#pragma unroll
+            for (int j = 0; j < B; ++j)
+                if (i0 + j < rows && __builtin_amdgcn_readlane(path, i0 + j) != g + i0 + j)
+                    *reinterpret_cast<vec_t*>(at + (int64_t)(g + i0 + j) * sn) = x[j];
         }
-#pragma unroll
-        for (int j = 0; j < B; ++j)
-            if (from[j] > i0 + j) *reinterpret_cast<uint4*>(at + (int64_t)(i0 + j) * sn) = x[j];
     }
 }
 
@@ -186,7 +192,7 @@ extern "C" int efm_draft_tree_move_kv(const efm_attention_ctx* ctx, uint32_t lay
     if (layers == 0) return EFM_OK;
     const int hd = (int)ctx->head_dim, chunks = (int)ctx->num_kv_heads * hd / 8;
     const int64_t row = (int64_t)ctx->num_kv_heads * hd;
-    hipLaunchKernelGGL(draft_tree_move_kernel, dim3((chunks + 255) / 256, layers, 2), dim3(256), 0, stream, static_cast<uint16_t*>(k_cache),
+    hipLaunchKernelGGL(draft_tree_move_kernel, dim3((chunks + kWave - 1) / kWave, layers, 2), dim3(kWave), 0, stream, static_cast<uint16_t*>(k_cache),
                        static_cast<uint16_t*>(v_cache), layer_stride, ctx->k_stride_n ? (int64_t)ctx->k_stride_n : row,
                        ctx->k_stride_h ? (int64_t)ctx->k_stride_h : hd, ctx->kv_stride_n ? (int64_t)ctx->kv_stride_n : row,
                        ctx->kv_stride_h ? (int64_t)ctx->kv_stride_h : hd, hd, chunks, max_rows, (int)nodes, commit);
