@@ -791,7 +791,7 @@ static TreePlan tree_plan(const efm_attention_ctx* c, uint32_t n, uint32_t kv_le
 // own need goes up and down with its sizes, and splits <= min(tiles, workgroups wanted / row blocks).
 static size_t tree_workspace(const efm_attention_ctx* c, uint32_t n, uint32_t kv_len) {
     const int64_t tiles = ((int64_t)kv_len + 31) / 32, cus = prefill_cus();
-    if (kv_len <= 128) return 0;
+    if (kv_len <= 256) return 0;   // one split in either kernel
     const int64_t splits = std::min<int64_t>(tiles, kTreeMaxSplits);
     const int64_t rows = std::min(splits * n * (int64_t)c->num_qo_heads, 128 * cus);   // 128 rows a workgroup at most
     return (size_t)rows * (c->head_dim + 2) * sizeof(float);

@@ -594,3 +594,172 @@ def test_move_of_a_path_that_does_not_rise(gpu, path, moved):
     C.call("efm_draft_tree_move_kv", c, 1, 0, ptr(k), ptr(v), 50, 8, ptr(d), stream())
     torch.cuda.synchronize()
     assert torch.equal(k, want) and torch.equal(v, want)
+
+
+# ---------------------------------------------------------------- a step
+
+class _Step:
+    """Steps of a model of one layer whose qkv rows depend on the token alone: its cache has to hold, bit for bit, what a
+    prefill of the accepted text writes."""
+    VOCAB, MAX = 16, 1600
+
+    def __init__(self, hq, hkv, hd, n, prefix, seed=5, ws=None):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        self.hq, self.hkv, self.hd, self.n = hq, hkv, hd, n
+        bf = lambda *s, std: (torch.randn(*s, generator=g, device="cuda") * std).bfloat16()
+        self.table = bf(self.VOCAB, (hq + 2 * hkv) * hd, std=1.0)
+        self.head, self.qw, self.kw = bf(self.VOCAB, hq * hd, std=2 / math.sqrt(hd)), bf(hd, std=1.0), bf(hd, std=1.0)
+        self.ctx = C.make_attention_ctx(hq, hkv, hd, rope=True)
+        self.plain = C.make_attention_ctx(hq, hkv, hd, rope=False)
+        self.text = torch.randint(0, self.VOCAB, (prefix,), generator=g, device="cuda").tolist()
+        self.cache = torch.full((2, self.MAX, hkv, hd), math.nan, dtype=torch.bfloat16, device="cuda")
+        self.write(self.text, self.cache)
+        # every node but the root guesses a token; the children of a node guess different ones
+        self.parents = [-1] + [(i - 1) // 3 for i in range(1, n)]
+        i32 = lambda *s: torch.zeros(*s, dtype=torch.int32, device="cuda")
+        self.d_parents, self.drafts, self.len = _i32(self.parents), i32(n), _i32([prefix + n])
+        self.mask, self.pos = torch.zeros(n, -(-n // 64), dtype=torch.int64, device="cuda"), i32(3, n)
+        self.qkv, self.o = self.table.new_zeros(n, self.table.shape[1]), self.table.new_zeros(n, hq * hd)
+        self.q = self.table.new_zeros(n, hq, hd)
+        self.logits, self.u = torch.zeros(n, self.VOCAB, device="cuda"), torch.zeros(n, device="cuda")
+        self.drawn, self.commit, self.tokens = i32(n), i32(n + 2), i32(n)
+        size = max(C.load().efm_attention_tree_workspace_bytes(self.plain, n, self.MAX),
+                   C.load().efm_sampler_filtered_workspace_bytes(n, self.VOCAB))
+        self.ws = _buf(size) if ws is None else ws
+        self.last = int(torch.randint(0, self.VOCAB, (1,), generator=g, device="cuda"))
+        self.g = torch.Generator().manual_seed(seed)
+
+    def write(self, text, cache):
+        qkv = self.table[torch.tensor(text, device="cuda")]
+        C.call("efm_qk_norm_rope_write_kv", self.ctx, ptr(qkv), 0, ptr(self.qw), ptr(self.kw), 1e-6, None, ptr(cache[0]), ptr(cache[1]),
+               self.MAX, len(text), 0, None, None, 0, 0, 0, 0, stream())
+
+    def feed(self):
+        """The next tree's tokens and random numbers."""
+        guess = [self.last] + [(int(torch.randint(0, self.VOCAB, (1,), generator=self.g)) // 3 * 3 + i) % self.VOCAB for i in range(1, self.n)]
+        self.drafts.copy_(_i32(guess))
+        self.u.copy_(torch.rand(self.n, generator=self.g))
+
+    def launch(self):
+        n, hq, hkv, hd = self.n, self.hq, self.hkv, self.hd
+        torch.index_select(self.table, 0, self.drafts, out=self.qkv)
+        C.call("efm_draft_tree_plan", n, ptr(self.d_parents), 0, ptr(self.len), 0, ptr(self.mask), ptr(self.pos), n, stream())
+        C.call("efm_qk_norm_rope_write_kv", self.ctx, ptr(self.qkv), 0, ptr(self.qw), ptr(self.kw), 1e-6, ptr(self.q), ptr(self.cache[0]),
+               ptr(self.cache[1]), self.MAX, n, 0, ptr(self.len), ptr(self.pos), n, hd // 8, hd // 8, hd // 4, stream())
+        C.call("efm_attention_tree", self.plain, ptr(self.q), ptr(self.cache[0]), ptr(self.cache[1]), ptr(self.mask), ptr(self.o), n, 0,
+               ptr(self.len), self.MAX, ptr(self.ws), self.ws.numel(), stream())
+        C.call("efm_linear", n, hq * hd, self.VOCAB, ptr(self.o), ptr(self.head), None, ptr(self.logits), C.EFM_DTYPE_F32, stream())
+        C.call("efm_sampler_filtered", n, self.VOCAB, ptr(self.logits), C.EFM_DTYPE_F32, 0, 0.8, 12, 0.95, 0.0, ptr(self.u), ptr(self.drawn),
+               ptr(self.ws), self.ws.numel(), stream())
+        C.call("efm_draft_tree_accept", n, ptr(self.d_parents), ptr(self.drafts), ptr(self.drawn), ptr(self.len), n, ptr(self.len),
+               ptr(self.commit), ptr(self.tokens), stream())
+        C.call("efm_draft_tree_move_kv", self.plain, 1, 0, ptr(self.cache[0]), ptr(self.cache[1]), self.MAX, n, ptr(self.commit), stream())
+
+    def take(self):
+        """Reads what the step emitted; returns it with the cache's rows of the text."""
+        torch.cuda.synchronize()
+        before, count = self.commit[:2].tolist()
+        new = self.tokens[:count].tolist()
+        assert before == len(self.text) and count >= 1
+        self.text += [self.last] + new[:-1]
+        self.last = new[-1]
+        assert int(self.len) == len(self.text) + self.n
+        return new, self.cache[:, :len(self.text)].clone()
+
+
+@pytest.mark.parametrize("hq,hkv,hd", HEADS)
+@pytest.mark.parametrize("n,prefix", [(1, 1), (13, 3), (40, 700), (70, 1100)])
+def test_steps(gpu, hq, hkv, hd, n, prefix):
+    """plan, rows, attention, logits, tokens, walk and move, step after step."""
+    st, accepted = _Step(hq, hkv, hd, n, prefix), 0
+    for _ in range(30):
+        st.feed()
+        st.launch()
+        torch.cuda.synchronize()
+        rows = len(st.text) + n
+        # the nodes' rows are overwritten by the move: q and the text's rows give what the attention saw
+        keys = torch.full_like(st.cache, math.nan)
+        keys[:, :len(st.text)] = st.cache[:, :len(st.text)]
+        C.call("efm_qk_norm_rope_write_kv", st.ctx, ptr(st.qkv), 0, ptr(st.qw), ptr(st.kw), 1e-6, None, ptr(keys[0]), ptr(keys[1]), st.MAX, n,
+               len(st.text), None, ptr(st.pos), n, hd // 8, hd // 8, hd // 4, stream())
+        ref, tol = R.attention(st.q.double(), keys[0, :rows].double(), keys[1, :rows].double(), R.bits(st.parents))
+        _close(st.o.view(n, hq, hd), ref, tol)
+        assert torch.equal(st.drawn, R.sample(st.logits, st.u, t=0.8, k=12, p=0.95))
+        path = R.accept(st.parents, st.drafts.tolist(), st.drawn.tolist())
+        drawn = st.drawn.tolist()
+        new, cache = st.take()
+        assert new == [drawn[i] for i in path]
+        accepted += len(path)
+        text = torch.full_like(st.cache, math.nan)
+        st.write(st.text, text)
+        assert torch.equal(cache, text[:, :len(st.text)])
+    # Some guess was right: a root has three, of 16 ids, so that none is in 30 steps with a chance of (13 / 16)^30 = 0.2%
+    # (of 5 steps 35%).
+    assert n < 13 or accepted > 30
+
+
+@pytest.mark.parametrize("hq,hkv,hd", HEADS)
+def test_captured_steps_that_share_a_workspace(gpu, hq, hkv, hd):
+    """Graphs of steps of two sizes over one workspace, replayed in turn, with eager work between."""
+    sizes = [(40, 700), (9, 900)]
+    ws = _buf(max(C.load().efm_attention_tree_workspace_bytes(C.make_attention_ctx(hq, hkv, hd, rope=False), n, _Step.MAX) for n, _ in sizes))
+    eager = [_Step(hq, hkv, hd, n, prefix) for n, prefix in sizes]
+    graphed = [_Step(hq, hkv, hd, n, prefix, ws=ws) for n, prefix in sizes]
+    side, graphs = torch.cuda.Stream(), []
+    torch.cuda.synchronize()
+    for st in graphed:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side, capture_error_mode="thread_local"):
+            st.launch()
+        graphs.append(graph)
+    for step in range(6):
+        for a, b, graph in zip(eager, graphed, graphs):
+            a.feed()
+            a.launch()
+            b.feed()
+            graph.replay()
+            (new, cache), (new_b, cache_b) = a.take(), b.take()
+            assert new == new_b and torch.equal(cache, cache_b) and torch.equal(a.o, b.o) and torch.equal(a.drawn, b.drawn)
+
+
+def test_two_streams_at_once(gpu):
+    """Steps of two texts on streams of their own, their launches in turn."""
+    args = [(14, 2, 64, 40, 700), (28, 4, 128, 24, 900)]
+    alone, both = [_Step(*a) for a in args], [_Step(*a) for a in args]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for step in range(4):
+        for st in alone:
+            st.feed()
+            st.launch()
+        for st in both:
+            st.feed()
+        torch.cuda.synchronize()
+        for st, s in zip(both, streams):
+            with torch.cuda.stream(s):
+                st.launch()
+        for a, b in zip(alone, both):
+            (new, cache), (new_b, cache_b) = a.take(), b.take()
+            assert new == new_b and torch.equal(cache, cache_b) and torch.equal(a.o, b.o)
+
+
+@pytest.mark.parametrize("rows,vocab,f", [(2, 3000, dict(p=0.9)), (3, 151936, dict(k=40, p=0.9)), (5, 151936, dict(p=0.9)), (5, 50000, dict(min_p=0.01))],
+                         ids=str)
+def test_captured_sampler_that_shares_a_workspace(gpu, rows, vocab, f):
+    """A graph replayed over new logits, with eager calls of other sizes over the same workspace between."""
+    ws = _buf(C.load().efm_sampler_filtered_workspace_bytes(9, 200000))
+    x, u = _logits(1, rows, vocab)
+    other, ou = _logits(2, 9, 200000)
+    out = torch.zeros(rows, dtype=torch.int32, device="cuda")
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=side, capture_error_mode="thread_local"):
+        C.call("efm_sampler_filtered", rows, vocab, ptr(x), C.EFM_DTYPE_F32, 0, 1.0, f.get("k", 0), f.get("p", 1.0), f.get("min_p", 0.0), ptr(u),
+               ptr(out), ptr(ws), ws.numel(), stream())
+    for seed in range(5):
+        y, v = _logits(10 + seed, rows, vocab)
+        x.copy_(y), u.copy_(v)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, R.sample(x, u, **f))
+        assert torch.equal(_sample(other, ou, ws=ws, p=0.8), R.sample(other, ou, p=0.8))
