@@ -423,7 +423,7 @@ __global__ __launch_bounds__(512, 2) void tree_rows_kernel(TreeArgs a) {
     constexpr int TILE = KT * T::kRow, STAGE = 2 * TILE, RING = 2 * STAGE;   // bytes: keys or values; both; a group's ring
     constexpr int NL = TILE / 1024 / 4;                                      // loads of a wave: keys, and as many of values
     typedef short s4_t __attribute__((ext_vector_type(4)));
-    static_assert(4 * 32 * HD * 4 <= RING, "the outputs fit in the rings");
+    static_assert(DT % 2 == 0 && 8 * DT / 2 * 4 * 1024 <= 2 * RING, "half of the outputs fits in the rings");
     __shared__ __align__(1024) unsigned char smem[2 * RING];
     __shared__ float ml[2][2][128];
     __shared__ int s_odd;
@@ -657,28 +657,39 @@ __global__ __launch_bounds__(512, 2) void tree_rows_kernel(TreeArgs a) {
         pv(3);
     }
     attn_pipe::vm_wait<0>();   // a tile past the length
-    // the groups' outputs meet in LDS (float4 chunk c of row r at c ^ (r & 15))
+    // The groups' outputs meet: each joins one half of the channels, and hands the other group's half over in LDS.
+    const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(l_part), __float_as_uint(l_part), false, false);
+    const float l_run = __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
     meet();
-    {
-        float4* const part = reinterpret_cast<float4*>(smem + (grp * 4 + wg) * 32 * HD * 4);
-#pragma unroll
-        for (int tt = 0; tt < DT; ++tt)
-#pragma unroll
-            for (int g = 0; g < 4; ++g)
-                part[ql * CPR + ((tt * 8 + g * 2 + hh) ^ (ql & 15))] =
-                    make_float4(oacc[tt][g * 4], oacc[tt][g * 4 + 1], oacc[tt][g * 4 + 2], oacc[tt][g * 4 + 3]);
-        const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(l_part), __float_as_uint(l_part), false, false);
-        if (hh == 0) {
-            ml[0][grp][wg * 32 + ql] = m_run * a.scale;
-            ml[1][grp][wg * 32 + ql] = __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
-        }
+    constexpr int HALF = DT / 2, PARTS = HALF * 4;
+    float4* const mine = reinterpret_cast<float4*>(smem + wave * PARTS * 1024) + lane;
+    const float4* const other = reinterpret_cast<const float4*>(smem + (wave ^ 4) * PARTS * 1024) + lane;
+    tree_each<PARTS>([&](auto ic) {
+        constexpr int I = decltype(ic)::value / 4, G = decltype(ic)::value % 4 * 4;
+        const f32x16_t& x = grp == 0 ? oacc[HALF + I] : oacc[I];
+        mine[decltype(ic)::value * 64] = make_float4(x[G], x[G + 1], x[G + 2], x[G + 3]);
+    });
+    if (hh == 0) {
+        ml[0][grp][wg * 32 + ql] = m_run * a.scale;
+        ml[1][grp][wg * 32 + ql] = l_run;
     }
     __syncthreads();
+    const float m0 = m_run * a.scale, m1 = ml[0][grp ^ 1][wg * 32 + ql], l1 = ml[1][grp ^ 1][wg * 32 + ql], m = fmaxf(m0, m1);
+    const bool any0 = m0 != -INFINITY || l_run != 0.f, any1 = m1 != -INFINITY || l1 != 0.f;   // a group that saw nothing has no part
+    const float x0 = any0 ? __builtin_amdgcn_exp2f(m0 - m) : 0.f, x1 = any1 ? __builtin_amdgcn_exp2f(m1 - m) : 0.f;
+    const float l = (any0 ? x0 * l_run : 0.f) + (any1 ? x1 * l1 : 0.f);
     const bool odd = s_odd != 0;
-    tree_join<HD, 2, 128 * CPR / 512>(a, tid, 512, kvh, split, r0, tile_end > t0, [&](int g, int r, int c) {
-        return reinterpret_cast<const float4*>(smem + (g * 4 + r / 32) * 32 * HD * 4)[r % 32 * CPR + (c ^ (r & 15))];
-    }, &ml[0][0][0], 128, [&](int gr, int c, float4& acc) {
+    const int gr = r0 + wg * 32 + ql;
+    if (gr >= a.rows) return;
+    tree_each<PARTS>([&](auto ic) {
+        constexpr int I = decltype(ic)::value / 4, G = decltype(ic)::value % 4 * 4;
+        const f32x16_t& x = grp == 0 ? oacc[I] : oacc[HALF + I];
+        const float4 y = other[decltype(ic)::value * 64];
+        const int c = (grp * HALF + I) * 8 + G / 2 + hh;
+        float4 acc = make_float4((any0 ? x0 * x[G] : 0.f) + (any1 ? x1 * y.x : 0.f), (any0 ? x0 * x[G + 1] : 0.f) + (any1 ? x1 * y.y : 0.f),
+                                 (any0 ? x0 * x[G + 2] : 0.f) + (any1 ? x1 * y.z : 0.f), (any0 ? x0 * x[G + 3] : 0.f) + (any1 ? x1 * y.w : 0.f));
         if (odd) tree_not_finite(a, vbase, gr, c, before, max(before / KT, t0) * KT, min(L, tile_end * KT), acc);
+        tree_store<HD>(a, kvh, split, gr, c, m, l, acc, tile_end > t0);
     });
 }
 
