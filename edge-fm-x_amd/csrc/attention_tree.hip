@@ -11,9 +11,9 @@
 // to one; maxima, sums and outputs stay in fp32.
 //
 // A short context is bound by latencies: a launch, a length and a tile that come from memory, the join. A long one reads
-// the cache at a part of the memory's rate, since each of a wave's steps waits for its tile, and the parts that the splits
-// write and the second launch weigh as much as a third of it (33 nodes at 32000 rows of 4 heads of 128: 66 MB in 22 us,
-// the join 5 us).
+// the cache at half of the memory's rate: a step's chain takes twice its matrix instructions' time, and the parts that the
+// splits write and the second launch weigh as much as a third (33 nodes at 32000 rows of 4 heads of 128: 66 MB and 16 MB
+// of parts in 25 us, the join 5 us).
 #include "attn_split.hpp"
 #include "common.hpp"
 
@@ -159,7 +159,7 @@ __device__ __forceinline__ void tree_each(F f) {
     (std::make_integer_sequence<int, N>{});
 }
 
-// Few rows: 32 a workgroup, whose waves take every KW-th tile of 8 KB of keys and 8 KB of values, each through a
+// Little work: 32 rows a workgroup, whose waves take every KW-th tile of 8 KB of keys and 8 KB of values, each through a
 // slot of its own in LDS that is requested again as soon as it is read out, so that no wave waits for another
 // before the end. Two workgroups share a CU: one's products run while the other's tiles arrive. (Two slots a wave and
 // loads two tiles ahead, one workgroup a CU: 11.4 -> 12.3 us for 24 nodes at 2003 rows, 28 -> 61 us for 250 at 3900.)
@@ -412,10 +412,11 @@ __global__ __launch_bounds__(256, 2) void tree_few_kernel(TreeArgs a) {
     });
 }
 
-// Many rows: a workgroup takes 128 rows, 32 a wave, and two groups of four waves take every other tile of
+// Much work: a workgroup takes 128 rows, 32 a wave, and two groups of four waves take every other tile of
 // 64 keys. A group's tiles go through a ring of two in LDS that its waves read in common; the next tile is
-// requested before a tile is multiplied. Two waves a SIMD, one from each group, so that one's softmax runs
-// beside the other's products.
+// requested before a tile is multiplied. A step takes 2.1 us, of which the matrix instructions need 0.93 (32 cycles
+// each, two waves a SIMD) and the exponentials and sums about as much; keeping the groups half a step apart, or letting
+// each run on without the other, made it no faster (30 -> 31 to 33 us for 33 nodes at 32000 rows).
 template <int HD>
 __global__ __launch_bounds__(512, 2) void tree_rows_kernel(TreeArgs a) {
     typedef SplitTile<HD> T;
@@ -694,7 +695,7 @@ __global__ __launch_bounds__(512, 2) void tree_rows_kernel(TreeArgs a) {
 }
 
 // Joins the splits of a row: TPR threads a row, HD / 4 across its channels and P over the splits. The first
-// outputs are requested before it is known which splits have any.
+// outputs are requested before it is known which splits have any. 4000 rows of 8 splits, 16 MB: 5.0 us.
 template <int HD, int TPR>
 __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a) {
     constexpr int C = HD / 4, P = TPR / C, CH = 4, RW = 256 / TPR;

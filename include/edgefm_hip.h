@@ -615,9 +615,11 @@ int efm_draft_tree_plan(uint32_t nodes, const int32_t* parents, uint32_t kv_len,
 
 /* Attention of the nodes: q [nodes, Hq, hd] (ctx->q_stride_*), k, v the cache, whose first L rows
  * (L = *d_kv_len when d_kv_len is not NULL; then k, v must hold max_kv_len rows, which may be read
- * before the length is known; else kv_len) end with the nodes' own; o [nodes, Hq * hd] contiguous. Node i sees rows j < L - nodes, and row L - nodes + c where bit c of its row of mask
- * (as efm_draft_tree_plan lays it out; any bits may be set, those past the nodes are not looked at)
- * is set. fp32 softmax, P rounded to bf16 for the PV product, sm_scale = 1/sqrt(hd); a node that
+ * before the length is known, and the keys are split for that many: a bound near the length serves
+ * best; else kv_len) end with the nodes' own; o [nodes, Hq * hd] contiguous. Node i sees rows
+ * j < L - nodes, and row L - nodes + c where bit c of its row of mask (as efm_draft_tree_plan lays it
+ * out; any bits may be set, those past the nodes are not looked at) is set. fp32 softmax, P rounded
+ * to bf16 for the PV product, sm_scale = 1/sqrt(hd); a node that
  * sees no row gets zeros. Keys and values that a node does not see take no part in its output,
  * whatever they hold; a value seen that is not finite leaves its channel not finite. pos_encoding
  * must be EFM_POS_NONE: the cache holds keys as they are multiplied. A device length outside
@@ -641,8 +643,8 @@ int efm_attention_tree(const efm_attention_ctx* ctx, const void* q, const void* 
  * temperature >= 1e-6 (smaller means greedy: use efm_sampler_greedy), top_p > 0, min_p <= 1 (not
  * above 0: off), 1 <= vocab < 2^20. The same inputs give the same token, whatever the other rows
  * are. workspace: efm_sampler_filtered_workspace_bytes(rows, vocab) bytes (0: none), 16-byte
- * aligned, no initial contents required; calls that share one must be stream-ordered. Stands beside
- * efm_sampler_top_p, which draws its own random number for one row. */
+ * aligned, no initial contents required; calls that share one must be stream-ordered. Up to 65535
+ * rows. Stands beside efm_sampler_top_p, which draws its own random number for one row. */
 size_t efm_sampler_filtered_workspace_bytes(int64_t rows, int64_t vocab);
 int efm_sampler_filtered(int64_t rows, int64_t vocab, const void* logits, int32_t logits_dtype, int64_t logits_stride,
                          float temperature, int32_t top_k, float top_p, float min_p, const float* uniforms,

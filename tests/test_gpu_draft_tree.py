@@ -140,14 +140,30 @@ def test_attention_head_layouts(gpu, hq, hkv, hd, n, prefix):
     _close(a.call(), *a.ref())
 
 
+@pytest.mark.parametrize("hq,hkv,hd,n,prefix", [(28, 4, 128, 33, 17000), (14, 2, 64, 250, 9300), (12, 2, 128, 1000, 400), (28, 4, 128, 1000, 30),
+                                                (4, 2, 128, 1024, 7001), (9, 3, 64, 700, 8333)])
+def test_attention_much_work(gpu, hq, hkv, hd, n, prefix):
+    """Sizes at which 128 rows share a tile, with and without splits."""
+    a = _Attn(_gen(n), hq, hkv, hd, n, prefix)
+    _close(a.call(), *a.ref())
+
+
+@pytest.mark.parametrize("hq,hkv,hd", HEADS)
+@pytest.mark.parametrize("n,prefix,bound", [(40, 0, 60000), (75, 1000, 40000), (64, 8000, 70000), (130, 63, 9000)])
+def test_attention_far_below_the_bound(gpu, hq, hkv, hd, n, prefix, bound):
+    """The splits are laid out for the bound: most of them have no keys here."""
+    a = _Attn(_gen(n + 1), hq, hkv, hd, n, prefix)
+    _close(a.call(bound=bound), *a.ref())
+
+
 def test_attention_largest_tree(gpu):
     a = _Attn(_gen(4), 12, 2, 128, 1024, 100)
     _close(a.call(), *a.ref())
 
 
 @pytest.mark.parametrize("hq,hkv,hd", HEADS)
-@pytest.mark.parametrize("prefix", [0, 5, 1000])
-def test_attention_any_mask(gpu, hq, hkv, hd, prefix):
+@pytest.mark.parametrize("prefix,bound", [(0, None), (5, None), (1000, None), (0, 60000), (5, 60000), (1000, 60000)])
+def test_attention_any_mask(gpu, hq, hkv, hd, prefix, bound):
     """Masks that are no tree's: random bits, later nodes seen, rows without a bit (zeros without a prefix), all bits; and
     bits past the nodes in the mask's words, which are not looked at."""
     g = _gen(prefix)
@@ -156,18 +172,18 @@ def test_attention_any_mask(gpu, hq, hkv, hd, prefix):
     m[3], m[74], m[10], m[40, :64], m[41, 64:] = False, False, True, False, False
     a = _Attn(g, hq, hkv, hd, n, prefix, mask=m)
     ref, tol = a.ref()
-    got = a.call()
+    got = a.call(bound=bound)
     _close(got, ref, tol)
     if prefix == 0:
         assert (got[3] == 0).all() and (got[74] == 0).all()
     words = R.words(m)
     words[:, 1] |= -1 << (n - 64)
-    assert torch.equal(a.call(words=words), got)
+    assert torch.equal(a.call(words=words, bound=bound), got)
 
 
 @pytest.mark.parametrize("hq,hkv,hd", HEADS)
-@pytest.mark.parametrize("prefix", [0, 3, 700])
-def test_attention_not_finite_where_masked(gpu, hq, hkv, hd, prefix):
+@pytest.mark.parametrize("prefix,bound", [(0, None), (3, None), (700, None), (0, 60000), (3, 60000), (700, 60000)])
+def test_attention_not_finite_where_masked(gpu, hq, hkv, hd, prefix, bound):
     """A node's key and value hold NaN or infinities: the nodes that do not see it are as without it, and those that do
     are not finite in the channels of a value, or everywhere for a NaN key."""
     g = _gen(7)
@@ -185,51 +201,55 @@ def test_attention_not_finite_where_masked(gpu, hq, hkv, hd, prefix):
     for node in (11, 38):
         a.k[prefix + node] = math.nan
         sees |= clean.mask[:, node, None]
-    got = a.call().double().cpu()
+    got = a.call(bound=bound).double().cpu()
     for h in range(hq):
         assert not torch.isfinite(got[:, h][sees]).any()
         ok = ~sees
         assert bool(((got[:, h] - ref[:, h].cpu()).abs()[ok] <= tol[:, h].cpu()[ok]).all())
 
 
-def test_attention_prefix_not_finite(gpu):
+@pytest.mark.parametrize("bound", [None, 140000])
+def test_attention_prefix_not_finite(gpu, bound):
     """Every node sees the rows before the tree: an infinite value there reaches its channel of every node."""
     a = _Attn(_gen(9), 12, 2, 128, 9, 500)
     ref, tol = a.ref()
     a.v[100, 1, 7] = math.inf
-    got = a.call().double().cpu()
+    got = a.call(bound=bound).double().cpu()
     assert not torch.isfinite(got[:, 6:, 7]).any()
     got[:, 6:, 7], ref, tol = 0, ref.cpu(), tol.cpu()
     ref[:, 6:, 7] = 0
     _close(got, ref, tol)
 
 
-def test_attention_score_extremes(gpu):
+@pytest.mark.parametrize("bound", [None, 140000])
+def test_attention_score_extremes(gpu, bound):
     """Scores far apart, and equal ones: large keys, and keys of zeros."""
     a = _Attn(_gen(10), 12, 2, 128, 20, 3000)
     a.k[:1000] *= 30
     a.k[1000:2000] = 0
     a.q[3] = 0
-    _close(a.call(), *a.ref())
+    _close(a.call(bound=bound), *a.ref())
 
 
-def test_attention_minus_infinity_scores(gpu):
+@pytest.mark.parametrize("bound", [None, 600000])
+def test_attention_minus_infinity_scores(gpu, bound):
     """All of a row's visible scores are -inf: zeros, as in the other attention operators."""
     a = _Attn(_gen(11), 4, 2, 128, 3, 0, mask=torch.eye(3, dtype=torch.bool))
     a.q[1], a.k[1] = 1, 0
     a.k[1, :, 0] = -math.inf
-    got = a.call()
+    got = a.call(bound=bound)
     assert (got[1] == 0).all() and torch.isfinite(got).all()
 
 
 @pytest.mark.parametrize("hq,hkv,hd", HEADS)
-def test_attention_strides(gpu, hq, hkv, hd):
+@pytest.mark.parametrize("past", [9, 120000])
+def test_attention_strides(gpu, hq, hkv, hd, past):
     """Queries inside a fused q/k/v buffer; a cache with the heads outermost; a cache with wide rows."""
     g = _gen(12)
     n, prefix = 21, 1111
     a = _Attn(g, hq, hkv, hd, n, prefix)
     ref, tol = a.ref()
-    rows, bound, width = a.rows, a.rows + 9, (hq + 2 * hkv) * hd
+    rows, bound, width = a.rows, a.rows + past, (hq + 2 * hkv) * hd
     fused = torch.full((n, width), math.nan, dtype=torch.bfloat16, device="cuda")
     fused[:, :hq * hd] = a.q.cuda().flatten(1)
     mask, d = R.words(a.mask).cuda(), _i32([rows])
@@ -277,11 +297,12 @@ def test_attention_cache_past_32_bits(gpu):
     assert torch.equal(kd[prefix + 3:].cpu(), a.k[prefix + 3:]) and torch.equal(vd[:prefix + 1].cpu(), a.v[:prefix + 1])
 
 
-@pytest.mark.parametrize("length", [0, 6, 1001, 2 ** 31, 2 ** 32 - 1])
-def test_attention_device_length_out_of_range(gpu, length):
+@pytest.mark.parametrize("length", [0, 6, -1, 2 ** 31, 2 ** 32 - 1])
+@pytest.mark.parametrize("bound", [1000, 140000])
+def test_attention_device_length_out_of_range(gpu, length, bound):
     """Lengths below the nodes' number and past the bound: zeros."""
     a = _Attn(_gen(14), 12, 2, 128, 7, 900)
-    bound = 1000
+    length = bound + 1 if length == -1 else length
     c = C.make_attention_ctx(12, 2, 128, rope=False)
     k = torch.zeros(bound, 2, 128, dtype=torch.bfloat16, device="cuda")
     q, mask = a.q.cuda(), R.words(a.mask).cuda()
@@ -302,8 +323,9 @@ def test_attention_one_workspace_serves_smaller_calls(gpu):
         _close(a.call(ws=ws, bound=n + prefix), *a.ref(), f"{n} nodes behind {prefix}")
 
 
-def test_attention_repeats(gpu):
-    a = _Attn(_gen(15), 28, 4, 128, 33, 9000)
+@pytest.mark.parametrize("prefix", [9000, 19000])
+def test_attention_repeats(gpu, prefix):
+    a = _Attn(_gen(15), 28, 4, 128, 33, prefix)
     first = a.call()
     for _ in range(3):
         assert torch.equal(a.call(), first)
