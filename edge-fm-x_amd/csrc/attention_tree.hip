@@ -72,11 +72,36 @@ struct TreeBits {
     }
 };
 
+typedef short tree_s4_t __attribute__((ext_vector_type(4)));   // four values of a lane
+
+// Whether words of bf16 pairs hold infinities or NaN: an exponent of ones carries into the bit above it.
+struct TreeOdd {
+    uint32_t sum = 0;
+    __device__ __forceinline__ void look(uint32_t w) { sum |= (w & 0x7f807f80u) + 0x00800080u; }
+    __device__ __forceinline__ void look(tree_s4_t x) {
+        const uint2 w = __builtin_bit_cast(uint2, x);
+        look(w.x), look(w.y);
+    }
+    __device__ __forceinline__ bool any() const { return __any((sum & 0x80008000u) != 0); }
+};
+
+// A score, or -inf where bit i is not set.
+__device__ __forceinline__ float tree_masked(float s, uint32_t bits, int i) {
+    const uint32_t seen = (uint32_t)((int)(bits << (31 - i)) >> 31);
+    return __uint_as_float((__float_as_uint(s) & seen) | (0xff800000u & ~seen));
+}
+
 // A bf16 pair with zeros in the place of infinities and NaN.
 __device__ __forceinline__ uint32_t finite_pair(uint32_t w) {
     if ((w & 0x7f80u) == 0x7f80u) w &= 0xffff0000u;
     if ((w & 0x7f800000u) == 0x7f800000u) w &= 0xffffu;
     return w;
+}
+
+__device__ __forceinline__ tree_s4_t tree_finite(tree_s4_t x) {
+    uint2 w = __builtin_bit_cast(uint2, x);
+    w = make_uint2(finite_pair(w.x), finite_pair(w.y));
+    return __builtin_bit_cast(tree_s4_t, w);
 }
 
 // Channels 4 c to 4 c + 3 of a row: the output, or what a split hands on. some: the split has keys.
@@ -168,7 +193,6 @@ __global__ __launch_bounds__(256, 2) void tree_few_kernel(TreeArgs a) {
     typedef SplitTile<HD> T;
     constexpr int KW = 4, KT = T::kKeys, NH = KT / 32, KS = HD / 16, DT = HD / 32, NL = T::kLoads, KB = KT / 16;
     constexpr int SLOT = 2 * T::kBytes, CPR = HD / 4;
-    typedef short s4_t __attribute__((ext_vector_type(4)));
     __shared__ __align__(1024) unsigned char smem[KW * SLOT];
     __shared__ float ml[2][KW][32];
     __shared__ int s_odd[KW];
@@ -273,22 +297,6 @@ __global__ __launch_bounds__(256, 2) void tree_few_kernel(TreeArgs a) {
         for (int h = 0; h < NH; ++h)
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(kf[h][ks]));
-        // Values that a row does not see take no part in its output whatever they are: a zero weight
-        // times an infinity would be a NaN. V of the tree's rows and of rows past the end is made
-        // finite here, and what was not is added at the end where it is seen.
-        if (masked) {
-            uint4* const vp = reinterpret_cast<uint4*>(vslot);
-#pragma unroll
-            for (int i = 0; i < NL; ++i) {
-                const uint4 x = vp[i * 64 + lane];
-                const uint4 y = make_uint4(finite_pair(x.x), finite_pair(x.y), finite_pair(x.z), finite_pair(x.w));
-                if (x.x != y.x || x.y != y.y || x.z != y.z || x.w != y.w) {
-                    odd = true;
-                    vp[i * 64 + lane] = y;
-                }
-            }
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        }
         if (more) issue_k(t + KW);
         // S^T; element e of s[h]: key kb0 + 32 h + 8 (e / 4) + 4 hh + e % 4 of the lane's row
         f32x16_t s[NH];
@@ -304,7 +312,7 @@ __global__ __launch_bounds__(256, 2) void tree_few_kernel(TreeArgs a) {
             else attn_pipe::vm_wait<0>();
         }
         asm volatile("" ::: "memory");
-        s4_t vf[KB][DT][2];
+        tree_s4_t vf[KB][DT][2];
 #pragma unroll
         for (int tt = 0; tt < DT; ++tt) {
             attn_pipe::read_tr16<0>(vf[0][tt][0], va[tt]);
@@ -323,8 +331,7 @@ __global__ __launch_bounds__(256, 2) void tree_few_kernel(TreeArgs a) {
 #pragma unroll
             for (int h = 0; h < NH; ++h)
 #pragma unroll
-                for (int e = 0; e < 16; ++e)
-                    s[h][e] = (mine >> (32 * h + 8 * (e / 4) + e % 4) & 1) ? s[h][e] : -INFINITY;
+                for (int e = 0; e < 16; ++e) s[h][e] = tree_masked(s[h][e], (uint32_t)(mine >> (32 * h)), 8 * (e / 4) + e % 4);
         }
         float top = s[0][0];
 #pragma unroll
@@ -368,12 +375,31 @@ __global__ __launch_bounds__(256, 2) void tree_few_kernel(TreeArgs a) {
 #pragma unroll
             for (int tt = 0; tt < DT; ++tt) asm volatile("" : "+v"(vf[kb][tt][0]), "+v"(vf[kb][tt][1]));
         if (more) issue_v(t + KW);
+        // Values that a row does not see take no part in its output whatever they are: a zero weight times an infinity
+        // would be a NaN. V of the tree's rows and of rows past the end is made finite here, and what was not is added
+        // at the end where it is seen.
+        if (masked) {
+            TreeOdd look;
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                for (int tt = 0; tt < DT * 2; ++tt) {
+                    look.look(vf[kb][tt / 2][tt % 2]);
+                }
+            if (look.any()) {
+                odd = true;
+#pragma unroll
+                for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                    for (int tt = 0; tt < DT * 2; ++tt) vf[kb][tt / 2][tt % 2] = tree_finite(vf[kb][tt / 2][tt % 2]);
+            }
+        }
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
             for (int tt = 0; tt < DT; ++tt) {
                 union {
-                    s4_t h[2];
+                    tree_s4_t h[2];
                     bf16x8_t v;
                 } vv;
                 vv.h[0] = vf[kb][tt][0];
@@ -423,7 +449,6 @@ __global__ __launch_bounds__(512, 2) void tree_rows_kernel(TreeArgs a) {
     constexpr int KT = 64, KS = HD / 16, DT = HD / 32, CPR = HD / 4;
     constexpr int TILE = KT * T::kRow, STAGE = 2 * TILE, RING = 2 * STAGE;   // bytes: keys or values; both; a group's ring
     constexpr int NL = TILE / 1024 / 4;                                      // loads of a wave: keys, and as many of values
-    typedef short s4_t __attribute__((ext_vector_type(4)));
     static_assert(DT % 2 == 0 && 8 * DT / 2 * 4 * 1024 <= 2 * RING, "half of the outputs fits in the rings");
     __shared__ __align__(1024) unsigned char smem[2 * RING];
     __shared__ float ml[2][2][128];
@@ -532,23 +557,24 @@ __global__ __launch_bounds__(512, 2) void tree_rows_kernel(TreeArgs a) {
             if (L - kb0 < 64) bits &= (1ull << (L - kb0)) - 1;
         }
         meet();   // the tile is there, and the other slot is read out
-        unsigned char* const stage = ring + (st & 1) * STAGE;
         if (clean) {
-            // values that are not finite are made zeros, and added at the end where they are seen
-            bool odd = false;
+            // values that are not finite are made zeros, and added at the end where they are seen; a quarter a wave
             if (on && masked) {
-                uint4* const vp = reinterpret_cast<uint4*>(stage + TILE);
+                uint4* const vp = reinterpret_cast<uint4*>(ring + (st & 1) * STAGE + TILE);
+                uint4 x[NL];
+                TreeOdd look;
 #pragma unroll
                 for (int i = 0; i < NL; ++i) {
-                    const uint4 x = vp[(i * 4 + wg) * 64 + lane];
-                    const uint4 y = make_uint4(finite_pair(x.x), finite_pair(x.y), finite_pair(x.z), finite_pair(x.w));
-                    if (x.x != y.x || x.y != y.y || x.z != y.z || x.w != y.w) {
-                        odd = true;
-                        vp[(i * 4 + wg) * 64 + lane] = y;
-                    }
+                    x[i] = vp[(i * 4 + wg) * 64 + lane];
+                    look.look(x[i].x), look.look(x[i].y), look.look(x[i].z), look.look(x[i].w);
+                }
+                if (look.any()) {
+                    if (lane == 0) s_odd = 1;
+#pragma unroll
+                    for (int i = 0; i < NL; ++i)
+                        vp[(i * 4 + wg) * 64 + lane] = make_uint4(finite_pair(x[i].x), finite_pair(x[i].y), finite_pair(x[i].z), finite_pair(x[i].w));
                 }
             }
-            if (__any(odd) && lane == 0) s_odd = 1;
             meet();
         }
         if (t + 2 < tile_end) {
@@ -579,7 +605,7 @@ __global__ __launch_bounds__(512, 2) void tree_rows_kernel(TreeArgs a) {
         for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(kf[1][ks]));
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) s[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[1][ks], qf[ks], s[1], 0, 0, 0);
-        s4_t vf[4][DT][2];
+        tree_s4_t vf[4][DT][2];
         auto read_v = [&](auto kbc) {
             constexpr int kb = decltype(kbc)::value;
 #pragma unroll
@@ -595,8 +621,7 @@ __global__ __launch_bounds__(512, 2) void tree_rows_kernel(TreeArgs a) {
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int e = 0; e < 16; ++e)
-                    s[h][e] = (mine >> (32 * h + 8 * (e / 4) + e % 4) & 1) ? s[h][e] : -INFINITY;
+                for (int e = 0; e < 16; ++e) s[h][e] = tree_masked(s[h][e], (uint32_t)(mine >> (32 * h)), 8 * (e / 4) + e % 4);
         }
         float top = fmaxf(s[0][0], s[1][0]);
 #pragma unroll
@@ -637,7 +662,7 @@ __global__ __launch_bounds__(512, 2) void tree_rows_kernel(TreeArgs a) {
             for (int tt = 0; tt < DT; ++tt) {
                 asm volatile("" : "+v"(vf[kb][tt][0]), "+v"(vf[kb][tt][1]));
                 union {
-                    s4_t h[2];
+                    tree_s4_t h[2];
                     bf16x8_t v;
                 } vv;
                 vv.h[0] = vf[kb][tt][0];
