@@ -27,7 +27,7 @@ int validate_attention_ctx(const efm_attention_ctx* c, const char* who);
 int prefill_cus();
 
 constexpr int kTreeMaxSplits = 256;
-constexpr int kTreeMany = 16000, kTreeLeast = 8, kTreeManyLeast = 4;   // tree_plan
+constexpr int kTreeMany = 16000, kTreeWhole = 12, kTreeLeast = 4;   // tree_plan
 constexpr float kTreeLazy = 8.f;   // a maximum is followed once it is exceeded by 2^8 in weights
 
 struct TreeArgs {
@@ -798,24 +798,26 @@ struct TreePlan {
     size_t total() const { return o_bytes + ml_bytes; }
 };
 
-// tree_few_kernel or tree_rows_kernel: the first starts and joins faster, the second reads a tile for four times as many
-// rows. With the tiles of 8 KB that blocks of 32 rows visit, both measured in us:
-//   630 (24 nodes, 2000 rows) 11.5 | 14.8     8000 (33, 8000) 18.5 | 22.7     11000 (100, 4000) 23.4 | 26.3
-//   16000 (250, 3900) 28.2 | 27.4             16000 (33, 16000) 27.0 | 24.1   32000 (33, 32000) 40.3 | 32.3
+// tree_few_kernel or tree_rows_kernel: the first starts and joins faster and takes masks better, the second reads a tile
+// for four times as many rows. With the tiles of 8 KB before the tree that blocks of 32 rows visit, both measured in us:
+//   630 (24 nodes, 2000 rows) 10.2 | 13.4    8000 (33, 8000) 19.8 | 21.9       11000 (100, 4000) 23.7 | 25.5
+//   15400 (250, 3900) 26.9 | 28.5            16000 (1000, 1000) 32.8 | 38.7    16000 (33, 16000) 24.4 | 22.8
+//   32000 (33, 32000) 38.9 | 30.6            31500 (1000, 2000) 43.8 | 46.3    head_dim 64: 14000 (1000, 2000) 24.8 | 32.4
 // A workgroup a CU, or two where a row block has fewer than four splits, whose join is cheap (250 nodes at 3900 rows
-// 39 -> 28 us; 24 nodes at 32000, 25 splits instead of 51, 25 -> 20 us); a split of two tiles a wave at least.
+// 39 -> 28 us; 24 nodes at 32000, 25 splits instead of 51, 25 -> 20 us). Up to twelve tiles are not split (five: 6.3 us, in
+// two splits 7.8), more into splits of a tile a wave at least (24 nodes at 2003 10.2 us, two tiles a wave 10.8, three 11.4).
 static TreePlan tree_plan(const efm_attention_ctx* c, uint32_t n, uint32_t kv_len) {
     const int hd = (int)c->head_dim, Hkv = (int)c->num_kv_heads;
     const int64_t rows = (int64_t)n * (c->num_qo_heads / c->num_kv_heads), cus = prefill_cus();
     TreePlan p = {};
     const int few = hd == 128 ? 32 : 64;   // keys of 8 KB
-    p.many = (rows + 31) / 32 * Hkv * (((int64_t)kv_len + few - 1) / few) >= kTreeMany;
+    p.many = (rows + 31) / 32 * Hkv * (((int64_t)(kv_len - n) + few - 1) / few) >= kTreeMany;
     const int keys = p.many ? 64 : few;
     const int64_t tiles = ((int64_t)kv_len + keys - 1) / keys;
     p.blocks = (int)((rows + (p.many ? 127 : 31)) / (p.many ? 128 : 32));
     const int64_t pairs = (int64_t)p.blocks * Hkv, each = !p.many && cus / pairs < 4 ? 2 : 1;
     const int64_t want = std::max<int64_t>(1, each * cus / pairs);
-    p.split_tiles = (int)std::max<int64_t>({p.many ? kTreeManyLeast : kTreeLeast, (tiles + want - 1) / want, (tiles + kTreeMaxSplits - 1) / kTreeMaxSplits});
+    p.split_tiles = (int)std::max<int64_t>({tiles <= kTreeWhole ? tiles : kTreeLeast, (tiles + want - 1) / want, (tiles + kTreeMaxSplits - 1) / kTreeMaxSplits});
     p.splits = (int)std::max<int64_t>(1, (tiles + p.split_tiles - 1) / p.split_tiles);
     if (p.splits > 1) {
         p.o_bytes = (size_t)p.splits * Hkv * rows * hd * sizeof(float);

@@ -141,7 +141,7 @@ def test_attention_head_layouts(gpu, hq, hkv, hd, n, prefix):
 
 
 @pytest.mark.parametrize("hq,hkv,hd,n,prefix", [(28, 4, 128, 33, 17000), (14, 2, 64, 250, 9300), (12, 2, 128, 1000, 400), (28, 4, 128, 1000, 30),
-                                                (4, 2, 128, 1024, 7001), (9, 3, 64, 700, 8333)])
+                                                (4, 2, 128, 1024, 7001), (9, 3, 64, 700, 8333), (28, 4, 128, 1024, 2500)])
 def test_attention_much_work(gpu, hq, hkv, hd, n, prefix):
     """Sizes at which 128 rows share a tile, with and without splits."""
     a = _Attn(_gen(n), hq, hkv, hd, n, prefix)
