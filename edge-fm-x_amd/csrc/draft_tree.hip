@@ -86,7 +86,7 @@ __global__ __launch_bounds__(kTreeMax) void draft_tree_accept_kernel(int n, cons
 // Row base + path[i] of every layer's K and V goes to row base + i. A thread moves the same 16 bytes of all rows, in
 // order; path[i] >= i and the path rises, so that no row is written before it is read. A path that does not rise so ends
 // there. A wave holds 64 of the path's nodes, and its loads of 8 rows go out together: what bounds it is the chain of
-// launch, path, rows and stores (28 layers of 4 heads of 128: 6.2 -> 3.9 us, 2.4 at best; a workgroup that does nearly nothing takes 2.0).
+// launch, path, rows and stores (28 layers of 4 heads of 128: 6.2 -> 3.4 us; the walk's one workgroup takes 2.0).
 __global__ __launch_bounds__(kWave) void draft_tree_move_kernel(uint16_t* k, uint16_t* v, int64_t layer_stride, int64_t k_sn, int64_t k_sh,
                                                                 int64_t v_sn, int64_t v_sh, int hd, int chunks, uint32_t max_rows, int n,
                                                                 const int32_t* commit) {

@@ -414,6 +414,21 @@ def test_sampler_flat_rows(gpu, f, shift, rows, vocab):
         assert torch.equal(_sample(y, u, **f), R.sample(y, u, **f))
 
 
+@pytest.mark.parametrize("f", [dict(p=0.9), dict(p=0.3), dict(k=700), dict(k=2000, p=0.5), dict(p=0.95, min_p=0.9)], ids=str)
+@pytest.mark.parametrize("rows,width", [(1, 9600), (5, 1500), (3, 40), (130, 9600)])
+def test_sampler_clusters(gpu, f, rows, width):
+    """Neighbouring ids hold nearly all of the mass: few runs of many kept ids."""
+    vocab = 151936
+    g = torch.Generator(device="cuda").manual_seed(width)
+    x = torch.randn(rows, vocab, generator=g, device="cuda")
+    for r in range(rows):
+        at = (r * 7919 + 1001) % (vocab - width)
+        x[r, at:at + width] = 25 + 0.05 * x[r, at:at + width]
+    u = torch.rand(rows, generator=g, device="cuda")
+    for y in (x, x.bfloat16()):
+        assert torch.equal(_sample(y, u, **f), R.sample(y, u, **f))
+
+
 @pytest.mark.parametrize("f", [dict(), dict(k=20), dict(p=0.9), dict(min_p=0.1), dict(k=30, p=0.7, min_p=0.01)], ids=str)
 @pytest.mark.parametrize("vocab", [2000, 100000])
 def test_sampler_rows_that_are_not_finite(gpu, f, vocab):
@@ -616,6 +631,26 @@ def test_move_of_a_path_that_does_not_rise(gpu, path, moved):
     C.call("efm_draft_tree_move_kv", c, 1, 0, ptr(k), ptr(v), 50, 8, ptr(d), stream())
     torch.cuda.synchronize()
     assert torch.equal(k, want) and torch.equal(v, want)
+
+
+@pytest.mark.parametrize("hq,hkv,hd", [(9, 9, 128), (6, 3, 64)])
+@pytest.mark.parametrize("end", [None, 1, 63, 64, 65, 127, 128, 200])
+def test_move_of_long_paths(gpu, hq, hkv, hd, end):
+    """Hundreds of accepted nodes, whole or up to entry `end`, which repeats the one before it."""
+    n, base, g = 700, 5, _gen(hkv)
+    path = torch.cat([torch.arange(70), 70 + torch.randperm(n - 70, generator=g)[:190].sort().values]).tolist()
+    moved = len(path) if end is None else end
+    if end is not None:
+        path[end] = path[end - 1]
+    k, v = _bf(g, base + n, hkv * hd).cuda(), _bf(g, base + n, hkv * hd).cuda()
+    k0, v0 = k.clone(), v.clone()
+    at = torch.tensor(path[:moved], device="cuda") + base
+    k0[base:base + moved], v0[base:base + moved] = k[at], v[at]
+    c = C.make_attention_ctx(hq, hkv, hd, rope=False)
+    commit = _i32([base, len(path)] + path + [-1] * (n - len(path)))
+    C.call("efm_draft_tree_move_kv", c, 1, 0, ptr(k), ptr(v), base + n, n, ptr(commit), stream())
+    torch.cuda.synchronize()
+    assert torch.equal(k, k0) and torch.equal(v, v0)
 
 
 # ---------------------------------------------------------------- a step
