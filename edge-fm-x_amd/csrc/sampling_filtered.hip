@@ -49,7 +49,6 @@ constexpr int kFiltTiles = 1024;                 // of a row: 1024 logits or mor
 constexpr int kFiltMassBins = 1024, kFiltBinsPerOctave = 22;   // masses from 2^0 to below 2^-46
 constexpr int kFiltRuns = 5120;                  // runs of neighbouring logits whose maxima are kept, at most
 constexpr int kFiltRunBins = 1024;
-constexpr int kFiltFewRuns = 512;                // that one workgroup goes through
 constexpr int kFiltHeld = 1024, kFiltHeldK = 2048;   // entries of a list that a workgroup holds with their masses; top-k
 constexpr int kFiltLong = 8192;                  // entries of a row's list in the workspace
 constexpr int kFiltOneVocab = 16384;             // vocabularies of one launch
@@ -859,7 +858,7 @@ __global__ __launch_bounds__(kFiltThreads) void filt_draw_kernel(FiltArgs a) {
     constexpr int NT = kFiltThreads, TILE = (BF16 ? 8 : 4) * NT;
     __shared__ FiltShared<NT> s;
     __shared__ FiltLast<kFiltHeld> z;
-    __shared__ uint32_t picked[MODE == kFiltTopP ? kFiltFewRuns : 1];
+    __shared__ uint32_t picked[MODE == kFiltTopP ? kFiltHeld / 4 : 1];
     __shared__ uint32_t n_picked;
     const int tid = threadIdx.x;
     FiltRow& w = a.ws[blockIdx.y];
@@ -882,7 +881,8 @@ __global__ __launch_bounds__(kFiltThreads) void filt_draw_kernel(FiltArgs a) {
 #pragma unroll
         for (int i = 0; i < kFiltRuns / NT; ++i) mine += i * NT + tid < a.runs && x[i] > -INFINITY && reach.takes(x[i]);
         const uint64_t few = filt_sum<NT>(mine, s);
-        if (few <= kFiltFewRuns) {   // the first block has them all
+        constexpr int E = BF16 ? 8 : 4;
+        if (few * (E * a.run_lanes) <= kFiltHeld) {   // the first block has them all, and whatever they hold fits in its list
             if (blockIdx.x != 0) return;
 #pragma unroll
             for (int i = 0; i < kFiltRuns / NT; ++i)
@@ -890,18 +890,7 @@ __global__ __launch_bounds__(kFiltThreads) void filt_draw_kernel(FiltArgs a) {
             __syncthreads();
             filt_list_runs<NT, BF16>(a, row, picked, (int)n_picked, reach, z);
             __syncthreads();
-            int token;
-            if (z.count <= kFiltHeld) {
-                token = filt_last<NT, BF16, kFiltTopK>(a, row, m, a.u[blockIdx.y], bin, 0, W, z.count, nullptr, s, z);
-            } else {
-                __syncthreads();
-                if (tid == 0) z.count = 0;
-                for (int i = tid; i < kFiltTiles; i += NT) z.tile[i] = 0;
-                __syncthreads();
-                filt_gather<NT, BF16, kFiltTopP>(a, row, 0, a.V, m, bin, bound, z);
-                __syncthreads();
-                token = filt_last<NT, BF16, kFiltTopP>(a, row, m, a.u[blockIdx.y], bin, above, W, z.count, nullptr, s, z);
-            }
+            const int token = filt_last<NT, BF16, kFiltTopK>(a, row, m, a.u[blockIdx.y], bin, 0, W, z.count, nullptr, s, z);
             if (tid == 0) a.out[blockIdx.y] = token;
             return;
         }
