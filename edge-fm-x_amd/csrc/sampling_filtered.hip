@@ -276,6 +276,15 @@ __device__ __forceinline__ uint64_t filt_need(float top_p, uint64_t W) {
     return need < 1 ? 1 : need > W ? W : need;
 }
 
+// Last of the 2^shift values from lo on, no further than hi. The difference is compared: lo + 2^shift may pass 2^32, where
+// the lowest logits' keys lie.
+constexpr uint32_t filt_bin_end(uint32_t lo, uint32_t hi, int shift) {
+    const uint32_t past = (1u << shift) - 1;
+    return hi - lo > past ? lo + past : hi;
+}
+static_assert(filt_bin_end(0xff5fffffu, 0xff7fffffu, 24) == 0xff7fffffu && filt_bin_end(0xff5fffffu, 0xffffffffu, 16) == 0xff60fffeu &&
+              filt_bin_end(5, 5, 0) == 5 && filt_bin_end(0, ~0u, 24) == 0xffffffu);
+
 // The entry that holds unit `rank` of the weights of a source, each(f): f(id, key, whether it is one, weight()) by whole
 // waves where ROW; in the sampler's order (keys of [low, high]), or by id alone (ids of [low, high]). The range that may
 // hold it is cut into 256 bins until one entry is left, four times for keys and three for the ids of equal keys at most;
@@ -322,7 +331,7 @@ __device__ __forceinline__ FiltCut filt_pick(bool by_id, uint32_t low, uint32_t 
         if (excl <= rank && rank - excl < own) s.sel[0] = tid, s.sel[1] = excl, s.found[2] = s.counts[b][tid];
         __syncthreads();
         rank -= s.sel[1];
-        lo += ((uint32_t)s.sel[0] & 255u) << shift, hi = min(hi, lo + ((1u << shift) - 1));
+        lo += ((uint32_t)s.sel[0] & 255u) << shift, hi = filt_bin_end(lo, hi, shift);
         if (s.found[2] == 1) {
             each([&](int i, uint32_t k, bool in, auto weight) {
                 if (in && active(i, k) && weight() != 0) s.found[0] = k, s.found[1] = (uint32_t)i;
