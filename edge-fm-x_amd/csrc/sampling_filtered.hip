@@ -264,10 +264,10 @@ struct FiltCut {
     __device__ __forceinline__ bool keeps(uint32_t k, int i) const { return k > key || (k == key && i <= id); }
 };
 
-// floor(u M), at most M - 1.
+// floor(u M), at most M - 1. M may be anything below 2^64; 2^64 - 2^11 is the largest double there.
 __device__ __forceinline__ uint64_t filt_draw(float u, uint64_t M) {
     const double x = (double)u * (double)M;
-    const uint64_t r = x > 0.0 ? (uint64_t)__builtin_fmin(x, 9.2e18) : 0ull;
+    const uint64_t r = x > 0.0 ? (uint64_t)__builtin_fmin(x, 18446744073709549568.0) : 0ull;
     return r < M ? r : M - 1;
 }
 
