@@ -529,7 +529,7 @@ __device__ __forceinline__ int filt_choose_row(const FiltArgs& a, const void* ro
 
 // Top-k: what a logit has to reach to be listed. Logits fall into bins of equal width from the row's
 // maximum down to the smallest maximum of a run (-inf apart: it has no mass), and those of the bins down
-// to the one at which the runs are top_k are listed.
+// to the one at which the runs are top_k are listed; where that is the last one, all that has mass.
 struct FiltBound {
     float m, width, past;   // listed unless (m - l) width >= past
     __device__ __forceinline__ bool takes(float l) const { return !((m - l) * width >= past); }
@@ -552,14 +552,13 @@ __device__ __forceinline__ FiltBound filt_bound(const FiltArgs& a, const float* 
         least = x[i] > -INFINITY ? fminf(least, x[i]) : least;
     }
     m = filt_max<NT>(m, &least, s);
-    // few runs for so large a top_k, equal runs or infinite ones: all but -inf is listed
-    FiltBound b{m, (float)(kFiltRunBins - 1) / (m - least), INFINITY};
-    if (a.top_k > a.runs || !(b.width < INFINITY) || !(b.width > 0.f)) {
-        b.width = 1.f;
-    } else {
+    // few runs for so large a top_k, equal runs, infinite ones or ones of nothing but -inf: all that has mass is listed
+    FiltBound b{m, a.to_log2f, -a.low};
+    const float width = (float)(kFiltRunBins - 1) / (m - least);
+    if (a.top_k <= a.runs && width < INFINITY && width > 0.f) {
 #pragma unroll
         for (int i = 0; i < HELD; ++i)
-            if (i * NT < a.runs && i * NT + tid < a.runs) atomicAdd(&bins[(int)fminf((m - x[i]) * b.width, kFiltRunBins - 1)], 1u);
+            if (i * NT < a.runs && i * NT + tid < a.runs) atomicAdd(&bins[(int)fminf((m - x[i]) * width, kFiltRunBins - 1)], 1u);
         __syncthreads();
         uint32_t own = 0, c[PER];
 #pragma unroll
@@ -572,7 +571,7 @@ __device__ __forceinline__ FiltBound filt_bound(const FiltArgs& a, const float* 
             excl += c[i];
         }
         __syncthreads();
-        if ((int)s.sel[0] < kFiltRunBins - 1) b.past = (float)((int)s.sel[0] + 1);
+        if ((int)s.sel[0] < kFiltRunBins - 1) b.width = width, b.past = (float)((int)s.sel[0] + 1);
     }
 #pragma unroll
     for (int i = 0; i < HELD; ++i)

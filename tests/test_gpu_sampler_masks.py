@@ -57,3 +57,19 @@ def test_finite_masks_at_any_temperature(gpu, f, t):
     """A temperature at which masks of -1e9 have mass, and one at which they have none."""
     x, u = _masked(1, 30000, 3000, -1e9, torch.float32)
     assert torch.equal(_sample(x, u, t=t, **f), R.sample(x, u, t=t, **f))
+
+
+@pytest.mark.parametrize("f", [dict(k=50), dict(k=50, p=0.99), dict(k=40, min_p=0.01)], ids=str)
+@pytest.mark.parametrize("vocab", [10000, 151936])
+@pytest.mark.parametrize("gap", [4e-36, 1e-30, 1e-7, 3e-38])
+def test_groups_whose_maxima_are_close(gpu, gap, vocab, f):
+    """Two groups of neighbouring ids are allowed, with largest logits that differ by next to nothing and others units
+    below."""
+    g = torch.Generator(device="cuda").manual_seed(4)
+    x = torch.full((8, vocab), -math.inf, device="cuda")
+    x[:, 256:272] = -1 - 4 * torch.rand(8, 16, generator=g, device="cuda")
+    x[:, 1024:1040] = -1 - 4 * torch.rand(8, 16, generator=g, device="cuda")
+    x[:, 260], x[:, 1030] = 0.0, -gap
+    u = (torch.arange(8, device="cuda") + 0.5) / 8
+    u[0], u[7] = 0.0, 1.0
+    assert torch.equal(_sample(x, u, **f), R.sample(x, u, **f))
