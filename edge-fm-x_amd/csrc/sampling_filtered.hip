@@ -83,6 +83,9 @@ struct FiltArgs {
 
 enum { kFiltAll, kFiltTopP, kFiltTopK };
 
+// Whether a logit may have mass, m the row's largest; so do all that are larger. fp32, which lets some through that have none.
+__device__ __forceinline__ bool filt_counts(const FiltArgs& a, float l, float m) { return (l == m) | ((l - m) * a.to_log2f > a.low); }
+
 // w of a logit, m the row's largest. 2^t, t = (l - m) log2(e) / T, is 2^n 2^f with the series of
 // exp(f ln 2), |f| <= 1/2: the term after the last is below 2^-52. Adding 1.5 2^52 rounds t to an integer,
 // and a last step to p 2^(n + 44) + 2^52 leaves w in the low bits. Without branches, so that a thread's
@@ -108,8 +111,7 @@ __device__ __forceinline__ uint64_t filt_mass(const FiltArgs& a, float l, float 
     const double scale = __builtin_bit_cast(double, (uint64_t)((uint32_t)__builtin_bit_cast(uint64_t, near) + 44u + 1023u) << 52);
     const uint64_t w = __builtin_bit_cast(uint64_t, __builtin_fma(p, scale, 4503599627370496.0)) & 0xfffffffffffffull;
     // fp32 decides what is far below (no 2^n is made of those); the largest is there even where it is infinite
-    const bool counts = (l == m) | ((l - m) * a.to_log2f > a.low);
-    return (counts & (w >= a.min_mass)) ? w : 0;
+    return (filt_counts(a, l, m) & (w >= a.min_mass)) ? w : 0;
 }
 
 // Bin of a mass histogram, 0 for the largest logit; it rises as the logit falls.
@@ -288,7 +290,7 @@ static_assert(filt_bin_end(0xff5fffffu, 0xff7fffffu, 24) == 0xff7fffffu && filt_
 // The entry that holds unit `rank` of the weights of a source, each(f): f(id, key, whether it is one, weight()) by whole
 // waves where ROW; in the sampler's order (keys of [low, high]), or by id alone (ids of [low, high]). The range that may
 // hold it is cut into 256 bins until one entry is left, four times for keys and three for the ids of equal keys at most;
-// weights outside it are not asked for. rank is below the sum of the weights.
+// weights outside it are not asked for. A rank that the sum of the weights does not reach keeps every entry.
 template <int NT, bool ROW, typename Each>
 __device__ __forceinline__ FiltCut filt_pick(bool by_id, uint32_t low, uint32_t high, uint64_t rank, const FiltArgs& a, FiltShared<NT>& s,
                                              Each each) {
@@ -328,6 +330,7 @@ __device__ __forceinline__ FiltCut filt_pick(bool by_id, uint32_t low, uint32_t 
         __syncthreads();
         uint64_t all;
         const uint64_t own = tid < 256 ? s.bins[b][tid] : 0ull, excl = filt_scan<NT>(own, s, &all);
+        if (all <= rank) return FiltCut{0u, a.V};   // at the first step, if at all
         if (excl <= rank && rank - excl < own) s.sel[0] = tid, s.sel[1] = excl, s.found[2] = s.counts[b][tid];
         __syncthreads();
         rank -= s.sel[1];
@@ -469,8 +472,8 @@ __device__ __forceinline__ int filt_tile_draw(const FiltArgs& a, const void* row
     return (int)s.found[0];
 }
 
-// The choice where the list does not fit, from the row itself, a pass a step of filt_pick. bin < 0: from the start;
-// otherwise N ends in that bin of masses, `above` is the mass of the bins before it and `tile` theirs by tile.
+// The choice where the list does not fit, from the row itself, a pass a step of filt_pick. bin < 0: from the start, of
+// what may have mass; otherwise N ends in that bin of masses, `above` is the mass of the bins before it and `tile` theirs by tile.
 template <int NT, bool BF16>
 __device__ __forceinline__ int filt_choose_row(const FiltArgs& a, const void* row, float m, float u, int bin, uint64_t above, uint64_t W,
                                                unsigned long long* tile, FiltShared<NT>& s) {
@@ -485,7 +488,7 @@ __device__ __forceinline__ int filt_choose_row(const FiltArgs& a, const void* ro
             for (int e = 0; e < E; ++e) {
                 const float x = filt_clean(l[e]);
                 const uint32_t k = filt_key(x);
-                y += f(i + e, k, x, e < n && kept.keeps(k, i + e) && (bin < 0 || filt_bin(a, x, m) == bin));
+                y += f(i + e, k, x, e < n && kept.keeps(k, i + e) && (bin < 0 ? filt_counts(a, x, m) : filt_bin(a, x, m) == bin));
             }
             if (!tiles) return;
             y = filt_last_lane(filt_wave_scan(y));
@@ -528,8 +531,10 @@ __device__ __forceinline__ int filt_choose_row(const FiltArgs& a, const void* ro
 }
 
 // Top-k: what a logit has to reach to be listed. Logits fall into bins of equal width from the row's
-// maximum down to the smallest maximum of a run (-inf apart: it has no mass), and those of the bins down
-// to the one at which the runs are top_k are listed; where that is the last one, all that has mass.
+// maximum down to the smallest maximum of a run, or to where a logit has no mass if that is higher, and
+// those of the bins down to the one at which the runs are top_k are listed; where that is the last one,
+// all that has mass. (Bins down to the smallest maximum whatever it is: with a few ids masked by -1e4 or
+// less all that matters is in one bin, a row of 151936 and top_k 50 329 us instead of 12.)
 struct FiltBound {
     float m, width, past;   // listed unless (m - l) width >= past
     __device__ __forceinline__ bool takes(float l) const { return !((m - l) * width >= past); }
@@ -552,7 +557,8 @@ __device__ __forceinline__ FiltBound filt_bound(const FiltArgs& a, const float* 
         least = x[i] > -INFINITY ? fminf(least, x[i]) : least;
     }
     m = filt_max<NT>(m, &least, s);
-    // few runs for so large a top_k, equal runs, infinite ones or ones of nothing but -inf: all that has mass is listed
+    least = fmaxf(least, m + a.low / a.to_log2f);
+    // few runs for so large a top_k, equal runs or infinite ones: all that has mass is listed
     FiltBound b{m, a.to_log2f, -a.low};
     const float width = (float)(kFiltRunBins - 1) / (m - least);
     if (a.top_k <= a.runs && width < INFINITY && width > 0.f) {
@@ -693,7 +699,7 @@ __device__ __forceinline__ void filt_gather(const FiltArgs& a, const void* row, 
         if (MODE == kFiltTopK && some) {
 #pragma unroll
             for (int e = 0; e < E; ++e)
-                if (e < n && bound.takes(l[e])) enlist(i + e, filt_clean(l[e]));
+                if (e < n && bound.takes(filt_clean(l[e]))) enlist(i + e, l[e]);
         }
         if constexpr (MODE != kFiltTopK) {
             if (!__any(some)) return;

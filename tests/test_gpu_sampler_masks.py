@@ -73,3 +73,39 @@ def test_groups_whose_maxima_are_close(gpu, gap, vocab, f):
     u = (torch.arange(8, device="cuda") + 0.5) / 8
     u[0], u[7] = 0.0, 1.0
     assert torch.equal(_sample(x, u, **f), R.sample(x, u, **f))
+
+
+def _time(x, u, **f):
+    """The least of 7 times of 10 calls, in us a call."""
+    rows, vocab = x.shape
+    out = torch.empty(rows, dtype=torch.int32, device="cuda")
+    ws = torch.empty(max(C.load().efm_sampler_filtered_workspace_bytes(rows, vocab), 256), dtype=torch.uint8, device="cuda")
+    times = []
+    for _ in range(7):
+        a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        a.record()
+        for _ in range(10):
+            C.call("efm_sampler_filtered", rows, vocab, ptr(x), C.EFM_DTYPE_F32, 0, 1.0, f["k"], f.get("p", 1.0), 0.0, ptr(u), ptr(out), ptr(ws),
+                   ws.numel(), stream())
+        b.record()
+        torch.cuda.synchronize()
+        times.append(a.elapsed_time(b) * 100)
+    return min(times)
+
+
+@pytest.mark.parametrize("mask", [-1e4, -1e9, "lowest"])
+@pytest.mark.parametrize("rows,vocab,first", [(1, 151936, 151643), (33, 151936, 151643), (33, 151936, 2000), (4, 16000, 15000)])
+def test_masked_ids_do_not_cost_the_short_list(gpu, rows, vocab, first, mask):
+    """A few logits of a finite mask value, or nearly all of a row: the same tokens as with -inf, in about the same time. (With
+    a list of all that is not -inf a call takes 20 to 40 times as long; the margin is that of a noisy clock.)"""
+    g = torch.Generator(device="cuda").manual_seed(6)
+    x = 2.5 * torch.randn(rows, vocab, generator=g, device="cuda")
+    x[:, 7:1900:100] += 10
+    masked, infinite = x.clone(), x.clone()
+    masked[:, first:], infinite[:, first:] = F32_MIN if mask == "lowest" else mask, -math.inf
+    u = torch.rand(rows, generator=g, device="cuda")
+    for f in (dict(k=50), dict(k=200, p=0.9)):
+        assert torch.equal(_sample(masked, u, **f), R.sample(infinite, u, **f))
+        clean, other = _time(x, u, **f), _time(masked, u, **f)
+        print(f"{f} clean {clean:.1f} masked {other:.1f} us")
+        assert other < 3 * clean
