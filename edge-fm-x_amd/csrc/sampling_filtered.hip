@@ -1071,9 +1071,10 @@ extern "C" int efm_sampler_filtered(int64_t rows, int64_t vocab, const void* log
         return set_error(EFM_ERR_UNSUPPORTED, "sampler_filtered: logits dtype %d (fp32 or bf16)", logits_dtype);
     if (logits_stride != 0 && logits_stride < vocab)
         return set_error(EFM_ERR_INVALID_ARGUMENT, "sampler_filtered: logits_stride %lld below the vocabulary", (long long)logits_stride);
-    if (!(temperature >= 1e-6f) || !(temperature < INFINITY))
+    // past 1e36 logits whose distance overflows in fp32 would have mass (FLT_MAX / 1e36 is far above the 31.2 at which none is left)
+    if (!(temperature >= 1e-6f) || !(temperature <= 1e36f))
         return set_error(EFM_ERR_INVALID_ARGUMENT,
-                         "sampler_filtered: temperature must be finite and >= 1e-6 (below that sampling is greedy)");
+                         "sampler_filtered: temperature must be of [1e-6, 1e36] (below that sampling is greedy)");
     if (!(top_p > 0.0f)) return set_error(EFM_ERR_INVALID_ARGUMENT, "sampler_filtered: top_p must be > 0");
     if (!(min_p <= 1.0f)) return set_error(EFM_ERR_INVALID_ARGUMENT, "sampler_filtered: min_p must be at most 1");
     if (!logits || !uniforms || !token_out) return set_error(EFM_ERR_INVALID_ARGUMENT, "sampler_filtered: null pointer");

@@ -640,8 +640,8 @@ int efm_attention_tree(const efm_attention_ctx* ctx, const void* q, const void* 
  * max(1, ceil(top_p W)), W the mass of K (all of K when top_p >= 1); the token is the smallest id
  * of N whose inclusive mass, in the order of ids, exceeds floor(u M), M the mass of N. A row
  * without mass (all -inf or NaN) gives -1. u outside [0, 1) or NaN is taken as the nearest end (0).
- * temperature >= 1e-6 (smaller means greedy: use efm_sampler_greedy), top_p > 0, min_p <= 1 (not
- * above 0: off), 1 <= vocab < 2^20. The same inputs give the same token, whatever the other rows
+ * 1e-6 <= temperature <= 1e36 (smaller means greedy: use efm_sampler_greedy), top_p > 0, min_p <= 1
+ * (not above 0: off), 1 <= vocab < 2^20. The same inputs give the same token, whatever the other rows
  * are. workspace: efm_sampler_filtered_workspace_bytes(rows, vocab) bytes (0: none), 16-byte
  * aligned, no initial contents required; calls that share one must be stream-ordered. Up to 65535
  * rows. Stands beside efm_sampler_top_p, which draws its own random number for one row. */

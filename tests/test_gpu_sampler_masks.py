@@ -109,3 +109,14 @@ def test_masked_ids_do_not_cost_the_short_list(gpu, rows, vocab, first, mask):
         clean, other = _time(x, u, **f), _time(masked, u, **f)
         print(f"{f} clean {clean:.1f} masked {other:.1f} us")
         assert other < 3 * clean
+
+
+@pytest.mark.parametrize("f", [dict(), dict(k=50), dict(k=3000, p=0.9), dict(p=0.9), dict(min_p=0.1)], ids=str)
+@pytest.mark.parametrize("vocab", [5000, 60000])
+def test_logits_near_the_ends_of_fp32(gpu, vocab, f):
+    """The largest temperature, logits whose distances have mass and ones whose distance is no finite fp32 number."""
+    g = torch.Generator(device="cuda").manual_seed(8)
+    x = 3.3e38 - 4e37 * torch.rand(6, vocab, generator=g, device="cuda")
+    x[:, ::3] = -3.3e38
+    u = torch.rand(6, generator=g, device="cuda")
+    assert torch.equal(_sample(x, u, t=1e36, **f), R.sample(x, u, t=1e36, **f))
