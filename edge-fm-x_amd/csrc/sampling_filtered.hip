@@ -563,21 +563,25 @@ __device__ __forceinline__ FiltBound filt_bound(const FiltArgs& a, const float* 
     const float width = (float)(kFiltRunBins - 1) / (m - least);
     if (a.top_k <= a.runs && width < INFINITY && width > 0.f) {
 #pragma unroll
-        for (int i = 0; i < HELD; ++i)
-            if (i * NT < a.runs && i * NT + tid < a.runs) atomicAdd(&bins[(int)fminf((m - x[i]) * width, kFiltRunBins - 1)], 1u);
+        for (int i = 0; i < HELD; ++i) {   // what would be in the last bin is not counted: thousands of additions to one word
+            const float bin = (m - x[i]) * width;
+            if (i * NT < a.runs && bin < kFiltRunBins - 1) atomicAdd(&bins[(int)bin], 1u);
+        }
         __syncthreads();
         uint32_t own = 0, c[PER];
 #pragma unroll
         for (int i = 0; i < PER; ++i) own += c[i] = bins[tid * PER + i];
         uint64_t all, excl = filt_scan<NT>(own, s, &all);
         const uint64_t rank = (uint64_t)a.top_k - 1;
+        if (all > rank) {
 #pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            if (excl <= rank && rank - excl < c[i]) s.sel[0] = tid * PER + i;
-            excl += c[i];
+            for (int i = 0; i < PER; ++i) {
+                if (excl <= rank && rank - excl < c[i]) s.sel[0] = tid * PER + i;
+                excl += c[i];
+            }
+            __syncthreads();
+            b.width = width, b.past = (float)((int)s.sel[0] + 1);
         }
-        __syncthreads();
-        if ((int)s.sel[0] < kFiltRunBins - 1) b.width = width, b.past = (float)((int)s.sel[0] + 1);
     }
 #pragma unroll
     for (int i = 0; i < HELD; ++i)
