@@ -34,6 +34,7 @@
 #include "common.hpp"
 
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 
 namespace efm {
@@ -72,6 +73,7 @@ struct FiltArgs {
     float top_p;
     double to_log2;       // log2(e) / T
     float to_log2f, low;  // a logit with (l - m) to_log2f <= low has no mass that counts
+    float reach;          // low / to_log2f
     float to_bin;         // bins a unit of m - l
     uint64_t min_mass;    // max(1, ceil(min_p 2^44))
     const float* u;
@@ -82,9 +84,6 @@ struct FiltArgs {
 };
 
 enum { kFiltAll, kFiltTopP, kFiltTopK };
-
-// Whether a logit may have mass, m the row's largest; so do all that are larger. fp32, which lets some through that have none.
-__device__ __forceinline__ bool filt_counts(const FiltArgs& a, float l, float m) { return (l == m) | ((l - m) * a.to_log2f > a.low); }
 
 // w of a logit, m the row's largest. 2^t, t = (l - m) log2(e) / T, is 2^n 2^f with the series of
 // exp(f ln 2), |f| <= 1/2: the term after the last is below 2^-52. Adding 1.5 2^52 rounds t to an integer,
@@ -111,7 +110,8 @@ __device__ __forceinline__ uint64_t filt_mass(const FiltArgs& a, float l, float 
     const double scale = __builtin_bit_cast(double, (uint64_t)((uint32_t)__builtin_bit_cast(uint64_t, near) + 44u + 1023u) << 52);
     const uint64_t w = __builtin_bit_cast(uint64_t, __builtin_fma(p, scale, 4503599627370496.0)) & 0xfffffffffffffull;
     // fp32 decides what is far below (no 2^n is made of those); the largest is there even where it is infinite
-    return (filt_counts(a, l, m) & (w >= a.min_mass)) ? w : 0;
+    const bool counts = (l == m) | ((l - m) * a.to_log2f > a.low);
+    return (counts & (w >= a.min_mass)) ? w : 0;
 }
 
 // Bin of a mass histogram, 0 for the largest logit; it rises as the logit falls.
@@ -478,7 +478,9 @@ template <int NT, bool BF16>
 __device__ __forceinline__ int filt_choose_row(const FiltArgs& a, const void* row, float m, float u, int bin, uint64_t above, uint64_t W,
                                                unsigned long long* tile, FiltShared<NT>& s) {
     constexpr int E = BF16 ? 8 : 4;
-    FiltCut kept{0u, a.V};
+    // what may have mass, with 2^-20 of each of the terms to spare
+    const uint32_t least = filt_key(m + a.reach * (1.f + 0x1p-20f) - (m < INFINITY ? 0x1p-20f * fabsf(m) : 0.f));
+    FiltCut kept{bin < 0 ? least : 0u, a.V};
     uint64_t sum = 0;
     bool tiles = false;   // the pass adds masses by tile
     auto pass = [&](auto f) {
@@ -488,7 +490,7 @@ __device__ __forceinline__ int filt_choose_row(const FiltArgs& a, const void* ro
             for (int e = 0; e < E; ++e) {
                 const float x = filt_clean(l[e]);
                 const uint32_t k = filt_key(x);
-                y += f(i + e, k, x, e < n && kept.keeps(k, i + e) && (bin < 0 ? filt_counts(a, x, m) : filt_bin(a, x, m) == bin));
+                y += f(i + e, k, x, e < n && kept.keeps(k, i + e) && (bin < 0 || filt_bin(a, x, m) == bin));
             }
             if (!tiles) return;
             y = filt_last_lane(filt_wave_scan(y));
@@ -509,7 +511,7 @@ __device__ __forceinline__ int filt_choose_row(const FiltArgs& a, const void* ro
     } else {
         for (int i = threadIdx.x; i < kFiltTiles; i += NT) tile[i] = 0;
         if (a.top_k < a.V)
-            kept = filt_pick<NT, true>(false, 0u, high, (uint64_t)a.top_k - 1, a, s, [&](auto f) {
+            kept = filt_pick<NT, true>(false, least, high, (uint64_t)a.top_k - 1, a, s, [&](auto f) {
                 pass([&](int i, uint32_t k, float, bool in) {
                     f(i, k, in, [] { return (uint64_t)1; });
                     return 0ull;
@@ -536,11 +538,19 @@ __device__ __forceinline__ int filt_choose_row(const FiltArgs& a, const void* ro
 // all that has mass. (Bins down to the smallest maximum whatever it is: with a few ids masked by -1e4 or
 // less all that matters is in one bin, a row of 151936 and top_k 50 329 us instead of 12.)
 struct FiltBound {
-    float m, width, past;   // listed unless (m - l) width >= past
-    __device__ __forceinline__ bool takes(float l) const { return !((m - l) * width >= past); }
+    float m, least;   // the row's maximum; listed from least on: one comparison a logit, which a NaN fails
+    // Logits up to `far` below m, with 2^-22 of both to spare for the roundings by which far and the distances were found
+    // (listing more is no mistake); never -inf.
+    __device__ __forceinline__ FiltBound(float m, float far) : m(m) {
+        const float spare = m < INFINITY ? 0x1p-22f * (fabsf(m) + far) : 0.f;
+        least = fmaxf(m - (far + spare), -FLT_MAX);
+    }
+    __device__ __forceinline__ bool takes(float l) const { return l >= least; }
 };
 
-// From the maxima of the row's runs; pick(run) for the runs that hold such logits.
+// From the maxima of the row's runs; pick(run) for the runs that hold such logits. What would be in the last bin is not
+// counted but added to words behind the bins that nothing reads: thousands of runs may be in it, and additions to one word
+// go one at a time (151936 logits, top-k 50, min-p 0.02: 9.3 -> 13.3 us; a branch around them: 2000 logits 8.0 -> 8.5).
 template <int NT, typename Pick>
 __device__ __forceinline__ FiltBound filt_bound(const FiltArgs& a, const float* run, uint32_t* bins, FiltShared<NT>& s, Pick pick) {
     constexpr int PER = kFiltRunBins / NT, HELD = kFiltRuns / NT;
@@ -557,16 +567,17 @@ __device__ __forceinline__ FiltBound filt_bound(const FiltArgs& a, const float* 
         least = x[i] > -INFINITY ? fminf(least, x[i]) : least;
     }
     m = filt_max<NT>(m, &least, s);
-    least = fmaxf(least, m + a.low / a.to_log2f);
+    least = fmaxf(least, m + a.reach);
     // few runs for so large a top_k, equal runs or infinite ones: all that has mass is listed
-    FiltBound b{m, a.to_log2f, -a.low};
+    float far = -a.reach;
     const float width = (float)(kFiltRunBins - 1) / (m - least);
     if (a.top_k <= a.runs && width < INFINITY && width > 0.f) {
 #pragma unroll
-        for (int i = 0; i < HELD; ++i) {   // what would be in the last bin is not counted: thousands of additions to one word
-            const float bin = (m - x[i]) * width;
-            if (i * NT < a.runs && bin < kFiltRunBins - 1) atomicAdd(&bins[(int)bin], 1u);
-        }
+        for (int i = 0; i < HELD; ++i)
+            if (i * NT < a.runs) {
+                const float bin = (m - x[i]) * width;
+                atomicAdd(&bins[bin < kFiltRunBins - 1 ? (int)bin : kFiltRunBins + tid % kWave], 1u);
+            }
         __syncthreads();
         uint32_t own = 0, c[PER];
 #pragma unroll
@@ -580,12 +591,13 @@ __device__ __forceinline__ FiltBound filt_bound(const FiltArgs& a, const float* 
                 excl += c[i];
             }
             __syncthreads();
-            b.width = width, b.past = (float)((int)s.sel[0] + 1);
+            far = (float)((int)s.sel[0] + 1) / width;
         }
     }
+    const FiltBound b(m, far);
 #pragma unroll
     for (int i = 0; i < HELD; ++i)
-        if (i * NT < a.runs && x[i] > -INFINITY && b.takes(x[i])) pick(i * NT + tid);
+        if (i * NT < a.runs && b.takes(x[i])) pick(i * NT + tid);
     return b;
 }
 
@@ -703,7 +715,7 @@ __device__ __forceinline__ void filt_gather(const FiltArgs& a, const void* row, 
         if (MODE == kFiltTopK && some) {
 #pragma unroll
             for (int e = 0; e < E; ++e)
-                if (e < n && bound.takes(filt_clean(l[e]))) enlist(i + e, l[e]);
+                if (e < n && bound.takes(l[e])) enlist(i + e, l[e]);
         }
         if constexpr (MODE != kFiltTopK) {
             if (!__any(some)) return;
@@ -748,10 +760,9 @@ __device__ __forceinline__ void filt_list_runs(const FiltArgs& a, const void* ro
             filt_unpack<BF16>(x[j], l);
 #pragma unroll
             for (int e = 0; e < E; ++e) {
-                const float y = filt_clean(l[e]);
-                if (at[j] + e < a.V && bound.takes(y)) {
+                if (at[j] + e < a.V && bound.takes(l[e])) {
                     const uint32_t to = atomicAdd(&z.count, 1u);
-                    if (to < Last::kHeld) z.list[to] = (unsigned long long)filt_key(y) << 32 | (uint32_t)(at[j] + e);
+                    if (to < Last::kHeld) z.list[to] = (unsigned long long)filt_key(l[e]) << 32 | (uint32_t)(at[j] + e);
                 }
             }
         }
@@ -886,7 +897,7 @@ __global__ __launch_bounds__(kFiltThreads) void filt_draw_kernel(FiltArgs a) {
     for (int i = tid; i < tiles; i += NT) z.tile[i] = 0;
     int bin = 0;
     uint64_t above = 0, W = 0;
-    const FiltBound bound{0.f, 0.f, 0.f};
+    const FiltBound bound(0.f, 0.f);
     const float m = filt_row_max(a, w, s);
     if constexpr (MODE == kFiltTopP) {
         float x[kFiltRuns / NT];
@@ -894,17 +905,17 @@ __global__ __launch_bounds__(kFiltThreads) void filt_draw_kernel(FiltArgs a) {
         for (int i = 0; i < kFiltRuns / NT; ++i) x[i] = w.run[min(i * NT + tid, a.runs - 1)];
         bin = filt_mass_cut<NT>(a, w.mass_bins, s, &above, &W);
         // the runs that reach N's end
-        const FiltBound reach{m, a.to_bin, bin < kFiltMassBins - 1 ? (float)(bin + 1) : INFINITY};
+        const FiltBound reach(m, bin < kFiltMassBins - 1 ? (float)(bin + 1) / a.to_bin : INFINITY);
         uint32_t mine = 0;
 #pragma unroll
-        for (int i = 0; i < kFiltRuns / NT; ++i) mine += i * NT + tid < a.runs && x[i] > -INFINITY && reach.takes(x[i]);
+        for (int i = 0; i < kFiltRuns / NT; ++i) mine += i * NT + tid < a.runs && reach.takes(x[i]);
         const uint64_t few = filt_sum<NT>(mine, s);
         constexpr int E = BF16 ? 8 : 4;
         if (few * (E * a.run_lanes) <= kFiltHeld) {   // the first block has them all, and whatever they hold fits in its list
             if (blockIdx.x != 0) return;
 #pragma unroll
             for (int i = 0; i < kFiltRuns / NT; ++i)
-                if (i * NT + tid < a.runs && x[i] > -INFINITY && reach.takes(x[i])) picked[atomicAdd(&n_picked, 1u)] = i * NT + tid;
+                if (i * NT + tid < a.runs && reach.takes(x[i])) picked[atomicAdd(&n_picked, 1u)] = i * NT + tid;
             __syncthreads();
             filt_list_runs<NT, BF16>(a, row, picked, (int)n_picked, reach, z);
             __syncthreads();
@@ -956,7 +967,7 @@ __global__ __launch_bounds__(NT) void filt_list_kernel(FiltArgs a) {
     constexpr int E = BF16 ? 8 : 4;
     __shared__ FiltShared<NT> s;
     __shared__ FiltLast<kFiltHeldK> z;
-    __shared__ uint32_t run_bins[kFiltRunBins];
+    __shared__ uint32_t run_bins[kFiltRunBins + kWave];
     __shared__ uint32_t picked[kFiltHeldK];
     __shared__ uint32_t n_picked;
     const int tid = threadIdx.x;
@@ -982,7 +993,7 @@ template <int NT, bool BF16, int MODE>
 __global__ __launch_bounds__(NT) void filt_one_kernel(FiltArgs a) {
     __shared__ FiltShared<NT> s;
     __shared__ FiltLast<MODE == kFiltTopK ? kFiltHeldK : kFiltHeld> z;
-    __shared__ uint32_t run_bins[MODE == kFiltTopK ? kFiltRunBins : 1];
+    __shared__ uint32_t run_bins[MODE == kFiltTopK ? kFiltRunBins + kWave : 1];
     __shared__ float runs[MODE == kFiltTopK ? kFiltRuns : 1];
     __shared__ unsigned long long masses[MODE == kFiltTopP ? kFiltMassBins : 1];
     const int tid = threadIdx.x;
@@ -994,7 +1005,7 @@ __global__ __launch_bounds__(NT) void filt_one_kernel(FiltArgs a) {
     float m = filt_maxima<NT, BF16>(a, row, 0, a.V, MODE == kFiltTopK ? runs : nullptr), least = 0.f;
     int bin = 0;
     uint64_t above = 0, W = 0;
-    FiltBound bound{0.f, 0.f, 0.f};
+    FiltBound bound(0.f, 0.f);
     if constexpr (MODE == kFiltTopK) {
         __syncthreads();
         bound = filt_bound<NT>(a, runs, run_bins, s, [](int) {});
@@ -1102,6 +1113,7 @@ extern "C" int efm_sampler_filtered(int64_t rows, int64_t vocab, const void* log
     a.min_mass = std::max<uint64_t>(1, min_p > 0.f ? (uint64_t)std::ceil((double)min_p * kFiltOne) : 0);
     a.to_log2f = (float)a.to_log2;
     a.low = (float)(std::log2((double)a.min_mass - 0.5) - 44.0 - 0.01);   // fp32 moves (l - m) log2(e) / T by 46 2^-22 at most
+    a.reach = (float)((double)a.low / a.to_log2);
     a.to_bin = (float)(a.to_log2 * kFiltBinsPerOctave);
     a.u = uniforms;
     a.out = token_out;
