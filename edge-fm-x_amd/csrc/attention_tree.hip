@@ -819,9 +819,12 @@ struct TreePlan {
 
 // tree_few_kernel or tree_rows_kernel: the first starts and joins faster and takes masks better, the second reads a tile
 // for four times as many rows. With the tiles of 8 KB before the tree that blocks of 32 rows visit, both measured in us:
-//   630 (24 nodes, 2000 rows) 10.2 | 13.4    8000 (33, 8000) 19.8 | 21.9       11000 (100, 4000) 23.7 | 25.5
-//   15400 (250, 3900) 26.9 | 28.5            16000 (1000, 1000) 32.8 | 38.7    16000 (33, 16000) 24.4 | 22.8
-//   32000 (33, 32000) 38.9 | 30.6            31500 (1000, 2000) 43.8 | 46.3    head_dim 64: 14000 (1000, 2000) 24.8 | 32.4
+//   630 (24 nodes, 2000 rows) 10.3 | 13.8    8000 (33, 8000) 20.0 | 22.8       11000 (100, 4000) 23.7 | 25.5
+//   15400 (250, 3900) 27.6 | 28.3            15800 (500, 2000) 31.2 | 30.7     16000 (33, 16000) 26.5 | 23.5
+//   16000 (1000, 1000) 36.2 | 42.4           16500 (700, 1500) 34.5 | 35.8     31500 (1000, 2000) 47.2 | 48.2
+//   32000 (33, 32000) 41.2 | 31.7            head_dim 64: 14000 (1000, 2000) 27.9 | 34.0
+// The visits alone do not tell few row blocks over a long context from many over a short one: from 16000 on the second
+// is taken for 700 and 1000 nodes too, where it is slower by 2 to 17 %.
 // A workgroup a CU, or two where a row block has fewer than four splits, whose join is cheap (250 nodes at 3900 rows
 // 39 -> 28 us; 24 nodes at 32000, 25 splits instead of 51, 25 -> 20 us). Up to twelve tiles are not split (five: 6.3 us, in
 // two splits 7.8), more into splits of a tile a wave at least (24 nodes at 2003 10.2 us, two tiles a wave 10.8, three 11.4).

@@ -642,9 +642,9 @@ int efm_attention_tree(const efm_attention_ctx* ctx, const void* q, const void* 
  * without mass (all -inf or NaN) gives -1. u outside [0, 1) or NaN is taken as the nearest end (0).
  * 1e-6 <= temperature <= 1e36 (smaller means greedy: use efm_sampler_greedy), top_p > 0, min_p <= 1
  * (not above 0: off), 1 <= vocab < 2^20. The same inputs give the same token, whatever the other rows
- * are. workspace: efm_sampler_filtered_workspace_bytes(rows, vocab) bytes (0: none), 16-byte
- * aligned, no initial contents required; calls that share one must be stream-ordered. Up to 65535
- * rows. Stands beside efm_sampler_top_p, which draws its own random number for one row. */
+ * are. workspace: efm_sampler_filtered_workspace_bytes(rows, vocab) bytes (0: none, up to 16384 ids;
+ * then 102928 a row), 16-byte aligned, no initial contents required; calls that share one must be
+ * stream-ordered. Up to 65535 rows. Stands beside efm_sampler_top_p, which draws its own random number for one row. */
 size_t efm_sampler_filtered_workspace_bytes(int64_t rows, int64_t vocab);
 int efm_sampler_filtered(int64_t rows, int64_t vocab, const void* logits, int32_t logits_dtype, int64_t logits_stride,
                          float temperature, int32_t top_k, float top_p, float min_p, const float* uniforms,
