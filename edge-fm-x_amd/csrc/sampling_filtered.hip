@@ -133,8 +133,8 @@ __device__ __forceinline__ float filt_clean(float l) { return l == l ? l : -INFI
 
 constexpr int kFiltBatch = 4;   // 16-byte loads of a thread under way
 
-// 16 bytes of a row's logits from i on, -inf past the end. A row that does not start on 16 bytes, as three of four do where
-// the vocabulary is odd, is loaded an element at a time (33 rows of 151935 against 151936, fp32 and bf16: top-k 17 | 13 and
+// 16 bytes of a row's logits from i on, -inf past the end. A row that does not start on 16 bytes, as three of four (bf16: seven
+// of eight) do where the vocabulary is odd, is loaded an element at a time (33 rows of 151935 against 151936, fp32 and bf16: top-k 17 | 13 and
 // 18 | 13 us, top-p 43 | 37 and 54 | 39, min-p 19 | 12 and 23 | 13).
 template <bool BF16>
 __device__ __forceinline__ uint4 filt_raw(const void* row, bool aligned, int i, int end) {
